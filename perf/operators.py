@@ -257,7 +257,7 @@ def _run_clip(s):
     s["max_norm"] *= 0.999
     if own:
         import mamba2d_b200
-        return mamba2d_b200.clip_grad_norm_(s["grads"], s["max_norm"]), s["flat"]
+        return mamba2d_b200.clip_norm_(s["grads"], s["max_norm"]), s["flat"]
     total = torch.sqrt(sum(g.float().square().sum().double() for g in s["grads"])).float()
     factor = torch.clamp(s["max_norm"] / (total + 1e-6), max=1.0)
     [g.copy_(g.float() * factor) for g in s["grads"]]
