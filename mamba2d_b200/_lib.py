@@ -1,4 +1,5 @@
-"""ctypes binding of the C-ABI library (include/m2d_scan.h, include/m2d_proj.h).
+"""ctypes binding of the C-ABI library (include/m2d_scan.h, include/m2d_proj.h; include/m2d_seq.h is called from
+csrc/torch_seq.cpp).
 
 The library is prebuilt by ``python -m mamba2d_b200.build``.  There is no fallback: if the shared
 object is missing or a call fails, this module raises.
@@ -30,7 +31,11 @@ EXPORTS = ("m2d_abi_version", "m2d_strerror", "m2d_scan_fwd_workspace", "m2d_sca
            "m2d_wait_failure_mark",
            "m2d_proj_workspace", "m2d_dtproj_fwd", "m2d_dtproj_bwd", "m2d_xproj_wgrad",
            "m2d_xproj_wgrad_on_tensor_cores", "m2d_proj_bwd", "m2d_rows_gemm_f32",
-           "m2d_scan_fwd_cleared")
+           "m2d_scan_fwd_cleared",
+           "m2d_attn_fwd_workspace", "m2d_attn_bwd_workspace", "m2d_attn_fwd", "m2d_attn_bwd", "m2d_attn_step",
+           "m2d_norm_fwd_workspace", "m2d_norm_bwd_workspace", "m2d_norm_fwd", "m2d_norm_bwd",
+           "m2d_clip_workspace", "m2d_clip_grad_norm")
+ATTN_MAX_DIM = 256                   # M2D_ATTN_MAX_DIM in include/m2d_seq.h
 PROJ_MAX_E, PROJ_MAX_R = 640, 64     # M2D_PROJ_MAX_E / M2D_PROJ_MAX_R in include/m2d_proj.h
 
 
@@ -133,7 +138,7 @@ _ENTRY = None
 
 
 def entry():
-    """The native eager entry points (csrc/torch_entry.cpp), loaded once; raises if they are not built."""
+    """The native eager entry points (csrc/torch_entry.cpp, csrc/torch_seq.cpp), loaded once; raises if they are not built."""
     global _ENTRY
     if _ENTRY is None:
         lib()                                   # the library first: same checks, same message

@@ -16,7 +16,9 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "libm2d_scan.so")
 ENTRY = os.path.join(HERE, "_entry.so")  # native eager entry points (Python extension)
 OBJ = os.path.join(HERE, "_obj")          # per-source objects (git-ignored, not shipped)
-SOURCES = ["m2d_abi.cu", "m2d_scan_fwd.cu", "m2d_scan_bwd.cu", "m2d_scan_fwd_noalloc.cu", "m2d_proj.cu", "m2d_gemm.cu"]
+SOURCES = ["m2d_abi.cu", "m2d_scan_fwd.cu", "m2d_scan_bwd.cu", "m2d_scan_fwd_noalloc.cu", "m2d_proj.cu", "m2d_gemm.cu",
+           "m2d_attn.cu", "m2d_norm.cu", "m2d_clip.cu"]
+ENTRY_SOURCES = ["torch_entry.cpp", "torch_seq.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -45,28 +47,41 @@ def _compile(nvcc, src, obj):
 
 
 def build_entry(force=False):
-    """The native eager entry points (torch_entry.cpp): a Python extension linked against the library."""
-    src = os.path.join(CSRC, "torch_entry.cpp")
-    deps = [src, OUT] + [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
-    if not force and os.path.exists(ENTRY) and os.path.getmtime(ENTRY) >= max(os.path.getmtime(d) for d in deps):
+    """The native eager entry points (ENTRY_SOURCES): a Python extension linked against the library."""
+    from concurrent.futures import ThreadPoolExecutor
+    headers = [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
+    newest_header = max(os.path.getmtime(h) for h in headers)
+    jobs = []
+    for name in ENTRY_SOURCES:
+        src, obj = os.path.join(CSRC, name), os.path.join(OBJ, name[:-4] + ".o")
+        stale = force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header)
+        jobs.append((src, obj, stale))
+    sources = [os.path.getmtime(j[0]) for j in jobs]
+    if not force and os.path.exists(ENTRY) and os.path.getmtime(ENTRY) >= max([newest_header, os.path.getmtime(OUT)] + sources):
         return ENTRY
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-    cmd = ["/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+    gxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-DTORCH_EXTENSION_NAME=_entry", "-I", INCLUDE, "-isystem", sysconfig.get_paths()["include"]]
     for d in include_paths() + [os.path.join(cuda, "include")]:
         cmd += ["-isystem", d]
-    cmd += [src, "-o", ENTRY]
+
+    def run(args, what):
+        res = subprocess.run(args, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{what} failed:\n" + res.stdout)
+
+    os.makedirs(OBJ, exist_ok=True)
+    with ThreadPoolExecutor(max_workers=len(jobs)) as pool:
+        list(pool.map(lambda j: j[2] and run([*cmd, "-c", j[0], "-o", j[1]], "building " + os.path.basename(j[0])), jobs))
+    link = [gxx, "-shared", *[j[1] for j in jobs], "-o", ENTRY]
     for d in library_paths() + [os.path.join(cuda, "lib64")]:
-        cmd += ["-L", d]
-    cmd += ["-L", HERE, "-l:libm2d_scan.so", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
-            "-ltorch_python", "-lcudart", "-lcublas"]
-    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("building torch_entry.cpp failed:\n" + res.stdout)
+        link += ["-L", d]
+    run([*link, "-L", HERE, "-l:libm2d_scan.so", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+         "-ltorch_python", "-lcudart", "-lcublas"], "linking the native entry points")
     return ENTRY
 
 

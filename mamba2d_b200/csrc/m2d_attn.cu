@@ -1,0 +1,616 @@
+// Linear attention: entry points, and the kernels for any head size, type and alignment.
+#include "attn_core.cuh"
+
+namespace m2d {
+
+// ------------------------------------------------------------------------------------------------
+// attn_core.cuh's computation on chunks of 64 tokens.  A CTA owns a sequence's head, VT columns of z and of the
+// state, and one segment of the tokens; its products run on mma.sync in tf32, every operand split into two tf32 parts
+// and three products per term, which leaves an error of about 2^-21 (operands in bf16 are exact in one part).
+// ------------------------------------------------------------------------------------------------
+constexpr int kC = 64, kAttnThreads = 256, kPStride = kC + 4;
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// v = hi + lo exactly; hi is v rounded to tf32's 11 bits, of lo the first 11 are read (its sign varies: no bias)
+struct Split {
+    unsigned hi, lo;
+    __device__ __forceinline__ Split(float v) {
+        hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
+        lo = __float_as_uint(v - __uint_as_float(hi));
+    }
+};
+// acc[n] += A (16 x 8) B_n (8 x 8), n < NT; fa(i): the four values of A's fragment, fb(n, i): the two of B's
+template <int NT, typename FA, typename FB>
+__device__ __forceinline__ void mma_step(float (&acc)[NT][4], FA fa, FB fb) {
+    unsigned ah[4], al[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const Split s(fa(i));
+        ah[i] = s.hi; al[i] = s.lo;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const Split b0(fb(n, 0)), b1(fb(n, 1));
+        mma_tf32(acc[n], ah, b0.lo, b1.lo);
+        mma_tf32(acc[n], al, b0.hi, b1.hi);
+        mma_tf32(acc[n], ah, b0.hi, b1.hi);
+    }
+}
+
+// rows [0, 64) x cols [0, width) of a tile, zero behind `valid` rows and `n` columns
+template <typename io_t>
+__device__ __forceinline__ void load_rows(float* dst, int stride, const io_t* src, long long st, int valid, int n, int width, int vec) {
+    const int quads = width / 4;
+    for (int i = threadIdx.x; i < kC * quads; i += kAttnThreads) {
+        const int r = i / quads, c = (i - r * quads) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < valid) {
+            const io_t* p = src + (long long)r * st + c;
+            if (vec && c + 4 <= n) {
+                if constexpr (sizeof(io_t) == 4) {
+                    v = __ldg(reinterpret_cast<const float4*>(p));
+                } else {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+                    v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+                }
+            } else {
+                if (c < n) v.x = load1(p, 0);
+                if (c + 1 < n) v.y = load1(p, 1);
+                if (c + 2 < n) v.z = load1(p, 2);
+                if (c + 3 < n) v.w = load1(p, 3);
+            }
+        }
+        *reinterpret_cast<float4*>(dst + r * stride + c) = v;
+    }
+}
+
+__host__ __device__ inline int attn_pad(int d) { return (d + 15) / 16 * 16; }
+inline size_t attn_smem(int Kd, int VT) {
+    const int kd = attn_pad(Kd);
+    return sizeof(float) * ((size_t)2 * kC * (kd + 4) + (size_t)(kC + kd) * (VT + 8) + (size_t)kC * kPStride + 7 * kC);
+}
+
+template <typename io_t, int VT, bool STATE_ONLY>
+__global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_constant__ AttnLaunch a) {
+    const AttnCore& k = a.core[blockIdx.z];
+    const int v0 = blockIdx.y * VT;
+    if (v0 >= k.Vd) return;
+    extern __shared__ float4 smem4[];
+    const int kd = attn_pad(k.Kd), ks = kd + 4;
+    constexpr int VS = VT + 8, NT = VT / 16;
+    float* X = reinterpret_cast<float*>(smem4);
+    float* Y = X + kC * ks;
+    float* Z = Y + kC * ks;
+    float* S = Z + kC * VS;
+    float* P = S + kd * VS;
+    float* c_hi = P + kC * kPStride;
+    float *c_lo = c_hi + kC, *w = c_lo + kC, *u = w + kC, *dot = u + kC, *whole = dot + 2 * kC;
+
+    const int seg = blockIdx.x % a.nseg, bh = blockIdx.x / a.nseg, h = bh % a.H, b = bh / a.H;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
+    const int wm = (warp & 3) * 16, wn = (warp >> 2) * (VT / 2);
+    const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
+    const int nv = min(VT, k.Vd - v0), chunks = (t_hi - t_lo + kC - 1) / kC;
+    const io_t* const x = static_cast<const io_t*>(attn_at(k.x, b, h, sizeof(io_t)));
+    const io_t* const y = static_cast<const io_t*>(attn_at(k.y, b, h, sizeof(io_t)));
+    const io_t* const z = static_cast<const io_t*>(attn_at(k.z, b, h, sizeof(io_t))) + v0;
+    const float* const g = a.g + (long long)b * a.gb + (long long)h * a.gh;
+
+    for (int i = tid; i < kd * VS; i += kAttnThreads) S[i] = 0.f;
+    __syncthreads();
+    if (!STATE_ONLY) {
+        const float* init = nullptr;
+        long long sr = k.init.sr, sc = k.init.sc;
+        if (a.nseg > 1) {
+            init = k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd;
+            sr = k.Vd; sc = 1;
+        } else if (k.init.p) {
+            init = k.init.p + b * k.init.sb + h * k.init.sh;
+        }
+        if (init)
+            for (int i = tid; i < k.Kd * VT; i += kAttnThreads) {
+                const int r = i / VT, c = i % VT;
+                if (c < nv) S[r * VS + c] = init[r * sr + (v0 + c) * sc];
+            }
+    }
+    double total = 0.0;
+
+    for (int it = 0; it < chunks; ++it) {
+        const int t0 = t_lo + (k.rev ? chunks - 1 - it : it) * kC;
+        const int rows = min(kC, t_hi - t0), valid = max(0, min(rows, len - t0));
+        const bool run_end = !STATE_ONLY && k.anchors && ((t0 + kC) % kAnchor == 0 || t0 + kC >= a.T);
+        auto keep_state = [&] {
+            float* to = k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd + v0;
+            for (int i = tid; i < k.Kd * VT; i += kAttnThreads) {
+                const int r = i / VT, c = i % VT;
+                if (c < nv) to[(size_t)r * k.Vd + c] = S[r * VS + c];
+            }
+        };
+        __syncthreads();
+        if (run_end && k.rev) keep_state();
+        if (valid == 0) {
+            if (!STATE_ONLY) {
+                for (int i = tid; i < rows * nv; i += kAttnThreads) {
+                    const long long at = b * k.ob + (long long)(t0 + i / nv) * k.ot + h * k.oh + v0 + i % nv;
+                    if (k.out_f32) static_cast<float*>(k.out)[at] = 0.f;
+                    else store1(static_cast<io_t*>(k.out), at, 0.f);
+                }
+                if (k.dots && tid < rows) k.dots[(((size_t)blockIdx.y * a.B + b) * a.T + t0 + tid) * a.H + h] = 0.f;
+                if (run_end && !k.rev) keep_state();
+            }
+            continue;
+        }
+        if (!STATE_ONLY) load_rows(X, ks, x + (long long)t0 * k.x.st, k.x.st, valid, k.Kd, kd, k.x.vec);
+        load_rows(Y, ks, y + (long long)t0 * k.y.st, k.y.st, valid, k.Kd, kd, k.y.vec);
+        load_rows(Z, VS, z + (long long)t0 * k.z.st, k.z.st, valid, nv, VT, k.z.vec);
+        if (warp == 0) {
+            double d[2], up;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) d[j] = 2 * lane + j < valid ? attn_decay(__ldg(g + (long long)(t0 + 2 * lane + j) * a.gt)) : 0.0;
+            up = d[0] + d[1];
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const double o = __shfl_up_sync(0xffffffffu, up, s);
+                if (lane >= s) up += o;
+            }
+            const double end = __shfl_sync(0xffffffffu, up, 31);
+            d[0] = up - d[1];      // inclusive sums of the lane's two tokens
+            d[1] = up;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int t = 2 * lane + j;
+                const float hi = (float)d[j];
+                c_hi[t] = hi;
+                c_lo[t] = (float)(d[j] - hi);
+                const float from_start = ex2((float)d[j]), to_end = ex2((float)(end - d[j]));
+                w[t] = k.rev ? to_end : from_start;
+                u[t] = (k.rev ? from_start : to_end) * k.s_update;
+            }
+            if (lane == 0) *whole = ex2((float)end);
+            total += end;
+        }
+        __syncthreads();
+
+        if (!STATE_ONLY) {
+            // P = s_intra D (X Y^T), 16 rows x 32 columns a warp
+            const int pn = (warp >> 2) * 32;
+            float acc[4][4] = {};
+            if (k.rev ? pn + 31 >= wm : pn <= wm + 15) {
+                for (int kk = 0; kk < kd; kk += 8)
+                    mma_step<4>(acc, [&](int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
+                                [&](int n, int i) { return Y[(pn + n * 8 + gq) * ks + kk + tq + i * 4]; });
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = wm + gq + (i >> 1) * 8, c = pn + n * 8 + tq * 2 + (i & 1);
+                    const float d = (c_hi[r] - c_hi[c]) + (c_lo[r] - c_lo[c]);
+                    const bool on = (k.rev ? c >= r : c <= r) && c < valid && r < valid;
+                    P[r * kPStride + c] = on ? k.s_intra * ex2(k.rev ? -d : d) * acc[n][i] : 0.f;
+                }
+            __syncthreads();
+            // out, 16 rows x VT / 2 columns a warp
+            float o1[NT][4] = {}, o2[NT][4] = {};
+            const int c_from = k.rev ? wm : 0, c_to = k.rev ? kC : wm + 16;
+            for (int kk = c_from; kk < c_to; kk += 8)
+                mma_step<NT>(o1, [&](int i) { return P[(wm + gq + (i & 1) * 8) * kPStride + kk + tq + (i >> 1) * 4]; },
+                             [&](int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+            for (int kk = 0; kk < kd; kk += 8)
+                mma_step<NT>(o2, [&](int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
+                             [&](int n, int i) { return S[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = wm + gq + half * 8;
+                const float wr = k.s_inter * w[r];
+                const long long row = b * k.ob + (long long)(t0 + r) * k.ot + h * k.oh + v0;
+                const io_t* e = k.dots ? static_cast<const io_t*>(attn_at(k.e, b, h, sizeof(io_t))) + (long long)(t0 + r) * k.e.st + v0 : nullptr;
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int c = wn + n * 8 + tq * 2 + i;
+                        const float v = r < valid ? o1[n][half * 2 + i] + wr * o2[n][half * 2 + i] : 0.f;
+                        if (r < rows && c < nv) {
+                            if (k.out_f32) static_cast<float*>(k.out)[row + c] = v;
+                            else store1(static_cast<io_t*>(k.out), row + c, v);
+                            if (e && r < valid) sum += v * load1(e, c);
+                        }
+                    }
+                if (k.dots) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    if (tq == 0) dot[(warp >> 2) * kC + r] = sum;
+                }
+            }
+            __syncthreads();
+            if (k.dots && tid < rows) k.dots[(((size_t)blockIdx.y * a.B + b) * a.T + t0 + tid) * a.H + h] = dot[tid] + dot[kC + tid];
+        }
+        // state: 16 rows x VT / 2 columns at a time
+        const float decay = *whole;
+        for (int m = (warp & 3) * 16; m < kd; m += 64) {
+            float acc[NT][4] = {};
+            for (int kk = 0; kk < kC; kk += 8)
+                mma_step<NT>(acc,
+                             [&](int i) {
+                                 const int c = kk + tq + (i >> 1) * 4;
+                                 return Y[c * ks + m + gq + (i & 1) * 8] * u[c];
+                             },
+                             [&](int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float& s = S[(m + gq + (i >> 1) * 8) * VS + wn + n * 8 + tq * 2 + (i & 1)];
+                    s = fmaf(s, decay, acc[n][i]);
+                }
+        }
+        if (run_end && !k.rev) {
+            __syncthreads();
+            keep_state();
+        }
+    }
+    __syncthreads();
+    float* fin = nullptr;
+    long long sr = k.fin.sr, sc = k.fin.sc;
+    if (STATE_ONLY) {
+        fin = k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd;
+        sr = k.Vd; sc = 1;
+        if (tid == 0 && v0 == 0) k.seg_decay[(size_t)bh * a.nseg + seg] = (float)total;
+    } else if (k.fin.p && seg == (k.rev ? 0 : a.nseg - 1)) {
+        fin = k.fin.p + b * k.fin.sb + h * k.fin.sh;
+    }
+    if (fin)
+        for (int i = tid; i < k.Kd * VT; i += kAttnThreads) {
+            const int r = i / VT, c = i % VT;
+            if (c < nv) fin[r * sr + (v0 + c) * sc] = S[r * VS + c];
+        }
+}
+
+// The segments' own states become the states that they start from.
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnLaunch a) {
+    const AttnCore& k = a.core[blockIdx.z];
+    const int bh = blockIdx.x, h = bh % a.H, b = bh / a.H, n = k.Kd * k.Vd;
+    const int i = blockIdx.y * 256 + threadIdx.x;
+    if (i >= n) return;
+    float carry = k.init.p ? k.init.p[b * k.init.sb + h * k.init.sh + (i / k.Vd) * k.init.sr + (i % k.Vd) * k.init.sc] : 0.f;
+    for (int j = 0; j < a.nseg; ++j) {
+        const int seg = k.rev ? a.nseg - 1 - j : j;
+        const size_t at = (size_t)bh * a.nseg + seg;
+        const float own = k.seg_state[at * n + i];
+        k.seg_state[at * n + i] = carry;
+        carry = fmaf(carry, ex2(k.seg_decay[at]), own);
+    }
+}
+
+// e[b][h][run] = <S, R> of two kept states
+__global__ void __launch_bounds__(256) attn_anchor_kernel(const float* __restrict__ s, const float* __restrict__ r, float* __restrict__ e, int n) {
+    __shared__ float part[8];
+    const size_t at = (size_t)blockIdx.x * n;
+    float sum = 0.f;
+    for (int i = threadIdx.x; i < n; i += 256) sum = fmaf(s[at + i], r[at + i], sum);
+#pragma unroll
+    for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) sum += part[i];
+        e[blockIdx.x] = sum;
+    }
+}
+
+// The decay's gradient from the dots and the anchors: suffix sums over a run.  Dots: [blocks][B][T][H], one of dq and one of dk.
+__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* __restrict__ rq, const float* __restrict__ rk, int blocks, const float* __restrict__ e,
+                                                             const int* __restrict__ lengths, float* __restrict__ dg, int B, int T, int H, int runs) {
+    __shared__ double part[kAnchor / 32];
+    const int run = blockIdx.x % runs, bh = blockIdx.x / runs, h = bh % H, b = bh / H;
+    const int t = run * kAnchor + (kAnchor - 1 - threadIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;      // from the last token on
+    double v = 0.0;
+    if (t < T)
+        for (int j = 0; j < blocks; ++j) {
+            const size_t at = (((size_t)j * B + b) * T + t) * H + h;
+            v += (double)rq[at] - (double)rk[at];
+        }
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, v, s);
+        if (lane >= s) v += o;
+    }
+    if (lane == 31) part[warp] = v;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) v += part[i];
+    const int len = lengths ? min(max(lengths[b], 0), T) : T;
+    if (t < T) dg[((size_t)b * T + t) * H + h] = t < len ? (float)(v + (double)e[blockIdx.x]) : 0.f;
+}
+
+// Gradients of shared queries or keys: (rows,H,K) fp32 -> (rows,G,K), heads summed in order.
+template <typename io_t>
+__global__ void __launch_bounds__(256) attn_share_kernel(const float* __restrict__ p0, const float* __restrict__ p1, io_t* __restrict__ o0, io_t* __restrict__ o1, long long n,
+                                                         int K, int per) {
+    const float* p = blockIdx.y ? p1 : p0;
+    io_t* o = blockIdx.y ? o1 : o0;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        const long long rg = i / K, c = i - rg * K;
+        float sum = 0.f;
+        for (int j = 0; j < per; ++j) sum += p[(rg * per + j) * K + c];
+        store1(o, i, sum);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// One token.  The state is read and written once and nothing else is large: a CTA owns a head's state rows (or, where
+// there are few heads, some of its columns), a warp every eighth row of it, all of a thread's rows requested
+// before the first is used.
+// ------------------------------------------------------------------------------------------------
+template <typename io_t, int NV>      // NV columns a lane
+__global__ void __launch_bounds__(256) attn_step_kernel(AttnTensor q, AttnTensor k, AttnTensor v, const float* __restrict__ g, long long gb, long long gh, float scale, int H, int K, int V,
+                                                        const float* state, float* state_out, long long sb, long long sh, void* out) {
+    __shared__ float qs[M2D_ATTN_MAX_DIM], ks[M2D_ATTN_MAX_DIM], part[8][32 * NV];
+    const int h = blockIdx.x % H, b = blockIdx.x / H, c = (blockIdx.y * 32 + (threadIdx.x & 31)) * NV, warp = threadIdx.x >> 5;
+    const io_t* const qp = static_cast<const io_t*>(attn_at(q, b, h, sizeof(io_t)));
+    const io_t* const kp = static_cast<const io_t*>(attn_at(k, b, h, sizeof(io_t)));
+    const io_t* const vp = static_cast<const io_t*>(attn_at(v, b, h, sizeof(io_t)));
+    const size_t at = (size_t)(b * sb + h * sh) + c;
+    const bool on = c < V;
+    constexpr int kAhead = 16;
+    float s[kAhead][NV];
+    auto request = [&](int r0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int r = r0 + warp + j * 8;
+            if (on && r < K) {
+                const float* p = state + at + (size_t)r * V;
+                if constexpr (NV == 4) { const float4 t = *reinterpret_cast<const float4*>(p); s[j][0] = t.x; s[j][1] = t.y; s[j][2] = t.z; s[j][3] = t.w; }
+                else s[j][0] = *p;
+            }
+        }
+    };
+    request(0);
+    if (threadIdx.x < K) {
+        qs[threadIdx.x] = load1(qp, threadIdx.x);
+        ks[threadIdx.x] = load1(kp, threadIdx.x);
+    }
+    const float gv = __ldg(g + b * gb + h * gh), a = ex2((float)attn_decay(gv));
+    float vv[NV], o[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        vv[i] = on ? load1(vp, c + i) : 0.f;
+        o[i] = 0.f;
+    }
+    __syncthreads();
+    for (int r0 = 0; r0 < K; r0 += 8 * kAhead) {
+        if (r0) request(r0);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int r = r0 + warp + j * 8;
+            if (on && r < K) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    s[j][i] = fmaf(s[j][i], a, ks[r] * vv[i]);
+                    o[i] = fmaf(qs[r], s[j][i], o[i]);
+                }
+                float* p = state_out + at + (size_t)r * V;
+                if constexpr (NV == 4) *reinterpret_cast<float4*>(p) = make_float4(s[j][0], s[j][1], s[j][2], s[j][3]);
+                else *p = s[j][0];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) part[warp][(threadIdx.x & 31) * NV + i] = o[i];
+    __syncthreads();
+    const int n0 = blockIdx.y * 32 * NV;
+    for (int i = threadIdx.x; i < 32 * NV; i += 256)
+        if (n0 + i < V) {
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += part[j][i];
+            store1(static_cast<io_t*>(out), (size_t)blockIdx.x * V + n0 + i, scale * sum);
+        }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+
+static int check_attn(const m2d_attn_desc* d, bool ptrs) {
+    if (!d) return M2D_ERR_NULL;
+    if (d->struct_bytes != sizeof(m2d_attn_desc)) return M2D_ERR_ABI;
+    if (d->dtype != M2D_F32 && d->dtype != M2D_BF16) return M2D_ERR_DTYPE;
+    if (d->flags & ~(uint32_t)M2D_ATTN_CUDA_CORES) return M2D_ERR_FLAGS;
+    if (d->B < 1 || d->T < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->K < 1 || d->V < 1 || d->K > M2D_ATTN_MAX_DIM || d->V > M2D_ATTN_MAX_DIM) return M2D_ERR_SHAPE;
+    if ((int64_t)d->B * d->H > (1 << 24) || (int64_t)d->B * d->H * ((d->T + kAnchor - 1) / kAnchor) >= (1ll << 31)) return M2D_ERR_TOO_LARGE;
+    if (ptrs && (!d->q.data || !d->k.data || !d->v.data || !d->log_decay)) return M2D_ERR_NULL;
+    return M2D_OK;
+}
+
+static AttnTensor attn_tensor(const m2d_attn_desc* d, const m2d_attn_tensor& t, int per, int dim) {
+    const uintptr_t bytes = d->dtype == M2D_F32 ? 16 : 8;
+    const bool vec = dim % 4 == 0 && (reinterpret_cast<uintptr_t>(t.data) % bytes) == 0 && t.batch % 4 == 0 && t.token % 4 == 0 && t.head % 4 == 0;
+    return {t.data, t.batch, t.token, t.head, per, vec ? 1 : 0};
+}
+static AttnState dense_state(const m2d_attn_desc* d, const float* p, bool transposed) {
+    const long long n = (long long)d->K * d->V;
+    return {const_cast<float*>(p), n * d->H, n, 0, transposed ? 1 : d->V, transposed ? d->V : 1};
+}
+
+// Segments: as many as fill the GPU, none shorter than a run of kAnchor tokens.  A second pass over y and z and a
+// launch more: taken where it at least halves the time of the first.
+static void plan_segments(const m2d_attn_desc* d, long long ctas, int per_sm, AttnLaunch* a) {
+    a->runs = (d->T + kAnchor - 1) / kAnchor;
+    const long long want = ctas > 0 ? (long long)sm_count() * per_sm / ctas : 1;
+    a->nseg = 1;
+    if (want >= 2 && a->runs >= 2) a->nseg = (int)std::min<long long>(want, a->runs);
+    const int per = (a->runs + a->nseg - 1) / a->nseg;
+    a->seg_len = per * kAnchor;
+    a->nseg = (a->runs + per - 1) / per;
+}
+
+struct AttnPlan {
+    AttnLaunch a{};
+    int cores = 1, col_blocks = 1, VT = 64, dot_blocks = 1;
+    size_t smem = 0, bytes = 0;
+    size_t at_seg[3] = {}, at_decay[3] = {}, at_dots[2] = {}, at_anchor[2] = {}, at_e = 0, at_heads[2] = {};
+};
+static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd) {
+    AttnPlan p;
+    const int big = bwd ? std::max(d->K, d->V) : d->K, out = bwd ? big : d->V;
+    p.VT = big > 192 ? 32 : 64;
+    p.smem = attn_smem(big, p.VT);
+    p.col_blocks = (out + p.VT - 1) / p.VT;
+    p.cores = bwd ? 3 : 1;
+    p.dot_blocks = (d->K + p.VT - 1) / p.VT;
+    const int per_sm = std::max<int>(1, (int)((kMaxSmem + 1024) / (p.smem + 1024)));
+    plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, &p.a);
+    auto take = [&](size_t n) {
+        const size_t at = p.bytes;
+        p.bytes += (n + 255) / 256 * 256;
+        return at;
+    };
+    const size_t bh = (size_t)d->B * d->H, kv = (size_t)d->K * d->V, tokens = bh * d->T;
+    if (p.a.nseg > 1)
+        for (int i = 0; i < p.cores; ++i) {
+            p.at_seg[i] = take(4 * bh * p.a.nseg * kv);
+            p.at_decay[i] = take(4 * bh * p.a.nseg);
+        }
+    if (bwd && d->d_log_decay) {
+        for (size_t& at : p.at_dots) at = take(4 * tokens * p.dot_blocks);
+        for (size_t& at : p.at_anchor) at = take(4 * bh * p.a.runs * kv);
+        p.at_e = take(4 * bh * p.a.runs);
+    }
+    if (bwd && d->G != d->H)
+        for (size_t& at : p.at_heads) at = take(4 * tokens * d->K);
+    return p;
+}
+
+template <typename io_t, int VT>
+static int launch_core(const AttnPlan& p, cudaStream_t st) {
+    const dim3 grid((unsigned)(p.a.B * p.a.H * p.a.nseg), p.col_blocks, p.cores);
+    auto full = attn_core_kernel<io_t, VT, false>;
+    if (!allow_smem(reinterpret_cast<const void*>(full), p.smem)) return M2D_ERR_LAUNCH;
+    if (p.a.nseg > 1) {
+        auto part = attn_core_kernel<io_t, VT, true>;
+        if (!allow_smem(reinterpret_cast<const void*>(part), p.smem)) return M2D_ERR_LAUNCH;
+        part<<<grid, kAttnThreads, p.smem, st>>>(p.a);
+        const int n = p.a.core[0].Kd * p.a.core[0].Vd;
+        attn_join_kernel<<<dim3(p.a.B * p.a.H, (n + 255) / 256, p.cores), 256, 0, st>>>(p.a);
+    }
+    full<<<grid, kAttnThreads, p.smem, st>>>(p.a);
+    return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+}
+static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t st) {
+    if (d->dtype == M2D_F32) return p.VT == 64 ? launch_core<float, 64>(p, st) : launch_core<float, 32>(p, st);
+    return p.VT == 64 ? launch_core<__nv_bfloat16, 64>(p, st) : launch_core<__nv_bfloat16, 32>(p, st);
+}
+
+static void fill_launch(const m2d_attn_desc* d, AttnPlan& p) {
+    AttnLaunch& a = p.a;
+    a.g = d->log_decay; a.gb = d->g_batch; a.gt = d->g_token; a.gh = d->g_head;
+    a.lengths = d->lengths;
+    a.B = d->B; a.T = d->T; a.H = d->H;
+    char* const ws = static_cast<char*>(d->workspace);
+    for (int i = 0; i < p.cores; ++i) {
+        a.core[i].seg_state = reinterpret_cast<float*>(ws + p.at_seg[i]);
+        a.core[i].seg_decay = reinterpret_cast<float*>(ws + p.at_decay[i]);
+    }
+}
+static int check_workspace(const m2d_attn_desc* d, size_t bytes) {
+    if (!bytes) return M2D_OK;
+    return d->workspace && d->workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(d->workspace) & 255) == 0 ? M2D_OK : M2D_ERR_WORKSPACE;
+}
+
+}  // namespace m2d
+
+using namespace m2d;
+
+extern "C" uint64_t m2d_attn_fwd_workspace(const m2d_attn_desc* d) { return check_attn(d, false) == M2D_OK ? plan_attn(d, false).bytes : 0; }
+extern "C" uint64_t m2d_attn_bwd_workspace(const m2d_attn_desc* d) { return check_attn(d, false) == M2D_OK ? plan_attn(d, true).bytes : 0; }
+
+extern "C" int m2d_attn_fwd(const m2d_attn_desc* d, void* stream) {
+    int rc = check_attn(d, true);
+    if (rc != M2D_OK) return rc;
+    if (!d->o) return M2D_ERR_NULL;
+    AttnPlan p = plan_attn(d, false);
+    if ((rc = check_workspace(d, p.bytes)) != M2D_OK) return rc;
+    fill_launch(d, p);
+    AttnCore& c = p.a.core[0];
+    const int per = d->H / d->G;
+    c.x = attn_tensor(d, d->q, per, d->K); c.y = attn_tensor(d, d->k, per, d->K); c.z = attn_tensor(d, d->v, 1, d->V);
+    c.Kd = d->K; c.Vd = d->V;
+    c.out = d->o; c.oh = d->V; c.ot = (long long)d->H * d->V; c.ob = c.ot * d->T;
+    c.s_intra = c.s_inter = d->scale; c.s_update = 1.f;
+    c.init = dense_state(d, d->state, false);
+    c.fin = dense_state(d, d->state_out, false);
+    return launch_core(d, p, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
+    int rc = check_attn(d, true);
+    if (rc != M2D_OK) return rc;
+    if (!d->d_o.data || !d->d_q || !d->d_k || !d->d_v) return M2D_ERR_NULL;
+    AttnPlan p = plan_attn(d, true);
+    if ((rc = check_workspace(d, p.bytes)) != M2D_OK) return rc;
+    fill_launch(d, p);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* const ws = static_cast<char*>(d->workspace);
+    const int per = d->H / d->G;
+    const AttnTensor q = attn_tensor(d, d->q, per, d->K), k = attn_tensor(d, d->k, per, d->K), v = attn_tensor(d, d->v, 1, d->V), go = attn_tensor(d, d->d_o, 1, d->V);
+    AttnCore &dq = p.a.core[0], &dk = p.a.core[1], &dv = p.a.core[2];
+    dq.x = go; dq.y = v; dq.z = k; dq.e = q; dq.rev = 0;
+    dk.x = v; dk.y = go; dk.z = q; dk.e = k; dk.rev = 1;
+    dv.x = k; dv.y = q; dv.z = go; dv.rev = 1;
+    dq.Kd = dk.Kd = dv.Vd = d->V;
+    dq.Vd = dk.Vd = dv.Kd = d->K;
+    dq.s_intra = dq.s_inter = d->scale; dq.s_update = 1.f;
+    dk.s_intra = dv.s_intra = dk.s_update = dv.s_update = d->scale;
+    dk.s_inter = dv.s_inter = 1.f;
+    for (int i = 0; i < 2; ++i) {
+        AttnCore& c = i ? dk : dq;
+        c.out = d->G == d->H ? (i ? d->d_k : d->d_q) : ws + p.at_heads[i];
+        c.out_f32 = d->G != d->H;
+        c.oh = d->K; c.ot = (long long)d->H * d->K; c.ob = c.ot * d->T;
+        if (d->d_log_decay) {
+            c.dots = reinterpret_cast<float*>(ws + p.at_dots[i]);
+            c.anchors = reinterpret_cast<float*>(ws + p.at_anchor[i]);
+        }
+    }
+    dv.out = d->d_v; dv.oh = d->V; dv.ot = (long long)d->H * d->V; dv.ob = dv.ot * d->T;
+    dq.init = dense_state(d, d->state, true);
+    dk.init = dense_state(d, d->d_state_out, true);
+    dv.init = dense_state(d, d->d_state_out, false);
+    dv.fin = dense_state(d, d->d_state, false);
+    if ((rc = launch_core(d, p, st)) != M2D_OK) return rc;
+    if (d->d_log_decay) {
+        float* const e = reinterpret_cast<float*>(ws + p.at_e);
+        const unsigned n = (unsigned)(d->B * d->H * p.a.runs);
+        attn_anchor_kernel<<<n, 256, 0, st>>>(dq.anchors, dk.anchors, e, d->K * d->V);
+        attn_decay_kernel<<<n, kAnchor, 0, st>>>(dq.dots, dk.dots, p.dot_blocks, e, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs);
+    }
+    if (d->G != d->H) {
+        const long long n = (long long)d->B * d->T * d->G * d->K;
+        const dim3 grid((unsigned)std::min<long long>((n + 255) / 256, 16ll * sm_count()), 2);
+        const float *h0 = reinterpret_cast<const float*>(ws + p.at_heads[0]), *h1 = reinterpret_cast<const float*>(ws + p.at_heads[1]);
+        if (d->dtype == M2D_F32) attn_share_kernel<float><<<grid, 256, 0, st>>>(h0, h1, static_cast<float*>(d->d_q), static_cast<float*>(d->d_k), n, d->K, per);
+        else attn_share_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(h0, h1, static_cast<__nv_bfloat16*>(d->d_q), static_cast<__nv_bfloat16*>(d->d_k), n, d->K, per);
+    }
+    return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+}
+
+extern "C" int m2d_attn_step(const m2d_attn_desc* d, int64_t state_batch, int64_t state_head, void* stream) {
+    const int rc = check_attn(d, true);
+    if (rc != M2D_OK) return rc;
+    if (d->T != 1) return M2D_ERR_SHAPE;
+    if (!d->o || !d->state || !d->state_out) return M2D_ERR_NULL;
+    const int per = d->H / d->G;
+    const AttnTensor q = attn_tensor(d, d->q, per, d->K), k = attn_tensor(d, d->k, per, d->K), v = attn_tensor(d, d->v, 1, d->V);
+    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    const bool vec = d->V % 4 == 0 && state_batch % 4 == 0 && state_head % 4 == 0 && aligned(d->state) && aligned(d->state_out);
+    const dim3 grid(d->B * d->H, (d->V + (vec ? 127 : 31)) / (vec ? 128 : 32));
+    auto launch = [&](auto kern) {
+        kern<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(q, k, v, d->log_decay, d->g_batch, d->g_head, d->scale, d->H, d->K, d->V, d->state, d->state_out, state_batch, state_head, d->o);
+    };
+    if (d->dtype == M2D_F32) vec ? launch(attn_step_kernel<float, 4>) : launch(attn_step_kernel<float, 1>);
+    else vec ? launch(attn_step_kernel<__nv_bfloat16, 4>) : launch(attn_step_kernel<__nv_bfloat16, 1>);
+    return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+}

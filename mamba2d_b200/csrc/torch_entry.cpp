@@ -567,7 +567,10 @@ c10::optional<Tensor> scan(const Tensor& x, const Tensor& dT, const Tensor& dL, 
 
 }  // namespace
 
+void bind_sequence_operators(pybind11::module& m);      // torch_seq.cpp
+
 PYBIND11_MODULE(_entry, m) {
+    bind_sequence_operators(m);
     // check_status: raise where a launch whose CTAs wait on one another went wrong (looked_at); the hooks are test hooks of include/m2d_scan.h
     using pybind11::arg;
     m.def("block", &block, "wavefront_scan_cuda as one autograd node; None where it does not apply", arg("x"), arg("AT_log"), arg("AL_log"),

@@ -1,0 +1,318 @@
+// Eager entry points of the sequence operators (sequence.py): linear attention, group normalisation, clipping.
+//
+// Their arguments have been checked and cast by sequence.py; what is checked here is what the kernels rely on.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "m2d_seq.h"
+
+namespace {
+
+using at::Tensor;
+using c10::optional;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check(int rc, const char* fn) { TORCH_CHECK(rc == M2D_OK, fn, " failed: ", m2d_strerror(rc), " (status ", rc, ")"); }
+void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? M2D_F32 : M2D_BF16; }
+Tensor scratch(uint64_t bytes, const Tensor& like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
+
+// Whether a call on these makes a node (one with a forward-mode tangent does: the node refuses it).
+bool wants_grad(std::initializer_list<const Tensor*> inputs) {
+    bool grad = false;
+    for (const Tensor* t : inputs)
+        if (t->defined()) grad = grad || (at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
+    return grad;
+}
+Tensor or_none(const optional<Tensor>& t) { return t ? *t : Tensor(); }
+// neighbours along the last dimension
+Tensor rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+m2d_attn_tensor attn_tensor(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+void wrote(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// ---- linear attention -------------------------------------------------------------------------------
+
+struct Attn {
+    Tensor q, k, v, g, state, lengths;        // as the kernels read them
+    m2d_attn_desc d{};
+    Attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& state_, const Tensor& lengths_, double scale, int64_t flags)
+        : q(rows(q_)), k(rows(k_)), v(rows(v_)), g(g_), state(dense(state_)), lengths(dense(lengths_)) {
+        d.struct_bytes = sizeof(d);
+        d.dtype = dtype_of(v);
+        d.B = (int)v.size(0); d.T = (int)v.size(1); d.H = (int)v.size(2); d.V = (int)v.size(3);
+        d.G = (int)q.size(2); d.K = (int)q.size(3);
+        d.flags = (uint32_t)flags;
+        d.scale = (float)scale;
+        d.q = attn_tensor(q); d.k = attn_tensor(k); d.v = attn_tensor(v);
+        d.log_decay = fptr(g);
+        const bool per_head = g.dim() == 1;
+        d.g_batch = per_head ? 0 : g.stride(0);
+        d.g_token = per_head ? 0 : g.stride(1);
+        d.g_head = per_head ? g.stride(0) : g.stride(2);
+        d.state = fptr(state);
+        d.lengths = static_cast<const int32_t*>(ptr(lengths));
+    }
+};
+
+Tensor attn_forward(Attn& a, Tensor* state_out) {
+    const Tensor o = at::empty({a.d.B, a.d.T, a.d.H, a.d.V}, a.v.options());
+    a.d.o = o.data_ptr();
+    if (state_out) {
+        *state_out = at::empty({a.d.B, a.d.H, a.d.K, a.d.V}, a.v.options().dtype(at::kFloat));
+        a.d.state_out = fptr(*state_out);
+    }
+    a.d.workspace_bytes = m2d_attn_fwd_workspace(&a.d);
+    Tensor ws;
+    if (a.d.workspace_bytes) {
+        ws = scratch(a.d.workspace_bytes, a.v);
+        a.d.workspace = ws.data_ptr();
+    }
+    check(m2d_attn_fwd(&a.d, stream_of(a.v)), "m2d_attn_fwd");
+    return o;
+}
+
+class AttnFn : public torch::autograd::Function<AttnFn> {
+public:
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const optional<Tensor>& state_,
+                                 const optional<Tensor>& lengths_, double scale, bool want_state, int64_t flags) {
+        const Tensor state = or_none(state_), lengths = or_none(lengths_);
+        const c10::cuda::CUDAGuard guard(v.device());
+        Attn a(q, k, v, g, state, lengths, scale, flags);
+        Tensor out_state;
+        const Tensor o = attn_forward(a, want_state ? &out_state : nullptr);
+        ctx->save_for_backward({q, k, v, g, state, lengths});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["flags"] = flags;
+        ctx->set_materialize_grads(false);
+        return want_state ? variable_list{o, out_state} : variable_list{o};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const at::NoGradGuard no_grad;
+        const variable_list s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[2].device());
+        const bool have_state_grad = grads.size() > 1 && grads[1].defined();
+        if (!grads[0].defined() && !have_state_grad) return variable_list(9);
+        Attn a(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["flags"].toInt());
+        m2d_attn_desc& d = a.d;
+        const Tensor d_o = grads[0].defined() ? rows(grads[0].to(a.v.scalar_type())) : at::zeros(a.v.sizes(), a.v.options());
+        const Tensor d_out = have_state_grad ? grads[1].to(at::kFloat).contiguous() : Tensor();
+        d.d_o = attn_tensor(d_o);
+        d.d_state_out = fptr(d_out);
+        Tensor dq = at::empty({d.B, d.T, d.G, d.K}, a.v.options()), dk = at::empty_like(dq), dv = at::empty({d.B, d.T, d.H, d.V}, a.v.options());
+        d.d_q = dq.data_ptr(); d.d_k = dk.data_ptr(); d.d_v = dv.data_ptr();
+        Tensor dg, ds;
+        if (s[3].requires_grad()) {
+            dg = at::empty({d.B, d.T, d.H}, a.g.options());
+            d.d_log_decay = fptr(dg);
+        }
+        if (s[4].defined() && s[4].requires_grad()) {
+            ds = at::empty(s[4].sizes(), s[4].options());
+            d.d_state = fptr(ds);
+        }
+        d.workspace_bytes = m2d_attn_bwd_workspace(&d);
+        Tensor ws;
+        if (d.workspace_bytes) {
+            ws = scratch(d.workspace_bytes, a.v);
+            d.workspace = ws.data_ptr();
+        }
+        check(m2d_attn_bwd(&d, stream_of(a.v)), "m2d_attn_bwd");
+        if (dg.defined() && s[3].dim() == 1) dg = dg.sum(at::IntArrayRef{0, 1});
+        return {dq, dk, dv, dg, ds, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+void check_devices(const Tensor& like, std::initializer_list<const Tensor*> others) {
+    for (const Tensor* t : others) TORCH_CHECK(!t->defined() || t->device() == like.device(), "linear attention: tensors on ", t->device(), " and ", like.device());
+}
+void check_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state, int64_t tokens_dims) {
+    TORCH_CHECK(v.is_cuda() && (v.scalar_type() == at::kFloat || v.scalar_type() == at::kBFloat16) && q.scalar_type() == v.scalar_type() && k.scalar_type() == v.scalar_type(),
+                "linear attention: q, k, v must be CUDA tensors of one type, float32 or bfloat16");
+    TORCH_CHECK(g.scalar_type() == at::kFloat && (!state.defined() || state.scalar_type() == at::kFloat), "linear attention: decays and states are float32");
+    TORCH_CHECK(v.dim() == tokens_dims + 2 && q.dim() == v.dim() && k.dim() == v.dim(), "linear attention: q, k, v have ", tokens_dims + 2, " dimensions");
+    for (const Tensor* t : {&q, &k, &v}) TORCH_CHECK(t->numel() > 0 && t->size(0) <= INT_MAX && t->size(1) <= INT_MAX, "linear attention: a size out of range");
+}
+
+std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale, const optional<Tensor>& state_,
+                                                      const optional<Tensor>& lengths_, bool want_state, int64_t flags) {
+    const Tensor state = or_none(state_), lengths = or_none(lengths_);
+    check_attn(q, k, v, g, state, 2);
+    check_devices(v, {&q, &k, &g, &state, &lengths});
+    TORCH_CHECK(!lengths.defined() || lengths.scalar_type() == at::kInt, "linear attention: lengths are int32");
+    if (wants_grad({&q, &k, &v, &g, &state})) {
+        const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths_, scale, want_state, flags);
+        return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
+    }
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(v.device());
+    Attn a(q, k, v, g, state, lengths, scale, flags);
+    Tensor out_state;
+    const Tensor o = attn_forward(a, want_state ? &out_state : nullptr);
+    return {o, want_state ? optional<Tensor>(out_state) : c10::nullopt};
+}
+
+Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale, const Tensor& state) {
+    check_attn(q, k, v, g, state, 1);
+    check_devices(v, {&q, &k, &g, &state});
+    TORCH_CHECK(!wants_grad({&q, &k, &v, &g, &state}), "linear_attention_step updates the state in place and has no gradients: call it without gradients");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(v.device());
+    const Tensor qr = rows(q), kr = rows(k), vr = rows(v);
+    m2d_attn_desc d{};
+    d.struct_bytes = sizeof(d);
+    d.dtype = dtype_of(v);
+    d.B = (int)v.size(0); d.T = 1; d.H = (int)v.size(1); d.V = (int)v.size(2);
+    d.G = (int)q.size(1); d.K = (int)q.size(2);
+    d.scale = (float)scale;
+    auto token = [](const Tensor& t) { return m2d_attn_tensor{t.data_ptr(), t.stride(0), 0, t.stride(1)}; };
+    d.q = token(qr); d.k = token(kr); d.v = token(vr);
+    d.log_decay = fptr(g);
+    d.g_batch = g.dim() == 1 ? 0 : g.stride(0);
+    d.g_head = g.stride(-1);
+    d.state = d.state_out = fptr(state);
+    const Tensor o = at::empty({d.B, d.H, d.V}, v.options());
+    d.o = o.data_ptr();
+    check(m2d_attn_step(&d, state.stride(0), state.stride(1), stream_of(v)), "m2d_attn_step");
+    wrote(state);
+    return o;
+}
+
+// ---- group normalisation ----------------------------------------------------------------------------
+
+m2d_norm_desc norm_desc(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, int64_t act, double eps) {
+    m2d_norm_desc d{};
+    d.struct_bytes = sizeof(d);
+    d.dtype = dtype_of(x);
+    d.N = x.size(0); d.C = (int)x.size(-1);
+    d.S = x.numel() / (d.N * d.C);
+    d.groups = (int)groups; d.act = (int)act; d.eps = (float)eps;
+    const Tensor& p = weight.defined() ? weight : bias;
+    d.params_f32 = p.defined() && p.scalar_type() == at::kFloat;
+    d.x = x.data_ptr(); d.weight = ptr(weight); d.bias = ptr(bias);
+    return d;
+}
+Tensor norm_forward(m2d_norm_desc& d, const Tensor& x) {
+    const Tensor y = at::empty(x.sizes(), x.options());
+    d.y = y.data_ptr();
+    d.workspace_bytes = m2d_norm_fwd_workspace(&d);
+    Tensor ws;
+    if (d.workspace_bytes) {
+        ws = scratch(d.workspace_bytes, x);
+        d.workspace = ws.data_ptr();
+    }
+    check(m2d_norm_fwd(&d, stream_of(x)), "m2d_norm_fwd");
+    return y;
+}
+
+class NormFn : public torch::autograd::Function<NormFn> {
+public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, int64_t groups, int64_t act, double eps) {
+        const Tensor weight = or_none(weight_), bias = or_none(bias_);
+        const c10::cuda::CUDAGuard guard(x_.device());
+        const Tensor x = x_.contiguous(), w = dense(weight), b = dense(bias);
+        m2d_norm_desc d = norm_desc(x, w, b, groups, act, eps);
+        const Tensor stats = at::empty({d.N, d.groups, 2}, x.options().dtype(at::kFloat));
+        d.stats = fptr(stats);
+        const Tensor y = norm_forward(d, x);
+        ctx->save_for_backward({x_, weight, bias, stats});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["eps"] = eps;
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const at::NoGradGuard no_grad;
+        const variable_list s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[0].device());
+        const Tensor x = s[0].contiguous(), w = dense(s[1]), b = dense(s[2]), dy = grads[0].to(x.scalar_type()).contiguous();
+        m2d_norm_desc d = norm_desc(x, w, b, ctx->saved_data["groups"].toInt(), ctx->saved_data["act"].toInt(), ctx->saved_data["eps"].toDouble());
+        d.stats = fptr(s[3]);
+        d.d_y = dy.data_ptr();
+        const Tensor dx = at::empty(x.sizes(), x.options());
+        d.d_x = dx.data_ptr();
+        Tensor dw, db;
+        if ((w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())) {
+            const auto options = w.defined() ? w.options() : b.options();
+            dw = at::empty({d.C}, options);
+            db = at::empty({d.C}, options);
+            d.d_weight = dw.data_ptr();
+            d.d_bias = db.data_ptr();
+        }
+        d.workspace_bytes = m2d_norm_bwd_workspace(&d);
+        Tensor ws;
+        if (d.workspace_bytes) {
+            ws = scratch(d.workspace_bytes, x);
+            d.workspace = ws.data_ptr();
+        }
+        check(m2d_norm_bwd(&d, stream_of(x)), "m2d_norm_bwd");
+        return {dx, w.defined() ? dw : Tensor(), b.defined() ? db : Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor group_norm(const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, int64_t groups, int64_t act, double eps) {
+    const Tensor weight = or_none(weight_), bias = or_none(bias_);
+    TORCH_CHECK(x_.is_cuda() && (x_.scalar_type() == at::kFloat || x_.scalar_type() == at::kBFloat16), "group_norm: x must be a CUDA tensor, float32 or bfloat16");
+    TORCH_CHECK(x_.dim() >= 2 && x_.numel() > 0 && x_.size(-1) <= INT_MAX, "group_norm: x is (N, ..., C)");
+    for (const Tensor* p : {&weight, &bias})
+        if (p->defined())
+            TORCH_CHECK(p->device() == x_.device() && p->sizes() == at::IntArrayRef({x_.size(-1)}) && (p->scalar_type() == at::kFloat || p->scalar_type() == x_.scalar_type()) &&
+                            (!weight.defined() || p->scalar_type() == weight.scalar_type()),
+                        "group_norm: weight and bias are (C), on x's device, of one type, float32 or x's");
+    if (wants_grad({&x_, &weight, &bias})) return NormFn::apply(x_, weight_, bias_, groups, act, eps);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = x_.contiguous(), w = dense(weight), b = dense(bias);
+    m2d_norm_desc d = norm_desc(x, w, b, groups, act, eps);
+    return norm_forward(d, x);
+}
+
+// ---- clipping ---------------------------------------------------------------------------------------
+
+Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm) {
+    TORCH_CHECK(!grads.empty(), "clip_grad_norm_: no gradients");
+    const Tensor& first = grads[0];
+    std::vector<m2d_clip_tensor> table;
+    std::vector<std::pair<const char*, const char*>> spans;
+    table.reserve(grads.size());
+    spans.reserve(grads.size());
+    for (const Tensor& g : grads) {
+        TORCH_CHECK(g.layout() == at::kStrided && g.is_cuda() && (g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16),
+                    "clip_grad_norm_: gradients must be CUDA tensors, float32 or bfloat16");
+        TORCH_CHECK(g.device() == first.device(), "clip_grad_norm_: gradients on ", g.device(), " and ", first.device());
+        TORCH_CHECK(g.is_non_overlapping_and_dense(), "clip_grad_norm_: a gradient has gaps or overlaps itself (sizes ", g.sizes(), ", strides ", g.strides(), ")");
+        if (!g.numel()) continue;
+        table.push_back({g.data_ptr(), g.numel(), dtype_of(g)});
+        const char* p = static_cast<const char*>(g.data_ptr());
+        spans.emplace_back(p, p + g.numel() * g.element_size());
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i) TORCH_CHECK(spans[i - 1].second <= spans[i].first, "clip_grad_norm_: two gradients share memory");
+    const c10::cuda::CUDAGuard guard(first.device());
+    const Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
+    const uint64_t bytes = m2d_clip_workspace(table.data(), (int32_t)table.size());
+    const Tensor ws = scratch(bytes, first);
+    check(m2d_clip_grad_norm(table.data(), (int32_t)table.size(), (float)max_norm, fptr(norm), ws.data_ptr(), bytes, stream_of(first)), "m2d_clip_grad_norm");
+    for (const Tensor& g : grads) wrote(g);
+    return norm;
+}
+
+}  // namespace
+
+void bind_sequence_operators(pybind11::module& m) {
+    using pybind11::arg;
+    m.def("linear_attention", &linear_attention, "linear attention of whole sequences: (o, state or None)", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale"),
+          arg("state").none(true), arg("lengths").none(true), arg("want_state"), arg("flags") = 0);
+    m.def("linear_attention_step", &linear_attention_step, "linear attention of one token; the state is updated in place", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale"),
+          arg("state"));
+    m.def("group_norm", &group_norm, "group normalisation with an activation, channels last", arg("x"), arg("weight").none(true), arg("bias").none(true), arg("groups"), arg("act"),
+          arg("eps"));
+    m.def("clip_grad_norm", &clip_grad_norm, "global norm; the tensors are scaled in place", arg("grads"), arg("max_norm"));
+}

@@ -22,6 +22,7 @@ import torch
 import torch.nn as nn
 
 from . import inject
+from .sequence import clip_grad_norm_
 
 _REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -113,11 +114,12 @@ def make_optimizer(model, lr=0.004, weight_decay=0.05):
     return torch.optim.AdamW(param_groups(model, weight_decay), lr=lr, betas=(0.9, 0.999), eps=1e-8)
 
 
-def train_step(model, optimizer, images, labels, micro_batch, autocast_dtype=torch.bfloat16):
+def train_step(model, optimizer, images, labels, micro_batch, autocast_dtype=torch.bfloat16, max_grad_norm=None):
     """One optimiser step on this rank's share of the global batch: forward + backward over
     micro-batches (gradients accumulate; under DistributedDataParallel only the last micro-batch
     triggers the weight-gradient all-reduce), then AdamW.  Cross-entropy on hard labels, mean over the
-    rank's whole share.  Returns the loss (a detached scalar tensor)."""
+    rank's whole share.  With ``max_grad_norm`` the gradients are clipped by their global norm first
+    (``clip_grad_norm_``; CUDA gradients).  Returns the loss (a detached scalar tensor)."""
     n = images.shape[0]
     chunks = [(s, min(s + micro_batch, n)) for s in range(0, n, micro_batch)]
     optimizer.zero_grad(set_to_none=True)
@@ -133,5 +135,7 @@ def train_step(model, optimizer, images, labels, micro_batch, autocast_dtype=tor
             loss = torch.nn.functional.cross_entropy(logits.float(), labels[s:e], reduction="sum") / n
             loss.backward()
         total = loss.detach() if total is None else total + loss.detach()
+    if max_grad_norm is not None:
+        clip_grad_norm_([p for group in optimizer.param_groups for p in group["params"]], max_grad_norm)
     optimizer.step()
     return total

@@ -1,0 +1,193 @@
+"""Sequence operators next to the 2-D scan: linear attention with a decay per head (the scan's relative in one dimension,
+with a matrix for a state), group normalisation with an activation on the channels-last tensors that all of this
+package works on, and clipping of gradients by their global norm.
+
+  linear_attention(q, k, v, log_decay, ...)         whole sequences, forward and backward
+  linear_attention_step(q, k, v, log_decay, state)  one token of every sequence, the state updated in place
+  group_norm(x, groups, weight, bias, ...)          x (N, ..., C)
+  clip_norm_(tensors, max_norm)                     global norm of many tensors, all scaled in place
+  clip_grad_norm_(parameters, max_norm)             of parameters' gradients: what ``refmodel.train_step`` calls
+
+Like the scan they run on the current stream, take float32 and bfloat16 tensors, compute and carry state in float32, and
+have no CPU or PyTorch path: tensors elsewhere, of another type or shape raise ``RuntimeError``; an option out of range
+raises ``ValueError``.  The kernels are behind the C ABI in ``include/m2d_seq.h``.
+"""
+import torch
+
+from . import _lib
+
+__all__ = ["linear_attention", "linear_attention_step", "group_norm", "clip_norm_", "clip_grad_norm_"]
+
+_TYPES = (torch.float32, torch.bfloat16)
+_ACTS = {None: 0, "silu": 1, "gelu": 2}
+
+
+def _check_attention(q, k, v, log_decay, state, tokens, what):
+    if v.dim() != len(tokens) + 2:
+        raise RuntimeError(f"{what}: v must be ({', '.join(tokens)}, H, V), got {tuple(v.shape)}")
+    lead, (H, V) = tuple(v.shape[:-2]), v.shape[-2:]
+    if q.dim() != v.dim() or tuple(q.shape[:-2]) != lead or k.shape != q.shape:
+        raise RuntimeError(f"{what}: q and k must be ({', '.join(tokens)}, G, K) next to v {tuple(v.shape)}, got {tuple(q.shape)} and {tuple(k.shape)}")
+    G, K = q.shape[-2:]
+    if H < 1 or G < 1 or H % G:
+        raise RuntimeError(f"{what}: {G} heads of q and k cannot be shared by {H} heads of v")
+    if not 1 <= K <= _lib.ATTN_MAX_DIM or not 1 <= V <= _lib.ATTN_MAX_DIM:
+        raise RuntimeError(f"{what}: head sizes of 1 to {_lib.ATTN_MAX_DIM}, got K={K}, V={V}")
+    if tuple(log_decay.shape) not in ((H,), lead + (H,)):
+        raise RuntimeError(f"{what}: log_decay must be {(H,)} or {lead + (H,)}, got {tuple(log_decay.shape)}")
+    if not log_decay.is_floating_point():
+        raise RuntimeError(f"{what}: log_decay has dtype {log_decay.dtype}")
+    if state is not None and (tuple(state.shape) != (lead[0], H, K, V) or state.dtype != torch.float32):
+        raise RuntimeError(f"{what}: the state must be {(lead[0], H, K, V)} in float32, got {tuple(state.shape)} {state.dtype}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype not in _TYPES or t.dtype != v.dtype:
+            raise RuntimeError(f"{what}: {name} has dtype {t.dtype}; q, k and v share one, float32 or bfloat16")
+    if not v.is_cuda:
+        raise RuntimeError(f"{what}: tensors must be on a CUDA device (there is no CPU path)")
+    for name, t in (("q", q), ("k", k), ("log_decay", log_decay), ("state", state)):
+        if t is not None and t.device != v.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, expected {v.device}")
+    return K
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
+    """``S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T``, ``o_t = scale q_t^T S_t`` for every sequence and head.
+
+    Args:
+        q, k: (B, T, G, K); G divides H, each of their heads is shared by H / G neighbouring heads of v.
+        v: (B, T, H, V).  Any strides (a last dimension that is not dense is copied); K and V up to 256.
+        log_decay: (H,), a fixed decay per head, or (B, T, H), one per token; used in float32.  At most 0: a
+            positive value grows the state and is not checked for.  -inf forgets all earlier tokens.
+        scale: default ``K ** -0.5``.
+        initial_state: (B, H, K, V) float32, or None for zero.
+        lengths: (B,) integers on the device, tokens of each sequence (clamped to 0 ... T), or None for T.  Rows
+            behind them are not read; outputs and gradients there are zero.
+        return_state: also return the state after each sequence's last token, (B, H, K, V) float32.
+    Returns:
+        o (B, T, H, V) in ``v.dtype``, or ``(o, state)``.
+    Differentiable in q, k, v, log_decay and initial_state, through o and the state.  A token that is not finite
+    may spoil the outputs of up to 127 tokens before it, besides all later ones of its sequence and head.
+    """
+    what = "linear_attention"
+    K = _check_attention(q, k, v, log_decay, initial_state, ("B", "T"), what)
+    B, T, H, V = v.shape
+    if lengths is not None:
+        if tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"{what}: lengths must be {(B,)} integers, got {tuple(lengths.shape)} {lengths.dtype}")
+        if lengths.device != v.device:
+            raise RuntimeError(f"{what}: lengths are on {lengths.device}, expected {v.device}")
+        lengths = lengths.clamp(max=T).to(torch.int32) if lengths.dtype == torch.int64 else lengths
+    scale = K ** -0.5 if scale is None else float(scale)
+    if B == 0 or T == 0:
+        if not return_state:
+            return v.clone()
+        zero = initial_state if initial_state is not None else torch.zeros(B, H, K, V, device=v.device)
+        return v.clone(), zero.clone()
+    o, state = _lib.entry().linear_attention(q, k, v, log_decay.float(), scale, initial_state, lengths, return_state)
+    return (o, state) if return_state else o
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
+    """One token of every sequence: ``state`` becomes ``exp(log_decay) state + k v^T`` in place, and the result is
+    ``scale q^T state``.
+
+    Args:
+        q, k: (B, G, K); v: (B, H, V); log_decay: (H,) or (B, H); as ``linear_attention`` takes them.
+        state: (B, H, K, V) float32 with dense (K, V); sequences and heads may lie apart (a layer's slice of a
+            cache) but must not overlap.
+    No gradients: it raises where one is wanted.
+    """
+    what = "linear_attention_step"
+    if state is None:
+        raise RuntimeError(f"{what}: there is no state")
+    K = _check_attention(q, k, v, log_decay, state, ("B",), what)
+    B, H, V = v.shape
+    if B == 0:
+        return v.clone()
+    sb, sh, sk, sv = state.stride()
+    span = K * V
+    dense = (V == 1 or sv == 1) and (K == 1 or sk == V)
+    apart = all(n == 1 or s >= span for n, s in ((B, sb), (H, sh))) and (B == 1 or H == 1 or sb >= (H - 1) * sh + span or sh >= (B - 1) * sb + span)
+    if not dense or not apart:
+        raise RuntimeError(f"{what}: the state must be dense in (K, V) and must not overlap itself, got strides {state.stride()}")
+    return _lib.entry().linear_attention_step(q, k, v, log_decay.float(), K ** -0.5 if scale is None else float(scale), state)
+
+
+def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None):
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)``, channels last.
+
+    Args:
+        x: (N, ..., C).  Mean and (biased) variance are taken over everything between the first and the last
+            dimension and the C / groups channels of a group.  For a norm over the heads of each token pass
+            (tokens, heads * size) with ``groups = heads``.
+        weight, bias: (C,) or None; float32, or both of x's type.
+        act: None, "silu" or "gelu" (erf form, as the block's ``act2``, models/mamba2d.py:169).
+    Differentiable in x, weight and bias.
+    """
+    if act not in _ACTS:
+        raise ValueError(f"Unknown activation, got {act}...")
+    if x.dim() < 2:
+        raise RuntimeError(f"group_norm: x must be (N, ..., C), got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if not isinstance(groups, int) or groups < 1 or C % groups:
+        raise ValueError(f"group_norm: {C} channels do not make {groups} groups")
+    if not eps >= 0:
+        raise ValueError(f"group_norm: eps must not be negative, got {eps}")
+    if x.dtype not in _TYPES:
+        raise RuntimeError(f"group_norm: unsupported dtype {x.dtype} (float32 and bfloat16 only)")
+    if not x.is_cuda:
+        raise RuntimeError("group_norm: tensors must be on a CUDA device (there is no CPU path)")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if tuple(p.shape) != (C,):
+            raise RuntimeError(f"group_norm: {name} must have shape {(C,)}, got {tuple(p.shape)}")
+        if p.dtype not in (torch.float32, x.dtype) or (weight is not None and p.dtype != weight.dtype):
+            raise RuntimeError(f"group_norm: {name} has dtype {p.dtype}; weight and bias share one, float32 or {x.dtype}")
+        if p.device != x.device:
+            raise RuntimeError(f"group_norm: {name} is on {p.device}, expected {x.device}")
+    if x.numel() == 0:
+        return x.clone()
+    return _lib.entry().group_norm(x, weight, bias, groups, _ACTS[act], float(eps))
+
+
+def clip_norm_(tensors, max_norm, error_if_nonfinite=False):
+    """Scale tensors in place so that their global 2-norm is at most ``max_norm``; returns the norm before (float32, on
+    the device).
+
+    The factor is ``max_norm / (norm + 1e-6)``, at most 1; an infinite norm makes finite values zero and infinite ones
+    NaN, a NaN spoils everything.  Two launches for up to 512 tensors; nothing is written where the factor is 1.  The sum
+    is taken in an order that does not change, in float64 beyond a thread's share of 32 KB.
+
+    Args:
+        tensors: one or several; float32 or bfloat16, on one device, without gaps; they share no memory.
+        max_norm: not negative; ``inf`` only measures.
+        error_if_nonfinite: raise where the norm is infinite or NaN, before anything is scaled (waits for the GPU).
+    """
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_norm_: max_norm must not be negative, got {max_norm}")
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError("clip_norm_: tensors must be on a CUDA device (there is no CPU path)")
+        if t.dtype not in _TYPES:
+            raise RuntimeError(f"clip_norm_: unsupported dtype {t.dtype} (float32 and bfloat16 only)")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("clip_norm_: a tensor that requires a gradient is not scaled in place")
+    entry = _lib.entry()
+    if error_if_nonfinite:
+        total = entry.clip_grad_norm(tensors, float("inf"))
+        if not bool(torch.isfinite(total)):
+            raise RuntimeError(f"clip_norm_: the norm is {float(total)}; the tensors are left as they were")
+    return entry.clip_grad_norm(tensors, max_norm)
+
+
+def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+    """``clip_norm_`` of the parameters' gradients, as ``torch.nn.utils.clip_grad_norm_``: parameters (one or several)
+    without a gradient are skipped."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    with torch.no_grad():
+        return clip_norm_([p.grad for p in parameters if p.grad is not None], max_norm, error_if_nonfinite)
