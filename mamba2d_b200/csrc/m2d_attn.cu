@@ -1,5 +1,7 @@
-// Linear attention: entry points, and the kernels for any head size, type and alignment.
+// Linear attention: entry points, and the kernels for any head size, type and alignment (attn_tc.cuh has the tcgen05 form).
 #include "attn_core.cuh"
+#include "attn_tc.cuh"
+#include "launch.cuh"
 
 namespace m2d {
 
@@ -449,19 +451,24 @@ static void plan_segments(const m2d_attn_desc* d, long long ctas, int per_sm, At
 
 struct AttnPlan {
     AttnLaunch a{};
+    bool tc = false;
     int cores = 1, col_blocks = 1, VT = 64, dot_blocks = 1;
     size_t smem = 0, bytes = 0;
     size_t at_seg[3] = {}, at_decay[3] = {}, at_dots[2] = {}, at_anchor[2] = {}, at_e = 0, at_heads[2] = {};
 };
-static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd) {
+static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     AttnPlan p;
-    const int big = bwd ? std::max(d->K, d->V) : d->K, out = bwd ? big : d->V;
-    p.VT = big > 192 ? 32 : 64;
-    p.smem = attn_smem(big, p.VT);
-    p.col_blocks = (out + p.VT - 1) / p.VT;
+    p.tc = tc;
     p.cores = bwd ? 3 : 1;
-    p.dot_blocks = (d->K + p.VT - 1) / p.VT;
-    const int per_sm = std::max<int>(1, (int)((kMaxSmem + 1024) / (p.smem + 1024)));
+    int per_sm = 1;
+    if (!tc) {
+        const int big = bwd ? std::max(d->K, d->V) : d->K, out = bwd ? big : d->V;
+        p.VT = big > 192 ? 32 : 64;
+        p.smem = attn_smem(big, p.VT);
+        p.col_blocks = (out + p.VT - 1) / p.VT;
+        p.dot_blocks = (d->K + p.VT - 1) / p.VT;
+        per_sm = std::max<int>(1, (int)((kMaxSmem + 1024) / (p.smem + 1024)));
+    }
     plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, &p.a);
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
@@ -484,8 +491,64 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd) {
     return p;
 }
 
+// Whether the tcgen05 form takes the call: bf16, head sizes of whole 16-byte pieces up to 128, and tensors that TMA can address.
+static bool tc_applies(const m2d_attn_desc* d, bool bwd) {
+    if (d->dtype != M2D_BF16 || (d->flags & M2D_ATTN_CUDA_CORES) || d->K > 128 || d->V > 128 || d->K % 8 || d->V % 8 || !tc_encoder()) return false;
+    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    auto fits = [&](const m2d_attn_tensor& t, int heads) {
+        auto stride = [](int n, int64_t s) { return n == 1 || (s > 0 && s % 8 == 0 && s < (1ll << 36)); };
+        return aligned(t.data) && stride(d->B, t.batch) && stride(d->T, t.token) && stride(heads, t.head);
+    };
+    if (!fits(d->q, d->G) || !fits(d->k, d->G) || !fits(d->v, d->H)) return false;
+    return bwd ? fits(d->d_o, d->H) && aligned(d->d_q) && aligned(d->d_k) && aligned(d->d_v) : aligned(d->o);
+}
+
+static bool attn_map(CUtensorMap* map, const m2d_attn_desc* d, const AttnTensor& t, int dim) {
+    const int heads = d->H / t.per;
+    // (a stride that no step is taken along may be anything: the map gets a valid one)
+    auto bytes = [](int n, long long s) { return n == 1 ? (cuuint64_t)16 : (cuuint64_t)s * 2; };
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)d->T, (cuuint64_t)d->B};
+    const cuuint64_t strides[3] = {bytes(heads, t.sh), bytes(d->T, t.st), bytes(d->B, t.sb)};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)kTc, 1}, step[4] = {1, 1, 1, 1};
+    return tc_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A launch of `count` cores from `first` on, all with the same head sizes.
+template <int KD, int VD, bool STATE_ONLY>
+static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int count, cudaStream_t st) {
+    TcLaunch L;
+    TcMaps maps;
+    L.a = p.a;
+    L.cores = count;
+    L.fine = 0;
+    for (int i = 0; i < count; ++i) {
+        const AttnCore& c = L.a.core[i] = p.a.core[first + i];
+        if (c.dots) L.fine |= 1 << i;
+        if (!(STATE_ONLY || attn_map(&maps.m[i][0], d, c.x, c.Kd)) || !attn_map(&maps.m[i][1], d, c.y, c.Kd) || !attn_map(&maps.m[i][2], d, c.z, c.Vd)) return M2D_ERR_LAUNCH;
+    }
+    const bool fine = !STATE_ONLY && L.fine;
+    L.slots = tc_slots(KD, VD, fine);
+    L.host_flag = wait_failure_flag();
+    const size_t smem = tc_smem(KD, VD, fine, L.slots);
+    auto kern = attn_tc_kernel<KD, VD, STATE_ONLY>;
+    if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
+    kern<<<(unsigned)(d->B * d->H * p.a.nseg * count), kTcThreads, smem, st>>>(maps, L);
+    return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+}
+template <bool STATE_ONLY>
+static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int count, cudaStream_t st) {
+    const bool k64 = p.a.core[first].Kd <= 64, v64 = p.a.core[first].Vd <= 64;
+    if (k64) return v64 ? launch_tc<64, 64, STATE_ONLY>(d, p, first, count, st) : launch_tc<64, 128, STATE_ONLY>(d, p, first, count, st);
+    return v64 ? launch_tc<128, 64, STATE_ONLY>(d, p, first, count, st) : launch_tc<128, 128, STATE_ONLY>(d, p, first, count, st);
+}
+
+static void launch_join(const AttnPlan& p, cudaStream_t st) {
+    const int n = p.a.core[0].Kd * p.a.core[0].Vd;
+    attn_join_kernel<<<dim3(p.a.B * p.a.H, (n + 255) / 256, p.cores), 256, 0, st>>>(p.a);
+}
 template <typename io_t, int VT>
-static int launch_core(const AttnPlan& p, cudaStream_t st) {
+static int launch_any(const AttnPlan& p, cudaStream_t st) {
     const dim3 grid((unsigned)(p.a.B * p.a.H * p.a.nseg), p.col_blocks, p.cores);
     auto full = attn_core_kernel<io_t, VT, false>;
     if (!allow_smem(reinterpret_cast<const void*>(full), p.smem)) return M2D_ERR_LAUNCH;
@@ -493,15 +556,29 @@ static int launch_core(const AttnPlan& p, cudaStream_t st) {
         auto part = attn_core_kernel<io_t, VT, true>;
         if (!allow_smem(reinterpret_cast<const void*>(part), p.smem)) return M2D_ERR_LAUNCH;
         part<<<grid, kAttnThreads, p.smem, st>>>(p.a);
-        const int n = p.a.core[0].Kd * p.a.core[0].Vd;
-        attn_join_kernel<<<dim3(p.a.B * p.a.H, (n + 255) / 256, p.cores), 256, 0, st>>>(p.a);
+        launch_join(p, st);
     }
     full<<<grid, kAttnThreads, p.smem, st>>>(p.a);
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
 }
 static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t st) {
-    if (d->dtype == M2D_F32) return p.VT == 64 ? launch_core<float, 64>(p, st) : launch_core<float, 32>(p, st);
-    return p.VT == 64 ? launch_core<__nv_bfloat16, 64>(p, st) : launch_core<__nv_bfloat16, 32>(p, st);
+    if (p.tc) {
+        // dq and dk have (V,K) states, dv a (K,V) one: one launch where the kernel is the same
+        const bool together = p.cores == 1 || (d->K <= 64) == (d->V <= 64);
+        const int counts[2] = {together ? p.cores : 2, together ? 0 : 1};
+        for (int pass = p.a.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
+            for (int i = 0; i < 2; ++i) {
+                if (!counts[i]) continue;
+                const int first = i ? counts[0] : 0;
+                const int rc = pass ? launch_tc<false>(d, p, first, counts[i], st) : launch_tc<true>(d, p, first, counts[i], st);
+                if (rc != M2D_OK) return rc;
+            }
+            if (!pass) launch_join(p, st);
+        }
+        return M2D_OK;
+    }
+    if (d->dtype == M2D_F32) return p.VT == 64 ? launch_any<float, 64>(p, st) : launch_any<float, 32>(p, st);
+    return p.VT == 64 ? launch_any<__nv_bfloat16, 64>(p, st) : launch_any<__nv_bfloat16, 32>(p, st);
 }
 
 static void fill_launch(const m2d_attn_desc* d, AttnPlan& p) {
@@ -519,19 +596,21 @@ static int check_workspace(const m2d_attn_desc* d, size_t bytes) {
     if (!bytes) return M2D_OK;
     return d->workspace && d->workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(d->workspace) & 255) == 0 ? M2D_OK : M2D_ERR_WORKSPACE;
 }
+// What either form may need: a query does not depend on the tensors' addresses.
+static size_t attn_workspace(const m2d_attn_desc* d, bool bwd) { return std::max(plan_attn(d, bwd, false).bytes, d->dtype == M2D_BF16 ? plan_attn(d, bwd, true).bytes : 0); }
 
 }  // namespace m2d
 
 using namespace m2d;
 
-extern "C" uint64_t m2d_attn_fwd_workspace(const m2d_attn_desc* d) { return check_attn(d, false) == M2D_OK ? plan_attn(d, false).bytes : 0; }
-extern "C" uint64_t m2d_attn_bwd_workspace(const m2d_attn_desc* d) { return check_attn(d, false) == M2D_OK ? plan_attn(d, true).bytes : 0; }
+extern "C" uint64_t m2d_attn_fwd_workspace(const m2d_attn_desc* d) { return check_attn(d, false) == M2D_OK ? attn_workspace(d, false) : 0; }
+extern "C" uint64_t m2d_attn_bwd_workspace(const m2d_attn_desc* d) { return check_attn(d, false) == M2D_OK ? attn_workspace(d, true) : 0; }
 
 extern "C" int m2d_attn_fwd(const m2d_attn_desc* d, void* stream) {
     int rc = check_attn(d, true);
     if (rc != M2D_OK) return rc;
     if (!d->o) return M2D_ERR_NULL;
-    AttnPlan p = plan_attn(d, false);
+    AttnPlan p = plan_attn(d, false, tc_applies(d, false));
     if ((rc = check_workspace(d, p.bytes)) != M2D_OK) return rc;
     fill_launch(d, p);
     AttnCore& c = p.a.core[0];
@@ -549,7 +628,7 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     int rc = check_attn(d, true);
     if (rc != M2D_OK) return rc;
     if (!d->d_o.data || !d->d_q || !d->d_k || !d->d_v) return M2D_ERR_NULL;
-    AttnPlan p = plan_attn(d, true);
+    AttnPlan p = plan_attn(d, true, tc_applies(d, true));
     if ((rc = check_workspace(d, p.bytes)) != M2D_OK) return rc;
     fill_launch(d, p);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -28,6 +28,8 @@ bool wants_grad(std::initializer_list<const Tensor*> inputs) {
         if (t->defined()) grad = grad || (at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
     return grad;
 }
+// A wait between warps of an earlier launch that gave up (its results are NaN) surfaces at the next call.
+void check_waits() { TORCH_CHECK(!m2d_take_wait_failure(), "linear attention: a wait inside an earlier launch timed out; the results of that launch are invalid"); }
 Tensor or_none(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 // neighbours along the last dimension
 Tensor rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
@@ -98,6 +100,7 @@ public:
         const at::NoGradGuard no_grad;
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[2].device());
+        check_waits();
         const bool have_state_grad = grads.size() > 1 && grads[1].defined();
         if (!grads[0].defined() && !have_state_grad) return variable_list(9);
         Attn a(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["flags"].toInt());
@@ -146,6 +149,7 @@ std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Ten
     check_attn(q, k, v, g, state, 2);
     check_devices(v, {&q, &k, &g, &state, &lengths});
     TORCH_CHECK(!lengths.defined() || lengths.scalar_type() == at::kInt, "linear attention: lengths are int32");
+    check_waits();
     if (wants_grad({&q, &k, &v, &g, &state})) {
         const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths_, scale, want_state, flags);
         return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
