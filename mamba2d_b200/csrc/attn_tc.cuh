@@ -3,24 +3,28 @@
 // A chunk is 128 tokens, the rows of one accumulator.  Per chunk, with the tiles of x, y, z in shared memory (TMA, 128-byte
 // swizzle, blocks of 128 rows x 64 columns) and St in bf16 next to them:
 //     (1)  pairs = x y^T            128 x 128    both operands as they arrived
-//     (2)  O2    = x St             128 x VD
-//     (3)  O1    = P z              128 x VD     P = s_intra D pairs, bf16 in tensor memory in the place of pairs
+//     (2)  O     = x St             128 x VD
+//     (3)  O    += P z              128 x VD     P, from pairs, as bf16 in tensor memory in the place of pairs
 //     (4)  delta = (u y)^T z        KD x VD      u y scaled in place, in two bf16 parts: St is carried in fp32 and a state
 //                                                is an output; one part would leave it at 2^-9
-//     out = O1 + s_inter w O2,  St <- exp(c_end) St + delta
+// A decay D_rc = exp(c_r - c_c) is a product of exp(c_r - m) and f_c = exp(m - c_c), m half of the chunk's decay: P is pairs times
+// f, the copy of St is scaled by exp(m), and out = exp(c_r - m) O; all factors lie within 2^+-80 or the chunk is not `mild`
+// (m would have to lie further from its ends than that: decays of more than 0.87 a token on average, a sequence that starts
+// anew inside).  P of such a chunk takes its D from differences of c, and O of (2) is scaled by its rows where it lies
+// before (3) adds.  c is summed in 64 bits.
 // The work is dealt to warps that wait on one another through mbarriers only:
-//     warps 0 - 3   a token row a thread: pairs -> P, O1 and O2 -> out
-//     warps 4 - 7   a token row a thread: y -> u y; a row of St a thread: St in registers, its bf16 copy in shared memory
-//     warp 8        TMA loads into a ring of tiles        warp 9   issues the products       warp 10   the decays' tables
-// Decays: c is summed in 64 bits; D_rc of one 32 x 32 block on the diagonal is exp of a difference that the table holds in
-// two floats, and factors into exp(c_r - b) exp(b - c_c) elsewhere, b the sum up to the row block: both at most one, and
-// 32 exponentials a row instead of 128.
+//     warps 0 - 7    a token row and half of the columns a thread: pairs -> P, O -> out
+//     warps 8 - 15   half of a token row a thread: y -> u y; half of a row of St a thread: St in registers, its bf16 copy
+//     warp 16  TMA loads    warps 17, 18  issue (1), (4) and (2), (3)     warp 19  the decays' tables
+// pairs has two places, so that (1) of the next chunk runs beside (3) of this one.  The copy of St is written while (4) runs, after
+// u y: what bounds a chunk is the chain u y -> (4) -> St.  out goes through the tile of x (or z, where that is the larger
+// one), which nothing reads any more, and by TMA: rows stored from registers took 2000 cycles of a chunk, 32 lines a request.
 //
 // `fine` (wanted where the decay's gradient is): P and St also in two parts each, so that the dots that out is summed
 // into are exact to 2^-17 like the states that they meet.
 //
-// Every wait is bounded: one that gives up makes all of the CTA's roles leave, rows not written yet become NaN, and a word in
-// host memory says so.
+// Every wait is bounded: one that gives up makes all of the CTA's roles leave, its rows become NaN, and a word in host memory
+// says so.
 #pragma once
 
 #include "attn_core.cuh"
@@ -29,14 +33,17 @@
 namespace m2d {
 
 constexpr int kTc = 128;                      // tokens of a chunk
-constexpr int kTcThreads = 352;
+constexpr int kTcThreads = 640;
 constexpr int kTcBlock = kTc * 128;           // 128 rows x 64 columns of bf16
-constexpr int kTcMaxSlots = 12;
+constexpr int kTcTiles = 3;                   // tiles of x, y, z each in flight, at most
+constexpr float kTcMild = 80.f;
 
-struct TcMaps { CUtensorMap m[3][3]; };       // [core][x, y, z]
+struct TcMaps { CUtensorMap m[3][4]; };       // [core][x, y, z, out]
 struct TcLaunch {
     AttnLaunch a;
-    int cores, slots;
+    int cores;
+    int n[3];                                 // tiles of x, y, z
+    uint32_t small;                           // where TcSmall lies in shared memory
     int fine;                                 // bit per core
     int* host_flag;
 };
@@ -46,17 +53,51 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The issuing warps run as a whole and one lane's predicate is on: operands then stay in uniform registers, where the
+// instruction wants them.  (One lane alone in a branch moved them there for every product, 160 cycles a product instead of its 64.)
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+    return on;
+}
+__device__ __forceinline__ void umma_ss(uint32_t on, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t on, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t on, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(on) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
                  ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
                    "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr) : "memory");
+}
+// 16 columns of this thread's row
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -70,145 +111,170 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool a_mn, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// Decay tables of a chunk, in log2 where they are not exponentials yet.
+// Decay tables of a chunk.
 struct alignas(16) TcTable {
-    float2 l[kTc];          // c within the 32-token block, in two floats
+    float f[kTc];           // mild: exp(m - c), times s_intra / s_inter; else c in log2
+    float e[kTc];           // mild: exp(c - m), times s_inter; else what c lost to its rounding
     float u[kTc];           // update weight times s_update
-    float f[192];           // exp(b - c_c): columns of the blocks before (rev: behind) row block 1, 2, 3 (0, 1, 2)
-    float2 base[4];         // forwards the sum before the block, backwards from its start to the end
-    float2 total[4];        // of the block
-    float whole;            // exp(c_end)
+    float2 end;             // c_end in log2, in two floats
+    float whole, copy;      // exp(c_end); mild: exp(m), else one
+    int mild;
 };
-__device__ __forceinline__ int tc_f(int rev, int i) { return rev ? (i == 0 ? 0 : i == 1 ? 96 : 160) : (i <= 1 ? 0 : i == 2 ? 32 : 96); }
+struct alignas(16) TcSmall {
+    TcTable tab;
+    uint64_t bars[40];
+    uint32_t tmem;
+    int abort;
+};
 
-// (KD = 64: a block behind the ring, since (4) computes 128 rows: the upper 64, of whatever lies behind y, are not used)
-inline size_t tc_fixed_smem(int KD, int VD, bool fine) { return (size_t)KD * VD * 2 * (fine ? 2 : 1) + (size_t)kTc * KD * 2 + 1024 + (KD == 64 ? kTcBlock : 0); }
-inline int tc_slots(int KD, int VD, bool fine) {
-    const size_t tile = (size_t)kTc * 2 * (KD > VD ? KD : VD);
-    const int n = (int)((kMaxSmem - 2944 - tc_fixed_smem(KD, VD, fine)) / tile);
-    return n < kTcMaxSlots ? n : kTcMaxSlots;
+// Shared memory: St in bf16 (one or two parts), the second part of u y, tiles.  (KD = 64: (4) computes 128 rows; the upper 64, of
+// whatever lies behind y, are not used, and a tile lies there.)
+inline size_t tc_fixed_smem(int KD, int VD, bool fine, bool state_only) { return (state_only ? 0 : (size_t)KD * VD * 2 * (fine ? 2 : 1)) + (size_t)kTc * KD * 2; }
+// Tiles of x, y, z: x first, whose tile is held longest, z last, which is needed last.
+inline size_t tc_plan_tiles(int KD, int VD, bool fine, bool state_only, int (&n)[3]) {
+    const size_t tile[3] = {(size_t)kTc * KD * 2, (size_t)kTc * KD * 2, (size_t)kTc * VD * 2};
+    n[0] = state_only ? 0 : 1; n[1] = n[2] = 1;
+    size_t bytes = tc_fixed_smem(KD, VD, fine, state_only) + n[0] * tile[0] + tile[1] + tile[2];
+    for (int round = 1; round < kTcTiles; ++round)
+        for (int i = state_only ? 1 : 0; i < 3; ++i)
+            if (n[i] == round && bytes + tile[i] + sizeof(TcSmall) <= kMaxSmem) {
+                ++n[i];
+                bytes += tile[i];
+            }
+    return bytes;
 }
-inline size_t tc_smem(int KD, int VD, bool fine, int slots) { return tc_fixed_smem(KD, VD, fine) + (size_t)slots * kTc * 2 * (KD > VD ? KD : VD); }
 
 template <int KD, int VD, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcLaunch L) {
-    extern __shared__ uint8_t tc_smem_raw[];
-    __shared__ TcTable tab;
-    enum { kSc, kP, kY, kO, kOFree, kDelta, kS, kMma2, kTabFull, kTabFree, kBars };
-    __shared__ uint64_t bars[kBars + 2 * kTcMaxSlots];
-    __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
-    constexpr int KB = KD / 64, VB = VD / 64;                     // 64-column blocks
-    constexpr uint32_t kTile = kTc * 2 * (KD > VD ? KD : VD);
-    constexpr uint32_t kSc0 = 0, kO1 = 128, kO2 = 128 + VD, kDl = 128 + 2 * VD;      // columns of tensor memory
+    extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
+    // (kSc, kY, kO, kDelta: one for even chunks, one for odd, where a barrier may complete again before all have seen it)
+    enum { kSc, kP = kSc + 2, kY, kO = kY + 2, kOFree = kO + 2, kDelta, kS = kDelta + 2, kMma2, kTabFull, kTabFree, kFull, kEmpty = kFull + 3 * kTcTiles, kBars = kEmpty + 3 * kTcTiles };
+    static_assert(kBars <= 40, "room for the barriers");
+    constexpr bool kStageX = VD <= KD;                            // out goes through x's tile, else z's
+    constexpr int kHalf = VD / 2;                                 // columns of a thread
+    constexpr uint32_t kTileX = kTc * KD * 2, kTileZ = kTc * VD * 2;
+    constexpr uint32_t kO0 = 256;                                 // columns of tensor memory: pairs (2 x 128), O, delta
     constexpr uint32_t kCols = STATE_ONLY ? (VD <= 64 ? 64 : 128) : 512;
-    constexpr uint32_t kDelta0 = STATE_ONLY ? 0 : kDl;
+    constexpr uint32_t kDelta0 = STATE_ONLY ? 0 : kO0 + VD;
 
     const AttnLaunch& a = L.a;
     const int ci = blockIdx.x % L.cores, unit = blockIdx.x / L.cores;
     const AttnCore& k = a.core[ci];
     const bool fine = !STATE_ONLY && (L.fine >> ci & 1);
     const int seg = unit % a.nseg, bh = unit / a.nseg, h = bh % a.H, b = bh / a.H;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rev = k.rev;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rev = k.rev;
     const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
     const int active = max(0, min(len, t_hi) - t_lo), chunks = (active + kTc - 1) / kTc;         // the others hold nothing
 
-    const uint32_t smem0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u;
-    const uint32_t s_hi = smem0, s_lo = s_hi + KD * VD * 2, y_lo = s_hi + KD * VD * 2 * (fine ? 2 : 1), ring = y_lo + kTc * KD * 2;
-    const uint32_t bar0 = smem_u32(bars);
+    TcSmall& small = *reinterpret_cast<TcSmall*>(tc_smem_raw + L.small);
+    TcTable& tab = small.tab;
+    // (the launch's second parts take room whether this core has them or not)
+    const uint32_t s_hi = smem_u32(tc_smem_raw), s_lo = s_hi + KD * VD * 2, y_lo = STATE_ONLY ? s_hi : s_hi + KD * VD * 2 * (L.fine ? 2 : 1);
+    const uint32_t ring_x = y_lo + kTileX, ring_y = ring_x + L.n[0] * kTileX, ring_z = ring_y + L.n[1] * kTileX;
+    const uint32_t bar0 = smem_u32(small.bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
-    auto full = [&](int s) { return bar0 + 8u * (kBars + s); };
-    auto empty = [&](int s) { return bar0 + 8u * (kBars + kTcMaxSlots + s); };
-    volatile int* const abort = &abort_flag;
-    constexpr int kTiles = STATE_ONLY ? 2 : 3;                    // a chunk's tiles in the ring: y, x, z
-    constexpr int kTileX = 1, kTileZ = kTiles - 1;
-    auto slot_of = [&](int it, int tile) { return (it * kTiles + tile) % L.slots; };
-    auto phase_of = [&](int it, int tile) { return (uint32_t)((it * kTiles + tile) / L.slots) & 1u; };
-    auto tile_at = [&](int it, int tile) { return ring + (uint32_t)slot_of(it, tile) * kTile; };
+    enum { X, Y, Z };
+    auto tile_at = [&](int which, int it) { return which == X ? ring_x + (uint32_t)(it % L.n[X]) * kTileX : which == Y ? ring_y + (uint32_t)(it % L.n[Y]) * kTileX : ring_z + (uint32_t)(it % L.n[Z]) * kTileZ; };
+    auto full = [&](int which, int it) { return bar(kFull + which * kTcTiles + it % L.n[which]); };
+    auto empty = [&](int which, int it) { return bar(kEmpty + which * kTcTiles + it % L.n[which]); };
+    auto turn = [&](int which, int it) { return (uint32_t)(it / L.n[which]) & 1u; };
     auto chunk_at = [&](int it) { return t_lo + (rev ? chunks - 1 - it : it) * kTc; };
+    volatile int* const abort = &small.abort;
     auto wait = [&](uint32_t bar_, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar_, parity, abort)) != 0; };      // whole warps
+    auto wait2 = [&](int bar_, int it) { return wait(bar(bar_ + (it & 1)), it >> 1 & 1); };                                          // of a pair
+    auto loaded = [&](int which, int it) { return mbar_wait(full(which, it), turn(which, it), abort); };
 
     if (tid == 0) {
-        for (int i = 0; i < kBars; ++i) {
-            const int n = i == kP || i == kY || i == kOFree || i == kS ? 4 : i == kTabFree ? (STATE_ONLY ? 4 : 8) : 1;
-            mbar_init(bar(i), n);
-        }
-        for (int s = 0; s < L.slots; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
-        }
-        abort_flag = 0;
+        for (int i = 0; i < kFull; ++i) mbar_init(bar(i), i == kP || i == kY || i == kY + 1 || i == kOFree || i == kS ? 8 : i == kTabFree ? (STATE_ONLY ? 8 : 16) : 1);
+        for (int i = kFull; i < kEmpty; ++i) mbar_init(bar(i), 1);
+        // who gives a tile back: y after (4); the one that out goes through after that; another after its two products
+        for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || i / kTcTiles == (kStageX ? X : Z) ? 1 : 2);
+        small.abort = (smem_u32(tc_smem_raw) & 1023u) != 0;      // (swizzled tiles have to be aligned; nothing runs if they are not)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc(smem_u32(&tmem_slot), kCols);
+    if (warp == 16) tmem_alloc(smem_u32(&small.tmem), kCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = small.tmem;
 
-    if (warp < 4) {
+    // 16-byte piece c of a tile's row (64-column blocks of `rows` rows, swizzled)
+    auto piece = [&](uint32_t base, int rows, int r, int c) { return base + (uint32_t)(c / 8) * rows * 128 + (uint32_t)r * 128 + (uint32_t)(((c ^ r) & 7) << 4); };
+    auto sts = [&](uint32_t addr, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory"); };
+
+    if (warp < 8) {
         // ---- token rows ----
         if constexpr (!STATE_ONLY) {
-            const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+            const int q = warp & 3, half = warp >> 2, r = tid & 127;
+            const uint32_t mine = tmem + ((uint32_t)(q * 32) << 16), oc = mine + kO0 + half * kHalf;
             for (int it = 0; it < chunks; ++it) {
-                const int t0 = chunk_at(it), valid = min(kTc, len - t0), r = tid;
-                const uint32_t ph = it & 1;
-                if (!wait(bar(kTabFull), ph)) break;
-                const float2 lr = tab.l[r], base = tab.base[warp], total = tab.total[warp];
-                const float w = k.s_inter * (rev ? ex2((base.x - lr.x) + (base.y - lr.y)) : ex2((base.x + lr.x) + (base.y + lr.y)));
-                const float e = k.s_intra * (rev ? ex2((total.x - lr.x) + (total.y - lr.y)) : ex2(lr.x + lr.y));
-                if (!wait(bar(kSc), ph)) break;
+                // pairs -> P
+                const int t0 = chunk_at(it), valid = min(kTc, len - t0);
+                const uint32_t pairs = mine + 128 * (it & 1);
+                if (!wait(bar(kTabFull), it & 1)) break;
+                const bool mild = tab.mild;
+                float e = tab.e[r];
+                if (!wait2(kSc, it)) break;
                 tc_fence_after();
-                uint32_t lo[2][16];                               // second parts that wait for their columns to be read
+                // blocks of 32 columns: 0 and 3, or 1 and 2, so that no warp has more than two that are not masked
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i) {
+                    const int j = half ? 1 + i : 3 * i;
+                    const uint32_t at = pairs + 32 * j;
+                    uint32_t p[16];
+                    if (rev ? j < q : j > q) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                        for (int c = 0; c < 16; ++c) p[c] = 0;
+                        tmem_st16(at, p);
+                        if (fine) tmem_st16(at + 16, p);
+                        continue;
+                    }
                     float v[32];
-                    uint32_t hi[16], low[16];
-                    const bool on = rev ? j >= warp : j <= warp;
-                    tmem_ld32(mine + kSc0 + 32 * j, v);
-                    if (on && j == warp) {
-                        const float4* const lp = reinterpret_cast<const float4*>(tab.l + 32 * j);
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            const float4 lc = lp[c / 2];
-                            float d0 = (lr.x - lc.x) + (lr.y - lc.y), d1 = (lr.x - lc.z) + (lr.y - lc.w);
-                            if (rev) { d0 = -d0; d1 = -d1; }
-                            v[c] = (rev ? c >= lane : c <= lane) ? v[c] * (k.s_intra * ex2(d0)) : 0.f;
-                            v[c + 1] = (rev ? c + 1 >= lane : c + 1 <= lane) ? v[c + 1] * (k.s_intra * ex2(d1)) : 0.f;
-                        }
-                    } else if (on) {
-                        const float4* const f = reinterpret_cast<const float4*>(tab.f + tc_f(rev, warp) + (rev ? 32 * (j - warp - 1) : 32 * j));
+                    tmem_ld32(at, v);
+                    const float4* const f = reinterpret_cast<const float4*>(tab.f + 32 * j);
+                    if (mild) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4) {
-                            const float4 q = f[c / 4];
-                            v[c] *= e * q.x; v[c + 1] *= e * q.y; v[c + 2] *= e * q.z; v[c + 3] *= e * q.w;
+                            const float4 g = f[c / 4];
+                            const float2 v0 = __fmul2_rn(make_float2(v[c], v[c + 1]), make_float2(g.x, g.y)), v1 = __fmul2_rn(make_float2(v[c + 2], v[c + 3]), make_float2(g.z, g.w));
+                            v[c] = v0.x; v[c + 1] = v0.y; v[c + 2] = v1.x; v[c + 3] = v1.y;
                         }
                     } else {
+                        const float cr = tab.f[r], ratio = rev ? k.s_intra : 1.f, sign = rev ? -1.f : 1.f;
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) v[c] = 0.f;
+                        for (int c = 0; c < 32; ++c) v[c] *= ratio * ex2(sign * ((cr - tab.f[32 * j + c]) + (e - tab.e[32 * j + c])));
+                    }
+                    if (j == q) {
+                        const unsigned on = rev ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) v[c] = on >> c & 1 ? v[c] : 0.f;
                     }
                     if (valid < kTc) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) v[c] = 32 * j + c < valid ? v[c] : 0.f;
                     }
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) hi[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
-                    tmem_st16(mine + kSc0 + 16 * j, hi);
+                    for (int c = 0; c < 16; ++c) p[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
+                    tmem_st16(at, p);
                     if (fine) {
 #pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            low[c] = pack_bf16x2(v[2 * c] - __uint_as_float(hi[c] << 16), v[2 * c + 1] - __uint_as_float(hi[c] & 0xffff0000u));
-                        if (j == 2) {
-                            tmem_st16(mine + kSc0 + 64, lo[0]);
-                            tmem_st16(mine + kSc0 + 80, lo[1]);
-                        }
-                        if (j == 3) {
-                            tmem_st16(mine + kSc0 + 96, lo[0]);
-                            tmem_st16(mine + kSc0 + 112, low);
-                        } else {
+                        for (int c = 0; c < 16; ++c) p[c] = pack_bf16x2(v[2 * c] - __uint_as_float(p[c] << 16), v[2 * c + 1] - __uint_as_float(p[c] & 0xffff0000u));
+                        tmem_st16(at + 16, p);
+                    }
+                }
+                if (!mild) {                                      // O2 -> w O2
+                    const float c = tab.f[r], w = rev ? ex2((tab.end.x - c) + (tab.end.y - e)) : ex2(c + e);
+                    e = k.s_inter;
+                    if (!wait(bar(kMma2), it & 1)) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < kHalf; c0 += 16) {
+                        float v[16];
+                        uint32_t p[16];
+                        tmem_ld16(oc + c0, v);
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) lo[j & 1][c] = low[c];
-                        }
+                        for (int c = 0; c < 16; ++c) p[c] = __float_as_uint(w * v[c]);
+                        tmem_st16(oc + c0, p);
                     }
                 }
                 tmem_st_wait();
@@ -218,54 +284,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     mbar_arrive(bar(kP));
                     mbar_arrive(bar(kTabFree));
                 }
-                if (!wait(bar(kO), ph)) break;
-                tc_fence_after();
+                // O -> out
                 const bool row = t0 + r < t_hi, live = r < valid;
-                const long long at = b * k.ob + (long long)(t0 + r) * k.ot + h * k.oh;
-                const __nv_bfloat16* const er = k.dots ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st : nullptr;
+                const __nv_bfloat16* const er = k.dots && live ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st + half * kHalf : nullptr;
+                const uint32_t stage = tile_at(kStageX ? X : Z, it);
                 float sum = 0.f;
+                if (!wait2(kO, it)) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = 0; c0 < kHalf; c0 += 32) {
+                    float o[32];
+                    const int col = half * kHalf + c0;
+                    tmem_ld32(oc + c0, o);
 #pragma unroll
-                for (int j = 0; j < VD / 32; ++j) {
-                    float o[32], o2[32];
-                    tmem_ld32(mine + kO1 + 32 * j, o);
-                    tmem_ld32(mine + kO2 + 32 * j, o2);
+                    for (int c = 0; c < 32; ++c) o[c] *= e;
+                    if (valid < kTc) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) o[c] = live ? fmaf(w, o2[c], o[c]) : 0.f;
-                    if (row) {
+                        for (int c = 0; c < 32; ++c) o[c] = live ? o[c] : 0.f;
+                    }
+                    if (!k.out_f32) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 8) {
-                            if (32 * j + c >= k.Vd) continue;
-                            if (k.out_f32) {
-                                float4* p = reinterpret_cast<float4*>(static_cast<float*>(k.out) + at + 32 * j + c);
-                                p[0] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-                                p[1] = make_float4(o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
-                            } else {
-                                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(k.out) + at + 32 * j + c) =
-                                    make_uint4(pack_bf16x2(o[c], o[c + 1]), pack_bf16x2(o[c + 2], o[c + 3]), pack_bf16x2(o[c + 4], o[c + 5]), pack_bf16x2(o[c + 6], o[c + 7]));
+                        for (int c = 0; c < 32; c += 8)
+                            sts(piece(stage, kTc, r, (col + c) / 8), pack_bf16x2(o[c], o[c + 1]), pack_bf16x2(o[c + 2], o[c + 3]), pack_bf16x2(o[c + 4], o[c + 5]), pack_bf16x2(o[c + 6], o[c + 7]));
+                    } else if (row) {
+                        float4* const p = reinterpret_cast<float4*>(static_cast<float*>(k.out) + b * k.ob + (long long)(t0 + r) * k.ot + h * k.oh + col);
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8)
+                            if (col + c < k.Vd) {
+                                p[c / 4] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                                p[c / 4 + 1] = make_float4(o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
                             }
-                            if (er && live) {
-                                const uint4 q = __ldg(reinterpret_cast<const uint4*>(er + 32 * j + c));
-                                const uint32_t qq[4] = {q.x, q.y, q.z, q.w};
+                    }
+                    if (er) {
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) sum = fmaf(o[c + 2 * i], __uint_as_float(qq[i] << 16), fmaf(o[c + 2 * i + 1], __uint_as_float(qq[i] & 0xffff0000u), sum));
+                        for (int c = 0; c < 32; c += 8)
+                            if (col + c < k.Vd) {
+                                const uint4 g = __ldg(reinterpret_cast<const uint4*>(er + c0 + c));
+                                const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) sum = fmaf(o[c + 2 * i], __uint_as_float(gg[i] << 16), fmaf(o[c + 2 * i + 1], __uint_as_float(gg[i] & 0xffff0000u), sum));
                             }
-                        }
                     }
                 }
                 tc_fence_before();
+                async_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(kOFree));
-                if (k.dots && row) k.dots[((size_t)b * a.T + t0 + r) * a.H + h] = sum;
+                if (k.dots && row) k.dots[(((size_t)half * a.B + b) * a.T + t0 + r) * a.H + h] = sum;
             }
         }
-    } else if (warp < 8) {
+    } else if (warp < 16) {
         // ---- y and the state ----
-        const int r = tid - 128, sw = warp - 4;
-        const uint32_t mine = tmem + ((uint32_t)(sw * 32) << 16) + kDelta0;
-        float S[VD];
+        const int r = tid & 127, half = (warp >> 2) & 1, v0 = half * kHalf;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kDelta0 + v0;
+        float S[kHalf];
         const bool have_row = r < k.Kd;
 #pragma unroll
-        for (int c = 0; c < VD; ++c) S[c] = 0.f;
+        for (int c = 0; c < kHalf; ++c) S[c] = 0.f;
         if (!STATE_ONLY && have_row) {
             const float* init = nullptr;
             long long sr = k.init.sr, sc = k.init.sc;
@@ -275,249 +350,270 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             } else if (k.init.p) {
                 init = k.init.p + b * k.init.sb + h * k.init.sh;
             }
-            if (init && sc == 1 && (reinterpret_cast<uintptr_t>(init) & 15) == 0) {
+            if (init) {
+                init += r * sr + v0 * sc;
 #pragma unroll
-                for (int c = 0; c < VD; c += 4)
-                    if (c < k.Vd) {
-                        const float4 v = *reinterpret_cast<const float4*>(init + r * sr + c);
-                        S[c] = v.x; S[c + 1] = v.y; S[c + 2] = v.z; S[c + 3] = v.w;
-                    }
-            } else if (init) {
-#pragma unroll
-                for (int c = 0; c < VD; ++c)
-                    if (c < k.Vd) S[c] = init[r * sr + c * sc];
+                for (int c = 0; c < kHalf; ++c)
+                    if (v0 + c < k.Vd) S[c] = init[c * sc];
             }
         }
         auto put = [&](float* to, long long sr, long long sc) {
+            to += r * sr + v0 * sc;
             if (have_row && sc == 1 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
 #pragma unroll
-                for (int c = 0; c < VD; c += 4)
-                    if (c < k.Vd) *reinterpret_cast<float4*>(to + r * sr + c) = make_float4(S[c], S[c + 1], S[c + 2], S[c + 3]);
+                for (int c = 0; c < kHalf; c += 4)
+                    if (v0 + c < k.Vd) *reinterpret_cast<float4*>(to + c) = make_float4(S[c], S[c + 1], S[c + 2], S[c + 3]);
             } else if (have_row) {
 #pragma unroll
-                for (int c = 0; c < VD; ++c)
-                    if (c < k.Vd) to[r * sr + c * sc] = S[c];
+                for (int c = 0; c < kHalf; ++c)
+                    if (v0 + c < k.Vd) to[c * sc] = S[c];
             }
         };
-        auto keep = [&](int t0) {                                 // if the chunk at t0 ends a run
-            if (k.anchors && ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T)) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, k.Vd, 1);
+        // St before (rev) or after the chunk at t0, if that ends a run; also of the chunks that hold nothing
+        auto keep = [&](int from, int to) {
+            if (!k.anchors) return;
+            for (int t0 = from; t0 < to; t0 += kTc)
+                if ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, k.Vd, 1);
         };
-        // 16-byte piece c of 64-column block j of this thread's row
-        auto piece = [&](uint32_t base, int rows, int j, int c) { return base + (uint32_t)j * rows * 128 + (uint32_t)r * 128 + (uint32_t)((c ^ (r & 7)) << 4); };
-        auto sts = [&](uint32_t addr, uint4 v) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); };
-        auto publish = [&] {                                      // the state's bf16 copy
-            if (r < KD) {
-#pragma unroll
-                for (int c = 0; c < VD / 8; ++c) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float v0 = S[8 * c + 2 * i], v1 = S[8 * c + 2 * i + 1];
-                        hi[i] = pack_bf16x2(v0, v1);
-                        lo[i] = pack_bf16x2(v0 - __uint_as_float(hi[i] << 16), v1 - __uint_as_float(hi[i] & 0xffff0000u));
-                    }
-                    sts(piece(s_hi, KD, c / 8, c % 8), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                    if (fine) sts(piece(s_lo, KD, c / 8, c % 8), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                }
-            }
-            async_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kS));
-        };
-        if constexpr (!STATE_ONLY) {
-            if (rev)
-                for (int t0 = t_lo + chunks * kTc; t0 < t_hi; t0 += kTc) keep(t0);
-            if (chunks) publish();
-        }
+        const int behind = t_lo + chunks * kTc;
         for (int it = 0; it < chunks; ++it) {
             const int t0 = chunk_at(it), valid = min(kTc, len - t0);
-            const uint32_t ph = it & 1;
-            if (!STATE_ONLY && rev) keep(t0);
-            if (!wait(bar(kTabFull), ph)) break;
-            const float u = r < valid ? tab.u[r] : 0.f, whole = tab.whole;
-            const uint32_t y = tile_at(it, 0);
+            if (!STATE_ONLY && rev) keep(t0, it ? t0 + kTc : t_hi);
+            if (!wait(bar(kTabFull), it & 1)) break;
+            const float u = r < valid ? tab.u[r] : 0.f, whole = tab.whole, copy = tab.copy;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kTabFree));
+            const uint32_t y = tile_at(Y, it);
             // y is free to change once (1) has read it
-            if (!wait(full(slot_of(it, 0)), phase_of(it, 0)) || (!STATE_ONLY && !wait(bar(kSc), ph))) break;
-#pragma unroll 4
-            for (int c = 0; c < KD / 8; ++c) {
-                const uint32_t at = piece(y, kTc, c / 8, c % 8);
-                uint32_t q[4], hi[4], lo[4];
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(at) : "memory");
+            if (!__all_sync(0xffffffffu, loaded(Y, it)) || (!STATE_ONLY && !wait2(kSc, it))) break;
+#pragma unroll 2
+            for (int i = 0; i < KD / 16; ++i) {
+                const int c = half * (KD / 16) + i;
+                const uint32_t at = piece(y, kTc, r, c);
+                uint32_t g[4], hi[4], lo[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(at) : "memory");
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     // (a row behind the last token may hold anything: it becomes zero, not a product with zero)
-                    const float v0 = r < valid ? u * __uint_as_float(q[i] << 16) : 0.f, v1 = r < valid ? u * __uint_as_float(q[i] & 0xffff0000u) : 0.f;
-                    hi[i] = pack_bf16x2(v0, v1);
-                    lo[i] = pack_bf16x2(v0 - __uint_as_float(hi[i] << 16), v1 - __uint_as_float(hi[i] & 0xffff0000u));
+                    if (r >= valid) g[i] = 0;
+                    const float2 y2 = make_float2(__uint_as_float(g[i] << 16), __uint_as_float(g[i] & 0xffff0000u)), u2 = make_float2(u, u);
+                    const float2 h2 = __fmul2_rn(y2, u2);
+                    hi[i] = pack_bf16x2(h2.x, h2.y);
+                    const float2 l2 = __ffma2_rn(y2, u2, make_float2(__uint_as_float((hi[i] << 16) ^ 0x80000000u), __uint_as_float((hi[i] & 0xffff0000u) ^ 0x80000000u)));
+                    lo[i] = pack_bf16x2(l2.x, l2.y);
                 }
-                sts(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                sts(piece(y_lo, kTc, c / 8, c % 8), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                sts(at, hi[0], hi[1], hi[2], hi[3]);
+                sts(piece(y_lo, kTc, r, c), lo[0], lo[1], lo[2], lo[3]);
             }
             if (valid < kTc) {                                    // z's rows there meet zeros in P and in u y
-                if (!wait(full(slot_of(it, kTileZ)), phase_of(it, kTileZ))) break;
+                if (!__all_sync(0xffffffffu, loaded(Z, it))) break;
                 if (r >= valid) {
-                    const uint32_t z = tile_at(it, kTileZ);
-#pragma unroll
-                    for (int c = 0; c < VD / 8; ++c) sts(piece(z, kTc, c / 8, c % 8), make_uint4(0, 0, 0, 0));
+#pragma unroll 1
+                    for (int c = 0; c < VD / 16; ++c) sts(piece(tile_at(Z, it), kTc, r, half * (VD / 16) + c), 0, 0, 0, 0);
                 }
             }
             async_fence();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(bar(kY));
-                mbar_arrive(bar(kTabFree));
+            if (lane == 0) mbar_arrive(bar(kY + (it & 1)));
+            if constexpr (!STATE_ONLY) {                          // the state's copy for (2)
+                if (it > 0 && !wait(bar(kMma2), (it & 1) ^ 1)) break;
+                if (r < KD) {
+#pragma unroll
+                    for (int c = 0; c < kHalf / 8; ++c) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float s0 = copy * S[8 * c + 2 * i], s1 = copy * S[8 * c + 2 * i + 1];
+                            hi[i] = pack_bf16x2(s0, s1);
+                            if (fine) lo[i] = pack_bf16x2(s0 - __uint_as_float(hi[i] << 16), s1 - __uint_as_float(hi[i] & 0xffff0000u));
+                        }
+                        sts(piece(s_hi, KD, r, v0 / 8 + c), hi[0], hi[1], hi[2], hi[3]);
+                        if (fine) sts(piece(s_lo, KD, r, v0 / 8 + c), lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(kS));
             }
-            if (!wait(bar(kDelta), ph)) break;
+            if (!wait2(kDelta, it)) break;
             tc_fence_after();
 #pragma unroll
-            for (int j = 0; j < VD / 32; ++j) {
-                float d[32];
-                tmem_ld32(mine + 32 * j, d);
+            for (int c0 = 0; c0 < kHalf; c0 += 16) {
+                float d[16];
+                tmem_ld16(mine + c0, d);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) S[32 * j + c] = fmaf(S[32 * j + c], whole, d[c]);
+                for (int c = 0; c < 16; ++c) S[c0 + c] = fmaf(S[c0 + c], whole, d[c]);
             }
             tc_fence_before();
-            if (!STATE_ONLY) {
-                if (it + 1 < chunks) {
-                    if (!wait(bar(kMma2), ph)) break;             // (2) has read the copy
-                    publish();
-                }
-                if (!rev) keep(t0);
-            }
+            if (!STATE_ONLY && !rev) keep(t0, it == chunks - 1 ? t_hi : t0 + kTc);
         }
         if constexpr (STATE_ONLY) {
             put(k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd, k.Vd, 1);
         } else {
-            if (!rev)
-                for (int t0 = t_lo + chunks * kTc; t0 < t_hi; t0 += kTc) keep(t0);
+            if (!chunks) keep(behind, t_hi);
             if (k.fin.p && seg == (rev ? 0 : a.nseg - 1)) {
                 if (*abort) {
 #pragma unroll
-                    for (int c = 0; c < VD; ++c) S[c] = __int_as_float(0x7fc00000);
+                    for (int c = 0; c < kHalf; ++c) S[c] = __int_as_float(0x7fc00000);
                 }
                 put(k.fin.p + b * k.fin.sb + h * k.fin.sh, k.fin.sr, k.fin.sc);
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         // ---- loads ----
         if (lane == 0) {
-            const CUtensorMap* const m = maps.m[ci];
-            int armed = 0;
-            for (int i = 0; i < chunks * kTiles; ++i) {
-                const int it = i / kTiles, tile = i % kTiles, s = i % L.slots;
-                if (!mbar_wait(empty(s), ((uint32_t)(i / L.slots) & 1u) ^ 1u, abort)) break;
+            int armed[3] = {0, 0, 0};
+            for (int it = 0; it < chunks && !*abort; ++it) {
                 const int t0 = chunk_at(it);
-                const int which = tile == 0 ? 1 : tile == kTileZ ? 2 : 0;
-                const int blocks = which == 2 ? VB : KB, head = h / (which == 0 ? k.x.per : which == 1 ? k.y.per : k.z.per);
-                mbar_expect_tx(full(s), (uint32_t)blocks * kTcBlock);
-                for (int j = 0; j < blocks; ++j) tma_load_4d(ring + (uint32_t)s * kTile + j * kTcBlock, m + which, 64 * j, head, t0, b, full(s));
-                armed = i + 1;
+                for (int i = STATE_ONLY ? 1 : 0; i < 3; ++i) {
+                    const int which = STATE_ONLY ? i : i == 0 ? Y : i == 1 ? X : Z;      // y's tile comes free first
+                    if (!mbar_wait(empty(which, it), turn(which, it) ^ 1u, abort)) break;
+                    const int blocks = (which == Z ? VD : KD) / 64, head = h / (which == X ? k.x.per : which == Y ? k.y.per : k.z.per);
+                    mbar_expect_tx(full(which, it), (uint32_t)blocks * kTcBlock);
+                    for (int j = 0; j < blocks; ++j) tma_load_4d(tile_at(which, it) + j * kTcBlock, &maps.m[ci][which], 64 * j, head, t0, b, full(which, it));
+                    armed[which] = it + 1;
+                }
             }
-            if (*abort)
-                for (int i = max(0, armed - L.slots); i < armed; ++i)
-                    for (int n = 0; n < kTcWaitLimit && !mbar_try_wait(full(i % L.slots), (uint32_t)(i / L.slots) & 1u); ++n) {}
+            if (*abort)                                           // let the copies land (bounded)
+                for (int which = STATE_ONLY ? Y : X; which <= Z; ++which)
+                    for (int it = max(0, armed[which] - L.n[which]); it < armed[which]; ++it)
+                        for (int n = 0; n < kTcWaitLimit && !mbar_try_wait(full(which, it), turn(which, it)); ++n) {}
         }
-    } else if (warp == 9) {
-        // ---- products ----
-        if (lane == 0) {
-            constexpr uint32_t i1 = tc_idesc(128, false, false), i2 = tc_idesc(VD, false, true), i4 = tc_idesc(VD, true, true);
-            for (int it = 0; it < chunks; ++it) {
-                const uint32_t ph = it & 1;
-                const uint32_t y = tile_at(it, 0), x = tile_at(it, kTileX), z = tile_at(it, kTileZ);
-                if constexpr (!STATE_ONLY) {
-                    if (it > 0 && !mbar_wait(bar(kO), ph ^ 1u, abort)) break;          // P has been read
-                    if (!mbar_wait(full(slot_of(it, 0)), phase_of(it, 0), abort) || !mbar_wait(full(slot_of(it, kTileX)), phase_of(it, kTileX), abort)) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int kk = 0; kk < KD / 16; ++kk) {
-                        const uint32_t off = (uint32_t)(kk / 4) * kTcBlock + (kk % 4) * 32;
-                        umma_bf16(tmem + kSc0, desc_k(x + off), desc_k(y + off), i1, kk > 0);
-                    }
-                    umma_commit(bar(kSc));
-                }
-                // (4)
-                if (!mbar_wait(full(slot_of(it, kTileZ)), phase_of(it, kTileZ), abort) || !mbar_wait(bar(kY), ph, abort)) break;
+    } else if (warp == 17) {
+        // ---- products (1) and (4) ----
+        constexpr uint32_t i1 = tc_idesc(128, false, false), i4 = tc_idesc(VD, true, true);
+        const uint32_t on = elect_one(), tm = __reduce_max_sync(0xffffffffu, tmem);
+        const int count = __reduce_max_sync(0xffffffffu, chunks);
+        for (int it = -1; it < count; ++it) {
+            if (it >= 0) {
+                if (!wait(full(Y, it), turn(Y, it)) || !wait(full(Z, it), turn(Z, it)) || !wait2(kY, it)) break;
                 tc_fence_after();
+                const uint64_t y = desc_mn(tile_at(Y, it), kTcBlock), yl = desc_mn(y_lo, kTcBlock), z = desc_mn(tile_at(Z, it), kTcBlock);
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                for (int kk = 0; kk < kTc / 16; ++kk) umma_ss(on, tm + kDelta0, y + kk * 128, z + kk * 128, i4, kk > 0);
 #pragma unroll
-                    for (int kk = 0; kk < kTc / 16; ++kk)
-                        umma_bf16(tmem + kDelta0, desc_mn((part ? y_lo : y) + kk * 2048, kTcBlock), desc_mn(z + kk * 2048, kTcBlock), i4, part > 0 || kk > 0);
-                umma_commit(bar(kDelta));
-                umma_commit(empty(slot_of(it, 0)));
-                if constexpr (STATE_ONLY) {
-                    umma_commit(empty(slot_of(it, kTileZ)));
-                } else {
-                    // (2)
-                    if (!mbar_wait(bar(kS), ph, abort) || (it > 0 && !mbar_wait(bar(kOFree), ph ^ 1u, abort))) break;
-                    tc_fence_after();
-                    for (int part = 0; part < (fine ? 2 : 1); ++part)
-#pragma unroll
-                        for (int kk = 0; kk < KD / 16; ++kk)
-                            umma_bf16(tmem + kO2, desc_k(x + (uint32_t)(kk / 4) * kTcBlock + (kk % 4) * 32), desc_mn((part ? s_lo : s_hi) + kk * 2048, KD * 128), i2, part > 0 || kk > 0);
-                    umma_commit(bar(kMma2));
-                    umma_commit(empty(slot_of(it, kTileX)));
-                    // (3)
-                    if (!mbar_wait(bar(kP), ph, abort)) break;
-                    tc_fence_after();
-                    for (int part = 0; part < (fine ? 2 : 1); ++part)
-#pragma unroll
-                        for (int kk = 0; kk < kTc / 16; ++kk)
-                            umma_bf16_ts(tmem + kO1, tmem + kSc0 + part * 64 + kk * 8, desc_mn(z + kk * 2048, kTcBlock), i2, part > 0 || kk > 0);
-                    umma_commit(bar(kO));
-                    umma_commit(empty(slot_of(it, kTileZ)));
-                }
+                for (int kk = 0; kk < kTc / 16; ++kk) umma_ss(on, tm + kDelta0, yl + kk * 128, z + kk * 128, i4, 1);
+                commit_if(on, bar(kDelta + (it & 1)));
+                commit_if(on, empty(Y, it));
+                if (STATE_ONLY || kStageX) commit_if(on, empty(Z, it));
             }
+            const int n = it + 1;
+            if (!STATE_ONLY && n < count) {
+                if (n > 1 && !wait2(kO, n - 2)) break;            // P of two chunks ago has been read
+                if (!wait(full(X, n), turn(X, n)) || !wait(full(Y, n), turn(Y, n))) break;
+                tc_fence_after();
+                const uint64_t x = desc_k(tile_at(X, n)), y = desc_k(tile_at(Y, n));
+#pragma unroll
+                for (int kk = 0; kk < KD / 16; ++kk) {
+                    const int off = ((kk / 4) * kTcBlock + (kk % 4) * 32) >> 4;
+                    umma_ss(on, tm + 128 * (n & 1), x + off, y + off, i1, kk > 0);
+                }
+                commit_if(on, bar(kSc + (n & 1)));
+                if (!kStageX) commit_if(on, empty(X, n));
+            }
+        }
+    } else if (warp == 18) {
+        // ---- products (2) and (3), and what becomes of out ----
+        if constexpr (!STATE_ONLY) {
+            constexpr uint32_t i2 = tc_idesc(VD, false, true);
+            constexpr int kStage = kStageX ? X : Z;
+            const uint32_t on = elect_one(), tm = __reduce_max_sync(0xffffffffu, tmem);
+            const int count = __reduce_max_sync(0xffffffffu, chunks);
+            // chunk n's rows are in their tile (or have been stored from registers)
+            auto store = [&](int n) {
+                if (on) {
+                    if (!k.out_f32) {
+                        for (int j = 0; 64 * j < k.Vd; ++j) tma_store_4d(&maps.m[ci][3], tile_at(kStage, n) + j * kTcBlock, 64 * j, h, chunk_at(n), b);
+                        bulk_commit();
+                        bulk_wait_read();
+                    }
+                    mbar_arrive(empty(kStage, n));
+                }
+                __syncwarp();
+            };
+            int it = 0;
+            for (; it < count; ++it) {
+                const uint32_t ph = it & 1;
+                if (it > 0) {
+                    if (!wait(bar(kOFree), ph ^ 1u)) break;
+                    store(it - 1);
+                }
+                if (!wait(full(X, it), turn(X, it)) || !wait(bar(kS), ph)) break;
+                tc_fence_after();
+                const uint64_t x = desc_k(tile_at(X, it)), sh = desc_mn(s_hi, KD * 128), sl = desc_mn(s_lo, KD * 128);
+#pragma unroll
+                for (int kk = 0; kk < KD / 16; ++kk) umma_ss(on, tm + kO0, x + (((kk / 4) * kTcBlock + (kk % 4) * 32) >> 4), sh + kk * 128, i2, kk > 0);
+                if (fine) {
+#pragma unroll
+                    for (int kk = 0; kk < KD / 16; ++kk) umma_ss(on, tm + kO0, x + (((kk / 4) * kTcBlock + (kk % 4) * 32) >> 4), sl + kk * 128, i2, 1);
+                }
+                commit_if(on, bar(kMma2));
+                if (!kStageX) commit_if(on, empty(X, it));
+                if (!wait(full(Z, it), turn(Z, it)) || !wait(bar(kP), ph)) break;
+                if (len - chunk_at(it) < kTc && !wait2(kY, it)) break;          // z's last rows have been cleared
+                if (!kStageX && !wait2(kDelta, it)) break;                       // out will overwrite z: (4) has read it
+                tc_fence_after();
+                const uint64_t z = desc_mn(tile_at(Z, it), kTcBlock);
+                const uint32_t p = tm + 128 * ph;                                // (a block's first parts, then its second parts: 16 columns each)
+#pragma unroll
+                for (int kk = 0; kk < kTc / 16; ++kk) umma_ts(on, tm + kO0, p + (kk / 2) * 32 + (kk % 2) * 8, z + kk * 128, i2, 1);
+                if (fine) {
+#pragma unroll
+                    for (int kk = 0; kk < kTc / 16; ++kk) umma_ts(on, tm + kO0, p + (kk / 2) * 32 + (kk % 2) * 8 + 16, z + kk * 128, i2, 1);
+                }
+                commit_if(on, bar(kO + (it & 1)));
+                if (kStageX) commit_if(on, empty(Z, it));
+            }
+            if (it == count && count && wait(bar(kOFree), (count & 1) ^ 1u)) store(count - 1);
+            if (on) bulk_wait();
+            __syncwarp();
         }
     } else {
         // ---- decays: four tokens a lane ----
         const float* const g = a.g + (long long)b * a.gb + (long long)h * a.gh;
         double whole = 0.0;
+        const float ratio = rev ? k.s_intra : 1.f;                // s_intra / s_inter
         for (int it = 0; it < chunks; ++it) {
-            const int t0 = chunk_at(it), valid = min(kTc, len - t0), j = lane >> 3;
-            double d[4];
+            const int t0 = chunk_at(it), valid = min(kTc, len - t0);
+            double c[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = 4 * lane + i < valid ? attn_decay(__ldg(g + (long long)(t0 + 4 * lane + i) * a.gt)) : 0.0;
+            for (int i = 0; i < 4; ++i) c[i] = 4 * lane + i < valid ? attn_decay(__ldg(g + (long long)(t0 + 4 * lane + i) * a.gt)) : 0.0;
 #pragma unroll
-            for (int i = 1; i < 4; ++i) d[i] += d[i - 1];
-            double up = d[3];
+            for (int i = 1; i < 4; ++i) c[i] += c[i - 1];
+            double up = c[3];
 #pragma unroll
-            for (int s = 1; s < 8; s <<= 1) {
+            for (int s = 1; s < 32; s <<= 1) {
                 const double o = __shfl_up_sync(0xffffffffu, up, s);
-                if ((lane & 7) >= s) up += o;
+                if (lane >= s) up += o;
             }
-            const double before = up - d[3];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] += before;
-            double start[5];
-            start[0] = 0.0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) start[i + 1] = start[i] + __shfl_sync(0xffffffffu, up, 8 * i + 7);
-            whole += start[4];
-            if (it > 0 && !wait(bar(kTabFree), (uint32_t)(it & 1) ^ 1u)) break;
-            double mine = 0.0;
-#pragma unroll
-            for (int i = 1; i < 4; ++i) mine = j == i ? start[i] : mine;
+            const double before = up - c[3], end = __shfl_sync(0xffffffffu, up, 31), m = 0.5 * end;
+            bool near = true;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int t = 4 * lane + i;
-                const float hi = (float)d[i];
-                tab.l[t] = make_float2(hi, (float)(d[i] - hi));
-                const double c = mine + d[i];
-                tab.u[t] = k.s_update * ex2((float)(rev ? c : start[4] - c));
+                c[i] += before;
+                near = near && fabsf((float)(c[i] - m)) <= kTcMild;       // (not where it is NaN)
+            }
+            const bool mild = __all_sync(0xffffffffu, near && fabsf((float)m) <= kTcMild);
+            whole += end;
+            if (it > 0 && !wait(bar(kTabFree), (uint32_t)(it & 1) ^ 1u)) break;
+            float f[4], e[4], u[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (!rev && q > j) tab.f[tc_f(0, q) + t] = ex2((float)(start[q] - c));
-                    if (rev && q < j) tab.f[tc_f(1, q) + t - 32 * (q + 1)] = ex2((float)(c - start[q + 1]));
-                }
+            for (int i = 0; i < 4; ++i) {
+                const float hi = (float)c[i], from_m = (float)(rev ? m - c[i] : c[i] - m);      // backwards m - c takes the place of c - m
+                f[i] = mild ? ratio * ex2(-from_m) : hi;
+                e[i] = mild ? k.s_inter * ex2(from_m) : (float)(c[i] - hi);
+                u[i] = k.s_update * ex2((float)(rev ? c[i] : end - c[i]));
             }
-            if ((lane & 7) == 7) {
-                const double base = rev ? start[4] - mine : mine, total = d[3];
-                tab.base[j] = make_float2((float)base, (float)(base - (double)(float)base));
-                tab.total[j] = make_float2((float)total, (float)(total - (double)(float)total));
+            reinterpret_cast<float4*>(tab.f)[lane] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4*>(tab.e)[lane] = make_float4(e[0], e[1], e[2], e[3]);
+            reinterpret_cast<float4*>(tab.u)[lane] = make_float4(u[0], u[1], u[2], u[3]);
+            if (lane == 0) {
+                tab.whole = ex2((float)end);
+                tab.copy = mild ? ex2((float)m) : 1.f;
+                tab.end = make_float2((float)end, (float)(end - (double)(float)end));
+                tab.mild = mild;
             }
-            if (lane == 0) tab.whole = ex2((float)start[4]);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kTabFull));
         }
@@ -526,28 +622,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 
     __syncthreads();
     if constexpr (!STATE_ONLY) {
-        // rows of chunks behind the sequence's last token: zero; rows that a given-up wait has left: NaN
-        if (warp < 4) {
-            const bool lost = *abort != 0;
+        // rows of chunks behind the sequence's last token: zero; where a wait has given up: NaN
+        if (warp < 8) {
             auto fill = [&](int from, int to, float v) {
-                for (int t = from + tid; t < to; t += 128) {
+                for (int t = from + warp; t < to; t += 8) {
                     const long long at = b * k.ob + (long long)t * k.ot + h * k.oh;
-                    for (int c = 0; c < k.Vd; ++c) {
+                    for (int c = lane; c < k.Vd; c += 32) {
                         if (k.out_f32) static_cast<float*>(k.out)[at + c] = v;
                         else static_cast<__nv_bfloat16*>(k.out)[at + c] = __float2bfloat16_rn(v);
                     }
-                    if (k.dots) k.dots[((size_t)b * a.T + t) * a.H + h] = v;
+                    if (k.dots && lane < 2) k.dots[(((size_t)lane * a.B + b) * a.T + t) * a.H + h] = v;
                 }
             };
             if (t_lo + chunks * kTc < t_hi) fill(t_lo + chunks * kTc, t_hi, 0.f);
-            if (lost)
-                for (int it = 0; it < chunks; ++it) fill(chunk_at(it), min(t_hi, chunk_at(it) + kTc), __int_as_float(0x7fc00000));
+            if (*abort) fill(t_lo, min(t_hi, t_lo + chunks * kTc), __int_as_float(0x7fc00000));
         }
     }
-    if (tid == 0 && abort_flag && L.host_flag) *reinterpret_cast<volatile int*>(L.host_flag) = 1;
+    if (tid == 0 && *abort && L.host_flag) *reinterpret_cast<volatile int*>(L.host_flag) = 1;
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem, kCols);
+    if (warp == 16) tmem_dealloc(tmem, kCols);
 }
 
 }  // namespace m2d

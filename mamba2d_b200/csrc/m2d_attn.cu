@@ -273,19 +273,29 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
         }
 }
 
-// The segments' own states become the states that they start from.
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnLaunch a) {
+// The segments' own states become the states that they start from.  A thread has one element of the states; the reads of
+// eight segments are under way at once (one by one, their latency was 50 us for 16 segments).
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnLaunch a) {
     const AttnCore& k = a.core[blockIdx.z];
     const int bh = blockIdx.x, h = bh % a.H, b = bh / a.H, n = k.Kd * k.Vd;
-    const int i = blockIdx.y * 256 + threadIdx.x;
+    const int i = blockIdx.y * 128 + threadIdx.x;
     if (i >= n) return;
     float carry = k.init.p ? k.init.p[b * k.init.sb + h * k.init.sh + (i / k.Vd) * k.init.sr + (i % k.Vd) * k.init.sc] : 0.f;
-    for (int j = 0; j < a.nseg; ++j) {
-        const int seg = k.rev ? a.nseg - 1 - j : j;
-        const size_t at = (size_t)bh * a.nseg + seg;
-        const float own = k.seg_state[at * n + i];
-        k.seg_state[at * n + i] = carry;
-        carry = fmaf(carry, ex2(k.seg_decay[at]), own);
+    for (int j0 = 0; j0 < a.nseg; j0 += 8) {
+        float own[8], decay[8];
+        auto at = [&](int j) { return (size_t)bh * a.nseg + (k.rev ? a.nseg - 1 - j : j); };
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < a.nseg) {
+                own[j] = k.seg_state[at(j0 + j) * n + i];
+                decay[j] = k.seg_decay[at(j0 + j)];
+            }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < a.nseg) {
+                k.seg_state[at(j0 + j) * n + i] = carry;
+                carry = fmaf(carry, ex2(decay[j]), own[j]);
+            }
     }
 }
 
@@ -461,6 +471,7 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     p.tc = tc;
     p.cores = bwd ? 3 : 1;
     int per_sm = 1;
+    p.dot_blocks = 2;                  // (the tcgen05 form's threads have half of the columns each)
     if (!tc) {
         const int big = bwd ? std::max(d->K, d->V) : d->K, out = bwd ? big : d->V;
         p.VT = big > 192 ? 32 : 64;
@@ -526,11 +537,13 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
         const AttnCore& c = L.a.core[i] = p.a.core[first + i];
         if (c.dots) L.fine |= 1 << i;
         if (!(STATE_ONLY || attn_map(&maps.m[i][0], d, c.x, c.Kd)) || !attn_map(&maps.m[i][1], d, c.y, c.Kd) || !attn_map(&maps.m[i][2], d, c.z, c.Vd)) return M2D_ERR_LAUNCH;
+        if (!STATE_ONLY && !c.out_f32 && !attn_map(&maps.m[i][3], d, {c.out, c.ob, c.ot, c.oh, 1, 1}, c.Vd)) return M2D_ERR_LAUNCH;
     }
-    const bool fine = !STATE_ONLY && L.fine;
-    L.slots = tc_slots(KD, VD, fine);
+    if (STATE_ONLY) L.fine = 0;
+    const bool fine = L.fine != 0;
     L.host_flag = wait_failure_flag();
-    const size_t smem = tc_smem(KD, VD, fine, L.slots);
+    L.small = (uint32_t)tc_plan_tiles(KD, VD, fine, STATE_ONLY, L.n);
+    const size_t smem = L.small + sizeof(TcSmall);
     auto kern = attn_tc_kernel<KD, VD, STATE_ONLY>;
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     kern<<<(unsigned)(d->B * d->H * p.a.nseg * count), kTcThreads, smem, st>>>(maps, L);
@@ -545,7 +558,7 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
 
 static void launch_join(const AttnPlan& p, cudaStream_t st) {
     const int n = p.a.core[0].Kd * p.a.core[0].Vd;
-    attn_join_kernel<<<dim3(p.a.B * p.a.H, (n + 255) / 256, p.cores), 256, 0, st>>>(p.a);
+    attn_join_kernel<<<dim3(p.a.B * p.a.H, (n + 127) / 128, p.cores), 128, 0, st>>>(p.a);
 }
 template <typename io_t, int VT>
 static int launch_any(const AttnPlan& p, cudaStream_t st) {

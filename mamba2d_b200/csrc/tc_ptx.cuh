@@ -22,10 +22,21 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");   // suspends for at most ~1 us per try
     return ok != 0;
 }
+// Up to 32 tries in a loop of three instructions: what a waiting warp issues, others on its scheduler do not.
+__device__ __forceinline__ bool mbar_try_wait32(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 32;\n"
+        "again_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t@p bra done_%=;\n\t"
+        "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra again_%=;\n"
+        "done_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+    return ok != 0;
+}
 // Bounded wait; returns false (and raises *abort) when it gives up or another wait already has.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-    for (int n = 0; n < kTcWaitLimit; ++n) {
-        if (mbar_try_wait(bar, parity)) return true;
+    for (int n = 0; n < kTcWaitLimit / 32; ++n) {
+        if (mbar_try_wait32(bar, parity)) return true;
         if (*abort) return false;
     }
     *abort = 1;
