@@ -624,7 +624,7 @@ extern "C" int m2d_attn_fwd(const m2d_attn_desc* d, void* stream) {
     if (rc != M2D_OK) return rc;
     if (!d->o) return M2D_ERR_NULL;
     AttnPlan p = plan_attn(d, false, tc_applies(d, false));
-    if ((rc = check_workspace(d, p.bytes)) != M2D_OK) return rc;
+    if ((rc = check_workspace(d, attn_workspace(d, false))) != M2D_OK) return rc;
     fill_launch(d, p);
     AttnCore& c = p.a.core[0];
     const int per = d->H / d->G;
@@ -642,7 +642,7 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     if (rc != M2D_OK) return rc;
     if (!d->d_o.data || !d->d_q || !d->d_k || !d->d_v) return M2D_ERR_NULL;
     AttnPlan p = plan_attn(d, true, tc_applies(d, true));
-    if ((rc = check_workspace(d, p.bytes)) != M2D_OK) return rc;
+    if ((rc = check_workspace(d, attn_workspace(d, true))) != M2D_OK) return rc;
     fill_launch(d, p);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     char* const ws = static_cast<char*>(d->workspace);

@@ -281,24 +281,31 @@ Tensor group_norm(const Tensor& x_, const optional<Tensor>& weight_, const optio
 // ---- clipping ---------------------------------------------------------------------------------------
 
 Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm) {
-    TORCH_CHECK(!grads.empty(), "clip_grad_norm_: no gradients");
+    TORCH_CHECK(!grads.empty(), "clip_norm_: no tensors");
     const Tensor& first = grads[0];
     std::vector<m2d_clip_tensor> table;
     std::vector<std::pair<const char*, const char*>> spans;
     table.reserve(grads.size());
     spans.reserve(grads.size());
+    bool sorted = true;
+    const bool recording = at::GradMode::is_enabled();
     for (const Tensor& g : grads) {
-        TORCH_CHECK(g.layout() == at::kStrided && g.is_cuda() && (g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16),
-                    "clip_grad_norm_: gradients must be CUDA tensors, float32 or bfloat16");
-        TORCH_CHECK(g.device() == first.device(), "clip_grad_norm_: gradients on ", g.device(), " and ", first.device());
-        TORCH_CHECK(g.is_non_overlapping_and_dense(), "clip_grad_norm_: a gradient has gaps or overlaps itself (sizes ", g.sizes(), ", strides ", g.strides(), ")");
-        if (!g.numel()) continue;
-        table.push_back({g.data_ptr(), g.numel(), dtype_of(g)});
+        TORCH_CHECK(g.is_cuda() && g.layout() == at::kStrided, "clip_norm_: tensors must be dense and on a CUDA device (there is no CPU path)");
+        TORCH_CHECK(g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16, "clip_norm_: unsupported dtype ", g.scalar_type(), " (float32 and bfloat16 only)");
+        TORCH_CHECK(g.device() == first.device(), "clip_norm_: tensors on ", g.device(), " and ", first.device());
+        TORCH_CHECK(!recording || !g.requires_grad(), "clip_norm_: a tensor that requires a gradient is not scaled in place");
+        TORCH_CHECK(g.is_contiguous() || g.is_non_overlapping_and_dense(), "clip_norm_: a tensor has gaps or overlaps itself (sizes ", g.sizes(), ", strides ", g.strides(), ")");
+        const int64_t n = g.numel();
+        if (!n) continue;
         const char* p = static_cast<const char*>(g.data_ptr());
-        spans.emplace_back(p, p + g.numel() * g.element_size());
+        table.push_back({const_cast<char*>(p), n, dtype_of(g)});
+        sorted = sorted && (spans.empty() || spans.back().second <= p);
+        spans.emplace_back(p, p + n * g.element_size());
     }
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); ++i) TORCH_CHECK(spans[i - 1].second <= spans[i].first, "clip_grad_norm_: two gradients share memory");
+    if (!sorted) {
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i) TORCH_CHECK(spans[i - 1].second <= spans[i].first, "clip_norm_: two tensors share memory");
+    }
     const c10::cuda::CUDAGuard guard(first.device());
     const Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
     const uint64_t bytes = m2d_clip_workspace(table.data(), (int32_t)table.size());

@@ -170,13 +170,6 @@ def clip_norm_(tensors, max_norm, error_if_nonfinite=False):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError("clip_norm_: tensors must be on a CUDA device (there is no CPU path)")
-        if t.dtype not in _TYPES:
-            raise RuntimeError(f"clip_norm_: unsupported dtype {t.dtype} (float32 and bfloat16 only)")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("clip_norm_: a tensor that requires a gradient is not scaled in place")
     entry = _lib.entry()
     if error_if_nonfinite:
         total = entry.clip_grad_norm(tensors, float("inf"))
