@@ -17,8 +17,9 @@
 //     warps 8 - 15   half of a token row a thread: y -> u y; half of a row of St a thread: St in registers, its bf16 copy
 //     warp 16  TMA loads    warps 17, 18  issue (1), (4) and (2), (3)     warp 19  the decays' tables
 // pairs has two places, so that (1) of the next chunk runs beside (3) of this one.  The copy of St is written while (4) runs, after
-// u y: what bounds a chunk is the chain u y -> (4) -> St.  out goes through the tile of x (or z, where that is the larger
-// one), which nothing reads any more, and by TMA: rows stored from registers took 2000 cycles of a chunk, 32 lines a request.
+// u y: what bounds a chunk is the chain u y -> (4) -> St.  out goes through shared memory and by TMA: rows stored from registers
+// took 2000 cycles of a chunk, 32 lines a request.  It has a tile of its own where there is room (a head size of 64), else that of x,
+// which nothing reads any more, but whose next load then waits for it.
 //
 // `fine` (wanted where the decay's gradient is): P and St also in two parts each, so that the dots that out is summed
 // into are exact to 2^-17 like the states that they meet.
@@ -43,6 +44,7 @@ struct TcLaunch {
     AttnLaunch a;
     int cores;
     int n[3];                                 // tiles of x, y, z
+    int own_stage;                            // out has a tile of its own, else it goes through x's
     uint32_t small;                           // where TcSmall lies in shared memory
     int fine;                                 // bit per core
     int* host_flag;
@@ -68,17 +70,34 @@ __device__ __forceinline__ uint32_t elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
     return on;
 }
-__device__ __forceinline__ void umma_ss(uint32_t on, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// A descriptor's lower half (address and distance of blocks) in a uniform register, where a reduction over the warp leaves it; its
+// upper half is a constant.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t next) { return uniform(((addr & 0x3ffffu) >> 4) | ((next >> 4) << 16)); }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+template <uint32_t IDESC, bool ACCUMULATE>
+__device__ __forceinline__ void umma_ss(uint32_t on, uint32_t tmem_d, uint32_t a, uint32_t b) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 i;\n\tsetp.ne.b32 q, %3, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\tmov.b32 i, %5;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, i, p;\n\t}"
+        ::"r"(tmem_d), "r"(a), "r"(b), "r"(on), "n"(kDescHi), "n"(IDESC), "n"(ACCUMULATE ? 1 : 0) : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t on, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+template <uint32_t IDESC, bool ACCUMULATE>
+__device__ __forceinline__ void umma_ts(uint32_t on, uint32_t tmem_d, uint32_t tmem_a, uint32_t b) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t.reg .b32 i;\n\tsetp.ne.b32 q, %3, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 db, {%2, %4};\n\tmov.b32 i, %5;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, i, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(on), "n"(kDescHi), "n"(IDESC), "n"(ACCUMULATE ? 1 : 0) : "memory");
+}
+// `n` products, one for each 16 of the contraction: a and b of the k-th; the first one starts the accumulator unless GO_ON
+template <uint32_t IDESC, bool GO_ON, int N, typename FA, typename FB>
+__device__ __forceinline__ void umma_chain(uint32_t on, uint32_t tmem_d, FA fa, FB fb) {
+    if constexpr (GO_ON) umma_ss<IDESC, true>(on, tmem_d, fa(0), fb(0));
+    else umma_ss<IDESC, false>(on, tmem_d, fa(0), fb(0));
+#pragma unroll
+    for (int k = 1; k < N; ++k) umma_ss<IDESC, true>(on, tmem_d, fa(k), fb(k));
 }
 __device__ __forceinline__ void commit_if(uint32_t on, uint32_t bar) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(on) : "memory");
@@ -101,12 +120,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// Operand descriptors of the 128-byte-swizzle layout (wgrad_tc.cuh): contraction along the 128-byte rows ("K-major"), or across
-// them ("MN-major", `next` bytes to the next 64 columns).
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return desc_mn(addr, 16); }
+// Operand descriptors of the 128-byte-swizzle layout are wgrad_tc.cuh's; an operand is contracted along its 128-byte rows
+// ("K-major"), or across them ("MN-major", `next` bytes to the next 64 columns).
 __host__ __device__ constexpr uint32_t tc_idesc(int n, bool a_mn, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
@@ -131,26 +146,35 @@ struct alignas(16) TcSmall {
 // whatever lies behind y, are not used, and a tile lies there.)
 inline size_t tc_fixed_smem(int KD, int VD, bool fine, bool state_only) { return (state_only ? 0 : (size_t)KD * VD * 2 * (fine ? 2 : 1)) + (size_t)kTc * KD * 2; }
 // Tiles of x, y, z: x first, whose tile is held longest, z last, which is needed last.
-inline size_t tc_plan_tiles(int KD, int VD, bool fine, bool state_only, int (&n)[3]) {
+inline size_t tc_plan_tiles(int KD, int VD, bool fine, bool state_only, int (&n)[3], int* own_stage) {
     const size_t tile[3] = {(size_t)kTc * KD * 2, (size_t)kTc * KD * 2, (size_t)kTc * VD * 2};
     n[0] = state_only ? 0 : 1; n[1] = n[2] = 1;
     size_t bytes = tc_fixed_smem(KD, VD, fine, state_only) + n[0] * tile[0] + tile[1] + tile[2];
-    for (int round = 1; round < kTcTiles; ++round)
+    *own_stage = 0;
+    for (int round = 1; round < kTcTiles; ++round) {
+        if (round == 2 && !state_only && (KD < VD || bytes + tile[2] + sizeof(TcSmall) <= kMaxSmem)) {
+            *own_stage = 1;
+            bytes += tile[2];
+        }
         for (int i = state_only ? 1 : 0; i < 3; ++i)
             if (n[i] == round && bytes + tile[i] + sizeof(TcSmall) <= kMaxSmem) {
                 ++n[i];
                 bytes += tile[i];
             }
+    }
     return bytes;
 }
 
-template <int KD, int VD, bool STATE_ONLY>
+// What a launch is for.  kTcPlain: bf16 out and nothing else, the least code (20 warps in five roles miss the instruction caches often).
+enum TcMode { kTcPlain, kTcFull, kTcStateOnly };
+
+template <int KD, int VD, TcMode MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcLaunch L) {
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
     // (kSc, kY, kO, kDelta: one for even chunks, one for odd, where a barrier may complete again before all have seen it)
     enum { kSc, kP = kSc + 2, kY, kO = kY + 2, kOFree = kO + 2, kDelta, kS = kDelta + 2, kMma2, kTabFull, kTabFree, kFull, kEmpty = kFull + 3 * kTcTiles, kBars = kEmpty + 3 * kTcTiles };
     static_assert(kBars <= 40, "room for the barriers");
-    constexpr bool kStageX = VD <= KD;                            // out goes through x's tile, else z's
+    constexpr bool STATE_ONLY = MODE == kTcStateOnly;
     constexpr int kHalf = VD / 2;                                 // columns of a thread
     constexpr uint32_t kTileX = kTc * KD * 2, kTileZ = kTc * VD * 2;
     constexpr uint32_t kO0 = 256;                                 // columns of tensor memory: pairs (2 x 128), O, delta
@@ -160,7 +184,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     const AttnLaunch& a = L.a;
     const int ci = blockIdx.x % L.cores, unit = blockIdx.x / L.cores;
     const AttnCore& k = a.core[ci];
-    const bool fine = !STATE_ONLY && (L.fine >> ci & 1);
+    const bool fine = MODE == kTcFull && (L.fine >> ci & 1), f32_out = MODE == kTcFull && k.out_f32, dots = MODE == kTcFull && k.dots;
     const int seg = unit % a.nseg, bh = unit / a.nseg, h = bh % a.H, b = bh / a.H;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rev = k.rev;
     const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
@@ -170,7 +194,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     TcTable& tab = small.tab;
     // (the launch's second parts take room whether this core has them or not)
     const uint32_t s_hi = smem_u32(tc_smem_raw), s_lo = s_hi + KD * VD * 2, y_lo = STATE_ONLY ? s_hi : s_hi + KD * VD * 2 * (L.fine ? 2 : 1);
-    const uint32_t ring_x = y_lo + kTileX, ring_y = ring_x + L.n[0] * kTileX, ring_z = ring_y + L.n[1] * kTileX;
+    const uint32_t ring_x = y_lo + kTileX, ring_y = ring_x + L.n[0] * kTileX, ring_z = ring_y + L.n[1] * kTileX, stage_own = ring_z + L.n[2] * kTileZ;
     const uint32_t bar0 = smem_u32(small.bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
     enum { X, Y, Z };
@@ -187,8 +211,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     if (tid == 0) {
         for (int i = 0; i < kFull; ++i) mbar_init(bar(i), i == kP || i == kY || i == kY + 1 || i == kOFree || i == kS ? 8 : i == kTabFree ? (STATE_ONLY ? 8 : 16) : 1);
         for (int i = kFull; i < kEmpty; ++i) mbar_init(bar(i), 1);
-        // who gives a tile back: y after (4); the one that out goes through after that; another after its two products
-        for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || i / kTcTiles == (kStageX ? X : Z) ? 1 : 2);
+        // who gives a tile back: its two products, (1) and (4) counted as one; x's where out goes through it, whoever stores that
+        for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || (i / kTcTiles == X && !L.own_stage) ? 1 : 2);
         small.abort = (smem_u32(tc_smem_raw) & 1023u) != 0;      // (swizzled tiles have to be aligned; nothing runs if they are not)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -221,38 +245,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 for (int i = 0; i < 2; ++i) {
                     const int j = half ? 1 + i : 3 * i;
                     const uint32_t at = pairs + 32 * j;
-                    uint32_t p[16];
-                    if (rev ? j < q : j > q) {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) p[c] = 0;
-                        tmem_st16(at, p);
-                        if (fine) tmem_st16(at + 16, p);
-                        continue;
-                    }
+                    const bool off = rev ? j < q : j > q;
                     float v[32];
-                    tmem_ld32(at, v);
-                    const float4* const f = reinterpret_cast<const float4*>(tab.f + 32 * j);
-                    if (mild) {
+                    if (off) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4) {
-                            const float4 g = f[c / 4];
-                            const float2 v0 = __fmul2_rn(make_float2(v[c], v[c + 1]), make_float2(g.x, g.y)), v1 = __fmul2_rn(make_float2(v[c + 2], v[c + 3]), make_float2(g.z, g.w));
-                            v[c] = v0.x; v[c + 1] = v0.y; v[c + 2] = v1.x; v[c + 3] = v1.y;
-                        }
+                        for (int c = 0; c < 32; ++c) v[c] = 0.f;
                     } else {
-                        const float cr = tab.f[r], ratio = rev ? k.s_intra : 1.f, sign = rev ? -1.f : 1.f;
+                        tmem_ld32(at, v);
+                        const float4* const f = reinterpret_cast<const float4*>(tab.f + 32 * j);
+                        if (__builtin_expect(mild, 1)) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) v[c] *= ratio * ex2(sign * ((cr - tab.f[32 * j + c]) + (e - tab.e[32 * j + c])));
-                    }
-                    if (j == q) {
-                        const unsigned on = rev ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);
+                            for (int c = 0; c < 32; c += 4) {
+                                const float4 g = f[c / 4];
+                                const float2 v0 = __fmul2_rn(make_float2(v[c], v[c + 1]), make_float2(g.x, g.y)), v1 = __fmul2_rn(make_float2(v[c + 2], v[c + 3]), make_float2(g.z, g.w));
+                                v[c] = v0.x; v[c + 1] = v0.y; v[c + 2] = v1.x; v[c + 3] = v1.y;
+                            }
+                        } else {
+                            const float cr = tab.f[r], ratio = rev ? k.s_intra : 1.f, sign = rev ? -1.f : 1.f;
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) v[c] = on >> c & 1 ? v[c] : 0.f;
-                    }
-                    if (valid < kTc) {
+                            for (int c = 0; c < 32; ++c) v[c] *= ratio * ex2(sign * ((cr - tab.f[32 * j + c]) + (e - tab.e[32 * j + c])));
+                        }
+                        unsigned on = 0xffffffffu;
+                        if (j == q) on = rev ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);
+                        if (valid < 32 * j + 32) on &= valid <= 32 * j ? 0u : 0xffffffffu >> (32 * j + 32 - valid);
+                        if (__any_sync(0xffffffffu, on != 0xffffffffu)) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) v[c] = 32 * j + c < valid ? v[c] : 0.f;
+                            for (int c = 0; c < 32; ++c) v[c] = on >> c & 1 ? v[c] : 0.f;
+                        }
                     }
+                    uint32_t p[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) p[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
                     tmem_st16(at, p);
@@ -262,7 +283,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                         tmem_st16(at + 16, p);
                     }
                 }
-                if (!mild) {                                      // O2 -> w O2
+                if (__builtin_expect(!mild, 0)) {                 // O2 -> w O2
                     const float c = tab.f[r], w = rev ? ex2((tab.end.x - c) + (tab.end.y - e)) : ex2(c + e);
                     e = k.s_inter;
                     if (!wait(bar(kMma2), it & 1)) break;
@@ -286,8 +307,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 }
                 // O -> out
                 const bool row = t0 + r < t_hi, live = r < valid;
-                const __nv_bfloat16* const er = k.dots && live ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st + half * kHalf : nullptr;
-                const uint32_t stage = tile_at(kStageX ? X : Z, it);
+                const __nv_bfloat16* const er = dots && live ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st + half * kHalf : nullptr;
+                const uint32_t stage = L.own_stage ? stage_own : tile_at(X, it);
                 float sum = 0.f;
                 if (!wait2(kO, it)) break;
                 tc_fence_after();
@@ -298,11 +319,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     tmem_ld32(oc + c0, o);
 #pragma unroll
                     for (int c = 0; c < 32; ++c) o[c] *= e;
-                    if (valid < kTc) {
+                    if (__builtin_expect(valid < kTc, 0)) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) o[c] = live ? o[c] : 0.f;
                     }
-                    if (!k.out_f32) {
+                    if (!f32_out) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 8)
                             sts(piece(stage, kTc, r, (col + c) / 8), pack_bf16x2(o[c], o[c + 1]), pack_bf16x2(o[c + 2], o[c + 3]), pack_bf16x2(o[c + 4], o[c + 5]), pack_bf16x2(o[c + 6], o[c + 7]));
@@ -330,7 +351,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 async_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(kOFree));
-                if (k.dots && row) k.dots[(((size_t)half * a.B + b) * a.T + t0 + r) * a.H + h] = sum;
+                if (dots && row) k.dots[(((size_t)half * a.B + b) * a.T + t0 + r) * a.H + h] = sum;
             }
         }
     } else if (warp < 16) {
@@ -371,8 +392,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         };
         // St before (rev) or after the chunk at t0, if that ends a run; also of the chunks that hold nothing
         auto keep = [&](int from, int to) {
-            if (!k.anchors) return;
-            for (int t0 = from; t0 < to; t0 += kTc)
+            for (int t0 = from; MODE == kTcFull && k.anchors && t0 < to; t0 += kTc)
                 if ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, k.Vd, 1);
         };
         const int behind = t_lo + chunks * kTc;
@@ -392,20 +412,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 const uint32_t at = piece(y, kTc, r, c);
                 uint32_t g[4], hi[4], lo[4];
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(at) : "memory");
+                if (__builtin_expect(valid < kTc, 0) && r >= valid) g[0] = g[1] = g[2] = g[3] = 0;      // (such a row may hold anything: no product with zero)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // (a row behind the last token may hold anything: it becomes zero, not a product with zero)
-                    if (r >= valid) g[i] = 0;
-                    const float2 y2 = make_float2(__uint_as_float(g[i] << 16), __uint_as_float(g[i] & 0xffff0000u)), u2 = make_float2(u, u);
-                    const float2 h2 = __fmul2_rn(y2, u2);
-                    hi[i] = pack_bf16x2(h2.x, h2.y);
-                    const float2 l2 = __ffma2_rn(y2, u2, make_float2(__uint_as_float((hi[i] << 16) ^ 0x80000000u), __uint_as_float((hi[i] & 0xffff0000u) ^ 0x80000000u)));
-                    lo[i] = pack_bf16x2(l2.x, l2.y);
+                    const float2 v = __fmul2_rn(make_float2(__uint_as_float(g[i] << 16), __uint_as_float(g[i] & 0xffff0000u)), make_float2(u, u));
+                    hi[i] = pack_bf16x2(v.x, v.y);
+                    const float2 rest = __ffma2_rn(make_float2(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), make_float2(-1.f, -1.f), v);
+                    lo[i] = pack_bf16x2(rest.x, rest.y);
                 }
                 sts(at, hi[0], hi[1], hi[2], hi[3]);
                 sts(piece(y_lo, kTc, r, c), lo[0], lo[1], lo[2], lo[3]);
             }
-            if (valid < kTc) {                                    // z's rows there meet zeros in P and in u y
+            if (__builtin_expect(valid < kTc, 0)) {               // z's rows there meet zeros in P and in u y
                 if (!__all_sync(0xffffffffu, loaded(Z, it))) break;
                 if (r >= valid) {
 #pragma unroll 1
@@ -483,52 +501,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     } else if (warp == 17) {
         // ---- products (1) and (4) ----
         constexpr uint32_t i1 = tc_idesc(128, false, false), i4 = tc_idesc(VD, true, true);
-        const uint32_t on = elect_one(), tm = __reduce_max_sync(0xffffffffu, tmem);
+        const uint32_t on = elect_one(), tm = uniform(tmem);
         const int count = __reduce_max_sync(0xffffffffu, chunks);
         for (int it = -1; it < count; ++it) {
             if (it >= 0) {
                 if (!wait(full(Y, it), turn(Y, it)) || !wait(full(Z, it), turn(Z, it)) || !wait2(kY, it)) break;
                 tc_fence_after();
-                const uint64_t y = desc_mn(tile_at(Y, it), kTcBlock), yl = desc_mn(y_lo, kTcBlock), z = desc_mn(tile_at(Z, it), kTcBlock);
-#pragma unroll
-                for (int kk = 0; kk < kTc / 16; ++kk) umma_ss(on, tm + kDelta0, y + kk * 128, z + kk * 128, i4, kk > 0);
-#pragma unroll
-                for (int kk = 0; kk < kTc / 16; ++kk) umma_ss(on, tm + kDelta0, yl + kk * 128, z + kk * 128, i4, 1);
+                const uint32_t y = desc_lo(tile_at(Y, it), kTcBlock), yl = desc_lo(y_lo, kTcBlock), z = desc_lo(tile_at(Z, it), kTcBlock);
+                umma_chain<i4, false, kTc / 16>(on, tm + kDelta0, [&](int k) { return y + k * 128; }, [&](int k) { return z + k * 128; });
+                umma_chain<i4, true, kTc / 16>(on, tm + kDelta0, [&](int k) { return yl + k * 128; }, [&](int k) { return z + k * 128; });
                 commit_if(on, bar(kDelta + (it & 1)));
                 commit_if(on, empty(Y, it));
-                if (STATE_ONLY || kStageX) commit_if(on, empty(Z, it));
+                commit_if(on, empty(Z, it));
             }
             const int n = it + 1;
             if (!STATE_ONLY && n < count) {
                 if (n > 1 && !wait2(kO, n - 2)) break;            // P of two chunks ago has been read
                 if (!wait(full(X, n), turn(X, n)) || !wait(full(Y, n), turn(Y, n))) break;
                 tc_fence_after();
-                const uint64_t x = desc_k(tile_at(X, n)), y = desc_k(tile_at(Y, n));
-#pragma unroll
-                for (int kk = 0; kk < KD / 16; ++kk) {
-                    const int off = ((kk / 4) * kTcBlock + (kk % 4) * 32) >> 4;
-                    umma_ss(on, tm + 128 * (n & 1), x + off, y + off, i1, kk > 0);
-                }
+                const uint32_t x = desc_lo(tile_at(X, n), 16), y = desc_lo(tile_at(Y, n), 16);
+                umma_chain<i1, false, KD / 16>(on, tm + 128 * (n & 1), [&](int k) { return x + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4); },
+                                               [&](int k) { return y + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4); });
                 commit_if(on, bar(kSc + (n & 1)));
-                if (!kStageX) commit_if(on, empty(X, n));
+                if (L.own_stage) commit_if(on, empty(X, n));
             }
         }
     } else if (warp == 18) {
         // ---- products (2) and (3), and what becomes of out ----
         if constexpr (!STATE_ONLY) {
             constexpr uint32_t i2 = tc_idesc(VD, false, true);
-            constexpr int kStage = kStageX ? X : Z;
-            const uint32_t on = elect_one(), tm = __reduce_max_sync(0xffffffffu, tmem);
+            const uint32_t on = elect_one(), tm = uniform(tmem);
             const int count = __reduce_max_sync(0xffffffffu, chunks);
             // chunk n's rows are in their tile (or have been stored from registers)
             auto store = [&](int n) {
                 if (on) {
-                    if (!k.out_f32) {
-                        for (int j = 0; 64 * j < k.Vd; ++j) tma_store_4d(&maps.m[ci][3], tile_at(kStage, n) + j * kTcBlock, 64 * j, h, chunk_at(n), b);
+                    if (!f32_out) {
+                        for (int j = 0; 64 * j < k.Vd; ++j) tma_store_4d(&maps.m[ci][3], (L.own_stage ? stage_own : tile_at(X, n)) + j * kTcBlock, 64 * j, h, chunk_at(n), b);
                         bulk_commit();
                         bulk_wait_read();
                     }
-                    mbar_arrive(empty(kStage, n));
+                    if (!L.own_stage) mbar_arrive(empty(X, n));
                 }
                 __syncwarp();
             };
@@ -541,29 +553,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 }
                 if (!wait(full(X, it), turn(X, it)) || !wait(bar(kS), ph)) break;
                 tc_fence_after();
-                const uint64_t x = desc_k(tile_at(X, it)), sh = desc_mn(s_hi, KD * 128), sl = desc_mn(s_lo, KD * 128);
-#pragma unroll
-                for (int kk = 0; kk < KD / 16; ++kk) umma_ss(on, tm + kO0, x + (((kk / 4) * kTcBlock + (kk % 4) * 32) >> 4), sh + kk * 128, i2, kk > 0);
-                if (fine) {
-#pragma unroll
-                    for (int kk = 0; kk < KD / 16; ++kk) umma_ss(on, tm + kO0, x + (((kk / 4) * kTcBlock + (kk % 4) * 32) >> 4), sl + kk * 128, i2, 1);
-                }
+                const uint32_t x = desc_lo(tile_at(X, it), 16), sh = desc_lo(s_hi, KD * 128), sl = desc_lo(s_lo, KD * 128);
+                auto xk = [&](int k) { return x + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4); };
+                umma_chain<i2, false, KD / 16>(on, tm + kO0, xk, [&](int k) { return sh + k * 128; });
+                if (fine) umma_chain<i2, true, KD / 16>(on, tm + kO0, xk, [&](int k) { return sl + k * 128; });
                 commit_if(on, bar(kMma2));
-                if (!kStageX) commit_if(on, empty(X, it));
+                if (L.own_stage) commit_if(on, empty(X, it));
                 if (!wait(full(Z, it), turn(Z, it)) || !wait(bar(kP), ph)) break;
                 if (len - chunk_at(it) < kTc && !wait2(kY, it)) break;          // z's last rows have been cleared
-                if (!kStageX && !wait2(kDelta, it)) break;                       // out will overwrite z: (4) has read it
                 tc_fence_after();
-                const uint64_t z = desc_mn(tile_at(Z, it), kTcBlock);
-                const uint32_t p = tm + 128 * ph;                                // (a block's first parts, then its second parts: 16 columns each)
+                const uint32_t z = desc_lo(tile_at(Z, it), kTcBlock), p = uniform(tm + 128 * ph);       // (a block's first parts, then its second parts: 16 columns each)
 #pragma unroll
-                for (int kk = 0; kk < kTc / 16; ++kk) umma_ts(on, tm + kO0, p + (kk / 2) * 32 + (kk % 2) * 8, z + kk * 128, i2, 1);
+                for (int k = 0; k < kTc / 16; ++k) umma_ts<i2, true>(on, tm + kO0, p + (k / 2) * 32 + (k % 2) * 8, z + k * 128);
                 if (fine) {
 #pragma unroll
-                    for (int kk = 0; kk < kTc / 16; ++kk) umma_ts(on, tm + kO0, p + (kk / 2) * 32 + (kk % 2) * 8 + 16, z + kk * 128, i2, 1);
+                    for (int k = 0; k < kTc / 16; ++k) umma_ts<i2, true>(on, tm + kO0, p + (k / 2) * 32 + (k % 2) * 8 + 16, z + k * 128);
                 }
                 commit_if(on, bar(kO + (it & 1)));
-                if (kStageX) commit_if(on, empty(Z, it));
+                commit_if(on, empty(Z, it));
             }
             if (it == count && count && wait(bar(kOFree), (count & 1) ^ 1u)) store(count - 1);
             if (on) bulk_wait();
@@ -628,10 +635,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 for (int t = from + warp; t < to; t += 8) {
                     const long long at = b * k.ob + (long long)t * k.ot + h * k.oh;
                     for (int c = lane; c < k.Vd; c += 32) {
-                        if (k.out_f32) static_cast<float*>(k.out)[at + c] = v;
+                        if (f32_out) static_cast<float*>(k.out)[at + c] = v;
                         else static_cast<__nv_bfloat16*>(k.out)[at + c] = __float2bfloat16_rn(v);
                     }
-                    if (k.dots && lane < 2) k.dots[(((size_t)lane * a.B + b) * a.T + t) * a.H + h] = v;
+                    if (dots && lane < 2) k.dots[(((size_t)lane * a.B + b) * a.T + t) * a.H + h] = v;
                 }
             };
             if (t_lo + chunks * kTc < t_hi) fill(t_lo + chunks * kTc, t_hi, 0.f);

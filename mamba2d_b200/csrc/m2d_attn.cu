@@ -526,13 +526,14 @@ static bool attn_map(CUtensorMap* map, const m2d_attn_desc* d, const AttnTensor&
 }
 
 // A launch of `count` cores from `first` on, all with the same head sizes.
-template <int KD, int VD, bool STATE_ONLY>
+template <int KD, int VD, TcMode MODE>
 static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int count, cudaStream_t st) {
     TcLaunch L;
     TcMaps maps;
     L.a = p.a;
     L.cores = count;
     L.fine = 0;
+    constexpr bool STATE_ONLY = MODE == kTcStateOnly;
     for (int i = 0; i < count; ++i) {
         const AttnCore& c = L.a.core[i] = p.a.core[first + i];
         if (c.dots) L.fine |= 1 << i;
@@ -542,18 +543,18 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
     if (STATE_ONLY) L.fine = 0;
     const bool fine = L.fine != 0;
     L.host_flag = wait_failure_flag();
-    L.small = (uint32_t)tc_plan_tiles(KD, VD, fine, STATE_ONLY, L.n);
+    L.small = (uint32_t)tc_plan_tiles(KD, VD, fine, STATE_ONLY, L.n, &L.own_stage);
     const size_t smem = L.small + sizeof(TcSmall);
-    auto kern = attn_tc_kernel<KD, VD, STATE_ONLY>;
+    auto kern = attn_tc_kernel<KD, VD, MODE>;
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     kern<<<(unsigned)(d->B * d->H * p.a.nseg * count), kTcThreads, smem, st>>>(maps, L);
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
 }
-template <bool STATE_ONLY>
+template <TcMode MODE>
 static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int count, cudaStream_t st) {
     const bool k64 = p.a.core[first].Kd <= 64, v64 = p.a.core[first].Vd <= 64;
-    if (k64) return v64 ? launch_tc<64, 64, STATE_ONLY>(d, p, first, count, st) : launch_tc<64, 128, STATE_ONLY>(d, p, first, count, st);
-    return v64 ? launch_tc<128, 64, STATE_ONLY>(d, p, first, count, st) : launch_tc<128, 128, STATE_ONLY>(d, p, first, count, st);
+    if (k64) return v64 ? launch_tc<64, 64, MODE>(d, p, first, count, st) : launch_tc<64, 128, MODE>(d, p, first, count, st);
+    return v64 ? launch_tc<128, 64, MODE>(d, p, first, count, st) : launch_tc<128, 128, MODE>(d, p, first, count, st);
 }
 
 static void launch_join(const AttnPlan& p, cudaStream_t st) {
@@ -583,7 +584,10 @@ static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t s
             for (int i = 0; i < 2; ++i) {
                 if (!counts[i]) continue;
                 const int first = i ? counts[0] : 0;
-                const int rc = pass ? launch_tc<false>(d, p, first, counts[i], st) : launch_tc<true>(d, p, first, counts[i], st);
+                bool plain = true;
+                for (int j = first; j < first + counts[i]; ++j) plain = plain && !p.a.core[j].out_f32 && !p.a.core[j].dots;
+                const int rc = !pass ? launch_tc<kTcStateOnly>(d, p, first, counts[i], st)
+                               : plain ? launch_tc<kTcPlain>(d, p, first, counts[i], st) : launch_tc<kTcFull>(d, p, first, counts[i], st);
                 if (rc != M2D_OK) return rc;
             }
             if (!pass) launch_join(p, st);
