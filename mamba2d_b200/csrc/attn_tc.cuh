@@ -43,10 +43,6 @@ struct TcMaps { CUtensorMap m[3][4]; };       // [core][x, y, z, out]
 struct TcLaunch {
     AttnLaunch a;
     int cores;
-    int n[3];                                 // tiles of x, y, z
-    int own_stage;                            // out has a tile of its own, else it goes through x's
-    uint32_t small;                           // where TcSmall lies in shared memory
-    int fine;                                 // bit per core
     int* host_flag;
 };
 
@@ -142,31 +138,44 @@ struct alignas(16) TcSmall {
     int abort;
 };
 
-// Shared memory: St in bf16 (one or two parts), the second part of u y, tiles.  (KD = 64: (4) computes 128 rows; the upper 64, of
-// whatever lies behind y, are not used, and a tile lies there.)
-inline size_t tc_fixed_smem(int KD, int VD, bool fine, bool state_only) { return (state_only ? 0 : (size_t)KD * VD * 2 * (fine ? 2 : 1)) + (size_t)kTc * KD * 2; }
-// Tiles of x, y, z: x first, whose tile is held longest, z last, which is needed last.
-inline size_t tc_plan_tiles(int KD, int VD, bool fine, bool state_only, int (&n)[3], int* own_stage) {
-    const size_t tile[3] = {(size_t)kTc * KD * 2, (size_t)kTc * KD * 2, (size_t)kTc * VD * 2};
-    n[0] = state_only ? 0 : 1; n[1] = n[2] = 1;
-    size_t bytes = tc_fixed_smem(KD, VD, fine, state_only) + n[0] * tile[0] + tile[1] + tile[2];
-    *own_stage = 0;
-    for (int round = 1; round < kTcTiles; ++round) {
-        if (round == 2 && !state_only && (KD < VD || bytes + tile[2] + sizeof(TcSmall) <= kMaxSmem)) {
-            *own_stage = 1;
-            bytes += tile[2];
-        }
-        for (int i = state_only ? 1 : 0; i < 3; ++i)
-            if (n[i] == round && bytes + tile[i] + sizeof(TcSmall) <= kMaxSmem) {
-                ++n[i];
-                bytes += tile[i];
-            }
-    }
-    return bytes;
-}
+// What a launch is for.  kTcPlain: bf16 out and nothing else, the least code (20 warps in five roles miss the instruction caches
+// often: with the branches of the others it takes 104 us where it takes 85).  kTcHeads: out in fp32, head by head.
+// kTcFine: dots and anchors, in two parts.
+enum TcMode { kTcPlain, kTcHeads, kTcFine, kTcStateOnly };
 
-// What a launch is for.  kTcPlain: bf16 out and nothing else, the least code (20 warps in five roles miss the instruction caches often).
-enum TcMode { kTcPlain, kTcFull, kTcStateOnly };
+// Shared memory: St in bf16 (one or two parts), the second part of u y, tiles, out's tile.  (KD = 64: (4) computes 128 rows; the upper
+// 64, of whatever lies behind y, are not used, and a tile lies there.)  Tiles of x, y, z: x first, whose tile is held longest, z
+// last, which is needed last; out's own tile before third ones.
+struct TcLayout {
+    int n[3] = {1, 1, 1};                     // tiles of x, y, z in flight
+    bool own_stage = false;                   // out has a tile of its own, else it goes through x's
+    uint32_t s_lo = 0, y_lo = 0, ring[3] = {}, stage = 0, small = 0;
+    __host__ __device__ constexpr TcLayout(int KD, int VD, TcMode mode) {
+        const bool state_only = mode == kTcStateOnly;
+        const uint32_t tile[3] = {(uint32_t)kTc * KD * 2, (uint32_t)kTc * KD * 2, (uint32_t)kTc * VD * 2};
+        if (state_only) n[0] = 0;
+        s_lo = state_only ? 0 : KD * VD * 2;
+        y_lo = state_only ? 0 : s_lo * (mode == kTcFine ? 2 : 1);
+        uint32_t bytes = y_lo + tile[0] + n[0] * tile[0] + tile[1] + tile[2];
+        const uint32_t most = (uint32_t)(kMaxSmem - sizeof(TcSmall));
+        for (int round = 1; round < kTcTiles; ++round) {
+            if (round == 2 && !state_only && (KD < VD || bytes + tile[2] <= most)) {
+                own_stage = true;
+                bytes += tile[2];
+            }
+            for (int i = state_only ? 1 : 0; i < 3; ++i)
+                if (n[i] == round && bytes + tile[i] <= most) {
+                    ++n[i];
+                    bytes += tile[i];
+                }
+        }
+        ring[0] = y_lo + tile[0];
+        ring[1] = ring[0] + n[0] * tile[0];
+        ring[2] = ring[1] + n[1] * tile[1];
+        stage = ring[2] + n[2] * tile[2];
+        small = bytes;
+    }
+};
 
 template <int KD, int VD, TcMode MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcLaunch L) {
@@ -175,6 +184,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     enum { kSc, kP = kSc + 2, kY, kO = kY + 2, kOFree = kO + 2, kDelta, kS = kDelta + 2, kMma2, kTabFull, kTabFree, kFull, kEmpty = kFull + 3 * kTcTiles, kBars = kEmpty + 3 * kTcTiles };
     static_assert(kBars <= 40, "room for the barriers");
     constexpr bool STATE_ONLY = MODE == kTcStateOnly;
+    constexpr TcLayout lay(KD, VD, MODE);
     constexpr int kHalf = VD / 2;                                 // columns of a thread
     constexpr uint32_t kTileX = kTc * KD * 2, kTileZ = kTc * VD * 2;
     constexpr uint32_t kO0 = 256;                                 // columns of tensor memory: pairs (2 x 128), O, delta
@@ -184,35 +194,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     const AttnLaunch& a = L.a;
     const int ci = blockIdx.x % L.cores, unit = blockIdx.x / L.cores;
     const AttnCore& k = a.core[ci];
-    const bool fine = MODE == kTcFull && (L.fine >> ci & 1), f32_out = MODE == kTcFull && k.out_f32, dots = MODE == kTcFull && k.dots;
+    const bool dots = MODE == kTcFine && k.dots, fine = dots, f32_out = (MODE == kTcHeads || MODE == kTcFine) && k.out_f32;
     const int seg = unit % a.nseg, bh = unit / a.nseg, h = bh % a.H, b = bh / a.H;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rev = k.rev;
     const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
     const int active = max(0, min(len, t_hi) - t_lo), chunks = (active + kTc - 1) / kTc;         // the others hold nothing
 
-    TcSmall& small = *reinterpret_cast<TcSmall*>(tc_smem_raw + L.small);
+    TcSmall& small = *reinterpret_cast<TcSmall*>(tc_smem_raw + lay.small);
     TcTable& tab = small.tab;
-    // (the launch's second parts take room whether this core has them or not)
-    const uint32_t s_hi = smem_u32(tc_smem_raw), s_lo = s_hi + KD * VD * 2, y_lo = STATE_ONLY ? s_hi : s_hi + KD * VD * 2 * (L.fine ? 2 : 1);
-    const uint32_t ring_x = y_lo + kTileX, ring_y = ring_x + L.n[0] * kTileX, ring_z = ring_y + L.n[1] * kTileX, stage_own = ring_z + L.n[2] * kTileZ;
+    const uint32_t smem0 = smem_u32(tc_smem_raw), s_hi = smem0, s_lo = smem0 + lay.s_lo, y_lo = smem0 + lay.y_lo;
     const uint32_t bar0 = smem_u32(small.bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
     enum { X, Y, Z };
-    auto tile_at = [&](int which, int it) { return which == X ? ring_x + (uint32_t)(it % L.n[X]) * kTileX : which == Y ? ring_y + (uint32_t)(it % L.n[Y]) * kTileX : ring_z + (uint32_t)(it % L.n[Z]) * kTileZ; };
-    auto full = [&](int which, int it) { return bar(kFull + which * kTcTiles + it % L.n[which]); };
-    auto empty = [&](int which, int it) { return bar(kEmpty + which * kTcTiles + it % L.n[which]); };
-    auto turn = [&](int which, int it) { return (uint32_t)(it / L.n[which]) & 1u; };
+    // (`which` is a constant wherever these are inlined; X has no tiles in a pass over states only)
+    auto tiles_of = [&](int which) { return which == X ? (lay.n[X] ? lay.n[X] : 1) : which == Y ? lay.n[Y] : lay.n[Z]; };
+    auto tile_at = [&](int which, int it) { return smem0 + lay.ring[which] + (uint32_t)(it % tiles_of(which)) * (which == Z ? kTileZ : kTileX); };
+    auto full = [&](int which, int it) { return bar(kFull + which * kTcTiles + it % tiles_of(which)); };
+    auto empty = [&](int which, int it) { return bar(kEmpty + which * kTcTiles + it % tiles_of(which)); };
+    auto turn = [&](int which, int it) { return (uint32_t)(it / tiles_of(which)) & 1u; };
     auto chunk_at = [&](int it) { return t_lo + (rev ? chunks - 1 - it : it) * kTc; };
     volatile int* const abort = &small.abort;
-    auto wait = [&](uint32_t bar_, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar_, parity, abort)) != 0; };      // whole warps
+    auto wait = [&](uint32_t bar_, uint32_t parity) {            // whole warps
+        if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar_, parity)), 1)) return true;
+        return __all_sync(0xffffffffu, mbar_wait(bar_, parity, abort)) != 0;
+    };
     auto wait2 = [&](int bar_, int it) { return wait(bar(bar_ + (it & 1)), it >> 1 & 1); };                                          // of a pair
-    auto loaded = [&](int which, int it) { return mbar_wait(full(which, it), turn(which, it), abort); };
+    auto loaded = [&](int which, int it) { return wait(full(which, it), turn(which, it)); };
 
     if (tid == 0) {
         for (int i = 0; i < kFull; ++i) mbar_init(bar(i), i == kP || i == kY || i == kY + 1 || i == kOFree || i == kS ? 8 : i == kTabFree ? (STATE_ONLY ? 8 : 16) : 1);
         for (int i = kFull; i < kEmpty; ++i) mbar_init(bar(i), 1);
         // who gives a tile back: its two products, (1) and (4) counted as one; x's where out goes through it, whoever stores that
-        for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || (i / kTcTiles == X && !L.own_stage) ? 1 : 2);
+        for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || (i / kTcTiles == X && !lay.own_stage) ? 1 : 2);
         small.abort = (smem_u32(tc_smem_raw) & 1023u) != 0;      // (swizzled tiles have to be aligned; nothing runs if they are not)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -308,7 +321,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 // O -> out
                 const bool row = t0 + r < t_hi, live = r < valid;
                 const __nv_bfloat16* const er = dots && live ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st + half * kHalf : nullptr;
-                const uint32_t stage = L.own_stage ? stage_own : tile_at(X, it);
+                const uint32_t stage = lay.own_stage ? smem0 + lay.stage : tile_at(X, it);
                 float sum = 0.f;
                 if (!wait2(kO, it)) break;
                 tc_fence_after();
@@ -392,7 +405,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         };
         // St before (rev) or after the chunk at t0, if that ends a run; also of the chunks that hold nothing
         auto keep = [&](int from, int to) {
-            for (int t0 = from; MODE == kTcFull && k.anchors && t0 < to; t0 += kTc)
+            for (int t0 = from; MODE == kTcFine && k.anchors && t0 < to; t0 += kTc)
                 if ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, k.Vd, 1);
         };
         const int behind = t_lo + chunks * kTc;
@@ -405,7 +418,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             if (lane == 0) mbar_arrive(bar(kTabFree));
             const uint32_t y = tile_at(Y, it);
             // y is free to change once (1) has read it
-            if (!__all_sync(0xffffffffu, loaded(Y, it)) || (!STATE_ONLY && !wait2(kSc, it))) break;
+            if (!loaded(Y, it) || (!STATE_ONLY && !wait2(kSc, it))) break;
 #pragma unroll 2
             for (int i = 0; i < KD / 16; ++i) {
                 const int c = half * (KD / 16) + i;
@@ -424,7 +437,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 sts(piece(y_lo, kTc, r, c), lo[0], lo[1], lo[2], lo[3]);
             }
             if (__builtin_expect(valid < kTc, 0)) {               // z's rows there meet zeros in P and in u y
-                if (!__all_sync(0xffffffffu, loaded(Z, it))) break;
+                if (!loaded(Z, it)) break;
                 if (r >= valid) {
 #pragma unroll 1
                     for (int c = 0; c < VD / 16; ++c) sts(piece(tile_at(Z, it), kTc, r, half * (VD / 16) + c), 0, 0, 0, 0);
@@ -484,18 +497,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             int armed[3] = {0, 0, 0};
             for (int it = 0; it < chunks && !*abort; ++it) {
                 const int t0 = chunk_at(it);
-                for (int i = STATE_ONLY ? 1 : 0; i < 3; ++i) {
-                    const int which = STATE_ONLY ? i : i == 0 ? Y : i == 1 ? X : Z;      // y's tile comes free first
-                    if (!mbar_wait(empty(which, it), turn(which, it) ^ 1u, abort)) break;
-                    const int blocks = (which == Z ? VD : KD) / 64, head = h / (which == X ? k.x.per : which == Y ? k.y.per : k.z.per);
+                auto load = [&](int which, int per) {
+                    if (!mbar_wait(empty(which, it), turn(which, it) ^ 1u, abort)) return;
+                    const int blocks = (which == Z ? VD : KD) / 64;
                     mbar_expect_tx(full(which, it), (uint32_t)blocks * kTcBlock);
-                    for (int j = 0; j < blocks; ++j) tma_load_4d(tile_at(which, it) + j * kTcBlock, &maps.m[ci][which], 64 * j, head, t0, b, full(which, it));
+                    for (int j = 0; j < blocks; ++j) tma_load_4d(tile_at(which, it) + j * kTcBlock, &maps.m[ci][which], 64 * j, h / per, t0, b, full(which, it));
                     armed[which] = it + 1;
-                }
+                };
+                load(Y, k.y.per);                                 // (its tile comes free first)
+                if (!STATE_ONLY) load(X, k.x.per);
+                load(Z, k.z.per);
             }
             if (*abort)                                           // let the copies land (bounded)
                 for (int which = STATE_ONLY ? Y : X; which <= Z; ++which)
-                    for (int it = max(0, armed[which] - L.n[which]); it < armed[which]; ++it)
+                    for (int it = max(0, armed[which] - tiles_of(which)); it < armed[which]; ++it)
                         for (int n = 0; n < kTcWaitLimit && !mbar_try_wait(full(which, it), turn(which, it)); ++n) {}
         }
     } else if (warp == 17) {
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 umma_chain<i1, false, KD / 16>(on, tm + 128 * (n & 1), [&](int k) { return x + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4); },
                                                [&](int k) { return y + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4); });
                 commit_if(on, bar(kSc + (n & 1)));
-                if (L.own_stage) commit_if(on, empty(X, n));
+                if (lay.own_stage) commit_if(on, empty(X, n));
             }
         }
     } else if (warp == 18) {
@@ -536,11 +551,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             auto store = [&](int n) {
                 if (on) {
                     if (!f32_out) {
-                        for (int j = 0; 64 * j < k.Vd; ++j) tma_store_4d(&maps.m[ci][3], (L.own_stage ? stage_own : tile_at(X, n)) + j * kTcBlock, 64 * j, h, chunk_at(n), b);
+                        for (int j = 0; 64 * j < k.Vd; ++j) tma_store_4d(&maps.m[ci][3], (lay.own_stage ? smem0 + lay.stage : tile_at(X, n)) + j * kTcBlock, 64 * j, h, chunk_at(n), b);
                         bulk_commit();
                         bulk_wait_read();
                     }
-                    if (!L.own_stage) mbar_arrive(empty(X, n));
+                    if (!lay.own_stage) mbar_arrive(empty(X, n));
                 }
                 __syncwarp();
             };
@@ -558,7 +573,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 umma_chain<i2, false, KD / 16>(on, tm + kO0, xk, [&](int k) { return sh + k * 128; });
                 if (fine) umma_chain<i2, true, KD / 16>(on, tm + kO0, xk, [&](int k) { return sl + k * 128; });
                 commit_if(on, bar(kMma2));
-                if (L.own_stage) commit_if(on, empty(X, it));
+                if (lay.own_stage) commit_if(on, empty(X, it));
                 if (!wait(full(Z, it), turn(Z, it)) || !wait(bar(kP), ph)) break;
                 if (len - chunk_at(it) < kTc && !wait2(kY, it)) break;          // z's last rows have been cleared
                 tc_fence_after();

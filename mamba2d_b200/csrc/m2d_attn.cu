@@ -532,19 +532,15 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
     TcMaps maps;
     L.a = p.a;
     L.cores = count;
-    L.fine = 0;
-    constexpr bool STATE_ONLY = MODE == kTcStateOnly;
+    L.host_flag = wait_failure_flag();
     for (int i = 0; i < count; ++i) {
         const AttnCore& c = L.a.core[i] = p.a.core[first + i];
-        if (c.dots) L.fine |= 1 << i;
-        if (!(STATE_ONLY || attn_map(&maps.m[i][0], d, c.x, c.Kd)) || !attn_map(&maps.m[i][1], d, c.y, c.Kd) || !attn_map(&maps.m[i][2], d, c.z, c.Vd)) return M2D_ERR_LAUNCH;
-        if (!STATE_ONLY && !c.out_f32 && !attn_map(&maps.m[i][3], d, {c.out, c.ob, c.ot, c.oh, 1, 1}, c.Vd)) return M2D_ERR_LAUNCH;
+        if (!(MODE == kTcStateOnly || attn_map(&maps.m[i][0], d, c.x, c.Kd)) || !attn_map(&maps.m[i][1], d, c.y, c.Kd) || !attn_map(&maps.m[i][2], d, c.z, c.Vd)) return M2D_ERR_LAUNCH;
+        if (MODE != kTcStateOnly && !c.out_f32 && !attn_map(&maps.m[i][3], d, {c.out, c.ob, c.ot, c.oh, 1, 1}, c.Vd)) return M2D_ERR_LAUNCH;
     }
-    if (STATE_ONLY) L.fine = 0;
-    const bool fine = L.fine != 0;
-    L.host_flag = wait_failure_flag();
-    L.small = (uint32_t)tc_plan_tiles(KD, VD, fine, STATE_ONLY, L.n, &L.own_stage);
-    const size_t smem = L.small + sizeof(TcSmall);
+    constexpr TcLayout lay(KD, VD, MODE);
+    constexpr size_t smem = lay.small + sizeof(TcSmall);
+    static_assert(smem <= kMaxSmem, "shared memory of a CTA");
     auto kern = attn_tc_kernel<KD, VD, MODE>;
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     kern<<<(unsigned)(d->B * d->H * p.a.nseg * count), kTcThreads, smem, st>>>(maps, L);
@@ -584,10 +580,10 @@ static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t s
             for (int i = 0; i < 2; ++i) {
                 if (!counts[i]) continue;
                 const int first = i ? counts[0] : 0;
-                bool plain = true;
-                for (int j = first; j < first + counts[i]; ++j) plain = plain && !p.a.core[j].out_f32 && !p.a.core[j].dots;
+                const AttnCore& c = p.a.core[first];                // (dv, which wants least, is never the first of several)
                 const int rc = !pass ? launch_tc<kTcStateOnly>(d, p, first, counts[i], st)
-                               : plain ? launch_tc<kTcPlain>(d, p, first, counts[i], st) : launch_tc<kTcFull>(d, p, first, counts[i], st);
+                               : c.dots ? launch_tc<kTcFine>(d, p, first, counts[i], st)
+                               : c.out_f32 ? launch_tc<kTcHeads>(d, p, first, counts[i], st) : launch_tc<kTcPlain>(d, p, first, counts[i], st);
                 if (rc != M2D_OK) return rc;
             }
             if (!pass) launch_join(p, st);
