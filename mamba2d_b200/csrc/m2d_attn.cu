@@ -447,16 +447,17 @@ static AttnState dense_state(const m2d_attn_desc* d, const float* p, bool transp
     return {const_cast<float*>(p), n * d->H, n, 0, transposed ? 1 : d->V, transposed ? d->V : 1};
 }
 
-// Segments: as many as fill the GPU, none shorter than a run of kAnchor tokens.  A second pass over y and z and a
-// launch more: taken where it at least halves the time of the first.
-static void plan_segments(const m2d_attn_desc* d, long long ctas, int per_sm, AttnLaunch* a) {
+// Segments: as many as fill the GPU, of `least` chunks of `chunk` tokens at least.  A second pass over y and z and two launches
+// more: taken where it at least halves the time of the first.
+static void plan_segments(const m2d_attn_desc* d, long long ctas, int per_sm, int chunk, int least, AttnLaunch* a) {
     a->runs = (d->T + kAnchor - 1) / kAnchor;
-    const long long want = ctas > 0 ? (long long)sm_count() * per_sm / ctas : 1;
+    const long long chunks = (d->T + chunk - 1) / chunk, want = std::min<long long>((long long)sm_count() * per_sm / ctas, chunks / least);
     a->nseg = 1;
-    if (want >= 2 && a->runs >= 2) a->nseg = (int)std::min<long long>(want, a->runs);
-    const int per = (a->runs + a->nseg - 1) / a->nseg;
-    a->seg_len = per * kAnchor;
-    a->nseg = (a->runs + per - 1) / per;
+    a->seg_len = (int)(chunks * chunk);
+    if (want < 2) return;
+    const long long per = (chunks + want - 1) / want;
+    a->seg_len = (int)(per * chunk);
+    a->nseg = (int)((chunks + per - 1) / per);
 }
 
 struct AttnPlan {
@@ -480,7 +481,7 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
         p.dot_blocks = (d->K + p.VT - 1) / p.VT;
         per_sm = std::max<int>(1, (int)((kMaxSmem + 1024) / (p.smem + 1024)));
     }
-    plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, &p.a);
+    plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, tc ? 128 : 64, tc ? 4 : 1, &p.a);
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;

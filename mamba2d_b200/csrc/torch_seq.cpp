@@ -1,9 +1,13 @@
 // Eager entry points of the sequence operators (sequence.py): linear attention, group normalisation, clipping.
 //
-// Their arguments have been checked and cast by sequence.py; what is checked here is what the kernels rely on.
+// Arguments are checked here (in Python the checks took longer than a small call's kernel).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
 
 #include "m2d_seq.h"
 
@@ -132,26 +136,50 @@ public:
     }
 };
 
-void check_devices(const Tensor& like, std::initializer_list<const Tensor*> others) {
-    for (const Tensor* t : others) TORCH_CHECK(!t->defined() || t->device() == like.device(), "linear attention: tensors on ", t->device(), " and ", like.device());
-}
-void check_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state, int64_t tokens_dims) {
-    TORCH_CHECK(v.is_cuda() && (v.scalar_type() == at::kFloat || v.scalar_type() == at::kBFloat16) && q.scalar_type() == v.scalar_type() && k.scalar_type() == v.scalar_type(),
-                "linear attention: q, k, v must be CUDA tensors of one type, float32 or bfloat16");
-    TORCH_CHECK(g.scalar_type() == at::kFloat && (!state.defined() || state.scalar_type() == at::kFloat), "linear attention: decays and states are float32");
-    TORCH_CHECK(v.dim() == tokens_dims + 2 && q.dim() == v.dim() && k.dim() == v.dim(), "linear attention: q, k, v have ", tokens_dims + 2, " dimensions");
-    for (const Tensor* t : {&q, &k, &v}) TORCH_CHECK(t->numel() > 0 && t->size(0) <= INT_MAX && t->size(1) <= INT_MAX, "linear attention: a size out of range");
+// What q, k, v, log_decay and a state have to be: (tokens..., heads, dim) with one or two dimensions of tokens.
+void check_attn(const char* what, const char* tokens, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state) {
+    const int64_t lead = tokens[1] ? 2 : 1;
+    TORCH_CHECK(v.dim() == lead + 2, what, ": v must be (", tokens[0], lead > 1 ? ", T" : "", ", H, V), got ", v.sizes());
+    TORCH_CHECK(q.dim() == v.dim() && k.sizes() == q.sizes() && q.sizes().slice(0, lead) == v.sizes().slice(0, lead), what, ": q and k must be (", tokens[0], lead > 1 ? ", T" : "",
+                ", G, K) next to v ", v.sizes(), ", got ", q.sizes(), " and ", k.sizes());
+    const int64_t H = v.size(lead), V = v.size(lead + 1), G = q.size(lead), K = q.size(lead + 1);
+    TORCH_CHECK(H >= 1 && G >= 1 && H % G == 0, what, ": ", G, " heads of q and k cannot be shared by ", H, " heads of v");
+    TORCH_CHECK(K >= 1 && K <= M2D_ATTN_MAX_DIM && V >= 1 && V <= M2D_ATTN_MAX_DIM, what, ": head sizes of 1 to ", M2D_ATTN_MAX_DIM, ", got K=", K, ", V=", V);
+    TORCH_CHECK((g.dim() == 1 || g.dim() == lead + 1) && g.size(-1) == H && (g.dim() == 1 || g.sizes().slice(0, lead) == v.sizes().slice(0, lead)), what,
+                ": log_decay must be one per head, or one per token and head of v ", v.sizes(), ", got ", g.sizes());
+    TORCH_CHECK(g.is_floating_point(), what, ": log_decay has dtype ", g.scalar_type());
+    if (state.defined())
+        TORCH_CHECK(state.dim() == 4 && state.size(0) == v.size(0) && state.size(1) == H && state.size(2) == K && state.size(3) == V && state.scalar_type() == at::kFloat, what,
+                    ": the state must be (B, H, K, V) = (", v.size(0), ", ", H, ", ", K, ", ", V, ") in float32, got ", state.sizes(), " ", state.scalar_type());
+    for (const Tensor* t : {&q, &k, &v})
+        TORCH_CHECK((t->scalar_type() == at::kFloat || t->scalar_type() == at::kBFloat16) && t->scalar_type() == v.scalar_type(), what, ": dtype ", t->scalar_type(),
+                    "; q, k and v share one, float32 or bfloat16");
+    TORCH_CHECK(v.is_cuda(), what, ": tensors must be on a CUDA device (there is no CPU path)");
+    for (const Tensor* t : {&q, &k, &g, &state}) TORCH_CHECK(!t->defined() || t->device() == v.device(), what, ": tensors on ", t->device(), " and ", v.device());
+    for (int64_t d = 0; d < lead; ++d) TORCH_CHECK(v.size(d) <= INT_MAX, what, ": a size out of range");
 }
 
-std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale, const optional<Tensor>& state_,
-                                                      const optional<Tensor>& lengths_, bool want_state, int64_t flags) {
-    const Tensor state = or_none(state_), lengths = or_none(lengths_);
-    check_attn(q, k, v, g, state, 2);
-    check_devices(v, {&q, &k, &g, &state, &lengths});
-    TORCH_CHECK(!lengths.defined() || lengths.scalar_type() == at::kInt, "linear attention: lengths are int32");
+std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const optional<double>& scale_,
+                                                      const optional<Tensor>& state_, const optional<Tensor>& lengths_, bool want_state, int64_t flags) {
+    const char* const what = "linear_attention";
+    const Tensor state = or_none(state_);
+    Tensor lengths = or_none(lengths_);
+    check_attn(what, "BT", q, k, v, log_decay, state);
+    if (lengths.defined()) {
+        TORCH_CHECK(lengths.dim() == 1 && lengths.size(0) == v.size(0) && (lengths.scalar_type() == at::kInt || lengths.scalar_type() == at::kLong), what,
+                    ": lengths must be (B) integers, got ", lengths.sizes(), " ", lengths.scalar_type());
+        TORCH_CHECK(lengths.device() == v.device(), what, ": lengths are on ", lengths.device(), ", expected ", v.device());
+        if (lengths.scalar_type() == at::kLong) lengths = lengths.clamp(0, v.size(1)).to(at::kInt);
+    }
+    if (v.size(0) == 0 || v.size(1) == 0) {
+        if (!want_state) return {v.clone(), c10::nullopt};
+        return {v.clone(), state.defined() ? state.clone() : at::zeros({v.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat))};
+    }
     check_waits();
+    const Tensor g = log_decay.to(at::kFloat);
+    const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)q.size(-1));
     if (wants_grad({&q, &k, &v, &g, &state})) {
-        const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths_, scale, want_state, flags);
+        const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths.defined() ? optional<Tensor>(lengths) : c10::nullopt, scale, want_state, flags);
         return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
     }
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -162,19 +190,25 @@ std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Ten
     return {o, want_state ? optional<Tensor>(out_state) : c10::nullopt};
 }
 
-Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale, const Tensor& state) {
-    check_attn(q, k, v, g, state, 1);
-    check_devices(v, {&q, &k, &g, &state});
-    TORCH_CHECK(!wants_grad({&q, &k, &v, &g, &state}), "linear_attention_step updates the state in place and has no gradients: call it without gradients");
+Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, const optional<double>& scale) {
+    const char* const what = "linear_attention_step";
+    TORCH_CHECK(state.defined(), what, ": there is no state");
+    check_attn(what, "B", q, k, v, log_decay, state);
+    const int64_t B = v.size(0), H = v.size(1), K = q.size(2), V = v.size(2), span = K * V, sb = state.stride(0), sh = state.stride(1);
+    const bool dense_kv = (V == 1 || state.stride(3) == 1) && (K == 1 || state.stride(2) == V);
+    const bool apart = (B == 1 || sb >= span) && (H == 1 || sh >= span) && (B == 1 || H == 1 || sb >= (H - 1) * sh + span || sh >= (B - 1) * sb + span);
+    TORCH_CHECK(B == 0 || (dense_kv && apart), what, ": the state must be dense in (K, V) and must not overlap itself, got strides ", state.strides());
+    TORCH_CHECK(!wants_grad({&q, &k, &v, &log_decay, &state}), what, " updates the state in place and has no gradients: call it without gradients");
+    if (B == 0) return v.clone();
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
-    const Tensor qr = rows(q), kr = rows(k), vr = rows(v);
+    const Tensor qr = rows(q), kr = rows(k), vr = rows(v), g = log_decay.to(at::kFloat);
     m2d_attn_desc d{};
     d.struct_bytes = sizeof(d);
     d.dtype = dtype_of(v);
-    d.B = (int)v.size(0); d.T = 1; d.H = (int)v.size(1); d.V = (int)v.size(2);
-    d.G = (int)q.size(1); d.K = (int)q.size(2);
-    d.scale = (float)scale;
+    d.B = (int)B; d.T = 1; d.H = (int)H; d.V = (int)V;
+    d.G = (int)q.size(1); d.K = (int)K;
+    d.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)K));
     auto token = [](const Tensor& t) { return m2d_attn_tensor{t.data_ptr(), t.stride(0), 0, t.stride(1)}; };
     d.q = token(qr); d.k = token(kr); d.v = token(vr);
     d.log_decay = fptr(g);
@@ -183,7 +217,7 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
     d.state = d.state_out = fptr(state);
     const Tensor o = at::empty({d.B, d.H, d.V}, v.options());
     d.o = o.data_ptr();
-    check(m2d_attn_step(&d, state.stride(0), state.stride(1), stream_of(v)), "m2d_attn_step");
+    check(m2d_attn_step(&d, sb, sh, stream_of(v)), "m2d_attn_step");
     wrote(state);
     return o;
 }
@@ -261,15 +295,23 @@ public:
     }
 };
 
-Tensor group_norm(const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, int64_t groups, int64_t act, double eps) {
+Tensor group_norm(const Tensor& x_, int64_t groups, const optional<Tensor>& weight_, const optional<Tensor>& bias_, double eps, int64_t act) {
     const Tensor weight = or_none(weight_), bias = or_none(bias_);
-    TORCH_CHECK(x_.is_cuda() && (x_.scalar_type() == at::kFloat || x_.scalar_type() == at::kBFloat16), "group_norm: x must be a CUDA tensor, float32 or bfloat16");
-    TORCH_CHECK(x_.dim() >= 2 && x_.numel() > 0 && x_.size(-1) <= INT_MAX, "group_norm: x is (N, ..., C)");
+    TORCH_CHECK(x_.dim() >= 2, "group_norm: x must be (N, ..., C), got ", x_.sizes());
+    const int64_t C = x_.size(-1);
+    TORCH_CHECK_VALUE(groups >= 1 && C % groups == 0, "group_norm: ", C, " channels do not make ", groups, " groups");
+    TORCH_CHECK_VALUE(eps >= 0, "group_norm: eps must not be negative, got ", eps);
+    TORCH_CHECK(x_.scalar_type() == at::kFloat || x_.scalar_type() == at::kBFloat16, "group_norm: unsupported dtype ", x_.scalar_type(), " (float32 and bfloat16 only)");
+    TORCH_CHECK(x_.is_cuda(), "group_norm: tensors must be on a CUDA device (there is no CPU path)");
+    TORCH_CHECK(C <= INT_MAX, "group_norm: a size out of range");
     for (const Tensor* p : {&weight, &bias})
-        if (p->defined())
-            TORCH_CHECK(p->device() == x_.device() && p->sizes() == at::IntArrayRef({x_.size(-1)}) && (p->scalar_type() == at::kFloat || p->scalar_type() == x_.scalar_type()) &&
-                            (!weight.defined() || p->scalar_type() == weight.scalar_type()),
-                        "group_norm: weight and bias are (C), on x's device, of one type, float32 or x's");
+        if (p->defined()) {
+            TORCH_CHECK(p->dim() == 1 && p->size(0) == C, "group_norm: weight and bias must have shape (", C, "), got ", p->sizes());
+            TORCH_CHECK((p->scalar_type() == at::kFloat || p->scalar_type() == x_.scalar_type()) && (!weight.defined() || p->scalar_type() == weight.scalar_type()),
+                        "group_norm: dtype ", p->scalar_type(), "; weight and bias share one, float32 or ", x_.scalar_type());
+            TORCH_CHECK(p->device() == x_.device(), "group_norm: tensors on ", p->device(), " and ", x_.device());
+        }
+    if (!x_.numel()) return x_.clone();
     if (wants_grad({&x_, &weight, &bias})) return NormFn::apply(x_, weight_, bias_, groups, act, eps);
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(x_.device());
@@ -319,11 +361,10 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm) {
 
 void bind_sequence_operators(pybind11::module& m) {
     using pybind11::arg;
-    m.def("linear_attention", &linear_attention, "linear attention of whole sequences: (o, state or None)", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale"),
+    m.def("linear_attention", &linear_attention, "linear attention of whole sequences: (o, state or None)", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale").none(true),
           arg("state").none(true), arg("lengths").none(true), arg("want_state"), arg("flags") = 0);
-    m.def("linear_attention_step", &linear_attention_step, "linear attention of one token; the state is updated in place", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale"),
-          arg("state"));
-    m.def("group_norm", &group_norm, "group normalisation with an activation, channels last", arg("x"), arg("weight").none(true), arg("bias").none(true), arg("groups"), arg("act"),
-          arg("eps"));
+    m.def("linear_attention_step", &linear_attention_step, "linear attention of one token; the state is updated in place", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("state"),
+          arg("scale").none(true));
+    m.def("group_norm", &group_norm, "group normalisation with an activation, channels last", arg("x"), arg("groups"), arg("weight").none(true), arg("bias").none(true), arg("eps"), arg("act"));
     m.def("clip_grad_norm", &clip_grad_norm, "global norm; the tensors are scaled in place", arg("grads"), arg("max_norm"));
 }

@@ -18,36 +18,7 @@ from . import _lib
 
 __all__ = ["linear_attention", "linear_attention_step", "group_norm", "clip_norm_", "clip_grad_norm_"]
 
-_TYPES = (torch.float32, torch.bfloat16)
 _ACTS = {None: 0, "silu": 1, "gelu": 2}
-
-
-def _check_attention(q, k, v, log_decay, state, tokens, what):
-    if v.dim() != len(tokens) + 2:
-        raise RuntimeError(f"{what}: v must be ({', '.join(tokens)}, H, V), got {tuple(v.shape)}")
-    lead, (H, V) = tuple(v.shape[:-2]), v.shape[-2:]
-    if q.dim() != v.dim() or tuple(q.shape[:-2]) != lead or k.shape != q.shape:
-        raise RuntimeError(f"{what}: q and k must be ({', '.join(tokens)}, G, K) next to v {tuple(v.shape)}, got {tuple(q.shape)} and {tuple(k.shape)}")
-    G, K = q.shape[-2:]
-    if H < 1 or G < 1 or H % G:
-        raise RuntimeError(f"{what}: {G} heads of q and k cannot be shared by {H} heads of v")
-    if not 1 <= K <= _lib.ATTN_MAX_DIM or not 1 <= V <= _lib.ATTN_MAX_DIM:
-        raise RuntimeError(f"{what}: head sizes of 1 to {_lib.ATTN_MAX_DIM}, got K={K}, V={V}")
-    if tuple(log_decay.shape) not in ((H,), lead + (H,)):
-        raise RuntimeError(f"{what}: log_decay must be {(H,)} or {lead + (H,)}, got {tuple(log_decay.shape)}")
-    if not log_decay.is_floating_point():
-        raise RuntimeError(f"{what}: log_decay has dtype {log_decay.dtype}")
-    if state is not None and (tuple(state.shape) != (lead[0], H, K, V) or state.dtype != torch.float32):
-        raise RuntimeError(f"{what}: the state must be {(lead[0], H, K, V)} in float32, got {tuple(state.shape)} {state.dtype}")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype not in _TYPES or t.dtype != v.dtype:
-            raise RuntimeError(f"{what}: {name} has dtype {t.dtype}; q, k and v share one, float32 or bfloat16")
-    if not v.is_cuda:
-        raise RuntimeError(f"{what}: tensors must be on a CUDA device (there is no CPU path)")
-    for name, t in (("q", q), ("k", k), ("log_decay", log_decay), ("state", state)):
-        if t is not None and t.device != v.device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, expected {v.device}")
-    return K
 
 
 def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
@@ -68,22 +39,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
     Differentiable in q, k, v, log_decay and initial_state, through o and the state.  A token that is not finite
     may spoil the outputs of up to 127 tokens before it, besides all later ones of its sequence and head.
     """
-    what = "linear_attention"
-    K = _check_attention(q, k, v, log_decay, initial_state, ("B", "T"), what)
-    B, T, H, V = v.shape
-    if lengths is not None:
-        if tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
-            raise RuntimeError(f"{what}: lengths must be {(B,)} integers, got {tuple(lengths.shape)} {lengths.dtype}")
-        if lengths.device != v.device:
-            raise RuntimeError(f"{what}: lengths are on {lengths.device}, expected {v.device}")
-        lengths = lengths.clamp(max=T).to(torch.int32) if lengths.dtype == torch.int64 else lengths
-    scale = K ** -0.5 if scale is None else float(scale)
-    if B == 0 or T == 0:
-        if not return_state:
-            return v.clone()
-        zero = initial_state if initial_state is not None else torch.zeros(B, H, K, V, device=v.device)
-        return v.clone(), zero.clone()
-    o, state = _lib.entry().linear_attention(q, k, v, log_decay.float(), scale, initial_state, lengths, return_state)
+    o, state = _lib.entry().linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
     return (o, state) if return_state else o
 
 
@@ -97,20 +53,9 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
             cache) but must not overlap.
     No gradients: it raises where one is wanted.
     """
-    what = "linear_attention_step"
     if state is None:
-        raise RuntimeError(f"{what}: there is no state")
-    K = _check_attention(q, k, v, log_decay, state, ("B",), what)
-    B, H, V = v.shape
-    if B == 0:
-        return v.clone()
-    sb, sh, sk, sv = state.stride()
-    span = K * V
-    dense = (V == 1 or sv == 1) and (K == 1 or sk == V)
-    apart = all(n == 1 or s >= span for n, s in ((B, sb), (H, sh))) and (B == 1 or H == 1 or sb >= (H - 1) * sh + span or sh >= (B - 1) * sb + span)
-    if not dense or not apart:
-        raise RuntimeError(f"{what}: the state must be dense in (K, V) and must not overlap itself, got strides {state.stride()}")
-    return _lib.entry().linear_attention_step(q, k, v, log_decay.float(), K ** -0.5 if scale is None else float(scale), state)
+        raise RuntimeError("linear_attention_step: there is no state")
+    return _lib.entry().linear_attention_step(q, k, v, log_decay, state, scale)
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None):
@@ -126,29 +71,9 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None):
     """
     if act not in _ACTS:
         raise ValueError(f"Unknown activation, got {act}...")
-    if x.dim() < 2:
-        raise RuntimeError(f"group_norm: x must be (N, ..., C), got {tuple(x.shape)}")
-    C = x.shape[-1]
-    if not isinstance(groups, int) or groups < 1 or C % groups:
-        raise ValueError(f"group_norm: {C} channels do not make {groups} groups")
-    if not eps >= 0:
-        raise ValueError(f"group_norm: eps must not be negative, got {eps}")
-    if x.dtype not in _TYPES:
-        raise RuntimeError(f"group_norm: unsupported dtype {x.dtype} (float32 and bfloat16 only)")
-    if not x.is_cuda:
-        raise RuntimeError("group_norm: tensors must be on a CUDA device (there is no CPU path)")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if tuple(p.shape) != (C,):
-            raise RuntimeError(f"group_norm: {name} must have shape {(C,)}, got {tuple(p.shape)}")
-        if p.dtype not in (torch.float32, x.dtype) or (weight is not None and p.dtype != weight.dtype):
-            raise RuntimeError(f"group_norm: {name} has dtype {p.dtype}; weight and bias share one, float32 or {x.dtype}")
-        if p.device != x.device:
-            raise RuntimeError(f"group_norm: {name} is on {p.device}, expected {x.device}")
-    if x.numel() == 0:
-        return x.clone()
-    return _lib.entry().group_norm(x, weight, bias, groups, _ACTS[act], float(eps))
+    if not isinstance(groups, int):
+        raise ValueError(f"group_norm: groups must be an integer, got {groups}")
+    return _lib.entry().group_norm(x, groups, weight, bias, eps, _ACTS[act])
 
 
 def clip_norm_(tensors, max_norm, error_if_nonfinite=False):
