@@ -43,8 +43,8 @@ struct AttnCore {
     float s_intra, s_inter, s_update;
     float* dots;              // [column block][B][T][H], or nullptr
     AttnState init, fin;      // p may be nullptr
-    float* anchors;           // [B][H][runs][Kd][Vd], or nullptr
-    float* seg_state;         // [B][H][segments][Kd][Vd]
+    float* anchors;           // [B][H][runs][Kd Vd], or nullptr; in the order that a kernel likes, the same for dq and dk
+    float* seg_state;         // [B][H][segments][Kd Vd]
     float* seg_decay;         // [B][H][segments], log2
 };
 struct AttnLaunch {
@@ -54,6 +54,7 @@ struct AttnLaunch {
     const int* lengths;
     int B, T, H;
     int nseg, seg_len, runs;
+    int seg_columns;          // segments' states have a column's rows next to one another, else a row's columns
 };
 
 __device__ __forceinline__ const void* attn_at(const AttnTensor& t, int b, int h, size_t elem) {

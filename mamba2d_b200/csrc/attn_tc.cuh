@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     constexpr uint32_t kCols = STATE_ONLY ? (VD <= 64 ? 64 : 128) : 512;
     constexpr uint32_t kDelta0 = STATE_ONLY ? 0 : kO0 + VD;
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // (a launch that needs nothing of this one may fill its last wave)
     const AttnLaunch& a = L.a;
     const int ci = blockIdx.x % L.cores, unit = blockIdx.x / L.cores;
     const AttnCore& k = a.core[ci];
@@ -323,9 +324,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 const __nv_bfloat16* const er = dots && live ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st + half * kHalf : nullptr;
                 const uint32_t stage = lay.own_stage ? smem0 + lay.stage : tile_at(X, it);
                 float sum = 0.f;
+                uint4 eg[kHalf / 8];                              // e's columns, on their way while (3) runs
+                if (MODE == kTcFine) {
+#pragma unroll
+                    for (int c = 0; c < kHalf; c += 8)
+                        if (er && half * kHalf + c < k.Vd) eg[c / 8] = __ldg(reinterpret_cast<const uint4*>(er + c));
+                }
                 if (!wait2(kO, it)) break;
                 tc_fence_after();
-#pragma unroll 1
+#pragma unroll(MODE == kTcFine ? 2 : 1)
                 for (int c0 = 0; c0 < kHalf; c0 += 32) {
                     float o[32];
                     const int col = half * kHalf + c0;
@@ -349,11 +356,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                                 p[c / 4 + 1] = make_float4(o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
                             }
                     }
-                    if (er) {
+                    if (MODE == kTcFine && er) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 8)
                             if (col + c < k.Vd) {
-                                const uint4 g = __ldg(reinterpret_cast<const uint4*>(er + c0 + c));
+                                const uint4 g = eg[(c0 + c) / 8];
                                 const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) sum = fmaf(o[c + 2 * i], __uint_as_float(gg[i] << 16), fmaf(o[c + 2 * i + 1], __uint_as_float(gg[i] & 0xffff0000u), sum));
@@ -380,7 +387,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             long long sr = k.init.sr, sc = k.init.sc;
             if (a.nseg > 1) {
                 init = k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd;
-                sr = k.Vd; sc = 1;
+                sr = 1; sc = k.Kd;
             } else if (k.init.p) {
                 init = k.init.p + b * k.init.sb + h * k.init.sh;
             }
@@ -391,6 +398,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     if (v0 + c < k.Vd) S[c] = init[c * sc];
             }
         }
+        // (states kept between kernels and runs have a column's rows next to one another: a warp's store is one line, not 32, which
+        // held the other warps' shared memory up for 7000 cycles every four chunks)
         auto put = [&](float* to, long long sr, long long sc) {
             to += r * sr + v0 * sc;
             if (have_row && sc == 1 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
@@ -406,7 +415,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         // St before (rev) or after the chunk at t0, if that ends a run; also of the chunks that hold nothing
         auto keep = [&](int from, int to) {
             for (int t0 = from; MODE == kTcFine && k.anchors && t0 < to; t0 += kTc)
-                if ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, k.Vd, 1);
+                if ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, 1, k.Kd);
         };
         const int behind = t_lo + chunks * kTc;
         for (int it = 0; it < chunks; ++it) {
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             if (!STATE_ONLY && !rev) keep(t0, it == chunks - 1 ? t_hi : t0 + kTc);
         }
         if constexpr (STATE_ONLY) {
-            put(k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd, k.Vd, 1);
+            put(k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd, 1, k.Kd);
         } else {
             if (!chunks) keep(behind, t_hi);
             if (k.fin.p && seg == (rev ? 0 : a.nseg - 1)) {
@@ -660,6 +669,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             if (*abort) fill(t_lo, min(t_hi, t_lo + chunks * kTc), __int_as_float(0x7fc00000));
         }
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");                   // (but does not end before it)
     if (tid == 0 && *abort && L.host_flag) *reinterpret_cast<volatile int*>(L.host_flag) = 1;
     tc_fence_before();
     __syncthreads();

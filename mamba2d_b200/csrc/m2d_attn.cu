@@ -280,7 +280,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     const int bh = blockIdx.x, h = bh % a.H, b = bh / a.H, n = k.Kd * k.Vd;
     const int i = blockIdx.y * 128 + threadIdx.x;
     if (i >= n) return;
-    float carry = k.init.p ? k.init.p[b * k.init.sb + h * k.init.sh + (i / k.Vd) * k.init.sr + (i % k.Vd) * k.init.sc] : 0.f;
+    const int row = a.seg_columns ? i % k.Kd : i / k.Vd, col = a.seg_columns ? i / k.Kd : i % k.Vd;
+    float carry = k.init.p ? k.init.p[b * k.init.sb + h * k.init.sh + row * k.init.sr + col * k.init.sc] : 0.f;
     for (int j0 = 0; j0 < a.nseg; j0 += 8) {
         float own[8], decay[8];
         auto at = [&](int j) { return (size_t)bh * a.nseg + (k.rev ? a.nseg - 1 - j : j); };
@@ -481,6 +482,7 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
         p.dot_blocks = (d->K + p.VT - 1) / p.VT;
         per_sm = std::max<int>(1, (int)((kMaxSmem + 1024) / (p.smem + 1024)));
     }
+    p.a.seg_columns = tc;
     plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, tc ? 128 : 64, tc ? 4 : 1, &p.a);
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
@@ -544,8 +546,18 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
     static_assert(smem <= kMaxSmem, "shared memory of a CTA");
     auto kern = attn_tc_kernel<KD, VD, MODE>;
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
-    kern<<<(unsigned)(d->B * d->H * p.a.nseg * count), kTcThreads, smem, st>>>(maps, L);
-    return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(d->B * d->H * p.a.nseg * count));
+    c.blockDim = dim3(kTcThreads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    // what follows another group of the same pass needs nothing of it
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr;
+    c.numAttrs = first > 0 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, kern, maps, L) == cudaSuccess ? M2D_OK : (cudaGetLastError(), M2D_ERR_LAUNCH);
 }
 template <TcMode MODE>
 static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int count, cudaStream_t st) {
@@ -574,8 +586,9 @@ static int launch_any(const AttnPlan& p, cudaStream_t st) {
 }
 static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t st) {
     if (p.tc) {
-        // dq and dk have (V,K) states, dv a (K,V) one: one launch where the kernel is the same
-        const bool together = p.cores == 1 || (d->K <= 64) == (d->V <= 64);
+        // dq and dk have (V,K) states, dv a (K,V) one: one launch where the kernel is the same; not where dv would run in the
+        // kernel of those with dots, which takes twice as long for a chunk
+        const bool together = p.cores == 1 || ((d->K <= 64) == (d->V <= 64) && !p.a.core[0].dots && !p.a.core[0].out_f32);
         const int counts[2] = {together ? p.cores : 2, together ? 0 : 1};
         for (int pass = p.a.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
             for (int i = 0; i < 2; ++i) {
