@@ -156,7 +156,7 @@ struct TcLayout {
         if (state_only) n[0] = 0;
         s_lo = state_only ? 0 : KD * VD * 2;
         y_lo = state_only ? 0 : s_lo * (mode == kTcFine ? 2 : 1);
-        uint32_t bytes = y_lo + tile[0] + n[0] * tile[0] + tile[1] + tile[2];
+        uint32_t bytes = y_lo + (state_only ? 2 : 1) * tile[0] + n[0] * tile[0] + tile[1] + tile[2];
         const uint32_t most = (uint32_t)(kMaxSmem - sizeof(TcSmall));
         for (int round = 1; round < kTcTiles; ++round) {
             if (round == 2 && !state_only && (KD < VD || bytes + tile[2] <= most)) {
@@ -169,7 +169,7 @@ struct TcLayout {
                     bytes += tile[i];
                 }
         }
-        ring[0] = y_lo + tile[0];
+        ring[0] = y_lo + (state_only ? 2 : 1) * tile[0];
         ring[1] = ring[0] + n[0] * tile[0];
         ring[2] = ring[1] + n[1] * tile[1];
         stage = ring[2] + n[2] * tile[2];
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     constexpr int kHalf = VD / 2;                                 // columns of a thread
     constexpr uint32_t kTileX = kTc * KD * 2, kTileZ = kTc * VD * 2;
     constexpr uint32_t kO0 = 256;                                 // columns of tensor memory: pairs (2 x 128), O, delta
-    constexpr uint32_t kCols = STATE_ONLY ? (VD <= 64 ? 64 : 128) : 512;
+    constexpr uint32_t kCols = STATE_ONLY ? 2 * VD : 512;           // (two places for delta where states are all that is wanted)
     constexpr uint32_t kDelta0 = STATE_ONLY ? 0 : kO0 + VD;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // (a launch that needs nothing of this one may fill its last wave)
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     auto loaded = [&](int which, int it) { return wait(full(which, it), turn(which, it)); };
 
     if (tid == 0) {
-        for (int i = 0; i < kFull; ++i) mbar_init(bar(i), i == kP || i == kY || i == kY + 1 || i == kOFree || i == kS ? 8 : i == kTabFree ? (STATE_ONLY ? 8 : 16) : 1);
+        for (int i = 0; i < kFull; ++i) mbar_init(bar(i), i == kP || i == kY || i == kY + 1 || i == kOFree || i == kS || (STATE_ONLY && (i == kO || i == kO + 1)) ? 8 : i == kTabFree ? 16 : 1);
         for (int i = kFull; i < kEmpty; ++i) mbar_init(bar(i), 1);
         // who gives a tile back: its two products, (1) and (4) counted as one; x's where out goes through it, whoever stores that
         for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || (i / kTcTiles == X && !lay.own_stage) ? 1 : 2);
@@ -240,8 +240,54 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     auto piece = [&](uint32_t base, int rows, int r, int c) { return base + (uint32_t)(c / 8) * rows * 128 + (uint32_t)r * 128 + (uint32_t)(((c ^ r) & 7) << 4); };
     auto sts = [&](uint32_t addr, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v0), "r"(v1), "r"(v2), "r"(v3) : "memory"); };
 
+    // y -> u y, half of row r a thread; false if a wait has given up
+    auto scale_y = [&](int it, int valid, int r, int half, float u) {
+        const uint32_t y = tile_at(Y, it);
+        // y is free to change once (1) has read it; its second part has two places where states are all that is wanted
+        if (!loaded(Y, it) || (!STATE_ONLY && !wait2(kSc, it)) || (STATE_ONLY && it > 1 && !wait2(kDelta, it - 2))) return false;
+#pragma unroll 2
+        for (int i = 0; i < KD / 16; ++i) {
+            const int c = half * (KD / 16) + i;
+            const uint32_t at = piece(y, kTc, r, c);
+            uint32_t g[4], hi[4], lo[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(at) : "memory");
+            if (__builtin_expect(valid < kTc, 0) && r >= valid) g[0] = g[1] = g[2] = g[3] = 0;      // (such a row may hold anything: no product with zero)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = __fmul2_rn(make_float2(__uint_as_float(g[i] << 16), __uint_as_float(g[i] & 0xffff0000u)), make_float2(u, u));
+                hi[i] = pack_bf16x2(v.x, v.y);
+                const float2 rest = __ffma2_rn(make_float2(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), make_float2(-1.f, -1.f), v);
+                lo[i] = pack_bf16x2(rest.x, rest.y);
+            }
+            sts(at, hi[0], hi[1], hi[2], hi[3]);
+            sts(piece(y_lo + (STATE_ONLY ? (it & 1) * kTileX : 0), kTc, r, c), lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (__builtin_expect(valid < kTc, 0)) {               // z's rows there meet zeros in P and in u y
+            if (!loaded(Z, it)) return false;
+            if (r >= valid) {
+#pragma unroll 1
+                for (int c = 0; c < VD / 16; ++c) sts(piece(tile_at(Z, it), kTc, r, half * (VD / 16) + c), 0, 0, 0, 0);
+            }
+        }
+        async_fence();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kY + (it & 1)));
+        return true;
+    };
+
     if (warp < 8) {
         // ---- token rows ----
+        if constexpr (STATE_ONLY) {                               // (they scale y, so that warps 8 - 15 only add what comes of it)
+            for (int it = 0; it < chunks; ++it) {
+                const int r = tid & 127, valid = min(kTc, len - chunk_at(it));
+                if (!wait(bar(kTabFull), it & 1)) break;
+                const float u = r < valid ? tab.u[r] : 0.f;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(kTabFree));
+                if (!scale_y(it, valid, r, warp >> 2, u)) break;
+            }
+        }
         if constexpr (!STATE_ONLY) {
             const int q = warp & 3, half = warp >> 2, r = tid & 127;
             const uint32_t mine = tmem + ((uint32_t)(q * 32) << 16), oc = mine + kO0 + half * kHalf;
@@ -408,8 +454,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     if (v0 + c < k.Vd) *reinterpret_cast<float4*>(to + c) = make_float4(S[c], S[c + 1], S[c + 2], S[c + 3]);
             } else if (have_row) {
 #pragma unroll
-                for (int c = 0; c < kHalf; ++c)
-                    if (v0 + c < k.Vd) to[c * sc] = S[c];
+                for (int c = 0; c < kHalf; ++c) {
+                    if (v0 + c < k.Vd) *to = S[c];
+                    to += sc;
+                }
             }
         };
         // St before (rev) or after the chunk at t0, if that ends a run; also of the chunks that hold nothing
@@ -422,40 +470,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             const int t0 = chunk_at(it), valid = min(kTc, len - t0);
             if (!STATE_ONLY && rev) keep(t0, it ? t0 + kTc : t_hi);
             if (!wait(bar(kTabFull), it & 1)) break;
-            const float u = r < valid ? tab.u[r] : 0.f, whole = tab.whole, copy = tab.copy;
+            const float u = !STATE_ONLY && r < valid ? tab.u[r] : 0.f, whole = tab.whole, copy = tab.copy;
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kTabFree));
-            const uint32_t y = tile_at(Y, it);
-            // y is free to change once (1) has read it
-            if (!loaded(Y, it) || (!STATE_ONLY && !wait2(kSc, it))) break;
-#pragma unroll 2
-            for (int i = 0; i < KD / 16; ++i) {
-                const int c = half * (KD / 16) + i;
-                const uint32_t at = piece(y, kTc, r, c);
-                uint32_t g[4], hi[4], lo[4];
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(g[0]), "=r"(g[1]), "=r"(g[2]), "=r"(g[3]) : "r"(at) : "memory");
-                if (__builtin_expect(valid < kTc, 0) && r >= valid) g[0] = g[1] = g[2] = g[3] = 0;      // (such a row may hold anything: no product with zero)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 v = __fmul2_rn(make_float2(__uint_as_float(g[i] << 16), __uint_as_float(g[i] & 0xffff0000u)), make_float2(u, u));
-                    hi[i] = pack_bf16x2(v.x, v.y);
-                    const float2 rest = __ffma2_rn(make_float2(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)), make_float2(-1.f, -1.f), v);
-                    lo[i] = pack_bf16x2(rest.x, rest.y);
-                }
-                sts(at, hi[0], hi[1], hi[2], hi[3]);
-                sts(piece(y_lo, kTc, r, c), lo[0], lo[1], lo[2], lo[3]);
+            if constexpr (!STATE_ONLY) {
+                if (!scale_y(it, valid, r, half, u)) break;
             }
-            if (__builtin_expect(valid < kTc, 0)) {               // z's rows there meet zeros in P and in u y
-                if (!loaded(Z, it)) break;
-                if (r >= valid) {
-#pragma unroll 1
-                    for (int c = 0; c < VD / 16; ++c) sts(piece(tile_at(Z, it), kTc, r, half * (VD / 16) + c), 0, 0, 0, 0);
-                }
-            }
-            async_fence();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kY + (it & 1)));
             if constexpr (!STATE_ONLY) {                          // the state's copy for (2)
                 if (it > 0 && !wait(bar(kMma2), (it & 1) ^ 1)) break;
                 if (r < KD) {
@@ -481,11 +501,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 #pragma unroll
             for (int c0 = 0; c0 < kHalf; c0 += 16) {
                 float d[16];
-                tmem_ld16(mine + c0, d);
+                tmem_ld16(mine + (STATE_ONLY ? (it & 1) * VD : 0) + c0, d);
 #pragma unroll
                 for (int c = 0; c < 16; ++c) S[c0 + c] = fmaf(S[c0 + c], whole, d[c]);
             }
             tc_fence_before();
+            if (STATE_ONLY) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(kO + (it & 1)));
+            }
             if (!STATE_ONLY && !rev) keep(t0, it == chunks - 1 ? t_hi : t0 + kTc);
         }
         if constexpr (STATE_ONLY) {
@@ -531,11 +555,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             if (it >= 0) {
                 if (!wait(full(Y, it), turn(Y, it)) || !wait(full(Z, it), turn(Z, it)) || !wait2(kY, it)) break;
                 tc_fence_after();
-                const uint32_t y = desc_lo(tile_at(Y, it), kTcBlock), yl = desc_lo(y_lo, kTcBlock), z = desc_lo(tile_at(Z, it), kTcBlock);
-                umma_chain<i4, false, kTc / 16>(on, tm + kDelta0, [&](int k) { return y + k * 128; }, [&](int k) { return z + k * 128; });
-                umma_chain<i4, true, kTc / 16>(on, tm + kDelta0, [&](int k) { return yl + k * 128; }, [&](int k) { return z + k * 128; });
-                commit_if(on, bar(kDelta + (it & 1)));
+                if (STATE_ONLY && it > 1 && !wait2(kO, it - 2)) break;      // delta of two chunks ago has been read
+                const uint32_t y = desc_lo(tile_at(Y, it), kTcBlock), yl = desc_lo(y_lo + (STATE_ONLY ? (it & 1) * kTileX : 0), kTcBlock), z = desc_lo(tile_at(Z, it), kTcBlock);
+                const uint32_t delta = uniform(tm + kDelta0 + (STATE_ONLY ? (it & 1) * VD : 0));
+                umma_chain<i4, false, kTc / 16>(on, delta, [&](int k) { return y + k * 128; }, [&](int k) { return z + k * 128; });
                 commit_if(on, empty(Y, it));
+                umma_chain<i4, true, kTc / 16>(on, delta, [&](int k) { return yl + k * 128; }, [&](int k) { return z + k * 128; });
+                commit_if(on, bar(kDelta + (it & 1)));
                 commit_if(on, empty(Z, it));
             }
             const int n = it + 1;
@@ -605,11 +631,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         const float* const g = a.g + (long long)b * a.gb + (long long)h * a.gh;
         double whole = 0.0;
         const float ratio = rev ? k.s_intra : 1.f;                // s_intra / s_inter
+        float next[4];                                            // the next chunk's decays, on their way
+        auto fetch = [&](int it) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = it < chunks ? chunk_at(it) + 4 * lane + i : len;
+                next[i] = t < len ? __ldg(g + (long long)t * a.gt) : 0.f;
+            }
+        };
+        fetch(0);
         for (int it = 0; it < chunks; ++it) {
-            const int t0 = chunk_at(it), valid = min(kTc, len - t0);
             double c[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = 4 * lane + i < valid ? attn_decay(__ldg(g + (long long)(t0 + 4 * lane + i) * a.gt)) : 0.0;
+            for (int i = 0; i < 4; ++i) c[i] = attn_decay(next[i]);
+            fetch(it + 1);
 #pragma unroll
             for (int i = 1; i < 4; ++i) c[i] += c[i - 1];
             double up = c[3];
