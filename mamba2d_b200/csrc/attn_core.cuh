@@ -54,6 +54,7 @@ struct AttnLaunch {
     const int* lengths;
     int B, T, H;
     int nseg, seg_len, runs;
+    int join_here;            // the kernel joins the segments before its own, no launch has
     int seg_columns;          // segments' states have a column's rows next to one another, else a row's columns
 };
 

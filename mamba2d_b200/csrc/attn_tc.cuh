@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         if (!STATE_ONLY && have_row) {
             const float* init = nullptr;
             long long sr = k.init.sr, sc = k.init.sc;
-            if (a.nseg > 1) {
+            if (a.nseg > 1 && !a.join_here) {
                 init = k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd;
                 sr = 1; sc = k.Kd;
             } else if (k.init.p) {
@@ -444,6 +444,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     if (v0 + c < k.Vd) S[c] = init[c * sc];
             }
         }
+        // a few segments: each joins the states of those before it itself, a launch less
+        if (!STATE_ONLY && a.join_here && have_row)
+            for (int j = rev ? a.nseg - 1 : 0; j != seg; j += rev ? -1 : 1) {
+                const size_t at = (size_t)bh * a.nseg + j;
+                const float decay = ex2(k.seg_decay[at]);
+                const float* own = k.seg_state + at * k.Kd * k.Vd + r + (size_t)v0 * k.Kd;
+#pragma unroll
+                for (int c = 0; c < kHalf; ++c) {
+                    if (v0 + c < k.Vd) S[c] = fmaf(S[c], decay, *own);
+                    own += k.Kd;
+                }
+            }
         // (states kept between kernels and runs have a column's rows next to one another: a warp's store is one line, not 32, which
         // held the other warps' shared memory up for 7000 cycles every four chunks)
         auto put = [&](float* to, long long sr, long long sc) {

@@ -484,6 +484,8 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     }
     p.a.seg_columns = tc;
     plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, tc ? 128 : 64, tc ? 4 : 1, &p.a);
+    // (two segments: 139 us with a launch for the joining, 128 without; 18: a CTA would read up to 17 states one after another)
+    p.a.join_here = tc && p.a.nseg > 1 && p.a.nseg <= 4;
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
@@ -600,7 +602,7 @@ static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t s
                                : c.out_f32 ? launch_tc<kTcHeads>(d, p, first, counts[i], st) : launch_tc<kTcPlain>(d, p, first, counts[i], st);
                 if (rc != M2D_OK) return rc;
             }
-            if (!pass) launch_join(p, st);
+            if (!pass && !p.a.join_here) launch_join(p, st);
         }
         return M2D_OK;
     }
