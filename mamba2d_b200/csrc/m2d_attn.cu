@@ -24,48 +24,59 @@ struct Split {
         lo = __float_as_uint(v - __uint_as_float(hi));
     }
 };
-// acc[n] += A (16 x 8) B_n (8 x 8), n < NT; fa(i): the four values of A's fragment, fb(n, i): the two of B's
+// acc[n] += A (16 x 8) B_n (8 x 8), n < NT; fa(i): the four values of A's fragment, fb(n, i): the two of B's.  (One of the three
+// products for all n before the next: those of one accumulator wait for one another.)
 template <int NT, typename FA, typename FB>
 __device__ __forceinline__ void mma_step(float (&acc)[NT][4], FA fa, FB fb) {
-    unsigned ah[4], al[4];
+    unsigned ah[4], al[4], bh[NT][2], bl[NT][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const Split s(fa(i));
         ah[i] = s.hi; al[i] = s.lo;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const Split b0(fb(n, 0)), b1(fb(n, 1));
-        mma_tf32(acc[n], ah, b0.lo, b1.lo);
-        mma_tf32(acc[n], al, b0.hi, b1.hi);
-        mma_tf32(acc[n], ah, b0.hi, b1.hi);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Split s(fb(n, i));
+            bh[n][i] = s.hi; bl[n][i] = s.lo;
+        }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma_tf32(acc[n], ah, bl[n][0], bl[n][1]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma_tf32(acc[n], al, bh[n][0], bh[n][1]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma_tf32(acc[n], ah, bh[n][0], bh[n][1]);
 }
 
-// rows [0, 64) x cols [0, width) of a tile, zero behind `valid` rows and `n` columns
+// rows [0, 64) x cols [0, width) of a tile, zero behind `valid` rows and `n` columns.  fp32 goes straight to shared memory (the caller
+// waits for it); of bf16 four pieces a thread are under way at once.
 template <typename io_t>
 __device__ __forceinline__ void load_rows(float* dst, int stride, const io_t* src, long long st, int valid, int n, int width, int vec) {
     const int quads = width / 4;
+#pragma unroll 4
     for (int i = threadIdx.x; i < kC * quads; i += kAttnThreads) {
         const int r = i / quads, c = (i - r * quads) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < valid) {
-            const io_t* p = src + (long long)r * st + c;
-            if (vec && c + 4 <= n) {
-                if constexpr (sizeof(io_t) == 4) {
-                    v = __ldg(reinterpret_cast<const float4*>(p));
-                } else {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-                    v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-                }
+        const io_t* p = src + (long long)r * st + c;
+        float* const to = dst + r * stride + c;
+        if (r < valid && vec && c + 4 <= n) {
+            if constexpr (sizeof(io_t) == 4) {
+                cp_async16(smem_u32(to), p);
             } else {
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+                *reinterpret_cast<float4*>(to) =
+                    make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+            }
+        } else {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < valid) {
                 if (c < n) v.x = load1(p, 0);
                 if (c + 1 < n) v.y = load1(p, 1);
                 if (c + 2 < n) v.z = load1(p, 2);
                 if (c + 3 < n) v.w = load1(p, 3);
             }
+            *reinterpret_cast<float4*>(to) = v;
         }
-        *reinterpret_cast<float4*>(dst + r * stride + c) = v;
     }
 }
 
@@ -145,13 +156,19 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             }
             continue;
         }
+        float g2[2] = {0.f, 0.f};
+        if (warp == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (2 * lane + j < valid) g2[j] = __ldg(g + (long long)(t0 + 2 * lane + j) * a.gt);
+        }
         if (!STATE_ONLY) load_rows(X, ks, x + (long long)t0 * k.x.st, k.x.st, valid, k.Kd, kd, k.x.vec);
         load_rows(Y, ks, y + (long long)t0 * k.y.st, k.y.st, valid, k.Kd, kd, k.y.vec);
         load_rows(Z, VS, z + (long long)t0 * k.z.st, k.z.st, valid, nv, VT, k.z.vec);
         if (warp == 0) {
             double d[2], up;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) d[j] = 2 * lane + j < valid ? attn_decay(__ldg(g + (long long)(t0 + 2 * lane + j) * a.gt)) : 0.0;
+            for (int j = 0; j < 2; ++j) d[j] = attn_decay(g2[j]);
             up = d[0] + d[1];
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
@@ -174,6 +191,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             if (lane == 0) *whole = ex2((float)end);
             total += end;
         }
+        if (sizeof(io_t) == 4) cp_async_wait_all();
         __syncthreads();
 
         if (!STATE_ONLY) {
@@ -181,6 +199,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             const int pn = (warp >> 2) * 32;
             float acc[4][4] = {};
             if (k.rev ? pn + 31 >= wm : pn <= wm + 15) {
+#pragma unroll 2
                 for (int kk = 0; kk < kd; kk += 8)
                     mma_step<4>(acc, [&](int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
                                 [&](int n, int i) { return Y[(pn + n * 8 + gq) * ks + kk + tq + i * 4]; });
@@ -198,9 +217,11 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             // out, 16 rows x VT / 2 columns a warp
             float o1[NT][4] = {}, o2[NT][4] = {};
             const int c_from = k.rev ? wm : 0, c_to = k.rev ? kC : wm + 16;
+#pragma unroll 2
             for (int kk = c_from; kk < c_to; kk += 8)
                 mma_step<NT>(o1, [&](int i) { return P[(wm + gq + (i & 1) * 8) * kPStride + kk + tq + (i >> 1) * 4]; },
                              [&](int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+#pragma unroll 2
             for (int kk = 0; kk < kd; kk += 8)
                 mma_step<NT>(o2, [&](int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
                              [&](int n, int i) { return S[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
@@ -236,6 +257,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
         const float decay = *whole;
         for (int m = (warp & 3) * 16; m < kd; m += 64) {
             float acc[NT][4] = {};
+#pragma unroll 2
             for (int kk = 0; kk < kC; kk += 8)
                 mma_step<NT>(acc,
                              [&](int i) {
