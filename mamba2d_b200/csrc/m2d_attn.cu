@@ -1,4 +1,6 @@
 // Linear attention: entry points, and the kernels for any head size, type and alignment (attn_tc.cuh has the tcgen05 form).
+#include <climits>
+
 #include "attn_core.cuh"
 #include "attn_tc.cuh"
 #include "launch.cuh"
@@ -455,6 +457,7 @@ static int check_attn(const m2d_attn_desc* d, bool ptrs) {
     if (d->dtype != M2D_F32 && d->dtype != M2D_BF16) return M2D_ERR_DTYPE;
     if (d->flags & ~(uint32_t)M2D_ATTN_CUDA_CORES) return M2D_ERR_FLAGS;
     if (d->B < 1 || d->T < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->K < 1 || d->V < 1 || d->K > M2D_ATTN_MAX_DIM || d->V > M2D_ATTN_MAX_DIM) return M2D_ERR_SHAPE;
+    if (d->T > INT_MAX - 4 * kAnchor) return M2D_ERR_TOO_LARGE;      // (token numbers go up to the end of the last chunk)
     if ((int64_t)d->B * d->H > (1 << 24) || (int64_t)d->B * d->H * ((d->T + kAnchor - 1) / kAnchor) >= (1ll << 31)) return M2D_ERR_TOO_LARGE;
     if (ptrs && (!d->q.data || !d->k.data || !d->v.data || !d->log_decay)) return M2D_ERR_NULL;
     return M2D_OK;

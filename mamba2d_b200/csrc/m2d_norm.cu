@@ -705,7 +705,7 @@ static int check_norm(const m2d_norm_desc* d) {
     if (d->dtype != M2D_F32 && d->dtype != M2D_BF16) return M2D_ERR_DTYPE;
     if (d->act < M2D_ACT_NONE || d->act > M2D_ACT_GELU) return M2D_ERR_FLAGS;
     if (d->N < 1 || d->S < 1 || d->C < 1 || d->groups < 1 || d->C % d->groups) return M2D_ERR_SHAPE;
-    if (d->N > (1ll << 40) || d->S > (1ll << 40) || d->N * d->groups >= (1ll << 31)) return M2D_ERR_TOO_LARGE;
+    if (d->C > (1 << 29) || d->N > (1ll << 40) || d->S > (1ll << 40) || d->N * d->groups >= (1ll << 31)) return M2D_ERR_TOO_LARGE;
     return M2D_OK;
 }
 static NormArgs norm_args(const m2d_norm_desc* d) {
@@ -746,11 +746,12 @@ static NormPlan plan_norm(const m2d_norm_desc* d, bool bwd) {
     if (d->S == 1) {
         const int lanes = per / v;
         if (per % v || lanes < 1 || lanes > 32) return p;
-        p.kind = NormPlan::kRows;
-        p.lanes = lanes;
         const int slots = 8 * (32 / lanes);              // groups of a block
         p.cols = std::min(d->groups, slots);
         p.grid_y = (d->groups + p.cols - 1) / p.cols;
+        if (p.grid_y > 65535) return p;                  // (not a grid)
+        p.kind = NormPlan::kRows;
+        p.lanes = lanes;
         const long long rows = slots / p.cols, steps = (d->N + rows - 1) / rows;
         // as many blocks as run at once; few rows: a block for each of its steps
         p.grid = (int)std::max<long long>(1, std::min<long long>(steps, (bwd ? 2ll : 4ll) * sm_count() / p.grid_y));

@@ -101,7 +101,7 @@ public:
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const at::NoGradGuard no_grad;
+        TORCH_CHECK(!at::GradMode::is_enabled(), "linear_attention: gradients of gradients (create_graph) are not supported");
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[2].device());
         check_waits();
@@ -267,7 +267,7 @@ public:
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const at::NoGradGuard no_grad;
+        TORCH_CHECK(!at::GradMode::is_enabled(), "group_norm: gradients of gradients (create_graph) are not supported");
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[0].device());
         const Tensor x = s[0].contiguous(), w = dense(s[1]), b = dense(s[2]), dy = grads[0].to(x.scalar_type()).contiguous();

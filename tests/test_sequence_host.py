@@ -55,7 +55,7 @@ OK, NULL, DTYPE, SHAPE, WORKSPACE, ABI, LARGE, FLAGS, PITCH = 0, -1, -2, -3, -6,
 
 def test_attention_descriptors(L):
     for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 7}, DTYPE), ({"flags": 1 << 20}, FLAGS), ({"G": 3}, SHAPE), ({"K": 257}, SHAPE), ({"V": 0}, SHAPE),
-                   ({"T": 0}, SHAPE), ({"B": 1 << 23}, LARGE)):
+                   ({"T": 0}, SHAPE), ({"B": 1 << 23}, LARGE), ({"B": 1, "H": 1, "G": 1, "T": (1 << 31) - 1}, LARGE)):
         for fn in (L.m2d_attn_fwd, L.m2d_attn_bwd):
             assert fn(ctypes.byref(attn(**kw)), None) == rc, kw
     assert L.m2d_attn_fwd(None, None) == NULL
@@ -88,7 +88,7 @@ def test_norm_and_clip_descriptors(L):
         for k, v in kw.items():
             setattr(d, k, v)
         return ctypes.byref(d)
-    for kw, rc in (({}, NULL), ({"struct_bytes": 4}, ABI), ({"dtype": 3}, DTYPE), ({"act": 3}, FLAGS), ({"groups": 5}, SHAPE), ({"S": 0}, SHAPE), ({"N": 1 << 30}, LARGE)):
+    for kw, rc in (({}, NULL), ({"struct_bytes": 4}, ABI), ({"dtype": 3}, DTYPE), ({"act": 3}, FLAGS), ({"groups": 5}, SHAPE), ({"S": 0}, SHAPE), ({"N": 1 << 30}, LARGE), ({"C": 1 << 30, "groups": 1}, LARGE)):
         assert L.m2d_norm_fwd(norm(**kw), None) == rc and L.m2d_norm_bwd(norm(**kw), None) == rc
     p = dict(x=256, d_y=256, d_x=256, stats=256)
     assert L.m2d_norm_bwd(norm(d_weight=256, **p), None) == NULL                          # one of the two gradients
