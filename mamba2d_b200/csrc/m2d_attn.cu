@@ -55,29 +55,29 @@ __device__ __forceinline__ void mma_step(float (&acc)[NT][4], FA fa, FB fb) {
 // waits for it); of bf16 four pieces a thread are under way at once.
 template <typename io_t>
 __device__ __forceinline__ void load_rows(float* dst, int stride, const io_t* src, long long st, int valid, int n, int width, int vec) {
-    const int quads = width / 4;
+    const int r = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 4;      // four threads a row (no division: it took a third of this)
+    const io_t* const p = src + (long long)r * st;
+    float* const to = dst + r * stride;
+    static_assert(kAttnThreads == 4 * kC, "rows of a tile");
 #pragma unroll 4
-    for (int i = threadIdx.x; i < kC * quads; i += kAttnThreads) {
-        const int r = i / quads, c = (i - r * quads) * 4;
-        const io_t* p = src + (long long)r * st + c;
-        float* const to = dst + r * stride + c;
+    for (int c = c0; c < width; c += 16) {
         if (r < valid && vec && c + 4 <= n) {
             if constexpr (sizeof(io_t) == 4) {
-                cp_async16(smem_u32(to), p);
+                cp_async16(smem_u32(to + c), p + c);
             } else {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-                *reinterpret_cast<float4*>(to) =
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(p + c));
+                *reinterpret_cast<float4*>(to + c) =
                     make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
             }
         } else {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < valid) {
-                if (c < n) v.x = load1(p, 0);
-                if (c + 1 < n) v.y = load1(p, 1);
-                if (c + 2 < n) v.z = load1(p, 2);
-                if (c + 3 < n) v.w = load1(p, 3);
+                if (c < n) v.x = load1(p, c);
+                if (c + 1 < n) v.y = load1(p, c + 1);
+                if (c + 2 < n) v.z = load1(p, c + 2);
+                if (c + 3 < n) v.w = load1(p, c + 3);
             }
-            *reinterpret_cast<float4*>(to) = v;
+            *reinterpret_cast<float4*>(to + c) = v;
         }
     }
 }
@@ -108,29 +108,45 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     const int wm = (warp & 3) * 16, wn = (warp >> 2) * (VT / 2);
     const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
+    const bool pairs = k.Vd % 2 == 0 && (reinterpret_cast<uintptr_t>(k.out) & 7) == 0;      // out may be written two columns at a time
     const int nv = min(VT, k.Vd - v0), chunks = (t_hi - t_lo + kC - 1) / kC;
     const io_t* const x = static_cast<const io_t*>(attn_at(k.x, b, h, sizeof(io_t)));
     const io_t* const y = static_cast<const io_t*>(attn_at(k.y, b, h, sizeof(io_t)));
     const io_t* const z = static_cast<const io_t*>(attn_at(k.z, b, h, sizeof(io_t))) + v0;
     const float* const g = a.g + (long long)b * a.gb + (long long)h * a.gh;
 
-    for (int i = tid; i < kd * VS; i += kAttnThreads) S[i] = 0.f;
-    __syncthreads();
-    if (!STATE_ONLY) {
-        const float* init = nullptr;
+    // The state before the segment, where it is needed first: until then this launch may run beside the one over the segments' own
+    // states.  A few segments are joined here, else attn_join_kernel has done it.
+    bool begun = false;
+    auto begin = [&] {
+        if (begun) return;
+        begun = true;
+        const float* init = k.init.p ? k.init.p + b * k.init.sb + h * k.init.sh : nullptr;
         long long sr = k.init.sr, sc = k.init.sc;
-        if (a.nseg > 1) {
+        if (!STATE_ONLY) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!STATE_ONLY && a.nseg > 1 && !a.join_here) {
             init = k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd;
             sr = k.Vd; sc = 1;
-        } else if (k.init.p) {
-            init = k.init.p + b * k.init.sb + h * k.init.sh;
         }
-        if (init)
-            for (int i = tid; i < k.Kd * VT; i += kAttnThreads) {
-                const int r = i / VT, c = i % VT;
-                if (c < nv) S[r * VS + c] = init[r * sr + (v0 + c) * sc];
+        for (int i = tid; i < kd * VT; i += kAttnThreads) {
+            const int r = i / VT, c = i % VT;
+            S[r * VS + c] = !STATE_ONLY && init && r < k.Kd && c < nv ? init[r * sr + (v0 + c) * sc] : 0.f;
+        }
+        if (!STATE_ONLY && a.join_here)
+            for (int j = k.rev ? a.nseg - 1 : 0; j != seg; j += k.rev ? -1 : 1) {
+                const size_t at = (size_t)bh * a.nseg + j;
+                const float decay = ex2(k.seg_decay[at]);
+                const float* own = k.seg_state + at * k.Kd * k.Vd + v0;
+#pragma unroll 8
+                for (int i = tid; i < k.Kd * VT; i += kAttnThreads) {
+                    const int r = i / VT, c = i % VT;
+                    if (c < nv) S[r * VS + c] = fmaf(S[r * VS + c], decay, own[(size_t)r * k.Vd + c]);
+                }
             }
-    }
+    };
+    if (STATE_ONLY) begin();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const bool last_wanted = STATE_ONLY || (k.fin.p && seg == (k.rev ? 0 : a.nseg - 1));
     double total = 0.0;
 
     for (int it = 0; it < chunks; ++it) {
@@ -145,7 +161,11 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             }
         };
         __syncthreads();
-        if (run_end && k.rev) keep_state();
+        if (run_end && k.rev) {
+            begin();
+            __syncthreads();
+            keep_state();
+        }
         if (valid == 0) {
             if (!STATE_ONLY) {
                 for (int i = tid; i < rows * nv; i += kAttnThreads) {
@@ -154,7 +174,11 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
                     else store1(static_cast<io_t*>(k.out), at, 0.f);
                 }
                 if (k.dots && tid < rows) k.dots[(((size_t)blockIdx.y * a.B + b) * a.T + t0 + tid) * a.H + h] = 0.f;
-                if (run_end && !k.rev) keep_state();
+                if (run_end && !k.rev) {
+                    begin();
+                    __syncthreads();
+                    keep_state();
+                }
             }
             continue;
         }
@@ -215,6 +239,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
                     const bool on = (k.rev ? c >= r : c <= r) && c < valid && r < valid;
                     P[r * kPStride + c] = on ? k.s_intra * ex2(k.rev ? -d : d) * acc[n][i] : 0.f;
                 }
+            begin();
             __syncthreads();
             // out, 16 rows x VT / 2 columns a warp
             float o1[NT][4] = {}, o2[NT][4] = {};
@@ -235,17 +260,27 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
                 const io_t* e = k.dots ? static_cast<const io_t*>(attn_at(k.e, b, h, sizeof(io_t))) + (long long)(t0 + r) * k.e.st + v0 : nullptr;
                 float sum = 0.f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    const int c = wn + n * 8 + tq * 2;
+                    const float v0 = r < valid ? fmaf(wr, o2[n][half * 2], o1[n][half * 2]) : 0.f, v1 = r < valid ? fmaf(wr, o2[n][half * 2 + 1], o1[n][half * 2 + 1]) : 0.f;
+                    if (r < rows && c < nv) {
+                        if (pairs) {
+                            if (sizeof(io_t) == 4 || k.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(k.out) + row + c) = make_float2(v0, v1);
+                            else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(k.out) + row + c) = pack_bf16x2(v0, v1);
+                        } else {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int c = wn + n * 8 + tq * 2 + i;
-                        const float v = r < valid ? o1[n][half * 2 + i] + wr * o2[n][half * 2 + i] : 0.f;
-                        if (r < rows && c < nv) {
-                            if (k.out_f32) static_cast<float*>(k.out)[row + c] = v;
-                            else store1(static_cast<io_t*>(k.out), row + c, v);
-                            if (e && r < valid) sum += v * load1(e, c);
+                            for (int i = 0; i < 2; ++i)
+                                if (c + i < nv) {
+                                    if (k.out_f32) static_cast<float*>(k.out)[row + c + i] = i ? v1 : v0;
+                                    else store1(static_cast<io_t*>(k.out), row + c + i, i ? v1 : v0);
+                                }
+                        }
+                        if (e && r < valid) {
+                            sum = fmaf(v0, load1(e, c), sum);
+                            if (c + 1 < nv) sum = fmaf(v1, load1(e, c + 1), sum);
                         }
                     }
+                }
                 if (k.dots) {
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -255,9 +290,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             __syncthreads();
             if (k.dots && tid < rows) k.dots[(((size_t)blockIdx.y * a.B + b) * a.T + t0 + tid) * a.H + h] = dot[tid] + dot[kC + tid];
         }
-        // state: 16 rows x VT / 2 columns at a time
+        // state: 16 rows x VT / 2 columns at a time (after a segment's last chunk only where somebody takes it)
         const float decay = *whole;
-        for (int m = (warp & 3) * 16; m < kd; m += 64) {
+        for (int m = (warp & 3) * 16; m < kd && (it + 1 < chunks || last_wanted || run_end); m += 64) {
             float acc[NT][4] = {};
 #pragma unroll 2
             for (int kk = 0; kk < kC; kk += 8)
@@ -280,6 +315,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             keep_state();
         }
     }
+    begin();
     __syncthreads();
     float* fin = nullptr;
     long long sr = k.fin.sr, sc = k.fin.sc;
@@ -510,7 +546,7 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     p.a.seg_columns = tc;
     plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, tc ? 128 : 64, tc ? 4 : 1, &p.a);
     // (two segments: 139 us with a launch for the joining, 128 without; 18: a CTA would read up to 17 states one after another)
-    p.a.join_here = tc && p.a.nseg > 1 && p.a.nseg <= 4;
+    p.a.join_here = p.a.nseg > 1 && p.a.nseg <= (tc ? 4 : 12);
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
@@ -606,7 +642,21 @@ static int launch_any(const AttnPlan& p, cudaStream_t st) {
         auto part = attn_core_kernel<io_t, VT, true>;
         if (!allow_smem(reinterpret_cast<const void*>(part), p.smem)) return M2D_ERR_LAUNCH;
         part<<<grid, kAttnThreads, p.smem, st>>>(p.a);
-        launch_join(p, st);
+        if (!p.a.join_here) launch_join(p, st);
+    }
+    if (p.a.nseg > 1 && p.a.join_here) {
+        // (what it does before it takes a state needs nothing of the launch before)
+        cudaLaunchConfig_t c{};
+        c.gridDim = grid;
+        c.blockDim = dim3(kAttnThreads);
+        c.dynamicSmemBytes = p.smem;
+        c.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        c.attrs = &attr;
+        c.numAttrs = 1;
+        return cudaLaunchKernelEx(&c, full, p.a) == cudaSuccess ? M2D_OK : (cudaGetLastError(), M2D_ERR_LAUNCH);
     }
     full<<<grid, kAttnThreads, p.smem, st>>>(p.a);
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
