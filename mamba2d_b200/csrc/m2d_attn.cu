@@ -544,8 +544,11 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
         per_sm = std::max<int>(1, (int)((kMaxSmem + 1024) / (p.smem + 1024)));
     }
     p.a.seg_columns = tc;
-    plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm, tc ? 128 : 64, tc ? 4 : 1, &p.a);
-    // (two segments: 139 us with a launch for the joining, 128 without; 18: a CTA would read up to 17 states one after another)
+    // lengths: only the GPU knows how much of T there is, so twice as many as run at once (6x1395x3x64 fp32, training: 138 us for 153;
+    // the tcgen05 form's segments cost too much for that, 8x2048x16x128: 443 for 424)
+    plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm * (d->lengths && !tc ? 2 : 1), tc ? 128 : 64, tc ? 4 : 1, &p.a);
+    // Joined by the kernels that start from them, or by a launch.  tcgen05 form, two segments: 128 us against 139 with a launch; 18: a
+    // CTA would read up to 17 states one after another.  The other form, four segments of single chunks: 16 us against 27, 11 and 5: 166 against 182.
     p.a.join_here = p.a.nseg > 1 && p.a.nseg <= (tc ? 4 : 12);
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
