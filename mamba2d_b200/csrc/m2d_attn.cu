@@ -360,44 +360,45 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     }
 }
 
-// e[b][h][run] = <S, R> of two kept states
-__global__ void __launch_bounds__(256) attn_anchor_kernel(const float* __restrict__ s, const float* __restrict__ r, float* __restrict__ e, int n) {
-    __shared__ float part[8];
-    const size_t at = (size_t)blockIdx.x * n;
-    float sum = 0.f;
-    for (int i = threadIdx.x; i < n; i += 256) sum = fmaf(s[at + i], r[at + i], sum);
-#pragma unroll
-    for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) sum += part[i];
-        e[blockIdx.x] = sum;
-    }
-}
-
-// The decay's gradient from the dots and the anchors: suffix sums over a run.  Dots: [blocks][B][T][H], one of dq and one of dk.
-__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* __restrict__ rq, const float* __restrict__ rk, int blocks, const float* __restrict__ e,
-                                                             const int* __restrict__ lengths, float* __restrict__ dg, int B, int T, int H, int runs) {
-    __shared__ double part[kAnchor / 32];
+// The decay's gradient from the dots and the anchors: suffix sums over a run, and <S, R> of its two kept states (n elements each).
+// Dots: [blocks][B][T][H], one of dq and one of dk.
+__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* __restrict__ rq, const float* __restrict__ rk, int blocks, const float* __restrict__ anchor_s,
+                                                             const float* __restrict__ anchor_r, int n, const int* __restrict__ lengths, float* __restrict__ dg, int B, int T, int H,
+                                                             int runs) {
+    __shared__ double part[kAnchor / 32], whole[kAnchor / 32];
     const int run = blockIdx.x % runs, bh = blockIdx.x / runs, h = bh % H, b = bh / H;
     const int t = run * kAnchor + (kAnchor - 1 - threadIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;      // from the last token on
-    double v = 0.0;
+    const float *const s = anchor_s + (size_t)blockIdx.x * n, *const r = anchor_r + (size_t)blockIdx.x * n;
+    float e = 0.f;
+    if (n % 4 == 0) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n / 4; i += kAnchor) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>(s) + i), y = __ldg(reinterpret_cast<const float4*>(r) + i);
+            e = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, e))));
+        }
+    } else {
+        for (int i = threadIdx.x; i < n; i += kAnchor) e = fmaf(s[i], r[i], e);
+    }
+    double v = 0.0, sum = (double)e;
     if (t < T)
         for (int j = 0; j < blocks; ++j) {
             const size_t at = (((size_t)j * B + b) * T + t) * H + h;
             v += (double)rq[at] - (double)rk[at];
         }
 #pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-        const double o = __shfl_up_sync(0xffffffffu, v, s);
-        if (lane >= s) v += o;
+    for (int m = 1; m < 32; m <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, v, m);
+        if (lane >= m) v += o;
+        sum += __shfl_xor_sync(0xffffffffu, sum, m);
     }
-    if (lane == 31) part[warp] = v;
+    if (lane == 31) {
+        part[warp] = v;
+        whole[warp] = sum;
+    }
     __syncthreads();
-    for (int i = 0; i < warp; ++i) v += part[i];
+    for (int i = 0; i < kAnchor / 32; ++i) v += (i < warp ? part[i] : 0.0) + whole[i];
     const int len = lengths ? min(max(lengths[b], 0), T) : T;
-    if (t < T) dg[((size_t)b * T + t) * H + h] = t < len ? (float)(v + (double)e[blockIdx.x]) : 0.f;
+    if (t < T) dg[((size_t)b * T + t) * H + h] = t < len ? (float)v : 0.f;
 }
 
 // Gradients of shared queries or keys: (rows,H,K) fp32 -> (rows,G,K), heads summed in order.
@@ -527,7 +528,7 @@ struct AttnPlan {
     bool tc = false;
     int cores = 1, col_blocks = 1, VT = 64, dot_blocks = 1;
     size_t smem = 0, bytes = 0;
-    size_t at_seg[3] = {}, at_decay[3] = {}, at_dots[2] = {}, at_anchor[2] = {}, at_e = 0, at_heads[2] = {};
+    size_t at_seg[3] = {}, at_decay[3] = {}, at_dots[2] = {}, at_anchor[2] = {}, at_heads[2] = {};
 };
 static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     AttnPlan p;
@@ -564,7 +565,6 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     if (bwd && d->d_log_decay) {
         for (size_t& at : p.at_dots) at = take(4 * tokens * p.dot_blocks);
         for (size_t& at : p.at_anchor) at = take(4 * bh * p.a.runs * kv);
-        p.at_e = take(4 * bh * p.a.runs);
     }
     if (bwd && d->G != d->H)
         for (size_t& at : p.at_heads) at = take(4 * tokens * d->K);
@@ -768,10 +768,8 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     dv.fin = dense_state(d, d->d_state, false);
     if ((rc = launch_core(d, p, st)) != M2D_OK) return rc;
     if (d->d_log_decay) {
-        float* const e = reinterpret_cast<float*>(ws + p.at_e);
         const unsigned n = (unsigned)(d->B * d->H * p.a.runs);
-        attn_anchor_kernel<<<n, 256, 0, st>>>(dq.anchors, dk.anchors, e, d->K * d->V);
-        attn_decay_kernel<<<n, kAnchor, 0, st>>>(dq.dots, dk.dots, p.dot_blocks, e, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs);
+        attn_decay_kernel<<<n, kAnchor, 0, st>>>(dq.dots, dk.dots, p.dot_blocks, dq.anchors, dk.anchors, d->K * d->V, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs);
     }
     if (d->G != d->H) {
         const long long n = (long long)d->B * d->T * d->G * d->K;
