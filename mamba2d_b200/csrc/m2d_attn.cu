@@ -26,29 +26,38 @@ struct Split {
         lo = __float_as_uint(v - __uint_as_float(hi));
     }
 };
-// acc[n] += A (16 x 8) B_n (8 x 8), n < NT; fa(i): the four values of A's fragment, fb(n, i): the two of B's.  (One of the three
-// products for all n before the next: those of one accumulator wait for one another.)
+// acc[n] += A (16 x 8) B_n (8 x 8) over steps of 8 in [from, to), n < NT; fa(kk, i): the four values of A's fragment, fb(kk, n, i):
+// the two of B's.  (The unit cuts off what it adds to an accumulator: the small products have one of their own, which leaves the large
+// ones a third of the steps.  One of the three products for all n before the next: those of one accumulator wait for one another.)
 template <int NT, typename FA, typename FB>
-__device__ __forceinline__ void mma_step(float (&acc)[NT][4], FA fa, FB fb) {
-    unsigned ah[4], al[4], bh[NT][2], bl[NT][2];
+__device__ __forceinline__ void mma_chain(float (&acc)[NT][4], int from, int to, FA fa, FB fb) {
+    float low[NT][4] = {};
+#pragma unroll 2
+    for (int kk = from; kk < to; kk += 8) {
+        unsigned ah[4], al[4], bh[NT][2], bl[NT][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const Split s(fa(i));
-        ah[i] = s.hi; al[i] = s.lo;
+        for (int i = 0; i < 4; ++i) {
+            const Split s(fa(kk, i));
+            ah[i] = s.hi; al[i] = s.lo;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const Split s(fb(kk, n, i));
+                bh[n][i] = s.hi; bl[n][i] = s.lo;
+            }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_tf32(low[n], ah, bl[n][0], bl[n][1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_tf32(acc[n], ah, bh[n][0], bh[n][1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_tf32(low[n], al, bh[n][0], bh[n][1]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const Split s(fb(n, i));
-            bh[n][i] = s.hi; bl[n][i] = s.lo;
-        }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) mma_tf32(acc[n], ah, bl[n][0], bl[n][1]);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) mma_tf32(acc[n], al, bh[n][0], bh[n][1]);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) mma_tf32(acc[n], ah, bh[n][0], bh[n][1]);
+        for (int i = 0; i < 4; ++i) acc[n][i] += low[n][i];
 }
 
 // rows [0, 64) x cols [0, width) of a tile, zero behind `valid` rows and `n` columns.  fp32 goes straight to shared memory (the caller
@@ -224,12 +233,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             // P = s_intra D (X Y^T), 16 rows x 32 columns a warp
             const int pn = (warp >> 2) * 32;
             float acc[4][4] = {};
-            if (k.rev ? pn + 31 >= wm : pn <= wm + 15) {
-#pragma unroll 2
-                for (int kk = 0; kk < kd; kk += 8)
-                    mma_step<4>(acc, [&](int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
-                                [&](int n, int i) { return Y[(pn + n * 8 + gq) * ks + kk + tq + i * 4]; });
-            }
+            if (k.rev ? pn + 31 >= wm : pn <= wm + 15)
+                mma_chain<4>(acc, 0, kd, [&](int kk, int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
+                             [&](int kk, int n, int i) { return Y[(pn + n * 8 + gq) * ks + kk + tq + i * 4]; });
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -243,15 +249,10 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             __syncthreads();
             // out, 16 rows x VT / 2 columns a warp
             float o1[NT][4] = {}, o2[NT][4] = {};
-            const int c_from = k.rev ? wm : 0, c_to = k.rev ? kC : wm + 16;
-#pragma unroll 2
-            for (int kk = c_from; kk < c_to; kk += 8)
-                mma_step<NT>(o1, [&](int i) { return P[(wm + gq + (i & 1) * 8) * kPStride + kk + tq + (i >> 1) * 4]; },
-                             [&](int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
-#pragma unroll 2
-            for (int kk = 0; kk < kd; kk += 8)
-                mma_step<NT>(o2, [&](int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
-                             [&](int n, int i) { return S[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+            mma_chain<NT>(o1, k.rev ? wm : 0, k.rev ? kC : wm + 16, [&](int kk, int i) { return P[(wm + gq + (i & 1) * 8) * kPStride + kk + tq + (i >> 1) * 4]; },
+                          [&](int kk, int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+            mma_chain<NT>(o2, 0, kd, [&](int kk, int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
+                          [&](int kk, int n, int i) { return S[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int r = wm + gq + half * 8;
@@ -262,22 +263,22 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int c = wn + n * 8 + tq * 2;
-                    const float v0 = r < valid ? fmaf(wr, o2[n][half * 2], o1[n][half * 2]) : 0.f, v1 = r < valid ? fmaf(wr, o2[n][half * 2 + 1], o1[n][half * 2 + 1]) : 0.f;
+                    const float a0 = r < valid ? fmaf(wr, o2[n][half * 2], o1[n][half * 2]) : 0.f, a1 = r < valid ? fmaf(wr, o2[n][half * 2 + 1], o1[n][half * 2 + 1]) : 0.f;
                     if (r < rows && c < nv) {
                         if (pairs) {
-                            if (sizeof(io_t) == 4 || k.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(k.out) + row + c) = make_float2(v0, v1);
-                            else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(k.out) + row + c) = pack_bf16x2(v0, v1);
+                            if (sizeof(io_t) == 4 || k.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(k.out) + row + c) = make_float2(a0, a1);
+                            else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(k.out) + row + c) = pack_bf16x2(a0, a1);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
                                 if (c + i < nv) {
-                                    if (k.out_f32) static_cast<float*>(k.out)[row + c + i] = i ? v1 : v0;
-                                    else store1(static_cast<io_t*>(k.out), row + c + i, i ? v1 : v0);
+                                    if (k.out_f32) static_cast<float*>(k.out)[row + c + i] = i ? a1 : a0;
+                                    else store1(static_cast<io_t*>(k.out), row + c + i, i ? a1 : a0);
                                 }
                         }
                         if (e && r < valid) {
-                            sum = fmaf(v0, load1(e, c), sum);
-                            if (c + 1 < nv) sum = fmaf(v1, load1(e, c + 1), sum);
+                            sum = fmaf(a0, load1(e, c), sum);
+                            if (c + 1 < nv) sum = fmaf(a1, load1(e, c + 1), sum);
                         }
                     }
                 }
@@ -294,14 +295,12 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
         const float decay = *whole;
         for (int m = (warp & 3) * 16; m < kd && (it + 1 < chunks || last_wanted || run_end); m += 64) {
             float acc[NT][4] = {};
-#pragma unroll 2
-            for (int kk = 0; kk < kC; kk += 8)
-                mma_step<NT>(acc,
-                             [&](int i) {
-                                 const int c = kk + tq + (i >> 1) * 4;
-                                 return Y[c * ks + m + gq + (i & 1) * 8] * u[c];
-                             },
-                             [&](int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
+            mma_chain<NT>(acc, 0, kC,
+                          [&](int kk, int i) {
+                              const int c = kk + tq + (i >> 1) * 4;
+                              return Y[c * ks + m + gq + (i & 1) * 8] * u[c];
+                          },
+                          [&](int kk, int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
