@@ -3,6 +3,7 @@
 
 #include "attn_core.cuh"
 #include "attn_tc.cuh"
+#include "follow.cuh"
 #include "launch.cuh"
 
 namespace m2d {
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
         begun = true;
         const float* init = k.init.p ? k.init.p + b * k.init.sb + h * k.init.sh : nullptr;
         long long sr = k.init.sr, sc = k.init.sc;
-        if (!STATE_ONLY) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!STATE_ONLY) follow_wait();
         if (!STATE_ONLY && a.nseg > 1 && !a.join_here) {
             init = k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd;
             sr = k.Vd; sc = 1;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             }
     };
     if (STATE_ONLY) begin();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    let_follow();
     const bool last_wanted = STATE_ONLY || (k.fin.p && seg == (k.rev ? 0 : a.nseg - 1));
     double total = 0.0;
 
@@ -338,6 +339,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     const AttnCore& k = a.core[blockIdx.z];
     const int bh = blockIdx.x, h = bh % a.H, b = bh / a.H, n = k.Kd * k.Vd;
     const int i = blockIdx.y * 128 + threadIdx.x;
+    let_follow();
     if (i >= n) return;
     const int row = a.seg_columns ? i % k.Kd : i / k.Vd, col = a.seg_columns ? i / k.Kd : i % k.Vd;
     float carry = k.init.p ? k.init.p[b * k.init.sb + h * k.init.sh + row * k.init.sr + col * k.init.sc] : 0.f;
@@ -361,18 +363,19 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
 
 // The decay's gradient from the dots and the anchors: suffix sums over a run, and <S, R> of its two kept states (n elements each).
 // Dots: [blocks][B][T][H], one of dq and one of dk.
-__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* __restrict__ rq, const float* __restrict__ rk, int blocks, const float* __restrict__ anchor_s,
-                                                             const float* __restrict__ anchor_r, int n, const int* __restrict__ lengths, float* __restrict__ dg, int B, int T, int H,
+__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* rq, const float* rk, int blocks, const float* anchor_s, const float* anchor_r, int n, const int* __restrict__ lengths, float* dg, int B, int T, int H,
                                                              int runs) {
     __shared__ double part[kAnchor / 32], whole[kAnchor / 32];
     const int run = blockIdx.x % runs, bh = blockIdx.x / runs, h = bh % H, b = bh / H;
     const int t = run * kAnchor + (kAnchor - 1 - threadIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;      // from the last token on
     const float *const s = anchor_s + (size_t)blockIdx.x * n, *const r = anchor_r + (size_t)blockIdx.x * n;
     float e = 0.f;
+    let_follow();
+    follow_wait();
     if (n % 4 == 0) {
 #pragma unroll 4
         for (int i = threadIdx.x; i < n / 4; i += kAnchor) {
-            const float4 x = __ldg(reinterpret_cast<const float4*>(s) + i), y = __ldg(reinterpret_cast<const float4*>(r) + i);
+            const float4 x = reinterpret_cast<const float4*>(s)[i], y = reinterpret_cast<const float4*>(r)[i];
             e = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, e))));
         }
     } else {
@@ -402,8 +405,9 @@ __global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* __rest
 
 // Gradients of shared queries or keys: (rows,H,K) fp32 -> (rows,G,K), heads summed in order.
 template <typename io_t>
-__global__ void __launch_bounds__(256) attn_share_kernel(const float* __restrict__ p0, const float* __restrict__ p1, io_t* __restrict__ o0, io_t* __restrict__ o1, long long n,
+__global__ void __launch_bounds__(256) attn_share_kernel(const float* p0, const float* p1, io_t* o0, io_t* o1, long long n,
                                                          int K, int per) {
+    follow_wait();
     const float* p = blockIdx.y ? p1 : p0;
     io_t* o = blockIdx.y ? o1 : o0;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
@@ -631,6 +635,7 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
     return v64 ? launch_tc<128, 64, MODE>(d, p, first, count, st) : launch_tc<128, 128, MODE>(d, p, first, count, st);
 }
 
+// (Not as a launch that follows: its CTAs would gather on the few SMs that the states leave free, 1x65536x8: 180 us against 174.)
 static void launch_join(const AttnPlan& p, cudaStream_t st) {
     const int n = p.a.core[0].Kd * p.a.core[0].Vd;
     attn_join_kernel<<<dim3(p.a.B * p.a.H, (n + 127) / 128, p.cores), 128, 0, st>>>(p.a);
@@ -646,20 +651,7 @@ static int launch_any(const AttnPlan& p, cudaStream_t st) {
         part<<<grid, kAttnThreads, p.smem, st>>>(p.a);
         if (!p.a.join_here) launch_join(p, st);
     }
-    if (p.a.nseg > 1 && p.a.join_here) {
-        // (what it does before it takes a state needs nothing of the launch before)
-        cudaLaunchConfig_t c{};
-        c.gridDim = grid;
-        c.blockDim = dim3(kAttnThreads);
-        c.dynamicSmemBytes = p.smem;
-        c.stream = st;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        c.attrs = &attr;
-        c.numAttrs = 1;
-        return cudaLaunchKernelEx(&c, full, p.a) == cudaSuccess ? M2D_OK : (cudaGetLastError(), M2D_ERR_LAUNCH);
-    }
+    if (p.a.nseg > 1) return launch_following(full, grid, dim3(kAttnThreads), p.smem, st, p.a) ? M2D_OK : M2D_ERR_LAUNCH;
     full<<<grid, kAttnThreads, p.smem, st>>>(p.a);
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
 }
@@ -768,14 +760,15 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     if ((rc = launch_core(d, p, st)) != M2D_OK) return rc;
     if (d->d_log_decay) {
         const unsigned n = (unsigned)(d->B * d->H * p.a.runs);
-        attn_decay_kernel<<<n, kAnchor, 0, st>>>(dq.dots, dk.dots, p.dot_blocks, dq.anchors, dk.anchors, d->K * d->V, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs);
+if (!launch_following(attn_decay_kernel, dim3(n), dim3(kAnchor), 0, st, (const float*)dq.dots, (const float*)dk.dots, p.dot_blocks, (const float*)dq.anchors, (const float*)dk.anchors, d->K * d->V, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs)) return M2D_ERR_LAUNCH;
     }
     if (d->G != d->H) {
         const long long n = (long long)d->B * d->T * d->G * d->K;
         const dim3 grid((unsigned)std::min<long long>((n + 255) / 256, 16ll * sm_count()), 2);
         const float *h0 = reinterpret_cast<const float*>(ws + p.at_heads[0]), *h1 = reinterpret_cast<const float*>(ws + p.at_heads[1]);
-        if (d->dtype == M2D_F32) attn_share_kernel<float><<<grid, 256, 0, st>>>(h0, h1, static_cast<float*>(d->d_q), static_cast<float*>(d->d_k), n, d->K, per);
-        else attn_share_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(h0, h1, static_cast<__nv_bfloat16*>(d->d_q), static_cast<__nv_bfloat16*>(d->d_k), n, d->K, per);
+        if (d->dtype == M2D_F32) rc = launch_following(attn_share_kernel<float>, grid, dim3(256), 0, st, h0, h1, static_cast<float*>(d->d_q), static_cast<float*>(d->d_k), n, d->K, per) ? M2D_OK : M2D_ERR_LAUNCH;
+        else rc = launch_following(attn_share_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, h0, h1, static_cast<__nv_bfloat16*>(d->d_q), static_cast<__nv_bfloat16*>(d->d_k), n, d->K, per) ? M2D_OK : M2D_ERR_LAUNCH;
+        if (rc != M2D_OK) return rc;
     }
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
 }

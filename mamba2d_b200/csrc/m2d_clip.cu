@@ -5,6 +5,7 @@
 // partial sum per CTA; in the second every CTA adds the partial sums up for itself, in the same order, so that
 // all have the same factor and no counter or flag is needed.  It walks the pieces backwards: what the
 // first kernel read last is what the L2 still holds.  Where the factor is 1 nothing is written.
+#include "follow.cuh"
 #include "plan.cuh"
 #include "m2d_seq.h"
 
@@ -58,6 +59,7 @@ __device__ __forceinline__ double clip_block_sum(double v) {
 }
 
 __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_constant__ ClipTable t, double* __restrict__ partial) {
+    let_follow();
     double total = 0.0;
     for (unsigned piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
         const int i = clip_find(t, piece);
@@ -83,8 +85,8 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_co
     if (threadIdx.x == 0) partial[blockIdx.x] = total;
 }
 
-__global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_constant__ ClipTable t, const double* __restrict__ partial, int partials, float max_norm,
-                                                                  float* __restrict__ norm) {
+__global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_constant__ ClipTable t, const double* partial, int partials, float max_norm, float* norm) {
+    follow_wait();
     double total = 0.0;
     for (int i = threadIdx.x; i < partials; i += kClipThreads) total += partial[i];
     total = sqrt(clip_block_sum(total));
@@ -168,7 +170,7 @@ extern "C" int m2d_clip_grad_norm(const m2d_clip_tensor* tensors, int32_t count,
                 t.first[t.count] = (unsigned)pieces;
             }
             if (!pass) clip_norm_kernel<<<grid, kClipThreads, 0, st>>>(t, partial + (size_t)l * grid);
-            else clip_scale_kernel<<<grid, kClipThreads, 0, st>>>(t, partial, launches * grid, max_norm, l ? nullptr : norm);
+            else if (!launch_following(clip_scale_kernel, dim3(grid), dim3(kClipThreads), 0, st, t, (const double*)partial, launches * grid, max_norm, l ? (float*)nullptr : norm)) return M2D_ERR_LAUNCH;
         }
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
 }

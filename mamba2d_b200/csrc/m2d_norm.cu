@@ -1,6 +1,7 @@
 // Group normalisation with an activation, channels last: entry points and kernels.
 #include <cooperative_groups.h>
 
+#include "follow.cuh"
 #include "plan.cuh"
 #include "m2d_seq.h"
 
@@ -138,6 +139,7 @@ __global__ void __launch_bounds__(256, BWD ? 2 : 4) norm_rows_kernel(const NormA
     const unsigned mask = __ballot_sync(0xffffffffu, on);       // (whole groups)
     const int c0 = col * V::n;
     const bool even = (lanes & (lanes - 1)) == 0;
+    let_follow();
     float2 w[V::pairs], bias[V::pairs], dw[V::pairs] = {}, db[V::pairs] = {};
 #pragma unroll
     for (int i = 0; i < V::pairs; ++i) {
@@ -300,6 +302,8 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
         w[i] = make_float2(norm_param<io_t>(a.weight, c0 + 2 * i, a.params_f32, 1.f), norm_param<io_t>(a.weight, c0 + 2 * i + 1, a.params_f32, 1.f));
         bias[i] = make_float2(norm_param<io_t>(a.bias, c0 + 2 * i, a.params_f32, 0.f), norm_param<io_t>(a.bias, c0 + 2 * i + 1, a.params_f32, 0.f));
     }
+    let_follow();
+    if (PHASE == 2) follow_wait();
     // chan[k][c] = sum over the threads of channel c
     auto channel_sums = [&](float2 (&v)[V::pairs], int k) {
         if (fold)
@@ -541,6 +545,8 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
 
 // Images in pieces: (mean, sum of squares about it) of the pieces' groups -> (mean, rstd).  A warp per image and group.
 __global__ void __launch_bounds__(256) norm_join_kernel(const NormArgs a) {
+    let_follow();
+    follow_wait();
     const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
     if (at >= a.N * a.groups) return;
     const long long n = at / a.groups;
@@ -564,6 +570,8 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const NormArgs a) {
 // Images in pieces, backward: the pieces' channel sums ([N][pieces][2][C], dz h and dz) -> means of dh and dh h.  A warp per image and group.
 template <typename io_t>
 __global__ void __launch_bounds__(256) norm_join_bwd_kernel(const NormArgs a) {
+    let_follow();
+    follow_wait();
     const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
     if (at >= a.N * a.groups) return;
     const long long n = at / a.groups;
@@ -676,7 +684,8 @@ __global__ void __launch_bounds__(256) norm_wgrad_any(const NormArgs a) {
 // thread under way at once.
 constexpr int kSumRows = 32;
 template <typename io_t>
-__global__ void __launch_bounds__(32 * kSumRows) norm_wgrad_sum(const float* __restrict__ partial, int splits, int C, int f32, void* d_weight, void* d_bias) {
+__global__ void __launch_bounds__(32 * kSumRows) norm_wgrad_sum(const float* partial, int splits, int C, int f32, void* d_weight, void* d_bias) {
+    follow_wait();
     __shared__ float part[kSumRows][33];
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float v[4] = {};
@@ -684,7 +693,7 @@ __global__ void __launch_bounds__(32 * kSumRows) norm_wgrad_sum(const float* __r
         for (int s = row; s < splits; s += 4 * kSumRows)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (s + j * kSumRows < splits) v[j] += __ldg(partial + (size_t)(s + j * kSumRows) * 2 * C + i);
+                if (s + j * kSumRows < splits) v[j] += partial[(size_t)(s + j * kSumRows) * 2 * C + i];
     part[row][lane] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
     float sum = part[lane][row];                        // (warp `row` adds column `row` up)
@@ -819,12 +828,14 @@ static int launch_image(const NormArgs& a, const NormPlan& p, cudaStream_t st) {
     c.blockDim = dim3(kNormThreads);
     c.dynamicSmemBytes = p.smem;
     c.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = PHASE == 0 ? p.pieces : 1;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    c.attrs = &attr;
-    c.numAttrs = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PHASE == 0 ? p.pieces : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = attr;
+    c.numAttrs = PHASE == 2 ? 2 : 1;
     return cudaLaunchKernelEx(&c, kern, a) == cudaSuccess ? M2D_OK : (cudaGetLastError(), M2D_ERR_LAUNCH);
 }
 template <typename io_t, int ACT, bool BWD>
@@ -838,8 +849,7 @@ static int launch_norm(NormArgs a, const NormPlan& p, cudaStream_t st) {
         int rc = launch_image<io_t, ACT, BWD, 1>(a, p, st);
         if (rc != M2D_OK) return rc;
         const unsigned grid = (unsigned)((a.N * a.groups + 7) / 8);
-        if (BWD) norm_join_bwd_kernel<io_t><<<grid, 256, 0, st>>>(a);
-        else norm_join_kernel<<<grid, 256, 0, st>>>(a);
+        if (!launch_following(BWD ? norm_join_bwd_kernel<io_t> : norm_join_kernel, dim3(grid), dim3(256), 0, st, a)) return M2D_ERR_LAUNCH;
         return launch_image<io_t, ACT, BWD, 2>(a, p, st);
     }
     const unsigned grid = (unsigned)(a.N * a.groups);
@@ -916,8 +926,10 @@ extern "C" int m2d_norm_bwd(const m2d_norm_desc* d, void* stream) {
     if ((rc = launch_norm<true>(d, a, p, st)) != M2D_OK) return rc;
     if (d->d_weight) {
         const unsigned grid = (2 * d->C + 31) / 32;
-        if (d->dtype == M2D_F32) norm_wgrad_sum<float><<<grid, 32 * kSumRows, 0, st>>>(a.partial, (int)p.partial, d->C, 1, d->d_weight, d->d_bias);
-        else norm_wgrad_sum<__nv_bfloat16><<<grid, 32 * kSumRows, 0, st>>>(a.partial, (int)p.partial, d->C, d->params_f32, d->d_weight, d->d_bias);
+        const bool f32 = d->dtype == M2D_F32;
+        if (!launch_following(f32 ? norm_wgrad_sum<float> : norm_wgrad_sum<__nv_bfloat16>, dim3(grid), dim3(32 * kSumRows), 0, st, (const float*)a.partial, (int)p.partial, d->C,
+                              f32 ? 1 : d->params_f32, d->d_weight, d->d_bias))
+            return M2D_ERR_LAUNCH;
     }
     return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
 }
