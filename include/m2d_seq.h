@@ -19,6 +19,12 @@ extern "C" {
  *     S_t = exp(g_t) S_{t-1} + k_t v_t^T,      o_t = scale * q_t^T S_t.
  * q and k have G heads, each shared by H / G neighbouring heads of v.  g = log_decay, fp32, at most 0 (-inf forgets
  * everything before the token; a positive value grows the state and is not checked for).
+ *
+ * State, its gradient and that of the decay are fp32 whatever the tensors' type.  bf16 tensors with K and V of up to 128 in whole
+ * 16-byte pieces, 16-byte aligned and with such strides, take a form on the tensor cores (tcgen05), all others one for any
+ * size.  Long sequences of few heads are cut into segments whose states the workspace holds; the workspace queries read the
+ * sizes, G, dtype and, for the backward pass, whether d_log_decay is given.  B * H up to 2^24, T below 2^31 - 2048.
+ * A wait inside the tensor-core form that gives up makes its rows NaN and shows in m2d_take_wait_failure().
  */
 #define M2D_ATTN_MAX_DIM 256      /* K and V, each */
 
@@ -66,7 +72,8 @@ int m2d_attn_step(const m2d_attn_desc *desc, int64_t state_batch, int64_t state_
 
 /* ---- group normalisation ----------------------------------------------------------------------------------------
  * x (N,S,C), channels last: y = act((x - mean) * rstd * weight + bias), mean and variance over S and the C / groups
- * channels of a group.
+ * channels of a group.  C up to 2^29, N * groups below 2^31; tensors that are not 16-byte aligned, or whose rows are not whole 16-byte
+ * pieces, take a slower form.
  */
 typedef enum { M2D_ACT_NONE = 0, M2D_ACT_SILU = 1, M2D_ACT_GELU = 2 /* erf form */ } m2d_act;
 
@@ -95,7 +102,7 @@ int m2d_norm_bwd(const m2d_norm_desc *desc, void *stream);
 
 /* ---- clipping by the global norm --------------------------------------------------------------------------------
  * norm = sqrt(sum of squares over all tensors); every tensor is multiplied by min(1, max_norm / (norm + 1e-6)).  The
- * tensors must not overlap.
+ * tensors must not overlap.  Squares are taken in fp32: a value beyond 1.8e19 makes the norm infinite.
  */
 typedef struct m2d_clip_tensor {
     void *data;                    /* aligned to its elements */

@@ -21,6 +21,10 @@
 // took 2000 cycles of a chunk, 32 lines a request.  It has a tile of its own where there is room (a head size of 64), else that of x,
 // which nothing reads any more, but whose next load then waits for it.
 //
+// Measured, forward at 8x2048x16x128: 84 us for 128 CTAs of 16 chunks, 10000 cycles a chunk: the tensor cores are busy for 29 % of them,
+// the schedulers issue in 26 %, and what most warps wait for, besides each other, is instructions (1.9 of the 6 cycles between
+// two instructions of a warp).  The bytes would take 34 us.  With dots and anchors 235 us for dq and dk (256 CTAs in two waves), dv 83.
+//
 // `fine` (wanted where the decay's gradient is): P and St also in two parts each, so that the dots that out is summed
 // into are exact to 2^-17 like the states that they meet.
 //

@@ -12,6 +12,10 @@ namespace m2d {
 // attn_core.cuh's computation on chunks of 64 tokens.  A CTA owns a sequence's head, VT columns of z and of the
 // state, and one segment of the tokens; its products run on mma.sync in tf32, every operand split into two tf32 parts
 // and three products per term, which leaves an error of about 2^-21 (operands in bf16 are exact in one part).
+//
+// What bounds it: at 6x1395x3x64 fp32 (training, 129 us) two CTAs on an SM issue in 39 % of their cycles, a third of that for the
+// operands' splitting, and the longest sequences' CTAs end last; at 196 tokens (16 us) two launches of one chunk each.  64 tokens and
+// 64 columns: larger tiles leave one CTA on an SM.
 // ------------------------------------------------------------------------------------------------
 constexpr int kC = 64, kAttnThreads = 256, kPStride = kC + 4;
 
@@ -361,10 +365,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     }
 }
 
-// The decay's gradient from the dots and the anchors: suffix sums over a run, and <S, R> of its two kept states (n elements each).
+// The decay's gradient from the dots and the anchors: suffix sums over a run, and <S, R> of its two kept states (n elements each), which
+// is what it reads: 71 MB at 8x2048x16x128, 21 us (a launch of its own for <S, R>: 16 and 7 us).
 // Dots: [blocks][B][T][H], one of dq and one of dk.
-__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* rq, const float* rk, int blocks, const float* anchor_s, const float* anchor_r, int n, const int* __restrict__ lengths, float* dg, int B, int T, int H,
-                                                             int runs) {
+__global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* rq, const float* rk, int blocks, const float* anchor_s, const float* anchor_r, int n,
+                                                             const int* __restrict__ lengths, float* dg, int B, int T, int H, int runs) {
     __shared__ double part[kAnchor / 32], whole[kAnchor / 32];
     const int run = blockIdx.x % runs, bh = blockIdx.x / runs, h = bh % H, b = bh / H;
     const int t = run * kAnchor + (kAnchor - 1 - threadIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;      // from the last token on
@@ -421,7 +426,7 @@ __global__ void __launch_bounds__(256) attn_share_kernel(const float* p0, const 
 // ------------------------------------------------------------------------------------------------
 // One token.  The state is read and written once and nothing else is large: a CTA owns a head's state rows (or, where
 // there are few heads, some of its columns), a warp every eighth row of it, all of a thread's rows requested
-// before the first is used.
+// before the first is used.  256x16x128x128: 537 MB in 90 us, 6.0 TB/s (92 % of a copy's rate); 1x8x64x64: 6 us, a launch and one round trip.
 // ------------------------------------------------------------------------------------------------
 template <typename io_t, int NV>      // NV columns a lane
 __global__ void __launch_bounds__(256) attn_step_kernel(AttnTensor q, AttnTensor k, AttnTensor v, const float* __restrict__ g, long long gb, long long gh, float scale, int H, int K, int V,

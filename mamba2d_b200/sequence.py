@@ -37,7 +37,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
     Returns:
         o (B, T, H, V) in ``v.dtype``, or ``(o, state)``.
     Differentiable in q, k, v, log_decay and initial_state, through o and the state.  A token that is not finite
-    may spoil the outputs of up to 127 tokens before it, besides all later ones of its sequence and head.
+    may spoil the outputs of up to 127 tokens before it, besides all later ones of its sequence and head.  Gradients of
+    gradients (``create_graph``) raise.
     """
     o, state = _lib.entry().linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
     return (o, state) if return_state else o
@@ -67,7 +68,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None):
             (tokens, heads * size) with ``groups = heads``.
         weight, bias: (C,) or None; float32, or both of x's type.
         act: None, "silu" or "gelu" (erf form, as the block's ``act2``, models/mamba2d.py:169).
-    Differentiable in x, weight and bias.
+    Differentiable in x, weight and bias, once (``create_graph`` raises).
     """
     if act not in _ACTS:
         raise ValueError(f"Unknown activation, got {act}...")
@@ -82,7 +83,8 @@ def clip_norm_(tensors, max_norm, error_if_nonfinite=False):
 
     The factor is ``max_norm / (norm + 1e-6)``, at most 1; an infinite norm makes finite values zero and infinite ones
     NaN, a NaN spoils everything.  Two launches for up to 512 tensors; nothing is written where the factor is 1.  The sum
-    is taken in an order that does not change, in float64 beyond a thread's share of 32 KB.
+    is taken in an order that does not change, in float64 beyond a thread's share of 32 KB (squares in float32: a value
+    beyond 1.8e19 makes the norm infinite).
 
     Args:
         tensors: one or several; float32 or bfloat16, on one device, without gaps; they share no memory.
