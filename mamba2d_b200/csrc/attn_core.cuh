@@ -55,6 +55,8 @@ struct AttnLaunch {
     int B, T, H;
     int nseg, seg_len, runs;
     int join_here;            // the kernel joins the segments before its own, no launch has
+    int parts, part_len;      // tcgen05 form where segments are joined so: states are those of the segments' parts, of all segments
+                              // but the one that nothing comes after: (B,H,(nseg - 1) parts) of them.  Else one part a segment, of all.
     int seg_columns;          // segments' states have a column's rows next to one another, else a row's columns
 };
 

@@ -200,9 +200,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     const int ci = blockIdx.x % L.cores, unit = blockIdx.x / L.cores;
     const AttnCore& k = a.core[ci];
     const bool dots = MODE == kTcFine && k.dots, fine = dots, f32_out = (MODE == kTcHeads || MODE == kTcFine) && k.out_f32;
-    const int seg = unit % a.nseg, bh = unit / a.nseg, h = bh % a.H, b = bh / a.H;
+    const int states = a.join_here ? (a.nseg - 1) * a.parts : a.nseg, units = STATE_ONLY ? states : a.nseg;
+    const int seg = unit % units, bh = unit / units, h = bh % a.H, b = bh / a.H;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rev = k.rev;
-    const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
+    const int len = attn_length(a, b);
+    int t_lo = seg * a.seg_len, t_hi = t_lo + a.seg_len;
+    if (STATE_ONLY && a.join_here) {
+        const int from = (seg / a.parts + rev) * a.seg_len;
+        t_lo = from + seg % a.parts * a.part_len;
+        t_hi = min(from + a.seg_len, t_lo + a.part_len);
+    }
+    t_hi = min(a.T, t_hi);
     const int active = max(0, min(len, t_hi) - t_lo), chunks = (active + kTc - 1) / kTc;         // the others hold nothing
 
     TcSmall& small = *reinterpret_cast<TcSmall*>(tc_smem_raw + lay.small);
@@ -450,8 +458,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         }
         // a few segments: each joins the states of those before it itself, a launch less
         if (!STATE_ONLY && a.join_here && have_row)
-            for (int j = rev ? a.nseg - 1 : 0; j != seg; j += rev ? -1 : 1) {
-                const size_t at = (size_t)bh * a.nseg + j;
+            for (int j = rev ? states - 1 : 0; rev ? j >= seg * a.parts : j < seg * a.parts; j += rev ? -1 : 1) {
+                const size_t at = (size_t)bh * states + j;
                 const float decay = ex2(k.seg_decay[at]);
                 const float* own = k.seg_state + at * k.Kd * k.Vd + r + (size_t)v0 * k.Kd;
 #pragma unroll
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             if (!STATE_ONLY && !rev) keep(t0, it == chunks - 1 ? t_hi : t0 + kTc);
         }
         if constexpr (STATE_ONLY) {
-            put(k.seg_state + ((size_t)bh * a.nseg + seg) * k.Kd * k.Vd, 1, k.Kd);
+            put(k.seg_state + ((size_t)bh * states + seg) * k.Kd * k.Vd, 1, k.Kd);
         } else {
             if (!chunks) keep(behind, t_hi);
             if (k.fin.p && seg == (rev ? 0 : a.nseg - 1)) {
@@ -699,7 +707,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kTabFull));
         }
-        if (STATE_ONLY && lane == 0) k.seg_decay[(size_t)bh * a.nseg + seg] = (float)whole;
+        if (STATE_ONLY && lane == 0) k.seg_decay[(size_t)bh * states + seg] = (float)whole;
     }
 
     __syncthreads();

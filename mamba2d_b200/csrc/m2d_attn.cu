@@ -559,6 +559,16 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     // Joined by the kernels that start from them, or by a launch.  tcgen05 form, two segments: 128 us against 139 with a launch; 18: a
     // CTA would read up to 17 states one after another.  The other form, four segments of single chunks: 16 us against 27, 11 and 5: 166 against 182.
     p.a.join_here = p.a.nseg > 1 && p.a.nseg <= (tc ? 4 : 12);
+    // Nothing needs the own state of the last segment: where the others leave half of the GPU free (two segments), their states are
+    // computed in parts (of two chunks at least, four states at most to read): 4x4096x16x128 131 -> 121 us.
+    int states = p.a.nseg;
+    p.a.parts = 1;
+    if (tc && p.a.join_here) {
+        const int per = p.a.seg_len / 128, others = p.a.nseg - 1;
+        p.a.parts = (int)std::max<long long>(1, std::min<long long>({(long long)sm_count() / ((long long)d->B * d->H * p.cores * others), per / 2, 4 / others}));
+        p.a.part_len = (per + p.a.parts - 1) / p.a.parts * 128;
+        states = others * p.a.parts;
+    }
     auto take = [&](size_t n) {
         const size_t at = p.bytes;
         p.bytes += (n + 255) / 256 * 256;
@@ -567,8 +577,8 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     const size_t bh = (size_t)d->B * d->H, kv = (size_t)d->K * d->V, tokens = bh * d->T;
     if (p.a.nseg > 1)
         for (int i = 0; i < p.cores; ++i) {
-            p.at_seg[i] = take(4 * bh * p.a.nseg * kv);
-            p.at_decay[i] = take(4 * bh * p.a.nseg);
+            p.at_seg[i] = take(4 * bh * states * kv);
+            p.at_decay[i] = take(4 * bh * states);
         }
     if (bwd && d->d_log_decay) {
         for (size_t& at : p.at_dots) at = take(4 * tokens * p.dot_blocks);
@@ -621,7 +631,7 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
     auto kern = attn_tc_kernel<KD, VD, MODE>;
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3((unsigned)(d->B * d->H * p.a.nseg * count));
+    c.gridDim = dim3((unsigned)(d->B * d->H * (MODE == kTcStateOnly && p.a.join_here ? (p.a.nseg - 1) * p.a.parts : p.a.nseg) * count));
     c.blockDim = dim3(kTcThreads);
     c.dynamicSmemBytes = smem;
     c.stream = st;
