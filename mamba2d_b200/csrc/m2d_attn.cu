@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
 }
 
 // The decay's gradient from the dots and the anchors: suffix sums over a run, and <S, R> of its two kept states (n elements each), which
-// is what it reads: 71 MB at 8x2048x16x128, 21 us (a launch of its own for <S, R>: 16 and 7 us).
+// is what it reads: 71 MB at 8x2048x16x128, 18 us (a launch of its own for <S, R>: 16 and 7 us).
 // Dots: [blocks][B][T][H], one of dq and one of dk.
 __global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* rq, const float* rk, int blocks, const float* anchor_s, const float* anchor_r, int n,
                                                              const int* __restrict__ lengths, float* dg, int B, int T, int H, int runs) {
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kAnchor) attn_decay_kernel(const float* rq, co
     let_follow();
     follow_wait();
     if (n % 4 == 0) {
-#pragma unroll 4
+#pragma unroll 8
         for (int i = threadIdx.x; i < n / 4; i += kAnchor) {
             const float4 x = reinterpret_cast<const float4*>(s)[i], y = reinterpret_cast<const float4*>(r)[i];
             e = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, e))));
