@@ -86,6 +86,12 @@ typedef CUresult (*tc_encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 inline tc_encode_fn tc_encoder() {
+    // (the encoder wants a context, which a thread has only after its first call of the runtime that needs one)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
     static tc_encode_fn fn = []() -> tc_encode_fn {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;

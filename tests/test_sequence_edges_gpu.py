@@ -195,3 +195,18 @@ def test_a_training_step_with_clipped_gradients():
     for old, p, g in zip(model.parameters(), nets[0].parameters(), grads):
         want = old.detach().double() - 0.5 * (0.05 / (total + 1e-6)) * g.double()
         assert float((p.detach().double() - want).abs().max()) < 1e-6
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_a_thread_that_has_not_used_the_gpu(dt):
+    """A call that allocates nothing new is the first thing a thread does with the device (an autograd thread's first
+    backward pass, a server's worker)."""
+    import threading
+    args = make(2, 700, 2, 1, 64, 64, dt, state=True)
+    run = lambda: linear_attention(*args[:4], initial_state=args[4], return_state=True)  # noqa: E731
+    want = [t.clone() for t in run()]
+    got = []
+    thread = threading.Thread(target=lambda: got.extend(run()))
+    thread.start()
+    thread.join()
+    assert len(got) == 2 and all(torch.equal(x, y) for x, y in zip(got, want))
