@@ -23,10 +23,7 @@
 //
 // Measured, forward at 8x2048x16x128: 84 us for 128 CTAs of 16 chunks, 10000 cycles a chunk: the tensor cores are busy for 29 % of them,
 // the schedulers issue in 26 %, and what most warps wait for, besides each other, is instructions (1.9 of the 6 cycles between
-// two instructions of a warp).  The bytes would take 34 us.  With dots and anchors 235 us for dq and dk (256 CTAs in two waves), dv 83.
-//
-// `fine` (wanted where the decay's gradient is): P and St also in two parts each, so that the dots that out is summed
-// into are exact to 2^-17 like the states that they meet.
+// two instructions of a warp).  The bytes would take 34 us.
 //
 // Every wait is bounded: one that gives up makes all of the CTA's roles leave, its rows become NaN, and a word in host memory
 // says so.
@@ -144,22 +141,20 @@ struct alignas(16) TcSmall {
 
 // What a launch is for.  kTcPlain: bf16 out and nothing else, the least code (20 warps in five roles miss the instruction caches
 // often: with the branches of the others it takes 104 us where it takes 85).  kTcHeads: out in fp32, head by head.
-// kTcFine: dots and anchors, in two parts.
-enum TcMode { kTcPlain, kTcHeads, kTcFine, kTcStateOnly };
+enum TcMode { kTcPlain, kTcHeads, kTcStateOnly };
 
-// Shared memory: St in bf16 (one or two parts), the second part of u y, tiles, out's tile.  (KD = 64: (4) computes 128 rows; the upper
+// Shared memory: St in bf16, the second part of u y, tiles, out's tile.  (KD = 64: (4) computes 128 rows; the upper
 // 64, of whatever lies behind y, are not used, and a tile lies there.)  Tiles of x, y, z: x first, whose tile is held longest, z
 // last, which is needed last; out's own tile before third ones.
 struct TcLayout {
     int n[3] = {1, 1, 1};                     // tiles of x, y, z in flight
     bool own_stage = false;                   // out has a tile of its own, else it goes through x's
-    uint32_t s_lo = 0, y_lo = 0, ring[3] = {}, stage = 0, small = 0;
+    uint32_t y_lo = 0, ring[3] = {}, stage = 0, small = 0;
     __host__ __device__ constexpr TcLayout(int KD, int VD, TcMode mode) {
         const bool state_only = mode == kTcStateOnly;
         const uint32_t tile[3] = {(uint32_t)kTc * KD * 2, (uint32_t)kTc * KD * 2, (uint32_t)kTc * VD * 2};
         if (state_only) n[0] = 0;
-        s_lo = state_only ? 0 : KD * VD * 2;
-        y_lo = state_only ? 0 : s_lo * (mode == kTcFine ? 2 : 1);
+        y_lo = state_only ? 0 : KD * VD * 2;
         uint32_t bytes = y_lo + (state_only ? 2 : 1) * tile[0] + n[0] * tile[0] + tile[1] + tile[2];
         const uint32_t most = (uint32_t)(kMaxSmem - sizeof(TcSmall));
         for (int round = 1; round < kTcTiles; ++round) {
@@ -199,7 +194,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     const AttnLaunch& a = L.a;
     const int ci = blockIdx.x % L.cores, unit = blockIdx.x / L.cores;
     const AttnCore& k = a.core[ci];
-    const bool dots = MODE == kTcFine && k.dots, fine = dots, f32_out = (MODE == kTcHeads || MODE == kTcFine) && k.out_f32;
+    constexpr bool f32_out = MODE == kTcHeads;
     const int states = a.join_here ? (a.nseg - 1) * a.parts : a.nseg, units = STATE_ONLY ? states : a.nseg;
     const int seg = unit % units, bh = unit / units, h = bh % a.H, b = bh / a.H;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rev = k.rev;
@@ -215,7 +210,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 
     TcSmall& small = *reinterpret_cast<TcSmall*>(tc_smem_raw + lay.small);
     TcTable& tab = small.tab;
-    const uint32_t smem0 = smem_u32(tc_smem_raw), s_hi = smem0, s_lo = smem0 + lay.s_lo, y_lo = smem0 + lay.y_lo;
+    const uint32_t smem0 = smem_u32(tc_smem_raw), s_hi = smem0, y_lo = smem0 + lay.y_lo;
     const uint32_t bar0 = smem_u32(small.bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
     enum { X, Y, Z };
@@ -349,11 +344,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 #pragma unroll
                     for (int c = 0; c < 16; ++c) p[c] = pack_bf16x2(v[2 * c], v[2 * c + 1]);
                     tmem_st16(at, p);
-                    if (fine) {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) p[c] = pack_bf16x2(v[2 * c] - __uint_as_float(p[c] << 16), v[2 * c + 1] - __uint_as_float(p[c] & 0xffff0000u));
-                        tmem_st16(at + 16, p);
-                    }
                 }
                 if (__builtin_expect(!mild, 0)) {                 // O2 -> w O2
                     const float c = tab.f[r], w = rev ? ex2((tab.end.x - c) + (tab.end.y - e)) : ex2(c + e);
@@ -379,18 +369,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 }
                 // O -> out
                 const bool row = t0 + r < t_hi, live = r < valid;
-                const __nv_bfloat16* const er = dots && live ? static_cast<const __nv_bfloat16*>(attn_at(k.e, b, h, 2)) + (long long)(t0 + r) * k.e.st + half * kHalf : nullptr;
                 const uint32_t stage = lay.own_stage ? smem0 + lay.stage : tile_at(X, it);
-                float sum = 0.f;
-                uint4 eg[kHalf / 8];                              // e's columns, on their way while (3) runs
-                if (MODE == kTcFine) {
-#pragma unroll
-                    for (int c = 0; c < kHalf; c += 8)
-                        if (er && half * kHalf + c < k.Vd) eg[c / 8] = __ldg(reinterpret_cast<const uint4*>(er + c));
-                }
                 if (!wait2(kO, it)) break;
                 tc_fence_after();
-#pragma unroll(MODE == kTcFine ? 2 : 1)
+#pragma unroll 1
                 for (int c0 = 0; c0 < kHalf; c0 += 32) {
                     float o[32];
                     const int col = half * kHalf + c0;
@@ -414,22 +396,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                                 p[c / 4 + 1] = make_float4(o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
                             }
                     }
-                    if (MODE == kTcFine && er) {
-#pragma unroll
-                        for (int c = 0; c < 32; c += 8)
-                            if (col + c < k.Vd) {
-                                const uint4 g = eg[(c0 + c) / 8];
-                                const uint32_t gg[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) sum = fmaf(o[c + 2 * i], __uint_as_float(gg[i] << 16), fmaf(o[c + 2 * i + 1], __uint_as_float(gg[i] & 0xffff0000u), sum));
-                            }
-                    }
                 }
                 tc_fence_before();
                 async_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(kOFree));
-                if (dots && row) k.dots[(((size_t)half * a.B + b) * a.T + t0 + r) * a.H + h] = sum;
             }
         }
     } else if (warp < 16) {
@@ -484,15 +455,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 }
             }
         };
-        // St before (rev) or after the chunk at t0, if that ends a run; also of the chunks that hold nothing
-        auto keep = [&](int from, int to) {
-            for (int t0 = from; MODE == kTcFine && k.anchors && t0 < to; t0 += kTc)
-                if ((t0 + kTc) % kAnchor == 0 || t0 + kTc >= a.T) put(k.anchors + ((size_t)bh * a.runs + t0 / kAnchor) * k.Kd * k.Vd, 1, k.Kd);
-        };
-        const int behind = t_lo + chunks * kTc;
         for (int it = 0; it < chunks; ++it) {
             const int t0 = chunk_at(it), valid = min(kTc, len - t0);
-            if (!STATE_ONLY && rev) keep(t0, it ? t0 + kTc : t_hi);
             if (!wait(bar(kTabFull), it & 1)) break;
             const float u = !STATE_ONLY && r < valid ? tab.u[r] : 0.f, whole = tab.whole, copy = tab.copy;
             __syncwarp();
@@ -505,15 +469,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 if (r < KD) {
 #pragma unroll
                     for (int c = 0; c < kHalf / 8; ++c) {
-                        uint32_t hi[4], lo[4];
+                        uint32_t hi[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float s0 = copy * S[8 * c + 2 * i], s1 = copy * S[8 * c + 2 * i + 1];
-                            hi[i] = pack_bf16x2(s0, s1);
-                            if (fine) lo[i] = pack_bf16x2(s0 - __uint_as_float(hi[i] << 16), s1 - __uint_as_float(hi[i] & 0xffff0000u));
-                        }
+                        for (int i = 0; i < 4; ++i) hi[i] = pack_bf16x2(copy * S[8 * c + 2 * i], copy * S[8 * c + 2 * i + 1]);
                         sts(piece(s_hi, KD, r, v0 / 8 + c), hi[0], hi[1], hi[2], hi[3]);
-                        if (fine) sts(piece(s_lo, KD, r, v0 / 8 + c), lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
                 async_fence();
@@ -534,12 +493,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(kO + (it & 1)));
             }
-            if (!STATE_ONLY && !rev) keep(t0, it == chunks - 1 ? t_hi : t0 + kTc);
         }
         if constexpr (STATE_ONLY) {
             put(k.seg_state + ((size_t)bh * states + seg) * k.Kd * k.Vd, 1, k.Kd);
         } else {
-            if (!chunks) keep(behind, t_hi);
             if (k.fin.p && seg == (rev ? 0 : a.nseg - 1)) {
                 if (*abort) {
 #pragma unroll
@@ -627,22 +584,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 }
                 if (!wait(full(X, it), turn(X, it)) || !wait(bar(kS), ph)) break;
                 tc_fence_after();
-                const uint32_t x = desc_lo(tile_at(X, it), 16), sh = desc_lo(s_hi, KD * 128), sl = desc_lo(s_lo, KD * 128);
+                const uint32_t x = desc_lo(tile_at(X, it), 16), sh = desc_lo(s_hi, KD * 128);
                 auto xk = [&](int k) { return x + (((k / 4) * kTcBlock + (k % 4) * 32) >> 4); };
                 umma_chain<i2, false, KD / 16>(on, tm + kO0, xk, [&](int k) { return sh + k * 128; });
-                if (fine) umma_chain<i2, true, KD / 16>(on, tm + kO0, xk, [&](int k) { return sl + k * 128; });
                 commit_if(on, bar(kMma2));
                 if (lay.own_stage) commit_if(on, empty(X, it));
                 if (!wait(full(Z, it), turn(Z, it)) || !wait(bar(kP), ph)) break;
                 if (len - chunk_at(it) < kTc && !wait2(kY, it)) break;          // z's last rows have been cleared
                 tc_fence_after();
-                const uint32_t z = desc_lo(tile_at(Z, it), kTcBlock), p = uniform(tm + 128 * ph);       // (a block's first parts, then its second parts: 16 columns each)
+                const uint32_t z = desc_lo(tile_at(Z, it), kTcBlock), p = uniform(tm + 128 * ph);       // (a block of 32 columns is in its first 16)
 #pragma unroll
                 for (int k = 0; k < kTc / 16; ++k) umma_ts<i2, true>(on, tm + kO0, p + (k / 2) * 32 + (k % 2) * 8, z + k * 128);
-                if (fine) {
-#pragma unroll
-                    for (int k = 0; k < kTc / 16; ++k) umma_ts<i2, true>(on, tm + kO0, p + (k / 2) * 32 + (k % 2) * 8 + 16, z + k * 128);
-                }
                 commit_if(on, bar(kO + (it & 1)));
                 commit_if(on, empty(Z, it));
             }
@@ -721,7 +673,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                         if (f32_out) static_cast<float*>(k.out)[at + c] = v;
                         else static_cast<__nv_bfloat16*>(k.out)[at + c] = __float2bfloat16_rn(v);
                     }
-                    if (dots && lane < 2) k.dots[(((size_t)lane * a.B + b) * a.T + t) * a.H + h] = v;
                 }
             };
             if (t_lo + chunks * kTc < t_hi) fill(t_lo + chunks * kTc, t_hi, 0.f);

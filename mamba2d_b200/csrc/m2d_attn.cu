@@ -598,6 +598,9 @@ static bool tc_applies(const m2d_attn_desc* d, bool bwd) {
         return aligned(t.data) && stride(d->B, t.batch) && stride(d->T, t.token) && stride(heads, t.head);
     };
     if (!fits(d->q, d->G) || !fits(d->k, d->G) || !fits(d->v, d->H)) return false;
+    // The decay's gradient sums dots of 512 tokens that cancel: operands in two bf16 parts left it at up to 4e-5 (2x1000x4x128), split
+    // tf32 ones at 1e-6.
+    if (bwd && d->d_log_decay) return false;
     return bwd ? fits(d->d_o, d->H) && aligned(d->d_q) && aligned(d->d_k) && aligned(d->d_v) : aligned(d->o);
 }
 
@@ -672,9 +675,8 @@ static int launch_any(const AttnPlan& p, cudaStream_t st) {
 }
 static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t st) {
     if (p.tc) {
-        // dq and dk have (V,K) states, dv a (K,V) one: one launch where the kernel is the same; not where dv would run in the
-        // kernel of those with dots, which takes twice as long for a chunk
-        const bool together = p.cores == 1 || ((d->K <= 64) == (d->V <= 64) && !p.a.core[0].dots && !p.a.core[0].out_f32);
+        // dq and dk have (V,K) states, dv a (K,V) one: one launch where the kernel is the same
+        const bool together = p.cores == 1 || ((d->K <= 64) == (d->V <= 64) && !p.a.core[0].out_f32);
         const int counts[2] = {together ? p.cores : 2, together ? 0 : 1};
         for (int pass = p.a.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
             for (int i = 0; i < 2; ++i) {
@@ -682,7 +684,6 @@ static int launch_core(const m2d_attn_desc* d, const AttnPlan& p, cudaStream_t s
                 const int first = i ? counts[0] : 0;
                 const AttnCore& c = p.a.core[first];                // (dv, which wants least, is never the first of several)
                 const int rc = !pass ? launch_tc<kTcStateOnly>(d, p, first, counts[i], st)
-                               : c.dots ? launch_tc<kTcFine>(d, p, first, counts[i], st)
                                : c.out_f32 ? launch_tc<kTcHeads>(d, p, first, counts[i], st) : launch_tc<kTcPlain>(d, p, first, counts[i], st);
                 if (rc != M2D_OK) return rc;
             }
