@@ -34,7 +34,8 @@ struct Split {
 // acc[n] += A (16 x 8) B_n (8 x 8) over steps of 8 in [from, to), n < NT; fa(kk, i): the four values of A's fragment, fb(kk, n, i):
 // the two of B's.  (The unit cuts off what it adds to an accumulator: the small products have one of their own, which leaves the large
 // ones a third of the steps.  One of the three products for all n before the next: those of one accumulator wait for one another.)
-template <int NT, typename FA, typename FB>
+// A1, B1: A's or B's values are bf16, exact in one part; the products with its second one are left out.
+template <int NT, bool A1, bool B1, typename FA, typename FB>
 __device__ __forceinline__ void mma_chain(float (&acc)[NT][4], int from, int to, FA fa, FB fb) {
     float low[NT][4] = {};
 #pragma unroll 2
@@ -42,22 +43,32 @@ __device__ __forceinline__ void mma_chain(float (&acc)[NT][4], int from, int to,
         unsigned ah[4], al[4], bh[NT][2], bl[NT][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const Split s(fa(kk, i));
-            ah[i] = s.hi; al[i] = s.lo;
+            if constexpr (A1) {
+                ah[i] = __float_as_uint(fa(kk, i));
+            } else {
+                const Split s(fa(kk, i));
+                ah[i] = s.hi; al[i] = s.lo;
+            }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const Split s(fb(kk, n, i));
-                bh[n][i] = s.hi; bl[n][i] = s.lo;
+                if constexpr (B1) {
+                    bh[n][i] = __float_as_uint(fb(kk, n, i));
+                } else {
+                    const Split s(fb(kk, n, i));
+                    bh[n][i] = s.hi; bl[n][i] = s.lo;
+                }
             }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_tf32(low[n], ah, bl[n][0], bl[n][1]);
+        for (int n = 0; n < NT; ++n)
+            if constexpr (!B1) mma_tf32(low[n], ah, bl[n][0], bl[n][1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_tf32(acc[n], ah, bh[n][0], bh[n][1]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_tf32(low[n], al, bh[n][0], bh[n][1]);
+        for (int n = 0; n < NT; ++n)
+            if constexpr (!A1) mma_tf32(low[n], al, bh[n][0], bh[n][1]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -110,6 +121,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
     extern __shared__ float4 smem4[];
     const int kd = attn_pad(k.Kd), ks = kd + 4;
     constexpr int VS = VT + 8, NT = VT / 16;
+    constexpr bool kOne = sizeof(io_t) == 2;
     float* X = reinterpret_cast<float*>(smem4);
     float* Y = X + kC * ks;
     float* Z = Y + kC * ks;
@@ -239,7 +251,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             const int pn = (warp >> 2) * 32;
             float acc[4][4] = {};
             if (k.rev ? pn + 31 >= wm : pn <= wm + 15)
-                mma_chain<4>(acc, 0, kd, [&](int kk, int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
+                mma_chain<4, kOne, kOne>(acc, 0, kd, [&](int kk, int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
                              [&](int kk, int n, int i) { return Y[(pn + n * 8 + gq) * ks + kk + tq + i * 4]; });
 #pragma unroll
             for (int n = 0; n < 4; ++n)
@@ -254,9 +266,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
             __syncthreads();
             // out, 16 rows x VT / 2 columns a warp
             float o1[NT][4] = {}, o2[NT][4] = {};
-            mma_chain<NT>(o1, k.rev ? wm : 0, k.rev ? kC : wm + 16, [&](int kk, int i) { return P[(wm + gq + (i & 1) * 8) * kPStride + kk + tq + (i >> 1) * 4]; },
+            mma_chain<NT, false, kOne>(o1, k.rev ? wm : 0, k.rev ? kC : wm + 16, [&](int kk, int i) { return P[(wm + gq + (i & 1) * 8) * kPStride + kk + tq + (i >> 1) * 4]; },
                           [&](int kk, int n, int i) { return Z[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
-            mma_chain<NT>(o2, 0, kd, [&](int kk, int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
+            mma_chain<NT, kOne, false>(o2, 0, kd, [&](int kk, int i) { return X[(wm + gq + (i & 1) * 8) * ks + kk + tq + (i >> 1) * 4]; },
                           [&](int kk, int n, int i) { return S[(kk + tq + i * 4) * VS + wn + n * 8 + gq]; });
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -300,7 +312,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
         const float decay = *whole;
         for (int m = (warp & 3) * 16; m < kd && (it + 1 < chunks || last_wanted || run_end); m += 64) {
             float acc[NT][4] = {};
-            mma_chain<NT>(acc, 0, kC,
+            mma_chain<NT, false, kOne>(acc, 0, kC,
                           [&](int kk, int i) {
                               const int c = kk + tq + (i >> 1) * 4;
                               return Y[c * ks + m + gq + (i & 1) * 8] * u[c];
