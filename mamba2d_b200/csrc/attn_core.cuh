@@ -43,7 +43,7 @@ struct AttnCore {
     float s_intra, s_inter, s_update;
     float* dots;              // [column block][B][T][H], or nullptr
     AttnState init, fin;      // p may be nullptr
-    float* anchors;           // [B][H][runs][Kd Vd], or nullptr; in the order that a kernel likes, the same for dq and dk
+    float* anchors;           // [B][H][runs][Kd Vd], or nullptr; the same order for dq and dk
     float* seg_state;         // [B][H][segments][Kd Vd]
     float* seg_decay;         // [B][H][segments], log2
 };

@@ -555,7 +555,6 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     p.tc = tc;
     p.cores = bwd ? 3 : 1;
     int per_sm = 1;
-    p.dot_blocks = 2;                  // (the tcgen05 form's threads have half of the columns each)
     if (!tc) {
         const int big = bwd ? std::max(d->K, d->V) : d->K, out = bwd ? big : d->V;
         p.VT = big > 192 ? 32 : 64;
@@ -566,7 +565,7 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
     }
     p.a.seg_columns = tc;
     // lengths: only the GPU knows how much of T there is, so twice as many as run at once (6x1395x3x64 fp32, training: 138 us for 153;
-    // the tcgen05 form's segments cost too much for that, 8x2048x16x128: 443 for 424)
+    // a segment of the tcgen05 form costs too much for that, 8x2048x16x128 forward: 19 us more)
     plan_segments(d, (long long)d->B * d->H * p.col_blocks * p.cores, per_sm * (d->lengths && !tc ? 2 : 1), tc ? 128 : 64, tc ? 4 : 1, &p.a);
     // Joined by the kernels that start from them, or by a launch.  tcgen05 form, two segments: 128 us against 139 with a launch; 18: a
     // CTA would read up to 17 states one after another.  The other form, four segments of single chunks: 16 us against 27, 11 and 5: 166 against 182.
@@ -611,7 +610,7 @@ static bool tc_applies(const m2d_attn_desc* d, bool bwd) {
     };
     if (!fits(d->q, d->G) || !fits(d->k, d->G) || !fits(d->v, d->H)) return false;
     // The decay's gradient sums dots of 512 tokens that cancel: operands in two bf16 parts left it at up to 4e-5 (2x1000x4x128), split
-    // tf32 ones at 1e-6.
+    // tf32 ones leave it at 1e-6.  (8x2048x16x128, training: 3525 us, 430 with the parts.)
     if (bwd && d->d_log_decay) return false;
     return bwd ? fits(d->d_o, d->H) && aligned(d->d_q) && aligned(d->d_k) && aligned(d->d_v) : aligned(d->o);
 }
@@ -723,7 +722,9 @@ static int check_workspace(const m2d_attn_desc* d, size_t bytes) {
     return d->workspace && d->workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(d->workspace) & 255) == 0 ? M2D_OK : M2D_ERR_WORKSPACE;
 }
 // What either form may need: a query does not depend on the tensors' addresses.
-static size_t attn_workspace(const m2d_attn_desc* d, bool bwd) { return std::max(plan_attn(d, bwd, false).bytes, d->dtype == M2D_BF16 ? plan_attn(d, bwd, true).bytes : 0); }
+static size_t attn_workspace(const m2d_attn_desc* d, bool bwd) {
+    return std::max(plan_attn(d, bwd, false).bytes, d->dtype == M2D_BF16 && !(bwd && d->d_log_decay) ? plan_attn(d, bwd, true).bytes : 0);
+}
 
 }  // namespace m2d
 

@@ -210,3 +210,15 @@ def test_a_thread_that_has_not_used_the_gpu(dt):
     thread.start()
     thread.join()
     assert len(got) == 2 and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("B,T,H,G,K,V", [(2, 1000, 4, 4, 128, 128), (2, 1500, 4, 1, 48, 64)])
+def test_the_decays_gradient_of_bf16_tensors_has_fp32s_precision(B, T, H, G, K, V):
+    """It is float32: 1e-5 of its 2-norm (split products leave 2^-21 of each of up to 512 dots, whose sum is some tenth of
+    their magnitude), whatever the tensors are rounded to."""
+    q, k, v, d, s, _ = make(B, T, H, G, K, V, BF, state=True)
+    d_o = torch.randn(v.shape, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(BF)
+    leaf = d.clone().requires_grad_(True)
+    got, = torch.autograd.grad(linear_attention(q, k, v, leaf, initial_state=s), leaf, d_o)
+    _, _, want = seq_ref.attention_grads(q, k, v, d, K ** -0.5, s, None, d_o, None)
+    assert float((got.double() - want[3]).norm() / want[3].norm()) < 1e-5
