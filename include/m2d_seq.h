@@ -21,8 +21,8 @@ extern "C" {
  * everything before the token; a positive value grows the state and is not checked for).
  *
  * State, its gradient and that of the decay are fp32 whatever the tensors' type.  bf16 tensors with K and V of up to 128 in whole
- * 16-byte pieces, 16-byte aligned and with such strides, take a form on the tensor cores (tcgen05), all others, and backward passes
- * that want the decay's gradient, one for any size and more exact products.  Long sequences of few heads are cut into segments whose states the workspace holds; the workspace queries read the
+ * 16-byte pieces, 16-byte aligned and with such strides, take a form on the tensor cores (tcgen05), all others, and d_q and d_k
+ * where the decay's gradient is wanted, one for any size and with more exact products.  Long sequences of few heads are cut into segments whose states the workspace holds; the workspace queries read the
  * sizes, G, dtype and, for the backward pass, whether d_log_decay is given.  B * H up to 2^24, T below 2^31 - 2048.
  * A wait inside the tensor-core form that gives up makes its rows NaN and shows in m2d_take_wait_failure().
  */

@@ -550,10 +550,12 @@ struct AttnPlan {
     size_t smem = 0, bytes = 0;
     size_t at_seg[3] = {}, at_decay[3] = {}, at_dots[2] = {}, at_anchor[2] = {}, at_heads[2] = {};
 };
-static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc) {
+// Of the forward pass's one core, or of `cores` of the backward's; its scratch begins at `base`.
+static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc, int cores = 3, size_t base = 0) {
     AttnPlan p;
     p.tc = tc;
-    p.cores = bwd ? 3 : 1;
+    p.cores = bwd ? cores : 1;
+    p.bytes = base;
     int per_sm = 1;
     if (!tc) {
         const int big = bwd ? std::max(d->K, d->V) : d->K, out = bwd ? big : d->V;
@@ -609,9 +611,6 @@ static bool tc_applies(const m2d_attn_desc* d, bool bwd) {
         return aligned(t.data) && stride(d->B, t.batch) && stride(d->T, t.token) && stride(heads, t.head);
     };
     if (!fits(d->q, d->G) || !fits(d->k, d->G) || !fits(d->v, d->H)) return false;
-    // The decay's gradient sums dots of 512 tokens that cancel: operands in two bf16 parts left it at up to 4e-5 (2x1000x4x128), split
-    // tf32 ones leave it at 1e-6.  (8x2048x16x128, training: 3525 us, 430 with the parts.)
-    if (bwd && d->d_log_decay) return false;
     return bwd ? fits(d->d_o, d->H) && aligned(d->d_q) && aligned(d->d_k) && aligned(d->d_v) : aligned(d->o);
 }
 
@@ -723,7 +722,9 @@ static int check_workspace(const m2d_attn_desc* d, size_t bytes) {
 }
 // What either form may need: a query does not depend on the tensors' addresses.
 static size_t attn_workspace(const m2d_attn_desc* d, bool bwd) {
-    return std::max(plan_attn(d, bwd, false).bytes, d->dtype == M2D_BF16 && !(bwd && d->d_log_decay) ? plan_attn(d, bwd, true).bytes : 0);
+    size_t tc = 0;
+    if (d->dtype == M2D_BF16) tc = bwd && d->d_log_decay ? plan_attn(d, false, true, 1, plan_attn(d, true, false, 2).bytes).bytes : plan_attn(d, bwd, true).bytes;
+    return std::max(plan_attn(d, bwd, false).bytes, tc);
 }
 
 }  // namespace m2d
@@ -755,14 +756,19 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     int rc = check_attn(d, true);
     if (rc != M2D_OK) return rc;
     if (!d->d_o.data || !d->d_q || !d->d_k || !d->d_v) return M2D_ERR_NULL;
-    AttnPlan p = plan_attn(d, true, tc_applies(d, true));
+    // The decay's gradient sums dots of 512 tokens that cancel: dq and dk with operands in two bf16 parts left it at up to 4e-5
+    // (2x1000x4x128), split tf32 ones leave it at 1e-6.  (8x2048x16x128, training: 2650 us, 3525 with dv in this form too, 430 with the parts.)
+    const bool tc = tc_applies(d, true), apart = tc && d->d_log_decay;       // dv, which has no part in it, in the tcgen05 form
+    AttnPlan p = plan_attn(d, true, tc && !apart, apart ? 2 : 3), pv = p;
+    if (apart) pv = plan_attn(d, false, true, 1, p.bytes);
     if ((rc = check_workspace(d, attn_workspace(d, true))) != M2D_OK) return rc;
     fill_launch(d, p);
+    if (apart) fill_launch(d, pv);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     char* const ws = static_cast<char*>(d->workspace);
     const int per = d->H / d->G;
     const AttnTensor q = attn_tensor(d, d->q, per, d->K), k = attn_tensor(d, d->k, per, d->K), v = attn_tensor(d, d->v, 1, d->V), go = attn_tensor(d, d->d_o, 1, d->V);
-    AttnCore &dq = p.a.core[0], &dk = p.a.core[1], &dv = p.a.core[2];
+    AttnCore &dq = p.a.core[0], &dk = p.a.core[1], &dv = apart ? pv.a.core[0] : p.a.core[2];
     dq.x = go; dq.y = v; dq.z = k; dq.e = q; dq.rev = 0;
     dk.x = v; dk.y = go; dk.z = q; dk.e = k; dk.rev = 1;
     dv.x = k; dv.y = q; dv.z = go; dv.rev = 1;
@@ -786,6 +792,7 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     dk.init = dense_state(d, d->d_state_out, true);
     dv.init = dense_state(d, d->d_state_out, false);
     dv.fin = dense_state(d, d->d_state, false);
+    if (apart && (rc = launch_core(d, pv, st)) != M2D_OK) return rc;
     if ((rc = launch_core(d, p, st)) != M2D_OK) return rc;
     if (d->d_log_decay) {
         const unsigned n = (unsigned)(d->B * d->H * p.a.runs);
