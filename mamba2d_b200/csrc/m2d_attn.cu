@@ -796,7 +796,9 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     if ((rc = launch_core(d, p, st)) != M2D_OK) return rc;
     if (d->d_log_decay) {
         const unsigned n = (unsigned)(d->B * d->H * p.a.runs);
-if (!launch_following(attn_decay_kernel, dim3(n), dim3(kAnchor), 0, st, (const float*)dq.dots, (const float*)dk.dots, p.dot_blocks, (const float*)dq.anchors, (const float*)dk.anchors, d->K * d->V, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs)) return M2D_ERR_LAUNCH;
+        if (!launch_following(attn_decay_kernel, dim3(n), dim3(kAnchor), 0, st, (const float*)dq.dots, (const float*)dk.dots, p.dot_blocks,
+                              (const float*)dq.anchors, (const float*)dk.anchors, d->K * d->V, d->lengths, d->d_log_decay, d->B, d->T, d->H, p.a.runs))
+            return M2D_ERR_LAUNCH;
     }
     if (d->G != d->H) {
         const long long n = (long long)d->B * d->T * d->G * d->K;
