@@ -294,6 +294,13 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
     float2* const all = reinterpret_cast<float2*>(sums + (BWD ? 2 * a.C : 0));      // [groups]
     float2* const inbox = all + a.groups;                                           // [2][ranks][groups]
     int turn = 0;
+    // No CTA writes to another that has not begun: all arrive here, and wait for the rest behind the first image's requests.
+    bool met = PHASE > 0 || ranks == 1;
+    if (!met) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    auto meet = [&] {
+        if (!met) asm volatile("barrier.cluster.wait;" ::: "memory");
+        met = true;
+    };
     auto send = [&](int g, float2 v) {                          // (one thread per group)
         for (int q = 0; q < ranks; ++q) (ranks > 1 ? cluster.map_shared_rank(inbox, q) : inbox)[(turn * ranks + rank) * a.groups + g] = v;
     };
@@ -359,6 +366,7 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
                 cp_async16(xa + 16 * i, xg + i);
                 if (BWD) cp_async16(ga + 16 * i, dg + i);
             }
+            meet();
             cp_async_wait_all();
             __syncthreads();
         }
@@ -540,6 +548,7 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
         __syncthreads();                                        // the tile is free again
         turn ^= 1;
     }
+    meet();                                                     // (of a CTA without an image)
     if (PHASE == 0 && ranks > 1) cluster.sync();                // (no CTA leaves while another writes to it)
     if (BWD && PHASE == 0 && a.partial) {
         for (int i = tid; i < 2 * a.C; i += kNormThreads) a.partial[(size_t)blockIdx.x * 2 * a.C + i] = sums[i];
