@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_core_kernel(const __grid_co
     const int seg = blockIdx.x % a.nseg, bh = blockIdx.x / a.nseg, h = bh % a.H, b = bh / a.H;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     const int wm = (warp & 3) * 16, wn = (warp >> 2) * (VT / 2);
-    const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = min(a.T, t_lo + a.seg_len);
+    const int len = attn_length(a, b), t_lo = seg * a.seg_len, t_hi = t_lo + min(a.seg_len, a.T - t_lo);      // (t_lo + seg_len may lie beyond 2^31)
     const bool pairs = k.Vd % 2 == 0 && (reinterpret_cast<uintptr_t>(k.out) & 7) == 0;      // out may be written two columns at a time
     const int nv = min(VT, k.Vd - v0), chunks = (t_hi - t_lo + kC - 1) / kC;
     const io_t* const x = static_cast<const io_t*>(attn_at(k.x, b, h, sizeof(io_t)));
