@@ -277,7 +277,8 @@ public:
         const Tensor dx = at::empty(x.sizes(), x.options());
         d.d_x = dx.data_ptr();
         Tensor dw, db;
-        if ((w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())) {
+        // (asked of the inputs: a copy made here, where gradients are off, requires none)
+        if ((s[1].defined() && s[1].requires_grad()) || (s[2].defined() && s[2].requires_grad())) {
             const auto options = w.defined() ? w.options() : b.options();
             dw = at::empty({d.C}, options);
             db = at::empty({d.C}, options);

@@ -28,3 +28,46 @@ def test_clusters_that_begin_at_different_times(shape, groups, dt):
     close(ys[0], want.detach(), 2e-5)
     close(dxs[0], grad, 1e-4)
     assert all(torch.equal(ys[0], y) for y in ys) and all(torch.equal(dxs[0], d) for d in dxs)
+
+
+# a row a token, clusters, pieces, any shape (rows that are not whole 16-byte pieces)
+KINDS = [((300, 256), 4), ((5, 131, 64), 8), ((40, 3136, 64), 16), ((3, 50, 30), 5)]
+
+
+def dense_and_not(C, dt):
+    """(weight, bias) pairs: every second value of a table, one value for all channels, neither."""
+    table, gain = (torch.randn(C, 2, device="cuda") * 0.5 + 1).to(dt), torch.full((1,), 0.75, device="cuda", dtype=dt)
+    return [(table[:, 0], table[:, 1]), (gain.expand(C), None), (gain.expand(C), table[:, 1]), (table[:, 0], gain.expand(C)), (None, table[:, 1]), (table[:, 0], None)]
+
+
+@pytest.mark.parametrize("dt,params", [(F32, F32), (BF, F32), (BF, BF)])
+@pytest.mark.parametrize("shape,groups", KINDS)
+def test_parameters_that_are_not_dense(shape, groups, dt, params):
+    """Their gradients are those of dense ones, whichever of the two is wanted."""
+    x, dy = torch.randn(shape, device="cuda").to(dt), torch.randn(shape, device="cuda").to(dt)
+    for pair in dense_and_not(shape[-1], params):
+        for wanted in ((True, True), (True, False), (False, True)):
+            if not any(w and t is not None for w, t in zip(wanted, pair)):
+                continue
+
+            def call(tensors):
+                y = group_norm(x, groups, *tensors, act="silu")
+                return torch.autograd.grad(y, [t for t in tensors if t is not None and t.requires_grad], dy, allow_unused=True)
+            strided = [t.detach().requires_grad_(w) if t is not None else None for t, w in zip(pair, wanted)]
+            dense = [t.detach().contiguous().requires_grad_(w) if t is not None else None for t, w in zip(pair, wanted)]
+            assert not all(t.is_contiguous() for t in strided if t is not None)
+            got, want = call(strided), call(dense)
+            assert len(got) == len(want)
+            for a, b in zip(got, want):
+                assert a is not None and torch.equal(a, b)
+
+
+def test_a_gain_that_all_channels_share_gets_its_gradient():
+    x = torch.randn(6, 50, 32, device="cuda")
+    gain, table = torch.tensor([0.75], device="cuda", requires_grad=True), torch.randn(32, 2, device="cuda", requires_grad=True)
+    y = group_norm(x, 4, gain.expand(32), table[:, 1])
+    y.square().sum().backward()
+    g, t = gain.detach().double().requires_grad_(True), table.detach().double().requires_grad_(True)
+    seq_ref.norm(x.double(), 4, g.expand(32), t[:, 1], 1e-5, None).square().sum().backward()
+    close(gain.grad, g.grad, 1e-4)
+    close(table.grad, t.grad, 1e-4)
