@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
     const size_t slice = kDirect ? 0 : (size_t)a.rows * cv;
     uint4* const xs = tile;
     uint4* const gs = tile + slice;
+    const float inv_per = 1.f / (float)a.per;
     const bool fold = cv < 32 && (cv & (cv - 1)) == 0;          // lanes that hold the same channels are summed in the warp
     const int parts = fold ? kNormWarps : rp;
     float* const red = reinterpret_cast<float*>(tile + slice * (BWD ? 2 : 1));      // [parts][C]
@@ -373,7 +374,8 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
         auto x_at = [&](int i) { return kDirect ? __ldg(xg + i) : xs[i]; };
         auto g_at = [&](int i) { return kDirect ? __ldg(dg + i) : gs[i]; };
         const float count = (float)((double)a.S * a.per);
-        auto group_of = [&](int c) { return c / a.per; };
+        // c / per, without a division: half a channel from the next whole number at least, of at most 2048
+        auto group_of = [&](int c) { return (int)(((float)c + 0.5f) * inv_per); };
         if constexpr (!BWD) {
             float2 A[V::pairs], B[V::pairs];
             if constexpr (PHASE < 2) {
@@ -398,21 +400,28 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
                         }
                     }
                 }
-                // sum -> that of x; sq -> that about the thread's mean, which pivot becomes (negated)
+                // sum -> that of x - base, base the group's first value in this CTA (of x itself, equal values far from zero gave a
+                // mean some steps away from theirs); sq -> that about the thread's mean, which pivot becomes (negated)
+                auto base = [&](int first) {
+                    if (rows == 0) return 0.f;
+                    if constexpr (kDirect) return load1(reinterpret_cast<const io_t*>(xg), first);
+                    else if constexpr (sizeof(io_t) == 4) return reinterpret_cast<const float*>(xs)[first];
+                    else return bf16_bits_to_float(reinterpret_cast<const unsigned short*>(xs)[first]);
+                };
                 const float each = n_own > 0.f ? 1.f / n_own : 0.f;
 #pragma unroll
                 for (int i = 0; i < V::pairs; ++i) {
                     const float2 d = __fmul2_rn(sum[i], make_float2(each, each));
                     sq[i] = __ffma2_rn(make_float2(-sum[i].x, -sum[i].y), d, sq[i]);      // (below zero by rounding, at most)
                     pivot[i] = make_float2(pivot[i].x - d.x, pivot[i].y - d.y);
-                    sum[i] = __fmul2_rn(pivot[i], make_float2(-n_own, -n_own));
+                    sum[i] = __fmul2_rn(__fadd2_rn(pivot[i], make_float2(base(group_of(c0 + 2 * i) * a.per), base(group_of(c0 + 2 * i + 1) * a.per))), make_float2(-n_own, -n_own));
                 }
                 channel_sums(sum, 0);
                 // this CTA's groups: mean, then sum of squares about it
                 const float here = 1.f / fmaxf((float)rows * (float)a.per, 1.f);
                 for (int g = tid >> 5; g < a.groups; g += kNormWarps) {
-                    const float v = over_group(g, [&](int c) { return chan[c]; });
-                    if ((tid & 31) == 0) all[g].x = v * here;
+                    const float first = base(g * a.per), v = over_group(g, [&](int c) { return chan[c]; });
+                    if ((tid & 31) == 0) all[g].x = fmaf(v, here, first);
                 }
                 __syncthreads();
 #pragma unroll
@@ -433,9 +442,9 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
                 receive();
                 for (int g = tid; g < a.groups; g += kNormThreads) {
                     const float2* const in = inbox + (size_t)turn * ranks * a.groups + g;
-                    float mean = 0.f, sq_all = 0.f;
-                    for (int q = 0; q < ranks; ++q) mean = fmaf(rows_of(q), in[q * a.groups].x, mean);
-                    mean /= (float)a.S;
+                    float mean = 0.f, sq_all = 0.f;              // (about the first CTA's, for the same reason)
+                    for (int q = 1; q < ranks; ++q) mean = fmaf(rows_of(q), in[q * a.groups].x - in[0].x, mean);
+                    mean = in[0].x + mean / (float)a.S;
                     for (int q = 0; q < ranks; ++q) {
                         const float2 v = in[q * a.groups];
                         const float d = v.x - mean;

@@ -71,3 +71,14 @@ def test_a_gain_that_all_channels_share_gets_its_gradient():
     seq_ref.norm(x.double(), 4, g.expand(32), t[:, 1], 1e-5, None).square().sum().backward()
     close(gain.grad, g.grad, 1e-4)
     close(table.grad, t.grad, 1e-4)
+
+
+@pytest.mark.parametrize("shape,groups,dt", [(s, g, dt) for s, g in (((1, 128, 64), 8), ((9, 300, 96), 32), ((200, 49, 64), 1), ((40, 3136, 64), 16), ((1, 700, 700, 16), 2))
+                                             for dt in (F32, BF)] + [((1, 700, 700, 12), 3, F32)])
+def test_images_of_one_value(shape, groups, dt):
+    """Every value the same, and no power of two: the mean is that value and the result the bias, whatever the number of
+    threads, CTAs and pieces that took part in the sum."""
+    w, b = torch.full((shape[-1],), 0.5, device="cuda"), torch.full((shape[-1],), 0.25, device="cuda")
+    for value in (1000.3, -0.7, 3e-5):
+        x = torch.full(shape, value, device="cuda").to(dt)
+        assert bool((group_norm(x, groups, w, b) == 0.25).all()), value
