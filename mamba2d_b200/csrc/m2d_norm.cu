@@ -295,6 +295,8 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
     float2* const all = reinterpret_cast<float2*>(sums + (BWD ? 2 * a.C : 0));      // [groups]
     float2* const inbox = all + a.groups;                                           // [2][ranks][groups]
     int turn = 0;
+    // (Short loops whose count only the launch knows are not unrolled: small images spend their time on fetching code that runs once,
+    // 14x14x320 fp32 9.6 -> 8.5 us, 2000x36x64 bf16 27.4 -> 23.5.)
     // No CTA writes to another that has not begun: all arrive here, and wait for the rest behind the first image's requests.
     bool met = PHASE > 0 || ranks == 1;
     if (!met) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
@@ -303,6 +305,7 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
         met = true;
     };
     auto send = [&](int g, float2 v) {                          // (one thread per group)
+#pragma unroll 1
         for (int q = 0; q < ranks; ++q) (ranks > 1 ? cluster.map_shared_rank(inbox, q) : inbox)[(turn * ranks + rank) * a.groups + g] = v;
     };
     auto receive = [&] { if (ranks > 1) cluster.sync(); else __syncthreads(); };
@@ -343,6 +346,7 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
     // a warp's sum over the channels of group g of value(c), in every lane
     auto over_group = [&](int g, auto value) {
         float v = 0.f;
+#pragma unroll 1
         for (int c = g * a.per + (tid & 31); c < (g + 1) * a.per; c += 32) v += value(c);
 #pragma unroll
         for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
@@ -443,8 +447,10 @@ __global__ void __launch_bounds__(kNormThreads, BWD ? 2 : 4) norm_image_kernel(c
                 for (int g = tid; g < a.groups; g += kNormThreads) {
                     const float2* const in = inbox + (size_t)turn * ranks * a.groups + g;
                     float mean = 0.f, sq_all = 0.f;              // (about the first CTA's, for the same reason)
+#pragma unroll 1
                     for (int q = 1; q < ranks; ++q) mean = fmaf(rows_of(q), in[q * a.groups].x - in[0].x, mean);
                     mean = in[0].x + mean / (float)a.S;
+#pragma unroll 1
                     for (int q = 0; q < ranks; ++q) {
                         const float2 v = in[q * a.groups];
                         const float d = v.x - mean;
