@@ -82,3 +82,45 @@ def test_images_of_one_value(shape, groups, dt):
     for value in (1000.3, -0.7, 3e-5):
         x = torch.full(shape, value, device="cuda").to(dt)
         assert bool((group_norm(x, groups, w, b) == 0.25).all()), value
+
+
+# rows that are not whole 16-byte pieces, images of many channels, a tensor that starts at an odd element
+ANY = [((1, 700, 700, 12), 3, 0), ((2, 40000, 30), 5, 0), ((3, 30000, 2), 1, 0), ((1, 300, 300, 64), 2, 1), ((1, 3000, 2056), 1, 0)]
+
+
+def odd_start(x, offset):
+    if not offset:
+        return x
+    flat = torch.empty(x.numel() + offset, dtype=x.dtype, device=x.device)
+    flat[offset:] = x.view(-1)
+    return flat[offset:].view(x.shape)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("shape,groups,offset", ANY)
+def test_large_mean_and_constant_groups_of_any_shape(shape, groups, offset, dt):
+    """As ``test_large_mean_and_constant_groups``, by the kernel for any shape."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(shape, generator=g, device="cuda") + 1000.0).to(dt)
+    constant = torch.full(shape, 1000.3, device="cuda").to(dt)
+    w, b = torch.full((shape[-1],), 0.5, device="cuda"), torch.full((shape[-1],), 0.25, device="cuda")
+    assert bool((group_norm(odd_start(constant, offset), groups, w, b) == 0.25).all())
+    y = group_norm(odd_start(x, offset), groups, w, b)
+    want = seq_ref.norm(x.double(), groups, w.double(), b.double(), 1e-5, None)
+    # the mean is off by up to 2^-24 of 1000, against a deviation of one
+    bound = 4e-4 + (want.abs() * 2.0 ** -8 if dt == BF else 0.0)
+    assert bool(((y.double() - want).abs() < bound).all())
+
+
+@pytest.mark.parametrize("shape,groups,offset", ANY)
+def test_gradients_that_cancel_in_any_shape(shape, groups, offset):
+    """The same dy everywhere: dx is zero, db the number of values.  What is left of dx is h times the mean of dh h, whose
+    terms are off by half a step of theirs: 2^-24 times a mean |h| of 0.8, times |h| < 6, below 3e-7; as much again where the
+    mean of x lies half a step off."""
+    x = odd_start(torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda"), offset).requires_grad_(True)
+    b = torch.zeros(shape[-1], device="cuda", requires_grad=True)
+    y = group_norm(x, groups, None, b)
+    dx, db = torch.autograd.grad(y, (x, b), torch.full_like(y, 1.0003))
+    assert float(dx.abs().max()) < 1e-6
+    want = 1.0003 * (x.numel() / shape[-1])
+    assert float((db.double() / want - 1).abs().max()) < 1e-6
