@@ -37,7 +37,7 @@ typedef struct m2d_attn_desc {
     uint32_t struct_bytes;         /* = sizeof(m2d_attn_desc) */
     int32_t dtype;                 /* m2d_dtype of q, k, v, o and their gradients */
     int32_t B, T, H, G, K, V;      /* G divides H */
-    uint32_t flags;                /* 0 or M2D_ATTN_* bits */
+    uint32_t flags;                /* 0 */
     float scale;
     m2d_attn_tensor q, k, v;       /* the latter with H heads */
     const float *log_decay;        /* log_decay[b * g_batch + t * g_token + h * g_head] */
@@ -56,8 +56,6 @@ typedef struct m2d_attn_desc {
     void *workspace;               /* scratch, 256-byte aligned */
     uint64_t workspace_bytes;
 } m2d_attn_desc;
-
-#define M2D_ATTN_CUDA_CORES 1      /* the form for any size and alignment where the tcgen05 form would be taken too */
 
 uint64_t m2d_attn_fwd_workspace(const m2d_attn_desc *desc);
 uint64_t m2d_attn_bwd_workspace(const m2d_attn_desc *desc);

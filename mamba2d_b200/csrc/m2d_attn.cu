@@ -512,7 +512,7 @@ static int check_attn(const m2d_attn_desc* d, bool ptrs) {
     if (!d) return M2D_ERR_NULL;
     if (d->struct_bytes != sizeof(m2d_attn_desc)) return M2D_ERR_ABI;
     if (d->dtype != M2D_F32 && d->dtype != M2D_BF16) return M2D_ERR_DTYPE;
-    if (d->flags & ~(uint32_t)M2D_ATTN_CUDA_CORES) return M2D_ERR_FLAGS;
+    if (d->flags) return M2D_ERR_FLAGS;
     if (d->B < 1 || d->T < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->K < 1 || d->V < 1 || d->K > M2D_ATTN_MAX_DIM || d->V > M2D_ATTN_MAX_DIM) return M2D_ERR_SHAPE;
     if (d->T > INT_MAX - 4 * kAnchor) return M2D_ERR_TOO_LARGE;      // (token numbers go up to the end of the last chunk)
     if ((int64_t)d->B * d->H > (1 << 24) || (int64_t)d->B * d->H * ((d->T + kAnchor - 1) / kAnchor) >= (1ll << 31)) return M2D_ERR_TOO_LARGE;
@@ -604,7 +604,7 @@ static AttnPlan plan_attn(const m2d_attn_desc* d, bool bwd, bool tc, int cores =
 
 // Whether the tcgen05 form takes the call: bf16, head sizes of whole 16-byte pieces up to 128, and tensors that TMA can address.
 static bool tc_applies(const m2d_attn_desc* d, bool bwd) {
-    if (d->dtype != M2D_BF16 || (d->flags & M2D_ATTN_CUDA_CORES) || d->K > 128 || d->V > 128 || d->K % 8 || d->V % 8 || !tc_encoder()) return false;
+    if (d->dtype != M2D_BF16 || d->K > 128 || d->V > 128 || d->K % 8 || d->V % 8 || !tc_encoder()) return false;
     auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     auto fits = [&](const m2d_attn_tensor& t, int heads) {
         auto stride = [](int n, int64_t s) { return n == 1 || (s > 0 && s % 8 == 0 && s < (1ll << 36)); };

@@ -48,13 +48,12 @@ void wrote(const Tensor& t) {
 struct Attn {
     Tensor q, k, v, g, state, lengths;        // as the kernels read them
     m2d_attn_desc d{};
-    Attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& state_, const Tensor& lengths_, double scale, int64_t flags)
+    Attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& state_, const Tensor& lengths_, double scale)
         : q(rows(q_)), k(rows(k_)), v(rows(v_)), g(g_), state(dense(state_)), lengths(dense(lengths_)) {
         d.struct_bytes = sizeof(d);
         d.dtype = dtype_of(v);
         d.B = (int)v.size(0); d.T = (int)v.size(1); d.H = (int)v.size(2); d.V = (int)v.size(3);
         d.G = (int)q.size(2); d.K = (int)q.size(3);
-        d.flags = (uint32_t)flags;
         d.scale = (float)scale;
         d.q = attn_tensor(q); d.k = attn_tensor(k); d.v = attn_tensor(v);
         d.log_decay = fptr(g);
@@ -87,15 +86,14 @@ Tensor attn_forward(Attn& a, Tensor* state_out) {
 class AttnFn : public torch::autograd::Function<AttnFn> {
 public:
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const optional<Tensor>& state_,
-                                 const optional<Tensor>& lengths_, double scale, bool want_state, int64_t flags) {
+                                 const optional<Tensor>& lengths_, double scale, bool want_state) {
         const Tensor state = or_none(state_), lengths = or_none(lengths_);
         const c10::cuda::CUDAGuard guard(v.device());
-        Attn a(q, k, v, g, state, lengths, scale, flags);
+        Attn a(q, k, v, g, state, lengths, scale);
         Tensor out_state;
         const Tensor o = attn_forward(a, want_state ? &out_state : nullptr);
         ctx->save_for_backward({q, k, v, g, state, lengths});
         ctx->saved_data["scale"] = scale;
-        ctx->saved_data["flags"] = flags;
         ctx->set_materialize_grads(false);
         return want_state ? variable_list{o, out_state} : variable_list{o};
     }
@@ -106,8 +104,8 @@ public:
         const c10::cuda::CUDAGuard guard(s[2].device());
         check_waits();
         const bool have_state_grad = grads.size() > 1 && grads[1].defined();
-        if (!grads[0].defined() && !have_state_grad) return variable_list(9);
-        Attn a(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["flags"].toInt());
+        if (!grads[0].defined() && !have_state_grad) return variable_list(8);
+        Attn a(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble());
         m2d_attn_desc& d = a.d;
         const Tensor d_o = grads[0].defined() ? rows(grads[0].to(a.v.scalar_type())) : at::zeros(a.v.sizes(), a.v.options());
         const Tensor d_out = have_state_grad ? grads[1].to(at::kFloat).contiguous() : Tensor();
@@ -132,7 +130,7 @@ public:
         }
         check(m2d_attn_bwd(&d, stream_of(a.v)), "m2d_attn_bwd");
         if (dg.defined() && s[3].dim() == 1) dg = dg.sum(at::IntArrayRef{0, 1});
-        return {dq, dk, dv, dg, ds, Tensor(), Tensor(), Tensor(), Tensor()};
+        return {dq, dk, dv, dg, ds, Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -160,7 +158,7 @@ void check_attn(const char* what, const char* tokens, const Tensor& q, const Ten
 }
 
 std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const optional<double>& scale_,
-                                                      const optional<Tensor>& state_, const optional<Tensor>& lengths_, bool want_state, int64_t flags) {
+                                                      const optional<Tensor>& state_, const optional<Tensor>& lengths_, bool want_state) {
     const char* const what = "linear_attention";
     const Tensor state = or_none(state_);
     Tensor lengths = or_none(lengths_);
@@ -179,12 +177,12 @@ std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Ten
     const Tensor g = log_decay.to(at::kFloat);
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)q.size(-1));
     if (wants_grad({&q, &k, &v, &g, &state})) {
-        const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths.defined() ? optional<Tensor>(lengths) : c10::nullopt, scale, want_state, flags);
+        const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths.defined() ? optional<Tensor>(lengths) : c10::nullopt, scale, want_state);
         return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
     }
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
-    Attn a(q, k, v, g, state, lengths, scale, flags);
+    Attn a(q, k, v, g, state, lengths, scale);
     Tensor out_state;
     const Tensor o = attn_forward(a, want_state ? &out_state : nullptr);
     return {o, want_state ? optional<Tensor>(out_state) : c10::nullopt};
@@ -363,7 +361,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm) {
 void bind_sequence_operators(pybind11::module& m) {
     using pybind11::arg;
     m.def("linear_attention", &linear_attention, "linear attention of whole sequences: (o, state or None)", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale").none(true),
-          arg("state").none(true), arg("lengths").none(true), arg("want_state"), arg("flags") = 0);
+          arg("state").none(true), arg("lengths").none(true), arg("want_state"));
     m.def("linear_attention_step", &linear_attention_step, "linear attention of one token; the state is updated in place", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("state"),
           arg("scale").none(true));
     m.def("group_norm", &group_norm, "group normalisation with an activation, channels last", arg("x"), arg("groups"), arg("weight").none(true), arg("bias").none(true), arg("eps"), arg("act"));
