@@ -199,13 +199,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     const int seg = unit % units, bh = unit / units, h = bh % a.H, b = bh / a.H;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, rev = k.rev;
     const int len = attn_length(a, b);
-    // (never t_lo + seg_len, which may lie beyond 2^31)
-    int t_lo = seg * a.seg_len, t_hi = t_lo + min(a.seg_len, a.T - t_lo);
+    unsigned lo = seg * a.seg_len, hi = lo + a.seg_len;              // (may lie beyond 2^31)
     if (STATE_ONLY && a.join_here) {
-        const int from = (seg / a.parts + rev) * a.seg_len, most = min(a.seg_len, a.T - from), at = min(seg % a.parts * a.part_len, most);
-        t_lo = from + at;
-        t_hi = t_lo + min(a.part_len, most - at);
+        const unsigned from = (seg / a.parts + rev) * a.seg_len;
+        lo = from + seg % a.parts * a.part_len;
+        hi = min(from + a.seg_len, lo + a.part_len);
     }
+    const int t_lo = STATE_ONLY ? (int)min(lo, (unsigned)a.T) : (int)lo, t_hi = (int)min(hi, (unsigned)a.T);
     const int active = max(0, min(len, t_hi) - t_lo), chunks = (active + kTc - 1) / kTc;         // the others hold nothing
 
     TcSmall& small = *reinterpret_cast<TcSmall*>(tc_smem_raw + lay.small);
