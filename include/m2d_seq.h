@@ -24,7 +24,8 @@ extern "C" {
  * 16-byte pieces, 16-byte aligned and with such strides, take a form on the tensor cores (tcgen05), all others, and d_q and d_k
  * where the decay's gradient is wanted, one for any size and with more exact products.  Long sequences of few heads are cut into segments whose states the workspace holds; the workspace queries read the
  * sizes, G, dtype and, for the backward pass, whether d_log_decay is given.  B * H up to 2^24, T below 2^31 - 2048.
- * A wait inside the tensor-core form that gives up makes its rows NaN and shows in m2d_take_wait_failure().
+ * A wait inside the tensor-core form that gives up makes its rows NaN, or the state that its CTA was to leave for other rows, and so
+ * those; it shows in m2d_take_wait_failure().
  */
 #define M2D_ATTN_MAX_DIM 256      /* K and V, each */
 
@@ -37,7 +38,7 @@ typedef struct m2d_attn_desc {
     uint32_t struct_bytes;         /* = sizeof(m2d_attn_desc) */
     int32_t dtype;                 /* m2d_dtype of q, k, v, o and their gradients */
     int32_t B, T, H, G, K, V;      /* G divides H */
-    uint32_t flags;                /* 0 */
+    uint32_t flags;                /* 0, or the test hook */
     float scale;
     m2d_attn_tensor q, k, v;       /* the latter with H heads */
     const float *log_decay;        /* log_decay[b * g_batch + t * g_token + h * g_head] */
@@ -56,6 +57,13 @@ typedef struct m2d_attn_desc {
     void *workspace;               /* scratch, 256-byte aligned */
     uint64_t workspace_bytes;
 } m2d_attn_desc;
+
+/*
+ * Test hook, rejected with M2D_ERR_FLAGS unless the environment variable M2D_TEST_HOOKS is 1: in the first CTA of every launch of
+ * the tcgen05 form that computes segments' states the first wait that does not succeed at once gives up.  Nothing faults or
+ * hangs; the launch ends as after a wait that ran out.
+ */
+#define M2D_ATTN_TEST_GIVE_UP 0x100u
 
 uint64_t m2d_attn_fwd_workspace(const m2d_attn_desc *desc);
 uint64_t m2d_attn_bwd_workspace(const m2d_attn_desc *desc);

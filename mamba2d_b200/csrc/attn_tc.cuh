@@ -25,8 +25,8 @@
 // the schedulers issue in 26 %, and what most warps wait for, besides each other, is instructions (1.9 of the 6 cycles between
 // two instructions of a warp).  The bytes would take 34 us.
 //
-// Every wait is bounded: one that gives up makes all of the CTA's roles leave, its rows become NaN, and a word in host memory
-// says so.
+// Every wait is bounded: one that gives up makes all of the CTA's roles leave, its rows become NaN (or, where it computes a segment's
+// state, that does, and with it the rows that come of it), and a word in host memory says so.
 #pragma once
 
 #include "attn_core.cuh"
@@ -45,6 +45,7 @@ struct TcLaunch {
     AttnLaunch a;
     int cores;
     int* host_flag;
+    int give_up;                // test hook: the first CTA's, of a launch over states
 };
 
 // ---- PTX ---------------------------------------------------------------------------------------
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         for (int i = kFull; i < kEmpty; ++i) mbar_init(bar(i), 1);
         // who gives a tile back: its two products, (1) and (4) counted as one; x's where out goes through it, whoever stores that
         for (int i = 0; i < 3 * kTcTiles; ++i) mbar_init(bar(kEmpty + i), STATE_ONLY || i / kTcTiles == Y || (i / kTcTiles == X && !lay.own_stage) ? 1 : 2);
-        small.abort = (smem_u32(tc_smem_raw) & 1023u) != 0;      // (swizzled tiles have to be aligned; nothing runs if they are not)
+        small.abort = (smem_u32(tc_smem_raw) & 1023u) != 0 || (STATE_ONLY && L.give_up && blockIdx.x == 0);      // (swizzled tiles have to be aligned; nothing runs if they are not)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 16) tmem_alloc(smem_u32(&small.tmem), kCols);
@@ -494,14 +495,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(bar(kO + (it & 1)));
             }
         }
+        // a warp that has left its chunks early has seen (or made) the abort: what it has is no state
+        auto void_it = [&] {
+            if (*abort) {
+#pragma unroll
+                for (int c = 0; c < kHalf; ++c) S[c] = __int_as_float(0x7fc00000);
+            }
+        };
         if constexpr (STATE_ONLY) {
+            void_it();
             put(k.seg_state + ((size_t)bh * states + seg) * k.Kd * k.Vd, 1, k.Kd);
         } else {
             if (k.fin.p && seg == (rev ? 0 : a.nseg - 1)) {
-                if (*abort) {
-#pragma unroll
-                    for (int c = 0; c < kHalf; ++c) S[c] = __int_as_float(0x7fc00000);
-                }
+                void_it();
                 put(k.fin.p + b * k.fin.sb + h * k.fin.sh, k.fin.sr, k.fin.sc);
             }
         }

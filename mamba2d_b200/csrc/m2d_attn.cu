@@ -512,7 +512,7 @@ static int check_attn(const m2d_attn_desc* d, bool ptrs) {
     if (!d) return M2D_ERR_NULL;
     if (d->struct_bytes != sizeof(m2d_attn_desc)) return M2D_ERR_ABI;
     if (d->dtype != M2D_F32 && d->dtype != M2D_BF16) return M2D_ERR_DTYPE;
-    if (d->flags) return M2D_ERR_FLAGS;
+    if (d->flags && ((d->flags & ~M2D_ATTN_TEST_GIVE_UP) || !test_hooks_enabled())) return M2D_ERR_FLAGS;
     if (d->B < 1 || d->T < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->K < 1 || d->V < 1 || d->K > M2D_ATTN_MAX_DIM || d->V > M2D_ATTN_MAX_DIM) return M2D_ERR_SHAPE;
     if (d->T > INT_MAX - 4 * kAnchor) return M2D_ERR_TOO_LARGE;      // (token numbers go up to the end of the last chunk)
     if ((int64_t)d->B * d->H > (1 << 24) || (int64_t)d->B * d->H * ((d->T + kAnchor - 1) / kAnchor) >= (1ll << 31)) return M2D_ERR_TOO_LARGE;
@@ -633,6 +633,7 @@ static int launch_tc(const m2d_attn_desc* d, const AttnPlan& p, int first, int c
     L.a = p.a;
     L.cores = count;
     L.host_flag = wait_failure_flag();
+    L.give_up = (d->flags & M2D_ATTN_TEST_GIVE_UP) != 0;
     for (int i = 0; i < count; ++i) {
         const AttnCore& c = L.a.core[i] = p.a.core[first + i];
         if (!(MODE == kTcStateOnly || attn_map(&maps.m[i][0], d, c.x, c.Kd)) || !attn_map(&maps.m[i][1], d, c.y, c.Kd) || !attn_map(&maps.m[i][2], d, c.z, c.Vd)) return M2D_ERR_LAUNCH;
