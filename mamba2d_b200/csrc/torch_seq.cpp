@@ -33,7 +33,7 @@ bool wants_grad(std::initializer_list<const Tensor*> inputs) {
     return grad;
 }
 // A wait between warps of an earlier launch that gave up (its results are NaN) surfaces at the next call.
-void check_waits() { TORCH_CHECK(!m2d_take_wait_failure(), "linear attention: a wait inside an earlier launch timed out; the results of that launch are invalid"); }
+void check_waits(const char* what) { TORCH_CHECK(!m2d_take_wait_failure(), what, ": a wait inside an earlier launch timed out; the results of that launch are invalid"); }
 Tensor or_none(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 // neighbours along the last dimension
 Tensor rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
@@ -102,7 +102,7 @@ public:
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_attention: gradients of gradients (create_graph) are not supported");
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[2].device());
-        check_waits();
+        check_waits("linear_attention");
         const bool have_state_grad = grads.size() > 1 && grads[1].defined();
         if (!grads[0].defined() && !have_state_grad) return variable_list(8);
         Attn a(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble());
@@ -173,7 +173,7 @@ std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Ten
         if (!want_state) return {v.clone(), c10::nullopt};
         return {v.clone(), state.defined() ? state.clone() : at::zeros({v.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat))};
     }
-    check_waits();
+    check_waits(what);
     const Tensor g = log_decay.to(at::kFloat);
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)q.size(-1));
     if (wants_grad({&q, &k, &v, &g, &state})) {
@@ -198,6 +198,7 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
     TORCH_CHECK(B == 0 || (dense_kv && apart), what, ": the state must be dense in (K, V) and must not overlap itself, got strides ", state.strides());
     TORCH_CHECK(!wants_grad({&q, &k, &v, &log_decay, &state}), what, " updates the state in place and has no gradients: call it without gradients");
     if (B == 0) return v.clone();
+    check_waits(what);                       // (the state may be that of a prompt)
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
     const Tensor qr = rows(q), kr = rows(k), vr = rows(v), g = log_decay.to(at::kFloat);

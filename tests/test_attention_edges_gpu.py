@@ -8,7 +8,7 @@ import torch
 
 from test_attention_gpu import BF, make
 from test_sequence_host import AttnDesc, Tensor
-from mamba2d_b200 import _lib, linear_attention
+from mamba2d_b200 import _lib, linear_attention, linear_attention_step
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,14 @@ def test_a_wait_that_gives_up_leaves_nothing_that_looks_right(B, T, H, K, V, mon
         linear_attention(q, k, v, d)
     assert not _lib.take_wait_failure()
     check(Out(*_through_the_library(q, k, v, d, s, 0)), want, {})
+
+
+def test_a_token_behind_a_prompt_that_went_wrong_tells(monkeypatch):
+    monkeypatch.setenv("M2D_TEST_HOOKS", "1")
+    _lib.lib()
+    q, k, v, d, s, _ = make(2, 1100, 2, 2, 64, 64, BF, state=True)
+    _, state = _through_the_library(q, k, v, d, s, 0x100)
+    with pytest.raises(RuntimeError, match="linear_attention_step: a wait inside an earlier launch timed out"):
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], d[:, 0], state)
+    assert not _lib.take_wait_failure()
+    assert bool(torch.isfinite(linear_attention_step(q[:, 0], k[:, 0], v[:, 0], d[:, 0], s)).all())      # told once
