@@ -26,6 +26,17 @@ __device__ __forceinline__ float rcp_of(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// The smaller of the two (the larger), NaN where z is.
+__device__ __forceinline__ float at_most(float z, float top) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(top));
+    return r;
+}
+__device__ __forceinline__ float at_least(float z, float bottom) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(bottom));
+    return r;
+}
 // Phi(-|z|) = erfc(|z| / sqrt 2) / 2 and exp(-z^2 / 2), by formula 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions,
 // erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) with t = 1 / (1 + p x), within 1.5e-7: the exponential is the one that phi needs.  (In
 // scalars: a packed multiply-add takes no constant, and the constants' registers cost more than it saves.)
@@ -38,19 +49,25 @@ __device__ __forceinline__ float gauss_tail(float z, float* e) {
     q = fmaf(q, t, 0.5f * 0.254829592f);
     return q * t * *e;
 }
-// act(z) and act'(z).  (A NaN stays one; the slope at an infinity is that of the largest floats.)
+// act(z) and act'(z).  A NaN stays one.  Value and slope at an infinity are their limits: z is bounded where an infinity would meet a
+// zero, at a value beyond which exp has long been zero or infinite.
+constexpr float kActFar = 256.f;
 template <int ACT>
 __device__ __forceinline__ float act_value1(float z) {
-    if constexpr (ACT == M2D_ACT_SILU) return z * rcp_of(1.f + ex2(z * -kLog2e));
+    if constexpr (ACT == M2D_ACT_SILU) {
+        z = at_least(z, -kActFar);
+        return z * rcp_of(1.f + ex2(z * -kLog2e));
+    }
     if constexpr (ACT == M2D_ACT_GELU) {
         float e;
         const float tail = gauss_tail(z, &e);
-        return fmaf(-fabsf(z), tail, z < 0.f ? 0.f : z);      // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+        return fmaf(-at_most(fabsf(z), kActFar), tail, z < 0.f ? 0.f : z);      // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
     }
     return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope1(float z) {
+    if constexpr (ACT != M2D_ACT_NONE) z = at_least(at_most(z, kActFar), -kActFar);
     if constexpr (ACT == M2D_ACT_SILU) {
         const float s = rcp_of(1.f + ex2(z * -kLog2e));
         return s * fmaf(z, 1.f - s, 1.f);                     // s (1 + z (1 - s)), s the logistic function

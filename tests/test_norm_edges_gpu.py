@@ -124,3 +124,36 @@ def test_gradients_that_cancel_in_any_shape(shape, groups, offset):
     assert float(dx.abs().max()) < 1e-6
     want = 1.0003 * (x.numel() / shape[-1])
     assert float((db.double() / want - 1).abs().max()) < 1e-6
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("shape,groups", KINDS)
+def test_activation_at_infinity(shape, groups, act, dt):
+    """At +inf it is +inf and its slope one, at -inf both are zero: the gradients are those of biases that are merely
+    large.  A NaN stays one."""
+    x, dy = torch.randn(shape, device="cuda").to(dt), torch.randn(shape, device="cuda").to(dt)
+    C = shape[-1]
+    b = torch.randn(C, device="cuda")
+    far = b.clone()
+    b[3], b[5], far[3], far[5] = float("inf"), -float("inf"), 1e6, -1e6
+    results = []
+    for bias in (b, far):
+        leaves = [x.clone().requires_grad_(True), bias.clone().requires_grad_(True)]
+        y = group_norm(leaves[0], groups, None, leaves[1], act=act)
+        results.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+    (y, dx, db), (y_far, dx_far, db_far) = results
+    assert bool((y[..., 3] == float("inf")).all()) and not y[..., 5].any()
+    assert torch.equal(dx, dx_far) and torch.equal(db, db_far) and bool(torch.isfinite(dx).all())
+    keep = [c for c in range(C) if c not in (3, 5)]
+    assert torch.equal(y[..., keep], y_far[..., keep])
+    w = torch.ones(C, device="cuda")
+    w[7] = 3e38                                               # h w beyond the largest float
+    y = group_norm(x, groups, w, act=act)
+    assert not bool(torch.isnan(y).any()) and bool((y[..., 7] == float("inf")).any())
+    b[4] = float("nan")
+    leaf = x.clone().requires_grad_(True)
+    y = group_norm(leaf, groups, None, b, act=act)
+    assert bool(torch.isnan(y[..., 4]).all()) and not bool(torch.isnan(y[..., 3]).any())
+    dx, = torch.autograd.grad(y, leaf, dy)
+    assert bool(torch.isnan(dx[..., 4]).all())
