@@ -721,11 +721,17 @@ static int check_workspace(const m2d_attn_desc* d, size_t bytes) {
     if (!bytes) return M2D_OK;
     return d->workspace && d->workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(d->workspace) & 255) == 0 ? M2D_OK : M2D_ERR_WORKSPACE;
 }
-// What either form may need: a query does not depend on the tensors' addresses.
-static size_t attn_workspace(const m2d_attn_desc* d, bool bwd) {
-    size_t tc = 0;
-    if (d->dtype == M2D_BF16) tc = bwd && d->d_log_decay ? plan_attn(d, false, true, 1, plan_attn(d, true, false, 2).bytes).bytes : plan_attn(d, bwd, true).bytes;
-    return std::max(plan_attn(d, bwd, false).bytes, tc);
+// What either form may need, with lengths or without: a query does not depend on the tensors' addresses.
+static size_t attn_workspace(const m2d_attn_desc* desc, bool bwd) {
+    size_t most = 0;
+    for (const int32_t* lengths : {(const int32_t*)nullptr, (const int32_t*)&desc->B}) {      // (whether there are any is all that a plan looks at)
+        m2d_attn_desc d = *desc;
+        d.lengths = lengths;
+        size_t tc = 0;
+        if (d.dtype == M2D_BF16) tc = bwd && d.d_log_decay ? plan_attn(&d, false, true, 1, plan_attn(&d, true, false, 2).bytes).bytes : plan_attn(&d, bwd, true).bytes;
+        most = std::max({most, plan_attn(&d, bwd, false).bytes, tc});
+    }
+    return most;
 }
 
 }  // namespace m2d
