@@ -8,10 +8,11 @@
 //     (4)  delta = (u y)^T z        KD x VD      u y scaled in place, in two bf16 parts: St is carried in fp32 and a state
 //                                                is an output; one part would leave it at 2^-9
 // A decay D_rc = exp(c_r - c_c) is a product of exp(c_r - m) and f_c = exp(m - c_c), m half of the chunk's decay: P is pairs times
-// f, the copy of St is scaled by exp(m), and out = exp(c_r - m) O; all factors lie within 2^+-80 or the chunk is not `mild`
-// (m would have to lie further from its ends than that: decays of more than 0.87 a token on average, a sequence that starts
+// f, the copy of St is scaled by exp(m), and out = exp(c_r - m) O; all factors lie within 2^+-48 or the chunk is not `mild`
+// (m would have to lie further from its ends than that: decays of more than 0.52 a token on average, a sequence that starts
 // anew inside).  P of such a chunk takes its D from differences of c, and O of (2) is scaled by its rows where it lies
-// before (3) adds.  c is summed in 64 bits.
+// before (3) adds.  What the factors take of the range of values is missing at its ends: with 2^+-80 values of 1e-17 lost bits and such of
+// 1e16 became infinite.  (If no chunk were mild: 4x4096x16x128 135 us for 124, 1x65536x8 194 for 178.)  c is summed in 64 bits.
 // The work is dealt to warps that wait on one another through mbarriers only:
 //     warps 0 - 7    a token row and half of the columns a thread: pairs -> P, O -> out
 //     warps 8 - 15   half of a token row a thread: y -> u y; half of a row of St a thread: St in registers, its bf16 copy
@@ -38,7 +39,7 @@ constexpr int kTc = 128;                      // tokens of a chunk
 constexpr int kTcThreads = 640;
 constexpr int kTcBlock = kTc * 128;           // 128 rows x 64 columns of bf16
 constexpr int kTcTiles = 3;                   // tiles of x, y, z each in flight, at most
-constexpr float kTcMild = 80.f;
+constexpr float kTcMild = 48.f;
 
 struct TcMaps { CUtensorMap m[3][4]; };       // [core][x, y, z, out]
 struct TcLaunch {

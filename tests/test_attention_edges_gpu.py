@@ -103,3 +103,26 @@ def test_a_token_behind_a_prompt_that_went_wrong_tells(monkeypatch):
         linear_attention_step(q[:, 0], k[:, 0], v[:, 0], d[:, 0], state)
     assert not _lib.take_wait_failure()
     assert bool(torch.isfinite(linear_attention_step(q[:, 0], k[:, 0], v[:, 0], d[:, 0], s)).all())      # told once
+
+
+@pytest.mark.parametrize("exponent", [-57, 57])
+@pytest.mark.parametrize("rate", [0.3, 0.55, 0.65, 0.8])
+def test_small_and_large_values_with_steep_decays(rate, exponent):
+    """v, and the gradient of the output, times a power of two, which changes no rounding: 2^-57 is 7e-18.  Everything that
+    is a product of them is that many times what it was, in every bit.  (Decays of 16 to 46 in a chunk's 128 tokens from its
+    middle, as powers of two 25 to 74: the tcgen05 form holds a pair's weight as a product of factors that large.)"""
+    q, k, v, _, s, _ = make(2, 1100, 2, 1, 64, 128, BF, state=True)
+    d = -rate * (0.9 + 0.2 * torch.rand(2, 1100, 2, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"))
+    d_o = torch.randn(v.shape, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(BF)
+
+    def call(scale):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v * scale, s * scale)]
+        o, final = linear_attention(*leaves[:3], d, initial_state=leaves[3], return_state=True)
+        _, _, dv, ds = torch.autograd.grad(o, leaves, d_o * scale, retain_graph=True)
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v, s)]
+        dq, dk = torch.autograd.grad(linear_attention(*leaves[:3], d, initial_state=leaves[3]), leaves[:2], d_o * scale)
+        return [t.detach() / scale for t in (o, final, dv, ds, dq, dk)]
+    for name, x, y in zip(("o", "state", "dv", "ds", "dq", "dk"), call(2.0 ** exponent), call(1.0)):
+        assert bool(torch.isfinite(x).all()), name
+        # (results that are themselves below the smallest normal float, or their parts, may differ)
+        assert torch.equal(x, y) or float((x.double() - y.double()).abs().max()) <= 1e-6 * float(y.abs().max()), name
