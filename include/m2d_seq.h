@@ -22,8 +22,11 @@ extern "C" {
  *
  * State, its gradient and that of the decay are fp32 whatever the tensors' type.  bf16 tensors with K and V of up to 128 in whole
  * 16-byte pieces, 16-byte aligned and with such strides, take a form on the tensor cores (tcgen05), all others, and d_q and d_k
- * where the decay's gradient is wanted, one for any size and with more exact products.  Long sequences of few heads are cut into segments whose states the workspace holds; the workspace queries read the
- * sizes, G, dtype and, for the backward pass, whether d_log_decay is given.  B * H up to 2^24, T below 2^31 - 2048.
+ * where the decay's gradient is wanted, one for any size and with more exact products.  With the former, products of values below 1e-17
+ * or above 1e17 may lose bits or range where decays sum to about 65 in 128 tokens (pairs' weights are products of factors of up to 2^48).
+ * Long sequences of few heads are cut into segments whose states the workspace holds; the workspace queries read the
+ * sizes, G, dtype and, for the backward pass, whether d_log_decay is given, and need no other pointer.  B * H up to 2^24, T below
+ * 2^31 - 2048.
  * A wait inside the tensor-core form that gives up makes its rows NaN, or the state that its CTA was to leave for other rows, and so
  * those; it shows in m2d_take_wait_failure().
  */
@@ -78,8 +81,10 @@ int m2d_attn_step(const m2d_attn_desc *desc, int64_t state_batch, int64_t state_
 
 /* ---- group normalisation ----------------------------------------------------------------------------------------
  * x (N,S,C), channels last: y = act((x - mean) * rstd * weight + bias), mean and variance over S and the C / groups
- * channels of a group.  C up to 2^29, N * groups below 2^31; tensors that are not 16-byte aligned, or whose rows are not whole 16-byte
- * pieces, take a slower form.
+ * channels of a group.  Value and slope of act at an infinity are their limits.  C up to 2^29, N * groups below 2^31.  A slower form
+ * takes tensors that are not 16-byte aligned or whose rows are not whole 16-byte pieces, images (S > 1) with rows of more than 4 KB,
+ * and S = 1 with groups of more than 512 bytes or not of whole pieces.  The backward pass's workspace query reads whether d_weight is
+ * given.
  */
 typedef enum { M2D_ACT_NONE = 0, M2D_ACT_SILU = 1, M2D_ACT_GELU = 2 /* erf form */ } m2d_act;
 

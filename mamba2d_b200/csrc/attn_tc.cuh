@@ -13,6 +13,10 @@
 // anew inside).  P of such a chunk takes its D from differences of c, and O of (2) is scaled by its rows where it lies
 // before (3) adds.  What the factors take of the range of values is missing at its ends: with 2^+-80 values of 1e-17 lost bits and such of
 // 1e16 became infinite.  (If no chunk were mild: 4x4096x16x128 135 us for 124, 1x65536x8 194 for 178.)  c is summed in 64 bits.
+// Rounded to bf16 on the way are P and St's copy, once each, of which one lies on a term's way: an output, itself rounded to bf16 after
+// that, is off by 2.3e-3 where its own rounding alone would leave 1.7e-3.  q, k and v come with as large a rounding.  u y has two
+// parts (16 bits; what a state is off by, 2.5e-6, is theirs): a third would be half as many products (4) again, on the longest chain, and take
+// a tile of the ring.
 // The work is dealt to warps that wait on one another through mbarriers only:
 //     warps 0 - 7    a token row and half of the columns a thread: pairs -> P, O -> out
 //     warps 8 - 15   half of a token row a thread: y -> u y; half of a row of St a thread: St in registers, its bf16 copy
@@ -24,7 +28,8 @@
 //
 // Measured, forward at 8x2048x16x128: 84 us for 128 CTAs of 16 chunks, 10000 cycles a chunk: the tensor cores are busy for 29 % of them,
 // the schedulers issue in 26 %, and what most warps wait for, besides each other, is instructions (1.9 of the 6 cycles between
-// two instructions of a warp).  The bytes would take 34 us.
+// two instructions of a warp).  The bytes would take 34 us.  At 96 registers a thread full passes spill 24 to 40 bytes (92 to 156 bytes of
+// loads); a pass over states 8 at most.
 //
 // Every wait is bounded: one that gives up makes all of the CTA's roles leave, its rows become NaN (or, where it computes a segment's
 // state, that does, and with it the rows that come of it), and a word in host memory says so.

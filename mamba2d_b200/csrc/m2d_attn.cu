@@ -764,7 +764,7 @@ extern "C" int m2d_attn_bwd(const m2d_attn_desc* d, void* stream) {
     if (rc != M2D_OK) return rc;
     if (!d->d_o.data || !d->d_q || !d->d_k || !d->d_v) return M2D_ERR_NULL;
     // The decay's gradient sums dots of 512 tokens that cancel: dq and dk with operands in two bf16 parts left it at up to 4e-5
-    // (2x1000x4x128), split tf32 ones leave it at 1e-6.  (8x2048x16x128, training: 2650 us, 3525 with dv in this form too, 430 with the parts.)
+    // (2x1000x4x128), split tf32 ones leave it at 1e-6.  (8x2048x16x128, training: 2690 us, 3525 with dv in this form too, 430 with the parts.)
     const bool tc = tc_applies(d, true), apart = tc && d->d_log_decay;       // dv, which has no part in it, in the tcgen05 form
     AttnPlan p = plan_attn(d, true, tc && !apart, apart ? 2 : 3), pv = p;
     if (apart) pv = plan_attn(d, false, true, 1, p.bytes);

@@ -143,8 +143,9 @@ __device__ __forceinline__ double2 block_sum2(double2 v) {
 // ------------------------------------------------------------------------------------------------
 // S = 1, groups of whole 16-byte vectors, at most 32: a group is that many neighbouring lanes of a warp (a warp holds as
 // many groups as fit).  A thread keeps its channels over all the rows that it walks: their parameters stay in registers, and
-// so do the sums of their gradients.  One read of x (and dy), one write: at 16384x16x128 bf16 with SiLU 37 us forward (3.6 TB/s),
-// 60 us backward (3.4 TB/s); what bounds it is the activation's instructions and the groups' shuffles at 16 (backward) and 32 warps an SM.
+// so do the sums of their gradients.  One read of x (and dy), one write: at 16384x16x128 bf16 with SiLU 39 us forward (3.5 TB/s),
+// 67 us backward with the parameters' sums (3.0 TB/s); what holds it up is the activation's instructions and the groups' shuffles at 16
+// (backward) and 32 warps an SM, which issue in 51 and 66 % of the cycles.
 // ------------------------------------------------------------------------------------------------
 template <typename io_t, int ACT, bool BWD>
 __global__ void __launch_bounds__(256, BWD ? 2 : 4) norm_rows_kernel(const NormArgs a, int lanes, int cols) {      // lanes of a group, groups of a row in this block
@@ -283,8 +284,9 @@ __global__ void __launch_bounds__(256, BWD ? 2 : 4) norm_rows_kernel(const NormA
 // A thread keeps a vector of channels and walks rows, with the channels' parameters and statistics in registers.
 // In the backward pass act' dy replaces dy in shared memory, in fp32; with bf16 tensors act' is evaluated twice (kept in bf16 the
 // product would carry a rounding as large as dx's own).
-// 128x3136x64 bf16 with GELU, in pieces: sums 18 and values 31 us forward (the second read comes from L2), 35 and 40 backward, 131 with
-// what joins them: the schedulers issue in 45 % of the cycles (30 % where the sums are), GELU's arithmetic twice in the backward pass.
+// 128x3136x64 bf16 with GELU, in pieces: sums 18 and values 31 us forward (the second read comes from L2: 9 of its 51 MB from memory),
+// 36 and 42 backward (the second read comes from memory again: 100 of 103 MB), 130 with what joins them.  The schedulers issue in 54 to
+// 64 % of the cycles and memory moves at 2.4 to 2.9 TB/s: neither is the bound, loads in flight at 16 warps an SM (backward) are too few.
 // ------------------------------------------------------------------------------------------------
 constexpr int kNormThreads = 256, kNormWarps = kNormThreads / 32;
 
@@ -652,7 +654,8 @@ __device__ __forceinline__ void walk_group(const NormArgs& a, F f) {
         }
     }
 }
-// Any shape: a CTA owns a group of an image and reads it three times (mean, variance about it, values).  A thread adds up a 256th of
+// Any shape: a CTA owns a group of an image and reads it three times (mean, variance about it, values).  One group per token, C = 320,
+// 100352 tokens: 310 us forward, 520 ... 530 backward, fp32 or bf16; 128x3136x30 bf16 90 and 167 (floors 20 ... 39, 29 ... 59; 7 and 11).  A thread adds up a 256th of
 // it one by one, without bound, so here and in the two kernels below that is done in 64 bits: in 32, values around 1000 left a mean
 // off by 0.2 after 49000 terms.
 template <typename io_t>
