@@ -203,8 +203,19 @@ __global__ void __launch_bounds__(256, BWD ? 2 : 4) norm_rows_kernel(const NormA
                     for (int i = 1; i < V::pairs; ++i) sum = __fadd2_rn(sum, xv[j].get(i));
                     s0[j] = sum.x + sum.y;
                 }
+                if (even) {
 #pragma unroll
-                for (int j = 0; j < kRows; ++j) s0[j] = group_sum(s0[j]) * inv;
+                    for (int j = 0; j < kRows; ++j) s0[j] = group_sum(s0[j]) * inv;
+                } else {          // about the group's first value: where the size is no power of two, equal values' sum and its share are rounded
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j) {
+                        const float base = __shfl_sync(mask, xv[j].get(0).x, lane - pos);
+                        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int i = 0; i < V::pairs; ++i) sum = __fadd2_rn(sum, __fadd2_rn(xv[j].get(i), make_float2(-base, -base)));
+                        s0[j] = fmaf(group_sum(sum.x + sum.y), inv, base);
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < kRows; ++j) {
                     float2 sum = make_float2(0.f, 0.f);

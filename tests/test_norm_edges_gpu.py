@@ -157,3 +157,13 @@ def test_activation_at_infinity(shape, groups, act, dt):
     assert bool(torch.isnan(y[..., 4]).all()) and not bool(torch.isnan(y[..., 3]).any())
     dx, = torch.autograd.grad(y, leaf, dy)
     assert bool(torch.isnan(dx[..., 4]).all())
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("per", [8, 24, 40, 48, 56, 72, 80, 104, 112, 120, 128])
+def test_rows_of_one_value(per, dt):
+    """As ``test_images_of_one_value``, a group a token: sizes that are a power of two and sizes that are none."""
+    C = 4 * per
+    w, b = torch.full((C,), 0.5, device="cuda"), torch.full((C,), 0.25, device="cuda")
+    for value in (1000.3, -0.7, 3e-5, 12345.67):
+        assert bool((group_norm(torch.full((64, C), value, device="cuda").to(dt), 4, w, b) == 0.25).all()), value
