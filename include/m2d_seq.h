@@ -1,6 +1,7 @@
 /*
  * m2d_seq.h -- C ABI of the sequence operators next to the wavefront scan: linear attention with a decay per head,
- * group normalisation with an activation on channels-last tensors, clipping by the global norm of many tensors.
+ * group normalisation with an activation on channels-last tensors, clipping by the global norm of many tensors, a gated
+ * recurrence per channel.
  *
  * Conventions are those of m2d_scan.h: device pointers, memory owned by the caller, asynchronous on `stream` (of the
  * current device), status codes, re-entrant, nothing kept between calls.  Strides are in elements.
@@ -124,6 +125,45 @@ typedef struct m2d_clip_tensor {
 uint64_t m2d_clip_workspace(const m2d_clip_tensor *tensors, int32_t count);
 int m2d_clip_grad_norm(const m2d_clip_tensor *tensors, int32_t count, float max_norm, float *norm, void *workspace,
                        uint64_t workspace_bytes, void *stream);
+
+/* ---- gated recurrence --------------------------------------------------------------------------------------------
+ * Per sequence and channel  h_t = a_t h_{t-1} + u_t:
+ *     M2D_GATE_DECAY:  a = exp(gate), u = x           (gate at most 0; positive ones grow the state and are not checked for)
+ *     M2D_GATE_FORGET: a = sigmoid(gate), u = (1 - a) x
+ * A gate of -inf forgets everything before the token.  States and their gradients are fp32 whatever the tensors' type.  B times C/32 up to
+ * 2^27, T below 2^31 - 1024.
+ */
+typedef enum { M2D_GATE_DECAY = 0, M2D_GATE_FORGET = 1 } m2d_gate;
+
+typedef struct m2d_recur_tensor {
+    const void *data;              /* (B,T,C), neighbours along C */
+    int64_t batch, token;          /* strides of the other two */
+} m2d_recur_tensor;
+
+typedef struct m2d_recur_desc {
+    uint32_t struct_bytes;         /* = sizeof(m2d_recur_desc) */
+    int32_t dtype;                 /* m2d_dtype of x, gate, y and their gradients */
+    int32_t B, T, C;
+    int32_t form;                  /* m2d_gate */
+    m2d_recur_tensor x, gate;
+    const int32_t *lengths;        /* (B) tokens of each sequence, clamped to 0 ... T, or NULL: T.  Rows behind a sequence's last are not
+                                      read; outputs there are zero */
+    const float *state;            /* (B,C) dense: the state before the first token, or NULL: zero */
+    float *state_out;              /* (B,C) dense: the state after the last one, or NULL                    [fwd] */
+    void *y;                       /* (B,T,C) dense: every h_t                                              [fwd] */
+    float *marks;                  /* m2d_recur_marks() values: written by fwd (NULL: not wanted), read by bwd */
+    m2d_recur_tensor d_y;          /*                                                                       [bwd] */
+    const float *d_state_out;      /* (B,C) dense, or NULL: zero */
+    void *d_x, *d_gate;            /* (B,T,C) dense */
+    float *d_state;                /* (B,C) dense, or NULL: not wanted */
+} m2d_recur_desc;
+
+uint64_t m2d_recur_marks(const m2d_recur_desc *desc);   /* states that the forward pass keeps for the backward pass (reads B, T and C) */
+int m2d_recur_fwd(const m2d_recur_desc *desc, void *stream);
+int m2d_recur_bwd(const m2d_recur_desc *desc, void *stream);
+
+/* One token of every sequence: T = 1; state is read and state_out written (they may be the same array), sequences state_batch apart. */
+int m2d_recur_step(const m2d_recur_desc *desc, int64_t state_batch, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,47 +1,15 @@
 // Eager entry points of the sequence operators (sequence.py): linear attention, group normalisation, clipping.
 //
 // Arguments are checked here (in Python the checks took longer than a small call's kernel).
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
+#include "torch_seq.h"
 
-#include <algorithm>
-#include <climits>
-#include <cmath>
-
-#include "m2d_seq.h"
+void bind_recurrence(pybind11::module& m);        // torch_recur.cpp
 
 namespace {
 
-using at::Tensor;
-using c10::optional;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace m2d_entry;
 
-void check(int rc, const char* fn) { TORCH_CHECK(rc == M2D_OK, fn, " failed: ", m2d_strerror(rc), " (status ", rc, ")"); }
-void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
-int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? M2D_F32 : M2D_BF16; }
-Tensor scratch(uint64_t bytes, const Tensor& like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
-
-// Whether a call on these makes a node (one with a forward-mode tangent does: the node refuses it).
-bool wants_grad(std::initializer_list<const Tensor*> inputs) {
-    bool grad = false;
-    for (const Tensor* t : inputs)
-        if (t->defined()) grad = grad || (at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
-    return grad;
-}
-// A wait between warps of an earlier launch that gave up (its results are NaN) surfaces at the next call.
-void check_waits(const char* what) { TORCH_CHECK(!m2d_take_wait_failure(), what, ": a wait inside an earlier launch timed out; the results of that launch are invalid"); }
-Tensor or_none(const optional<Tensor>& t) { return t ? *t : Tensor(); }
-// neighbours along the last dimension
-Tensor rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 m2d_attn_tensor attn_tensor(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
-void wrote(const Tensor& t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
 
 // ---- linear attention -------------------------------------------------------------------------------
 
@@ -161,14 +129,8 @@ std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Ten
                                                       const optional<Tensor>& state_, const optional<Tensor>& lengths_, bool want_state) {
     const char* const what = "linear_attention";
     const Tensor state = or_none(state_);
-    Tensor lengths = or_none(lengths_);
     check_attn(what, "BT", q, k, v, log_decay, state);
-    if (lengths.defined()) {
-        TORCH_CHECK(lengths.dim() == 1 && lengths.size(0) == v.size(0) && (lengths.scalar_type() == at::kInt || lengths.scalar_type() == at::kLong), what,
-                    ": lengths must be (B) integers, got ", lengths.sizes(), " ", lengths.scalar_type());
-        TORCH_CHECK(lengths.device() == v.device(), what, ": lengths are on ", lengths.device(), ", expected ", v.device());
-        if (lengths.scalar_type() == at::kLong) lengths = lengths.clamp(0, v.size(1)).to(at::kInt);
-    }
+    const Tensor lengths = token_counts(what, or_none(lengths_), v);
     if (v.size(0) == 0 || v.size(1) == 0) {
         if (!want_state) return {v.clone(), c10::nullopt};
         return {v.clone(), state.defined() ? state.clone() : at::zeros({v.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat))};
@@ -360,6 +322,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm) {
 }  // namespace
 
 void bind_sequence_operators(pybind11::module& m) {
+    bind_recurrence(m);
     using pybind11::arg;
     m.def("linear_attention", &linear_attention, "linear attention of whole sequences: (o, state or None)", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale").none(true),
           arg("state").none(true), arg("lengths").none(true), arg("want_state"));

@@ -1,9 +1,11 @@
 """Sequence operators next to the 2-D scan: linear attention with a decay per head (the scan's relative in one dimension,
-with a matrix for a state), group normalisation with an activation on the channels-last tensors that all of this
+with a matrix for a state), a gated recurrence with a state per channel, group normalisation with an activation on the channels-last tensors that all of this
 package works on, and clipping of gradients by their global norm.
 
   linear_attention(q, k, v, log_decay, ...)         whole sequences, forward and backward
   linear_attention_step(q, k, v, log_decay, state)  one token of every sequence, the state updated in place
+  gated_recurrence(x, gate, ...)                    whole sequences, forward and backward
+  gated_recurrence_step(x, gate, state, ...)        one token of every sequence, the state updated in place
   group_norm(x, groups, weight, bias, ...)          x (N, ..., C)
   clip_norm_(tensors, max_norm)                     global norm of many tensors, all scaled in place
   clip_grad_norm_(parameters, max_norm)             of parameters' gradients: what ``refmodel.train_step`` calls
@@ -16,9 +18,10 @@ import torch
 
 from . import _lib
 
-__all__ = ["linear_attention", "linear_attention_step", "group_norm", "clip_norm_", "clip_grad_norm_"]
+__all__ = ["linear_attention", "linear_attention_step", "gated_recurrence", "gated_recurrence_step", "group_norm", "clip_norm_", "clip_grad_norm_"]
 
 _ACTS = {None: 0, "silu": 1, "gelu": 2}
+_GATES = {"decay": 0, "forget": 1}
 
 
 def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
@@ -61,6 +64,46 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None):
     if state is None:
         raise RuntimeError("linear_attention_step: there is no state")
     return _lib.entry().linear_attention_step(q, k, v, log_decay, state, scale)
+
+
+def gated_recurrence(x, gate, *, form="decay", initial_state=None, lengths=None, return_state=False):
+    """``h_t = a_t h_{t-1} + u_t`` for every sequence and channel; returns all h.
+
+    Args:
+        x, gate: (B, T, C) of one type.  Any strides (a last dimension that is not dense is copied): a gate per channel or
+            per token may be expanded over the rest, and gets its gradient.
+        form: "decay": ``a = exp(gate)``, ``u = x``; gate at most 0, a positive value grows the state and is not checked for.
+            "forget": ``a = sigmoid(gate)``, ``u = (1 - a) x``.  A gate of -inf forgets all earlier tokens (if they
+            are finite).
+        initial_state: (B, C) float32, or None for zero.
+        lengths: (B,) integers on the device, tokens of each sequence (clamped to 0 ... T), or None for T.  Rows
+            behind them are not read; outputs and gradients there are zero.
+        return_state: also return the state after each sequence's last token, (B, C) float32.
+    Returns:
+        h (B, T, C) in ``x.dtype``, or ``(h, state)``.
+    Differentiable in x, gate and initial_state, once (``create_graph`` raises); those of x and gate are computed together.
+    States are carried in float32 and gradients computed from them, whatever the type of h.  A token that is not finite spoils
+    later ones of its sequence and channel (in the backward pass earlier ones), as by the formula.
+    """
+    if form not in _GATES:
+        raise ValueError(f"gated_recurrence: unknown form, got {form}...")
+    h, state = _lib.entry().gated_recurrence(x, gate, _GATES[form], initial_state, lengths, return_state)
+    return (h, state) if return_state else h
+
+
+def gated_recurrence_step(x, gate, state, *, form="decay"):
+    """One token of every sequence: ``state`` becomes ``a state + u`` in place, which is the result in ``x.dtype``.
+
+    Args:
+        x, gate: (B, C) of one type, as ``gated_recurrence`` takes them.
+        state: (B, C) float32, dense along C; sequences may lie apart (a layer's slice of a cache) but must not overlap.
+    No gradients: it raises where one is wanted.
+    """
+    if form not in _GATES:
+        raise ValueError(f"gated_recurrence_step: unknown form, got {form}...")
+    if state is None:
+        raise RuntimeError("gated_recurrence_step: there is no state")
+    return _lib.entry().gated_recurrence_step(x, gate, state, _GATES[form])
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None):

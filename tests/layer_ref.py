@@ -1,0 +1,83 @@
+"""Definitions in 64 bits of the gated recurrence, the layer norm and the distillation loss, and the recurrence's bound on what a result may be off by.
+
+The recurrence's weights are all positive, so what rounding does to h_t is bounded by the same operator on magnitudes, H_t = a_t H_{t-1} + |u_t|:
+  - a run's tokens (up to 16) are weighted by products of up to 16 gates, each off by 2^-22 of itself (the approximate exponential's and
+    reciprocal's error, and the gate's own rounding), and what is carried from run to run by the sum of their logarithms: 2^-17 of H_t covers
+    both, twice;
+  - every token's state is rounded once, and twice more where runs are joined: 1.25 * 2^-24 of H_t, each carried on like a state.
+"""
+import torch
+
+
+def terms(x, gate, form):
+    return (gate.exp(), x) if form == "decay" else (gate.sigmoid(), x * (-gate).sigmoid())
+
+
+def scan(a, u, state=None, lengths=None):
+    """(h, final state), token by token."""
+    B, T, C = u.shape
+    h = torch.zeros(B, C, dtype=u.dtype, device=u.device) if state is None else state
+    out = []
+    for t in range(T):
+        new = a[:, t] * h + u[:, t]
+        if lengths is not None:
+            inside = (lengths > t)[:, None]
+            h = torch.where(inside, new, h)
+            out.append(torch.where(inside, new, 0.0))
+        else:
+            h = new
+            out.append(new)
+    return torch.stack(out, 1), h
+
+
+def recurrence(x, gate, form, state=None, lengths=None):
+    if lengths is not None:              # rows behind a sequence may hold anything
+        live = (torch.arange(x.shape[1], device=x.device) < lengths[:, None])[..., None]
+        x, gate = torch.where(live, x, 0.0), torch.where(live, gate, 0.0)
+    return scan(*terms(x, gate, form), state, lengths)
+
+
+def rounded(a, H, lengths=None):
+    """The bound above, for states of magnitude H."""
+    return 2.0 ** -17 * H + 1.25 * 2.0 ** -24 * scan(a, H, None, lengths)[0]
+
+
+def recurrence_bounds(x, gate, form, state, lengths, dy=None, d_state=None):
+    """Bounds on h (and, with dy, on dx, dgate and the state's gradient), in the order of ``h, final, dx, dgate, dstate``."""
+    if lengths is not None:
+        live = (torch.arange(x.shape[1], device=x.device) < lengths[:, None])[..., None]
+        x, gate = torch.where(live, x, 0.0), torch.where(live, gate, 0.0)
+        dy = None if dy is None else torch.where(live, dy, 0.0)
+    a, u = terms(x, gate, form)
+    state = torch.zeros_like(x[:, 0]) if state is None else state.abs()
+    H, last = scan(a, u.abs(), state, lengths)
+    h = rounded(a, H, lengths)
+    n = torch.full((x.shape[0],), x.shape[1], device=x.device) if lengths is None else lengths
+    final = torch.where((n > 0)[:, None], h[torch.arange(len(h), device=h.device), (n - 1).clamp(min=0)], 0.0)
+    if dy is None:
+        return h, final
+    if lengths is not None:              # (rows behind a sequence pass the state's gradient on)
+        a = torch.where(live, a, 1.0)
+    D = scan(torch.cat((a[:, 1:], torch.ones_like(a[:, :1])), 1).flip(1), torch.cat((dy[:, :-1].abs(), dy[:, -1:].abs() + (0 if d_state is None else d_state.abs()[:, None])), 1).flip(1))[0].flip(1)
+    dD = rounded(torch.cat((a[:, 1:], torch.ones_like(a[:, :1])), 1).flip(1), D.flip(1)).flip(1)
+    before, dbefore = torch.cat((state[:, None], H[:, :-1]), 1), torch.cat((torch.zeros_like(h[:, :1]), h[:, :-1]), 1)
+    if form == "decay":
+        dx, dg = dD, a * (dD * before + D * dbefore)
+    else:
+        rest = (-gate).sigmoid()
+        dx, dg = rest * dD, a * rest * (dD * (before + x.abs()) + D * dbefore)
+    # (the gates' own factors: four of them, each off by 2^-21 at most)
+    dx = dx + 2.0 ** -19 * D
+    dg = dg + 2.0 ** -19 * a * D * (before + x.abs())
+    return h, final, dx, dg, a[:, 0] * (dD[:, 0] + 2.0 ** -19 * D[:, 0])
+
+
+def within(got, want, bound):
+    """Largest error over (bound + the result's own rounding); infinite where one is not finite and the other is."""
+    assert got.shape == want.shape, (got.shape, want.shape)
+    if not got.numel():
+        return 0.0
+    if not bool(torch.isfinite(got).all()):
+        return float("inf")
+    allowed = bound + torch.finfo(got.dtype).eps / 2 * want.abs() + 1e-36
+    return float(((got.double() - want).abs() / allowed).max())
