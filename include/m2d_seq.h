@@ -1,7 +1,7 @@
 /*
  * m2d_seq.h -- C ABI of the sequence operators next to the wavefront scan: linear attention with a decay per head,
  * group normalisation with an activation on channels-last tensors, clipping by the global norm of many tensors, a gated
- * recurrence per channel.
+ * recurrence per channel, layer normalisation.
  *
  * Conventions are those of m2d_scan.h: device pointers, memory owned by the caller, asynchronous on `stream` (of the
  * current device), status codes, re-entrant, nothing kept between calls.  Strides are in elements.
@@ -164,6 +164,40 @@ int m2d_recur_bwd(const m2d_recur_desc *desc, void *stream);
 
 /* One token of every sequence: T = 1; state is read and state_out written (they may be the same array), sequences state_batch apart. */
 int m2d_recur_step(const m2d_recur_desc *desc, int64_t state_batch, void *stream);
+
+/* ---- layer normalisation ----------------------------------------------------------------------------------------
+ * Rows x (N,C): s = x + residual, rounded to the tensors' type; y = (s - mean) / sqrt(var + eps) * weight + bias.  Rows lie as far apart as is
+ * given, neighbours along C.  Rows that begin at 16-byte boundaries and are whole 16-byte pieces, parameters too, are read in such pieces.  Rows of
+ * more than 16384 values (8192 in single reads and in the backward pass) are read three times.  N below 2^31, C up to 2^30.
+ */
+typedef struct m2d_ln_desc {
+    uint32_t struct_bytes;         /* = sizeof(m2d_ln_desc) */
+    int32_t dtype;                 /* m2d_dtype of x, residual, sum, y and their gradients */
+    int64_t N;
+    int32_t C;
+    int32_t params_f32;            /* weight and bias (and their gradients) are fp32, else of `dtype` */
+    float eps;
+    const void *x;                 /* fwd: x; bwd: what was normalised (x, or the sum) */
+    int64_t x_row;
+    const void *residual;          /* or NULL                                                      [fwd] */
+    int64_t residual_row;
+    const void *weight, *bias;     /* (C), or NULL: one and zero */
+    void *sum;                     /* (N,C) dense: x + residual, where there is one                [fwd] */
+    void *y;                       /* (N,C) dense                                                  [fwd] */
+    float *stats;                  /* (N,2): mean, 1 / sqrt(var + eps); written by fwd (NULL: not wanted), read by bwd */
+    const void *d_y;               /*                                                              [bwd] */
+    int64_t d_y_row;
+    const void *d_sum;             /* added to d_x, or NULL */
+    int64_t d_sum_row;
+    void *d_x;                     /* (N,C) dense */
+    void *d_weight, *d_bias;       /* (C), or NULL: not wanted */
+    void *workspace;               /* scratch, 256-byte aligned */
+    uint64_t workspace_bytes;
+} m2d_ln_desc;
+
+uint64_t m2d_ln_bwd_workspace(const m2d_ln_desc *desc);     /* asked with the call's own descriptor, all but the workspace in it */
+int m2d_ln_fwd(const m2d_ln_desc *desc, void *stream);
+int m2d_ln_bwd(const m2d_ln_desc *desc, void *stream);
 
 #ifdef __cplusplus
 }

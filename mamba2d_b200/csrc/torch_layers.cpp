@@ -1,4 +1,4 @@
-// Eager entry points of the gated recurrence (sequence.py).
+// Eager entry points of the gated recurrence and of layer normalisation (sequence.py).
 #include "torch_seq.h"
 
 namespace {
@@ -138,11 +138,127 @@ Tensor gated_recurrence_step(const Tensor& x, const Tensor& gate, const Tensor& 
     return y;
 }
 
+// ---- layer normalisation ----------------------------------------------------------------------------
+
+m2d_ln_desc ln_desc(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+    m2d_ln_desc d{};
+    d.struct_bytes = sizeof(d);
+    d.dtype = dtype_of(x);
+    d.N = x.size(0); d.C = (int)x.size(1);
+    const Tensor& p = weight.defined() ? weight : bias;
+    d.params_f32 = p.defined() && p.scalar_type() == at::kFloat;
+    d.eps = (float)eps;
+    d.x = x.data_ptr(); d.x_row = x.stride(0);
+    d.weight = ptr(weight); d.bias = ptr(bias);
+    return d;
+}
+// As rows (N, C) with neighbours along C: a view where there is one.
+Tensor matrix(const Tensor& t) {
+    const Tensor m = rows(t).reshape({-1, t.size(-1)});
+    return m.size(0) == 1 || m.stride(0) >= 0 ? m : m.contiguous();
+}
+Tensor ln_forward(m2d_ln_desc& d, const Tensor& x, const Tensor& residual, const Tensor& like, Tensor* sum) {
+    Tensor r;
+    if (residual.defined()) {
+        r = matrix(residual);
+        d.residual = r.data_ptr();
+        d.residual_row = r.stride(0);
+        *sum = at::empty(like.sizes(), x.options());
+        d.sum = sum->data_ptr();
+    }
+    const Tensor y = at::empty(like.sizes(), x.options());
+    d.y = y.data_ptr();
+    check(m2d_ln_fwd(&d, stream_of(x)), "m2d_ln_fwd");
+    return y;
+}
+
+class LnFn : public torch::autograd::Function<LnFn> {
+public:
+    static variable_list forward(AutogradContext* ctx, const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, const optional<Tensor>& residual_, double eps) {
+        const Tensor weight = or_none(weight_), bias = or_none(bias_), residual = or_none(residual_);
+        const c10::cuda::CUDAGuard guard(x_.device());
+        const Tensor x = matrix(x_), w = dense(weight), b = dense(bias);
+        m2d_ln_desc d = ln_desc(x, w, b, eps);
+        const Tensor stats = at::empty({d.N, 2}, x.options().dtype(at::kFloat));
+        d.stats = fptr(stats);
+        Tensor sum;
+        const Tensor y = ln_forward(d, x, residual, x_, &sum);
+        ctx->save_for_backward({sum.defined() ? sum : x_, weight, bias, stats});
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return sum.defined() ? variable_list{y, sum} : variable_list{y};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm: gradients of gradients (create_graph) are not supported");
+        const variable_list s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[0].device());
+        const bool residual = grads.size() > 1;
+        const Tensor ds_ = residual ? grads[1] : Tensor();
+        if (!grads[0].defined()) {                 // the sum alone was used
+            auto none = [](const Tensor& t) { return t.defined() && t.requires_grad() ? at::zeros(t.sizes(), t.options()) : Tensor(); };
+            return {ds_, none(s[1]), none(s[2]), ds_, Tensor()};
+        }
+        const Tensor x = matrix(s[0]), w = dense(s[1]), b = dense(s[2]), dy = matrix(grads[0].to(x.scalar_type())), ds = ds_.defined() ? matrix(ds_.to(x.scalar_type())) : ds_;
+        m2d_ln_desc d = ln_desc(x, w, b, ctx->saved_data["eps"].toDouble());
+        d.stats = fptr(s[3]);
+        d.d_y = dy.data_ptr(); d.d_y_row = dy.stride(0);
+        if (ds.defined()) { d.d_sum = ds.data_ptr(); d.d_sum_row = ds.stride(0); }
+        const Tensor dx = at::empty(s[0].sizes(), x.options());
+        d.d_x = dx.data_ptr();
+        Tensor dw, db;
+        if (s[1].defined() && s[1].requires_grad()) { dw = at::empty({d.C}, s[1].options()); d.d_weight = dw.data_ptr(); }
+        if (s[2].defined() && s[2].requires_grad()) { db = at::empty({d.C}, s[2].options()); d.d_bias = db.data_ptr(); }
+        d.workspace_bytes = m2d_ln_bwd_workspace(&d);
+        Tensor ws;
+        if (d.workspace_bytes) {
+            ws = scratch(d.workspace_bytes, x);
+            d.workspace = ws.data_ptr();
+        }
+        check(m2d_ln_bwd(&d, stream_of(x)), "m2d_ln_bwd");
+        return {dx, dw, db, residual ? dx : Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, optional<Tensor>> layer_norm(const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, const optional<Tensor>& residual_, double eps) {
+    const Tensor weight = or_none(weight_), bias = or_none(bias_), residual = or_none(residual_);
+    TORCH_CHECK(x_.dim() >= 1, "layer_norm: x must be (..., C), got a single value");
+    const int64_t C = x_.size(-1);
+    TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative, got ", eps);
+    TORCH_CHECK(x_.scalar_type() == at::kFloat || x_.scalar_type() == at::kBFloat16, "layer_norm: unsupported dtype ", x_.scalar_type(), " (float32 and bfloat16 only)");
+    for (const Tensor* p : {&weight, &bias})
+        if (p->defined()) {
+            TORCH_CHECK(p->dim() == 1 && p->size(0) == C, "layer_norm: weight and bias must have shape (", C, "), got ", p->sizes());
+            TORCH_CHECK((p->scalar_type() == at::kFloat || p->scalar_type() == x_.scalar_type()) && (!weight.defined() || p->scalar_type() == weight.scalar_type()),
+                        "layer_norm: dtype ", p->scalar_type(), "; weight and bias share one, float32 or ", x_.scalar_type());
+        }
+    if (residual.defined())
+        TORCH_CHECK(residual.sizes() == x_.sizes() && residual.scalar_type() == x_.scalar_type(), "layer_norm: the residual must be like x ", x_.sizes(), " ", x_.scalar_type(), ", got ",
+                    residual.sizes(), " ", residual.scalar_type());
+    TORCH_CHECK(x_.is_cuda(), "layer_norm: tensors must be on a CUDA device (there is no CPU path)");
+    for (const Tensor* p : {&weight, &bias, &residual}) TORCH_CHECK(!p->defined() || p->device() == x_.device(), "layer_norm: tensors on ", p->device(), " and ", x_.device());
+    TORCH_CHECK(C <= INT_MAX && x_.numel() / std::max<int64_t>(C, 1) <= INT_MAX, "layer_norm: a size out of range");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    if (!x_.numel()) return {x_.clone(), residual.defined() ? optional<Tensor>(x_ + residual) : c10::nullopt};
+    if (wants_grad({&x_, &weight, &bias, &residual})) {
+        const variable_list r = LnFn::apply(x_, weight_, bias_, residual_, eps);
+        return {r[0], r.size() > 1 ? optional<Tensor>(r[1]) : c10::nullopt};
+    }
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = matrix(x_), w = dense(weight), b = dense(bias);
+    m2d_ln_desc d = ln_desc(x, w, b, eps);
+    Tensor sum;
+    const Tensor y = ln_forward(d, x, residual, x_, &sum);
+    return {y, sum.defined() ? optional<Tensor>(sum) : c10::nullopt};
+}
+
 }  // namespace
 
-void bind_recurrence(pybind11::module& m) {
+void bind_layers(pybind11::module& m) {
     using pybind11::arg;
     m.def("gated_recurrence", &gated_recurrence, "gated recurrence of whole sequences: (h, state or None)", arg("x"), arg("gate"), arg("form"), arg("state").none(true), arg("lengths").none(true),
           arg("want_state"));
     m.def("gated_recurrence_step", &gated_recurrence_step, "gated recurrence of one token; the state is updated in place", arg("x"), arg("gate"), arg("state"), arg("form"));
+    m.def("layer_norm", &layer_norm, "layer normalisation of rows: (y, the sum that was normalised or None)", arg("x"), arg("weight").none(true), arg("bias").none(true),
+          arg("residual").none(true), arg("eps"));
 }

@@ -3,7 +3,7 @@
 // Arguments are checked here (in Python the checks took longer than a small call's kernel).
 #include "torch_seq.h"
 
-void bind_recurrence(pybind11::module& m);        // torch_recur.cpp
+void bind_layers(pybind11::module& m);            // torch_layers.cpp
 
 namespace {
 
@@ -322,7 +322,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm) {
 }  // namespace
 
 void bind_sequence_operators(pybind11::module& m) {
-    bind_recurrence(m);
+    bind_layers(m);
     using pybind11::arg;
     m.def("linear_attention", &linear_attention, "linear attention of whole sequences: (o, state or None)", arg("q"), arg("k"), arg("v"), arg("log_decay"), arg("scale").none(true),
           arg("state").none(true), arg("lengths").none(true), arg("want_state"));

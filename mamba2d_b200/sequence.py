@@ -7,6 +7,7 @@ package works on, and clipping of gradients by their global norm.
   gated_recurrence(x, gate, ...)                    whole sequences, forward and backward
   gated_recurrence_step(x, gate, state, ...)        one token of every sequence, the state updated in place
   group_norm(x, groups, weight, bias, ...)          x (N, ..., C)
+  layer_norm(x, weight, bias, residual=...)         x (..., C), with the residual sum before it
   clip_norm_(tensors, max_norm)                     global norm of many tensors, all scaled in place
   clip_grad_norm_(parameters, max_norm)             of parameters' gradients: what ``refmodel.train_step`` calls
 
@@ -18,7 +19,8 @@ import torch
 
 from . import _lib
 
-__all__ = ["linear_attention", "linear_attention_step", "gated_recurrence", "gated_recurrence_step", "group_norm", "clip_norm_", "clip_grad_norm_"]
+__all__ = ["linear_attention", "linear_attention_step", "gated_recurrence", "gated_recurrence_step", "group_norm", "layer_norm",
+           "clip_norm_", "clip_grad_norm_"]
 
 _ACTS = {None: 0, "silu": 1, "gelu": 2}
 _GATES = {"decay": 0, "forget": 1}
@@ -125,6 +127,23 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None):
     if not isinstance(groups, int):
         raise ValueError(f"group_norm: groups must be an integer, got {groups}")
     return _lib.entry().group_norm(x, groups, weight, bias, eps, _ACTS[act])
+
+
+def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
+    """``(s - mean) / sqrt(var + eps) * weight + bias`` of every row, ``s = x + residual``.
+
+    Args:
+        x: (..., C); mean and (biased) variance are taken over the last dimension, in float32.
+        weight, bias: (C,) or None; float32, or both of x's type.
+        residual: like x, or None.  The sum is rounded to x's type and that is what is normalised.
+    Returns:
+        y in x's type, or ``(y, s)`` where there is a residual: s goes on to the next layer.
+    Differentiable in x, weight, bias and residual, once (``create_graph`` raises); x and residual get the same gradient, one
+    tensor.  Rows may lie apart (a slice of a wider tensor); other strides are copied.  Rows that are not whole 16-byte
+    pieces are read value by value; rows of more than 16384 values (8192 of such, and in the backward pass) are read three times.
+    """
+    y, total = _lib.entry().layer_norm(x, weight, bias, residual, eps)
+    return y if residual is None else (y, total)
 
 
 def clip_norm_(tensors, max_norm, error_if_nonfinite=False):

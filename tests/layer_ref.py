@@ -1,4 +1,4 @@
-"""Definitions in 64 bits of the gated recurrence, the layer norm and the distillation loss, and the recurrence's bound on what a result may be off by.
+"""Definitions in 64 bits of the gated recurrence and the layer norm, and bounds on what their results may be off by.
 
 The recurrence's weights are all positive, so what rounding does to h_t is bounded by the same operator on magnitudes, H_t = a_t H_{t-1} + |u_t|:
   - a run's tokens (up to 16) are weighted by products of up to 16 gates, each off by 2^-22 of itself (the approximate exponential's and
@@ -81,3 +81,35 @@ def within(got, want, bound):
         return float("inf")
     allowed = bound + torch.finfo(got.dtype).eps / 2 * want.abs() + 1e-36
     return float(((got.double() - want).abs() / allowed).max())
+
+
+def norm(x, weight, bias, eps=1e-5):
+    d = x - x.mean(-1, keepdim=True)
+    h = d / (d.square().mean(-1, keepdim=True) + eps).sqrt()
+    return (h if weight is None else h * weight) + (0.0 if bias is None else bias)
+
+
+def norm_bounds(x, weight, bias, dy=None, eps=1e-5):
+    """What (y, dx, dw, db) may be off by before their own rounding, in steps e = 2^-24.  A sum of C values has k = 64 + C / 512 roundings on a
+    value's way (a thread's share, then a tree); the mean is taken about the first value, so its error is that of a mean of
+    distances from it; h is off by the mean's error and by some 3 k / 2 steps of its own."""
+    e, C, N = 2.0 ** -24, x.shape[-1], x.numel() // x.shape[-1]
+    k = 64 + C / 512
+    mean = x.mean(-1, keepdim=True)
+    d = x - mean
+    rstd = 1 / (d.square().mean(-1, keepdim=True) + eps).sqrt()
+    w = torch.ones_like(x[..., :1]) if weight is None else weight
+    off_mean = k * e * (x - x[..., :1]).abs().mean(-1, keepdim=True) + 2 * e * mean.abs()
+    h = d * rstd
+    dh = rstd * off_mean + 2 * k * e * h.abs()
+    y = w.abs() * dh + 4 * e * ((h * w).abs() + (0.0 if bias is None else bias.abs()))
+    if dy is None:
+        return y
+    g = dy * w
+    m0, m1 = g.mean(-1, keepdim=True), (g * h).mean(-1, keepdim=True)
+    off0 = k * e * g.abs().mean(-1, keepdim=True)
+    off1 = k * e * (g * h).abs().mean(-1, keepdim=True) + (g.abs() * dh).mean(-1, keepdim=True)
+    dx = rstd * (off0 + h.abs() * off1 + dh * m1.abs()) + (k + 8) * e * rstd * (g.abs() + m0.abs() + (h * m1).abs())
+    rows = 64 + N / 32                   # (a thread's rows one after another, then CTAs in turn)
+    over = lambda t: t.reshape(-1, C).sum(0)  # noqa: E731
+    return y, dx, over(dy.abs() * dh) + rows * e * over((dy * h).abs()), rows * e * over(dy.abs())

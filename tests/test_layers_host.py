@@ -1,11 +1,11 @@
-"""The gated recurrence without a device: refusals of the Python entry points and of the C ABI."""
+"""The gated recurrence and layer normalisation without a device: refusals of the Python entry points and of the C ABI."""
 import ctypes
 
 import pytest
 import torch
 
 import mamba2d_b200
-from mamba2d_b200 import _lib, gated_recurrence, gated_recurrence_step
+from mamba2d_b200 import _lib, gated_recurrence, gated_recurrence_step, layer_norm
 
 OK, NULL, DTYPE, SHAPE, WORKSPACE, ABI, LARGE, FLAGS, PITCH = 0, -1, -2, -3, -6, -8, -9, -10, -5
 
@@ -21,12 +21,20 @@ class RecurDesc(ctypes.Structure):
                 *[(n, ctypes.c_void_p) for n in ("d_state_out", "d_x", "d_gate", "d_state")]]
 
 
+class LnDesc(ctypes.Structure):
+    """Mirror of ``m2d_ln_desc``."""
+    _fields_ = [("struct_bytes", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("N", ctypes.c_int64), ("C", ctypes.c_int32), ("params_f32", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("x", ctypes.c_void_p), ("x_row", ctypes.c_int64), ("residual", ctypes.c_void_p), ("residual_row", ctypes.c_int64),
+                *[(n, ctypes.c_void_p) for n in ("weight", "bias", "sum", "y", "stats", "d_y")], ("d_y_row", ctypes.c_int64), ("d_sum", ctypes.c_void_p), ("d_sum_row", ctypes.c_int64),
+                *[(n, ctypes.c_void_p) for n in ("d_x", "d_weight", "d_bias", "workspace")], ("workspace_bytes", ctypes.c_uint64)]
+
+
 @pytest.fixture(scope="module")
 def L():
     from mamba2d_b200 import build
     build.build()
     raw = ctypes.CDLL(_lib.LIB_PATH)
-    raw.m2d_recur_marks.restype = ctypes.c_uint64
+    raw.m2d_recur_marks.restype = raw.m2d_ln_bwd_workspace.restype = ctypes.c_uint64
     return raw
 
 
@@ -68,6 +76,35 @@ def test_refusals_of_the_recurrence():
         gated_recurrence_step(x[:, 0], g[:, 0], None)
 
 
-def test_the_package_has_the_recurrence():
-    for n in ("gated_recurrence", "gated_recurrence_step"):
+def test_layer_norm_descriptors(L):
+    def desc(**kw):
+        d = LnDesc(struct_bytes=ctypes.sizeof(LnDesc), dtype=1, N=10, C=64, eps=1e-5)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return ctypes.byref(d)
+    for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"N": 0}, SHAPE), ({"C": 0}, SHAPE), ({"N": 1 << 31}, LARGE), ({"C": (1 << 30) + 1}, LARGE)):
+        assert L.m2d_ln_fwd(desc(**kw), None) == rc and L.m2d_ln_bwd(desc(**kw), None) == rc, kw
+    assert L.m2d_ln_fwd(None, None) == NULL and L.m2d_ln_fwd(desc(x=256, y=256, residual=256), None) == NULL        # nowhere to put the sum
+    p = dict(x=256, x_row=64, d_y=256, d_y_row=64, d_x=256, stats=256, d_weight=256)
+    need = L.m2d_ln_bwd_workspace(desc(**p))
+    assert need >= 2 * 4 * 64 and L.m2d_ln_bwd_workspace(desc(**{**p, "d_weight": None})) == 0
+    for kw in ({}, {"workspace": 256, "workspace_bytes": need - 1}, {"workspace": 128, "workspace_bytes": need}):
+        assert L.m2d_ln_bwd(desc(**p, **kw), None) == WORKSPACE
+
+
+def test_refusals_of_layer_norm():
+    x, w = torch.randn(3, 12), torch.randn(12)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        layer_norm(x, w, w, residual=x)
+    for args, kw in (((x.half(),), {}), ((x.double(),), {}), ((x, w[:5]), {}), ((x, w.bfloat16()), {}), ((x, w, w.double()), {}), ((x, w[None]), {}), ((x.sum(),), {}),
+                     ((x,), {"residual": x[:2]}), ((x,), {"residual": x.bfloat16()}), ((x,), {"residual": x[0]})):
+        with pytest.raises(RuntimeError):
+            layer_norm(*args, **kw)
+    for eps in (-1.0, float("nan")):
+        with pytest.raises(ValueError):
+            layer_norm(x, eps=eps)
+
+
+def test_the_package_has_them():
+    for n in ("gated_recurrence", "gated_recurrence_step", "layer_norm"):
         assert n in mamba2d_b200.__all__ and callable(getattr(mamba2d_b200, n))
