@@ -1,7 +1,7 @@
 /*
  * m2d_seq.h -- C ABI of the sequence operators next to the wavefront scan: linear attention with a decay per head,
  * group normalisation with an activation on channels-last tensors, clipping by the global norm of many tensors, a gated
- * recurrence per channel, layer normalisation.
+ * recurrence per channel, layer normalisation, distillation from a teacher's top logits.
  *
  * Conventions are those of m2d_scan.h: device pointers, memory owned by the caller, asynchronous on `stream` (of the
  * current device), status codes, re-entrant, nothing kept between calls.  Strides are in elements.
@@ -198,6 +198,40 @@ typedef struct m2d_ln_desc {
 uint64_t m2d_ln_bwd_workspace(const m2d_ln_desc *desc);     /* asked with the call's own descriptor, all but the workspace in it */
 int m2d_ln_fwd(const m2d_ln_desc *desc, void *stream);
 int m2d_ln_bwd(const m2d_ln_desc *desc, void *stream);
+
+/* ---- distillation from a teacher's top logits -----------------------------------------------------------------------
+ * Per row, with q = softmax(z / temperature) over its V logits and p = softmax(t / temperature) over the teacher's K entries (index, t):
+ *     loss = (1 - label_weight) temperature^2 sum_k p_k (log p_k - log q_{index_k}) + label_weight (log sum_j exp(z_j) - z_label).
+ * An entry whose index is not in 0 ... V - 1 is absent; a row without entries (or with t = -inf in all of them) has no first part, one whose
+ * label is not in 0 ... V - 1 no second.  An index may come more than once.  N below 2^25, V below 2^31 - 2^16, K up to M2D_DISTILL_MAX_TOP.
+ */
+#define M2D_DISTILL_MAX_TOP 512
+
+typedef struct m2d_distill_desc {
+    uint32_t struct_bytes;         /* = sizeof(m2d_distill_desc) */
+    int32_t dtype;                 /* m2d_dtype of logits and their gradient */
+    int32_t teacher_dtype;         /* m2d_dtype of teacher */
+    int32_t V, K;
+    int32_t index_64, labels_64;   /* int64_t, else int32_t */
+    float temperature, label_weight;   /* positive; 0 ... 1 */
+    int64_t N;
+    const void *logits;            /* (N,V), neighbours along V, rows logits_row apart */
+    int64_t logits_row;
+    const void *teacher;           /* (N,K) */
+    int64_t teacher_row;
+    const void *index;             /* (N,K) */
+    int64_t index_row;
+    const void *labels;            /* (N), read where label_weight > 0 */
+    float *loss;                   /* (N)                                                           [fwd] */
+    float *stats;                  /* m2d_distill_stats() values: written by fwd (NULL: not wanted), read by bwd */
+    const float *d_loss;           /* d_loss[n * d_loss_row]                                        [bwd] */
+    int64_t d_loss_row;
+    void *d_logits;                /* (N,V) dense */
+} m2d_distill_desc;
+
+uint64_t m2d_distill_stats(const m2d_distill_desc *desc);
+int m2d_distill_fwd(const m2d_distill_desc *desc, void *stream);
+int m2d_distill_bwd(const m2d_distill_desc *desc, void *stream);
 
 #ifdef __cplusplus
 }

@@ -6,12 +6,12 @@
 overlapped; ``mamba2d_b200.sequence`` has the sequence operators next to the scan.
 """
 from .host_pipeline import HostScanPipeline, ScanTicket  # noqa: F401
-from .sequence import (clip_grad_norm_, clip_norm_, gated_recurrence, gated_recurrence_step, group_norm,  # noqa: F401
-                       layer_norm, linear_attention, linear_attention_step)
+from .sequence import (clip_grad_norm_, clip_norm_, distillation_loss, gated_recurrence, gated_recurrence_step,  # noqa: F401
+                       group_norm, layer_norm, linear_attention, linear_attention_step)
 from .wavefront_cuda import (proj_params, scan_bwd, scan_fwd, wavefront_scan_cuda, wf_cuda_fn_fr,  # noqa: F401
                              wf_cuda_fn_pr)
 
 __all__ = ["wavefront_scan_cuda", "wf_cuda_fn_pr", "wf_cuda_fn_fr", "proj_params", "scan_fwd", "scan_bwd",
            "HostScanPipeline", "ScanTicket", "linear_attention", "linear_attention_step", "gated_recurrence",
-           "gated_recurrence_step", "group_norm", "layer_norm",
+           "gated_recurrence_step", "group_norm", "layer_norm", "distillation_loss",
            "clip_norm_", "clip_grad_norm_"]

@@ -17,7 +17,7 @@ OUT = os.path.join(HERE, "libm2d_scan.so")
 ENTRY = os.path.join(HERE, "_entry.so")  # native eager entry points (Python extension)
 OBJ = os.path.join(HERE, "_obj")          # per-source objects (git-ignored, not shipped)
 SOURCES = ["m2d_abi.cu", "m2d_scan_fwd.cu", "m2d_scan_bwd.cu", "m2d_scan_fwd_noalloc.cu", "m2d_proj.cu", "m2d_gemm.cu",
-           "m2d_attn.cu", "m2d_norm.cu", "m2d_clip.cu", "m2d_recur.cu", "m2d_ln.cu"]
+           "m2d_attn.cu", "m2d_norm.cu", "m2d_clip.cu", "m2d_recur.cu", "m2d_ln.cu", "m2d_distill.cu"]
 ENTRY_SOURCES = ["torch_entry.cpp", "torch_seq.cpp", "torch_layers.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -1,4 +1,4 @@
-// Eager entry points of the gated recurrence and of layer normalisation (sequence.py).
+// Eager entry points of the gated recurrence, layer normalisation and the distillation loss (sequence.py).
 #include "torch_seq.h"
 
 namespace {
@@ -252,6 +252,97 @@ std::tuple<Tensor, optional<Tensor>> layer_norm(const Tensor& x_, const optional
     return {y, sum.defined() ? optional<Tensor>(sum) : c10::nullopt};
 }
 
+// ---- distillation -----------------------------------------------------------------------------------
+
+struct Distill {
+    Tensor z, t, index, labels;               // as the kernels read them: rows
+    m2d_distill_desc d{};
+    Distill(const Tensor& z_, const Tensor& t_, const Tensor& index_, const Tensor& labels_, double temperature, double weight)
+        : z(matrix(z_)), t(matrix(t_)), index(matrix(index_)), labels(labels_.defined() ? labels_.reshape(-1).contiguous() : labels_) {
+        d.struct_bytes = sizeof(d);
+        d.dtype = dtype_of(z);
+        d.teacher_dtype = dtype_of(t);
+        d.N = z.size(0); d.V = (int)z.size(1); d.K = (int)t.size(1);
+        d.index_64 = index.scalar_type() == at::kLong;
+        d.labels_64 = labels.defined() && labels.scalar_type() == at::kLong;
+        d.temperature = (float)temperature;
+        d.label_weight = (float)weight;
+        d.logits = z.data_ptr(); d.logits_row = z.stride(0);
+        d.teacher = t.data_ptr(); d.teacher_row = t.stride(0);
+        d.index = index.data_ptr(); d.index_row = index.stride(0);
+        d.labels = ptr(labels);
+    }
+    Tensor forward(at::IntArrayRef shape, Tensor* stats) {
+        const auto f32 = z.options().dtype(at::kFloat);
+        const Tensor loss = at::empty(shape, f32);
+        d.loss = fptr(loss);
+        if (stats) {
+            *stats = at::empty({(int64_t)m2d_distill_stats(&d)}, f32);
+            d.stats = fptr(*stats);
+        }
+        check(m2d_distill_fwd(&d, stream_of(z)), "m2d_distill_fwd");
+        return loss;
+    }
+};
+
+class DistillFn : public torch::autograd::Function<DistillFn> {
+public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& z, const Tensor& t, const Tensor& index, const optional<Tensor>& labels_, double temperature, double weight) {
+        const Tensor labels = or_none(labels_);
+        const c10::cuda::CUDAGuard guard(z.device());
+        Distill r(z, t, index, labels, temperature, weight);
+        Tensor stats;
+        const Tensor loss = r.forward(z.sizes().slice(0, z.dim() - 1), &stats);
+        ctx->save_for_backward({z, t, index, labels, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["weight"] = weight;
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "distillation_loss: gradients of gradients (create_graph) are not supported");
+        const variable_list s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[0].device());
+        Distill r(s[0], s[1], s[2], s[3], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["weight"].toDouble());
+        const Tensor up = grads[0].to(at::kFloat).reshape(-1);
+        r.d.d_loss = fptr(up);
+        r.d.d_loss_row = up.size(0) > 1 ? up.stride(0) : 0;
+        r.d.stats = fptr(s[4]);
+        const Tensor dz = at::empty(s[0].sizes(), r.z.options());
+        r.d.d_logits = dz.data_ptr();
+        check(m2d_distill_bwd(&r.d, stream_of(r.z)), "m2d_distill_bwd");
+        return {dz, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor distillation_loss(const Tensor& z, const Tensor& t, const Tensor& index, const optional<Tensor>& labels_, double temperature, double weight) {
+    const char* const what = "distillation_loss";
+    const Tensor labels = or_none(labels_);
+    auto whole = [](const Tensor& i) { return i.scalar_type() == at::kInt || i.scalar_type() == at::kLong; };
+    auto real = [](const Tensor& f) { return f.scalar_type() == at::kFloat || f.scalar_type() == at::kBFloat16; };
+    TORCH_CHECK(z.dim() >= 1 && t.dim() == z.dim() && index.sizes() == t.sizes() && t.sizes().slice(0, t.dim() - 1) == z.sizes().slice(0, z.dim() - 1), what,
+                ": logits (..., V) and the teacher's logits and indices (..., K) do not match, got ", z.sizes(), ", ", t.sizes(), " and ", index.sizes());
+    TORCH_CHECK(t.size(-1) >= 1 && t.size(-1) <= M2D_DISTILL_MAX_TOP && z.size(-1) >= 1, what, ": 1 to ", M2D_DISTILL_MAX_TOP, " logits of the teacher and at least one class, got ", t.sizes(),
+                " and ", z.sizes());
+    TORCH_CHECK(real(z) && real(t), what, ": dtype ", z.scalar_type(), " and ", t.scalar_type(), " (float32 and bfloat16 only)");
+    TORCH_CHECK(whole(index), what, ": indices must be integers, got ", index.scalar_type());
+    TORCH_CHECK_VALUE(temperature > 0 && (float)temperature > 0.f && std::isfinite((float)temperature), what, ": the temperature must be positive, got ", temperature);
+    TORCH_CHECK_VALUE(weight >= 0 && weight <= 1, what, ": label_weight must be in 0 ... 1, got ", weight);
+    TORCH_CHECK_VALUE(labels.defined() == (weight > 0), what, ": labels and a label_weight above 0 go together");
+    if (labels.defined())
+        TORCH_CHECK(whole(labels) && labels.sizes() == z.sizes().slice(0, z.dim() - 1), what, ": labels must be one integer a row of ", z.sizes(), ", got ", labels.sizes(), " ",
+                    labels.scalar_type());
+    TORCH_CHECK(z.is_cuda(), what, ": tensors must be on a CUDA device (there is no CPU path)");
+    for (const Tensor* p : std::initializer_list<const Tensor*>{&t, &index, &labels}) TORCH_CHECK(!p->defined() || p->device() == z.device(), what, ": tensors on ", p->device(), " and ", z.device());
+    TORCH_CHECK(!wants_grad({&t}), what, ": the teacher gets no gradient: detach its logits");
+    const c10::cuda::CUDAGuard guard(z.device());
+    if (!z.numel()) return z.sum(-1).to(at::kFloat);
+    if (wants_grad({&z})) return DistillFn::apply(z, t, index, labels.defined() ? optional<Tensor>(labels) : c10::nullopt, temperature, weight);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    Distill r(z, t, index, labels, temperature, weight);
+    return r.forward(z.sizes().slice(0, z.dim() - 1), nullptr);
+}
+
 }  // namespace
 
 void bind_layers(pybind11::module& m) {
@@ -261,4 +352,6 @@ void bind_layers(pybind11::module& m) {
     m.def("gated_recurrence_step", &gated_recurrence_step, "gated recurrence of one token; the state is updated in place", arg("x"), arg("gate"), arg("state"), arg("form"));
     m.def("layer_norm", &layer_norm, "layer normalisation of rows: (y, the sum that was normalised or None)", arg("x"), arg("weight").none(true), arg("bias").none(true),
           arg("residual").none(true), arg("eps"));
+    m.def("distillation_loss", &distillation_loss, "distillation from a teacher's top logits, a loss a row", arg("logits"), arg("teacher"), arg("index"), arg("labels").none(true),
+          arg("temperature"), arg("label_weight"));
 }

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 
 from . import inject
-from .sequence import clip_grad_norm_
+from .sequence import clip_grad_norm_, distillation_loss
 
 _REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -114,12 +114,15 @@ def make_optimizer(model, lr=0.004, weight_decay=0.05):
     return torch.optim.AdamW(param_groups(model, weight_decay), lr=lr, betas=(0.9, 0.999), eps=1e-8)
 
 
-def train_step(model, optimizer, images, labels, micro_batch, autocast_dtype=torch.bfloat16, max_grad_norm=None):
+def train_step(model, optimizer, images, labels, micro_batch, autocast_dtype=torch.bfloat16, max_grad_norm=None, teacher=None, temperature=1.0,
+               label_weight=0.5):
     """One optimiser step on this rank's share of the global batch: forward + backward over
     micro-batches (gradients accumulate; under DistributedDataParallel only the last micro-batch
     triggers the weight-gradient all-reduce), then AdamW.  Cross-entropy on hard labels, mean over the
     rank's whole share.  With ``max_grad_norm`` the gradients are clipped by their global norm first
-    (``clip_grad_norm_``; CUDA gradients).  Returns the loss (a detached scalar tensor)."""
+    (``clip_grad_norm_``; CUDA gradients).  With ``teacher``, a pair of a teacher's top logits for these images and
+    their classes (both (images, K)), the loss is ``distillation_loss`` of them at ``temperature``, with the labels' cross-entropy at
+    ``label_weight`` (CUDA).  Returns the loss (a detached scalar tensor)."""
     n = images.shape[0]
     chunks = [(s, min(s + micro_batch, n)) for s in range(0, n, micro_batch)]
     optimizer.zero_grad(set_to_none=True)
@@ -132,7 +135,11 @@ def train_step(model, optimizer, images, labels, micro_batch, autocast_dtype=tor
         with sync:
             with torch.autocast("cuda", dtype=autocast_dtype, enabled=use_autocast):
                 logits = model(images[s:e])
-            loss = torch.nn.functional.cross_entropy(logits.float(), labels[s:e], reduction="sum") / n
+            if teacher is None:
+                loss = torch.nn.functional.cross_entropy(logits.float(), labels[s:e], reduction="sum") / n
+            else:
+                top, index = teacher
+                loss = distillation_loss(logits, top[s:e], index[s:e], labels[s:e] if label_weight > 0 else None, temperature=temperature, label_weight=label_weight).sum() / n
             loss.backward()
         total = loss.detach() if total is None else total + loss.detach()
     if max_grad_norm is not None:

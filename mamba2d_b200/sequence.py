@@ -8,6 +8,7 @@ package works on, and clipping of gradients by their global norm.
   gated_recurrence_step(x, gate, state, ...)        one token of every sequence, the state updated in place
   group_norm(x, groups, weight, bias, ...)          x (N, ..., C)
   layer_norm(x, weight, bias, residual=...)         x (..., C), with the residual sum before it
+  distillation_loss(logits, teacher_logits, ...)    a loss a row: what ``refmodel.train_step(teacher=...)`` calls
   clip_norm_(tensors, max_norm)                     global norm of many tensors, all scaled in place
   clip_grad_norm_(parameters, max_norm)             of parameters' gradients: what ``refmodel.train_step`` calls
 
@@ -20,7 +21,7 @@ import torch
 from . import _lib
 
 __all__ = ["linear_attention", "linear_attention_step", "gated_recurrence", "gated_recurrence_step", "group_norm", "layer_norm",
-           "clip_norm_", "clip_grad_norm_"]
+           "distillation_loss", "clip_norm_", "clip_grad_norm_"]
 
 _ACTS = {None: 0, "silu": 1, "gelu": 2}
 _GATES = {"decay": 0, "forget": 1}
@@ -144,6 +145,27 @@ def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
     """
     y, total = _lib.entry().layer_norm(x, weight, bias, residual, eps)
     return y if residual is None else (y, total)
+
+
+def distillation_loss(logits, teacher_logits, teacher_index, labels=None, *, temperature=1.0, label_weight=0.0):
+    """``(1 - label_weight) temperature^2 KL(p || q) + label_weight CE(logits, labels)`` of every row, float32.
+
+    q is the softmax of ``logits / temperature`` over all classes, p that of ``teacher_logits / temperature`` over the entries that
+    the teacher gives (its top logits); KL is summed over those entries.
+
+    Args:
+        logits: (..., V), float32 or bfloat16.
+        teacher_logits, teacher_index: (..., K), float32 or bfloat16 and integers; K up to 512.  An entry whose index is not in
+            0 ... V - 1 is absent (-1 pads a shorter list); a row without entries, or with -inf in all of them, has no KL.  An index
+            that comes twice is two entries.
+        labels: (...) integers where ``label_weight`` is above 0 (and only there); a row whose label is not in 0 ... V - 1 has no CE.
+    Returns:
+        losses (...), to be summed or averaged by the caller.
+    Differentiable in logits, once (``create_graph`` raises); teacher logits that require a gradient raise.  Logits of -inf, or
+    of the type's lowest value, mask classes.  Rows may lie apart; those of an odd number of bfloat16 values run as fast as others
+    if the rows of logits are dense.
+    """
+    return _lib.entry().distillation_loss(logits, teacher_logits, teacher_index, labels, float(temperature), float(label_weight))
 
 
 def clip_norm_(tensors, max_norm, error_if_nonfinite=False):

@@ -1,4 +1,4 @@
-"""Definitions in 64 bits of the gated recurrence and the layer norm, and bounds on what their results may be off by.
+"""Definitions in 64 bits of the gated recurrence, the layer norm and the distillation loss, and bounds on what their results may be off by.
 
 The recurrence's weights are all positive, so what rounding does to h_t is bounded by the same operator on magnitudes, H_t = a_t H_{t-1} + |u_t|:
   - a run's tokens (up to 16) are weighted by products of up to 16 gates, each off by 2^-22 of itself (the approximate exponential's and
@@ -113,3 +113,45 @@ def norm_bounds(x, weight, bias, dy=None, eps=1e-5):
     rows = 64 + N / 32                   # (a thread's rows one after another, then CTAs in turn)
     over = lambda t: t.reshape(-1, C).sum(0)  # noqa: E731
     return y, dx, over(dy.abs() * dh) + rows * e * over((dy * h).abs()), rows * e * over(dy.abs())
+
+
+def distillation(z, t, index, labels=None, temperature=1.0, label_weight=0.0):
+    """A loss a row, z (N, V) in 64 bits."""
+    tau, w, V = temperature, label_weight, z.shape[-1]
+    there = (index >= 0) & (index < V)
+    at = torch.where(there, index, 0).long()
+    t = torch.where(there, t.double(), -torch.inf)
+    teaches = (t > -torch.inf).any(-1) | torch.isnan(t).any(-1)
+    log_p = torch.log_softmax(torch.where(teaches[:, None], t, 0.0) / tau, -1)
+    log_q = torch.log_softmax(z / tau, -1).gather(-1, at)
+    p = torch.where(there, log_p.exp(), 0.0)
+    kl = torch.where(p != 0, p * (torch.where(p != 0, log_p, 0.0) - torch.where(p != 0, log_q, 0.0)), 0.0).sum(-1)
+    loss = (1 - w) * tau ** 2 * torch.where(teaches, kl, 0.0) if w < 1 else torch.zeros_like(kl)
+    if w > 0:
+        counted = (labels >= 0) & (labels < V)
+        label = torch.where(counted, labels, 0).long()
+        loss = loss - w * torch.where(counted, torch.log_softmax(z, -1).gather(-1, label[:, None])[:, 0], 0.0)
+    return loss
+
+
+def distillation_bounds(z, t, index, labels, temperature, label_weight, up):
+    """What (loss, dz) may be off by.  An exponential's argument (z - max) c is rounded twice and c = log2(e) / tau once, so it is off by
+    2^-22 of itself at most, the approximate exponential by 2^-22, and a row's sum by k more steps of 2^-24, k the values that a thread adds and
+    a tree above it."""
+    tau, w, V = temperature, label_weight, z.shape[-1]
+    k = 32 + max(V / 256, min(V, 4096) / 32)
+    base = 2.0 ** -21 + k * 2.0 ** -24
+    far = torch.where(torch.isfinite(z), z.max(-1, keepdim=True).values - z, 0.0).clamp(max=2e3)
+    there = (index >= 0) & (index < V)
+    at = torch.where(there, index, 0).long()
+    p = torch.nan_to_num(torch.softmax(torch.where(there, t.double(), -1e30) / tau, -1)) * there         # (of a list of -inf: nothing)
+    spread = 2.0 ** -22 * (far.gather(-1, at) * there).max(-1).values / tau + 2.0 ** -22 * torch.where(there & torch.isfinite(t), t.double().abs(), 0.0).max(-1).values / tau
+    loss = (1 - w) * tau ** 2 * (base + spread) + w * (base + 2.0 ** -22 * (0 if labels is None else far.gather(-1, labels.clamp(0, V - 1).long()[:, None])[:, 0]))
+    q, s = torch.softmax(z / tau, -1), torch.softmax(z, -1)
+    dz = (1 - w) * tau * q * (2 * base + 2.0 ** -21 * far / tau) + w * s * (2 * base + 2.0 ** -21 * far)
+    take = torch.zeros_like(z).scatter_add_(-1, at, p * (8 * 2.0 ** -22 + 2.0 ** -21 * torch.where(there & torch.isfinite(t), (t.double().max() - t.double()).abs().clamp(max=2e3), 0.0) / tau))
+    dz = dz + (1 - w) * tau * take + 2.0 ** -22 * (w + tau * (1 - w)) * (q + s) + 2.0 ** -23 * (torch.zeros_like(z).scatter_add_(-1, at, (1 - w) * tau * p))
+    if labels is not None:
+        inside = (labels >= 0) & (labels < V)
+        dz.scatter_add_(-1, labels.clamp(0, V - 1).long()[:, None], (2.0 ** -22 * w * inside)[:, None].double())
+    return loss, up.abs()[:, None] * dz

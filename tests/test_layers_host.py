@@ -1,11 +1,11 @@
-"""The gated recurrence and layer normalisation without a device: refusals of the Python entry points and of the C ABI."""
+"""The gated recurrence, layer normalisation and the distillation loss without a device: refusals of the Python entry points and of the C ABI."""
 import ctypes
 
 import pytest
 import torch
 
 import mamba2d_b200
-from mamba2d_b200 import _lib, gated_recurrence, gated_recurrence_step, layer_norm
+from mamba2d_b200 import _lib, distillation_loss, gated_recurrence, gated_recurrence_step, layer_norm
 
 OK, NULL, DTYPE, SHAPE, WORKSPACE, ABI, LARGE, FLAGS, PITCH = 0, -1, -2, -3, -6, -8, -9, -10, -5
 
@@ -29,12 +29,20 @@ class LnDesc(ctypes.Structure):
                 *[(n, ctypes.c_void_p) for n in ("d_x", "d_weight", "d_bias", "workspace")], ("workspace_bytes", ctypes.c_uint64)]
 
 
+class DistillDesc(ctypes.Structure):
+    """Mirror of ``m2d_distill_desc``."""
+    _fields_ = [("struct_bytes", ctypes.c_uint32), *[(n, ctypes.c_int32) for n in ("dtype", "teacher_dtype", "V", "K", "index_64", "labels_64")],
+                ("temperature", ctypes.c_float), ("label_weight", ctypes.c_float), ("N", ctypes.c_int64), ("logits", ctypes.c_void_p), ("logits_row", ctypes.c_int64),
+                ("teacher", ctypes.c_void_p), ("teacher_row", ctypes.c_int64), ("index", ctypes.c_void_p), ("index_row", ctypes.c_int64),
+                *[(n, ctypes.c_void_p) for n in ("labels", "loss", "stats", "d_loss")], ("d_loss_row", ctypes.c_int64), ("d_logits", ctypes.c_void_p)]
+
+
 @pytest.fixture(scope="module")
 def L():
     from mamba2d_b200 import build
     build.build()
     raw = ctypes.CDLL(_lib.LIB_PATH)
-    raw.m2d_recur_marks.restype = raw.m2d_ln_bwd_workspace.restype = ctypes.c_uint64
+    raw.m2d_recur_marks.restype = raw.m2d_ln_bwd_workspace.restype = raw.m2d_distill_stats.restype = ctypes.c_uint64
     return raw
 
 
@@ -105,6 +113,34 @@ def test_refusals_of_layer_norm():
             layer_norm(x, eps=eps)
 
 
+def test_distillation_descriptors(L):
+    def desc(**kw):
+        d = DistillDesc(struct_bytes=ctypes.sizeof(DistillDesc), V=100, K=8, N=10, temperature=2.0, logits=256, teacher=256, index=256)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return ctypes.byref(d)
+    for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"teacher_dtype": -1}, DTYPE), ({"N": 0}, SHAPE), ({"V": 0}, SHAPE), ({"K": 0}, SHAPE), ({"K": 513}, LARGE),
+                   ({"N": 1 << 26}, LARGE), ({"V": (1 << 31) - 1}, LARGE), ({"temperature": 0.0}, FLAGS), ({"temperature": float("nan")}, FLAGS), ({"temperature": float("inf")}, FLAGS),
+                   ({"label_weight": 1.5}, FLAGS), ({"label_weight": 0.5}, NULL), ({"logits": None}, NULL), ({"index": None}, NULL), ({"logits": 258}, PITCH)):
+        assert L.m2d_distill_fwd(desc(**kw), None) == rc and L.m2d_distill_bwd(desc(**kw), None) == rc, kw
+    assert L.m2d_distill_fwd(None, None) == NULL and L.m2d_distill_stats(desc()) > 0
+
+
+def test_refusals_of_the_distillation_loss():
+    z, t, i, n = torch.randn(4, 20), torch.randn(4, 3), torch.zeros(4, 3, dtype=torch.long), torch.zeros(4, dtype=torch.long)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        distillation_loss(z, t, i)
+    for args, kw in (((z.half(), t, i), {}), ((z, t.double(), i), {}), ((z, t, i.short()), {}), ((z, t[:3], i[:3]), {}), ((z, t, i[:, :2]), {}), ((z, t[:, :0], i[:, :0]), {}),
+                     ((z, t[0], i[0]), {}), ((z, torch.zeros(4, 600), torch.zeros(4, 600, dtype=torch.long)), {}), ((z, t, i, n[:3]), {"label_weight": 0.5}),
+                     ((z, t, i, n.float()), {"label_weight": 0.5}), ((z[:, :0], t, i), {})):
+        with pytest.raises(RuntimeError):
+            distillation_loss(*args, **kw)
+    for args, kw in (((z, t, i), {"temperature": 0.0}), ((z, t, i), {"temperature": float("nan")}), ((z, t, i), {"temperature": float("inf")}), ((z, t, i), {"temperature": 1e-60}),
+                     ((z, t, i, n), {"label_weight": 1.1}), ((z, t, i, n), {"label_weight": -0.1}), ((z, t, i, n), {}), ((z, t, i), {"label_weight": 0.5})):
+        with pytest.raises(ValueError):
+            distillation_loss(*args, **kw)
+
+
 def test_the_package_has_them():
-    for n in ("gated_recurrence", "gated_recurrence_step", "layer_norm"):
+    for n in ("distillation_loss", "gated_recurrence", "gated_recurrence_step", "layer_norm"):
         assert n in mamba2d_b200.__all__ and callable(getattr(mamba2d_b200, n))
