@@ -4,14 +4,18 @@
 //   backward:     D_t = dy_t + R_{t+1}, R_t = a_t D_t;   decay: dx = D, dgate = R_t h_{t-1};
 //                 forget: dx = (1 - f) D, dgate = (1 - f) R_t (h_{t-1} - x_t)
 //
-// A CTA owns the channels of 32 lanes and walks a sequence in tiles.  Inside a tile a warp takes kSteps tokens: it finds what they do
-// to any state, h -> A h + b, from registers; the warps' pairs (A, b) are joined in shared memory; then each warp goes over its tokens
-// again from the state before them, still from registers, and stores.  So memory is read once and written once, and the loads of the
-// next tile are under way meanwhile.
+// A cluster of CTAs owns the channels of LANES lanes and walks a sequence in strides, a tile of it for each CTA.  Inside a tile the lanes of a row
+// take L tokens: they find what those do to any state, h -> A h + b, from registers; the runs' pairs (A, b) are joined in shared memory, the tiles' in
+// that of every CTA of the cluster; then each goes over its tokens again from the state before them, still from registers, and stores.  So
+// memory is read once and written once, and the loads of the next tile are under way meanwhile.  What is wanted are loads in flight
+// (16 warps an SM with 64 bytes and more a thread): where sequences and channels are too few, rows are split into shorter pieces and
+// a tile into more runs, then the sequence over up to 8 CTAs.
 //
-// Precision: states and sums are fp32.  A channel may remember thousands of tokens: 1 - A of a warp's tokens is small then, and A
-// rounded to fp32 would be off by the same amount at every step, 2^-24 against a 1 - A of 2^-12 at a memory of 4096 tokens.  So a join has
-// E = A - 1 beside A, computed without cancellation (expm1 of the summed gates, or a sum of 1 - f), and adds E h to h.
+// Precision: states and sums are fp32.  A channel may remember thousands of tokens: 1 - A of a run is small then, and A
+// rounded to fp32 would be off by the same amount at every step, 2^-24 against a 1 - A of 2^-12 at a memory of 4096 tokens.  So A is held in two
+// parts, from E = A - 1 computed without cancellation (expm1 of the summed gates, or a sum of 1 - f).
+#include <cooperative_groups.h>
+
 #include "follow.cuh"
 #include "plan.cuh"
 #include "m2d_seq.h"
@@ -19,7 +23,8 @@
 namespace m2d {
 
 constexpr int kMark = 64;            // tokens between the states that the forward pass leaves for the backward pass
-constexpr int kRecurWarps = 8;       // warps of a CTA, at most
+constexpr int kRecurWarps = 16;      // warps of a CTA, at most
+constexpr int kRecurCluster = 8;     // CTAs of a cluster, at most
 
 struct RecurArgs {
     const void *x, *gate, *dy;
@@ -28,296 +33,467 @@ struct RecurArgs {
     const float *state, *d_state_out;
     float *state_out, *d_state, *marks;
     void *y, *dx, *dgate;
-    int B, T, C, groups;
+    int B, T, C, groups, ctas;         // channel groups, CTAs of a cluster
 };
+
+// One channel or two: packed arithmetic for two.  Single ones are rounded where those are: the same bits, however rows are aligned.
+template <int VEC> struct Num;
+template <> struct Num<1> {
+    float v;
+    __device__ __forceinline__ static Num all(float f) { return {f}; }
+    __device__ __forceinline__ float get(int) const { return v; }
+    __device__ __forceinline__ void set(int, float f) { v = f; }
+};
+template <> struct Num<2> {
+    unsigned long long v;
+    __device__ __forceinline__ static Num make(float a, float b) {
+        Num r;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+        return r;
+    }
+    __device__ __forceinline__ static Num all(float f) { return make(f, f); }
+    __device__ __forceinline__ float get(int i) const {
+        float a, b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+        return i ? b : a;
+    }
+    __device__ __forceinline__ void set(int i, float f) { *this = i ? make(get(0), f) : make(f, get(1)); }
+};
+__device__ __forceinline__ Num<1> fma_(Num<1> a, Num<1> b, Num<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Num<1> mul_(Num<1> a, Num<1> b) { return {__fmul_rn(a.v, b.v)}; }
+__device__ __forceinline__ Num<1> add_(Num<1> a, Num<1> b) { return {__fadd_rn(a.v, b.v)}; }
+__device__ __forceinline__ Num<2> fma_(Num<2> a, Num<2> b, Num<2> c) {
+    Num<2> r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Num<2> mul_(Num<2> a, Num<2> b) {
+    Num<2> r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Num<2> add_(Num<2> a, Num<2> b) {
+    Num<2> r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+template <int VEC> __device__ __forceinline__ Num<VEC> neg_(Num<VEC> a) { return mul_(a, Num<VEC>::all(-1.f)); }
 
 // VEC neighbouring values of a row as they are in memory, and as numbers.
 template <typename T, int VEC> struct Piece;
 template <> struct Piece<float, 1> {
     using Raw = float;
-    static __device__ __forceinline__ void get(Raw r, float* v) { v[0] = r; }
-    static __device__ __forceinline__ Raw put(const float* v) { return v[0]; }
+    static __device__ __forceinline__ Raw fill(float f) { return f; }
+    static __device__ __forceinline__ Num<1> get(Raw r) { return {r}; }
+    static __device__ __forceinline__ Raw put(Num<1> n) { return n.v; }
+};
+template <> struct Piece<float, 2> {
+    using Raw = float2;
+    static __device__ __forceinline__ Raw fill(float f) { return make_float2(f, f); }
+    static __device__ __forceinline__ Num<2> get(Raw r) { return Num<2>::make(r.x, r.y); }
+    static __device__ __forceinline__ Raw put(Num<2> n) { return make_float2(n.get(0), n.get(1)); }
 };
 template <> struct Piece<__nv_bfloat16, 1> {
     using Raw = unsigned short;
-    static __device__ __forceinline__ void get(Raw r, float* v) { v[0] = bf16_bits_to_float(r); }
-    static __device__ __forceinline__ Raw put(const float* v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v[0])); }
+    static __device__ __forceinline__ Raw fill(float f) { return (unsigned short)(__float_as_uint(f) >> 16); }
+    static __device__ __forceinline__ Num<1> get(Raw r) { return {bf16_bits_to_float(r)}; }
+    static __device__ __forceinline__ Raw put(Num<1> n) { return __bfloat16_as_ushort(__float2bfloat16_rn(n.v)); }
 };
 template <> struct Piece<__nv_bfloat16, 2> {
     using Raw = unsigned;
-    static __device__ __forceinline__ void get(Raw r, float* v) { v[0] = __uint_as_float(r << 16); v[1] = __uint_as_float(r & 0xffff0000u); }
-    static __device__ __forceinline__ Raw put(const float* v) { return pack_bf16x2(v[0], v[1]); }
+    static __device__ __forceinline__ Raw fill(float f) { return __float_as_uint(f) | __float_as_uint(f) >> 16; }
+    static __device__ __forceinline__ Num<2> get(Raw r) { return Num<2>::make(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)); }
+    static __device__ __forceinline__ Raw put(Num<2> n) { return pack_bf16x2(n.get(0), n.get(1)); }
 };
+// A gate that leaves the state as it is, where x is 0.  (Its lower 16 bits are zero.)
+template <int FORM> __device__ __forceinline__ float kept() { return FORM == M2D_GATE_DECAY ? 0.f : __int_as_float(0x7f800000); }
 
 __device__ __forceinline__ float rcp_approx(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// a = exp(gate), or f = sigmoid(gate) and 1 - f, each to its own precision: from exp(-|gate|), which is at most 1.
-template <int FORM>
-__device__ __forceinline__ void open_gate(float g, float& a, float& rest) {
+__device__ __forceinline__ float most(float a, float b) {          // a NaN stays one
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// a = exp(gate), or f = sigmoid(gate) and 1 - f, each to its own precision: e = exp(-gate), f = 1 / (1 + e), 1 - f = e f.  Gates below -87 count
+// as -87, whose f is 1.6e-38, so that e stays finite.
+template <int FORM, int VEC>
+__device__ __forceinline__ void open_gate(Num<VEC> g, Num<VEC>& a, Num<VEC>& rest) {
     if constexpr (FORM == M2D_GATE_DECAY) {
-        a = ex2(g * kLog2e);
-        rest = 1.f;
+        const Num<VEC> s = mul_(g, Num<VEC>::all(kLog2e));
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) a.set(v, ex2(s.get(v)));
+        rest = Num<VEC>::all(1.f);
     } else {
-        const float t = ex2(fabsf(g) * -kLog2e), r = rcp_approx(1.f + t), s = t * r;
-        a = g >= 0.f ? r : s;
-        rest = g >= 0.f ? s : r;
+        Num<VEC> e;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) e.set(v, most(g.get(v), -87.f));
+        e = mul_(e, Num<VEC>::all(-kLog2e));
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) e.set(v, ex2(e.get(v)));
+        const Num<VEC> d = add_(e, Num<VEC>::all(1.f));
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) a.set(v, rcp_approx(d.get(v)));
+        rest = mul_(e, a);
     }
 }
-// What some tokens do to a state: h -> A h + b, with E = A - 1.
+// What some tokens do to a state: h -> (hi + lo) h + b.
+template <int VEC>
 struct Step {
-    float A, E;
-    __device__ __forceinline__ void then(const Step& n) {
-        A *= n.A;
-        E = fmaf(E, n.E, E + n.E);
-    }
-    __device__ __forceinline__ float apply(float h, float b) const {
-        const bool near = A >= 0.5f;
-        return fmaf(near ? E : A, h, b) + (near ? h : 0.f);
+    Num<VEC> hi, lo;
+    __device__ __forceinline__ Num<VEC> apply(Num<VEC> h, Num<VEC> b) const { return fma_(hi, h, fma_(lo, h, b)); }
+    __device__ __forceinline__ void times(const Step& n) {          // the product of both, in two parts
+        const Num<VEC> p = mul_(hi, n.hi), rest = fma_(hi, n.hi, neg_(p));
+        lo = fma_(hi, n.lo, fma_(lo, n.hi, rest));
+        hi = p;
     }
 };
 // The same for a run of tokens, collected token by token: the sum of the gates, or the product of f and the sum that is 1 - A.
-template <int FORM>
+template <int FORM, int VEC>
 struct Collect {
-    float s = 0.f, p = 1.f;
-    __device__ __forceinline__ void add(float g, float a, float rest) {
+    Num<VEC> s = Num<VEC>::all(0.f), p = Num<VEC>::all(1.f);
+    __device__ __forceinline__ void add(Num<VEC> g, Num<VEC> a, Num<VEC> rest) {
         if constexpr (FORM == M2D_GATE_DECAY) {
-            s += g;
+            s = add_(s, g);
         } else {
-            p *= a;
-            s = fmaf(-s, rest, s + rest);
+            p = mul_(p, a);
+            s = fma_(neg_(s), rest, add_(s, rest));
         }
     }
-    __device__ __forceinline__ Step done() const {
-        if constexpr (FORM == M2D_GATE_DECAY) return {ex2(s * kLog2e), expm1f(s)};
-        else return {p, -s};
+    __device__ __forceinline__ Step<VEC> done() const {
+        Step<VEC> r;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float t = s.get(v), A = FORM == M2D_GATE_DECAY ? ex2(t * kLog2e) : p.get(v), E = FORM == M2D_GATE_DECAY ? expm1f(t) : -t;
+            const bool near = A >= 0.5f && A <= 2.f;
+            const float hi = near ? 1.f + E : A;
+            r.hi.set(v, hi);
+            r.lo.set(v, near ? E - (hi - 1.f) : 0.f);
+        }
+        return r;
+    }
+};
+// VEC neighbouring floats of shared memory
+template <int VEC> __device__ __forceinline__ Num<VEC> take(const float* p) {
+    if constexpr (VEC == 1) return {*p};
+    else return Num<2>{*reinterpret_cast<const unsigned long long*>(p)};
+}
+template <int VEC> __device__ __forceinline__ void give(float* p, Num<VEC> n) {
+    if constexpr (VEC == 1) *p = n.v;
+    else *reinterpret_cast<unsigned long long*>(p) = n.v;
+}
+template <int VEC> __device__ __forceinline__ Num<VEC> load_state(const float* p, bool on) {
+    Num<VEC> n = Num<VEC>::all(0.f);
+    if (on)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) n.set(v, p[v]);
+    return n;
+}
+template <int VEC> __device__ __forceinline__ void store_state(float* p, Num<VEC> n) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) p[v] = n.get(v);
+}
+
+// Where a thread stands: its channels, its run of a tile, its CTA of the cluster.
+template <int VEC, int LANES>
+struct Place {
+    static constexpr int width = LANES * VEC;      // channels of a CTA
+    int at, runs, run, b, c, rank, ctas, len;      // at: first of the thread's channels among the CTA's
+    bool mine;
+    __device__ __forceinline__ Place(const RecurArgs& p) {
+        const int lane = threadIdx.x & 31, per = 32 / LANES;
+        at = lane % LANES * VEC;
+        runs = (blockDim.x >> 5) * per;
+        run = (threadIdx.x >> 5) * per + lane / LANES;
+        ctas = p.ctas;
+        rank = blockIdx.x % ctas;
+        const int chain = blockIdx.x / ctas;
+        b = chain / p.groups;
+        c = chain % p.groups * width + at;
+        mine = c < p.C;
+        len = p.lengths ? max(0, min(p.T, p.lengths[b])) : p.T;
     }
 };
 
-template <typename T, int VEC, int FORM, int L>
+// Shared memory: [2][runs][PARTS][width] of the CTA's runs, [2][ctas][3][width] of the cluster's tiles.  Two of each: one barrier lies between
+// what is read of a tile and what is written of the next but one.
+template <int PARTS>
+constexpr size_t recur_smem(int runs, int ctas, int width) { return sizeof(float) * 2 * width * ((size_t)runs * PARTS + (ctas > 1 ? (size_t)ctas * 3 : 0)); }
+
+template <typename T, int VEC, int FORM, int L, int LANES>
 __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const RecurArgs p) {
+    namespace cg = cooperative_groups;
     using P = Piece<T, VEC>;
     using Raw = typename P::Raw;
-    __shared__ float part[2][kRecurWarps][3][32 * VEC];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, tile = warps * L;
-    const int b = blockIdx.x / p.groups, c = (blockIdx.x % p.groups) * 32 * VEC + lane * VEC;
-    const bool mine = c < p.C;
-    const int len = p.lengths ? max(0, min(p.T, p.lengths[b])) : p.T;
-    const T* const x = static_cast<const T*>(p.x) + b * p.xb + c;
-    const T* const g = static_cast<const T*>(p.gate) + b * p.gb + c;
-    T* const y = static_cast<T*>(p.y) + (long long)b * p.T * p.C + c;
+    using N = Num<VEC>;
+    constexpr int width = LANES * VEC;
+    extern __shared__ __align__(16) float smem[];
+    const Place<VEC, LANES> w(p);
+    cg::cluster_group cluster = cg::this_cluster();
+    if (w.ctas > 1) cluster.barrier_arrive();             // (all have begun before one writes to another)
+    const int tile = w.runs * L, stride = w.ctas * tile;
+    const T* const x = static_cast<const T*>(p.x) + w.b * p.xb + w.c;
+    const T* const g = static_cast<const T*>(p.gate) + w.b * p.gb + w.c;
+    T* const y = static_cast<T*>(p.y) + (long long)w.b * p.T * p.C + w.c;
     Raw rx[L], rg[L];
     auto load = [&](int t0) {
         const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt;
+        const int n = w.mine ? w.len - t0 : 0;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const bool on = mine && t0 + i < len;
-            rx[i] = on ? __ldcs(reinterpret_cast<const Raw*>(px + i * p.xt)) : Raw(0);
-            rg[i] = on ? __ldcs(reinterpret_cast<const Raw*>(pg + i * p.gt)) : Raw(0);
+            rx[i] = P::fill(0.f);
+            rg[i] = P::fill(kept<FORM>());
+            if (i < n) {
+                rx[i] = __ldcs(reinterpret_cast<const Raw*>(px));
+                rg[i] = __ldcs(reinterpret_cast<const Raw*>(pg));
+            }
+            px += p.xt;
+            pg += p.gt;
         }
     };
-    float carry[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = p.state && mine ? p.state[(long long)b * p.C + c + v] : 0.f;
-    load(warp * L);
-    for (int t1 = 0, buf = 0; t1 < len; t1 += tile, buf ^= 1) {
-        const int t0 = t1 + warp * L;
-        float a[L][VEC], u[L][VEC];
-        Collect<FORM> all[VEC];
-        float h[VEC] = {};
+    N carry = load_state<VEC>(p.state + (long long)w.b * p.C + w.c, p.state && w.mine);
+    int t0 = w.rank * tile + w.run * L;
+    load(t0);
+    if (w.ctas > 1) cluster.barrier_wait();
+    for (int s0 = 0, buf = 0; s0 < w.len; s0 += stride, t0 += stride, buf ^= 1) {
+        float* const part = smem + (size_t)buf * w.runs * 3 * width + w.at;
+        N a[L], u[L], h = N::all(0.f);
+        Collect<FORM, VEC> all;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            float xv[VEC], gv[VEC];
-            P::get(rx[i], xv);
-            P::get(rg[i], gv);
-            const bool on = t0 + i < len;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float rest;
-                open_gate<FORM>(gv[v], a[i][v], rest);
-                if (!on) { a[i][v] = 1.f; rest = 0.f; }            // (its gate and x are 0: the state stays as it is)
-                u[i][v] = FORM == M2D_GATE_DECAY ? xv[v] : rest * xv[v];
-                all[v].add(gv[v], a[i][v], rest);
-                h[v] = fmaf(a[i][v], h[v], u[i][v]);
+            const N gate = P::get(rg[i]);
+            N rest;
+            open_gate<FORM, VEC>(gate, a[i], rest);
+            u[i] = FORM == M2D_GATE_DECAY ? P::get(rx[i]) : mul_(rest, P::get(rx[i]));
+            all.add(gate, a[i], rest);
+            h = fma_(a[i], h, u[i]);
+        }
+        if (s0 + stride < w.len) load(t0 + stride);
+        Step<VEC> step = all.done();
+        give(part + (w.run * 3 + 0) * width, step.hi);
+        give(part + (w.run * 3 + 1) * width, step.lo);
+        give(part + (w.run * 3 + 2) * width, h);
+        __syncthreads();
+        auto entry = [&](const float* q, int k, Step<VEC>& s, N& b) {
+            s.hi = take<VEC>(q + (k * 3 + 0) * width);
+            s.lo = take<VEC>(q + (k * 3 + 1) * width);
+            b = take<VEC>(q + (k * 3 + 2) * width);
+        };
+        Step<VEC> s;
+        N b;
+        if (w.ctas > 1) {
+            // the tile's own, to every CTA of the cluster
+            Step<VEC> whole{N::all(1.f), N::all(0.f)};
+            N sum = N::all(0.f);
+#pragma unroll 4
+            for (int k = 0; k < w.runs; ++k) {
+                entry(part, k, s, b);
+                sum = s.apply(sum, b);
+                whole.times(s);
+            }
+            float* const tiles = smem + (size_t)2 * w.runs * 3 * width + (size_t)buf * w.ctas * 3 * width + w.at;
+            for (int k = threadIdx.x / 32; k < w.ctas; k += blockDim.x / 32) {
+                float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
+                if ((threadIdx.x & 31) < LANES) {
+                    give(to, whole.hi);
+                    give(to + width, whole.lo);
+                    give(to + 2 * width, sum);
+                }
+            }
+            cluster.sync();
+            h = carry;
+            for (int k = 0; k < w.ctas; ++k) {
+                if (k == w.rank) h = carry;
+                entry(tiles, k, s, b);
+                carry = s.apply(carry, b);
+            }
+#pragma unroll 4
+            for (int k = 0; k < w.run; ++k) {
+                entry(part, k, s, b);
+                h = s.apply(h, b);
+            }
+        } else {
+#pragma unroll 4
+            for (int k = 0; k < w.run; ++k) {
+                entry(part, k, s, b);
+                carry = s.apply(carry, b);
+            }
+            h = carry;
+#pragma unroll 4
+            for (int k = w.run; k < w.runs; ++k) {
+                entry(part, k, s, b);
+                carry = s.apply(carry, b);
             }
         }
-        if (t1 + tile < len) load(t0 + tile);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Step s = all[v].done();
-            part[buf][warp][0][lane * VEC + v] = s.A;
-            part[buf][warp][1][lane * VEC + v] = s.E;
-            part[buf][warp][2][lane * VEC + v] = h[v];
-        }
-        __syncthreads();                      // (one barrier a tile: what is read below is written over two tiles on)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = carry[v];
-        for (int w = 0; w < warps; ++w) {
-            if (w == warp) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) h[v] = carry[v];
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const Step s{part[buf][w][0][lane * VEC + v], part[buf][w][1][lane * VEC + v]};
-                carry[v] = s.apply(carry[v], part[buf][w][2][lane * VEC + v]);
-            }
-        }
-        if (p.marks && mine && t0 < len && t0 % kMark == 0) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) p.marks[((long long)b * ((p.T + kMark - 1) / kMark) + t0 / kMark) * p.C + c + v] = h[v];
-        }
+        const int n = w.mine ? w.len - t0 : 0;
+        if (p.marks && n > 0 && t0 % kMark == 0) store_state<VEC>(p.marks + ((long long)w.b * ((p.T + kMark - 1) / kMark) + t0 / kMark) * p.C + w.c, h);
         T* py = y + (long long)t0 * p.C;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = fmaf(a[i][v], h[v], u[i][v]);
-            if (mine && t0 + i < len) *reinterpret_cast<Raw*>(py + (long long)i * p.C) = P::put(h);
+            h = fma_(a[i], h, u[i]);
+            if (i < n) *reinterpret_cast<Raw*>(py) = P::put(h);
+            py += p.C;
         }
     }
-    if (!mine) return;
-    const float zero[VEC] = {};
-    for (long long t = len + warp; t < p.T; t += warps) *reinterpret_cast<Raw*>(y + t * p.C) = P::put(zero);
-    if (p.state_out && warp == 0) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) p.state_out[(long long)b * p.C + c + v] = carry[v];
-    }
+    if (!w.mine) return;
+    for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) *reinterpret_cast<Raw*>(y + t * p.C) = P::fill(0.f);
+    if (p.state_out && w.rank == 0 && w.run == 0) store_state<VEC>(p.state_out + (long long)w.b * p.C + w.c, carry);
 }
 
-// Tiles from the last to the first.  The states inside a tile come from the forward pass's mark before it.
-template <typename T, int VEC, int FORM, int L>
+// Tiles from the last to the first.  The states inside a tile come from the forward pass's mark before it: only what flows back is joined
+// between CTAs.
+template <typename T, int VEC, int FORM, int L, int LANES>
 __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const RecurArgs p) {
+    namespace cg = cooperative_groups;
     using P = Piece<T, VEC>;
     using Raw = typename P::Raw;
-    __shared__ float part[2][kRecurWarps][4][32 * VEC];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    constexpr int tile = kMark;
-    const int b = blockIdx.x / p.groups, c = (blockIdx.x % p.groups) * 32 * VEC + lane * VEC;
-    const bool mine = c < p.C;
-    const int len = p.lengths ? max(0, min(p.T, p.lengths[b])) : p.T;
-    const T* const x = static_cast<const T*>(p.x) + b * p.xb + c;
-    const T* const g = static_cast<const T*>(p.gate) + b * p.gb + c;
-    const T* const dy = static_cast<const T*>(p.dy) + b * p.db + c;
-    const long long out = (long long)b * p.T * p.C + c;
+    using N = Num<VEC>;
+    constexpr int width = LANES * VEC;
+    extern __shared__ __align__(16) float smem[];
+    const Place<VEC, LANES> w(p);
+    cg::cluster_group cluster = cg::this_cluster();
+    if (w.ctas > 1) cluster.barrier_arrive();
+    const int tile = w.runs * L, stride = w.ctas * tile;
+    const T* const x = static_cast<const T*>(p.x) + w.b * p.xb + w.c;
+    const T* const g = static_cast<const T*>(p.gate) + w.b * p.gb + w.c;
+    const T* const dy = static_cast<const T*>(p.dy) + w.b * p.db + w.c;
+    const long long out = (long long)w.b * p.T * p.C + w.c;
     T *const dx = static_cast<T*>(p.dx) + out, *const dgate = static_cast<T*>(p.dgate) + out;
-    const float* const marks = p.marks + (long long)b * ((p.T + kMark - 1) / kMark) * p.C + c;
+    const float* const marks = p.marks + (long long)w.b * ((p.T + kMark - 1) / kMark) * p.C + w.c;
     Raw rx[L], rg[L], rd[L];
-    float mark[VEC] = {};
+    N mark;
     auto load = [&](int t1) {
-        const int t0 = t1 + warp * L;
+        const int t0 = t1 + w.run * L, n = w.mine ? w.len - t0 : 0;
         const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt, *pd = dy + t0 * p.dt;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const bool on = mine && t0 + i < len;
-            rx[i] = on ? __ldcs(reinterpret_cast<const Raw*>(px + i * p.xt)) : Raw(0);
-            rg[i] = on ? __ldcs(reinterpret_cast<const Raw*>(pg + i * p.gt)) : Raw(0);
-            rd[i] = on ? __ldcs(reinterpret_cast<const Raw*>(pd + i * p.dt)) : Raw(0);
+            rx[i] = rd[i] = P::fill(0.f);
+            rg[i] = P::fill(kept<FORM>());
+            if (i < n) {
+                rx[i] = __ldcs(reinterpret_cast<const Raw*>(px));
+                rg[i] = __ldcs(reinterpret_cast<const Raw*>(pg));
+                rd[i] = __ldcs(reinterpret_cast<const Raw*>(pd));
+            }
+            px += p.xt;
+            pg += p.gt;
+            pd += p.dt;
         }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) mark[v] = mine ? marks[(long long)(t1 / kMark) * p.C + v] : 0.f;
+        mark = load_state<VEC>(marks + (long long)(t1 / kMark) * p.C, w.mine && t1 < w.len);
     };
-    float carry[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = p.d_state_out && mine ? p.d_state_out[(long long)b * p.C + c + v] : 0.f;
-    int t1 = (len - 1) / tile * tile;         // (of no tokens: none)
-    if (len > 0) load(t1);
-    for (int buf = 0; len > 0 && t1 >= 0; t1 -= tile, buf ^= 1) {
-        const int t0 = t1 + warp * L;
-        float a[L][VEC], rest[L][VEC], xv[L][VEC], dv[L][VEC], before[L][VEC];
-        Collect<FORM> all[VEC];
-        float h[VEC] = {}, R[VEC] = {};
+    N carry = load_state<VEC>(p.d_state_out + (long long)w.b * p.C + w.c, p.d_state_out && w.mine);
+    int s0 = w.len > 0 ? (w.len - 1) / stride * stride : -1;
+    if (s0 >= 0) load(s0 + w.rank * tile);
+    if (w.ctas > 1) cluster.barrier_wait();
+    for (int buf = 0; s0 >= 0; s0 -= stride, buf ^= 1) {
+        const int t0 = s0 + w.rank * tile + w.run * L;
+        float* const part = smem + (size_t)buf * w.runs * 4 * width + w.at;
+        N a[L], rest[L], xv[L], dv[L], before[L], h = N::all(0.f), R = N::all(0.f);
+        Collect<FORM, VEC> all;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            float gv[VEC];
-            P::get(rx[i], xv[i]);
-            P::get(rg[i], gv);
-            P::get(rd[i], dv[i]);
-            const bool on = t0 + i < len;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                open_gate<FORM>(gv[v], a[i][v], rest[i][v]);
-                if (!on) { a[i][v] = 1.f; rest[i][v] = 0.f; }
-                all[v].add(gv[v], a[i][v], rest[i][v]);
-                h[v] = fmaf(a[i][v], h[v], FORM == M2D_GATE_DECAY ? xv[i][v] : rest[i][v] * xv[i][v]);
-            }
+            const N gate = P::get(rg[i]);
+            xv[i] = P::get(rx[i]);
+            dv[i] = P::get(rd[i]);
+            open_gate<FORM, VEC>(gate, a[i], rest[i]);
+            all.add(gate, a[i], rest[i]);
+            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv[i] : mul_(rest[i], xv[i]));
         }
 #pragma unroll
-        for (int i = L - 1; i >= 0; --i)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) R[v] = a[i][v] * (dv[i][v] + R[v]);
-        float first[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) first[v] = mark[v];
-        if (t1 >= tile) load(t1 - tile);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Step s = all[v].done();
-            part[buf][warp][0][lane * VEC + v] = s.A;
-            part[buf][warp][1][lane * VEC + v] = s.E;
-            part[buf][warp][2][lane * VEC + v] = h[v];
-            part[buf][warp][3][lane * VEC + v] = R[v];
-        }
+        for (int i = L - 1; i >= 0; --i) R = mul_(a[i], add_(dv[i], R));
+        const N first = mark;
+        if (s0 >= stride) load(s0 - stride + w.rank * tile);
+        const Step<VEC> step = all.done();
+        give(part + (w.run * 4 + 0) * width, step.hi);
+        give(part + (w.run * 4 + 1) * width, step.lo);
+        give(part + (w.run * 4 + 2) * width, h);
+        give(part + (w.run * 4 + 3) * width, R);
         __syncthreads();
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = first[v];
-        for (int w = 0; w < warp; ++w)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const Step s{part[buf][w][0][lane * VEC + v], part[buf][w][1][lane * VEC + v]};
-                h[v] = s.apply(h[v], part[buf][w][2][lane * VEC + v]);
+        Step<VEC> s;
+        auto entry = [&](int k, int which) {
+            s.hi = take<VEC>(part + (k * 4 + 0) * width);
+            s.lo = take<VEC>(part + (k * 4 + 1) * width);
+            return take<VEC>(part + (k * 4 + which) * width);
+        };
+        if (w.ctas > 1) {
+            Step<VEC> whole{N::all(1.f), N::all(0.f)};
+            N sum = N::all(0.f);
+#pragma unroll 4
+            for (int k = w.runs - 1; k >= 0; --k) {
+                const N b = entry(k, 3);
+                sum = s.apply(sum, b);
+                whole.times(s);
             }
-        for (int w = warps - 1; w >= 0; --w) {
-            if (w == warp) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) R[v] = carry[v];
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const Step s{part[buf][w][0][lane * VEC + v], part[buf][w][1][lane * VEC + v]};
-                carry[v] = s.apply(carry[v], part[buf][w][3][lane * VEC + v]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < L; ++i)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                before[i][v] = h[v];
-                h[v] = fmaf(a[i][v], h[v], FORM == M2D_GATE_DECAY ? xv[i][v] : rest[i][v] * xv[i][v]);
-            }
-        const long long at = (long long)t0 * p.C;
-#pragma unroll
-        for (int i = L - 1; i >= 0; --i) {
-            float gx[VEC], gg[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float D = dv[i][v] + R[v];
-                R[v] = a[i][v] * D;
-                if constexpr (FORM == M2D_GATE_DECAY) {
-                    gx[v] = D;
-                    gg[v] = R[v] * before[i][v];
-                } else {
-                    gx[v] = rest[i][v] * D;
-                    gg[v] = rest[i][v] * R[v] * (before[i][v] - xv[i][v]);
+            float* const tiles = smem + (size_t)2 * w.runs * 4 * width + (size_t)buf * w.ctas * 3 * width + w.at;
+            for (int k = threadIdx.x / 32; k < w.ctas; k += blockDim.x / 32) {
+                float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
+                if ((threadIdx.x & 31) < LANES) {
+                    give(to, whole.hi);
+                    give(to + width, whole.lo);
+                    give(to + 2 * width, sum);
                 }
             }
-            if (mine && t0 + i < len) {
-                *reinterpret_cast<Raw*>(dx + at + (long long)i * p.C) = P::put(gx);
-                *reinterpret_cast<Raw*>(dgate + at + (long long)i * p.C) = P::put(gg);
+            cluster.sync();
+            R = carry;
+            for (int k = w.ctas - 1; k >= 0; --k) {
+                if (k == w.rank) R = carry;
+                s.hi = take<VEC>(tiles + (k * 3 + 0) * width);
+                s.lo = take<VEC>(tiles + (k * 3 + 1) * width);
+                carry = s.apply(carry, take<VEC>(tiles + (k * 3 + 2) * width));
+            }
+#pragma unroll 4
+            for (int k = w.runs - 1; k > w.run; --k) {
+                const N b = entry(k, 3);
+                R = s.apply(R, b);
+            }
+        } else {
+#pragma unroll 4
+            for (int k = w.runs - 1; k > w.run; --k) {
+                const N b = entry(k, 3);
+                carry = s.apply(carry, b);
+            }
+            R = carry;
+#pragma unroll 4
+            for (int k = w.run; k >= 0; --k) {
+                const N b = entry(k, 3);
+                carry = s.apply(carry, b);
             }
         }
-    }
-    if (!mine) return;
-    const float zero[VEC] = {};
-    for (long long t = len + warp; t < p.T; t += warps) {
-        *reinterpret_cast<Raw*>(dx + t * p.C) = P::put(zero);
-        *reinterpret_cast<Raw*>(dgate + t * p.C) = P::put(zero);
-    }
-    if (p.d_state && warp == 0) {
+        h = first;
+#pragma unroll 4
+        for (int k = 0; k < w.run; ++k) {
+            const N b = entry(k, 2);
+            h = s.apply(h, b);
+        }
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) p.d_state[(long long)b * p.C + c + v] = carry[v];
+        for (int i = 0; i < L; ++i) {
+            before[i] = h;
+            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv[i] : mul_(rest[i], xv[i]));
+        }
+        const int n = w.mine ? w.len - t0 : 0;
+        T *px = dx + (long long)(t0 + L - 1) * p.C, *pg = dgate + (long long)(t0 + L - 1) * p.C;
+#pragma unroll
+        for (int i = L - 1; i >= 0; --i) {
+            const N D = add_(dv[i], R);
+            R = mul_(a[i], D);
+            const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
+            const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv[i], N::all(-1.f), before[i]));
+            if (i < n) {
+                *reinterpret_cast<Raw*>(px) = P::put(gx);
+                *reinterpret_cast<Raw*>(pg) = P::put(gg);
+            }
+            px -= p.C;
+            pg -= p.C;
+        }
     }
+    if (!w.mine) return;
+    for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) {
+        *reinterpret_cast<Raw*>(dx + t * p.C) = P::fill(0.f);
+        *reinterpret_cast<Raw*>(dgate + t * p.C) = P::fill(0.f);
+    }
+    if (p.d_state && w.rank == 0 && w.run == 0) store_state<VEC>(p.d_state + (long long)w.b * p.C + w.c, carry);
 }
 
 // One token of every sequence.  state and state_out may be the same array.
@@ -328,17 +504,12 @@ __global__ void __launch_bounds__(128) recur_step_kernel(const RecurArgs p, long
     const int c = (blockIdx.x * 128 + threadIdx.x) * VEC;
     if (c >= p.C) return;
     for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
-        float xv[VEC], gv[VEC], h[VEC];
-        P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.x) + b * p.xb + c), xv);
-        P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.gate) + b * p.gb + c), gv);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float a, rest;
-            open_gate<FORM>(gv[v], a, rest);
-            h[v] = fmaf(a, p.state[b * sb + c + v], FORM == M2D_GATE_DECAY ? xv[v] : rest * xv[v]);
-        }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) p.state_out[b * sb + c + v] = h[v];
+        using N = Num<VEC>;
+        const N x = P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.x) + b * p.xb + c)), g = P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.gate) + b * p.gb + c));
+        N a, rest;
+        open_gate<FORM, VEC>(g, a, rest);
+        const N h = fma_(a, load_state<VEC>(p.state + b * sb + c, true), FORM == M2D_GATE_DECAY ? x : mul_(rest, x));
+        store_state<VEC>(p.state_out + b * sb + c, h);
         *reinterpret_cast<Raw*>(static_cast<T*>(p.y) + (long long)b * p.C + c) = P::put(h);
     }
 }
@@ -358,7 +529,7 @@ static int check_recur(const m2d_recur_desc* d, bool step) {
     }
     return M2D_OK;
 }
-static bool pairs_ok(const void* p, long long a, long long b) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 4 == 0 && a % 2 == 0 && b % 2 == 0); }
+static bool pairs_ok(const void* p, long long a, long long b, int es) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % (2 * es) == 0 && a % 2 == 0 && b % 2 == 0); }
 static RecurArgs recur_args(const m2d_recur_desc* d) {
     RecurArgs a{};
     a.x = d->x.data; a.xb = d->x.batch; a.xt = d->x.token;
@@ -370,17 +541,61 @@ static RecurArgs recur_args(const m2d_recur_desc* d) {
     a.B = d->B; a.T = d->T; a.C = d->C;
     return a;
 }
-// Calls fn(element, channels of a lane, form): two channels of bf16 where rows are whole 4-byte pieces.
+// Calls fn(element, channels of a lane, form): two channels where rows are whole pieces of two.
 template <typename F>
 static int for_recur(const m2d_recur_desc* d, bool pairs, F fn) {
+    using std::integral_constant;
     auto with_form = [&](auto elem, auto vec) {
-        return d->form == M2D_GATE_DECAY ? fn(elem, vec, std::integral_constant<int, M2D_GATE_DECAY>{}) : fn(elem, vec, std::integral_constant<int, M2D_GATE_FORGET>{});
+        return d->form == M2D_GATE_DECAY ? fn(elem, vec, integral_constant<int, M2D_GATE_DECAY>{}) : fn(elem, vec, integral_constant<int, M2D_GATE_FORGET>{});
     };
-    if (d->dtype == M2D_F32) return with_form(float{}, std::integral_constant<int, 1>{});
-    if (pairs) return with_form(__nv_bfloat16{}, std::integral_constant<int, 2>{});
-    return with_form(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+    if (d->dtype == M2D_F32) return pairs ? with_form(float{}, integral_constant<int, 2>{}) : with_form(float{}, integral_constant<int, 1>{});
+    return pairs ? with_form(__nv_bfloat16{}, integral_constant<int, 2>{}) : with_form(__nv_bfloat16{}, integral_constant<int, 1>{});
 }
-constexpr int kFwdSteps = 16, kBwdSteps = 8;
+// Lanes of a row, warps of a CTA and CTAs of a cluster: enough warps that an SM has 16, first by more runs in a tile, then
+// by rows cut into pieces of 16 and of 8 lanes (of two bf16: 64 and 32 bytes), then by the cluster.
+struct RecurPlan { int lanes, warps, ctas; };
+static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps) {
+    const long long want = 16ll * sm_count(), runs = (d->T + steps - 1) / steps;
+    RecurPlan pl{32, 1, 1};
+    auto warps = [&](int lanes) { return (long long)d->B * ((d->C + lanes * vec - 1) / (lanes * vec)); };
+    while (pl.lanes > 8 && warps(pl.lanes) * kRecurWarps * kRecurCluster * 4 < want * 3 && runs >= 64) pl.lanes /= 2;
+    const int per = 32 / pl.lanes;
+    const long long chains = warps(pl.lanes), need = std::max<long long>(4, (want + chains - 1) / chains), have = (runs + per - 1) / per;
+    pl.warps = (int)std::min<long long>(std::min<long long>(need, have), 8);
+    while (pl.ctas < kRecurCluster && pl.ctas * 2 * pl.warps <= std::min(need, have)) pl.ctas *= 2;
+    if (pl.ctas == kRecurCluster) pl.warps = (int)std::min<long long>(kRecurWarps, std::min(need, have) / pl.ctas);
+    return pl;
+}
+template <int PARTS, typename K>
+static int launch_recur(K kern, const RecurArgs& a, const RecurPlan& pl, int vec, cudaStream_t st) {
+    const size_t smem = recur_smem<PARTS>(pl.warps * (32 / pl.lanes), pl.ctas, pl.lanes * vec);
+    if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.B * a.groups * pl.ctas));
+    cfg.blockDim = dim3(pl.warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = pl.ctas; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) { cudaGetLastError(); return M2D_ERR_LAUNCH; }
+    return M2D_OK;
+}
+// Calls fn(lanes) with the plan's; rows of single values are not cut.
+template <int VEC, typename F>
+static int for_lanes(int lanes, F fn) {
+    using std::integral_constant;
+    if constexpr (VEC == 2) {
+        if (lanes == 8) return fn(integral_constant<int, 8>{});
+        if (lanes == 16) return fn(integral_constant<int, 16>{});
+    }
+    return fn(integral_constant<int, 32>{});
+}
+// Tokens of a run, by the registers that they take.
+template <typename T> constexpr int kFwdSteps = sizeof(T) == 4 ? 8 : 16;
+constexpr int kBwdSteps = 8;
 
 }  // namespace m2d
 
@@ -396,14 +611,19 @@ extern "C" int m2d_recur_fwd(const m2d_recur_desc* d, void* stream) {
     if (rc != M2D_OK) return rc;
     if (!d->y) return M2D_ERR_NULL;
     RecurArgs a = recur_args(d);
-    const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, a.xt) && pairs_ok(a.gate, a.gb, a.gt) && pairs_ok(a.y, 0, 0);
+    const int es = d->dtype == M2D_F32 ? 4 : 2;
+    const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, a.xt, es) && pairs_ok(a.gate, a.gb, a.gt, es) && pairs_ok(a.y, 0, 0, es);
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
-        constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value;
-        a.groups = (d->C + 32 * VEC - 1) / (32 * VEC);
-        const int warps = std::min(kRecurWarps, (d->T + kFwdSteps - 1) / kFwdSteps);
-        recur_fwd_kernel<T, VEC, FORM, kFwdSteps><<<d->B * a.groups, warps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
-        return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+        constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kFwdSteps<T>;
+        RecurPlan pl = plan_recur(d, VEC, L);
+        return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
+            constexpr int LANES = decltype(lanes)::value;
+            pl.lanes = LANES;
+            a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
+            a.ctas = pl.ctas;
+            return launch_recur<3>(recur_fwd_kernel<T, VEC, FORM, L, LANES>, a, pl, VEC, static_cast<cudaStream_t>(stream));
+        });
     });
 }
 
@@ -412,13 +632,20 @@ extern "C" int m2d_recur_bwd(const m2d_recur_desc* d, void* stream) {
     if (rc != M2D_OK) return rc;
     if (!d->d_y.data || !d->d_x || !d->d_gate || !d->marks) return M2D_ERR_NULL;
     RecurArgs a = recur_args(d);
-    const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, a.xt) && pairs_ok(a.gate, a.gb, a.gt) && pairs_ok(a.dy, a.db, a.dt) && pairs_ok(a.dx, 0, 0) && pairs_ok(a.dgate, 0, 0);
+    const int es = d->dtype == M2D_F32 ? 4 : 2;
+    const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, a.xt, es) && pairs_ok(a.gate, a.gb, a.gt, es) && pairs_ok(a.dy, a.db, a.dt, es) && pairs_ok(a.dx, 0, 0, es) && pairs_ok(a.dgate, 0, 0, es);
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
-        constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value;
-        a.groups = (d->C + 32 * VEC - 1) / (32 * VEC);
-        recur_bwd_kernel<T, VEC, FORM, kBwdSteps><<<d->B * a.groups, kMark / kBwdSteps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
-        return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+        constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kBwdSteps;
+        RecurPlan pl = plan_recur(d, VEC, L);
+        return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
+            constexpr int LANES = decltype(lanes)::value, runs = kMark / L * LANES / 32;       // (warps that hold the tokens between marks)
+            pl.lanes = LANES;
+            if (pl.ctas > 1 || pl.warps * (32 / LANES) * L < d->T) pl.warps = (pl.warps + runs - 1) / runs * runs;    // (one tile has the first mark)
+            a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
+            a.ctas = pl.ctas;
+            return launch_recur<4>(recur_bwd_kernel<T, VEC, FORM, L, LANES>, a, pl, VEC, static_cast<cudaStream_t>(stream));
+        });
     });
 }
 
@@ -427,7 +654,8 @@ extern "C" int m2d_recur_step(const m2d_recur_desc* d, int64_t state_batch, void
     if (rc != M2D_OK) return rc;
     if (!d->y || !d->state || !d->state_out) return M2D_ERR_NULL;
     const RecurArgs a = recur_args(d);
-    const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, 0) && pairs_ok(a.gate, a.gb, 0) && pairs_ok(a.y, 0, 0);
+    const int es = d->dtype == M2D_F32 ? 4 : 2;
+    const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, 0, es) && pairs_ok(a.gate, a.gb, 0, es) && pairs_ok(a.y, 0, 0, es);
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
         constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value;

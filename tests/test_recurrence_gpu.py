@@ -203,3 +203,53 @@ def test_a_prompt_and_its_tokens(form):
     got = torch.cat(rows, 1)
     assert float((got.float() - whole.float()).abs().max()) <= 2.0 ** -7 * float(whole.abs().max())
     assert float((state - last).abs().max()) <= 2.0 ** -17 * float(last.abs().max()) * 4
+
+
+def fast_scan(a, u):
+    """``layer_ref.scan`` from pairs of tokens."""
+    T = u.shape[1]
+    if T == 1:
+        return u
+    odd = fast_scan(a[:, 1::2] * a[:, :T - 1:2], u[:, 1::2] + a[:, 1::2] * u[:, :T - 1:2])
+    h = torch.empty_like(u)
+    h[:, 1::2], h[:, 0], h[:, 2::2] = odd, u[:, 0], u[:, 2::2] + a[:, 2::2] * odd[:, :(T - 1) // 2]
+    return h
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("B,T,C,ragged", [(1, 40001, 16, False), (1, 9000, 130, False), (2, 5000, 64, True), (1, 30000, 512, False), (3, 2049, 33, True), (9, 3000, 1026, True), (1, 200000, 2, False)])
+def test_long_sequences(B, T, C, dt, form, ragged):
+    """Sequences that several CTAs share.  The bound is ``layer_ref``'s."""
+    x, g, s, dy, ds = inputs(B, T, C, dt, form, 8, True)
+    lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(9)).cuda() if ragged else None
+    n = torch.full((B,), T, device="cuda") if lengths is None else lengths
+    live = (torch.arange(T, device="cuda") < n[:, None])[..., None]
+    a, u = layer_ref.terms(x.double(), g.double(), form)
+    a, u, up = torch.where(live, a, 1.0), torch.where(live, u, 0.0), torch.where(live, dy.double(), 0.0)
+    first = lambda u, s: torch.cat((u[:, :1] + a[:, :1] * s[:, None], u[:, 1:]), 1)  # noqa: E731
+    ahead = torch.cat((a[:, 1:], torch.ones_like(a[:, :1])), 1).flip(1)
+    back = lambda up, s: fast_scan(ahead, torch.cat((up[:, :-1], up[:, -1:] + s[:, None]), 1).flip(1)).flip(1)  # noqa: E731
+    bound = lambda a, H: 2.0 ** -17 * H + 1.25 * 2.0 ** -24 * fast_scan(a, H)  # noqa: E731
+    h, D = fast_scan(a, first(u, s.double())), back(up, ds.double())
+    H, E = fast_scan(a, first(u.abs(), s.double().abs())), back(up.abs(), ds.double().abs())
+    dh, dD = bound(a, H), bound(ahead, E.flip(1)).flip(1)
+    prior = lambda h, s: torch.cat((s[:, None], h[:, :-1]), 1)  # noqa: E731
+    leaves = [t.detach().requires_grad_(True) for t in (x, g, s)]
+    out = gated_recurrence(leaves[0], leaves[1], form=form, initial_state=leaves[2], lengths=lengths, return_state=True)
+    grads = torch.autograd.grad(out, leaves, (dy, ds))
+    assert layer_ref.within(out[0].detach(), torch.where(live, h, 0.0), dh) <= 1
+    assert layer_ref.within(out[1].detach(), h[:, -1], dh[:, -1]) <= 1
+    before, off = prior(h, s.double()), prior(dh, torch.zeros_like(s.double()))
+    size = prior(H, s.double().abs())
+    if form == "decay":
+        dx, dg, bx, bg = D, a * D * before, dD, a * (dD * size + E * off)
+    else:
+        rest = torch.sigmoid(-g.double())
+        dx, dg, bx, bg = rest * D, a * rest * D * (before - x.double()), rest * dD, a * rest * (dD * (size + x.double().abs()) + E * off)
+    where = lambda t: torch.where(live, t, 0.0)  # noqa: E731
+    assert layer_ref.within(grads[0], where(dx), bx + 2.0 ** -19 * E) <= 1
+    assert layer_ref.within(grads[1], where(dg), bg + 2.0 ** -19 * a * E * (size + x.double().abs())) <= 1
+    assert layer_ref.within(grads[2], a[:, 0] * D[:, 0], a[:, 0] * (dD[:, 0] + 2.0 ** -19 * E[:, 0])) <= 1
+    again = gated_recurrence(x, g, form=form, initial_state=s, lengths=lengths)
+    assert torch.equal(again, out[0])
