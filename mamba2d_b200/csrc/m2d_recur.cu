@@ -9,11 +9,11 @@
 // that of every CTA of the cluster; then each goes over its tokens again from the state before them, still from registers, and stores.  So
 // memory is read once and written once, and the loads of the next tile are under way meanwhile.  What is wanted are loads in flight
 // (16 warps an SM with 64 bytes and more a thread): where sequences and channels are too few, rows are split into shorter pieces and
-// a tile into more runs, then the sequence over up to 8 CTAs.
+// the sequence over up to 8 CTAs (plan_recur).
 //
 // Precision: states and sums are fp32.  A channel may remember thousands of tokens: 1 - A of a run is small then, and A
 // rounded to fp32 would be off by the same amount at every step, 2^-24 against a 1 - A of 2^-12 at a memory of 4096 tokens.  So A is held in two
-// parts, from E = A - 1 computed without cancellation (expm1 of the summed gates, or a sum of 1 - f).
+// parts, from E = A - 1 computed without cancellation (a series in the summed gates, or a sum of 1 - f).
 #include <cooperative_groups.h>
 
 #include "follow.cuh"
@@ -36,7 +36,7 @@ struct RecurArgs {
     int B, T, C, groups, ctas;         // channel groups, CTAs of a cluster
 };
 
-// One channel or two: packed arithmetic for two.  Single ones are rounded where those are: the same bits, however rows are aligned.
+// One channel or two: packed arithmetic for two.  Single ones are rounded where those are.
 template <int VEC> struct Num;
 template <> struct Num<1> {
     float v;
@@ -154,6 +154,7 @@ struct Step {
 // The same for a run of tokens, collected token by token: the sum of the gates, or the product of f and the sum that is 1 - A.
 template <int FORM, int VEC>
 struct Collect {
+    using N = Num<VEC>;
     Num<VEC> s = Num<VEC>::all(0.f), p = Num<VEC>::all(1.f);
     __device__ __forceinline__ void add(Num<VEC> g, Num<VEC> a, Num<VEC> rest) {
         if constexpr (FORM == M2D_GATE_DECAY) {
@@ -165,9 +166,18 @@ struct Collect {
     }
     __device__ __forceinline__ Step<VEC> done() const {
         Step<VEC> r;
+        N e = neg_(s);
+        if constexpr (FORM == M2D_GATE_DECAY) {
+            // exp(s) - 1 by its series, used for |s| <= log 2: the tenth power's term is below 2^-26 of the sum
+            e = N::all(1.f / 362880);
+            constexpr float c[] = {1.f / 40320, 1.f / 5040, 1.f / 720, 1.f / 120, 1.f / 24, 1.f / 6, 0.5f, 1.f};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e = fma_(e, s, N::all(c[k]));
+            e = mul_(e, s);
+        }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float t = s.get(v), A = FORM == M2D_GATE_DECAY ? ex2(t * kLog2e) : p.get(v), E = FORM == M2D_GATE_DECAY ? expm1f(t) : -t;
+            const float A = FORM == M2D_GATE_DECAY ? ex2(s.get(v) * kLog2e) : p.get(v), E = e.get(v);
             const bool near = A >= 0.5f && A <= 2.f;
             const float hi = near ? 1.f + E : A;
             r.hi.set(v, hi);
@@ -176,6 +186,21 @@ struct Collect {
         return r;
     }
 };
+// Two Nums of VEC channels side by side in shared memory: hi and lo of a step, or what goes with it.
+template <int VEC> struct Two { Num<VEC> a, b; };
+template <int VEC> __device__ __forceinline__ Two<VEC> take2(const float* p) {
+    if constexpr (VEC == 1) {
+        const float2 f = *reinterpret_cast<const float2*>(p);
+        return {{f.x}, {f.y}};
+    } else {
+        const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(p);
+        return {{f.x}, {f.y}};
+    }
+}
+template <int VEC> __device__ __forceinline__ void give2(float* p, Num<VEC> a, Num<VEC> b) {
+    if constexpr (VEC == 1) *reinterpret_cast<float2*>(p) = make_float2(a.v, b.v);
+    else *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(a.v, b.v);
+}
 // VEC neighbouring floats of shared memory
 template <int VEC> __device__ __forceinline__ Num<VEC> take(const float* p) {
     if constexpr (VEC == 1) return {*p};
@@ -197,17 +222,56 @@ template <int VEC> __device__ __forceinline__ void store_state(float* p, Num<VEC
     for (int v = 0; v < VEC; ++v) p[v] = n.get(v);
 }
 
+// Rows of fewer lanes than a warp has: its runs are joined by shuffles first.
+template <int VEC> __device__ __forceinline__ Num<VEC> moved(Num<VEC> n, int lanes, bool up) {
+    if constexpr (VEC == 1) return {up ? __shfl_up_sync(0xffffffffu, n.v, lanes) : __shfl_down_sync(0xffffffffu, n.v, lanes)};
+    else return Num<2>{up ? __shfl_up_sync(0xffffffffu, n.v, lanes) : __shfl_down_sync(0xffffffffu, n.v, lanes)};
+}
+// step and b of all runs of the warp up to and with the lane's own (UP: in the order of time, else against it).
+template <int VEC, int LANES, bool UP>
+__device__ __forceinline__ void join_warp(Step<VEC>& step, Num<VEC>& b) {
+    const int run = (threadIdx.x & 31) / LANES, before = UP ? run : 32 / LANES - 1 - run;
+#pragma unroll
+    for (int k = 1; k < 32 / LANES; k *= 2) {
+        const Step<VEC> first{moved<VEC>(step.hi, k * LANES, UP), moved<VEC>(step.lo, k * LANES, UP)};
+        const Num<VEC> c = moved<VEC>(b, k * LANES, UP);
+        if (before >= k) {
+            b = step.apply(c, b);
+            step.times(first);
+        }
+    }
+}
+// The state before the lane's own run, from that before the warp's runs and what join_warp left.
+template <int VEC, int LANES, bool UP>
+__device__ __forceinline__ Num<VEC> after_others(const Step<VEC>& step, Num<VEC> b, Num<VEC> h) {
+    if constexpr (LANES == 32) return h;
+    const int run = (threadIdx.x & 31) / LANES;
+    const Num<VEC> there = moved<VEC>(step.apply(h, b), LANES, UP);
+    return run == (UP ? 0 : 32 / LANES - 1) ? h : there;
+}
+
+// All CTAs of a cluster.  What the caller alone has written to others' shared memory is released; everything else, and stores to global memory
+// above all, need not be waited for.
+__device__ __forceinline__ void cluster_meet(bool wrote) {
+    if (wrote) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Where a thread stands: its channels, its run of a tile, its CTA of the cluster.
 template <int VEC, int LANES>
 struct Place {
     static constexpr int width = LANES * VEC;      // channels of a CTA
-    int at, runs, run, b, c, rank, ctas, len;      // at: first of the thread's channels among the CTA's
-    bool mine;
+    int at, runs, run, warps, warp, b, c, rank, ctas, len;         // at: first of the thread's channels among the CTA's
+    bool mine, first, last;                        // first, last: of the runs of its warp
     __device__ __forceinline__ Place(const RecurArgs& p) {
         const int lane = threadIdx.x & 31, per = 32 / LANES;
         at = lane % LANES * VEC;
-        runs = (blockDim.x >> 5) * per;
-        run = (threadIdx.x >> 5) * per + lane / LANES;
+        warps = blockDim.x >> 5;
+        warp = threadIdx.x >> 5;
+        runs = warps * per;
+        run = warp * per + lane / LANES;
+        first = lane < LANES;
+        last = lane >= 32 - LANES;
         ctas = p.ctas;
         rank = blockIdx.x % ctas;
         const int chain = blockIdx.x / ctas;
@@ -218,10 +282,10 @@ struct Place {
     }
 };
 
-// Shared memory: [2][runs][PARTS][width] of the CTA's runs, [2][ctas][3][width] of the cluster's tiles.  Two of each: one barrier lies between
+// Shared memory: [2][warps][PARTS][width] of the CTA's warps, [2][ctas][3][width] of the cluster's tiles.  Two of each: one barrier lies between
 // what is read of a tile and what is written of the next but one.
 template <int PARTS>
-constexpr size_t recur_smem(int runs, int ctas, int width) { return sizeof(float) * 2 * width * ((size_t)runs * PARTS + (ctas > 1 ? (size_t)ctas * 3 : 0)); }
+constexpr size_t recur_smem(int warps, int ctas, int width) { return sizeof(float) * 2 * width * ((size_t)warps * PARTS + (ctas > 1 ? (size_t)ctas * 3 : 0)); }
 
 template <typename T, int VEC, int FORM, int L, int LANES>
 __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const RecurArgs p) {
@@ -242,24 +306,27 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
     auto load = [&](int t0) {
         const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt;
         const int n = w.mine ? w.len - t0 : 0;
+        if (n >= L) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            rx[i] = P::fill(0.f);
-            rg[i] = P::fill(kept<FORM>());
-            if (i < n) {
+            for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt) {
                 rx[i] = __ldcs(reinterpret_cast<const Raw*>(px));
                 rg[i] = __ldcs(reinterpret_cast<const Raw*>(pg));
             }
-            px += p.xt;
-            pg += p.gt;
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt) {
+                rx[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(px)) : P::fill(0.f);
+                rg[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pg)) : P::fill(kept<FORM>());
+            }
         }
     };
+    float* const cluster_part = smem + (size_t)2 * w.warps * 3 * width;
     N carry = load_state<VEC>(p.state + (long long)w.b * p.C + w.c, p.state && w.mine);
     int t0 = w.rank * tile + w.run * L;
     load(t0);
     if (w.ctas > 1) cluster.barrier_wait();
     for (int s0 = 0, buf = 0; s0 < w.len; s0 += stride, t0 += stride, buf ^= 1) {
-        float* const part = smem + (size_t)buf * w.runs * 3 * width + w.at;
+        float *const steps = smem + (size_t)buf * w.warps * 3 * width + 2 * w.at, *const adds = smem + (size_t)(buf * 3 + 2) * w.warps * width + w.at;
         N a[L], u[L], h = N::all(0.f);
         Collect<FORM, VEC> all;
 #pragma unroll
@@ -273,69 +340,71 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
         }
         if (s0 + stride < w.len) load(t0 + stride);
         Step<VEC> step = all.done();
-        give(part + (w.run * 3 + 0) * width, step.hi);
-        give(part + (w.run * 3 + 1) * width, step.lo);
-        give(part + (w.run * 3 + 2) * width, h);
+        N add = h;
+        join_warp<VEC, LANES, true>(step, add);
+        if (w.last) {
+            give2(steps + 2 * w.warp * width, step.hi, step.lo);
+            give(adds + w.warp * width, add);
+        }
         __syncthreads();
-        auto entry = [&](const float* q, int k, Step<VEC>& s, N& b) {
-            s.hi = take<VEC>(q + (k * 3 + 0) * width);
-            s.lo = take<VEC>(q + (k * 3 + 1) * width);
-            b = take<VEC>(q + (k * 3 + 2) * width);
-        };
-        Step<VEC> s;
-        N b;
         if (w.ctas > 1) {
-            // the tile's own, to every CTA of the cluster
-            Step<VEC> whole{N::all(1.f), N::all(0.f)};
-            N sum = N::all(0.f);
-#pragma unroll 4
-            for (int k = 0; k < w.runs; ++k) {
-                entry(part, k, s, b);
-                sum = s.apply(sum, b);
-                whole.times(s);
-            }
-            float* const tiles = smem + (size_t)2 * w.runs * 3 * width + (size_t)buf * w.ctas * 3 * width + w.at;
-            for (int k = threadIdx.x / 32; k < w.ctas; k += blockDim.x / 32) {
-                float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
-                if ((threadIdx.x & 31) < LANES) {
-                    give(to, whole.hi);
-                    give(to + width, whole.lo);
-                    give(to + 2 * width, sum);
+            // one warp joins the tile's runs and tells every CTA of the cluster
+            float* const tiles = cluster_part + (size_t)buf * w.ctas * 3 * width;
+            if (threadIdx.x < LANES) {
+                Step<VEC> whole{N::all(1.f), N::all(0.f)};
+                N sum = N::all(0.f);
+#pragma unroll 8
+                for (int k = 0; k < w.warps; ++k) {
+                    const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
+                    const Step<VEC> next{s.a, s.b};
+                    sum = next.apply(sum, take<VEC>(adds + k * width));
+                    whole.times(next);
+                }
+                for (int k = 0; k < w.ctas; ++k) {
+                    float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
+                    give2(to + 2 * w.at, whole.hi, whole.lo);
+                    give(to + 2 * width + w.at, sum);
                 }
             }
-            cluster.sync();
+            cluster_meet(threadIdx.x < LANES);
             h = carry;
             for (int k = 0; k < w.ctas; ++k) {
                 if (k == w.rank) h = carry;
-                entry(tiles, k, s, b);
-                carry = s.apply(carry, b);
-            }
-#pragma unroll 4
-            for (int k = 0; k < w.run; ++k) {
-                entry(part, k, s, b);
-                h = s.apply(h, b);
+                const Two<VEC> s = take2<VEC>(tiles + k * 3 * width + 2 * w.at);
+                carry = Step<VEC>{s.a, s.b}.apply(carry, take<VEC>(tiles + k * 3 * width + 2 * width + w.at));
             }
         } else {
-#pragma unroll 4
-            for (int k = 0; k < w.run; ++k) {
-                entry(part, k, s, b);
-                carry = s.apply(carry, b);
-            }
             h = carry;
+        }
 #pragma unroll 4
-            for (int k = w.run; k < w.runs; ++k) {
-                entry(part, k, s, b);
-                carry = s.apply(carry, b);
+        for (int k = 0; k < w.warp; ++k) {
+            const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
+            h = Step<VEC>{s.a, s.b}.apply(h, take<VEC>(adds + k * width));
+        }
+        if (w.ctas == 1) {
+            carry = h;
+#pragma unroll 4
+            for (int k = w.warp; k < w.warps; ++k) {
+                const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
+                carry = Step<VEC>{s.a, s.b}.apply(carry, take<VEC>(adds + k * width));
             }
         }
+        h = after_others<VEC, LANES, true>(step, add, h);
         const int n = w.mine ? w.len - t0 : 0;
         if (p.marks && n > 0 && t0 % kMark == 0) store_state<VEC>(p.marks + ((long long)w.b * ((p.T + kMark - 1) / kMark) + t0 / kMark) * p.C + w.c, h);
         T* py = y + (long long)t0 * p.C;
+        if (n >= L) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            h = fma_(a[i], h, u[i]);
-            if (i < n) *reinterpret_cast<Raw*>(py) = P::put(h);
-            py += p.C;
+            for (int i = 0; i < L; ++i, py += p.C) {
+                h = fma_(a[i], h, u[i]);
+                *reinterpret_cast<Raw*>(py) = P::put(h);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; ++i, py += p.C) {
+                h = fma_(a[i], h, u[i]);
+                if (i < n) *reinterpret_cast<Raw*>(py) = P::put(h);
+            }
         }
     }
     if (!w.mine) return;
@@ -368,28 +437,31 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
     auto load = [&](int t1) {
         const int t0 = t1 + w.run * L, n = w.mine ? w.len - t0 : 0;
         const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt, *pd = dy + t0 * p.dt;
+        if (n >= L) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            rx[i] = rd[i] = P::fill(0.f);
-            rg[i] = P::fill(kept<FORM>());
-            if (i < n) {
+            for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt, pd += p.dt) {
                 rx[i] = __ldcs(reinterpret_cast<const Raw*>(px));
                 rg[i] = __ldcs(reinterpret_cast<const Raw*>(pg));
                 rd[i] = __ldcs(reinterpret_cast<const Raw*>(pd));
             }
-            px += p.xt;
-            pg += p.gt;
-            pd += p.dt;
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt, pd += p.dt) {
+                rx[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(px)) : P::fill(0.f);
+                rg[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pg)) : P::fill(kept<FORM>());
+                rd[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pd)) : P::fill(0.f);
+            }
         }
         mark = load_state<VEC>(marks + (long long)(t1 / kMark) * p.C, w.mine && t1 < w.len);
     };
+    float* const cluster_part = smem + (size_t)2 * w.warps * 4 * width;
     N carry = load_state<VEC>(p.d_state_out + (long long)w.b * p.C + w.c, p.d_state_out && w.mine);
     int s0 = w.len > 0 ? (w.len - 1) / stride * stride : -1;
     if (s0 >= 0) load(s0 + w.rank * tile);
     if (w.ctas > 1) cluster.barrier_wait();
     for (int buf = 0; s0 >= 0; s0 -= stride, buf ^= 1) {
         const int t0 = s0 + w.rank * tile + w.run * L;
-        float* const part = smem + (size_t)buf * w.runs * 4 * width + w.at;
+        float *const steps = smem + (size_t)buf * w.warps * 4 * width + 2 * w.at, *const adds = steps + (size_t)w.warps * 2 * width;
         N a[L], rest[L], xv[L], dv[L], before[L], h = N::all(0.f), R = N::all(0.f);
         Collect<FORM, VEC> all;
 #pragma unroll
@@ -405,68 +477,63 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         for (int i = L - 1; i >= 0; --i) R = mul_(a[i], add_(dv[i], R));
         const N first = mark;
         if (s0 >= stride) load(s0 - stride + w.rank * tile);
-        const Step<VEC> step = all.done();
-        give(part + (w.run * 4 + 0) * width, step.hi);
-        give(part + (w.run * 4 + 1) * width, step.lo);
-        give(part + (w.run * 4 + 2) * width, h);
-        give(part + (w.run * 4 + 3) * width, R);
+        Step<VEC> up = all.done(), down = up;
+        N add = h, flow = R;
+        join_warp<VEC, LANES, true>(up, add);
+        join_warp<VEC, LANES, false>(down, flow);
+        if (w.last) {
+            give2(steps + 2 * w.warp * width, up.hi, up.lo);
+            give(adds + 2 * w.warp * width, add);
+        }
+        if (w.first) give(adds + 2 * w.warp * width + VEC, flow);
         __syncthreads();
-        Step<VEC> s;
-        auto entry = [&](int k, int which) {
-            s.hi = take<VEC>(part + (k * 4 + 0) * width);
-            s.lo = take<VEC>(part + (k * 4 + 1) * width);
-            return take<VEC>(part + (k * 4 + which) * width);
+        auto back = [&](int k, N from) {
+            const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
+            return Step<VEC>{s.a, s.b}.apply(from, take<VEC>(adds + 2 * k * width + VEC));
         };
         if (w.ctas > 1) {
-            Step<VEC> whole{N::all(1.f), N::all(0.f)};
-            N sum = N::all(0.f);
-#pragma unroll 4
-            for (int k = w.runs - 1; k >= 0; --k) {
-                const N b = entry(k, 3);
-                sum = s.apply(sum, b);
-                whole.times(s);
-            }
-            float* const tiles = smem + (size_t)2 * w.runs * 4 * width + (size_t)buf * w.ctas * 3 * width + w.at;
-            for (int k = threadIdx.x / 32; k < w.ctas; k += blockDim.x / 32) {
-                float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
-                if ((threadIdx.x & 31) < LANES) {
-                    give(to, whole.hi);
-                    give(to + width, whole.lo);
-                    give(to + 2 * width, sum);
+            float* const tiles = cluster_part + (size_t)buf * w.ctas * 3 * width;
+            if (threadIdx.x < LANES) {
+                Step<VEC> whole{N::all(1.f), N::all(0.f)};
+                N sum = N::all(0.f);
+#pragma unroll 8
+                for (int k = w.warps - 1; k >= 0; --k) {
+                    const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
+                    const Step<VEC> next{s.a, s.b};
+                    sum = next.apply(sum, take<VEC>(adds + 2 * k * width + VEC));
+                    whole.times(next);
+                }
+                for (int k = 0; k < w.ctas; ++k) {
+                    float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
+                    give2(to + 2 * w.at, whole.hi, whole.lo);
+                    give(to + 2 * width + w.at, sum);
                 }
             }
-            cluster.sync();
+            cluster_meet(threadIdx.x < LANES);
             R = carry;
             for (int k = w.ctas - 1; k >= 0; --k) {
                 if (k == w.rank) R = carry;
-                s.hi = take<VEC>(tiles + (k * 3 + 0) * width);
-                s.lo = take<VEC>(tiles + (k * 3 + 1) * width);
-                carry = s.apply(carry, take<VEC>(tiles + (k * 3 + 2) * width));
-            }
-#pragma unroll 4
-            for (int k = w.runs - 1; k > w.run; --k) {
-                const N b = entry(k, 3);
-                R = s.apply(R, b);
+                const Two<VEC> s = take2<VEC>(tiles + k * 3 * width + 2 * w.at);
+                carry = Step<VEC>{s.a, s.b}.apply(carry, take<VEC>(tiles + k * 3 * width + 2 * width + w.at));
             }
         } else {
-#pragma unroll 4
-            for (int k = w.runs - 1; k > w.run; --k) {
-                const N b = entry(k, 3);
-                carry = s.apply(carry, b);
-            }
             R = carry;
-#pragma unroll 4
-            for (int k = w.run; k >= 0; --k) {
-                const N b = entry(k, 3);
-                carry = s.apply(carry, b);
-            }
         }
+#pragma unroll 4
+        for (int k = w.warps - 1; k > w.warp; --k) R = back(k, R);
+        if (w.ctas == 1) {
+            carry = R;
+#pragma unroll 4
+            for (int k = w.warp; k >= 0; --k) carry = back(k, carry);
+        }
+        R = after_others<VEC, LANES, false>(down, flow, R);
         h = first;
 #pragma unroll 4
-        for (int k = 0; k < w.run; ++k) {
-            const N b = entry(k, 2);
-            h = s.apply(h, b);
+        for (int k = 0; k < w.warp; ++k) {
+            const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
+            h = Step<VEC>{s.a, s.b}.apply(h, take<VEC>(adds + 2 * k * width));
         }
+        h = after_others<VEC, LANES, true>(up, add, h);
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             before[i] = h;
@@ -474,19 +541,21 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         }
         const int n = w.mine ? w.len - t0 : 0;
         T *px = dx + (long long)(t0 + L - 1) * p.C, *pg = dgate + (long long)(t0 + L - 1) * p.C;
+        auto write = [&](auto whole) {
 #pragma unroll
-        for (int i = L - 1; i >= 0; --i) {
-            const N D = add_(dv[i], R);
-            R = mul_(a[i], D);
-            const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
-            const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv[i], N::all(-1.f), before[i]));
-            if (i < n) {
-                *reinterpret_cast<Raw*>(px) = P::put(gx);
-                *reinterpret_cast<Raw*>(pg) = P::put(gg);
+            for (int i = L - 1; i >= 0; --i, px -= p.C, pg -= p.C) {
+                const N D = add_(dv[i], R);
+                R = mul_(a[i], D);
+                const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
+                const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv[i], N::all(-1.f), before[i]));
+                if (whole.value || i < n) {
+                    *reinterpret_cast<Raw*>(px) = P::put(gx);
+                    *reinterpret_cast<Raw*>(pg) = P::put(gg);
+                }
             }
-            px -= p.C;
-            pg -= p.C;
-        }
+        };
+        if (n >= L) write(std::true_type{});
+        else write(std::false_type{});
     }
     if (!w.mine) return;
     for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) {
@@ -551,24 +620,34 @@ static int for_recur(const m2d_recur_desc* d, bool pairs, F fn) {
     if (d->dtype == M2D_F32) return pairs ? with_form(float{}, integral_constant<int, 2>{}) : with_form(float{}, integral_constant<int, 1>{});
     return pairs ? with_form(__nv_bfloat16{}, integral_constant<int, 2>{}) : with_form(__nv_bfloat16{}, integral_constant<int, 1>{});
 }
-// Lanes of a row, warps of a CTA and CTAs of a cluster: enough warps that an SM has 16, first by more runs in a tile, then
-// by rows cut into pieces of 16 and of 8 lanes (of two bf16: 64 and 32 bytes), then by the cluster.
+// Lanes of a row, warps of a CTA and CTAs of a cluster: the least time by a model of it.  An SM holds 16 warps (128 registers a
+// thread); clusters of 4 and 8 leave some SMs of a GPC over (33 and 15 of such CTAs fit 148 SMs).  All clusters run in so many waves, and each takes so many
+// strides; a stride takes about a time of 10 for its chain of load, joins and store and 1 for each warp of the SM (its instructions).
+// Rows in pieces of 16 or 8 lanes (64 and 32 bytes of bf16), larger clusters and CTAs that have an SM for themselves cost a little more.
 struct RecurPlan { int lanes, warps, ctas; };
-static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps) {
-    const long long want = 16ll * sm_count(), runs = (d->T + steps - 1) / steps;
-    RecurPlan pl{32, 1, 1};
-    auto warps = [&](int lanes) { return (long long)d->B * ((d->C + lanes * vec - 1) / (lanes * vec)); };
-    while (pl.lanes > 8 && warps(pl.lanes) * kRecurWarps * kRecurCluster * 4 < want * 3 && runs >= 64) pl.lanes /= 2;
-    const int per = 32 / pl.lanes;
-    const long long chains = warps(pl.lanes), need = std::max<long long>(4, (want + chains - 1) / chains), have = (runs + per - 1) / per;
-    pl.warps = (int)std::min<long long>(std::min<long long>(need, have), 8);
-    while (pl.ctas < kRecurCluster && pl.ctas * 2 * pl.warps <= std::min(need, have)) pl.ctas *= 2;
-    if (pl.ctas == kRecurCluster) pl.warps = (int)std::min<long long>(kRecurWarps, std::min(need, have) / pl.ctas);
-    return pl;
+static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, bool bwd) {
+    const long long runs = (d->T + steps - 1) / steps, sms = sm_count();
+    RecurPlan best{32, 1, 1};
+    double least = 1e300;
+    for (int lanes = 32; lanes >= (vec == 2 ? 8 : 32); lanes /= 2) {
+        const long long chains = (long long)d->B * ((d->C + lanes * vec - 1) / (lanes * vec));
+        for (int warps = 1; warps <= kRecurWarps; warps *= 2)
+            for (int ctas = 1; ctas <= kRecurCluster; ctas *= 2) {
+                const long long tile = (long long)warps * (32 / lanes);            // in runs
+                if (ctas > 1 && tile * (ctas / 2) >= runs) break;                  // (half of them would do)
+                if (bwd && tile * steps % kMark && (ctas > 1 || tile < runs)) continue;        // (a tile begins at a mark)
+                const long long held = std::max(1ll, (ctas == 8 ? sms * 15 / 148 : ctas == 4 ? sms * 33 / 148 : sms / ctas)) * (kRecurWarps / warps);
+                const long long waves = (chains + held - 1) / held, strides = (runs + tile * ctas - 1) / (tile * ctas);
+                const long long per_sm = std::min<long long>(kRecurWarps, (chains * ctas + sms - 1) / sms * warps);
+                const double t = (double)(waves * strides) * (10 + per_sm) * (warps == 16 ? 1.1 : 1.0) * (lanes == 32 ? 1.0 : lanes == 16 ? 1.05 : 1.15) * (ctas == 1 ? 1.0 : 1.1 + 0.02 * ctas);
+                if (t < least) { least = t; best = {lanes, warps, ctas}; }
+            }
+    }
+    return best;
 }
 template <int PARTS, typename K>
 static int launch_recur(K kern, const RecurArgs& a, const RecurPlan& pl, int vec, cudaStream_t st) {
-    const size_t smem = recur_smem<PARTS>(pl.warps * (32 / pl.lanes), pl.ctas, pl.lanes * vec);
+    const size_t smem = recur_smem<PARTS>(pl.warps, pl.ctas, pl.lanes * vec);
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.B * a.groups * pl.ctas));
@@ -616,10 +695,9 @@ extern "C" int m2d_recur_fwd(const m2d_recur_desc* d, void* stream) {
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
         constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kFwdSteps<T>;
-        RecurPlan pl = plan_recur(d, VEC, L);
+        const RecurPlan pl = plan_recur(d, VEC, L, false);
         return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
             constexpr int LANES = decltype(lanes)::value;
-            pl.lanes = LANES;
             a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
             a.ctas = pl.ctas;
             return launch_recur<3>(recur_fwd_kernel<T, VEC, FORM, L, LANES>, a, pl, VEC, static_cast<cudaStream_t>(stream));
@@ -637,11 +715,9 @@ extern "C" int m2d_recur_bwd(const m2d_recur_desc* d, void* stream) {
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
         constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kBwdSteps;
-        RecurPlan pl = plan_recur(d, VEC, L);
+        const RecurPlan pl = plan_recur(d, VEC, L, true);
         return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
-            constexpr int LANES = decltype(lanes)::value, runs = kMark / L * LANES / 32;       // (warps that hold the tokens between marks)
-            pl.lanes = LANES;
-            if (pl.ctas > 1 || pl.warps * (32 / LANES) * L < d->T) pl.warps = (pl.warps + runs - 1) / runs * runs;    // (one tile has the first mark)
+            constexpr int LANES = decltype(lanes)::value;
             a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
             a.ctas = pl.ctas;
             return launch_recur<4>(recur_bwd_kernel<T, VEC, FORM, L, LANES>, a, pl, VEC, static_cast<cudaStream_t>(stream));
