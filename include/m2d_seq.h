@@ -168,7 +168,7 @@ int m2d_recur_step(const m2d_recur_desc *desc, int64_t state_batch, void *stream
 /* ---- layer normalisation ----------------------------------------------------------------------------------------
  * Rows x (N,C): s = x + residual, rounded to the tensors' type; y = (s - mean) / sqrt(var + eps) * weight + bias.  Rows lie as far apart as is
  * given, neighbours along C.  Rows that begin at 16-byte boundaries and are whole 16-byte pieces, parameters too, are read in such pieces.  Rows of
- * more than 16384 values (8192 in single reads and in the backward pass) are read three times.  N below 2^31, C up to 2^30.
+ * more than 8192 values are read three times.  N below 2^31, C up to 2^30.
  */
 typedef struct m2d_ln_desc {
     uint32_t struct_bytes;         /* = sizeof(m2d_ln_desc) */

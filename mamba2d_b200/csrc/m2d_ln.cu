@@ -8,6 +8,7 @@
 // has the same columns in every row that it meets: it sums their parameter gradients in registers, CTAs write their sums side by side, and a second
 // launch adds those up in a fixed order.  Rows too long for registers are read again where they are needed.
 #include "follow.cuh"
+#include "packed.cuh"
 #include "plan.cuh"
 #include "m2d_seq.h"
 
@@ -24,52 +25,63 @@ struct LnArgs {
     float eps;
 };
 
+// V neighbouring values as they are in memory, and as V / W packed numbers.
 template <typename T, int V> struct Lane;
 template <> struct Lane<float, 4> {
     using Raw = float4;
-    static __device__ __forceinline__ void get(const Raw& r, float* v) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
-    static __device__ __forceinline__ Raw put(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
+    using N = Num<2>;
+    static constexpr int n = 2;
+    static __device__ __forceinline__ void get(const Raw& r, N* v) { v[0] = N::make(r.x, r.y); v[1] = N::make(r.z, r.w); }
+    static __device__ __forceinline__ Raw put(const N* v) { return make_float4(v[0].get(0), v[0].get(1), v[1].get(0), v[1].get(1)); }
 };
 template <> struct Lane<float, 1> {
     using Raw = float;
-    static __device__ __forceinline__ void get(Raw r, float* v) { v[0] = r; }
-    static __device__ __forceinline__ Raw put(const float* v) { return v[0]; }
+    using N = Num<1>;
+    static constexpr int n = 1;
+    static __device__ __forceinline__ void get(Raw r, N* v) { v[0].v = r; }
+    static __device__ __forceinline__ Raw put(const N* v) { return v[0].v; }
 };
 template <> struct Lane<__nv_bfloat16, 8> {
     using Raw = uint4;
-    static __device__ __forceinline__ void get(const Raw& r, float* v) {
+    using N = Num<2>;
+    static constexpr int n = 4;
+    static __device__ __forceinline__ void get(const Raw& r, N* v) {
         const unsigned u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+        for (int i = 0; i < 4; ++i) v[i] = N::make(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
     }
-    static __device__ __forceinline__ Raw put(const float* v) {
-        return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    static __device__ __forceinline__ Raw put(const N* v) {
+        return make_uint4(pack_bf16x2(v[0].get(0), v[0].get(1)), pack_bf16x2(v[1].get(0), v[1].get(1)), pack_bf16x2(v[2].get(0), v[2].get(1)), pack_bf16x2(v[3].get(0), v[3].get(1)));
     }
 };
 template <> struct Lane<__nv_bfloat16, 1> {
     using Raw = unsigned short;
-    static __device__ __forceinline__ void get(Raw r, float* v) { v[0] = bf16_bits_to_float(r); }
-    static __device__ __forceinline__ Raw put(const float* v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v[0])); }
+    using N = Num<1>;
+    static constexpr int n = 1;
+    static __device__ __forceinline__ void get(Raw r, N* v) { v[0].v = bf16_bits_to_float(r); }
+    static __device__ __forceinline__ Raw put(const N* v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v[0].v)); }
 };
 // V neighbouring values of a parameter (fp32 or T); `none` where there is no such parameter.
 template <typename T, int V>
-__device__ __forceinline__ void parameter(const void* p, int f32, int c, float none, float* v) {
+__device__ __forceinline__ void parameter(const void* p, int f32, int c, float none, typename Lane<T, V>::N* v) {
+    using P = Lane<T, V>;
     if (!p) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = none;
+        for (int k = 0; k < P::n; ++k) v[k] = P::N::all(none);
     } else if (f32) {
         const float* q = static_cast<const float*>(p) + c;
         if constexpr (V % 4 == 0) {
 #pragma unroll
-            for (int k = 0; k < V; k += 4) Lane<float, 4>::get(__ldg(reinterpret_cast<const float4*>(q + k)), v + k);
+            for (int k = 0; k < V; k += 4) Lane<float, 4>::get(__ldg(reinterpret_cast<const float4*>(q + k)), v + k / 2);
         } else {
-            v[0] = __ldg(q);
+            v[0].v = __ldg(q);
         }
     } else {
-        using P = Lane<T, V>;
         P::get(__ldg(reinterpret_cast<const typename P::Raw*>(static_cast<const T*>(p) + c)), v);
     }
 }
+__device__ __forceinline__ float total(Num<1> n) { return n.v; }
+__device__ __forceinline__ float total(Num<2> n) { return n.get(0) + n.get(1); }
 template <typename T> __device__ __forceinline__ float value_of(const T* p) {
     if constexpr (sizeof(T) == 4) return *p;
     else return __bfloat162float(*p);
@@ -105,164 +117,221 @@ __device__ __forceinline__ void row_sum(float (&v)[K], int& slot) {
 }
 constexpr int kLnThreads = 256;        // of a CTA whose rows are held by parts of warps
 
-template <typename T, int V, int R, int NV>
-__global__ void __launch_bounds__(R ? kLnThreads : 1024) ln_fwd_kernel(const LnArgs p) {
+// A thread's share of the rows: columns (i span + l) V ..., i < NV, of every `step`-th row from `row` on, as many rows at a time as `step` says
+// all CTAs have.  The loads of its next row are under way while it works on one, and the parameters stay in registers.
+template <int V, int R>
+struct Share {
+    static constexpr int lanes = R ? R : 1;
+    int span, l;
+    long long row, step;
+    __device__ __forceinline__ Share() {
+        span = R ? R : blockDim.x;
+        l = R ? threadIdx.x % lanes : threadIdx.x;
+        const int rows = R ? kLnThreads / lanes : 1;
+        row = (long long)blockIdx.x * rows + (R ? threadIdx.x / lanes : 0);
+        step = (long long)gridDim.x * rows;
+    }
+    __device__ __forceinline__ int column(int i) const { return (i * span + l) * V; }
+    // rows that a CTA still meets: the same number for all of its threads, which reduce together
+    __device__ __forceinline__ bool more(long long N, long long at) const { return at - (R ? threadIdx.x / lanes : 0) < N; }
+};
+
+template <typename T, int V, int R, int NV, bool RES>
+__global__ void __launch_bounds__(R ? kLnThreads : 512) ln_fwd_kernel(const LnArgs p) {
     using P = Lane<T, V>;
     using Raw = typename P::Raw;
-    const int span = R ? R : blockDim.x, l = R ? threadIdx.x % R : threadIdx.x;
-    const long long row = R ? (long long)blockIdx.x * (kLnThreads / (R ? R : 1)) + threadIdx.x / (R ? R : 1) : blockIdx.x;
-    const bool on = row < p.N;
-    const T *const x = static_cast<const T*>(p.x) + (on ? row : 0) * p.xp, *const r = p.r ? static_cast<const T*>(p.r) + (on ? row : 0) * p.rp : nullptr;
-    float v[NV][V];
-    int slot = 0;
+    using N = typename P::N;
+    const Share<V, R> at;
+    N w[NV][P::n], b[NV][P::n];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * span + l) * V;
-        Raw a{};
-        if (on && c < p.C) a = __ldcs(reinterpret_cast<const Raw*>(x + c));
-        P::get(a, v[i]);
-    }
-    float first = value_of(x);
-    if (r) {
-        first = sum_as<T>(first, value_of(r));
+    for (int i = 0; i < NV; ++i)
+        if (at.column(i) < p.C) {
+            parameter<T, V>(p.w, p.params_f32, at.column(i), 1.f, w[i]);
+            parameter<T, V>(p.b, p.params_f32, at.column(i), 0.f, b[i]);
+        }
+    Raw rx[NV], rr[RES ? NV : 1];
+    float lead, lead_r = 0.f;               // the row's first values
+    auto load = [&](long long row) {
+        const T* const x = static_cast<const T*>(p.x) + (row < p.N ? row : 0) * p.xp;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.column(i) < p.C) rx[i] = __ldcs(reinterpret_cast<const Raw*>(x + at.column(i)));
+        lead = value_of(x);
+        if constexpr (RES) {
+            const T* const r = static_cast<const T*>(p.r) + (row < p.N ? row : 0) * p.rp;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (at.column(i) < p.C) rr[i] = __ldcs(reinterpret_cast<const Raw*>(r + at.column(i)));
+            lead_r = value_of(r);
+        }
+    };
+    int slot = 0;
+    long long row = at.row;
+    if (at.more(p.N, row)) load(row);
+    const float per = 1.f / (float)p.C;
+    for (; at.more(p.N, row); row += at.step) {
+        N v[NV][P::n];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * span + l) * V;
-            if (!on || c >= p.C) continue;
-            float t[V];
-            P::get(__ldcs(reinterpret_cast<const Raw*>(r + c)), t);
+            P::get(rx[i], v[i]);
+            if constexpr (RES) {
+                N r[P::n];
+                P::get(rr[i], r);
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[i][k] = sum_as<T>(v[i][k], t[k]);
-            *reinterpret_cast<Raw*>(static_cast<T*>(p.s) + row * p.C + c) = P::put(v[i]);
-        }
-    }
-    float sum[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if ((i * span + l) * V < p.C)
-#pragma unroll
-            for (int k = 0; k < V; ++k) sum[0] += v[i][k] - first;
-    row_sum<R>(sum, slot);
-    const float mean = first + sum[0] / (float)p.C;
-    sum[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if ((i * span + l) * V < p.C)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                v[i][k] -= mean;
-                sum[0] = fmaf(v[i][k], v[i][k], sum[0]);
+                for (int k = 0; k < P::n; ++k) v[i][k] = add_(v[i][k], r[k]);
+                rx[i] = P::put(v[i]);
+                if (row < p.N && at.column(i) < p.C) *reinterpret_cast<Raw*>(static_cast<T*>(p.s) + row * p.C + at.column(i)) = rx[i];
+                P::get(rx[i], v[i]);         // (rounded)
             }
-    row_sum<R>(sum, slot);
-    const float rstd = rsqrtf(sum[0] / (float)p.C + p.eps);
-    if (!on) return;
-    if (p.stats && l == 0) p.stats[row] = make_float2(mean, rstd);
+        }
+        const float first = RES ? sum_as<T>(lead, lead_r) : lead;
+        if (at.more(p.N, row + at.step)) load(row + at.step);
+        N acc = N::all(0.f);
+        const N less = N::all(-first);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * span + l) * V;
-        if (c >= p.C) continue;
-        float w[V], b[V];
-        parameter<T, V>(p.w, p.params_f32, c, 1.f, w);
-        parameter<T, V>(p.b, p.params_f32, c, 0.f, b);
+        for (int i = 0; i < NV; ++i)
+            if (at.column(i) < p.C)
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[i][k] = fmaf(v[i][k] * rstd, w[k], b[k]);
-        *reinterpret_cast<Raw*>(static_cast<T*>(p.y) + row * p.C + c) = P::put(v[i]);
+                for (int k = 0; k < P::n; ++k) acc = add_(acc, add_(v[i][k], less));
+        float sum[1] = {total(acc)};
+        row_sum<R>(sum, slot);
+        const float mean = first + sum[0] / (float)p.C;
+        const N off = N::all(-mean);
+        acc = N::all(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.column(i) < p.C)
+#pragma unroll
+                for (int k = 0; k < P::n; ++k) {
+                    v[i][k] = add_(v[i][k], off);
+                    acc = fma_(v[i][k], v[i][k], acc);
+                }
+        sum[0] = total(acc);
+        row_sum<R>(sum, slot);
+        const float rstd = rsqrtf(fmaf(sum[0], per, p.eps));
+        if (row >= p.N) continue;
+        if (p.stats && at.l == 0) p.stats[row] = make_float2(mean, rstd);
+        const N scale = N::all(rstd);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.column(i) < p.C) {
+#pragma unroll
+                for (int k = 0; k < P::n; ++k) v[i][k] = fma_(mul_(v[i][k], scale), w[i][k], b[i][k]);
+                *reinterpret_cast<Raw*>(static_cast<T*>(p.y) + row * p.C + at.column(i)) = P::put(v[i]);
+            }
     }
 }
 
-template <typename T, int V, int R, int NV>
+template <typename T, int V, int R, int NV, bool DS>
 __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnArgs p) {
     using P = Lane<T, V>;
     using Raw = typename P::Raw;
-    extern __shared__ float sums[];                // where parts of warps hold rows: [columns of all lanes][2]
+    using N = typename P::N;
+    extern __shared__ float sums[];                // where parts of warps hold rows: [warps][2][columns of R lanes]
     let_follow();
-    const int span = R ? R : blockDim.x, l = R ? threadIdx.x % R : threadIdx.x, rows = R ? kLnThreads / (R ? R : 1) : 1;
-    float dw[NV][V] = {}, db[NV][V] = {};
-    int slot = 0;
-    const float per = 1.f / (float)p.C;
-    for (long long first = (long long)blockIdx.x * rows; first < p.N; first += (long long)gridDim.x * rows) {
-        const long long row = first + (R ? threadIdx.x / (R ? R : 1) : 0);
+    const Share<V, R> at;
+    N w[NV][P::n], dw[NV][P::n], db[NV][P::n];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int k = 0; k < P::n; ++k) w[i][k] = dw[i][k] = db[i][k] = N::all(0.f);
+        if (at.column(i) < p.C) parameter<T, V>(p.w, p.params_f32, at.column(i), 1.f, w[i]);
+    }
+    Raw rx[NV], rd[NV], rs[DS ? NV : 1];
+    float2 st;
+    auto load = [&](long long row) {
         const bool on = row < p.N;
         const T *const x = static_cast<const T*>(p.x) + (on ? row : 0) * p.xp, *const dy = static_cast<const T*>(p.dy) + (on ? row : 0) * p.dyp;
-        Raw rx[NV], rd[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * span + l) * V;
             rx[i] = rd[i] = Raw{};
-            if (on && c < p.C) {
-                rx[i] = __ldcs(reinterpret_cast<const Raw*>(x + c));
-                rd[i] = __ldcs(reinterpret_cast<const Raw*>(dy + c));
+            if (on && at.column(i) < p.C) {
+                rx[i] = __ldcs(reinterpret_cast<const Raw*>(x + at.column(i)));
+                rd[i] = __ldcs(reinterpret_cast<const Raw*>(dy + at.column(i)));
+                if constexpr (DS) rs[i] = __ldcs(reinterpret_cast<const Raw*>(static_cast<const T*>(p.ds) + row * p.dsp + at.column(i)));
             }
         }
-        const float2 st = on ? p.stats[row] : make_float2(0.f, 0.f);
-        float h[NV][V], dh[NV][V], sum[2] = {0.f, 0.f};
+        st = on ? p.stats[row] : make_float2(0.f, 0.f);
+    };
+    int slot = 0;
+    long long row = at.row;
+    if (at.more(p.N, row)) load(row);
+    const float per = 1.f / (float)p.C;
+    for (; at.more(p.N, row); row += at.step) {
+        N h[NV][P::n], dh[NV][P::n], s0 = N::all(0.f), s1 = N::all(0.f);
+        Raw keep[DS ? NV : 1];
+        const N off = N::all(-st.x), scale = N::all(st.y);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * span + l) * V;
-            float w[V];
             P::get(rx[i], h[i]);
             P::get(rd[i], dh[i]);
-            if (c < p.C) parameter<T, V>(p.w, p.params_f32, c, 1.f, w);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                h[i][k] = (h[i][k] - st.x) * st.y;
-                if (!on || c >= p.C) h[i][k] = 0.f, w[k] = 0.f;
-                db[i][k] += dh[i][k];
-                dw[i][k] = fmaf(dh[i][k], h[i][k], dw[i][k]);
-                dh[i][k] *= w[k];
-                sum[0] += dh[i][k];
-                sum[1] = fmaf(dh[i][k], h[i][k], sum[1]);
-            }
+            if constexpr (DS) keep[i] = rs[i];
         }
+        const float rstd = st.y;
+        if (at.more(p.N, row + at.step)) load(row + at.step);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at.column(i) < p.C)                // (a row beyond the last: dy is zero and so is h)
+#pragma unroll
+                for (int k = 0; k < P::n; ++k) {
+                    h[i][k] = mul_(add_(h[i][k], off), scale);
+                    db[i][k] = add_(db[i][k], dh[i][k]);
+                    dw[i][k] = fma_(dh[i][k], h[i][k], dw[i][k]);
+                    dh[i][k] = mul_(dh[i][k], w[i][k]);
+                    s0 = add_(s0, dh[i][k]);
+                    s1 = fma_(dh[i][k], h[i][k], s1);
+                }
+        float sum[2] = {total(s0), total(s1)};
         row_sum<R>(sum, slot);
-        if (!on) continue;
-        const float m0 = sum[0] * per, m1 = sum[1] * per;
+        if (row >= p.N) continue;
+        const N m0 = N::all(-sum[0] * per), m1 = N::all(-sum[1] * per), factor = N::all(rstd);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * span + l) * V;
-            if (c >= p.C) continue;
-            float g[V] = {};
-            if (p.ds) P::get(__ldcs(reinterpret_cast<const Raw*>(static_cast<const T*>(p.ds) + row * p.dsp + c)), g);
+        for (int i = 0; i < NV; ++i)
+            if (at.column(i) < p.C) {
+                N g[P::n];
+                if constexpr (DS) P::get(keep[i], g);
 #pragma unroll
-            for (int k = 0; k < V; ++k) g[k] = fmaf(st.y, fmaf(-h[i][k], m1, dh[i][k] - m0), g[k]);
-            *reinterpret_cast<Raw*>(static_cast<T*>(p.dx) + row * p.C + c) = P::put(g);
-        }
+                for (int k = 0; k < P::n; ++k) {
+                    const N t = fma_(h[i][k], m1, add_(dh[i][k], m0));
+                    g[k] = DS ? fma_(factor, t, g[k]) : mul_(factor, t);
+                }
+                *reinterpret_cast<Raw*>(static_cast<T*>(p.dx) + row * p.C + at.column(i)) = P::put(g);
+            }
     }
     if (!p.partial) return;
     float* const out = p.partial + (long long)blockIdx.x * 2 * p.C;
+    constexpr int W = V / P::n;
     if constexpr (R == 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const int c = (i * span + l) * V + k;
-                if (c < p.C) { out[c] = dw[i][k]; out[p.C + c] = db[i][k]; }
+                const int c = at.column(i) + k;
+                if (c < p.C) { out[c] = dw[i][k / W].get(k % W); out[p.C + c] = db[i][k / W].get(k % W); }
             }
     } else {
         // lanes of one warp that have the same columns, then the warps in turn
         constexpr int cols = R * NV * V;
-#pragma unroll
-        for (int m = R; m < 32; m <<= 1)
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    dw[i][k] += __shfl_xor_sync(0xffffffffu, dw[i][k], m);
-                    db[i][k] += __shfl_xor_sync(0xffffffffu, db[i][k], m);
-                }
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        if (lane < R)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    sums[(warp * 2) * cols + (i * R + l) * V + k] = dw[i][k];
-                    sums[(warp * 2 + 1) * cols + (i * R + l) * V + k] = db[i][k];
+            for (int k = 0; k < V; ++k) {
+                float a = dw[i][k / W].get(k % W), b = db[i][k / W].get(k % W);
+#pragma unroll
+                for (int m = R; m < 32; m <<= 1) {
+                    a += __shfl_xor_sync(0xffffffffu, a, m);
+                    b += __shfl_xor_sync(0xffffffffu, b, m);
                 }
+                if (lane < R) {
+                    sums[(warp * 2) * cols + at.column(i) + k] = a;
+                    sums[(warp * 2 + 1) * cols + at.column(i) + k] = b;
+                }
+            }
         __syncthreads();
         for (int c = threadIdx.x; c < 2 * cols; c += kLnThreads) {
             float v = 0.f;
-            for (int w = 0; w < kLnThreads / 32; ++w) v += sums[w * 2 * cols + c];
+            for (int k = 0; k < kLnThreads / 32; ++k) v += sums[k * 2 * cols + c];
             const int col = c % cols;
             if (col < p.C) out[(c / cols) * p.C + col] = v;
         }
@@ -289,10 +358,10 @@ __global__ void __launch_bounds__(kLongThreads) ln_long_fwd_kernel(const LnArgs 
         if (p.stats && threadIdx.x == 0) p.stats[row] = make_float2(mean, rstd);
         for (int c = threadIdx.x; c < p.C; c += kLongThreads) {
             const float v = at(c);
-            float w, b;
+            Num<1> w, b;
             parameter<T, 1>(p.w, p.params_f32, c, 1.f, &w);
             parameter<T, 1>(p.b, p.params_f32, c, 0.f, &b);
-            store1(static_cast<T*>(p.y), row * p.C + c, fmaf((v - mean) * rstd, w, b));
+            store1(static_cast<T*>(p.y), row * p.C + c, fmaf((v - mean) * rstd, w.v, b.v));
             if (r) store1(static_cast<T*>(p.s), row * p.C + c, v);
         }
     }
@@ -304,10 +373,11 @@ __global__ void __launch_bounds__(kLongThreads) ln_long_bwd_kernel(const LnArgs 
     for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
         const T *const x = static_cast<const T*>(p.x) + row * p.xp, *const dy = static_cast<const T*>(p.dy) + row * p.dyp;
         const float2 st = p.stats[row];
-        float sum[2] = {0.f, 0.f}, w;
+        float sum[2] = {0.f, 0.f};
+        Num<1> w;
         for (int c = threadIdx.x; c < p.C; c += kLongThreads) {
             parameter<T, 1>(p.w, p.params_f32, c, 1.f, &w);
-            const float dh = value_of(dy + c) * w;
+            const float dh = value_of(dy + c) * w.v;
             sum[0] += dh;
             sum[1] = fmaf(dh, (value_of(x + c) - st.x) * st.y, sum[1]);
         }
@@ -316,7 +386,7 @@ __global__ void __launch_bounds__(kLongThreads) ln_long_bwd_kernel(const LnArgs 
         for (int c = threadIdx.x; c < p.C; c += kLongThreads) {
             parameter<T, 1>(p.w, p.params_f32, c, 1.f, &w);
             const float h = (value_of(x + c) - st.x) * st.y, g = p.ds ? value_of(static_cast<const T*>(p.ds) + row * p.dsp + c) : 0.f;
-            store1(static_cast<T*>(p.dx), row * p.C + c, fmaf(st.y, fmaf(-h, m1, value_of(dy + c) * w - m0), g));
+            store1(static_cast<T*>(p.dx), row * p.C + c, fmaf(st.y, fmaf(-h, m1, value_of(dy + c) * w.v - m0), g));
         }
     }
     // the parameters' sums: this CTA's rows, column by column
@@ -378,38 +448,42 @@ static LnPlan plan_ln(const m2d_ln_desc* d, bool bwd) {
     LnPlan pl{};
     pl.vec = v ? 16 / es : 1;
     pl.threads = kLnThreads;
-    // up to 16 values a lane
-    const int most = 16 / pl.vec;
-    static const int wide[][2] = {{8, 1}, {8, 2}, {16, 2}, {32, 2}, {32, 4}}, narrow[][2] = {{32, 4}, {32, 16}};
-    for (int i = 0; i < (v ? 5 : 2); ++i) {
-        pl.lanes = v ? wide[i][0] : narrow[i][0];
-        pl.nv = v ? wide[i][1] : narrow[i][1];
-        if (pl.nv <= most && d->C <= pl.lanes * pl.vec * pl.nv) return pl;
-    }
-    pl.lanes = 0;
-    pl.nv = most;
+    // whole pieces: one to three of bf16 a lane, twice as many of fp32, by parts of warps that leave the fewest lanes without work
+    const int unit = es == 4 ? 2 : 1;
+    long long least = INT64_MAX;
+    if (v)
+        for (int lanes = 32; lanes >= 8; lanes /= 2)
+            for (int n = 1; n <= 3; ++n) {
+                const long long room = (long long)lanes * n * unit * pl.vec;
+                if (room >= d->C && room < least) { least = room; pl.lanes = lanes; pl.nv = n * unit; }
+            }
+    else
+        for (int n : {4, 16})
+            if (!pl.lanes && d->C <= 32 * n) { pl.lanes = 32; pl.nv = n; }
+    if (pl.lanes) return pl;
+    pl.nv = v ? 2 * unit : 16;
     pl.threads = (d->C + pl.vec * pl.nv * 32 - 1) / (pl.vec * pl.nv * 32) * 32;
-    if (pl.threads > (bwd ? 512 : 1024)) { pl.lanes = -1; pl.threads = kLongThreads; }
+    if (pl.threads > 512) { pl.lanes = -1; pl.threads = kLongThreads; }
     return pl;
 }
-// Calls fn(element, values of a load, lanes, loads of a lane) with the plan's.
+// Calls fn(element, values of a load, lanes, loads of a lane, flag) with the plan's.
 template <typename F>
-static int for_ln(const m2d_ln_desc* d, const LnPlan& pl, F fn) {
+static int for_ln(const m2d_ln_desc* d, const LnPlan& pl, bool flag, F fn) {
+    using std::integral_constant;
     auto go = [&](auto elem, auto full) {
-        using std::integral_constant;
-        constexpr int V = decltype(full)::value;
-        auto with = [&](auto v, auto lanes, auto nv) { return fn(elem, v, lanes, nv); };
+        constexpr int V = decltype(full)::value, unit = V == 4 ? 2 : 1;
+        auto with = [&](auto v, auto lanes, auto nv) { return flag ? fn(elem, v, lanes, nv, std::true_type{}) : fn(elem, v, lanes, nv, std::false_type{}); };
         constexpr integral_constant<int, 0> cta{};
-        constexpr integral_constant<int, 8> l8{};
-        constexpr integral_constant<int, 16> l16{};
-        constexpr integral_constant<int, 32> l32{};
-        constexpr integral_constant<int, 1> n1{};
-        constexpr integral_constant<int, 2> n2{};
-        constexpr integral_constant<int, 16 / V> most{};
-        if (pl.vec == 1) return pl.lanes == 0 ? with(n1, cta, l16) : pl.nv == 4 ? with(n1, l32, integral_constant<int, 4>{}) : with(n1, l32, l16);
-        if (pl.lanes == 0) return with(full, cta, most);
-        if (pl.lanes == 32) return pl.nv == 2 ? with(full, l32, n2) : with(full, l32, most);
-        return pl.lanes == 16 ? with(full, l16, n2) : pl.nv == 2 ? with(full, l8, n2) : with(full, l8, n1);
+        constexpr integral_constant<int, 1> one{};
+        constexpr integral_constant<int, 4> four{};
+        constexpr integral_constant<int, 16> sixteen{};
+        constexpr integral_constant<int, 32> warp{};
+        if (pl.vec == 1) return pl.lanes == 0 ? with(one, cta, sixteen) : pl.nv == 4 ? with(one, warp, four) : with(one, warp, sixteen);
+        if (pl.lanes == 0) return with(full, cta, integral_constant<int, 2 * unit>{});
+        auto with_lanes = [&](auto lanes) {
+            return pl.nv == unit ? with(full, lanes, integral_constant<int, unit>{}) : pl.nv == 2 * unit ? with(full, lanes, integral_constant<int, 2 * unit>{}) : with(full, lanes, integral_constant<int, 3 * unit>{});
+        };
+        return pl.lanes == 8 ? with_lanes(integral_constant<int, 8>{}) : pl.lanes == 16 ? with_lanes(sixteen) : with_lanes(warp);
     };
     return d->dtype == M2D_F32 ? go(float{}, std::integral_constant<int, 4>{}) : go(__nv_bfloat16{}, std::integral_constant<int, 8>{});
 }
@@ -422,11 +496,24 @@ static LnArgs ln_args(const m2d_ln_desc* d) {
     a.N = d->N; a.C = d->C; a.params_f32 = d->params_f32; a.eps = d->eps;
     return a;
 }
-// CTAs of the backward pass: what the SMs hold at once, so that a CTA meets many rows.
-static long long ln_parts(const m2d_ln_desc* d, const LnPlan& pl) {
-    const long long tasks = (d->N + pl.rows() - 1) / pl.rows();
-    const int held = std::max(1, 768 / pl.threads);
-    return std::min<long long>(tasks, (long long)held * sm_count());
+// CTAs of a launch: what the SMs hold at once.
+static long long ln_grid(const m2d_ln_desc* d, const LnPlan& pl, int per_sm) { return std::min<long long>((d->N + pl.rows() - 1) / pl.rows(), (long long)std::max(1, per_sm) * sm_count()); }
+static size_t ln_bwd_smem(const LnPlan& pl, bool params) { return pl.lanes > 0 && params ? (size_t)kLnThreads / 32 * 2 * pl.lanes * pl.nv * pl.vec * sizeof(float) : 0; }
+// Calls fn(kernel, CTAs) of the backward pass.
+template <typename F>
+static int with_ln_bwd(const m2d_ln_desc* d, F fn) {
+    const LnPlan pl = plan_ln(d, true);
+    const bool params = d->d_weight || d->d_bias;
+    if (pl.lanes < 0) {
+        const long long grid = ln_grid(d, pl, 2);
+        return d->dtype == M2D_F32 ? fn(ln_long_bwd_kernel<float>, pl, grid, (size_t)0) : fn(ln_long_bwd_kernel<__nv_bfloat16>, pl, grid, (size_t)0);
+    }
+    return for_ln(d, pl, d->d_sum != nullptr, [&](auto elem, auto vec, auto lanes, auto nv, auto ds) {
+        auto kern = ln_bwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(ds)::value>;
+        const size_t smem = ln_bwd_smem(pl, params);
+        if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return (int)M2D_ERR_LAUNCH;
+        return fn(kern, pl, ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, smem)), smem);
+    });
 }
 
 }  // namespace m2d
@@ -435,7 +522,12 @@ using namespace m2d;
 
 extern "C" uint64_t m2d_ln_bwd_workspace(const m2d_ln_desc* d) {
     if (check_ln(d) != M2D_OK || (!d->d_weight && !d->d_bias)) return 0;
-    return (uint64_t)ln_parts(d, plan_ln(d, true)) * 2 * d->C * sizeof(float);
+    uint64_t bytes = 0;
+    with_ln_bwd(d, [&](auto, const LnPlan&, long long grid, size_t) {
+        bytes = (uint64_t)grid * 2 * d->C * sizeof(float);
+        return (int)M2D_OK;
+    });
+    return bytes;
 }
 
 extern "C" int m2d_ln_fwd(const m2d_ln_desc* d, void* stream) {
@@ -446,14 +538,15 @@ extern "C" int m2d_ln_fwd(const m2d_ln_desc* d, void* stream) {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const LnPlan pl = plan_ln(d, false);
     if (pl.lanes < 0) {
-        const unsigned grid = (unsigned)std::min<long long>(d->N, 4ll * sm_count());
+        const unsigned grid = (unsigned)ln_grid(d, pl, 4);
         if (d->dtype == M2D_F32) ln_long_fwd_kernel<float><<<grid, kLongThreads, 0, st>>>(a);
         else ln_long_fwd_kernel<__nv_bfloat16><<<grid, kLongThreads, 0, st>>>(a);
         return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
     }
-    return for_ln(d, pl, [&](auto elem, auto vec, auto lanes, auto nv) {
-        ln_fwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value><<<(unsigned)((d->N + pl.rows() - 1) / pl.rows()), pl.threads, 0, st>>>(a);
-        return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
+    return for_ln(d, pl, d->residual != nullptr, [&](auto elem, auto vec, auto lanes, auto nv, auto res) {
+        auto kern = ln_fwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(res)::value>;
+        kern<<<(unsigned)ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, 0)), pl.threads, 0, st>>>(a);
+        return cudaGetLastError() == cudaSuccess ? (int)M2D_OK : (int)M2D_ERR_LAUNCH;
     });
 }
 
@@ -463,26 +556,15 @@ extern "C" int m2d_ln_bwd(const m2d_ln_desc* d, void* stream) {
     if (!d->x || !d->stats || !d->d_y || !d->d_x) return M2D_ERR_NULL;
     LnArgs a = ln_args(d);
     const bool params = d->d_weight || d->d_bias;
-    if (params && (!d->workspace || d->workspace_bytes < m2d_ln_bwd_workspace(d) || (reinterpret_cast<uintptr_t>(d->workspace) & 255))) return M2D_ERR_WORKSPACE;
-    a.partial = params ? static_cast<float*>(d->workspace) : nullptr;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const LnPlan pl = plan_ln(d, true);
-    a.parts = (int)ln_parts(d, pl);
-    int done = M2D_OK;
-    if (pl.lanes < 0) {
-        if (d->dtype == M2D_F32) ln_long_bwd_kernel<float><<<a.parts, kLongThreads, 0, st>>>(a);
-        else ln_long_bwd_kernel<__nv_bfloat16><<<a.parts, kLongThreads, 0, st>>>(a);
-    } else {
-        done = for_ln(d, pl, [&](auto elem, auto vec, auto lanes, auto nv) {
-            constexpr int V = decltype(vec)::value, R = decltype(lanes)::value, NV = decltype(nv)::value;
-            const size_t smem = R && params ? (size_t)kLnThreads / 32 * 2 * R * NV * V * sizeof(float) : 0;
-            if (!allow_smem(reinterpret_cast<const void*>(ln_bwd_kernel<decltype(elem), V, R, NV>), smem)) return (int)M2D_ERR_LAUNCH;
-            ln_bwd_kernel<decltype(elem), V, R, NV><<<a.parts, pl.threads, smem, st>>>(a);
-            return (int)M2D_OK;
-        });
-    }
-    if (done != M2D_OK || cudaGetLastError() != cudaSuccess) return M2D_ERR_LAUNCH;
-    if (!params) return M2D_OK;
+    const int done = with_ln_bwd(d, [&](auto kern, const LnPlan& pl, long long grid, size_t smem) {
+        if (params && (!d->workspace || d->workspace_bytes < (uint64_t)grid * 2 * d->C * sizeof(float) || (reinterpret_cast<uintptr_t>(d->workspace) & 255))) return (int)M2D_ERR_WORKSPACE;
+        a.partial = params ? static_cast<float*>(d->workspace) : nullptr;
+        a.parts = (int)grid;
+        kern<<<a.parts, pl.threads, smem, st>>>(a);
+        return cudaGetLastError() == cudaSuccess ? (int)M2D_OK : (int)M2D_ERR_LAUNCH;
+    });
+    if (done != M2D_OK || !params) return done;
     const dim3 grid((d->C + 31) / 32, 2);
     const bool f32 = d->params_f32 || d->dtype == M2D_F32;
     if (!(f32 ? launch_following(ln_params_kernel<float>, grid, dim3(1024), 0, st, a) : launch_following(ln_params_kernel<__nv_bfloat16>, grid, dim3(1024), 0, st, a))) return M2D_ERR_LAUNCH;

@@ -141,7 +141,7 @@ def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
         y in x's type, or ``(y, s)`` where there is a residual: s goes on to the next layer.
     Differentiable in x, weight, bias and residual, once (``create_graph`` raises); x and residual get the same gradient, one
     tensor.  Rows may lie apart (a slice of a wider tensor); other strides are copied.  Rows that are not whole 16-byte
-    pieces are read value by value; rows of more than 16384 values (8192 of such, and in the backward pass) are read three times.
+    pieces are read value by value; rows of more than 8192 values are read three times.
     """
     y, total = _lib.entry().layer_norm(x, weight, bias, residual, eps)
     return y if residual is None else (y, total)
