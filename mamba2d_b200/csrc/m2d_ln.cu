@@ -115,7 +115,8 @@ __device__ __forceinline__ void row_sum(float (&v)[K], int& slot) {
         slot ^= 1;
     }
 }
-constexpr int kLnThreads = 256;        // of a CTA whose rows are held by parts of warps
+constexpr int kLnThreads = 128;        // of a CTA whose rows are held by parts of warps
+constexpr size_t kLnStatic = 1024;     // row_sum's shared memory counts towards what a kernel has without asking
 
 // A thread's share of the rows: columns (i span + l) V ..., i < NV, of every `step`-th row from `row` on, as many rows at a time as `step` says
 // all CTAs have.  The loads of its next row are under way while it works on one, and the parameters stay in registers.
@@ -136,6 +137,48 @@ struct Share {
     __device__ __forceinline__ bool more(long long N, long long at) const { return at - (R ? threadIdx.x / lanes : 0) < N; }
 };
 
+// Rows on their way: whole pieces through shared memory, two or three rows ahead, each thread its own pieces (nobody else looks at
+// them); single values in registers, one row ahead.  What is wanted are 40 KB and more of an SM under way, which registers have no room for.
+template <typename T, int V, int R, int NV, int TENSORS>
+struct Rows {
+    using Raw = typename Lane<T, V>::Raw;
+    static constexpr bool ring = V > 1;
+    static constexpr int room = 224 * 1024 / (TENSORS * NV * 16 * (R ? kLnThreads : 512)), ahead = !ring ? 1 : room < 3 ? room : 3;
+    static constexpr size_t bytes(int threads) { return ring ? (size_t)ahead * TENSORS * NV * threads * 16 : 0; }
+    Raw reg[ring ? 1 : TENSORS][ring ? 1 : NV];
+    unsigned base, slot;
+    __device__ __forceinline__ Rows(void* smem) { base = smem_u32(smem) + threadIdx.x * 16; slot = 0; }
+    __device__ __forceinline__ unsigned place(int t, int i) const { return base + ((slot * TENSORS + t) * NV + i) * blockDim.x * 16; }
+    // piece i of tensor t, if `on`; then done() once a row
+    __device__ __forceinline__ void fetch(int t, int i, const T* p, bool on) {
+        if constexpr (ring) {
+            cp_async16_if(on, place(t, i), p);
+        } else {
+            reg[t][i] = Raw{};
+            if (on) reg[t][i] = __ldcs(reinterpret_cast<const Raw*>(p));
+        }
+    }
+    __device__ __forceinline__ void done() {
+        if constexpr (ring) {
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            slot = slot + 1 == ahead ? 0 : slot + 1;
+        }
+    }
+    // waits for the oldest row on its way; its slot is the next to be filled
+    __device__ __forceinline__ void arrived() {
+        if constexpr (ring) asm volatile("cp.async.wait_group %0;" ::"n"(ahead - 1) : "memory");
+    }
+    __device__ __forceinline__ Raw take(int t, int i) const {
+        if constexpr (ring) {
+            uint4 r;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(place(t, i)) : "memory");
+            return *reinterpret_cast<const Raw*>(&r);
+        } else {
+            return reg[t][i];
+        }
+    }
+};
+
 template <typename T, int V, int R, int NV, bool RES>
 __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_fwd_kernel(const LnArgs p) {
     using P = Lane<T, V>;
@@ -149,43 +192,49 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_fwd_kernel(const LnAr
             parameter<T, V>(p.w, p.params_f32, at.column(i), 1.f, w[i]);
             parameter<T, V>(p.b, p.params_f32, at.column(i), 0.f, b[i]);
         }
-    Raw rx[NV], rr[RES ? NV : 1];
-    float lead, lead_r = 0.f;               // the row's first values
+    extern __shared__ __align__(16) char smem[];
+    Rows<T, V, R, NV, RES ? 2 : 1> rows(smem);
+    T lead, lead_r;                         // the next row's first values (as they are: nothing waits for them here)
     auto load = [&](long long row) {
-        const T* const x = static_cast<const T*>(p.x) + (row < p.N ? row : 0) * p.xp;
+        const bool on = row < p.N;
+        const T* const x = static_cast<const T*>(p.x) + (on ? row : 0) * p.xp;
+        const T* const r = RES ? static_cast<const T*>(p.r) + (on ? row : 0) * p.rp : nullptr;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (at.column(i) < p.C) rx[i] = __ldcs(reinterpret_cast<const Raw*>(x + at.column(i)));
-        lead = value_of(x);
-        if constexpr (RES) {
-            const T* const r = static_cast<const T*>(p.r) + (row < p.N ? row : 0) * p.rp;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (at.column(i) < p.C) rr[i] = __ldcs(reinterpret_cast<const Raw*>(r + at.column(i)));
-            lead_r = value_of(r);
+        for (int i = 0; i < NV; ++i) {
+            rows.fetch(0, i, x + at.column(i), on && at.column(i) < p.C);
+            if constexpr (RES) rows.fetch(1, i, r + at.column(i), on && at.column(i) < p.C);
         }
+        rows.done();
+    };
+    auto look = [&](long long row) {
+        lead = static_cast<const T*>(p.x)[(row < p.N ? row : 0) * p.xp];
+        if constexpr (RES) lead_r = static_cast<const T*>(p.r)[(row < p.N ? row : 0) * p.rp];
     };
     int slot = 0;
     long long row = at.row;
-    if (at.more(p.N, row)) load(row);
+#pragma unroll
+    for (int k = 0; k < rows.ahead; ++k) load(row + k * at.step);
+    look(row);
     const float per = 1.f / (float)p.C;
     for (; at.more(p.N, row); row += at.step) {
         N v[NV][P::n];
+        rows.arrived();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            P::get(rx[i], v[i]);
+            P::get(rows.take(0, i), v[i]);
             if constexpr (RES) {
                 N r[P::n];
-                P::get(rr[i], r);
+                P::get(rows.take(1, i), r);
 #pragma unroll
                 for (int k = 0; k < P::n; ++k) v[i][k] = add_(v[i][k], r[k]);
-                rx[i] = P::put(v[i]);
-                if (row < p.N && at.column(i) < p.C) *reinterpret_cast<Raw*>(static_cast<T*>(p.s) + row * p.C + at.column(i)) = rx[i];
-                P::get(rx[i], v[i]);         // (rounded)
+                const Raw sum = P::put(v[i]);
+                if (row < p.N && at.column(i) < p.C) *reinterpret_cast<Raw*>(static_cast<T*>(p.s) + row * p.C + at.column(i)) = sum;
+                P::get(sum, v[i]);           // (rounded)
             }
         }
-        const float first = RES ? sum_as<T>(lead, lead_r) : lead;
-        if (at.more(p.N, row + at.step)) load(row + at.step);
+        const float first = RES ? sum_as<T>(value_of(&lead), value_of(&lead_r)) : value_of(&lead);
+        load(row + rows.ahead * at.step);
+        look(row + at.step);
         N acc = N::all(0.f);
         const N less = N::all(-first);
 #pragma unroll
@@ -227,7 +276,6 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
     using P = Lane<T, V>;
     using Raw = typename P::Raw;
     using N = typename P::N;
-    extern __shared__ float sums[];                // where parts of warps hold rows: [warps][2][columns of R lanes]
     let_follow();
     const Share<V, R> at;
     N w[NV][P::n], dw[NV][P::n], db[NV][P::n];
@@ -237,41 +285,47 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
         for (int k = 0; k < P::n; ++k) w[i][k] = dw[i][k] = db[i][k] = N::all(0.f);
         if (at.column(i) < p.C) parameter<T, V>(p.w, p.params_f32, at.column(i), 1.f, w[i]);
     }
-    Raw rx[NV], rd[NV], rs[DS ? NV : 1];
+    extern __shared__ __align__(16) char smem[];   // the rows on their way; at the end sums, where parts of warps hold rows: [warps][2][columns of R lanes]
+    Rows<T, V, R, NV, DS ? 3 : 2> rows(smem);
     float2 st;
     auto load = [&](long long row) {
         const bool on = row < p.N;
         const T *const x = static_cast<const T*>(p.x) + (on ? row : 0) * p.xp, *const dy = static_cast<const T*>(p.dy) + (on ? row : 0) * p.dyp;
+        const T* const ds = DS ? static_cast<const T*>(p.ds) + (on ? row : 0) * p.dsp : nullptr;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            rx[i] = rd[i] = Raw{};
-            if (on && at.column(i) < p.C) {
-                rx[i] = __ldcs(reinterpret_cast<const Raw*>(x + at.column(i)));
-                rd[i] = __ldcs(reinterpret_cast<const Raw*>(dy + at.column(i)));
-                if constexpr (DS) rs[i] = __ldcs(reinterpret_cast<const Raw*>(static_cast<const T*>(p.ds) + row * p.dsp + at.column(i)));
-            }
+            const bool here = on && at.column(i) < p.C;
+            rows.fetch(0, i, x + at.column(i), here);
+            rows.fetch(1, i, dy + at.column(i), here);
+            if constexpr (DS) rows.fetch(2, i, ds + at.column(i), here);
         }
-        st = on ? p.stats[row] : make_float2(0.f, 0.f);
+        rows.done();
     };
+    auto look = [&](long long row) { st = row < p.N ? p.stats[row] : make_float2(0.f, 0.f); };
     int slot = 0;
     long long row = at.row;
-    if (at.more(p.N, row)) load(row);
+#pragma unroll
+    for (int k = 0; k < rows.ahead; ++k) load(row + k * at.step);
+    look(row);
     const float per = 1.f / (float)p.C;
     for (; at.more(p.N, row); row += at.step) {
         N h[NV][P::n], dh[NV][P::n], s0 = N::all(0.f), s1 = N::all(0.f);
         Raw keep[DS ? NV : 1];
         const N off = N::all(-st.x), scale = N::all(st.y);
+        rows.arrived();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            P::get(rx[i], h[i]);
-            P::get(rd[i], dh[i]);
-            if constexpr (DS) keep[i] = rs[i];
+            P::get(rows.take(0, i), h[i]);
+            P::get(rows.take(1, i), dh[i]);
+            if constexpr (DS) keep[i] = rows.take(2, i);
         }
         const float rstd = st.y;
-        if (at.more(p.N, row + at.step)) load(row + at.step);
+        load(row + rows.ahead * at.step);
+        look(row + at.step);
+        if (row < p.N)
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (at.column(i) < p.C)                // (a row beyond the last: dy is zero and so is h)
+            if (at.column(i) < p.C)
 #pragma unroll
                 for (int k = 0; k < P::n; ++k) {
                     h[i][k] = mul_(add_(h[i][k], off), scale);
@@ -298,6 +352,7 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
                 *reinterpret_cast<Raw*>(static_cast<T*>(p.dx) + row * p.C + at.column(i)) = P::put(g);
             }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!p.partial) return;
     float* const out = p.partial + (long long)blockIdx.x * 2 * p.C;
     constexpr int W = V / P::n;
@@ -313,6 +368,8 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
         // lanes of one warp that have the same columns, then the warps in turn
         constexpr int cols = R * NV * V;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        float* const sums = reinterpret_cast<float*>(smem);
+        __syncthreads();                           // (no row is on its way any more, for any thread)
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -412,8 +469,17 @@ __global__ void __launch_bounds__(1024) ln_params_kernel(const LnArgs p) {
     follow_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.f;
-    if (c < p.C)
-        for (int i = warp; i < p.parts; i += 32) v += p.partial[((long long)i * 2 + blockIdx.y) * p.C + c];
+    if (c < p.C) {
+        constexpr int U = 10;                      // loads under way at once: some 300 sums in one go
+        const float* const q = p.partial + (long long)blockIdx.y * p.C + c;
+        for (int i = warp; i < p.parts; i += 32 * U) {
+            float t[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) t[k] = i + 32 * k < p.parts ? q[(long long)(i + 32 * k) * 2 * p.C] : 0.f;
+#pragma unroll
+            for (int k = 0; k < U; ++k) v += t[k];
+        }
+    }
     part[warp][lane] = v;
     __syncthreads();
     v = part[lane][warp];
@@ -498,7 +564,6 @@ static LnArgs ln_args(const m2d_ln_desc* d) {
 }
 // CTAs of a launch: what the SMs hold at once.
 static long long ln_grid(const m2d_ln_desc* d, const LnPlan& pl, int per_sm) { return std::min<long long>((d->N + pl.rows() - 1) / pl.rows(), (long long)std::max(1, per_sm) * sm_count()); }
-static size_t ln_bwd_smem(const LnPlan& pl, bool params) { return pl.lanes > 0 && params ? (size_t)kLnThreads / 32 * 2 * pl.lanes * pl.nv * pl.vec * sizeof(float) : 0; }
 // Calls fn(kernel, CTAs) of the backward pass.
 template <typename F>
 static int with_ln_bwd(const m2d_ln_desc* d, F fn) {
@@ -510,8 +575,10 @@ static int with_ln_bwd(const m2d_ln_desc* d, F fn) {
     }
     return for_ln(d, pl, d->d_sum != nullptr, [&](auto elem, auto vec, auto lanes, auto nv, auto ds) {
         auto kern = ln_bwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(ds)::value>;
-        const size_t smem = ln_bwd_smem(pl, params);
-        if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return (int)M2D_ERR_LAUNCH;
+        constexpr int V = decltype(vec)::value, R = decltype(lanes)::value, NV = decltype(nv)::value;
+        const size_t rows = Rows<decltype(elem), V, R, NV, decltype(ds)::value ? 3 : 2>::bytes(pl.threads), last = R && params ? (size_t)kLnThreads / 32 * 2 * R * NV * V * sizeof(float) : 0;
+        const size_t smem = std::max(rows, last);
+        if (!allow_smem(reinterpret_cast<const void*>(kern), smem + kLnStatic)) return (int)M2D_ERR_LAUNCH;
         return fn(kern, pl, ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, smem)), smem);
     });
 }
@@ -545,7 +612,9 @@ extern "C" int m2d_ln_fwd(const m2d_ln_desc* d, void* stream) {
     }
     return for_ln(d, pl, d->residual != nullptr, [&](auto elem, auto vec, auto lanes, auto nv, auto res) {
         auto kern = ln_fwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(res)::value>;
-        kern<<<(unsigned)ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, 0)), pl.threads, 0, st>>>(a);
+        const size_t smem = Rows<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(res)::value ? 2 : 1>::bytes(pl.threads);
+        if (!allow_smem(reinterpret_cast<const void*>(kern), smem + kLnStatic)) return (int)M2D_ERR_LAUNCH;
+        kern<<<(unsigned)ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, smem)), pl.threads, smem, st>>>(a);
         return cudaGetLastError() == cudaSuccess ? (int)M2D_OK : (int)M2D_ERR_LAUNCH;
     });
 }
