@@ -227,9 +227,12 @@ typedef struct m2d_distill_desc {
     const float *d_loss;           /* d_loss[n * d_loss_row]                                        [bwd] */
     int64_t d_loss_row;
     void *d_logits;                /* (N,V) dense */
+    void *workspace;               /* scratch of fwd, 256-byte aligned */
+    uint64_t workspace_bytes;
 } m2d_distill_desc;
 
 uint64_t m2d_distill_stats(const m2d_distill_desc *desc);
+uint64_t m2d_distill_fwd_workspace(const m2d_distill_desc *desc);     /* reads N, V and dtype */
 int m2d_distill_fwd(const m2d_distill_desc *desc, void *stream);
 int m2d_distill_bwd(const m2d_distill_desc *desc, void *stream);
 

@@ -37,7 +37,7 @@ EXPORTS = ("m2d_abi_version", "m2d_strerror", "m2d_scan_fwd_workspace", "m2d_sca
            "m2d_clip_workspace", "m2d_clip_grad_norm",
            "m2d_recur_marks", "m2d_recur_fwd", "m2d_recur_bwd", "m2d_recur_step",
            "m2d_ln_bwd_workspace", "m2d_ln_fwd", "m2d_ln_bwd",
-           "m2d_distill_stats", "m2d_distill_fwd", "m2d_distill_bwd")
+           "m2d_distill_stats", "m2d_distill_fwd_workspace", "m2d_distill_fwd", "m2d_distill_bwd")
 ATTN_MAX_DIM = 256                   # M2D_ATTN_MAX_DIM in include/m2d_seq.h
 PROJ_MAX_E, PROJ_MAX_R = 640, 64     # M2D_PROJ_MAX_E / M2D_PROJ_MAX_R in include/m2d_proj.h
 

@@ -4,14 +4,13 @@
 //   loss = (1 - w) tau^2 sum_k p_k (log p_k - log q_{i_k}) + w (log sum_j exp(z_j) - z_label)
 //   dz_j = up ((1 - w) tau (q_j - sum_{k: i_k = j} p_k) + w (softmax(z)_j - [j = label]))
 //
-// One pass over a row with the running maximum and sums: by a warp where rows are short, by a CTA, or by a cluster of CTAs where there are few
-// rows.  The backward pass reads a row once more and writes its gradient; the few entries that the teacher or the label touch are written again
-// behind it by the same CTA, the first of entries with one index for all of them, so that every value is rounded once and does not depend on
+// One pass over the rows with running maxima and sums: by a warp each where rows are short; else all rows are cut into pieces, every CTA takes as
+// many neighbouring ones as any other, whatever rows they belong to, and a second launch joins what they found.  The backward pass reads a row once more and writes its gradient; the few entries that the teacher or the label touch are written again
+// behind it, the first of entries with one index for all of them, so that every value is rounded once and does not depend on
 // any order.  Exponents are (z - max) c with c = log2(e) / tau: exact where all values are equal, also at the type's lowest.  What is left of a row
 // (its sums' logarithms, the teacher's entries) is summed in 64 bits: a loss is a small difference of large logarithms.
-#include <cooperative_groups.h>
-
 #include "follow.cuh"
+#include "packed.cuh"
 #include "plan.cuh"
 #include "m2d_seq.h"
 
@@ -27,8 +26,11 @@ struct DistillArgs {
     long long N;
     int V, K, t_f32, index64, labels64, same_phase;
     float tau, w, c, c1;               // log2(e) / tau, log2(e)
-    int parts;
+    float4* found;                     // forward by pieces: largest value and sums of a CTA's share of a row, at [row + CTA]
+    int pieces, ctas;                  // pieces of a row
 };
+// Exponentials of a value: at one temperature, at tau and at 1, or at 2 and at 1, whose second is the first one's square.
+enum { kOne = 0, kTwo = 1, kSquare = 2 };
 // Of a row, for the backward pass: max, 1 / sum at tau, 1 / sum at 1, the teacher's largest logit, 1 / the teacher's sum (0: no entries).
 constexpr int kRowStats = 8;
 constexpr int kRowCta = 256;           // threads of a CTA that works on one row
@@ -37,18 +39,32 @@ constexpr int kRowWarps = 4;           // rows of a CTA whose warps work on one 
 template <typename T> struct Vec16;    // 16 bytes
 template <> struct Vec16<float> {
     static constexpr int n = 4;
-    static __device__ __forceinline__ void get(const uint4& r, float* v) { v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w); }
-    static __device__ __forceinline__ uint4 put(const float* v) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
+    static __device__ __forceinline__ void get(const uint4& r, Num<2>* v) { v[0] = Num<2>::make(__uint_as_float(r.x), __uint_as_float(r.y)); v[1] = Num<2>::make(__uint_as_float(r.z), __uint_as_float(r.w)); }
+    static __device__ __forceinline__ uint4 put(const Num<2>* v) {
+        return make_uint4(__float_as_uint(v[0].get(0)), __float_as_uint(v[0].get(1)), __float_as_uint(v[1].get(0)), __float_as_uint(v[1].get(1)));
+    }
+    static __device__ __forceinline__ float most(const uint4& r, float m) {
+        return fmaxf(fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))), m);
+    }
 };
 template <> struct Vec16<__nv_bfloat16> {
     static constexpr int n = 8;
-    static __device__ __forceinline__ void get(const uint4& r, float* v) {
+    static __device__ __forceinline__ void get(const uint4& r, Num<2>* v) {
         const unsigned u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+        for (int i = 0; i < 4; ++i) v[i] = Num<2>::make(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
     }
-    static __device__ __forceinline__ uint4 put(const float* v) {
-        return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    static __device__ __forceinline__ uint4 put(const Num<2>* v) {
+        return make_uint4(pack_bf16x2(v[0].get(0), v[0].get(1)), pack_bf16x2(v[1].get(0), v[1].get(1)), pack_bf16x2(v[2].get(0), v[2].get(1)), pack_bf16x2(v[3].get(0), v[3].get(1)));
+    }
+    static __device__ __forceinline__ unsigned two(unsigned a, unsigned b) {
+        unsigned r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float most(const uint4& r, float m) {
+        const unsigned t = two(two(r.x, r.y), two(r.z, r.w));
+        return fmaxf(fmaxf(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u)), m);
     }
 };
 __device__ __forceinline__ float number(const float* p) { return *p; }
@@ -65,37 +81,51 @@ struct RowCut {
     }
 };
 
-// Largest value so far, and sums of exp2((z - max) c) at tau and (TWO) at 1.
-template <bool TWO>
+// Largest value so far, and sums of exp2((z - max) c) at tau and at 1.
+template <int MODE>
 struct Running {
-    float m = -3.402823466e38f, s = 0.f, s1 = 0.f;
+    float m = -3.402823466e38f;
+    Num<2> s = Num<2>::all(0.f), s1 = Num<2>::all(0.f);
     __device__ __forceinline__ void raise(float to, float c, float c1) {
-        const float n = fmaxf(m, to);
-        s *= ex2((m - n) * c);
-        if constexpr (TWO) s1 *= ex2((m - n) * c1);
+        const float n = fmaxf(m, to), f = ex2((m - n) * c);
+        s = mul_(s, Num<2>::all(f));
+        if constexpr (MODE == kTwo) s1 = mul_(s1, Num<2>::all(ex2((m - n) * c1)));
+        if constexpr (MODE == kSquare) s1 = mul_(s1, Num<2>::all(f * f));
         m = n;
     }
-    __device__ __forceinline__ void add(float z, float c, float c1) {
-        const float d = z - m;
-        s += ex2(d * c);
-        if constexpr (TWO) s1 += ex2(d * c1);
+    __device__ __forceinline__ void add(Num<2> z, float c, float c1) {
+        const Num<2> d = add_(z, Num<2>::all(-m)), x = mul_(d, Num<2>::all(c)), e = Num<2>::make(ex2(x.get(0)), ex2(x.get(1)));
+        s = add_(s, e);
+        if constexpr (MODE == kTwo) {
+            const Num<2> x1 = mul_(d, Num<2>::all(c1));
+            s1 = add_(s1, Num<2>::make(ex2(x1.get(0)), ex2(x1.get(1))));
+        }
+        if constexpr (MODE == kSquare) s1 = fma_(e, e, s1);
     }
-    __device__ __forceinline__ void join(float om, float os, float os1, float c, float c1) {
-        raise(om, c, c1);
-        s = fmaf(os, ex2((om - m) * c), s);
-        if constexpr (TWO) s1 = fmaf(os1, ex2((om - m) * c1), s1);
+    __device__ __forceinline__ void one(float z, float c, float c1) {
+        raise(z, c, c1);
+        add(Num<2>::make(z, -__int_as_float(0x7f800000)), c, c1);
     }
+    __device__ __forceinline__ float4 found() const { return make_float4(m, s.get(0) + s.get(1), s1.get(0) + s1.get(1), 0.f); }
 };
-template <bool TWO>
-__device__ __forceinline__ void join_lanes(Running<TWO>& r, float c, float c1, int lanes = 32) {
-    for (int k = lanes / 2; k; k >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, r.m, k), s = __shfl_xor_sync(0xffffffffu, r.s, k), s1 = TWO ? __shfl_xor_sync(0xffffffffu, r.s1, k) : 0.f;
-        // (both sides do the same operations: the lanes agree to the last bit)
-        const float n = fmaxf(r.m, m), f = ex2((r.m - n) * c), g = ex2((m - n) * c);
-        r.s = __fadd_rn(__fmul_rn(r.s, f), __fmul_rn(s, g));
-        if constexpr (TWO) r.s1 = __fadd_rn(__fmul_rn(r.s1, ex2((r.m - n) * c1)), __fmul_rn(s1, ex2((m - n) * c1)));
-        r.m = n;
+// Two shares of a row as one; the same on both sides of an exchange, to the last bit.
+template <int MODE>
+__device__ __forceinline__ float4 joined(const float4& a, const float4& b, float c, float c1) {
+    const float n = fmaxf(a.x, b.x), f = ex2((a.x - n) * c), g = ex2((b.x - n) * c);
+    float4 r = make_float4(n, __fadd_rn(__fmul_rn(a.y, f), __fmul_rn(b.y, g)), 0.f, 0.f);
+    if constexpr (MODE != kOne) {
+        const float f1 = MODE == kSquare ? f * f : ex2((a.x - n) * c1), g1 = MODE == kSquare ? g * g : ex2((b.x - n) * c1);
+        r.z = __fadd_rn(__fmul_rn(a.z, f1), __fmul_rn(b.z, g1));
     }
+    return r;
+}
+template <int MODE>
+__device__ __forceinline__ float4 join_lanes(float4 r, float c, float c1, int lanes = 32) {
+    for (int k = lanes / 2; k; k >>= 1) {
+        const float4 o = make_float4(__shfl_xor_sync(0xffffffffu, r.x, k), __shfl_xor_sync(0xffffffffu, r.y, k), MODE != kOne ? __shfl_xor_sync(0xffffffffu, r.z, k) : 0.f, 0.f);
+        r = joined<MODE>(r, o, c, c1);
+    }
+    return r;
 }
 
 __device__ __forceinline__ long long whole_at(const void* p, int is64, long long i) { return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i]; }
@@ -117,178 +147,208 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// The loss of a row from its sums, by a warp.
-template <typename T, bool TWO>
-__device__ __forceinline__ void finish_row(const DistillArgs& p, long long row, const T* z, const Running<TWO>& r) {
+// What the teacher's entries give, by a warp and without the row's own sums: the largest logits, its and the student's, among them, the sum of
+// 2^(t - top) and that of 2^(t - top) (log2 p + log2 of the sum - (z - high) c).
+struct Taught {
+    float top, high;
+    double sum, dot;
+    bool any;
+};
+template <typename T>
+__device__ __forceinline__ Taught teach(const DistillArgs& p, long long row, const T* z) {
     const int lane = threadIdx.x & 31;
-    const double c = p.c, m = r.m;
-    float top = -__int_as_float(0x7f800000);
-    bool any = false;
-    for (int k = lane; k < p.K; k += 32)
-        if (entry_at(p, row, k) >= 0) {
-            const float t = teacher_at(p, row, k);
-            any = any || t != -__int_as_float(0x7f800000);        // (a NaN is there too)
-            top = fmaxf(top, t);
-        }
+    const float low = -__int_as_float(0x7f800000);
+    Taught r{low, low, 0.0, 0.0, false};
+    for (int k = lane; k < p.K; k += 32) {
+        const int i = entry_at(p, row, k);
+        if (i < 0) continue;
+        const float t = teacher_at(p, row, k);
+        r.any = r.any || t != low;                     // (a NaN is there too)
+        r.top = fmaxf(r.top, t);
+        r.high = fmaxf(r.high, number(z + i));
+    }
 #pragma unroll
-    for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    any = __any_sync(0xffffffffu, any) && p.w < 1.f;
-    double loss = 0.0;
-    float part = 0.f;
-    if (any) {
-        double sum = 0.0, dot = 0.0;                  // of 2^(t - top) and of that times (log2 p + log2 of its sum - (z - max) c)
+    for (int k = 16; k; k >>= 1) {
+        r.top = fmaxf(r.top, __shfl_xor_sync(0xffffffffu, r.top, k));
+        r.high = fmaxf(r.high, __shfl_xor_sync(0xffffffffu, r.high, k));
+    }
+    if (r.high == low) r.high = 0.f;
+    r.any = __any_sync(0xffffffffu, r.any) && p.w < 1.f;
+    if (r.any) {
         for (int k = lane; k < p.K; k += 32) {
             const int i = entry_at(p, row, k);
             if (i < 0) continue;
-            const double a = ((double)teacher_at(p, row, k) - (double)top) * c, e = exp2(a);
-            sum += e;
-            if (e != 0.0) dot += e * (a - ((double)number(z + i) - m) * c);
+            const double a = ((double)teacher_at(p, row, k) - (double)r.top) * (double)p.c, e = exp2(a);
+            r.sum += e;
+            if (e != 0.0) r.dot += e * (a - ((double)number(z + i) - (double)r.high) * (double)p.c);
         }
-        sum = warp_sum(sum);
-        dot = warp_sum(dot);
-        loss = (1.0 - (double)p.w) * (double)p.tau * (double)p.tau * 0.6931471805599453 * (dot / sum - log2(sum) + log2((double)r.s));
-        part = (float)(1.0 / sum);
+        r.sum = warp_sum(r.sum);
+        r.dot = warp_sum(r.dot);
     }
-    const int label = label_of(p, row);
-    if (label >= 0) loss += (double)p.w * (log((double)(TWO ? r.s1 : r.s)) - ((double)number(z + label) - m));
-    if (lane == 0) {
-        p.loss[row] = (float)loss;
-        if (p.stats) {
-            float* const s = p.stats + row * kRowStats;
-            s[0] = r.m;
-            s[1] = 1.f / r.s;
-            s[2] = 1.f / (TWO ? r.s1 : r.s);
-            s[3] = top;
-            s[4] = part;
-        }
+    return r;
+}
+// The loss of a row from its sums, by a warp.
+template <int MODE>
+__device__ __forceinline__ void finish_row(const DistillArgs& p, long long row, const Taught& t, int label, float at_label, const float4& r) {
+    const float at_one = MODE != kOne ? r.z : r.y;
+    if ((threadIdx.x & 31) != 0) return;
+    double loss = 0.0;
+    if (t.any)       // (dot is about `high`: exact where everything is at the type's lowest)
+        loss = (1.0 - (double)p.w) * (double)p.tau * (double)p.tau * 0.6931471805599453 * (t.dot / t.sum + ((double)r.x - (double)t.high) * (double)p.c - log2(t.sum) + log2((double)r.y));
+    if (label >= 0) loss += (double)p.w * (log((double)at_one) - ((double)at_label - (double)r.x));
+    p.loss[row] = (float)loss;
+    if (p.stats) {
+        float* const s = p.stats + row * kRowStats;
+        s[0] = r.x;
+        s[1] = 1.f / r.y;
+        s[2] = 1.f / at_one;
+        s[3] = t.top;
+        s[4] = t.any ? (float)(1.0 / t.sum) : 0.f;
     }
 }
 
-// Every step-th piece of a row from piece `first` on, and its head and tail where `ends`.
-template <typename T, bool TWO>
-__device__ __forceinline__ void read_row(const T* z, int V, int first, int step, bool ends, float c, float c1, Running<TWO>& r) {
+// 16-byte pieces first, first + step, ... below `end` of a row's body.
+template <typename T, int MODE>
+__device__ __forceinline__ void read_pieces(const uint4* body, int first, int step, int end, float c, float c1, Running<MODE>& r) {
     using W = Vec16<T>;
-    const RowCut<T> cut(z, V);
-    const uint4* const body = reinterpret_cast<const uint4*>(z + cut.head);
     constexpr int U = 4;
     int i = first;
-    for (; i < cut.pieces - (U - 1) * step; i += U * step) {
+    for (; i < end - (U - 1) * step; i += U * step) {
         uint4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) raw[u] = __ldcs(body + i + u * step);
         float top = r.m;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float v[W::n];
-            W::get(raw[u], v);
-#pragma unroll
-            for (int k = 0; k < W::n; ++k) top = fmaxf(top, v[k]);
-        }
+        for (int u = 0; u < U; ++u) top = W::most(raw[u], top);
         r.raise(top, c, c1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            float v[W::n];
+            Num<2> v[W::n / 2];
             W::get(raw[u], v);
 #pragma unroll
-            for (int k = 0; k < W::n; ++k) r.add(v[k], c, c1);
+            for (int k = 0; k < W::n / 2; ++k) r.add(v[k], c, c1);
         }
     }
-    for (; i < cut.pieces; i += step) {
-        float v[W::n], top = r.m;
-        W::get(__ldcs(body + i), v);
+    for (; i < end; i += step) {
+        const uint4 raw = __ldcs(body + i);
+        r.raise(W::most(raw, r.m), c, c1);
+        Num<2> v[W::n / 2];
+        W::get(raw, v);
 #pragma unroll
-        for (int k = 0; k < W::n; ++k) top = fmaxf(top, v[k]);
-        r.raise(top, c, c1);
-#pragma unroll
-        for (int k = 0; k < W::n; ++k) r.add(v[k], c, c1);
-    }
-    if (ends) {
-        if (first < cut.head) { const float v = number(z + first); r.raise(v, c, c1); r.add(v, c, c1); }
-        if (first < V - cut.tail) { const float v = number(z + cut.tail + first); r.raise(v, c, c1); r.add(v, c, c1); }
+        for (int k = 0; k < W::n / 2; ++k) r.add(v[k], c, c1);
     }
 }
+// A row's head and tail, by threads of which this is number `me`.
+template <typename T, int MODE>
+__device__ __forceinline__ void read_ends(const T* z, const RowCut<T>& cut, int V, int me, float c, float c1, Running<MODE>& r) {
+    if (me < cut.head) r.one(number(z + me), c, c1);
+    if (me < V - cut.tail) r.one(number(z + cut.tail + me), c, c1);
+}
 
-template <typename T, bool TWO>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kRowWarps * 32) distill_fwd_warp_kernel(const DistillArgs p) {
     const long long row = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
     if (row >= p.N) return;
+    const int lane = threadIdx.x & 31;
     const T* const z = static_cast<const T*>(p.z) + row * p.zp;
-    Running<TWO> r;
-    read_row<T, TWO>(z, p.V, threadIdx.x & 31, 32, true, p.c, p.c1, r);
-    join_lanes<TWO>(r, p.c, p.c1);
-    finish_row<T, TWO>(p, row, z, r);
+    const RowCut<T> cut(z, p.V);
+    Running<MODE> r;
+    read_pieces<T, MODE>(reinterpret_cast<const uint4*>(z + cut.head), lane, 32, cut.pieces, p.c, p.c1, r);
+    read_ends<T, MODE>(z, cut, p.V, lane, p.c, p.c1, r);
+    const float4 all = join_lanes<MODE>(r.found(), p.c, p.c1);
+    const Taught t = teach(p, row, z);
+    const int label = label_of(p, row);
+    finish_row<MODE>(p, row, t, label, label >= 0 ? number(z + label) : 0.f, all);
 }
 
-template <typename T, bool TWO>
+// All rows' pieces of kRowCta * UNIT times 16 bytes in order; CTA k of n has those from k total / n on.
+template <typename T, int MODE, int UNIT>
 __global__ void __launch_bounds__(kRowCta) distill_fwd_kernel(const DistillArgs p) {
-    namespace cg = cooperative_groups;
-    __shared__ float part[kRowCta / 32][3], whole[16][3];
-    cg::cluster_group cluster = cg::this_cluster();
-    if (p.parts > 1) cluster.barrier_arrive();           // (all have begun before one writes to another)
-    const long long row = blockIdx.x / p.parts;
-    const int rank = blockIdx.x % p.parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const T* const z = static_cast<const T*>(p.z) + row * p.zp;
-    Running<TWO> r;
-    read_row<T, TWO>(z, p.V, rank * kRowCta + threadIdx.x, p.parts * kRowCta, rank == 0, p.c, p.c1, r);
-    join_lanes<TWO>(r, p.c, p.c1);
-    if (lane == 0) { part[warp][0] = r.m; part[warp][1] = r.s; part[warp][2] = r.s1; }
-    __syncthreads();
-    if (warp == 0) {
-        constexpr int n = kRowCta / 32;
-        r.m = part[lane % n][0]; r.s = part[lane % n][1]; r.s1 = part[lane % n][2];
-        join_lanes<TWO>(r, p.c, p.c1, n);
-    }
-    if (p.parts > 1) {
-        cluster.barrier_wait();
-        if (threadIdx.x == 0) {
-            float* const to = cluster.map_shared_rank(&whole[0][0], 0) + rank * 3;
-            to[0] = r.m; to[1] = r.s; to[2] = r.s1;
+    __shared__ float4 part[2][kRowCta / 32];
+    let_follow();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long total = p.N * p.pieces, end = (blockIdx.x + 1ll) * total / p.ctas;
+    long long at = blockIdx.x * total / p.ctas;
+    for (int buf = 0; at < end; buf ^= 1) {
+        const long long row = at / p.pieces;
+        const int first = (int)(at - row * p.pieces), last = (int)min((long long)p.pieces, first + end - at);
+        const T* const z = static_cast<const T*>(p.z) + row * p.zp;
+        const RowCut<T> cut(z, p.V);
+        Running<MODE> r;
+        read_pieces<T, MODE>(reinterpret_cast<const uint4*>(z + cut.head), first * kRowCta * UNIT + threadIdx.x, kRowCta, min(cut.pieces, last * kRowCta * UNIT), p.c, p.c1, r);
+        if (first == 0) read_ends<T, MODE>(z, cut, p.V, threadIdx.x, p.c, p.c1, r);
+        const float4 f = join_lanes<MODE>(r.found(), p.c, p.c1);
+        if (lane == 0) part[buf][warp] = f;
+        __syncthreads();
+        if (warp == 0) {
+            const float4 whole = join_lanes<MODE>(part[buf][lane % (kRowCta / 32)], p.c, p.c1, kRowCta / 32);
+            if (lane == 0) p.found[row + blockIdx.x] = whole;
         }
-        cluster.sync();
-        if (rank != 0 || warp != 0) return;
-        r.m = whole[0][0]; r.s = whole[0][1]; r.s1 = whole[0][2];
-        for (int k = 1; k < p.parts; ++k) r.join(whole[k][0], whole[k][1], whole[k][2], p.c, p.c1);
+        at += last - first;
     }
-    if (warp == 0) finish_row<T, TWO>(p, row, z, r);
+}
+// Joins the shares of a row, a warp a row.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRowWarps * 32) distill_join_kernel(const DistillArgs p) {
+    const long long row = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    if (row >= p.N) return follow_wait();
+    const int lane = threadIdx.x & 31;
+    // (inputs: written before the launch that this one follows)
+    const T* const z = static_cast<const T*>(p.z) + row * p.zp;
+    const Taught t = teach(p, row, z);
+    const int label = label_of(p, row);
+    const float at_label = label >= 0 ? number(z + label) : 0.f;
+    follow_wait();
+    const long long total = p.N * p.pieces;
+    // the CTAs of its first piece and of its last: k total / n <= piece < (k + 1) total / n
+    const long long a = ((row * p.pieces + 1) * p.ctas - 1) / total, b = ((row + 1) * p.pieces * p.ctas - 1) / total;
+    float4 r = make_float4(-3.402823466e38f, 0.f, 0.f, 0.f);
+    for (long long k = a + lane; k <= b; k += 32) r = joined<MODE>(r, p.found[row + k], p.c, p.c1);
+    finish_row<MODE>(p, row, t, label, at_label, join_lanes<MODE>(r, p.c, p.c1));
 }
 
 // ---- backward -------------------------------------------------------------------------------------
 
 // dz_j of a row: a * 2^((z - m) c) + b * 2^((z - m) c1), less what the teacher and the label take.
-template <bool TWO>
+template <int MODE>
 struct Slope {
     float m, a, b, c, c1;
-    __device__ __forceinline__ float operator()(float z) const {
-        const float d = z - m, f = a * ex2(d * c);
-        if constexpr (TWO) return fmaf(b, ex2(d * c1), f);
-        return f;
+    __device__ __forceinline__ Num<2> operator()(Num<2> z) const {
+        const Num<2> d = add_(z, Num<2>::all(-m)), x = mul_(d, Num<2>::all(c)), e = Num<2>::make(ex2(x.get(0)), ex2(x.get(1)));
+        if constexpr (MODE == kOne) return mul_(e, Num<2>::all(a));
+        if constexpr (MODE == kSquare) return mul_(e, fma_(e, Num<2>::all(b), Num<2>::all(a)));
+        const Num<2> x1 = mul_(d, Num<2>::all(c1));
+        return fma_(Num<2>::make(ex2(x1.get(0)), ex2(x1.get(1))), Num<2>::all(b), mul_(e, Num<2>::all(a)));
     }
+    __device__ __forceinline__ float operator()(float z) const { return (*this)(Num<2>::all(z)).get(0); }
 };
 
-// A row's entries [lo, hi), by `threads` threads of which this is number `me`; sync() is theirs.  list: 2 K words of shared memory.
-template <typename T, bool TWO, typename Sync>
-__device__ __forceinline__ void write_row(const DistillArgs& p, long long row, int lo, int hi, int me, int threads, int* list, Sync sync) {
+// What a row's gradient is made of.
+template <int MODE>
+struct RowSlope {
+    Slope<MODE> f;
+    float teach, hard, top, share;         // of the teacher's and of the label's share of the loss; the teacher's largest logit and 1 / its sum
+    int label;                             // -1: none
+    bool has, zero;                        // whether there is a teacher; whether there is nothing to learn from
+    __device__ __forceinline__ RowSlope(const DistillArgs& p, long long row) {
+        const float* const st = p.stats + row * kRowStats;
+        const float up = p.up[row * p.upp];
+        teach = up * (1.f - p.w) * p.tau;
+        hard = up * p.w;
+        top = st[3];
+        share = st[4];
+        label = label_of(p, row);
+        has = share != 0.f;                // (NaN: there is one)
+        zero = !has && label < 0;
+        f = Slope<MODE>{st[0], has ? teach * st[1] : 0.f, label >= 0 ? hard * st[2] : 0.f, p.c, p.c1};
+        if (MODE == kOne) f.a += f.b;
+    }
+};
+// 16-byte pieces [b0, b1) of a row's body and, where `ends`, its head and tail, by `threads` threads of which this is number `me`: as if there were
+// neither list nor label.
+template <typename T, int MODE>
+__device__ __forceinline__ void write_dense(const DistillArgs& p, const RowSlope<MODE>& s, const T* z, T* out, const RowCut<T>& cut, int b0, int b1, bool ends, int me, int threads) {
     using W = Vec16<T>;
-    const T* const z = static_cast<const T*>(p.z) + row * p.zp;
-    T* const out = static_cast<T*>(p.dz) + row * p.V;
-    const float* const st = p.stats + row * kRowStats;
-    const float up = p.up[row * p.upp], teach = up * (1.f - p.w) * p.tau, iP = st[4];
-    const int label = label_of(p, row);
-    const bool has = iP != 0.f;                           // (NaN: there is one)
-    Slope<TWO> f{st[0], has ? teach * st[1] : 0.f, label >= 0 ? up * p.w * st[2] : 0.f, p.c, p.c1};
-    if (!TWO) f.a += f.b;
-    const bool zero = !has && label < 0;                  // nothing to learn from in this row
-    int* const at = list;
-    float* const share = reinterpret_cast<float*>(list + p.K);
-    if (has)
-        for (int k = me; k < p.K; k += threads) {
-            const int i = entry_at(p, row, k);
-            at[k] = i;
-            share[k] = i >= 0 ? ex2((teacher_at(p, row, k) - st[3]) * p.c) * iP : 0.f;
-        }
-    const RowCut<T> cut(z, p.V);
-    // (lo and hi lie on pieces' borders, or at the row's ends)
-    const int b0 = lo ? (lo - cut.head) / W::n : 0, b1 = hi < p.V ? (hi - cut.head) / W::n : cut.pieces;
     if (p.same_phase) {
         const uint4* const body = reinterpret_cast<const uint4*>(z + cut.head);
         uint4* const to = reinterpret_cast<uint4*>(out + cut.head);
@@ -296,60 +356,90 @@ __device__ __forceinline__ void write_row(const DistillArgs& p, long long row, i
         for (int i = b0 + me; i < b1; i += U * threads) {
             uint4 raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = i + u * threads < b1 ? __ldcs(body + i + u * threads) : make_uint4(0, 0, 0, 0);
+            for (int u = 0; u < U; ++u)
+                if (i + u * threads < b1) raw[u] = __ldcs(body + i + u * threads);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (i + u * threads >= b1) break;
-                float v[W::n];
+                Num<2> v[W::n / 2];
                 W::get(raw[u], v);
 #pragma unroll
-                for (int k = 0; k < W::n; ++k) v[k] = zero ? 0.f : f(v[k]);
-                to[i + u * threads] = W::put(v);
+                for (int k = 0; k < W::n / 2; ++k) v[k] = s.f(v[k]);
+                to[i + u * threads] = s.zero ? make_uint4(0, 0, 0, 0) : W::put(v);
             }
         }
     } else {
-        for (int i = cut.head + b0 * W::n + me; i < cut.head + b1 * W::n; i += threads) store1(out, i, zero ? 0.f : f(number(z + i)));
+        for (int i = cut.head + b0 * W::n + me; i < cut.head + b1 * W::n; i += threads) store1(out, i, s.zero ? 0.f : s.f(number(z + i)));
     }
-    if (lo == 0 && me < cut.head) store1(out, me, zero ? 0.f : f(number(z + me)));
-    if (hi == p.V && me < p.V - cut.tail) store1(out, cut.tail + me, zero ? 0.f : f(number(z + cut.tail + me)));
-    sync();
-    if (has)
-        for (int k = me; k < p.K; k += threads) {
-            const int i = at[k];
-            if (i < lo || i >= hi) continue;
+    if (!ends) return;
+    if (me < cut.head) store1(out, me, s.zero ? 0.f : s.f(number(z + me)));
+    if (me < p.V - cut.tail) store1(out, cut.tail + me, s.zero ? 0.f : s.f(number(z + cut.tail + me)));
+}
+// The entries that the teacher or the label touch, by a warp, of those that are mine(index): the first of entries with one index for all of them.
+// list: 2 K words of shared memory.
+template <typename T, int MODE, typename Mine>
+__device__ __forceinline__ void write_listed(const DistillArgs& p, const RowSlope<MODE>& s, long long row, const T* z, T* out, int* list, Mine mine) {
+    const int lane = threadIdx.x & 31;
+    float* const shares = reinterpret_cast<float*>(list + p.K);
+    if (s.has)
+        for (int k = lane; k < p.K; k += 32) {
+            const int i = entry_at(p, row, k);
+            list[k] = i;
+            shares[k] = i >= 0 ? ex2((teacher_at(p, row, k) - s.top) * p.c) * s.share : 0.f;
+        }
+    __syncwarp();
+    bool listed = false;
+    if (s.has)
+        for (int k = lane; k < p.K; k += 32) {
+            const int i = list[k];
+            if (i < 0 || !mine(i)) continue;
+            listed = listed || i == s.label;
+            const float value = s.f(number(z + i));
             float take = 0.f;
             bool first = true;
+#pragma unroll 4
             for (int j = 0; j < p.K; ++j)
-                if (at[j] == i) {
+                if (list[j] == i) {
                     first = first && j >= k;
-                    take += share[j];
+                    take += shares[j];
                 }
-            if (first) store1(out, i, f(number(z + i)) - teach * take - (i == label ? up * p.w : 0.f));
+            if (first) store1(out, i, value - s.teach * take - (i == s.label ? s.hard : 0.f));
         }
-    if (label >= lo && label < hi && me == 0) {
-        bool listed = false;
-        if (has)
-            for (int j = 0; j < p.K; ++j) listed = listed || at[j] == label;
-        if (!listed) store1(out, label, f(number(z + label)) - up * p.w);
-    }
+    if (s.label >= 0 && mine(s.label) && !__any_sync(0xffffffffu, listed) && lane == 0) store1(out, s.label, s.f(number(z + s.label)) - s.hard);
 }
 
-template <typename T, bool TWO>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kRowWarps * 32) distill_bwd_warp_kernel(const DistillArgs p) {
     extern __shared__ int lists[];
     const int warp = threadIdx.x >> 5;
     const long long row = (long long)blockIdx.x * kRowWarps + warp;
-    if (row < p.N) write_row<T, TWO>(p, row, 0, p.V, threadIdx.x & 31, 32, lists + warp * 2 * p.K, [] { __syncwarp(); });
+    if (row >= p.N) return;
+    const T* const z = static_cast<const T*>(p.z) + row * p.zp;
+    T* const out = static_cast<T*>(p.dz) + row * p.V;
+    const RowSlope<MODE> s(p, row);
+    const RowCut<T> cut(z, p.V);
+    write_dense<T, MODE>(p, s, z, out, cut, 0, cut.pieces, true, threadIdx.x & 31, 32);
+    __syncwarp();
+    write_listed<T, MODE>(p, s, row, z, out, lists + warp * 2 * p.K, [](int) { return true; });
 }
-template <typename T, bool TWO>
+// CTAs of a row have p.pieces loads of 16 bytes each; the listed entries among a CTA's own are written by its first warp behind the rest.
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kRowCta) distill_bwd_kernel(const DistillArgs p) {
     extern __shared__ int lists[];
-    const long long row = blockIdx.x / p.parts;
-    const int part = blockIdx.x % p.parts;
-    const RowCut<T> cut(static_cast<const T*>(p.z) + row * p.zp, p.V);
-    const int per = (cut.pieces + p.parts - 1) / p.parts;
-    const int lo = part ? min(cut.tail, cut.head + part * per * Vec16<T>::n) : 0, hi = part + 1 < p.parts ? min(cut.tail, cut.head + (part + 1) * per * Vec16<T>::n) : p.V;
-    write_row<T, TWO>(p, row, lo, hi, threadIdx.x, kRowCta, lists, [] { __syncthreads(); });
+    const long long row = blockIdx.x / p.ctas;
+    const int part = blockIdx.x % p.ctas;
+    const T* const z = static_cast<const T*>(p.z) + row * p.zp;
+    T* const out = static_cast<T*>(p.dz) + row * p.V;
+    const RowCut<T> cut(z, p.V);
+    const int b0 = min(cut.pieces, part * p.pieces), b1 = part + 1 < p.ctas ? min(cut.pieces, b0 + p.pieces) : cut.pieces;
+    const RowSlope<MODE> s(p, row);
+    write_dense<T, MODE>(p, s, z, out, cut, b0, b1, part == 0, threadIdx.x, kRowCta);
+    __syncthreads();
+    if (threadIdx.x < 32)
+        write_listed<T, MODE>(p, s, row, z, out, lists, [&](int i) {
+            const int piece = (i - cut.head) / Vec16<T>::n;
+            return i < cut.head || i >= cut.tail ? part == 0 : piece >= b0 && piece < b1;
+        });
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -380,14 +470,31 @@ static DistillArgs distill_args(const m2d_distill_desc* d) {
     a.c1 = kLog2e; a.c = (float)(1.4426950408889634 / (double)d->temperature);
     return a;
 }
-// A warp for a row of up to 8 KB: a CTA's threads would have less than two pieces each.
+// A warp for a row of up to 8 KB: a CTA's threads would have two loads each at most.
 static bool short_rows(const m2d_distill_desc* d) { return (long long)d->V * (d->dtype == M2D_F32 ? 4 : 2) <= 8192; }
 template <typename F>
 static int for_distill(const m2d_distill_desc* d, F fn) {
-    // both temperatures where they differ and both are wanted
-    const bool two = d->label_weight > 0.f && d->temperature != 1.f;
-    if (d->dtype == M2D_F32) return two ? fn(float{}, std::true_type{}) : fn(float{}, std::false_type{});
-    return two ? fn(__nv_bfloat16{}, std::true_type{}) : fn(__nv_bfloat16{}, std::false_type{});
+    using std::integral_constant;
+    auto with = [&](auto elem) {
+        // two exponentials where temperatures differ and both are wanted
+        if (d->label_weight == 0.f || d->temperature == 1.f) return fn(elem, integral_constant<int, kOne>{});
+        return d->temperature == 2.f ? fn(elem, integral_constant<int, kSquare>{}) : fn(elem, integral_constant<int, kTwo>{});
+    };
+    return d->dtype == M2D_F32 ? with(float{}) : with(__nv_bfloat16{});
+}
+// Pieces of 16 KB and all CTAs that the GPU holds; pieces of 4 KB where there are too few of those.
+struct DistillPlan { int unit, pieces, ctas; };
+static DistillPlan plan_distill(const m2d_distill_desc* d) {
+    const int loads = d->V / (d->dtype == M2D_F32 ? 4 : 8);
+    const long long most = 8ll * sm_count();
+    DistillPlan pl{};
+    for (pl.unit = 4; pl.unit >= 1; pl.unit -= 3) {
+        pl.pieces = std::max(1, (loads + kRowCta * pl.unit - 1) / (kRowCta * pl.unit));
+        pl.ctas = (int)std::min<long long>(most, d->N * pl.pieces);
+        if (pl.ctas == most) break;
+    }
+    pl.unit = std::max(1, pl.unit);
+    return pl;
 }
 
 }  // namespace m2d
@@ -396,32 +503,32 @@ using namespace m2d;
 
 extern "C" uint64_t m2d_distill_stats(const m2d_distill_desc* d) { return d && d->N > 0 ? (uint64_t)d->N * kRowStats : 0; }
 
+extern "C" uint64_t m2d_distill_fwd_workspace(const m2d_distill_desc* d) {
+    return d && d->N > 0 && d->V > 0 && !short_rows(d) ? (uint64_t)(d->N + plan_distill(d).ctas) * sizeof(float4) : 0;
+}
+
 extern "C" int m2d_distill_fwd(const m2d_distill_desc* d, void* stream) {
     const int rc = check_distill(d);
     if (rc != M2D_OK) return rc;
     if (!d->loss) return M2D_ERR_NULL;
+    if (!short_rows(d) && (!d->workspace || d->workspace_bytes < m2d_distill_fwd_workspace(d) || (reinterpret_cast<uintptr_t>(d->workspace) & 255))) return M2D_ERR_WORKSPACE;
     DistillArgs a = distill_args(d);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return for_distill(d, [&](auto elem, auto two) {
+    return for_distill(d, [&](auto elem, auto mode) {
         using T = decltype(elem);
-        constexpr bool TWO = decltype(two)::value;
+        constexpr int MODE = decltype(mode)::value;
+        const unsigned warps = (unsigned)((d->N + kRowWarps - 1) / kRowWarps);
         if (short_rows(d)) {
-            distill_fwd_warp_kernel<T, TWO><<<(unsigned)((d->N + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, st>>>(a);
+            distill_fwd_warp_kernel<T, MODE><<<warps, kRowWarps * 32, 0, st>>>(a);
             return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
         }
-        // few rows: up to eight CTAs each, while a thread has two pieces or more
-        a.parts = 1;
-        while (a.parts < 8 && d->N * a.parts * 2 <= 2ll * sm_count() && (long long)d->V * (int)sizeof(T) / 16 / (a.parts * 2 * kRowCta) >= 2) a.parts *= 2;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(d->N * a.parts));
-        cfg.blockDim = dim3(kRowCta);
-        cfg.stream = st;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = a.parts; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        if (cudaLaunchKernelEx(&cfg, distill_fwd_kernel<T, TWO>, a) != cudaSuccess) { cudaGetLastError(); return M2D_ERR_LAUNCH; }
+        const DistillPlan pl = plan_distill(d);
+        a.pieces = pl.pieces;
+        a.ctas = pl.ctas;
+        a.found = static_cast<float4*>(d->workspace);
+        if (pl.unit == 4) distill_fwd_kernel<T, MODE, 4><<<pl.ctas, kRowCta, 0, st>>>(a);
+        else distill_fwd_kernel<T, MODE, 1><<<pl.ctas, kRowCta, 0, st>>>(a);
+        if (cudaGetLastError() != cudaSuccess || !launch_following(distill_join_kernel<T, MODE>, dim3(warps), dim3(kRowWarps * 32), 0, st, a)) return M2D_ERR_LAUNCH;
         return M2D_OK;
     });
 }
@@ -435,15 +542,23 @@ extern "C" int m2d_distill_bwd(const m2d_distill_desc* d, void* stream) {
     // a row and its gradient begin at the same distance from a 16-byte boundary
     a.same_phase = (reinterpret_cast<uintptr_t>(d->logits) - reinterpret_cast<uintptr_t>(d->d_logits)) % 16 == 0 && (d->logits_row - d->V) * es % 16 == 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return for_distill(d, [&](auto elem, auto two) {
+    return for_distill(d, [&](auto elem, auto mode) {
         using T = decltype(elem);
-        constexpr bool TWO = decltype(two)::value;
+        constexpr int MODE = decltype(mode)::value;
+        const size_t smem = (size_t)kRowWarps * 2 * d->K * 4;
+        const unsigned warps = (unsigned)((d->N + kRowWarps - 1) / kRowWarps);
         if (short_rows(d)) {
-            const size_t smem = (size_t)kRowWarps * 2 * d->K * 4;
-            distill_bwd_warp_kernel<T, TWO><<<(unsigned)((d->N + kRowWarps - 1) / kRowWarps), kRowWarps * 32, smem, st>>>(a);
+            distill_bwd_warp_kernel<T, MODE><<<warps, kRowWarps * 32, smem, st>>>(a);
         } else {
-            a.parts = (int)std::min<long long>(32, std::max<long long>(1, (long long)d->V * (int)sizeof(T) / 32768));
-            distill_bwd_kernel<T, TWO><<<(unsigned)(d->N * a.parts), kRowCta, (size_t)2 * d->K * 4, st>>>(a);
+            // whole loads of all threads, 96 KB a CTA where there is enough to do and 16 KB where not, and a rest: 2048x131072 bf16 176 us, in equal
+            // parts of about that size 194, in parts of 16 KB 212
+            const long long loads = std::max(1, d->V / Vec16<T>::n);
+            for (int times = 6; times >= 1; --times) {
+                a.pieces = 4 * kRowCta * times;
+                a.ctas = (int)((loads + a.pieces - 1) / a.pieces);
+                if (d->N * a.ctas >= 8ll * sm_count()) break;
+            }
+            distill_bwd_kernel<T, MODE><<<(unsigned)(d->N * a.ctas), kRowCta, (size_t)2 * d->K * 4, st>>>(a);
         }
         return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
     });

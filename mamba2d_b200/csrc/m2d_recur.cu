@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
     T *const dx = static_cast<T*>(p.dx) + out, *const dgate = static_cast<T*>(p.dgate) + out;
     const float* const marks = p.marks + (long long)w.b * ((p.T + kMark - 1) / kMark) * p.C + w.c;
     Raw rx[L], rg[L], rd[L];
-    N mark;
+    float mark[VEC];                                      // (packed where it is used: nothing waits for it before)
     auto load = [&](int t1) {
         const int t0 = t1 + w.run * L, n = w.mine ? w.len - t0 : 0;
         const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt, *pd = dy + t0 * p.dt;
@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
                 rd[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pd)) : P::fill(0.f);
             }
         }
-        mark = load_state<VEC>(marks + (long long)(t1 / kMark) * p.C, w.mine && t1 < w.len);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) mark[v] = w.mine && t1 < w.len ? marks[(long long)(t1 / kMark) * p.C + v] : 0.f;
     };
     float* const cluster_part = smem + (size_t)2 * w.warps * 4 * width;
     N carry = load_state<VEC>(p.d_state_out + (long long)w.b * p.C + w.c, p.d_state_out && w.mine);
@@ -433,7 +434,8 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         }
 #pragma unroll
         for (int i = L - 1; i >= 0; --i) R = mul_(a[i], add_(dv[i], R));
-        const N first = mark;
+        N first = N::all(mark[0]);
+        if constexpr (VEC == 2) first.set(1, mark[1]);
         if (s0 >= stride) load(s0 - stride + w.rank * tile);
         Step<VEC> up = all.done(), down = up;
         N add = h, flow = R;

@@ -280,6 +280,12 @@ struct Distill {
             *stats = at::empty({(int64_t)m2d_distill_stats(&d)}, f32);
             d.stats = fptr(*stats);
         }
+        d.workspace_bytes = m2d_distill_fwd_workspace(&d);
+        Tensor ws;
+        if (d.workspace_bytes) {
+            ws = scratch(d.workspace_bytes, z);
+            d.workspace = ws.data_ptr();
+        }
         check(m2d_distill_fwd(&d, stream_of(z)), "m2d_distill_fwd");
         return loss;
     }

@@ -34,7 +34,7 @@ class DistillDesc(ctypes.Structure):
     _fields_ = [("struct_bytes", ctypes.c_uint32), *[(n, ctypes.c_int32) for n in ("dtype", "teacher_dtype", "V", "K", "index_64", "labels_64")],
                 ("temperature", ctypes.c_float), ("label_weight", ctypes.c_float), ("N", ctypes.c_int64), ("logits", ctypes.c_void_p), ("logits_row", ctypes.c_int64),
                 ("teacher", ctypes.c_void_p), ("teacher_row", ctypes.c_int64), ("index", ctypes.c_void_p), ("index_row", ctypes.c_int64),
-                *[(n, ctypes.c_void_p) for n in ("labels", "loss", "stats", "d_loss")], ("d_loss_row", ctypes.c_int64), ("d_logits", ctypes.c_void_p)]
+                *[(n, ctypes.c_void_p) for n in ("labels", "loss", "stats", "d_loss")], ("d_loss_row", ctypes.c_int64), ("d_logits", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
 @pytest.fixture(scope="module")
@@ -42,7 +42,7 @@ def L():
     from mamba2d_b200 import build
     build.build()
     raw = ctypes.CDLL(_lib.LIB_PATH)
-    raw.m2d_recur_marks.restype = raw.m2d_ln_bwd_workspace.restype = raw.m2d_distill_stats.restype = ctypes.c_uint64
+    raw.m2d_recur_marks.restype = raw.m2d_ln_bwd_workspace.restype = raw.m2d_distill_stats.restype = raw.m2d_distill_fwd_workspace.restype = ctypes.c_uint64
     return raw
 
 
@@ -124,6 +124,10 @@ def test_distillation_descriptors(L):
                    ({"label_weight": 1.5}, FLAGS), ({"label_weight": 0.5}, NULL), ({"logits": None}, NULL), ({"index": None}, NULL), ({"logits": 258}, PITCH)):
         assert L.m2d_distill_fwd(desc(**kw), None) == rc and L.m2d_distill_bwd(desc(**kw), None) == rc, kw
     assert L.m2d_distill_fwd(None, None) == NULL and L.m2d_distill_stats(desc()) > 0
+    assert L.m2d_distill_fwd_workspace(desc()) == 0                                       # (short rows)
+    need = L.m2d_distill_fwd_workspace(desc(V=50000))
+    for kw in ({}, {"workspace": 256, "workspace_bytes": need - 1}, {"workspace": 128, "workspace_bytes": need}):
+        assert L.m2d_distill_fwd(desc(V=50000, loss=256, **kw), None) == WORKSPACE
 
 
 def test_refusals_of_the_distillation_loss():
