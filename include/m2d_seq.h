@@ -131,7 +131,8 @@ int m2d_clip_grad_norm(const m2d_clip_tensor *tensors, int32_t count, float max_
  *     M2D_GATE_DECAY:  a = exp(gate), u = x           (gate at most 0; positive ones grow the state and are not checked for)
  *     M2D_GATE_FORGET: a = sigmoid(gate), u = (1 - a) x
  * A gate of -inf forgets everything before the token.  States and their gradients are fp32 whatever the tensors' type.  B times C/32 up to
- * 2^27, T below 2^31 - 1024.
+ * 2^27, T below 2^31 - 2^17.  Sequences of several strides whose rows begin at 16-byte boundaries come by TMA; a wait for such a copy that gives
+ * up makes what depends on it NaN and shows in m2d_take_wait_failure().
  */
 typedef enum { M2D_GATE_DECAY = 0, M2D_GATE_FORGET = 1 } m2d_gate;
 
@@ -145,6 +146,7 @@ typedef struct m2d_recur_desc {
     int32_t dtype;                 /* m2d_dtype of x, gate, y and their gradients */
     int32_t B, T, C;
     int32_t form;                  /* m2d_gate */
+    uint32_t flags;                /* 0, or the test hook */
     m2d_recur_tensor x, gate;
     const int32_t *lengths;        /* (B) tokens of each sequence, clamped to 0 ... T, or NULL: T.  Rows behind a sequence's last are not
                                       read; outputs there are zero */
@@ -157,6 +159,10 @@ typedef struct m2d_recur_desc {
     void *d_x, *d_gate;            /* (B,T,C) dense */
     float *d_state;                /* (B,C) dense, or NULL: not wanted */
 } m2d_recur_desc;
+
+/* Test hook, rejected with M2D_ERR_FLAGS unless the environment variable M2D_TEST_HOOKS is 1: the first CTA of a launch by TMA asks for nothing, so
+ * that its waits run out. */
+#define M2D_RECUR_TEST_GIVE_UP 0x100u
 
 uint64_t m2d_recur_marks(const m2d_recur_desc *desc);   /* states that the forward pass keeps for the backward pass (reads B, T and C) */
 int m2d_recur_fwd(const m2d_recur_desc *desc, void *stream);

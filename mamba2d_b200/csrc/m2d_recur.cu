@@ -7,18 +7,18 @@
 // A cluster of CTAs owns the channels of LANES lanes and walks a sequence in strides, a tile of it for each CTA.  Inside a tile the lanes of a row
 // take L tokens: they find what those do to any state, h -> A h + b, from registers; the runs' pairs (A, b) are joined in shared memory, the tiles' in
 // that of every CTA of the cluster; then each goes over its tokens again from the state before them, still from registers, and stores.  So
-// memory is read once and written once, and the loads of the next tile are under way meanwhile.  What is wanted are loads in flight
-// (16 warps an SM with 64 bytes and more a thread): where sequences and channels are too few, rows are split into shorter pieces and
-// the sequence over up to 8 CTAs (plan_recur).
+// memory is read once and written once.  Tiles come by TMA, two or three ahead of the one that is worked on; where rows are not whole 16-byte pieces, or
+// there is but one stride, by plain loads into registers, the next tile's while one is worked on.  Where sequences and channels are too few for all SMs, rows are
+// split into shorter pieces and the sequence over up to 8 CTAs (plan_recur).
 //
 // Precision: states and sums are fp32.  A channel may remember thousands of tokens: 1 - A of a run is small then, and A
 // rounded to fp32 would be off by the same amount at every step, 2^-24 against a 1 - A of 2^-12 at a memory of 4096 tokens.  So A is held in two
 // parts, from E = A - 1 computed without cancellation (a series in the summed gates, or a sum of 1 - f).
 #include <cooperative_groups.h>
 
-#include "follow.cuh"
+#include "launch.cuh"
 #include "packed.cuh"
-#include "plan.cuh"
+#include "tc_ptx.cuh"
 #include "m2d_seq.h"
 
 namespace m2d {
@@ -35,7 +35,11 @@ struct RecurArgs {
     float *state_out, *d_state, *marks;
     void *y, *dx, *dgate;
     int B, T, C, groups, ctas;         // channel groups, CTAs of a cluster
+    int stages, box;                   // tiles in shared memory; tokens of one TMA copy
+    int give_up;                       // test hook
+    int* host_flag;
 };
+struct RecurMaps { CUtensorMap x, gate, dy; };
 
 // VEC neighbouring values of a row as they are in memory, and as numbers.
 template <typename T, int VEC> struct Piece;
@@ -240,71 +244,168 @@ struct Place {
     }
 };
 
-// Shared memory: [2][warps][PARTS][width] of the CTA's warps, [2][ctas][3][width] of the cluster's tiles.  Two of each: one barrier lies between
-// what is read of a tile and what is written of the next but one.
-template <int PARTS>
-constexpr size_t recur_smem(int warps, int ctas, int width) { return sizeof(float) * 2 * width * ((size_t)warps * PARTS + (ctas > 1 ? (size_t)ctas * 3 : 0)); }
+// Shared memory: with TMA first [stages][TENSORS][tile][width] of the tensors; [2][warps][PARTS][width] of the CTA's warps, [2][ctas][3][width] of
+// the cluster's tiles (two of each: one barrier lies between what is read of a tile and what is written of the next but one); last the
+// barriers of the stages and the word that tells that a wait gave up.
+constexpr int kRecurStages = 4;
+inline size_t recur_joins(int parts, int warps, int ctas, int width) { return sizeof(float) * 2 * width * ((size_t)warps * parts + (ctas > 1 ? (size_t)ctas * 3 : 0)); }
+inline size_t recur_stage(int tensors, int tile, int width, int es) { return (size_t)tensors * tile * width * es; }
+constexpr size_t kRecurTail = (kRecurStages + 2) * 8;
 
-template <typename T, int VEC, int FORM, int L, int LANES>
-__global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const RecurArgs p) {
+// A thread's tokens of a tile: TENSORS raw values of each.  order() asks for a tile (thread 0), ready() waits for the oldest one that was asked for, raw()
+// reads it, next() goes on; or, without TMA, load() and raw().
+template <typename T, int VEC, int FORM, int L, int LANES, int TENSORS, bool TMA>
+struct Feed {
+    using P = Piece<T, VEC>;
+    using Raw = typename P::Raw;
+    static constexpr int width = LANES * VEC;
+    Raw reg[TMA ? 1 : TENSORS][TMA ? 1 : L];
+    char* ring;
+    uint32_t bars;
+    volatile int* abort;
+    int stage, stages, tile, box, at, run, ordered;
+    unsigned parity;
+    template <typename W>
+    __device__ __forceinline__ Feed(const RecurArgs& p, const W& w, char* smem, char* tail) {
+        if constexpr (TMA) {
+            ring = smem;
+            bars = smem_u32(tail);
+            abort = reinterpret_cast<volatile int*>(tail + kRecurStages * 8);
+            stage = ordered = 0;
+            parity = 0;
+            stages = p.stages;
+            tile = w.runs * L;
+            box = p.box;
+            at = w.at;
+            run = w.run;
+            if (threadIdx.x == 0) {
+                for (int k = 0; k < stages; ++k) mbar_init(bars + 8 * k, 1);
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                *abort = p.give_up && blockIdx.x == 0;
+            }
+            __syncthreads();
+        }
+    }
+    static __device__ __forceinline__ Raw nothing(int t) { return P::fill(t == 1 ? kept<FORM>() : 0.f); }
+    // the tile that begins at token t1 of sequence b, to channel c0 on
+    __device__ __forceinline__ void order(const RecurMaps& maps, int c0, int t1, int b) {
+        if (threadIdx.x != 0 || *abort) return;
+        const int k = ordered % stages;
+        const uint32_t bar = bars + 8 * k, one = (uint32_t)box * width * sizeof(T);
+        uint32_t to = smem_u32(ring) + (uint32_t)k * TENSORS * tile * width * sizeof(T);
+        mbar_expect_tx(bar, TENSORS * tile * width * sizeof(T));
+#pragma unroll
+        for (int t = 0; t < TENSORS; ++t) {
+            const CUtensorMap* const map = t == 0 ? &maps.x : t == 1 ? &maps.gate : &maps.dy;
+            for (int i = 0; i < tile; i += box, to += one)
+                asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                             ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(t1 + i), "r"(b), "r"(bar) : "memory");
+        }
+        ++ordered;
+    }
+    __device__ __forceinline__ Raw* place(int t, int i) const { return reinterpret_cast<Raw*>(ring + (((size_t)(stage * TENSORS + t) * tile + run * L + i) * width + at) * sizeof(T)); }
+    // false: gave up.  n: tokens that there are of the thread's run; the others' places get what changes nothing.
+    __device__ __forceinline__ bool ready(int n) {
+        if (!mbar_wait(bars + 8 * stage, parity, abort)) return false;
+        if (n < L) {
+#pragma unroll
+            for (int t = 0; t < TENSORS; ++t)
+                for (int i = max(0, n); i < L; ++i) *place(t, i) = nothing(t);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // (a later copy comes here)
+        }
+        return true;
+    }
+    __device__ __forceinline__ void next() {
+        if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
+    __device__ __forceinline__ Raw raw(int t, int i) const {
+        if constexpr (TMA) return *place(t, i);
+        else return reg[t][i];
+    }
+    // bounded wait for what is still on its way, after a wait that gave up; tells the host
+    __device__ __forceinline__ void leave(int* host_flag) {
+        if (threadIdx.x != 0 || !*abort) return;
+        for (int j = max(0, ordered - stages); j < ordered; ++j)
+            for (int n = 0; n < kTcWaitLimit / 32 && !mbar_try_wait32(bars + 8 * (j % stages), (j / stages) & 1); ++n) {}
+        if (host_flag) *reinterpret_cast<volatile int*>(host_flag) = 1;
+    }
+};
+
+template <typename T, int VEC, int FORM, int L, int LANES, bool TMA>
+__global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const RecurArgs p, const __grid_constant__ RecurMaps maps) {
     namespace cg = cooperative_groups;
     using P = Piece<T, VEC>;
     using Raw = typename P::Raw;
     using N = Num<VEC>;
     constexpr int width = LANES * VEC;
-    extern __shared__ __align__(16) float smem[];
+    extern __shared__ __align__(128) char ring[];
     const Place<VEC, LANES> w(p);
     cg::cluster_group cluster = cg::this_cluster();
     if (w.ctas > 1) cluster.barrier_arrive();             // (all have begun before one writes to another)
     const int tile = w.runs * L, stride = w.ctas * tile;
+    float* const smem = reinterpret_cast<float*>(ring + (TMA ? p.stages * (size_t)2 * tile * width * sizeof(T) : 0));
+    Feed<T, VEC, FORM, L, LANES, 2, TMA> feed(p, w, ring, reinterpret_cast<char*>(smem + 2 * width * (w.warps * 3 + (w.ctas > 1 ? w.ctas * 3 : 0))));
     const T* const x = static_cast<const T*>(p.x) + w.b * p.xb + w.c;
     const T* const g = static_cast<const T*>(p.gate) + w.b * p.gb + w.c;
     T* const y = static_cast<T*>(p.y) + (long long)w.b * p.T * p.C + w.c;
-    Raw rx[L], rg[L];
     auto load = [&](int t0) {
         const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt;
         const int n = w.mine ? w.len - t0 : 0;
         if (n >= L) {
 #pragma unroll
             for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt) {
-                rx[i] = __ldcs(reinterpret_cast<const Raw*>(px));
-                rg[i] = __ldcs(reinterpret_cast<const Raw*>(pg));
+                feed.reg[0][i] = __ldcs(reinterpret_cast<const Raw*>(px));
+                feed.reg[1][i] = __ldcs(reinterpret_cast<const Raw*>(pg));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt) {
-                rx[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(px)) : P::fill(0.f);
-                rg[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pg)) : P::fill(kept<FORM>());
+                feed.reg[0][i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(px)) : feed.nothing(0);
+                feed.reg[1][i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pg)) : feed.nothing(1);
             }
         }
     };
     float* const cluster_part = smem + (size_t)2 * w.warps * 3 * width;
     N carry = load_state<VEC>(p.state + (long long)w.b * p.C + w.c, p.state && w.mine);
     int t0 = w.rank * tile + w.run * L;
-    load(t0);
+    // (tokens are counted in 64 bits where a stride may end beyond 2^31)
+    auto order = [&](long long s0) {
+        if (s0 < w.len) feed.order(maps, w.c - w.at, (int)s0 + w.rank * tile, w.b);
+    };
+    if constexpr (TMA) {
+        for (int k = 0; k < p.stages; ++k) order((long long)k * stride);
+    } else {
+        load(t0);
+    }
     if (w.ctas > 1) cluster.barrier_wait();
     for (int s0 = 0, buf = 0; s0 < w.len; s0 += stride, t0 += stride, buf ^= 1) {
+        bool ok = true;
+        if constexpr (TMA) ok = feed.ready(w.mine ? w.len - t0 : 0);
         float *const steps = smem + (size_t)buf * w.warps * 3 * width + 2 * w.at, *const adds = smem + (size_t)(buf * 3 + 2) * w.warps * width + w.at;
         N a[L], u[L], h = N::all(0.f);
         Collect<FORM, VEC> all;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const N gate = P::get(rg[i]);
+            const N gate = P::get(feed.raw(1, i)), x = P::get(feed.raw(0, i));
             N rest;
             open_gate<FORM, VEC>(gate, a[i], rest);
-            u[i] = FORM == M2D_GATE_DECAY ? P::get(rx[i]) : mul_(rest, P::get(rx[i]));
+            u[i] = FORM == M2D_GATE_DECAY ? x : mul_(rest, x);
             all.add(gate, a[i], rest);
             h = fma_(a[i], h, u[i]);
         }
-        if (s0 + stride < w.len) load(t0 + stride);
+        if (!TMA && s0 + stride < w.len) load(t0 + stride);
         Step<VEC> step = all.done();
-        N add = h;
+        N add = ok ? h : N::all(__int_as_float(0x7fc00000));
         join_warp<VEC, LANES, true>(step, add);
         if (w.last) {
             give2(steps + 2 * w.warp * width, step.hi, step.lo);
             give(adds + w.warp * width, add);
         }
         __syncthreads();
+        if constexpr (TMA) {                              // (all have read the stage)
+            order((long long)s0 + (long long)p.stages * stride);
+            feed.next();
+        }
         if (w.ctas > 1) {
             // one warp joins the tile's runs and tells every CTA of the cluster
             float* const tiles = cluster_part + (size_t)buf * w.ctas * 3 * width;
@@ -348,6 +449,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
             }
         }
         h = after_others<VEC, LANES, true>(step, add, h);
+        if (!ok) h = N::all(__int_as_float(0x7fc00000));
         const int n = w.mine ? w.len - t0 : 0;
         if (p.marks && n > 0 && t0 % kMark == 0) store_state<VEC>(p.marks + ((long long)w.b * ((p.T + kMark - 1) / kMark) + t0 / kMark) * p.C + w.c, h);
         T* py = y + (long long)t0 * p.C;
@@ -365,6 +467,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
             }
         }
     }
+    if constexpr (TMA) feed.leave(p.host_flag);
     if (!w.mine) return;
     for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) *reinterpret_cast<Raw*>(y + t * p.C) = P::fill(0.f);
     if (p.state_out && w.rank == 0 && w.run == 0) store_state<VEC>(p.state_out + (long long)w.b * p.C + w.c, carry);
@@ -372,42 +475,45 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
 
 // Tiles from the last to the first.  The states inside a tile come from the forward pass's mark before it: only what flows back is joined
 // between CTAs.
-template <typename T, int VEC, int FORM, int L, int LANES>
-__global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const RecurArgs p) {
+template <typename T, int VEC, int FORM, int L, int LANES, bool TMA>
+__global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const RecurArgs p, const __grid_constant__ RecurMaps maps) {
     namespace cg = cooperative_groups;
     using P = Piece<T, VEC>;
     using Raw = typename P::Raw;
     using N = Num<VEC>;
     constexpr int width = LANES * VEC;
-    extern __shared__ __align__(16) float smem[];
+    extern __shared__ __align__(128) char ring[];
     const Place<VEC, LANES> w(p);
     cg::cluster_group cluster = cg::this_cluster();
     if (w.ctas > 1) cluster.barrier_arrive();
     const int tile = w.runs * L, stride = w.ctas * tile;
+    float* const smem = reinterpret_cast<float*>(ring + (TMA ? p.stages * (size_t)3 * tile * width * sizeof(T) : 0));
+    Feed<T, VEC, FORM, L, LANES, 3, TMA> feed(p, w, ring, reinterpret_cast<char*>(smem + 2 * width * (w.warps * 4 + (w.ctas > 1 ? w.ctas * 3 : 0))));
     const T* const x = static_cast<const T*>(p.x) + w.b * p.xb + w.c;
     const T* const g = static_cast<const T*>(p.gate) + w.b * p.gb + w.c;
     const T* const dy = static_cast<const T*>(p.dy) + w.b * p.db + w.c;
     const long long out = (long long)w.b * p.T * p.C + w.c;
     T *const dx = static_cast<T*>(p.dx) + out, *const dgate = static_cast<T*>(p.dgate) + out;
     const float* const marks = p.marks + (long long)w.b * ((p.T + kMark - 1) / kMark) * p.C + w.c;
-    Raw rx[L], rg[L], rd[L];
     float mark[VEC];                                      // (packed where it is used: nothing waits for it before)
     auto load = [&](int t1) {
-        const int t0 = t1 + w.run * L, n = w.mine ? w.len - t0 : 0;
-        const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt, *pd = dy + t0 * p.dt;
-        if (n >= L) {
+        if constexpr (!TMA) {
+            const int t0 = t1 + w.run * L, n = w.mine ? w.len - t0 : 0;
+            const T *px = x + t0 * p.xt, *pg = g + t0 * p.gt, *pd = dy + t0 * p.dt;
+            if (n >= L) {
 #pragma unroll
-            for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt, pd += p.dt) {
-                rx[i] = __ldcs(reinterpret_cast<const Raw*>(px));
-                rg[i] = __ldcs(reinterpret_cast<const Raw*>(pg));
-                rd[i] = __ldcs(reinterpret_cast<const Raw*>(pd));
-            }
-        } else {
+                for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt, pd += p.dt) {
+                    feed.reg[0][i] = __ldcs(reinterpret_cast<const Raw*>(px));
+                    feed.reg[1][i] = __ldcs(reinterpret_cast<const Raw*>(pg));
+                    feed.reg[2][i] = __ldcs(reinterpret_cast<const Raw*>(pd));
+                }
+            } else {
 #pragma unroll
-            for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt, pd += p.dt) {
-                rx[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(px)) : P::fill(0.f);
-                rg[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pg)) : P::fill(kept<FORM>());
-                rd[i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pd)) : P::fill(0.f);
+                for (int i = 0; i < L; ++i, px += p.xt, pg += p.gt, pd += p.dt) {
+                    feed.reg[0][i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(px)) : feed.nothing(0);
+                    feed.reg[1][i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pg)) : feed.nothing(1);
+                    feed.reg[2][i] = i < n ? __ldcs(reinterpret_cast<const Raw*>(pd)) : feed.nothing(2);
+                }
             }
         }
 #pragma unroll
@@ -416,29 +522,44 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
     float* const cluster_part = smem + (size_t)2 * w.warps * 4 * width;
     N carry = load_state<VEC>(p.d_state_out + (long long)w.b * p.C + w.c, p.d_state_out && w.mine);
     int s0 = w.len > 0 ? (w.len - 1) / stride * stride : -1;
+    auto order = [&](int s0) {
+        if (s0 >= 0) feed.order(maps, w.c - w.at, s0 + w.rank * tile, w.b);
+    };
+    int asked = s0;                                       // the next stride to ask for
+    if constexpr (TMA)
+        for (int k = 0; k < p.stages && asked >= 0; ++k, asked -= stride) order(asked);
     if (s0 >= 0) load(s0 + w.rank * tile);
     if (w.ctas > 1) cluster.barrier_wait();
+    bool again = false;                                   // from the second stride on the stage of the one before is free
     for (int buf = 0; s0 >= 0; s0 -= stride, buf ^= 1) {
         const int t0 = s0 + w.rank * tile + w.run * L;
+        bool ok = true;
+        if constexpr (TMA) ok = feed.ready(w.mine ? w.len - t0 : 0);
         float *const steps = smem + (size_t)buf * w.warps * 4 * width + 2 * w.at, *const adds = steps + (size_t)w.warps * 2 * width;
-        N a[L], rest[L], xv[L], dv[L], before[L], h = N::all(0.f), R = N::all(0.f);
+        N a[L], rest[L], before[L], h = N::all(0.f), R = N::all(0.f);
+        N xs[TMA ? 1 : L], ds[TMA ? 1 : L];               // (of a tile in shared memory x and dy are read again instead)
+        auto xv = [&](int i) { return TMA ? P::get(feed.raw(0, i)) : xs[TMA ? 0 : i]; };
+        auto dv = [&](int i) { return TMA ? P::get(feed.raw(2, i)) : ds[TMA ? 0 : i]; };
         Collect<FORM, VEC> all;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const N gate = P::get(rg[i]);
-            xv[i] = P::get(rx[i]);
-            dv[i] = P::get(rd[i]);
+            const N gate = P::get(feed.raw(1, i));
+            if constexpr (!TMA) {
+                xs[i] = P::get(feed.raw(0, i));
+                ds[i] = P::get(feed.raw(2, i));
+            }
             open_gate<FORM, VEC>(gate, a[i], rest[i]);
             all.add(gate, a[i], rest[i]);
-            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv[i] : mul_(rest[i], xv[i]));
+            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv(i) : mul_(rest[i], xv(i)));
         }
 #pragma unroll
-        for (int i = L - 1; i >= 0; --i) R = mul_(a[i], add_(dv[i], R));
+        for (int i = L - 1; i >= 0; --i) R = mul_(a[i], add_(dv(i), R));
         N first = N::all(mark[0]);
         if constexpr (VEC == 2) first.set(1, mark[1]);
         if (s0 >= stride) load(s0 - stride + w.rank * tile);
         Step<VEC> up = all.done(), down = up;
-        N add = h, flow = R;
+        const N nan = N::all(__int_as_float(0x7fc00000));
+        N add = ok ? h : nan, flow = ok ? R : nan;
         join_warp<VEC, LANES, true>(up, add);
         join_warp<VEC, LANES, false>(down, flow);
         if (w.last) {
@@ -447,6 +568,12 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         }
         if (w.first) give(adds + 2 * w.warp * width + VEC, flow);
         __syncthreads();
+        if constexpr (TMA)
+            if (again && asked >= 0) {
+                order(asked);
+                asked -= stride;
+            }
+        again = true;
         auto back = [&](int k, N from) {
             const Two<VEC> s = take2<VEC>(steps + 2 * k * width);
             return Step<VEC>{s.a, s.b}.apply(from, take<VEC>(adds + 2 * k * width + VEC));
@@ -494,20 +621,21 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
             h = Step<VEC>{s.a, s.b}.apply(h, take<VEC>(adds + 2 * k * width));
         }
         h = after_others<VEC, LANES, true>(up, add, h);
+        if (!ok) h = R = nan;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
             before[i] = h;
-            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv[i] : mul_(rest[i], xv[i]));
+            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv(i) : mul_(rest[i], xv(i)));
         }
         const int n = w.mine ? w.len - t0 : 0;
         T *px = dx + (long long)(t0 + L - 1) * p.C, *pg = dgate + (long long)(t0 + L - 1) * p.C;
         auto write = [&](auto whole) {
 #pragma unroll
             for (int i = L - 1; i >= 0; --i, px -= p.C, pg -= p.C) {
-                const N D = add_(dv[i], R);
+                const N D = add_(dv(i), R);
                 R = mul_(a[i], D);
                 const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
-                const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv[i], N::all(-1.f), before[i]));
+                const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv(i), N::all(-1.f), before[i]));
                 if (whole.value || i < n) {
                     *reinterpret_cast<Raw*>(px) = P::put(gx);
                     *reinterpret_cast<Raw*>(pg) = P::put(gg);
@@ -516,7 +644,9 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         };
         if (n >= L) write(std::true_type{});
         else write(std::false_type{});
+        if constexpr (TMA) feed.next();
     }
+    if constexpr (TMA) feed.leave(p.host_flag);
     if (!w.mine) return;
     for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) {
         *reinterpret_cast<Raw*>(dx + t * p.C) = P::fill(0.f);
@@ -548,9 +678,10 @@ static int check_recur(const m2d_recur_desc* d, bool step) {
     if (d->struct_bytes != sizeof(m2d_recur_desc)) return M2D_ERR_ABI;
     if (d->dtype != M2D_F32 && d->dtype != M2D_BF16) return M2D_ERR_DTYPE;
     if (d->form != M2D_GATE_DECAY && d->form != M2D_GATE_FORGET) return M2D_ERR_FLAGS;
+    if (d->flags && !(d->flags == M2D_RECUR_TEST_GIVE_UP && test_hooks_enabled())) return M2D_ERR_FLAGS;
     if (d->B < 1 || d->T < 1 || d->C < 1 || (step && d->T != 1)) return M2D_ERR_SHAPE;
     // (tokens are counted in 32 bits, a tile beyond the last included; CTAs too)
-    if (d->T > INT32_MAX - 1024 || (long long)d->B * ((d->C + 31) / 32) > INT32_MAX / 16) return M2D_ERR_TOO_LARGE;
+    if (d->T > INT32_MAX - (1 << 17) || (long long)d->B * ((d->C + 31) / 32) > INT32_MAX / 16) return M2D_ERR_TOO_LARGE;
     const uintptr_t es = d->dtype == M2D_F32 ? 4 : 2;
     for (const void* t : {d->x.data, d->gate.data}) {
         if (!t) return M2D_ERR_NULL;
@@ -605,9 +736,36 @@ static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, bool bw
     }
     return best;
 }
-template <int PARTS, typename K>
-static int launch_recur(K kern, const RecurArgs& a, const RecurPlan& pl, int vec, cudaStream_t st) {
-    const size_t smem = recur_smem<PARTS>(pl.warps, pl.ctas, pl.lanes * vec);
+// Whether a tensor can be fetched by TMA: 16-byte aligned rows.  (A stride that no step is taken along may be anything: the map gets a valid one.)
+static bool recur_fits(const m2d_recur_desc* d, const m2d_recur_tensor& t, int es) {
+    auto stride = [&](int n, int64_t s) { return n == 1 || (s > 0 && s * es % 16 == 0 && s * es < (1ll << 39)); };
+    return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && stride(d->T, t.token) && stride(d->B, t.batch);
+}
+static bool recur_map(CUtensorMap* map, const m2d_recur_desc* d, const m2d_recur_tensor& t, int es, int width, int box) {
+    const cuuint64_t dims[3] = {(cuuint64_t)d->C, (cuuint64_t)d->T, (cuuint64_t)d->B};
+    const cuuint64_t strides[2] = {d->T == 1 ? 16 : (cuuint64_t)t.token * es, d->B == 1 ? 16 : (cuuint64_t)t.batch * es};
+    const cuuint32_t boxes[3] = {(cuuint32_t)width, (cuuint32_t)box, 1}, step[3] = {1, 1, 1};
+    return tc_encoder()(map, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(t.data), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// TENSORS of two or three; fed and plain: the kernel's two forms.
+template <int TENSORS, typename K>
+static int launch_recur(K fed, K plain, const m2d_recur_desc* d, RecurArgs& a, const RecurPlan& pl, int vec, int steps, cudaStream_t st) {
+    const int es = d->dtype == M2D_F32 ? 4 : 2, width = pl.lanes * vec, tile = pl.warps * (32 / pl.lanes) * steps;
+    RecurMaps maps{};
+    size_t smem = recur_joins(TENSORS + 1, pl.warps, pl.ctas, width);
+    // more than one stride, and two stages or more in the CTA's share of an SM's memory
+    bool tma = (long long)tile * pl.ctas < d->T && fed != plain && recur_fits(d, d->x, es) && recur_fits(d, d->gate, es) && (TENSORS == 2 || recur_fits(d, d->d_y, es)) && tc_encoder();
+    if (tma) {
+        const size_t stage = recur_stage(TENSORS, tile, width, es), share = pl.warps > 8 ? kMaxSmem : kMaxSmem * pl.warps / kRecurWarps - 512, used = smem + kRecurTail;
+        a.stages = share > used ? (int)std::min<size_t>(kRecurStages, (share - used) / stage) : 0;
+        a.box = std::min(tile, 256);
+        tma = a.stages >= 2 && recur_map(&maps.x, d, d->x, es, width, a.box) && recur_map(&maps.gate, d, d->gate, es, width, a.box) && (TENSORS == 2 || recur_map(&maps.dy, d, d->d_y, es, width, a.box));
+        if (tma) smem += a.stages * stage + kRecurTail;
+    }
+    a.give_up = (d->flags & M2D_RECUR_TEST_GIVE_UP) != 0;
+    a.host_flag = tma ? wait_failure_flag() : nullptr;
+    const K kern = tma ? fed : plain;
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.B * a.groups * pl.ctas));
@@ -619,7 +777,7 @@ static int launch_recur(K kern, const RecurArgs& a, const RecurPlan& pl, int vec
     attr.val.clusterDim.x = pl.ctas; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) { cudaGetLastError(); return M2D_ERR_LAUNCH; }
+    if (cudaLaunchKernelEx(&cfg, kern, a, maps) != cudaSuccess) { cudaGetLastError(); return M2D_ERR_LAUNCH; }
     return M2D_OK;
 }
 // Calls fn(lanes) with the plan's; rows of single values are not cut.
@@ -660,7 +818,7 @@ extern "C" int m2d_recur_fwd(const m2d_recur_desc* d, void* stream) {
             constexpr int LANES = decltype(lanes)::value;
             a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
             a.ctas = pl.ctas;
-            return launch_recur<3>(recur_fwd_kernel<T, VEC, FORM, L, LANES>, a, pl, VEC, static_cast<cudaStream_t>(stream));
+            return launch_recur<2>(recur_fwd_kernel<T, VEC, FORM, L, LANES, VEC == 2>, recur_fwd_kernel<T, VEC, FORM, L, LANES, false>, d, a, pl, VEC, L, static_cast<cudaStream_t>(stream));
         });
     });
 }
@@ -680,7 +838,7 @@ extern "C" int m2d_recur_bwd(const m2d_recur_desc* d, void* stream) {
             constexpr int LANES = decltype(lanes)::value;
             a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
             a.ctas = pl.ctas;
-            return launch_recur<4>(recur_bwd_kernel<T, VEC, FORM, L, LANES>, a, pl, VEC, static_cast<cudaStream_t>(stream));
+            return launch_recur<3>(recur_bwd_kernel<T, VEC, FORM, L, LANES, VEC == 2>, recur_bwd_kernel<T, VEC, FORM, L, LANES, false>, d, a, pl, VEC, L, static_cast<cudaStream_t>(stream));
         });
     });
 }

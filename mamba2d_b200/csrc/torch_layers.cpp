@@ -55,6 +55,7 @@ public:
         TORCH_CHECK(!at::GradMode::is_enabled(), "gated_recurrence: gradients of gradients (create_graph) are not supported");
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[0].device());
+        check_waits("gated_recurrence");
         const bool have_state_grad = grads.size() > 1 && grads[1].defined();
         if (!grads[0].defined() && !have_state_grad) return variable_list(6);
         Recur r(s[0], s[1], s[2], s[3], ctx->saved_data["form"].toInt());
@@ -101,6 +102,7 @@ std::tuple<Tensor, optional<Tensor>> gated_recurrence(const Tensor& x, const Ten
         if (!want_state) return {x.clone(), c10::nullopt};
         return {x.clone(), state.defined() ? state.clone() : at::zeros({x.size(0), x.size(2)}, x.options().dtype(at::kFloat))};
     }
+    check_waits(what);
     if (wants_grad({&x, &gate, &state})) {
         const variable_list r = RecurFn::apply(x, gate, state_, lengths.defined() ? optional<Tensor>(lengths) : c10::nullopt, form, want_state);
         return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
@@ -120,6 +122,7 @@ Tensor gated_recurrence_step(const Tensor& x, const Tensor& gate, const Tensor& 
     TORCH_CHECK(!x.numel() || ((C == 1 || state.stride(1) == 1) && (B == 1 || sb >= C)), what, ": the state must be dense along C and must not overlap itself, got strides ", state.strides());
     TORCH_CHECK(!wants_grad({&x, &gate, &state}), what, " updates the state in place and has no gradients: call it without gradients");
     if (!x.numel()) return x.clone();
+    check_waits(what);                       // (the state may be that of a prompt)
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor xr = rows(x), gr = rows(gate);

@@ -16,7 +16,7 @@ class RecurTensor(ctypes.Structure):
 
 class RecurDesc(ctypes.Structure):
     """Mirror of ``m2d_recur_desc``."""
-    _fields_ = [("struct_bytes", ctypes.c_uint32), *[(n, ctypes.c_int32) for n in ("dtype", "B", "T", "C", "form")], ("x", RecurTensor), ("gate", RecurTensor),
+    _fields_ = [("struct_bytes", ctypes.c_uint32), *[(n, ctypes.c_int32) for n in ("dtype", "B", "T", "C", "form")], ("flags", ctypes.c_uint32), ("x", RecurTensor), ("gate", RecurTensor),
                 *[(n, ctypes.c_void_p) for n in ("lengths", "state", "state_out", "y", "marks")], ("d_y", RecurTensor),
                 *[(n, ctypes.c_void_p) for n in ("d_state_out", "d_x", "d_gate", "d_state")]]
 
@@ -54,7 +54,7 @@ def test_recurrence_descriptors(L):
         for k, v in kw.items():
             setattr(d, k, v)
         return ctypes.byref(d)
-    for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"form": 2}, FLAGS), ({"B": 0}, SHAPE), ({"T": 0}, SHAPE), ({"C": -1}, SHAPE),
+    for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"form": 2}, FLAGS), ({"flags": 0x100}, FLAGS), ({"flags": 1}, FLAGS), ({"B": 0}, SHAPE), ({"T": 0}, SHAPE), ({"C": -1}, SHAPE),
                    ({"T": (1 << 31) - 1}, LARGE), ({"B": 1 << 27}, LARGE), ({"x": RecurTensor(None, 0, 0)}, NULL), ({"gate": RecurTensor(258, 0, 0)}, PITCH)):
         assert L.m2d_recur_fwd(desc(**kw), None) == rc and L.m2d_recur_bwd(desc(**kw), None) == rc, kw
     step = lambda **kw: L.m2d_recur_step(desc(**kw), ctypes.c_int64(64), None)  # noqa: E731

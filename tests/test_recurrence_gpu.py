@@ -1,9 +1,12 @@
 """The gated recurrence against its definition in 64 bits, element by element, within the bound that ``layer_ref`` derives."""
+import ctypes
+
 import pytest
 import torch
 
 import layer_ref
-from mamba2d_b200 import gated_recurrence, gated_recurrence_step
+from mamba2d_b200 import _lib, gated_recurrence, gated_recurrence_step
+from test_layers_host import RecurDesc, RecurTensor
 
 pytestmark = pytest.mark.gpu
 F32, BF = torch.float32, torch.bfloat16
@@ -253,3 +256,31 @@ def test_long_sequences(B, T, C, dt, form, ragged):
     assert layer_ref.within(grads[2], a[:, 0] * D[:, 0], a[:, 0] * (dD[:, 0] + 2.0 ** -19 * E[:, 0])) <= 1
     again = gated_recurrence(x, g, form=form, initial_state=s, lengths=lengths)
     assert torch.equal(again, out[0])
+
+
+def test_a_wait_that_gives_up(monkeypatch):
+    """The first CTA asks for nothing: its results are NaN, and those of tokens behind its own, the next call raises, and the one after is right."""
+    monkeypatch.setenv("M2D_TEST_HOOKS", "1")
+    L = _lib.lib()
+    B, T, C = 2, 30000, 128             # (several strides)
+    x, g, s, dy, ds = inputs(B, T, C, BF, "decay", 10, True)
+    want, last = gated_recurrence(x, g, initial_state=s, return_state=True)
+    y, out, marks = torch.empty_like(x), torch.empty_like(s), torch.zeros(B, -(-T // 64), C, device="cuda")
+    dx, dg, d0 = torch.empty_like(x), torch.empty_like(x), torch.empty_like(s)
+    d = RecurDesc(struct_bytes=ctypes.sizeof(RecurDesc), dtype=1, B=B, T=T, C=C, form=0, flags=0x100)
+    for name, t in (("x", x), ("gate", g), ("d_y", dy)):
+        setattr(d, name, RecurTensor(t.data_ptr(), t.stride(0), t.stride(1)))
+    for name, t in (("state", s), ("state_out", out), ("y", y), ("marks", marks), ("d_state_out", ds), ("d_x", dx), ("d_gate", dg), ("d_state", d0)):
+        setattr(d, name, t.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for call, first, others in ((L.m2d_recur_fwd, (y[0], out[0]), (y[1], out[1])), (L.m2d_recur_bwd, (dx[0], dg[0], d0[0]), (dx[1], dg[1], d0[1]))):
+        assert call(ctypes.byref(d), stream) == 0
+        torch.cuda.synchronize()
+        assert all(bool(torch.isnan(t).any()) for t in first) and not any(bool(torch.isnan(t).any()) for t in others)
+        with pytest.raises(RuntimeError, match="timed out"):
+            gated_recurrence_step(x[:, 0], g[:, 0], s.clone())
+        d.flags = 0                      # (marks for the backward pass)
+        assert L.m2d_recur_fwd(ctypes.byref(d), stream) == 0
+        assert torch.equal(y, want) and torch.equal(out, last)
+        d.flags = 0x100
+    assert torch.equal(gated_recurrence(x, g, initial_state=s), want)
