@@ -452,18 +452,19 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
         if (!ok) h = N::all(__int_as_float(0x7fc00000));
         const int n = w.mine ? w.len - t0 : 0;
         if (p.marks && n > 0 && t0 % kMark == 0) store_state<VEC>(p.marks + ((long long)w.b * ((p.T + kMark - 1) / kMark) + t0 / kMark) * p.C + w.c, h);
-        T* py = y + (long long)t0 * p.C;
+        char* const py = reinterpret_cast<char*>(y + (long long)t0 * p.C);
+        const unsigned row = (unsigned)p.C * (unsigned)sizeof(T);
         if (n >= L) {
 #pragma unroll
-            for (int i = 0; i < L; ++i, py += p.C) {
+            for (int i = 0; i < L; ++i) {
                 h = fma_(a[i], h, u[i]);
-                *reinterpret_cast<Raw*>(py) = P::put(h);
+                *reinterpret_cast<Raw*>(py + (unsigned long long)row * (unsigned)i) = P::put(h);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < L; ++i, py += p.C) {
+            for (int i = 0; i < L; ++i) {
                 h = fma_(a[i], h, u[i]);
-                if (i < n) *reinterpret_cast<Raw*>(py) = P::put(h);
+                if (i < n) *reinterpret_cast<Raw*>(py + (unsigned long long)row * (unsigned)i) = P::put(h);
             }
         }
     }
@@ -628,17 +629,18 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
             h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv(i) : mul_(rest[i], xv(i)));
         }
         const int n = w.mine ? w.len - t0 : 0;
-        T *px = dx + (long long)(t0 + L - 1) * p.C, *pg = dgate + (long long)(t0 + L - 1) * p.C;
+        char *const px = reinterpret_cast<char*>(dx + (long long)t0 * p.C), *const pg = reinterpret_cast<char*>(dgate + (long long)t0 * p.C);
+        const unsigned row = (unsigned)p.C * (unsigned)sizeof(T);
         auto write = [&](auto whole) {
 #pragma unroll
-            for (int i = L - 1; i >= 0; --i, px -= p.C, pg -= p.C) {
+            for (int i = L - 1; i >= 0; --i) {
                 const N D = add_(dv(i), R);
                 R = mul_(a[i], D);
                 const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
                 const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv(i), N::all(-1.f), before[i]));
                 if (whole.value || i < n) {
-                    *reinterpret_cast<Raw*>(px) = P::put(gx);
-                    *reinterpret_cast<Raw*>(pg) = P::put(gg);
+                    *reinterpret_cast<Raw*>(px + (unsigned long long)row * (unsigned)i) = P::put(gx);
+                    *reinterpret_cast<Raw*>(pg + (unsigned long long)row * (unsigned)i) = P::put(gg);
                 }
             }
         };
@@ -680,8 +682,8 @@ static int check_recur(const m2d_recur_desc* d, bool step) {
     if (d->form != M2D_GATE_DECAY && d->form != M2D_GATE_FORGET) return M2D_ERR_FLAGS;
     if (d->flags && !(d->flags == M2D_RECUR_TEST_GIVE_UP && test_hooks_enabled())) return M2D_ERR_FLAGS;
     if (d->B < 1 || d->T < 1 || d->C < 1 || (step && d->T != 1)) return M2D_ERR_SHAPE;
-    // (tokens are counted in 32 bits, a tile beyond the last included; CTAs too)
-    if (d->T > INT32_MAX - (1 << 17) || (long long)d->B * ((d->C + 31) / 32) > INT32_MAX / 16) return M2D_ERR_TOO_LARGE;
+    // (tokens are counted in 32 bits, a tile beyond the last included; CTAs and the bytes of a row too)
+    if (d->T > INT32_MAX - (1 << 17) || d->C > (1 << 29) || (long long)d->B * ((d->C + 31) / 32) > INT32_MAX / 16) return M2D_ERR_TOO_LARGE;
     const uintptr_t es = d->dtype == M2D_F32 ? 4 : 2;
     for (const void* t : {d->x.data, d->gate.data}) {
         if (!t) return M2D_ERR_NULL;
@@ -712,7 +714,7 @@ static int for_recur(const m2d_recur_desc* d, bool pairs, F fn) {
     return pairs ? with_form(__nv_bfloat16{}, integral_constant<int, 2>{}) : with_form(__nv_bfloat16{}, integral_constant<int, 1>{});
 }
 // Lanes of a row, warps of a CTA and CTAs of a cluster: the least time by a model of it.  An SM holds 16 warps (128 registers a
-// thread); clusters of 4 and 8 leave some SMs of a GPC over (33 and 15 of such CTAs fit 148 SMs).  All clusters run in so many waves, and each takes so many
+// thread); clusters of 4 and 8 leave some SMs of a GPC over (of CTAs of 16 warps 33 and 15 fit 148 SMs, of 8 warps 71 and 33).  All clusters run in so many waves, and each takes so many
 // strides; a stride takes about a time of 10 for its chain of load, joins and store and 1 for each warp of the SM (its instructions).
 // Rows in pieces of 16 or 8 lanes (64 and 32 bytes of bf16), larger clusters and CTAs that have an SM for themselves cost a little more.
 struct RecurPlan { int lanes, warps, ctas; };
@@ -727,7 +729,8 @@ static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, bool bw
                 const long long tile = (long long)warps * (32 / lanes);            // in runs
                 if (ctas > 1 && tile * (ctas / 2) >= runs) break;                  // (half of them would do)
                 if (bwd && tile * steps % kMark && (ctas > 1 || tile < runs)) continue;        // (a tile begins at a mark)
-                const long long held = std::max(1ll, (ctas == 8 ? sms * 15 / 148 : ctas == 4 ? sms * 33 / 148 : sms / ctas)) * (kRecurWarps / warps);
+                const long long eights = (ctas == 8 ? 33 : ctas == 4 ? 71 : 296 / ctas) * sms / 148;            // clusters of CTAs of eight warps
+                const long long held = std::max(1ll, warps == 16 ? (ctas == 8 ? 15 : ctas == 4 ? 33 : 148 / ctas) * sms / 148 : eights * 8 / warps);
                 const long long waves = (chains + held - 1) / held, strides = (runs + tile * ctas - 1) / (tile * ctas);
                 const long long per_sm = std::min<long long>(kRecurWarps, (chains * ctas + sms - 1) / sms * warps);
                 const double t = (double)(waves * strides) * (10 + per_sm) * (warps == 16 ? 1.1 : 1.0) * (lanes == 32 ? 1.0 : lanes == 16 ? 1.05 : 1.15) * (ctas == 1 ? 1.0 : 1.1 + 0.02 * ctas);
@@ -748,24 +751,31 @@ static bool recur_map(CUtensorMap* map, const m2d_recur_desc* d, const m2d_recur
     return tc_encoder()(map, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(t.data), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// TENSORS of two or three; fed and plain: the kernel's two forms.
-template <int TENSORS, typename K>
-static int launch_recur(K fed, K plain, const m2d_recur_desc* d, RecurArgs& a, const RecurPlan& pl, int vec, int steps, cudaStream_t st) {
-    const int es = d->dtype == M2D_F32 ? 4 : 2, width = pl.lanes * vec, tile = pl.warps * (32 / pl.lanes) * steps;
+// Calls fn(plan, whether by TMA, maps, shared memory): TENSORS of two or three, runs of `fed` tokens by TMA and of `plain` without.
+template <int TENSORS, typename F>
+static int with_recur(const m2d_recur_desc* d, RecurArgs& a, int vec, int fed, int plain, F fn) {
+    const int es = d->dtype == M2D_F32 ? 4 : 2;
     RecurMaps maps{};
-    size_t smem = recur_joins(TENSORS + 1, pl.warps, pl.ctas, width);
-    // more than one stride, and two stages or more in the CTA's share of an SM's memory
-    bool tma = (long long)tile * pl.ctas < d->T && fed != plain && recur_fits(d, d->x, es) && recur_fits(d, d->gate, es) && (TENSORS == 2 || recur_fits(d, d->d_y, es)) && tc_encoder();
-    if (tma) {
-        const size_t stage = recur_stage(TENSORS, tile, width, es), share = pl.warps > 8 ? kMaxSmem : kMaxSmem * pl.warps / kRecurWarps - 512, used = smem + kRecurTail;
+    a.give_up = (d->flags & M2D_RECUR_TEST_GIVE_UP) != 0;
+    if (vec == 2 && recur_fits(d, d->x, es) && recur_fits(d, d->gate, es) && (TENSORS == 2 || recur_fits(d, d->d_y, es)) && tc_encoder()) {
+        const RecurPlan pl = plan_recur(d, vec, fed, TENSORS == 3);
+        const int width = pl.lanes * vec, tile = pl.warps * (32 / pl.lanes) * fed;
+        // more than one stride, and two stages or more in the CTA's share of an SM's memory
+        const size_t joins = recur_joins(TENSORS + 1, pl.warps, pl.ctas, width), used = joins + kRecurTail, stage = recur_stage(TENSORS, tile, width, es);
+        const size_t share = pl.warps > 8 ? kMaxSmem : kMaxSmem * pl.warps / kRecurWarps - 512;
         a.stages = share > used ? (int)std::min<size_t>(kRecurStages, (share - used) / stage) : 0;
         a.box = std::min(tile, 256);
-        tma = a.stages >= 2 && recur_map(&maps.x, d, d->x, es, width, a.box) && recur_map(&maps.gate, d, d->gate, es, width, a.box) && (TENSORS == 2 || recur_map(&maps.dy, d, d->d_y, es, width, a.box));
-        if (tma) smem += a.stages * stage + kRecurTail;
+        if ((long long)tile * pl.ctas < d->T && a.stages >= 2 && recur_map(&maps.x, d, d->x, es, width, a.box) && recur_map(&maps.gate, d, d->gate, es, width, a.box) &&
+            (TENSORS == 2 || recur_map(&maps.dy, d, d->d_y, es, width, a.box))) {
+            a.host_flag = wait_failure_flag();
+            return fn(pl, true, maps, used + a.stages * stage);
+        }
     }
-    a.give_up = (d->flags & M2D_RECUR_TEST_GIVE_UP) != 0;
-    a.host_flag = tma ? wait_failure_flag() : nullptr;
-    const K kern = tma ? fed : plain;
+    const RecurPlan pl = plan_recur(d, vec, plain, TENSORS == 3);
+    return fn(pl, false, maps, recur_joins(TENSORS + 1, pl.warps, pl.ctas, pl.lanes * vec));
+}
+template <typename K>
+static int launch_recur(K kern, const RecurArgs& a, const RecurMaps& maps, const RecurPlan& pl, size_t smem, cudaStream_t st) {
     if (!allow_smem(reinterpret_cast<const void*>(kern), smem)) return M2D_ERR_LAUNCH;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.B * a.groups * pl.ctas));
@@ -790,9 +800,10 @@ static int for_lanes(int lanes, F fn) {
     }
     return fn(integral_constant<int, 32>{});
 }
-// Tokens of a run, by the registers that they take.
+// Tokens of a run, by the registers that they take (and in the backward pass the shared memory).
 template <typename T> constexpr int kFwdSteps = sizeof(T) == 4 ? 8 : 16;
-constexpr int kBwdSteps = 8;
+template <typename T> constexpr int kBwdSteps = sizeof(T) == 4 ? 8 : 16;
+constexpr int kBwdPlain = 8;
 
 }  // namespace m2d
 
@@ -813,12 +824,13 @@ extern "C" int m2d_recur_fwd(const m2d_recur_desc* d, void* stream) {
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
         constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kFwdSteps<T>;
-        const RecurPlan pl = plan_recur(d, VEC, L, false);
-        return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
-            constexpr int LANES = decltype(lanes)::value;
-            a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
-            a.ctas = pl.ctas;
-            return launch_recur<2>(recur_fwd_kernel<T, VEC, FORM, L, LANES, VEC == 2>, recur_fwd_kernel<T, VEC, FORM, L, LANES, false>, d, a, pl, VEC, L, static_cast<cudaStream_t>(stream));
+        return with_recur<2>(d, a, VEC, L, L, [&](const RecurPlan& pl, bool fed, const RecurMaps& maps, size_t smem) {
+            return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
+                constexpr int LANES = decltype(lanes)::value;
+                a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
+                a.ctas = pl.ctas;
+                return launch_recur(fed ? recur_fwd_kernel<T, VEC, FORM, L, LANES, VEC == 2> : recur_fwd_kernel<T, VEC, FORM, L, LANES, false>, a, maps, pl, smem, static_cast<cudaStream_t>(stream));
+            });
         });
     });
 }
@@ -832,13 +844,15 @@ extern "C" int m2d_recur_bwd(const m2d_recur_desc* d, void* stream) {
     const bool pairs = d->C % 2 == 0 && pairs_ok(a.x, a.xb, a.xt, es) && pairs_ok(a.gate, a.gb, a.gt, es) && pairs_ok(a.dy, a.db, a.dt, es) && pairs_ok(a.dx, 0, 0, es) && pairs_ok(a.dgate, 0, 0, es);
     return for_recur(d, pairs, [&](auto elem, auto vec, auto form) {
         using T = decltype(elem);
-        constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kBwdSteps;
-        const RecurPlan pl = plan_recur(d, VEC, L, true);
-        return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
-            constexpr int LANES = decltype(lanes)::value;
-            a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
-            a.ctas = pl.ctas;
-            return launch_recur<3>(recur_bwd_kernel<T, VEC, FORM, L, LANES, VEC == 2>, recur_bwd_kernel<T, VEC, FORM, L, LANES, false>, d, a, pl, VEC, L, static_cast<cudaStream_t>(stream));
+        constexpr int VEC = decltype(vec)::value, FORM = decltype(form)::value, L = kBwdSteps<T>;
+        return with_recur<3>(d, a, VEC, L, kBwdPlain, [&](const RecurPlan& pl, bool fed, const RecurMaps& maps, size_t smem) {
+            return for_lanes<VEC>(pl.lanes, [&](auto lanes) {
+                constexpr int LANES = decltype(lanes)::value;
+                a.groups = (d->C + LANES * VEC - 1) / (LANES * VEC);
+                a.ctas = pl.ctas;
+                return launch_recur(fed ? recur_bwd_kernel<T, VEC, FORM, VEC == 2 ? L : kBwdPlain, LANES, VEC == 2> : recur_bwd_kernel<T, VEC, FORM, kBwdPlain, LANES, false>, a, maps, pl, smem,
+                                    static_cast<cudaStream_t>(stream));
+            });
         });
     });
 }
