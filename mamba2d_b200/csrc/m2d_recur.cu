@@ -212,13 +212,6 @@ __device__ __forceinline__ Num<VEC> after_others(const Step<VEC>& step, Num<VEC>
     return run == (UP ? 0 : 32 / LANES - 1) ? h : there;
 }
 
-// All CTAs of a cluster.  What the caller alone has written to others' shared memory is released; everything else, and stores to global memory
-// above all, need not be waited for.
-__device__ __forceinline__ void cluster_meet(bool wrote) {
-    if (wrote) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // Where a thread stands: its channels, its run of a tile, its CTA of the cluster.
 template <int VEC, int LANES>
 struct Place {
@@ -246,11 +239,52 @@ struct Place {
 
 // Shared memory: with TMA first [stages][TENSORS][tile][width] of the tensors; [2][warps][PARTS][width] of the CTA's warps, [2][ctas][3][width] of
 // the cluster's tiles (two of each: one barrier lies between what is read of a tile and what is written of the next but one); last the
-// barriers of the stages and the word that tells that a wait gave up.
+// barriers of the stages and of the cluster's tiles, and the word that tells that a wait gave up.
 constexpr int kRecurStages = 4;
 inline size_t recur_joins(int parts, int warps, int ctas, int width) { return sizeof(float) * 2 * width * ((size_t)warps * parts + (ctas > 1 ? (size_t)ctas * 3 : 0)); }
 inline size_t recur_stage(int tensors, int tile, int width, int es) { return (size_t)tensors * tile * width * es; }
-constexpr size_t kRecurTail = (kRecurStages + 2) * 8;
+constexpr size_t kRecurTail = (kRecurStages + 3) * 8;
+
+// Barriers and the abort word of a CTA.  A tile's join reaches every CTA of the cluster by stores that count towards the receiver's barrier:
+// nothing else is waited for.  All waits are bounded; where one gives up, what depends on it is NaN.
+struct Waits {
+    uint32_t stage_bars, join_bars;
+    volatile int* abort;
+    __device__ __forceinline__ Waits(const RecurArgs& p, char* tail) {
+        stage_bars = smem_u32(tail);
+        join_bars = stage_bars + 8 * kRecurStages;
+        abort = reinterpret_cast<volatile int*>(tail + 8 * (kRecurStages + 2));
+        if (threadIdx.x == 0) {
+            for (int k = 0; k < kRecurStages + 2; ++k) mbar_init(stage_bars + 8 * k, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            *abort = p.give_up && blockIdx.x == 0;
+        }
+        __syncthreads();
+    }
+    static __device__ __forceinline__ uint32_t there(uint32_t addr, int rank) {
+        uint32_t r;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+        return r;
+    }
+    // a lane's channels of a tile's join, to CTA `rank`: hi and lo, and what goes with them
+    template <int VEC>
+    __device__ __forceinline__ void send(int rank, const float* pair, const float* add, const Step<VEC>& s, Num<VEC> b, int buf) const {
+        const uint32_t p = there(smem_u32(pair), rank), a = there(smem_u32(add), rank), bar = there(join_bars + 8 * buf, rank);
+        if constexpr (VEC == 2) {
+            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(p), "l"(s.hi.v), "l"(s.lo.v), "r"(bar) : "memory");
+            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(a), "l"(b.v), "r"(bar) : "memory");
+        } else {
+            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(p), "r"(__float_as_uint(s.hi.v)), "r"(__float_as_uint(s.lo.v)), "r"(bar) : "memory");
+            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(a), "r"(__float_as_uint(b.v)), "r"(bar) : "memory");
+        }
+    }
+    // all CTAs' joins are there; `turn` counts the tiles
+    __device__ __forceinline__ bool joined(int turn, uint32_t bytes) const {
+        const uint32_t bar = join_bars + 8 * (turn & 1);
+        if (threadIdx.x == 0) mbar_expect_tx(bar, bytes);
+        return mbar_wait(bar, (turn >> 1) & 1, abort);
+    }
+};
 
 // A thread's tokens of a tile: TENSORS raw values of each.  order() asks for a tile (thread 0), ready() waits for the oldest one that was asked for, raw()
 // reads it, next() goes on; or, without TMA, load() and raw().
@@ -266,11 +300,11 @@ struct Feed {
     int stage, stages, tile, box, at, run, ordered;
     unsigned parity;
     template <typename W>
-    __device__ __forceinline__ Feed(const RecurArgs& p, const W& w, char* smem, char* tail) {
+    __device__ __forceinline__ Feed(const RecurArgs& p, const W& w, char* smem, const Waits& waits) {
+        abort = waits.abort;
         if constexpr (TMA) {
             ring = smem;
-            bars = smem_u32(tail);
-            abort = reinterpret_cast<volatile int*>(tail + kRecurStages * 8);
+            bars = waits.stage_bars;
             stage = ordered = 0;
             parity = 0;
             stages = p.stages;
@@ -278,12 +312,6 @@ struct Feed {
             box = p.box;
             at = w.at;
             run = w.run;
-            if (threadIdx.x == 0) {
-                for (int k = 0; k < stages; ++k) mbar_init(bars + 8 * k, 1);
-                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-                *abort = p.give_up && blockIdx.x == 0;
-            }
-            __syncthreads();
         }
     }
     static __device__ __forceinline__ Raw nothing(int t) { return P::fill(t == 1 ? kept<FORM>() : 0.f); }
@@ -325,8 +353,9 @@ struct Feed {
     // bounded wait for what is still on its way, after a wait that gave up; tells the host
     __device__ __forceinline__ void leave(int* host_flag) {
         if (threadIdx.x != 0 || !*abort) return;
-        for (int j = max(0, ordered - stages); j < ordered; ++j)
-            for (int n = 0; n < kTcWaitLimit / 32 && !mbar_try_wait32(bars + 8 * (j % stages), (j / stages) & 1); ++n) {}
+        if constexpr (TMA)
+            for (int j = max(0, ordered - stages); j < ordered; ++j)
+                for (int n = 0; n < kTcWaitLimit / 32 && !mbar_try_wait32(bars + 8 * (j % stages), (j / stages) & 1); ++n) {}
         if (host_flag) *reinterpret_cast<volatile int*>(host_flag) = 1;
     }
 };
@@ -341,10 +370,13 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
     extern __shared__ __align__(128) char ring[];
     const Place<VEC, LANES> w(p);
     cg::cluster_group cluster = cg::this_cluster();
-    if (w.ctas > 1) cluster.barrier_arrive();             // (all have begun before one writes to another)
     const int tile = w.runs * L, stride = w.ctas * tile;
     float* const smem = reinterpret_cast<float*>(ring + (TMA ? p.stages * (size_t)2 * tile * width * sizeof(T) : 0));
-    Feed<T, VEC, FORM, L, LANES, 2, TMA> feed(p, w, ring, reinterpret_cast<char*>(smem + 2 * width * (w.warps * 3 + (w.ctas > 1 ? w.ctas * 3 : 0))));
+    const Waits waits(p, reinterpret_cast<char*>(smem + 2 * width * (w.warps * 3 + (w.ctas > 1 ? w.ctas * 3 : 0))));
+    if (w.ctas > 1) cluster.barrier_arrive();             // (all have begun, their barriers too, before one writes to another)
+    Feed<T, VEC, FORM, L, LANES, 2, TMA> feed(p, w, ring, waits);
+    const uint32_t join_bytes = (uint32_t)w.ctas * 3 * width * sizeof(float);
+    int turn = 0;
     const T* const x = static_cast<const T*>(p.x) + w.b * p.xb + w.c;
     const T* const g = static_cast<const T*>(p.gate) + w.b * p.gb + w.c;
     T* const y = static_cast<T*>(p.y) + (long long)w.b * p.T * p.C + w.c;
@@ -419,19 +451,17 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
                     sum = next.apply(sum, take<VEC>(adds + k * width));
                     whole.times(next);
                 }
-                for (int k = 0; k < w.ctas; ++k) {
-                    float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
-                    give2(to + 2 * w.at, whole.hi, whole.lo);
-                    give(to + 2 * width + w.at, sum);
-                }
+                const float* const to = tiles + w.rank * 3 * width;
+                for (int k = 0; k < w.ctas; ++k) waits.send<VEC>(k, to + 2 * w.at, to + 2 * width + w.at, whole, sum, turn & 1);
             }
-            cluster_meet(threadIdx.x < LANES);
+            if (!waits.joined(turn++, join_bytes)) ok = false;
             h = carry;
             for (int k = 0; k < w.ctas; ++k) {
                 if (k == w.rank) h = carry;
                 const Two<VEC> s = take2<VEC>(tiles + k * 3 * width + 2 * w.at);
                 carry = Step<VEC>{s.a, s.b}.apply(carry, take<VEC>(tiles + k * 3 * width + 2 * width + w.at));
             }
+            if (!ok) carry = N::all(__int_as_float(0x7fc00000));
         } else {
             h = carry;
         }
@@ -468,7 +498,8 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
             }
         }
     }
-    if constexpr (TMA) feed.leave(p.host_flag);
+    feed.leave(p.host_flag);
+    if (w.ctas > 1) cluster.sync();                       // (none leaves while another may still write to it)
     if (!w.mine) return;
     for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) *reinterpret_cast<Raw*>(y + t * p.C) = P::fill(0.f);
     if (p.state_out && w.rank == 0 && w.run == 0) store_state<VEC>(p.state_out + (long long)w.b * p.C + w.c, carry);
@@ -486,10 +517,13 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
     extern __shared__ __align__(128) char ring[];
     const Place<VEC, LANES> w(p);
     cg::cluster_group cluster = cg::this_cluster();
-    if (w.ctas > 1) cluster.barrier_arrive();
     const int tile = w.runs * L, stride = w.ctas * tile;
     float* const smem = reinterpret_cast<float*>(ring + (TMA ? p.stages * (size_t)3 * tile * width * sizeof(T) : 0));
-    Feed<T, VEC, FORM, L, LANES, 3, TMA> feed(p, w, ring, reinterpret_cast<char*>(smem + 2 * width * (w.warps * 4 + (w.ctas > 1 ? w.ctas * 3 : 0))));
+    const Waits waits(p, reinterpret_cast<char*>(smem + 2 * width * (w.warps * 4 + (w.ctas > 1 ? w.ctas * 3 : 0))));
+    if (w.ctas > 1) cluster.barrier_arrive();             // (all have begun, their barriers too, before one writes to another)
+    Feed<T, VEC, FORM, L, LANES, 3, TMA> feed(p, w, ring, waits);
+    const uint32_t join_bytes = (uint32_t)w.ctas * 3 * width * sizeof(float);
+    int turn = 0;
     const T* const x = static_cast<const T*>(p.x) + w.b * p.xb + w.c;
     const T* const g = static_cast<const T*>(p.gate) + w.b * p.gb + w.c;
     const T* const dy = static_cast<const T*>(p.dy) + w.b * p.db + w.c;
@@ -591,19 +625,17 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
                     sum = next.apply(sum, take<VEC>(adds + 2 * k * width + VEC));
                     whole.times(next);
                 }
-                for (int k = 0; k < w.ctas; ++k) {
-                    float* const to = cluster.map_shared_rank(tiles, k) + w.rank * 3 * width;
-                    give2(to + 2 * w.at, whole.hi, whole.lo);
-                    give(to + 2 * width + w.at, sum);
-                }
+                const float* const to = tiles + w.rank * 3 * width;
+                for (int k = 0; k < w.ctas; ++k) waits.send<VEC>(k, to + 2 * w.at, to + 2 * width + w.at, whole, sum, turn & 1);
             }
-            cluster_meet(threadIdx.x < LANES);
+            if (!waits.joined(turn++, join_bytes)) ok = false;
             R = carry;
             for (int k = w.ctas - 1; k >= 0; --k) {
                 if (k == w.rank) R = carry;
                 const Two<VEC> s = take2<VEC>(tiles + k * 3 * width + 2 * w.at);
                 carry = Step<VEC>{s.a, s.b}.apply(carry, take<VEC>(tiles + k * 3 * width + 2 * width + w.at));
             }
+            if (!ok) carry = nan;
         } else {
             R = carry;
         }
@@ -648,7 +680,8 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         else write(std::false_type{});
         if constexpr (TMA) feed.next();
     }
-    if constexpr (TMA) feed.leave(p.host_flag);
+    feed.leave(p.host_flag);
+    if (w.ctas > 1) cluster.sync();                       // (none leaves while another may still write to it)
     if (!w.mine) return;
     for (long long t = (long long)w.len + w.rank * w.runs + w.run; t < p.T; t += w.ctas * w.runs) {
         *reinterpret_cast<Raw*>(dx + t * p.C) = P::fill(0.f);
@@ -756,7 +789,6 @@ template <int TENSORS, typename F>
 static int with_recur(const m2d_recur_desc* d, RecurArgs& a, int vec, int fed, int plain, F fn) {
     const int es = d->dtype == M2D_F32 ? 4 : 2;
     RecurMaps maps{};
-    a.give_up = (d->flags & M2D_RECUR_TEST_GIVE_UP) != 0;
     if (vec == 2 && recur_fits(d, d->x, es) && recur_fits(d, d->gate, es) && (TENSORS == 2 || recur_fits(d, d->d_y, es)) && tc_encoder()) {
         const RecurPlan pl = plan_recur(d, vec, fed, TENSORS == 3);
         const int width = pl.lanes * vec, tile = pl.warps * (32 / pl.lanes) * fed;
@@ -768,11 +800,13 @@ static int with_recur(const m2d_recur_desc* d, RecurArgs& a, int vec, int fed, i
         if ((long long)tile * pl.ctas < d->T && a.stages >= 2 && recur_map(&maps.x, d, d->x, es, width, a.box) && recur_map(&maps.gate, d, d->gate, es, width, a.box) &&
             (TENSORS == 2 || recur_map(&maps.dy, d, d->d_y, es, width, a.box))) {
             a.host_flag = wait_failure_flag();
+            a.give_up = (d->flags & M2D_RECUR_TEST_GIVE_UP) != 0;
             return fn(pl, true, maps, used + a.stages * stage);
         }
     }
     const RecurPlan pl = plan_recur(d, vec, plain, TENSORS == 3);
-    return fn(pl, false, maps, recur_joins(TENSORS + 1, pl.warps, pl.ctas, pl.lanes * vec));
+    a.host_flag = pl.ctas > 1 ? wait_failure_flag() : nullptr;
+    return fn(pl, false, maps, recur_joins(TENSORS + 1, pl.warps, pl.ctas, pl.lanes * vec) + kRecurTail);
 }
 template <typename K>
 static int launch_recur(K kern, const RecurArgs& a, const RecurMaps& maps, const RecurPlan& pl, size_t smem, cudaStream_t st) {
