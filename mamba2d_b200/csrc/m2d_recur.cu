@@ -80,8 +80,23 @@ __device__ __forceinline__ float most(float a, float b) {          // a NaN stay
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// a = exp(gate), or f = sigmoid(gate) and 1 - f, each to its own precision: e = exp(-gate), f = 1 / (1 + e), 1 - f = e f.  Gates below -87 count
-// as -87, whose f is 1.6e-38, so that e stays finite.
+// A gate as it is in memory.  Forget gates below -87 count as -87, whose f is 1.6e-38, so that exp(-gate) stays finite.
+template <typename T, int VEC, int FORM>
+__device__ __forceinline__ Num<VEC> gate_of(typename Piece<T, VEC>::Raw r) {
+    using P = Piece<T, VEC>;
+    if constexpr (FORM == M2D_GATE_DECAY) {
+        return P::get(r);
+    } else if constexpr (sizeof(T) == 2 && VEC == 2) {
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0xc2aec2aeu));
+        return P::get(r);
+    } else {
+        Num<VEC> g = P::get(r);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) g.set(v, most(g.get(v), -87.f));
+        return g;
+    }
+}
+// a = exp(gate), or f = sigmoid(gate) and 1 - f, each to its own precision: e = exp(-gate), f = 1 / (1 + e), 1 - f = e f.
 template <int FORM, int VEC>
 __device__ __forceinline__ void open_gate(Num<VEC> g, Num<VEC>& a, Num<VEC>& rest) {
     if constexpr (FORM == M2D_GATE_DECAY) {
@@ -90,10 +105,7 @@ __device__ __forceinline__ void open_gate(Num<VEC> g, Num<VEC>& a, Num<VEC>& res
         for (int v = 0; v < VEC; ++v) a.set(v, ex2(s.get(v)));
         rest = Num<VEC>::all(1.f);
     } else {
-        Num<VEC> e;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) e.set(v, most(g.get(v), -87.f));
-        e = mul_(e, Num<VEC>::all(-kLog2e));
+        Num<VEC> e = mul_(g, Num<VEC>::all(-kLog2e));
 #pragma unroll
         for (int v = 0; v < VEC; ++v) e.set(v, ex2(e.get(v)));
         const Num<VEC> d = add_(e, Num<VEC>::all(1.f));
@@ -113,7 +125,8 @@ struct Step {
         hi = p;
     }
 };
-// The same for a run of tokens, collected token by token: the sum of the gates, or the product of f and the sum that is 1 - A.
+// The same for a run of tokens, collected token by token: the sum of the gates, or the product of f and the sum that is 1 - A (every token takes
+// its 1 - f of what those before it left).
 template <int FORM, int VEC>
 struct Collect {
     using N = Num<VEC>;
@@ -122,8 +135,8 @@ struct Collect {
         if constexpr (FORM == M2D_GATE_DECAY) {
             s = add_(s, g);
         } else {
+            s = fma_(rest, p, s);
             p = mul_(p, a);
-            s = fma_(neg_(s), rest, add_(s, rest));
         }
     }
     __device__ __forceinline__ Step<VEC> done() const {
@@ -418,7 +431,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
         Collect<FORM, VEC> all;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const N gate = P::get(feed.raw(1, i)), x = P::get(feed.raw(0, i));
+            const N gate = gate_of<T, VEC, FORM>(feed.raw(1, i)), x = P::get(feed.raw(0, i));
             N rest;
             open_gate<FORM, VEC>(gate, a[i], rest);
             u[i] = FORM == M2D_GATE_DECAY ? x : mul_(rest, x);
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         Collect<FORM, VEC> all;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const N gate = P::get(feed.raw(1, i));
+            const N gate = gate_of<T, VEC, FORM>(feed.raw(1, i));
             if constexpr (!TMA) {
                 xs[i] = P::get(feed.raw(0, i));
                 ds[i] = P::get(feed.raw(2, i));
@@ -699,7 +712,7 @@ __global__ void __launch_bounds__(128) recur_step_kernel(const RecurArgs p, long
     if (c >= p.C) return;
     for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
         using N = Num<VEC>;
-        const N x = P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.x) + b * p.xb + c)), g = P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.gate) + b * p.gb + c));
+        const N x = P::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.x) + b * p.xb + c)), g = gate_of<T, VEC, FORM>(*reinterpret_cast<const Raw*>(static_cast<const T*>(p.gate) + b * p.gb + c));
         N a, rest;
         open_gate<FORM, VEC>(g, a, rest);
         const N h = fma_(a, load_state<VEC>(p.state + b * sb + c, true), FORM == M2D_GATE_DECAY ? x : mul_(rest, x));
