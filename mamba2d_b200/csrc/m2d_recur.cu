@@ -258,19 +258,35 @@ inline size_t recur_joins(int parts, int warps, int ctas, int width) { return si
 inline size_t recur_stage(int tensors, int tile, int width, int es) { return (size_t)tensors * tile * width * es; }
 constexpr size_t kRecurTail = (kRecurStages + 3) * 8;
 
-// Barriers and the abort word of a CTA.  A tile's join reaches every CTA of the cluster by stores that count towards the receiver's barrier:
-// nothing else is waited for.  All waits are bounded; where one gives up, what depends on it is NaN.
+// Waits for a barrier's phase, so many times 32 tries of a microsecond or more; gives up and tells so in *abort, or where that has been told.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* abort) {
+    for (int n = 0; n < limit; ++n) {
+        if (mbar_try_wait32(bar, parity)) return true;
+        if (*abort) return false;
+    }
+    *abort = 1;
+    return false;
+}
+// For a copy about a second; for other CTAs' joins four times that, since one of them may be giving up a copy.
+constexpr int kCopyLimit = 1 << 13, kJoinLimit = 1 << 15;
+
+// Barriers and the abort words of a CTA.  A tile's join reaches every CTA of the cluster by stores that count towards the receiver's barrier:
+// nothing else is waited for.  All waits are bounded; where one gives up, what depends on it is NaN.  A CTA that has given up a copy asks for no more
+// of them, but goes on joining and sending (NaN) like all others: the joins' barriers are armed once a phase, whatever happens to copies.  One that has given up
+// a join arms, waits and sends no more, and the others run out of its joins a tile later.
 struct Waits {
     uint32_t stage_bars, join_bars;
-    volatile int* abort;
+    volatile int *abort, *apart;              // a copy was given up; a join was
     __device__ __forceinline__ Waits(const RecurArgs& p, char* tail) {
         stage_bars = smem_u32(tail);
         join_bars = stage_bars + 8 * kRecurStages;
         abort = reinterpret_cast<volatile int*>(tail + 8 * (kRecurStages + 2));
+        apart = abort + 1;
         if (threadIdx.x == 0) {
             for (int k = 0; k < kRecurStages + 2; ++k) mbar_init(stage_bars + 8 * k, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             *abort = p.give_up && blockIdx.x == 0;
+            *apart = 0;
         }
         __syncthreads();
     }
@@ -294,8 +310,9 @@ struct Waits {
     // all CTAs' joins are there; `turn` counts the tiles
     __device__ __forceinline__ bool joined(int turn, uint32_t bytes) const {
         const uint32_t bar = join_bars + 8 * (turn & 1);
+        if (*apart) return false;
         if (threadIdx.x == 0) mbar_expect_tx(bar, bytes);
-        return mbar_wait(bar, (turn >> 1) & 1, abort);
+        return wait_for(bar, (turn >> 1) & 1, kJoinLimit, apart);
     }
 };
 
@@ -309,12 +326,13 @@ struct Feed {
     Raw reg[TMA ? 1 : TENSORS][TMA ? 1 : L];
     char* ring;
     uint32_t bars;
-    volatile int* abort;
+    volatile int *abort, *apart;
     int stage, stages, tile, box, at, run, ordered;
     unsigned parity;
     template <typename W>
     __device__ __forceinline__ Feed(const RecurArgs& p, const W& w, char* smem, const Waits& waits) {
         abort = waits.abort;
+        apart = waits.apart;
         if constexpr (TMA) {
             ring = smem;
             bars = waits.stage_bars;
@@ -347,7 +365,7 @@ struct Feed {
     __device__ __forceinline__ Raw* place(int t, int i) const { return reinterpret_cast<Raw*>(ring + (((size_t)(stage * TENSORS + t) * tile + run * L + i) * width + at) * sizeof(T)); }
     // false: gave up.  n: tokens that there are of the thread's run; the others' places get what changes nothing.
     __device__ __forceinline__ bool ready(int n) {
-        if (!mbar_wait(bars + 8 * stage, parity, abort)) return false;
+        if (!wait_for(bars + 8 * stage, parity, kCopyLimit, abort)) return false;
         if (n < L) {
 #pragma unroll
             for (int t = 0; t < TENSORS; ++t)
@@ -365,10 +383,10 @@ struct Feed {
     }
     // bounded wait for what is still on its way, after a wait that gave up; tells the host
     __device__ __forceinline__ void leave(int* host_flag) {
-        if (threadIdx.x != 0 || !*abort) return;
+        if (threadIdx.x != 0 || !(*abort || *apart)) return;
         if constexpr (TMA)
             for (int j = max(0, ordered - stages); j < ordered; ++j)
-                for (int n = 0; n < kTcWaitLimit / 32 && !mbar_try_wait32(bars + 8 * (j % stages), (j / stages) & 1); ++n) {}
+                for (int n = 0; n < kCopyLimit && !mbar_try_wait32(bars + 8 * (j % stages), (j / stages) & 1); ++n) {}
         if (host_flag) *reinterpret_cast<volatile int*>(host_flag) = 1;
     }
 };
@@ -454,7 +472,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
         if (w.ctas > 1) {
             // one warp joins the tile's runs and tells every CTA of the cluster
             float* const tiles = cluster_part + (size_t)buf * w.ctas * 3 * width;
-            if (threadIdx.x < LANES) {
+            if (threadIdx.x < LANES && !*waits.apart) {
                 Step<VEC> whole{N::all(1.f), N::all(0.f)};
                 N sum = N::all(0.f);
 #pragma unroll 8
@@ -628,7 +646,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         };
         if (w.ctas > 1) {
             float* const tiles = cluster_part + (size_t)buf * w.ctas * 3 * width;
-            if (threadIdx.x < LANES) {
+            if (threadIdx.x < LANES && !*waits.apart) {
                 Step<VEC> whole{N::all(1.f), N::all(0.f)};
                 N sum = N::all(0.f);
 #pragma unroll 8
@@ -761,12 +779,21 @@ static int for_recur(const m2d_recur_desc* d, bool pairs, F fn) {
 }
 // Lanes of a row, warps of a CTA and CTAs of a cluster: the least time by a model of it.  An SM holds 16 warps (128 registers a
 // thread); clusters of 4 and 8 leave some SMs of a GPC over (of CTAs of 16 warps 33 and 15 fit 148 SMs, of 8 warps 71 and 33).  All clusters run in so many waves, and each takes so many
-// strides; a stride takes about a time of 10 for its chain of load, joins and store and 1 for each warp of the SM (its instructions).
+// strides; a stride takes about a time of 10 for its chain of load, joins and store and 1 for each warp of the SM (its instructions), the start of a wave 30
+// (some 3 us).
 // Rows in pieces of 16 or 8 lanes (64 and 32 bytes of bf16), larger clusters and CTAs that have an SM for themselves cost a little more.
 struct RecurPlan { int lanes, warps, ctas; };
-static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, bool bwd) {
+// Tiles that a CTA's share of an SM's memory has room for, beside the joins.
+static int recur_stages(const RecurPlan& pl, int vec, int steps, int tensors, int es) {
+    const int width = pl.lanes * vec, tile = pl.warps * (32 / pl.lanes) * steps;
+    const size_t used = recur_joins(tensors + 1, pl.warps, pl.ctas, width) + kRecurTail, share = pl.warps > 8 ? kMaxSmem : kMaxSmem * pl.warps / kRecurWarps - 512;
+    return share > used ? (int)std::min<size_t>(kRecurStages, (share - used) / recur_stage(tensors, tile, width, es)) : 0;
+}
+// By TMA (fed) there is room for the tile, and for two where there are several strides.
+static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, int tensors, bool fed) {
     const long long runs = (d->T + steps - 1) / steps, sms = sm_count();
-    RecurPlan best{32, 1, 1};
+    const bool bwd = tensors == 3;
+    RecurPlan best{32, 0, 1};
     double least = 1e300;
     for (int lanes = 32; lanes >= (vec == 2 ? 8 : 32); lanes /= 2) {
         const long long chains = (long long)d->B * ((d->C + lanes * vec - 1) / (lanes * vec));
@@ -775,11 +802,12 @@ static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, bool bw
                 const long long tile = (long long)warps * (32 / lanes);            // in runs
                 if (ctas > 1 && tile * (ctas / 2) >= runs) break;                  // (half of them would do)
                 if (bwd && tile * steps % kMark && (ctas > 1 || tile < runs)) continue;        // (a tile begins at a mark)
+                if (fed && recur_stages({lanes, warps, ctas}, vec, steps, tensors, d->dtype == M2D_F32 ? 4 : 2) < (tile * ctas < runs ? 2 : 1)) continue;
                 const long long eights = (ctas == 8 ? 33 : ctas == 4 ? 71 : 296 / ctas) * sms / 148;            // clusters of CTAs of eight warps
                 const long long held = std::max(1ll, warps == 16 ? (ctas == 8 ? 15 : ctas == 4 ? 33 : 148 / ctas) * sms / 148 : eights * 8 / warps);
                 const long long waves = (chains + held - 1) / held, strides = (runs + tile * ctas - 1) / (tile * ctas);
                 const long long per_sm = std::min<long long>(kRecurWarps, (chains * ctas + sms - 1) / sms * warps);
-                const double t = (double)(waves * strides) * (10 + per_sm) * (warps == 16 ? 1.1 : 1.0) * (lanes == 32 ? 1.0 : lanes == 16 ? 1.05 : 1.15) * (ctas == 1 ? 1.0 : 1.1 + 0.02 * ctas);
+                const double t = (double)waves * (30 + strides * (10 + per_sm)) * (warps == 16 ? 1.1 : 1.0) * (lanes == 32 ? 1.0 : lanes == 16 ? 1.05 : 1.15) * (ctas == 1 ? 1.0 : 1.1 + 0.02 * ctas);
                 if (t < least) { least = t; best = {lanes, warps, ctas}; }
             }
     }
@@ -803,21 +831,19 @@ static int with_recur(const m2d_recur_desc* d, RecurArgs& a, int vec, int fed, i
     const int es = d->dtype == M2D_F32 ? 4 : 2;
     RecurMaps maps{};
     if (vec == 2 && recur_fits(d, d->x, es) && recur_fits(d, d->gate, es) && (TENSORS == 2 || recur_fits(d, d->d_y, es)) && tc_encoder()) {
-        const RecurPlan pl = plan_recur(d, vec, fed, TENSORS == 3);
+        const RecurPlan pl = plan_recur(d, vec, fed, TENSORS, true);
         const int width = pl.lanes * vec, tile = pl.warps * (32 / pl.lanes) * fed;
-        // more than one stride, and two stages or more in the CTA's share of an SM's memory
-        const size_t joins = recur_joins(TENSORS + 1, pl.warps, pl.ctas, width), used = joins + kRecurTail, stage = recur_stage(TENSORS, tile, width, es);
-        const size_t share = pl.warps > 8 ? kMaxSmem : kMaxSmem * pl.warps / kRecurWarps - 512;
-        a.stages = share > used ? (int)std::min<size_t>(kRecurStages, (share - used) / stage) : 0;
+        a.stages = pl.warps ? recur_stages(pl, vec, fed, TENSORS, es) : 0;
         a.box = std::min(tile, 256);
-        if ((long long)tile * pl.ctas < d->T && a.stages >= 2 && recur_map(&maps.x, d, d->x, es, width, a.box) && recur_map(&maps.gate, d, d->gate, es, width, a.box) &&
-            (TENSORS == 2 || recur_map(&maps.dy, d, d->d_y, es, width, a.box))) {
+        // forward a single stride takes as long without; backward the form by TMA needs fewer registers (25x2010x192 bf16 32 us for 54)
+        if (a.stages && ((long long)tile * pl.ctas < d->T || (TENSORS == 3 && d->T >= kMark)) && recur_map(&maps.x, d, d->x, es, width, a.box) &&
+            recur_map(&maps.gate, d, d->gate, es, width, a.box) && (TENSORS == 2 || recur_map(&maps.dy, d, d->d_y, es, width, a.box))) {
             a.host_flag = wait_failure_flag();
             a.give_up = (d->flags & M2D_RECUR_TEST_GIVE_UP) != 0;
-            return fn(pl, true, maps, used + a.stages * stage);
+            return fn(pl, true, maps, recur_joins(TENSORS + 1, pl.warps, pl.ctas, width) + kRecurTail + a.stages * recur_stage(TENSORS, tile, width, es));
         }
     }
-    const RecurPlan pl = plan_recur(d, vec, plain, TENSORS == 3);
+    const RecurPlan pl = plan_recur(d, vec, plain, TENSORS, false);
     a.host_flag = pl.ctas > 1 ? wait_failure_flag() : nullptr;
     return fn(pl, false, maps, recur_joins(TENSORS + 1, pl.warps, pl.ctas, pl.lanes * vec) + kRecurTail);
 }

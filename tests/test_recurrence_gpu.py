@@ -258,11 +258,12 @@ def test_long_sequences(B, T, C, dt, form, ragged):
     assert torch.equal(again, out[0])
 
 
-def test_a_wait_that_gives_up(monkeypatch):
-    """The first CTA asks for nothing: its results are NaN, and those of tokens behind its own, the next call raises, and the one after is right."""
+@pytest.mark.parametrize("B,T,C", [(2, 30000, 128), (64, 3000, 512)])
+def test_a_wait_that_gives_up(monkeypatch, B, T, C):
+    """The first CTA asks for nothing: its results are NaN, and those of tokens behind its own, the next call raises, and the one after is right.
+    Sequences of several CTAs and of one."""
     monkeypatch.setenv("M2D_TEST_HOOKS", "1")
     L = _lib.lib()
-    B, T, C = 2, 30000, 128             # (several strides)
     x, g, s, dy, ds = inputs(B, T, C, BF, "decay", 10, True)
     want, last = gated_recurrence(x, g, initial_state=s, return_state=True)
     y, out, marks = torch.empty_like(x), torch.empty_like(s), torch.zeros(B, -(-T // 64), C, device="cuda")
