@@ -39,6 +39,7 @@ constexpr int kRowWarps = 4;           // rows of a CTA whose warps work on one 
 template <typename T> struct Vec16;    // 16 bytes
 template <> struct Vec16<float> {
     static constexpr int n = 4;
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }       // -inf: adds nothing
     static __device__ __forceinline__ void get(const uint4& r, Num<2>* v) { v[0] = Num<2>::make(__uint_as_float(r.x), __uint_as_float(r.y)); v[1] = Num<2>::make(__uint_as_float(r.z), __uint_as_float(r.w)); }
     static __device__ __forceinline__ uint4 put(const Num<2>* v) {
         return make_uint4(__float_as_uint(v[0].get(0)), __float_as_uint(v[0].get(1)), __float_as_uint(v[1].get(0)), __float_as_uint(v[1].get(1)));
@@ -49,6 +50,7 @@ template <> struct Vec16<float> {
 };
 template <> struct Vec16<__nv_bfloat16> {
     static constexpr int n = 8;
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
     static __device__ __forceinline__ void get(const uint4& r, Num<2>* v) {
         const unsigned u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -212,11 +214,13 @@ template <typename T, int MODE>
 __device__ __forceinline__ void read_pieces(const uint4* body, int first, int step, int end, float c, float c1, Running<MODE>& r) {
     using W = Vec16<T>;
     constexpr int U = 4;
-    int i = first;
-    for (; i < end - (U - 1) * step; i += U * step) {
+    auto batch = [&](int i, auto whole) {
         uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = __ldcs(body + i + u * step);
+        for (int u = 0; u < U; ++u) {
+            if (!whole.value) raw[u] = W::none();
+            if (whole.value || i + u * step < end) raw[u] = __ldcs(body + i + u * step);
+        }
         float top = r.m;
 #pragma unroll
         for (int u = 0; u < U; ++u) top = W::most(raw[u], top);
@@ -228,15 +232,10 @@ __device__ __forceinline__ void read_pieces(const uint4* body, int first, int st
 #pragma unroll
             for (int k = 0; k < W::n / 2; ++k) r.add(v[k], c, c1);
         }
-    }
-    for (; i < end; i += step) {
-        const uint4 raw = __ldcs(body + i);
-        r.raise(W::most(raw, r.m), c, c1);
-        Num<2> v[W::n / 2];
-        W::get(raw, v);
-#pragma unroll
-        for (int k = 0; k < W::n / 2; ++k) r.add(v[k], c, c1);
-    }
+    };
+    int i = first;
+    for (; i < end - (U - 1) * step; i += U * step) batch(i, std::true_type{});
+    if (i < end) batch(i, std::false_type{});
 }
 // A row's head and tail, by threads of which this is number `me`.
 template <typename T, int MODE>
@@ -295,9 +294,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) distill_join_kernel(const Dist
     const int lane = threadIdx.x & 31;
     // (inputs: written before the launch that this one follows)
     const T* const z = static_cast<const T*>(p.z) + row * p.zp;
-    const Taught t = teach(p, row, z);
     const int label = label_of(p, row);
     const float at_label = label >= 0 ? number(z + label) : 0.f;
+    const Taught t = teach(p, row, z);
     follow_wait();
     const long long total = p.N * p.pieces;
     // the CTAs of its first piece and of its last: k total / n <= piece < (k + 1) total / n
@@ -470,8 +469,12 @@ static DistillArgs distill_args(const m2d_distill_desc* d) {
     a.c1 = kLog2e; a.c = (float)(1.4426950408889634 / (double)d->temperature);
     return a;
 }
-// A warp for a row of up to 8 KB: a CTA's threads would have two loads each at most.
-static bool short_rows(const m2d_distill_desc* d) { return (long long)d->V * (d->dtype == M2D_F32 ? 4 : 2) <= 8192; }
+// A warp for a row of up to 8 KB, whose loads would be two of a CTA's threads at most, and of up to 32 KB where rows are enough to fill the
+// GPU with warps (7361x7552 bf16, forward and backward: 100 us, by CTAs 150).
+static bool short_rows(const m2d_distill_desc* d) {
+    const long long bytes = (long long)d->V * (d->dtype == M2D_F32 ? 4 : 2);
+    return bytes <= 8192 || (bytes <= 32768 && d->N >= 24ll * sm_count());
+}
 template <typename F>
 static int for_distill(const m2d_distill_desc* d, F fn) {
     using std::integral_constant;
