@@ -781,7 +781,8 @@ static int for_recur(const m2d_recur_desc* d, bool pairs, F fn) {
 // thread); clusters of 4 and 8 leave some SMs of a GPC over (of CTAs of 16 warps 33 and 15 fit 148 SMs, of 8 warps 71 and 33).  All clusters run in so many waves, and each takes so many
 // strides; a stride takes about a time of 10 for its chain of load, joins and store and 1 for each warp of the SM (its instructions), the start of a wave 30
 // (some 3 us).
-// Rows in pieces of 16 or 8 lanes (64 and 32 bytes of bf16), larger clusters and CTAs that have an SM for themselves cost a little more.
+// Rows in pieces of 16 or 8 lanes (64 and 32 bytes of bf16), larger clusters and CTAs that have an SM for themselves cost a little more; the
+// backward pass without TMA spills registers there and takes twice as long.
 struct RecurPlan { int lanes, warps, ctas; };
 // Tiles that a CTA's share of an SM's memory has room for, beside the joins.
 static int recur_stages(const RecurPlan& pl, int vec, int steps, int tensors, int es) {
@@ -807,7 +808,7 @@ static RecurPlan plan_recur(const m2d_recur_desc* d, int vec, int steps, int ten
                 const long long held = std::max(1ll, warps == 16 ? (ctas == 8 ? 15 : ctas == 4 ? 33 : 148 / ctas) * sms / 148 : eights * 8 / warps);
                 const long long waves = (chains + held - 1) / held, strides = (runs + tile * ctas - 1) / (tile * ctas);
                 const long long per_sm = std::min<long long>(kRecurWarps, (chains * ctas + sms - 1) / sms * warps);
-                const double t = (double)waves * (30 + strides * (10 + per_sm)) * (warps == 16 ? 1.1 : 1.0) * (lanes == 32 ? 1.0 : lanes == 16 ? 1.05 : 1.15) * (ctas == 1 ? 1.0 : 1.1 + 0.02 * ctas);
+                const double t = (double)waves * (30 + strides * (10 + per_sm)) * (warps == 16 ? 1.1 : 1.0) * (lanes == 32 ? 1.0 : bwd && !fed ? 2.0 : lanes == 16 ? 1.05 : 1.15) * (ctas == 1 ? 1.0 : 1.1 + 0.02 * ctas);
                 if (t < least) { least = t; best = {lanes, warps, ctas}; }
             }
     }
