@@ -21,7 +21,7 @@ struct LnArgs {
     float2* stats;                     // mean, rstd of each row
     float* partial;                    // [CTAs][2][C]
     long long N;
-    int C, params_f32, parts;
+    int C, params_f32, parts, stages;  // stages: rows on their way, where those are not whole pieces
     float eps;
 };
 
@@ -137,45 +137,101 @@ struct Share {
     __device__ __forceinline__ bool more(long long N, long long at) const { return at - (R ? threadIdx.x / lanes : 0) < N; }
 };
 
-// Rows on their way: whole pieces through shared memory, two or three rows ahead, each thread its own pieces (nobody else looks at
-// them); single values in registers, one row ahead.  What is wanted are 40 KB and more of an SM under way, which registers have no room for.
+// Rows on their way, through shared memory: what is wanted are 40 KB and more of an SM under way, which registers have no room for.
+// Whole pieces (V > 1): each thread its own, two or three rows ahead; nobody else looks at them.  Others: the 16-byte pieces that a row touches, by all of
+// its lanes, one to three rows ahead, as they have room; a value is then where it lies in them.
 template <typename T, int V, int R, int NV, int TENSORS>
 struct Rows {
     using Raw = typename Lane<T, V>::Raw;
-    static constexpr bool ring = V > 1;
-    static constexpr int room = 224 * 1024 / (TENSORS * NV * 16 * (R ? kLnThreads : 512)), ahead = !ring ? 1 : room < 3 ? room : 3;
-    static constexpr size_t bytes(int threads) { return ring ? (size_t)ahead * TENSORS * NV * threads * 16 : 0; }
-    Raw reg[ring ? 1 : TENSORS][ring ? 1 : NV];
-    unsigned base, slot;
-    __device__ __forceinline__ Rows(void* smem) { base = smem_u32(smem) + threadIdx.x * 16; slot = 0; }
-    __device__ __forceinline__ unsigned place(int t, int i) const { return base + ((slot * TENSORS + t) * NV + i) * blockDim.x * 16; }
-    // piece i of tensor t, if `on`; then done() once a row
-    __device__ __forceinline__ void fetch(int t, int i, const T* p, bool on) {
-        if constexpr (ring) {
-            cp_async16_if(on, place(t, i), p);
+    static constexpr int room = 224 * 1024 / (TENSORS * NV * 16 * (R ? kLnThreads : 512)), fixed = room < 3 ? room : 3;
+    static constexpr int groups = R ? kLnThreads / (R ? R : 1) : 1;            // rows of a CTA at a time
+    static int stages(int C) { return V > 1 ? fixed : (int)std::max<size_t>(1, std::min<size_t>(3, 200 * 1024 / (TENSORS * groups * span_bytes(C)))); }
+    static size_t bytes(int C, int threads) { return V > 1 ? (size_t)fixed * TENSORS * NV * threads * 16 : stages(C) * TENSORS * groups * span_bytes(C); }
+    __host__ __device__ static size_t span_bytes(int C) { return (((size_t)C * sizeof(T) + 15) / 16 + 1) * 16; }
+
+    const T* from[TENSORS];
+    long long pitch[TENSORS];
+    unsigned base, slot, span, off[TENSORS];
+    int C, ahead, l, lanes;
+    template <typename S>
+    __device__ __forceinline__ Rows(void* smem, const S& at, const LnArgs& p) {
+        C = p.C;
+        slot = 0;
+        l = at.l;
+        lanes = at.span;
+        if constexpr (V > 1) {
+            ahead = fixed;
+            base = smem_u32(smem) + threadIdx.x * 16;
         } else {
-            reg[t][i] = Raw{};
-            if (on) reg[t][i] = __ldcs(reinterpret_cast<const Raw*>(p));
+            ahead = p.stages;
+            span = (unsigned)span_bytes(C);
+            base = smem_u32(smem) + (R ? threadIdx.x / (R ? R : 1) : 0) * (unsigned)ahead * TENSORS * span;
         }
     }
-    __device__ __forceinline__ void done() {
-        if constexpr (ring) {
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            slot = slot + 1 == ahead ? 0 : slot + 1;
-        }
+    __device__ __forceinline__ unsigned place(int t, int i) const {
+        if constexpr (V > 1) return base + ((slot * TENSORS + t) * NV + i) * blockDim.x * 16;
+        else return base + (slot * TENSORS + t) * span;
     }
-    // waits for the oldest row on its way; its slot is the next to be filled
-    __device__ __forceinline__ void arrived() {
-        if constexpr (ring) asm volatile("cp.async.wait_group %0;" ::"n"(ahead - 1) : "memory");
+    // asks for a row (an empty one where it is not `on`)
+    __device__ __forceinline__ void order(long long row, bool on) {
+#pragma unroll
+        for (int t = 0; t < TENSORS; ++t) {
+            const T* const p = from[t] + (on ? row : 0) * pitch[t];
+            if constexpr (V > 1) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) cp_async16_if(on && (i * lanes + l) * V < C, place(t, i), p + (i * lanes + l) * V);
+            } else if (on) {
+                const int head = (int)(reinterpret_cast<uintptr_t>(p) & 15), all = head + C * (int)sizeof(T);
+                const char* const q = reinterpret_cast<const char*>(p) - head;
+                for (int j = l * 16; j < all; j += lanes * 16) {
+                    const unsigned to = place(t, 0) + j;
+                    if (q + j >= reinterpret_cast<const char*>(from[t])) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(q + j), "r"(min(16, all - j)) : "memory");
+                    } else {                       // (the piece begins before the tensor)
+                        for (int k = head; k < min(16, all); k += (int)sizeof(T)) {
+                            if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + k), "r"(*reinterpret_cast<const unsigned*>(q + k)) : "memory");
+                            else asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + k), "h"(*reinterpret_cast<const unsigned short*>(q + k)) : "memory");
+                        }
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (++slot == (unsigned)ahead) slot = 0;
+    }
+    static __device__ __forceinline__ void together() {
+        if constexpr (R == 0) __syncthreads();
+        else __syncwarp();
+    }
+    // waits for the oldest row that was asked for; its slot is the next to be filled, after release()
+    __device__ __forceinline__ void arrived(long long row) {
+        if constexpr (V > 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(fixed - 1) : "memory");
+        } else {
+            if (ahead == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+            else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            together();
+#pragma unroll
+            for (int t = 0; t < TENSORS; ++t) off[t] = place(t, 0) + (unsigned)(reinterpret_cast<uintptr_t>(from[t] + row * pitch[t]) & 15);
+        }
     }
     __device__ __forceinline__ Raw take(int t, int i) const {
-        if constexpr (ring) {
+        if constexpr (V > 1) {
             uint4 r;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(place(t, i)) : "memory");
             return *reinterpret_cast<const Raw*>(&r);
         } else {
-            return reg[t][i];
+            const int c = i * lanes + l;
+            Raw r{};
+            if (c >= C) return r;
+            if constexpr (sizeof(T) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(off[t] + c * 4) : "memory");
+            else asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(off[t] + c * 2) : "memory");
+            return r;
         }
+    }
+    __device__ __forceinline__ void release() const {
+        if constexpr (V == 1) together();
     }
 };
 
@@ -193,32 +249,27 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_fwd_kernel(const LnAr
             parameter<T, V>(p.b, p.params_f32, at.column(i), 0.f, b[i]);
         }
     extern __shared__ __align__(16) char smem[];
-    Rows<T, V, R, NV, RES ? 2 : 1> rows(smem);
+    Rows<T, V, R, NV, RES ? 2 : 1> rows(smem, at, p);
+    rows.from[0] = static_cast<const T*>(p.x);
+    rows.pitch[0] = p.xp;
+    if constexpr (RES) {
+        rows.from[1] = static_cast<const T*>(p.r);
+        rows.pitch[1] = p.rp;
+    }
     T lead, lead_r;                         // the next row's first values (as they are: nothing waits for them here)
-    auto load = [&](long long row) {
-        const bool on = row < p.N;
-        const T* const x = static_cast<const T*>(p.x) + (on ? row : 0) * p.xp;
-        const T* const r = RES ? static_cast<const T*>(p.r) + (on ? row : 0) * p.rp : nullptr;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            rows.fetch(0, i, x + at.column(i), on && at.column(i) < p.C);
-            if constexpr (RES) rows.fetch(1, i, r + at.column(i), on && at.column(i) < p.C);
-        }
-        rows.done();
-    };
+    auto load = [&](long long row) { rows.order(row, row < p.N); };
     auto look = [&](long long row) {
         lead = static_cast<const T*>(p.x)[(row < p.N ? row : 0) * p.xp];
         if constexpr (RES) lead_r = static_cast<const T*>(p.r)[(row < p.N ? row : 0) * p.rp];
     };
     int slot = 0;
     long long row = at.row;
-#pragma unroll
     for (int k = 0; k < rows.ahead; ++k) load(row + k * at.step);
     look(row);
     const float per = 1.f / (float)p.C;
     for (; at.more(p.N, row); row += at.step) {
         N v[NV][P::n];
-        rows.arrived();
+        rows.arrived(row < p.N ? row : 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             P::get(rows.take(0, i), v[i]);
@@ -233,6 +284,7 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_fwd_kernel(const LnAr
             }
         }
         const float first = RES ? sum_as<T>(value_of(&lead), value_of(&lead_r)) : value_of(&lead);
+        rows.release();
         load(row + rows.ahead * at.step);
         look(row + at.step);
         N acc = N::all(0.f);
@@ -286,25 +338,20 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
         if (at.column(i) < p.C) parameter<T, V>(p.w, p.params_f32, at.column(i), 1.f, w[i]);
     }
     extern __shared__ __align__(16) char smem[];   // the rows on their way; at the end sums, where parts of warps hold rows: [warps][2][columns of R lanes]
-    Rows<T, V, R, NV, DS ? 3 : 2> rows(smem);
+    Rows<T, V, R, NV, DS ? 3 : 2> rows(smem, at, p);
+    rows.from[0] = static_cast<const T*>(p.x);
+    rows.from[1] = static_cast<const T*>(p.dy);
+    rows.pitch[0] = p.xp;
+    rows.pitch[1] = p.dyp;
+    if constexpr (DS) {
+        rows.from[2] = static_cast<const T*>(p.ds);
+        rows.pitch[2] = p.dsp;
+    }
     float2 st;
-    auto load = [&](long long row) {
-        const bool on = row < p.N;
-        const T *const x = static_cast<const T*>(p.x) + (on ? row : 0) * p.xp, *const dy = static_cast<const T*>(p.dy) + (on ? row : 0) * p.dyp;
-        const T* const ds = DS ? static_cast<const T*>(p.ds) + (on ? row : 0) * p.dsp : nullptr;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool here = on && at.column(i) < p.C;
-            rows.fetch(0, i, x + at.column(i), here);
-            rows.fetch(1, i, dy + at.column(i), here);
-            if constexpr (DS) rows.fetch(2, i, ds + at.column(i), here);
-        }
-        rows.done();
-    };
+    auto load = [&](long long row) { rows.order(row, row < p.N); };
     auto look = [&](long long row) { st = row < p.N ? p.stats[row] : make_float2(0.f, 0.f); };
     int slot = 0;
     long long row = at.row;
-#pragma unroll
     for (int k = 0; k < rows.ahead; ++k) load(row + k * at.step);
     look(row);
     const float per = 1.f / (float)p.C;
@@ -312,7 +359,7 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
         N h[NV][P::n], dh[NV][P::n], s0 = N::all(0.f), s1 = N::all(0.f);
         Raw keep[DS ? NV : 1];
         const N off = N::all(-st.x), scale = N::all(st.y);
-        rows.arrived();
+        rows.arrived(row < p.N ? row : 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             P::get(rows.take(0, i), h[i]);
@@ -320,6 +367,7 @@ __global__ void __launch_bounds__(R ? kLnThreads : 512) ln_bwd_kernel(const LnAr
             if constexpr (DS) keep[i] = rows.take(2, i);
         }
         const float rstd = st.y;
+        rows.release();
         load(row + rows.ahead * at.step);
         look(row + at.step);
         if (row < p.N)
@@ -571,15 +619,16 @@ static int with_ln_bwd(const m2d_ln_desc* d, F fn) {
     const bool params = d->d_weight || d->d_bias;
     if (pl.lanes < 0) {
         const long long grid = ln_grid(d, pl, 2);
-        return d->dtype == M2D_F32 ? fn(ln_long_bwd_kernel<float>, pl, grid, (size_t)0) : fn(ln_long_bwd_kernel<__nv_bfloat16>, pl, grid, (size_t)0);
+        return d->dtype == M2D_F32 ? fn(ln_long_bwd_kernel<float>, pl, grid, (size_t)0, 0) : fn(ln_long_bwd_kernel<__nv_bfloat16>, pl, grid, (size_t)0, 0);
     }
     return for_ln(d, pl, d->d_sum != nullptr, [&](auto elem, auto vec, auto lanes, auto nv, auto ds) {
         auto kern = ln_bwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(ds)::value>;
         constexpr int V = decltype(vec)::value, R = decltype(lanes)::value, NV = decltype(nv)::value;
-        const size_t rows = Rows<decltype(elem), V, R, NV, decltype(ds)::value ? 3 : 2>::bytes(pl.threads), last = R && params ? (size_t)kLnThreads / 32 * 2 * R * NV * V * sizeof(float) : 0;
+        using Way = Rows<decltype(elem), V, R, NV, decltype(ds)::value ? 3 : 2>;
+        const size_t rows = Way::bytes(d->C, pl.threads), last = R && params ? (size_t)kLnThreads / 32 * 2 * R * NV * V * sizeof(float) : 0;
         const size_t smem = std::max(rows, last);
         if (!allow_smem(reinterpret_cast<const void*>(kern), smem + kLnStatic)) return (int)M2D_ERR_LAUNCH;
-        return fn(kern, pl, ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, smem)), smem);
+        return fn(kern, pl, ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, smem)), smem, Way::stages(d->C));
     });
 }
 
@@ -590,7 +639,7 @@ using namespace m2d;
 extern "C" uint64_t m2d_ln_bwd_workspace(const m2d_ln_desc* d) {
     if (check_ln(d) != M2D_OK || (!d->d_weight && !d->d_bias)) return 0;
     uint64_t bytes = 0;
-    with_ln_bwd(d, [&](auto, const LnPlan&, long long grid, size_t) {
+    with_ln_bwd(d, [&](auto, const LnPlan&, long long grid, size_t, int) {
         bytes = (uint64_t)grid * 2 * d->C * sizeof(float);
         return (int)M2D_OK;
     });
@@ -601,7 +650,7 @@ extern "C" int m2d_ln_fwd(const m2d_ln_desc* d, void* stream) {
     const int rc = check_ln(d);
     if (rc != M2D_OK) return rc;
     if (!d->x || !d->y || (d->residual && !d->sum)) return M2D_ERR_NULL;
-    const LnArgs a = ln_args(d);
+    LnArgs a = ln_args(d);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const LnPlan pl = plan_ln(d, false);
     if (pl.lanes < 0) {
@@ -612,7 +661,9 @@ extern "C" int m2d_ln_fwd(const m2d_ln_desc* d, void* stream) {
     }
     return for_ln(d, pl, d->residual != nullptr, [&](auto elem, auto vec, auto lanes, auto nv, auto res) {
         auto kern = ln_fwd_kernel<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(res)::value>;
-        const size_t smem = Rows<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(res)::value ? 2 : 1>::bytes(pl.threads);
+        using Way = Rows<decltype(elem), decltype(vec)::value, decltype(lanes)::value, decltype(nv)::value, decltype(res)::value ? 2 : 1>;
+        const size_t smem = Way::bytes(d->C, pl.threads);
+        a.stages = Way::stages(d->C);
         if (!allow_smem(reinterpret_cast<const void*>(kern), smem + kLnStatic)) return (int)M2D_ERR_LAUNCH;
         kern<<<(unsigned)ln_grid(d, pl, resident_ctas(reinterpret_cast<const void*>(kern), pl.threads, smem)), pl.threads, smem, st>>>(a);
         return cudaGetLastError() == cudaSuccess ? (int)M2D_OK : (int)M2D_ERR_LAUNCH;
@@ -626,10 +677,11 @@ extern "C" int m2d_ln_bwd(const m2d_ln_desc* d, void* stream) {
     LnArgs a = ln_args(d);
     const bool params = d->d_weight || d->d_bias;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int done = with_ln_bwd(d, [&](auto kern, const LnPlan& pl, long long grid, size_t smem) {
+    const int done = with_ln_bwd(d, [&](auto kern, const LnPlan& pl, long long grid, size_t smem, int stages) {
         if (params && (!d->workspace || d->workspace_bytes < (uint64_t)grid * 2 * d->C * sizeof(float) || (reinterpret_cast<uintptr_t>(d->workspace) & 255))) return (int)M2D_ERR_WORKSPACE;
         a.partial = params ? static_cast<float*>(d->workspace) : nullptr;
         a.parts = (int)grid;
+        a.stages = stages;
         kern<<<a.parts, pl.threads, smem, st>>>(a);
         return cudaGetLastError() == cudaSuccess ? (int)M2D_OK : (int)M2D_ERR_LAUNCH;
     });
