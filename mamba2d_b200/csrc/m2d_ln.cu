@@ -575,7 +575,7 @@ static LnPlan plan_ln(const m2d_ln_desc* d, bool bwd) {
         for (int n : {4, 16})
             if (!pl.lanes && d->C <= 32 * n) { pl.lanes = 32; pl.nv = n; }
     if (pl.lanes) return pl;
-    pl.nv = v ? 2 * unit : 16;
+    pl.nv = v ? 2 * unit : d->C <= 4096 ? 8 : 16;         // (single values: fewer a lane leave registers for more warps)
     pl.threads = (d->C + pl.vec * pl.nv * 32 - 1) / (pl.vec * pl.nv * 32) * 32;
     if (pl.threads > 512) { pl.lanes = -1; pl.threads = kLongThreads; }
     return pl;
@@ -592,7 +592,7 @@ static int for_ln(const m2d_ln_desc* d, const LnPlan& pl, bool flag, F fn) {
         constexpr integral_constant<int, 4> four{};
         constexpr integral_constant<int, 16> sixteen{};
         constexpr integral_constant<int, 32> warp{};
-        if (pl.vec == 1) return pl.lanes == 0 ? with(one, cta, sixteen) : pl.nv == 4 ? with(one, warp, four) : with(one, warp, sixteen);
+        if (pl.vec == 1) return pl.lanes == 0 ? (pl.nv == 8 ? with(one, cta, integral_constant<int, 8>{}) : with(one, cta, sixteen)) : pl.nv == 4 ? with(one, warp, four) : with(one, warp, sixteen);
         if (pl.lanes == 0) return with(full, cta, integral_constant<int, 2 * unit>{});
         auto with_lanes = [&](auto lanes) {
             return pl.nv == unit ? with(full, lanes, integral_constant<int, unit>{}) : pl.nv == 2 * unit ? with(full, lanes, integral_constant<int, 2 * unit>{}) : with(full, lanes, integral_constant<int, 3 * unit>{});
