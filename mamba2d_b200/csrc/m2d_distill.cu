@@ -485,7 +485,7 @@ static int for_distill(const m2d_distill_desc* d, F fn) {
     };
     return d->dtype == M2D_F32 ? with(float{}) : with(__nv_bfloat16{});
 }
-// Pieces of 16 KB and all CTAs that the GPU holds; pieces of 4 KB where there are too few of those.
+// Pieces of 16 KB and CTAs as many as the GPU may hold; pieces of 4 KB where there are too few of those.
 struct DistillPlan { int unit, pieces, ctas; };
 static DistillPlan plan_distill(const m2d_distill_desc* d) {
     const int loads = d->V / (d->dtype == M2D_F32 ? 4 : 8);
@@ -526,11 +526,12 @@ extern "C" int m2d_distill_fwd(const m2d_distill_desc* d, void* stream) {
             return cudaGetLastError() == cudaSuccess ? M2D_OK : M2D_ERR_LAUNCH;
         }
         const DistillPlan pl = plan_distill(d);
+        auto kern = pl.unit == 4 ? distill_fwd_kernel<T, MODE, 4> : distill_fwd_kernel<T, MODE, 1>;
+        const long long held = (long long)std::max(1, resident_ctas(reinterpret_cast<const void*>(kern), kRowCta, 0)) * sm_count();
         a.pieces = pl.pieces;
-        a.ctas = pl.ctas;
+        a.ctas = (int)std::min<long long>(pl.ctas, held);            // one wave
         a.found = static_cast<float4*>(d->workspace);
-        if (pl.unit == 4) distill_fwd_kernel<T, MODE, 4><<<pl.ctas, kRowCta, 0, st>>>(a);
-        else distill_fwd_kernel<T, MODE, 1><<<pl.ctas, kRowCta, 0, st>>>(a);
+        kern<<<a.ctas, kRowCta, 0, st>>>(a);
         if (cudaGetLastError() != cudaSuccess || !launch_following(distill_join_kernel<T, MODE>, dim3(warps), dim3(kRowWarps * 32), 0, st, a)) return M2D_ERR_LAUNCH;
         return M2D_OK;
     });
