@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(1024) ln_params_kernel(const LnArgs p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (c < p.C) {
-        constexpr int U = 10;                      // loads under way at once: some 300 sums in one go
+        constexpr int U = 16;                      // loads under way at once: some 500 sums in one go
         const float* const q = p.partial + (long long)blockIdx.y * p.C + c;
         for (int i = warp; i < p.parts; i += 32 * U) {
             float t[U];

@@ -157,6 +157,7 @@ m2d_ln_desc ln_desc(const Tensor& x, const Tensor& weight, const Tensor& bias, d
 }
 // As rows (N, C) with neighbours along C: a view where there is one.
 Tensor matrix(const Tensor& t) {
+    if (t.dim() == 2 && t.stride(1) == 1) return t;
     const Tensor m = rows(t).reshape({-1, t.size(-1)});
     return m.size(0) == 1 || m.stride(0) >= 0 ? m : m.contiguous();
 }
@@ -187,7 +188,6 @@ public:
         Tensor sum;
         const Tensor y = ln_forward(d, x, residual, x_, &sum);
         ctx->save_for_backward({sum.defined() ? sum : x_, weight, bias, stats});
-        ctx->saved_data["eps"] = eps;
         ctx->set_materialize_grads(false);
         return sum.defined() ? variable_list{y, sum} : variable_list{y};
     }
@@ -203,7 +203,7 @@ public:
             return {ds_, none(s[1]), none(s[2]), ds_, Tensor()};
         }
         const Tensor x = matrix(s[0]), w = dense(s[1]), b = dense(s[2]), dy = matrix(grads[0].to(x.scalar_type())), ds = ds_.defined() ? matrix(ds_.to(x.scalar_type())) : ds_;
-        m2d_ln_desc d = ln_desc(x, w, b, ctx->saved_data["eps"].toDouble());
+        m2d_ln_desc d = ln_desc(x, w, b, 0.0);           // (eps is in the statistics)
         d.stats = fptr(s[3]);
         d.d_y = dy.data_ptr(); d.d_y_row = dy.stride(0);
         if (ds.defined()) { d.d_sum = ds.data_ptr(); d.d_sum_row = ds.stride(0); }
