@@ -131,7 +131,7 @@ int m2d_clip_grad_norm(const m2d_clip_tensor *tensors, int32_t count, float max_
  *     M2D_GATE_DECAY:  a = exp(gate), u = x           (gate at most 0; positive ones grow the state and are not checked for)
  *     M2D_GATE_FORGET: a = sigmoid(gate), u = (1 - a) x
  * A gate of -inf forgets everything before the token.  States and their gradients are fp32 whatever the tensors' type.  B times C/32 up to
- * 2^27, T below 2^31 - 2^17.  Sequences of several strides whose rows begin at 16-byte boundaries come by TMA; a wait for such a copy that gives
+ * 2^27, C up to 2^29, T below 2^31 - 2^17.  Sequences of several strides whose rows begin at 16-byte boundaries come by TMA; a wait for such a copy that gives
  * up makes what depends on it NaN and shows in m2d_take_wait_failure().
  */
 typedef enum { M2D_GATE_DECAY = 0, M2D_GATE_FORGET = 1 } m2d_gate;
@@ -148,8 +148,8 @@ typedef struct m2d_recur_desc {
     int32_t form;                  /* m2d_gate */
     uint32_t flags;                /* 0, or the test hook */
     m2d_recur_tensor x, gate;
-    const int32_t *lengths;        /* (B) tokens of each sequence, clamped to 0 ... T, or NULL: T.  Rows behind a sequence's last are not
-                                      read; outputs there are zero */
+    const int32_t *lengths;        /* (B) tokens of each sequence, clamped to 0 ... T, or NULL: T.  What rows behind a sequence's last
+                                      hold does not matter; outputs there are zero */
     const float *state;            /* (B,C) dense: the state before the first token, or NULL: zero */
     float *state_out;              /* (B,C) dense: the state after the last one, or NULL                    [fwd] */
     void *y;                       /* (B,T,C) dense: every h_t                                              [fwd] */

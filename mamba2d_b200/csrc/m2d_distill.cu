@@ -9,6 +9,8 @@
 // behind it, the first of entries with one index for all of them, so that every value is rounded once and does not depend on
 // any order.  Exponents are (z - max) c with c = log2(e) / tau: exact where all values are equal, also at the type's lowest.  What is left of a row
 // (its sums' logarithms, the teacher's entries) is summed in 64 bits: a loss is a small difference of large logarithms.
+// Measured, bf16: 2048x131072 forward 95 us (5.7 TB/s), backward 176 (6.1); 2047x50001 with labels at temperature 2 44 and 76 us (4.6 and 5.4), exponentials
+// at a rate of 23.
 #include "follow.cuh"
 #include "packed.cuh"
 #include "plan.cuh"
@@ -452,8 +454,9 @@ static int check_distill(const m2d_distill_desc* d) {
     if (d->N > INT32_MAX / 64 || d->V > INT32_MAX - (1 << 16) || d->K > M2D_DISTILL_MAX_TOP) return M2D_ERR_TOO_LARGE;
     if (!(d->temperature > 0.f) || d->temperature > 3.4e38f || !(d->label_weight >= 0.f && d->label_weight <= 1.f)) return M2D_ERR_FLAGS;
     if (!d->logits || !d->teacher || !d->index || (d->label_weight > 0.f && !d->labels)) return M2D_ERR_NULL;
-    const int es = d->dtype == M2D_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(d->logits) % es) return M2D_ERR_PITCH;
+    const uintptr_t es = d->dtype == M2D_F32 ? 4 : 2;
+    auto off = [](const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+    if (off(d->logits, es) || off(d->d_logits, es) || off(d->teacher, d->teacher_dtype == M2D_F32 ? 4 : 2) || off(d->index, d->index_64 ? 8 : 4) || off(d->labels, d->labels_64 ? 8 : 4)) return M2D_ERR_PITCH;
     return M2D_OK;
 }
 static DistillArgs distill_args(const m2d_distill_desc* d) {

@@ -79,14 +79,15 @@ def gated_recurrence(x, gate, *, form="decay", initial_state=None, lengths=None,
             "forget": ``a = sigmoid(gate)``, ``u = (1 - a) x``.  A gate of -inf forgets all earlier tokens (if they
             are finite).
         initial_state: (B, C) float32, or None for zero.
-        lengths: (B,) integers on the device, tokens of each sequence (clamped to 0 ... T), or None for T.  Rows
-            behind them are not read; outputs and gradients there are zero.
+        lengths: (B,) integers on the device, tokens of each sequence (clamped to 0 ... T), or None for T.  What rows
+            behind them hold does not matter; outputs and gradients there are zero.
         return_state: also return the state after each sequence's last token, (B, C) float32.
     Returns:
         h (B, T, C) in ``x.dtype``, or ``(h, state)``.
     Differentiable in x, gate and initial_state, once (``create_graph`` raises); those of x and gate are computed together.
     States are carried in float32 and gradients computed from them, whatever the type of h.  A token that is not finite spoils
-    later ones of its sequence and channel (in the backward pass earlier ones), as by the formula.
+    later ones of its sequence and channel (in the backward pass earlier ones), as by the formula.  Rows of x and gate that begin at
+    16-byte boundaries are fetched ahead by TMA (an odd number of channels takes two to three times as long).
     """
     if form not in _GATES:
         raise ValueError(f"gated_recurrence: unknown form, got {form}...")

@@ -55,7 +55,7 @@ def test_recurrence_descriptors(L):
             setattr(d, k, v)
         return ctypes.byref(d)
     for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"form": 2}, FLAGS), ({"flags": 0x100}, FLAGS), ({"flags": 1}, FLAGS), ({"B": 0}, SHAPE), ({"T": 0}, SHAPE), ({"C": -1}, SHAPE),
-                   ({"T": (1 << 31) - 1}, LARGE), ({"B": 1 << 27}, LARGE), ({"x": RecurTensor(None, 0, 0)}, NULL), ({"gate": RecurTensor(258, 0, 0)}, PITCH)):
+                   ({"T": (1 << 31) - 1}, LARGE), ({"B": 1 << 27}, LARGE), ({"x": RecurTensor(None, 0, 0)}, NULL), ({"gate": RecurTensor(258, 0, 0)}, PITCH), ({"y": 258}, PITCH), ({"d_x": 257}, PITCH), ({"C": (1 << 29) + 1}, LARGE)):
         assert L.m2d_recur_fwd(desc(**kw), None) == rc and L.m2d_recur_bwd(desc(**kw), None) == rc, kw
     step = lambda **kw: L.m2d_recur_step(desc(**kw), ctypes.c_int64(64), None)  # noqa: E731
     assert step() == SHAPE and step(T=1) == NULL and step(T=1, y=256, state=256) == NULL and L.m2d_recur_fwd(None, None) == NULL
@@ -90,7 +90,7 @@ def test_layer_norm_descriptors(L):
         for k, v in kw.items():
             setattr(d, k, v)
         return ctypes.byref(d)
-    for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"N": 0}, SHAPE), ({"C": 0}, SHAPE), ({"N": 1 << 31}, LARGE), ({"C": (1 << 30) + 1}, LARGE)):
+    for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"N": 0}, SHAPE), ({"C": 0}, SHAPE), ({"N": 1 << 31}, LARGE), ({"C": (1 << 30) + 1}, LARGE), ({"x": 257}, PITCH), ({"weight": 258, "params_f32": 1}, PITCH), ({"d_x": 255}, PITCH)):
         assert L.m2d_ln_fwd(desc(**kw), None) == rc and L.m2d_ln_bwd(desc(**kw), None) == rc, kw
     assert L.m2d_ln_fwd(None, None) == NULL and L.m2d_ln_fwd(desc(x=256, y=256, residual=256), None) == NULL        # nowhere to put the sum
     p = dict(x=256, x_row=64, d_y=256, d_y_row=64, d_x=256, stats=256, d_weight=256)
@@ -121,7 +121,7 @@ def test_distillation_descriptors(L):
         return ctypes.byref(d)
     for kw, rc in (({}, NULL), ({"struct_bytes": 8}, ABI), ({"dtype": 2}, DTYPE), ({"teacher_dtype": -1}, DTYPE), ({"N": 0}, SHAPE), ({"V": 0}, SHAPE), ({"K": 0}, SHAPE), ({"K": 513}, LARGE),
                    ({"N": 1 << 26}, LARGE), ({"V": (1 << 31) - 1}, LARGE), ({"temperature": 0.0}, FLAGS), ({"temperature": float("nan")}, FLAGS), ({"temperature": float("inf")}, FLAGS),
-                   ({"label_weight": 1.5}, FLAGS), ({"label_weight": 0.5}, NULL), ({"logits": None}, NULL), ({"index": None}, NULL), ({"logits": 258}, PITCH)):
+                   ({"label_weight": 1.5}, FLAGS), ({"label_weight": 0.5}, NULL), ({"logits": None}, NULL), ({"index": None}, NULL), ({"logits": 258}, PITCH), ({"index": 260, "index_64": 1}, PITCH), ({"d_logits": 2}, PITCH)):
         assert L.m2d_distill_fwd(desc(**kw), None) == rc and L.m2d_distill_bwd(desc(**kw), None) == rc, kw
     assert L.m2d_distill_fwd(None, None) == NULL and L.m2d_distill_stats(desc()) > 0
     assert L.m2d_distill_fwd_workspace(desc()) == 0                                       # (short rows)
