@@ -328,7 +328,7 @@ struct Feed {
     char* ring;
     uint32_t bars;
     volatile int *abort, *apart;
-    int stage, stages, tile, box, at, run, ordered;
+    int stage, stages, tile, box, at, run, ordered, turned;
     unsigned parity;
     template <typename W>
     __device__ __forceinline__ Feed(const RecurArgs& p, const W& w, char* smem, const Waits& waits) {
@@ -344,6 +344,7 @@ struct Feed {
             box = p.box;
             at = w.at;
             run = w.run;
+            turned = (threadIdx.x & 31) / LANES;
         }
     }
     static __device__ __forceinline__ Raw nothing(int t) { return P::fill(t == 1 ? kept<FORM>() : 0.f); }
@@ -378,9 +379,27 @@ struct Feed {
     __device__ __forceinline__ void next() {
         if (++stage == stages) { stage = 0; parity ^= 1; }
     }
-    __device__ __forceinline__ Raw raw(int t, int i) const {
-        if constexpr (TMA) return *place(t, i);
-        else return reg[t][i];
+    // Tokens i ... i + 3.  Where a warp has several rows at once, those of its runs lie in the same banks, 16 tokens apart: run q reads its tokens in
+    // the order i ^ q and sorts them in registers.
+    __device__ __forceinline__ void four(int t, int i, Raw (&r)[4]) const {
+        if constexpr (!TMA) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = reg[t][i + j];
+        } else if constexpr (LANES == 32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = *place(t, i + j);
+        } else {
+            const char* const p = reinterpret_cast<const char*>(place(t, i));
+            Raw q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const Raw*>(p + (j ^ turned) * (width * (int)sizeof(T)));
+            const bool one = turned & 1, two = turned & 2;
+            const Raw a0 = one ? q[1] : q[0], a1 = one ? q[0] : q[1], a2 = one ? q[3] : q[2], a3 = one ? q[2] : q[3];
+            r[0] = two ? a2 : a0;
+            r[1] = two ? a3 : a1;
+            r[2] = two ? a0 : a2;
+            r[3] = two ? a1 : a3;
+        }
     }
     // bounded wait for what is still on its way, after a wait that gave up; tells the host
     __device__ __forceinline__ void leave(int* host_flag) {
@@ -449,13 +468,20 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
         N a[L], u[L], h = N::all(0.f);
         Collect<FORM, VEC> all;
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const N gate = gate_of<T, VEC, FORM>(feed.raw(1, i)), x = P::get(feed.raw(0, i));
-            N rest;
-            open_gate<FORM, VEC>(gate, a[i], rest);
-            u[i] = FORM == M2D_GATE_DECAY ? x : mul_(rest, x);
-            all.add(gate, a[i], rest);
-            h = fma_(a[i], h, u[i]);
+        for (int i0 = 0; i0 < L; i0 += 4) {
+            Raw rx[4], rg[4];
+            feed.four(0, i0, rx);
+            feed.four(1, i0, rg);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j;
+                const N gate = gate_of<T, VEC, FORM>(rg[j]), x = P::get(rx[j]);
+                N rest;
+                open_gate<FORM, VEC>(gate, a[i], rest);
+                u[i] = FORM == M2D_GATE_DECAY ? x : mul_(rest, x);
+                all.add(gate, a[i], rest);
+                h = fma_(a[i], h, u[i]);
+            }
         }
         if (!TMA && s0 + stride < w.len) load(t0 + stride);
         Step<VEC> step = all.done();
@@ -604,23 +630,43 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         if constexpr (TMA) ok = feed.ready(w.mine ? w.len - t0 : 0);
         float *const steps = smem + (size_t)buf * w.warps * 4 * width + 2 * w.at, *const adds = steps + (size_t)w.warps * 2 * width;
         N a[L], rest[L], before[L], h = N::all(0.f), R = N::all(0.f);
-        N xs[TMA ? 1 : L], ds[TMA ? 1 : L];               // (of a tile in shared memory x and dy are read again instead)
-        auto xv = [&](int i) { return TMA ? P::get(feed.raw(0, i)) : xs[TMA ? 0 : i]; };
-        auto dv = [&](int i) { return TMA ? P::get(feed.raw(2, i)) : ds[TMA ? 0 : i]; };
         Collect<FORM, VEC> all;
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const N gate = gate_of<T, VEC, FORM>(feed.raw(1, i));
-            if constexpr (!TMA) {
-                xs[i] = P::get(feed.raw(0, i));
-                ds[i] = P::get(feed.raw(2, i));
+        for (int i0 = 0; i0 < L; i0 += 4) {
+            Raw rx[4], rg[4];
+            feed.four(0, i0, rx);
+            feed.four(1, i0, rg);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j;
+                const N gate = gate_of<T, VEC, FORM>(rg[j]), x = P::get(rx[j]);
+                open_gate<FORM, VEC>(gate, a[i], rest[i]);
+                all.add(gate, a[i], rest[i]);
+                h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? x : mul_(rest[i], x));
             }
-            open_gate<FORM, VEC>(gate, a[i], rest[i]);
-            all.add(gate, a[i], rest[i]);
-            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv(i) : mul_(rest[i], xv(i)));
         }
 #pragma unroll
-        for (int i = L - 1; i >= 0; --i) R = mul_(a[i], add_(dv(i), R));
+        for (int i0 = L - 4; i0 >= 0; i0 -= 4) {
+            Raw rd[4];
+            feed.four(2, i0, rd);
+#pragma unroll
+            for (int j = 3; j >= 0; --j) R = mul_(a[i0 + j], add_(P::get(rd[j]), R));
+        }
+        Raw xs[TMA ? 1 : L], ds[TMA ? 1 : L];             // (of a tile in shared memory x and dy are read again instead)
+        if constexpr (!TMA)
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                xs[i] = feed.reg[0][i];
+                ds[i] = feed.reg[2][i];
+            }
+        auto four = [&](int t, int i, Raw (&r)[4]) {
+            if constexpr (TMA) {
+                feed.four(t, i, r);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = t == 0 ? xs[i + j] : ds[i + j];
+            }
+        };
         N first = N::all(mark[0]);
         if constexpr (VEC == 2) first.set(1, mark[1]);
         if (s0 >= stride) load(s0 - stride + w.rank * tile);
@@ -688,23 +734,35 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         h = after_others<VEC, LANES, true>(up, add, h);
         if (!ok) h = R = nan;
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            before[i] = h;
-            h = fma_(a[i], h, FORM == M2D_GATE_DECAY ? xv(i) : mul_(rest[i], xv(i)));
+        for (int i0 = 0; i0 < L; i0 += 4) {
+            Raw rx[4];
+            four(0, i0, rx);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const N x = P::get(rx[j]);
+                before[i0 + j] = FORM == M2D_GATE_DECAY ? h : fma_(x, N::all(-1.f), h);        // (forget: h_{t-1} - x_t)
+                h = fma_(a[i0 + j], h, FORM == M2D_GATE_DECAY ? x : mul_(rest[i0 + j], x));
+            }
         }
         const int n = w.mine ? w.len - t0 : 0;
         char *const px = reinterpret_cast<char*>(dx + (long long)t0 * p.C), *const pg = reinterpret_cast<char*>(dgate + (long long)t0 * p.C);
         const unsigned row = (unsigned)p.C * (unsigned)sizeof(T);
         auto write = [&](auto whole) {
 #pragma unroll
-            for (int i = L - 1; i >= 0; --i) {
-                const N D = add_(dv(i), R);
-                R = mul_(a[i], D);
-                const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
-                const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), fma_(xv(i), N::all(-1.f), before[i]));
-                if (whole.value || i < n) {
-                    *reinterpret_cast<Raw*>(px + (unsigned long long)row * (unsigned)i) = P::put(gx);
-                    *reinterpret_cast<Raw*>(pg + (unsigned long long)row * (unsigned)i) = P::put(gg);
+            for (int i0 = L - 4; i0 >= 0; i0 -= 4) {
+                Raw rd[4];
+                four(2, i0, rd);
+#pragma unroll
+                for (int j = 3; j >= 0; --j) {
+                    const int i = i0 + j;
+                    const N D = add_(P::get(rd[j]), R);
+                    R = mul_(a[i], D);
+                    const N gx = FORM == M2D_GATE_DECAY ? D : mul_(rest[i], D);
+                    const N gg = FORM == M2D_GATE_DECAY ? mul_(R, before[i]) : mul_(mul_(rest[i], R), before[i]);
+                    if (whole.value || i < n) {
+                        *reinterpret_cast<Raw*>(px + (unsigned long long)row * (unsigned)i) = P::put(gx);
+                        *reinterpret_cast<Raw*>(pg + (unsigned long long)row * (unsigned)i) = P::put(gg);
+                    }
                 }
             }
         };
