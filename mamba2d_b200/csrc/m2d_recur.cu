@@ -492,10 +492,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
             give(adds + w.warp * width, add);
         }
         __syncthreads();
-        if constexpr (TMA) {                              // (all have read the stage)
-            order((long long)s0 + (long long)p.stages * stride);
-            feed.next();
-        }
+        if constexpr (TMA) feed.next();
         if (w.ctas > 1) {
             // one warp joins the tile's runs and tells every CTA of the cluster
             float* const tiles = cluster_part + (size_t)buf * w.ctas * 3 * width;
@@ -555,6 +552,8 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_fwd_kernel(const Recur
                 if (i < n) *reinterpret_cast<Raw*>(py + (unsigned long long)row * (unsigned)i) = P::put(h);
             }
         }
+        // (all have read the stage; asked for last, since the others wait for what this thread's warp joins)
+        if constexpr (TMA) order((long long)s0 + (long long)p.stages * stride);
     }
     feed.leave(p.host_flag);
     if (w.ctas > 1) cluster.sync();                       // (none leaves while another may still write to it)
@@ -681,7 +680,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
         }
         if (w.first) give(adds + 2 * w.warp * width + VEC, flow);
         __syncthreads();
-        if constexpr (TMA)
+        if constexpr (TMA)                    // (at once: there may be but two stages)
             if (again && asked >= 0) {
                 order(asked);
                 asked -= stride;
