@@ -10,7 +10,7 @@
 // memory is read once and written once.  Tiles come by TMA, two or three ahead of the one that is worked on; where rows are not whole 16-byte pieces, or
 // there is but one stride, by plain loads into registers, the next tile's while one is worked on.  Where sequences and channels are too few for all SMs, rows are
 // split into shorter pieces and the sequence over up to 8 CTAs (plan_recur).  Measured, bf16: 4x4096x2048 forget gates 47 us (201 MB at 4.3 TB/s: half
-// of the issue slots, two CTAs an SM), 1x65536x512 decays 68 us (the chain of waits of 16 strides), 8x4096x2048 forward 76 and backward 128 us (5.3 and 5.2 TB/s).
+// of the issue slots, two CTAs an SM), 1x65536x512 decays 57 us (the chain of waits of 16 strides), 8x4096x2048 forward 75 and backward 126 us (5.4 and 5.3 TB/s).
 //
 // Precision: states and sums are fp32.  A channel may remember thousands of tokens: 1 - A of a run is small then, and A
 // rounded to fp32 would be off by the same amount at every step, 2^-24 against a 1 - A of 2^-12 at a memory of 4096 tokens.  So A is held in two
