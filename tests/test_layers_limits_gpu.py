@@ -1,0 +1,70 @@
+"""Where the gated recurrence, the norms, linear attention and the distillation loss come to their ends: batches of nothing that are trained on, single
+tokens over a long memory, temperatures of any size, losses whose rounding to fp32 is the only one."""
+import pytest
+import torch
+
+import layer_ref
+from mamba2d_b200 import distillation_loss, gated_recurrence, gated_recurrence_step, group_norm, layer_norm, linear_attention
+from test_recurrence_gpu import fast_scan
+
+pytestmark = pytest.mark.gpu
+F32, BF = torch.float32, torch.bfloat16
+FORMS = ("decay", "forget")
+
+
+def leaf(*shape, dt=F32):
+    return torch.full(shape, 0.5, device="cuda", dtype=dt, requires_grad=True)
+
+
+def zeros_for(out, leaves):
+    """Every leaf gets a gradient of its own shape and type, which is zero."""
+    out = [t for t in (out if isinstance(out, tuple) else (out,))]
+    for t, g in zip(leaves, torch.autograd.grad(out, leaves, [torch.ones_like(t) for t in out])):
+        assert g.shape == t.shape and g.dtype == t.dtype and bool((g == 0).all())
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("form", FORMS)
+def test_single_tokens_over_a_long_memory(form, dt):
+    """A gate that all tokens share and a memory of some 8192 of them, M, for 20000 tokens.  What a token's rounding of its gate is off by has the same sign
+    every time and would add up, to M times 2^-25 or more (2.4e-4).  What may be left: each state's own rounding, at most 2^-24 of it and as often up as down (x is
+    random), whose share after M tokens has a deviation of 2^-24 (M / 2 / 3)^0.5 = 2.2e-6 at most, of which eight are allowed; and 2^-20, for what 1 - a and the
+    weight of x are off by."""
+    T, C = 20000, 32
+    k = 0.01 * torch.arange(C, device="cuda")
+    g = (-2.0 ** -13 * (1 + k) if form == "decay" else 9.01 - k)[None].to(dt)
+    x = (1 + 0.5 * torch.randn(1, T, C, generator=torch.Generator().manual_seed(11)).cuda()).to(dt)
+    a, u = layer_ref.terms(x.double(), g.double()[:, None].expand(1, T, C), form)
+    start = 1.0 if form == "forget" else float(1 / (1 - a).mean())
+    state = torch.full((1, C), start, device="cuda")
+    want = fast_scan(a, torch.cat((u[:, :1] + a[:, :1] * start, u[:, 1:]), 1))
+    allowed = 8 * 2.0 ** -24 * (8192 / 6) ** 0.5 + 2.0 ** -20
+    for t in range(T):
+        y = gated_recurrence_step(x[:, t], g, state, form=form)
+        if t % 2000 == 1999:
+            assert float((state.double() / want[:, t] - 1).abs().max()) <= allowed, t
+            assert torch.equal(y, state.to(dt))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_single_tokens_at_their_ends(form):
+    """Resets are exact, a state that nothing forgets stays, values that are not finite are the formula's, and no difference of large values overflows."""
+    big = 3e38
+    cases = [  # state, x, gate, what becomes of the state
+        (5.0, 0.25, -torch.inf, 0.25), (1e30, 0.25, -torch.inf, 0.25 if form == "decay" else None), (-7.5, 0.0, 0.0 if form == "decay" else torch.inf, -7.5), (torch.inf, 1.0, -0.25 if form == "decay" else 3.0, torch.inf),
+        (1.0, -torch.inf, -0.25 if form == "decay" else 3.0, -torch.inf), (torch.inf, torch.inf, -0.25 if form == "decay" else 3.0, torch.inf), (torch.nan, 1.0, -0.25, torch.nan), (1.0, torch.nan, -0.25, torch.nan),
+        (1.0, 1.0, torch.nan, torch.nan), (-big, big, -0.125 if form == "decay" else 2.0, None), (big, -big, -0.5 if form == "decay" else 0.25, None), (2.0, 3.0, -0.6931472 if form == "decay" else 0.0, None)]
+    s, x, g = (torch.tensor([c[k] for c in cases], device="cuda")[None] for k in range(3))
+    a, u = layer_ref.terms(x.double(), g.double(), form)
+    state = s.clone()
+    y = gated_recurrence_step(x, g, state, form=form)
+    assert torch.equal(torch.nan_to_num(y, nan=12345.0), torch.nan_to_num(state, nan=12345.0))
+    want, size = a * s.double() + u, a * s.double().abs() + u.abs()
+    for k, c in enumerate(cases):
+        got = float(state[0, k])
+        if c[3] is None:                 # (forget gates below -87 count as -87, of which 1.7e-38 of the state is left)
+            assert abs(got - float(want[0, k])) <= 2.0 ** -20 * float(size[0, k]) + 1.7e-38 * abs(c[0]), c
+        elif c[3] != c[3]:
+            assert got != got, c
+        else:
+            assert got == c[3], c
