@@ -181,12 +181,17 @@ public:
     static variable_list forward(AutogradContext* ctx, const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, const optional<Tensor>& residual_, double eps) {
         const Tensor weight = or_none(weight_), bias = or_none(bias_), residual = or_none(residual_);
         const c10::cuda::CUDAGuard guard(x_.device());
-        const Tensor x = matrix(x_), w = dense(weight), b = dense(bias);
-        m2d_ln_desc d = ln_desc(x, w, b, eps);
-        const Tensor stats = at::empty({d.N, 2}, x.options().dtype(at::kFloat));
-        d.stats = fptr(stats);
-        Tensor sum;
-        const Tensor y = ln_forward(d, x, residual, x_, &sum);
+        Tensor y, sum, stats;
+        if (x_.numel()) {
+            const Tensor x = matrix(x_), w = dense(weight), b = dense(bias);
+            m2d_ln_desc d = ln_desc(x, w, b, eps);
+            stats = at::empty({d.N, 2}, x.options().dtype(at::kFloat));
+            d.stats = fptr(stats);
+            y = ln_forward(d, x, residual, x_, &sum);
+        } else {                                   // (nothing to do, but the parameters have gradients: zero)
+            y = at::empty(x_.sizes(), x_.options());
+            if (residual.defined()) sum = at::empty(x_.sizes(), x_.options());
+        }
         ctx->save_for_backward({sum.defined() ? sum : x_, weight, bias, stats});
         ctx->set_materialize_grads(false);
         return sum.defined() ? variable_list{y, sum} : variable_list{y};
@@ -198,9 +203,11 @@ public:
         const c10::cuda::CUDAGuard guard(s[0].device());
         const bool residual = grads.size() > 1;
         const Tensor ds_ = residual ? grads[1] : Tensor();
-        if (!grads[0].defined()) {                 // the sum alone was used
-            auto none = [](const Tensor& t) { return t.defined() && t.requires_grad() ? at::zeros(t.sizes(), t.options()) : Tensor(); };
-            return {ds_, none(s[1]), none(s[2]), ds_, Tensor()};
+        auto none = [](const Tensor& t) { return t.defined() && t.requires_grad() ? at::zeros(t.sizes(), t.options()) : Tensor(); };
+        if (!grads[0].defined()) return {ds_, none(s[1]), none(s[2]), ds_, Tensor()};          // the sum alone was used
+        if (!s[0].numel()) {
+            const Tensor dx = at::empty(s[0].sizes(), s[0].options());
+            return {dx, none(s[1]), none(s[2]), residual ? dx : Tensor(), Tensor()};
         }
         const Tensor x = matrix(s[0]), w = dense(s[1]), b = dense(s[2]), dy = matrix(grads[0].to(x.scalar_type())), ds = ds_.defined() ? matrix(ds_.to(x.scalar_type())) : ds_;
         m2d_ln_desc d = ln_desc(x, w, b, 0.0);           // (eps is in the statistics)
@@ -242,11 +249,11 @@ std::tuple<Tensor, optional<Tensor>> layer_norm(const Tensor& x_, const optional
     for (const Tensor* p : {&weight, &bias, &residual}) TORCH_CHECK(!p->defined() || p->device() == x_.device(), "layer_norm: tensors on ", p->device(), " and ", x_.device());
     TORCH_CHECK(C <= INT_MAX && x_.numel() / std::max<int64_t>(C, 1) <= INT_MAX, "layer_norm: a size out of range");
     const c10::cuda::CUDAGuard guard(x_.device());
-    if (!x_.numel()) return {x_.clone(), residual.defined() ? optional<Tensor>(x_ + residual) : c10::nullopt};
     if (wants_grad({&x_, &weight, &bias, &residual})) {
         const variable_list r = LnFn::apply(x_, weight_, bias_, residual_, eps);
         return {r[0], r.size() > 1 ? optional<Tensor>(r[1]) : c10::nullopt};
     }
+    if (!x_.numel()) return {x_.clone(), residual.defined() ? optional<Tensor>(x_ + residual) : c10::nullopt};
     const at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x = matrix(x_), w = dense(weight), b = dense(bias);
     m2d_ln_desc d = ln_desc(x, w, b, eps);

@@ -24,6 +24,22 @@ def zeros_for(out, leaves):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("shape", [(0, 8), (4, 0, 8), (3, 0)])
+def test_layer_norm_of_nothing(shape, dt):
+    """Parameters get zeros for a share without rows, whether x needs a gradient or not: under DistributedDataParallel none may be left out."""
+    C = shape[-1]
+    x, r, w, b = leaf(*shape, dt=dt), leaf(*shape, dt=dt), leaf(C), leaf(C, dt=F32)
+    zeros_for(layer_norm(x, w, b), (x, w, b))
+    zeros_for(layer_norm(x.detach(), w, b), (w, b))
+    zeros_for(layer_norm(x.detach(), None, b), (b,))
+    y, s = layer_norm(x, w, b, residual=r)
+    assert y.shape == s.shape == x.shape and y.dtype == s.dtype == dt
+    zeros_for((y, s), (x, r, w, b))
+    zeros_for(layer_norm(x, w, b, residual=r)[1], (x, r, w, b))
+    assert not layer_norm(x.detach(), w.detach()).requires_grad
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("form", FORMS)
 def test_single_tokens_over_a_long_memory(form, dt):
     """A gate that all tokens share and a memory of some 8192 of them, M, for 20000 tokens.  What a token's rounding of its gate is off by has the same sign
