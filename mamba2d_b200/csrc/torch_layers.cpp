@@ -37,14 +37,24 @@ struct Recur {
     }
 };
 
+// The state after no tokens.
+Tensor same_state(const Tensor& x, const Tensor& state) {
+    return state.defined() ? state.clone() : at::zeros({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
+}
+
 class RecurFn : public torch::autograd::Function<RecurFn> {
 public:
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const optional<Tensor>& state_, const optional<Tensor>& lengths_, int64_t form, bool want_state) {
         const Tensor state = or_none(state_), lengths = or_none(lengths_);
         const c10::cuda::CUDAGuard guard(x.device());
-        Recur r(x, gate, state, lengths, form);
-        Tensor state_out, marks;
-        const Tensor y = r.forward(want_state ? &state_out : nullptr, &marks);
+        Tensor y, state_out, marks;
+        if (x.numel()) {
+            Recur r(x, gate, state, lengths, form);
+            y = r.forward(want_state ? &state_out : nullptr, &marks);
+        } else {
+            y = at::empty(x.sizes(), x.options());
+            if (want_state) state_out = same_state(x, state);
+        }
         ctx->save_for_backward({x, gate, state, lengths, marks});
         ctx->saved_data["form"] = form;
         ctx->set_materialize_grads(false);
@@ -58,6 +68,11 @@ public:
         check_waits("gated_recurrence");
         const bool have_state_grad = grads.size() > 1 && grads[1].defined();
         if (!grads[0].defined() && !have_state_grad) return variable_list(6);
+        if (!s[0].numel()) {
+            const Tensor dx = at::empty(s[0].sizes(), s[0].options());
+            const Tensor ds = !s[2].defined() || !s[2].requires_grad() ? Tensor() : have_state_grad ? grads[1] : at::zeros(s[2].sizes(), s[2].options());
+            return {dx, at::empty_like(dx), ds, Tensor(), Tensor(), Tensor()};
+        }
         Recur r(s[0], s[1], s[2], s[3], ctx->saved_data["form"].toInt());
         m2d_recur_desc& d = r.d;
         // (no gradient of h: one zero, expanded)
@@ -98,15 +113,12 @@ std::tuple<Tensor, optional<Tensor>> gated_recurrence(const Tensor& x, const Ten
     check_recur(what, "(B, T, C)", 3, x, gate, state);
     const Tensor lengths = token_counts(what, or_none(lengths_), x);
     const c10::cuda::CUDAGuard guard(x.device());
-    if (!x.numel()) {
-        if (!want_state) return {x.clone(), c10::nullopt};
-        return {x.clone(), state.defined() ? state.clone() : at::zeros({x.size(0), x.size(2)}, x.options().dtype(at::kFloat))};
-    }
-    check_waits(what);
+    if (x.numel()) check_waits(what);
     if (wants_grad({&x, &gate, &state})) {
         const variable_list r = RecurFn::apply(x, gate, state_, lengths.defined() ? optional<Tensor>(lengths) : c10::nullopt, form, want_state);
         return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
     }
+    if (!x.numel()) return {x.clone(), want_state ? optional<Tensor>(same_state(x, state)) : c10::nullopt};
     const at::AutoDispatchBelowADInplaceOrView below;
     Recur r(x, gate, state, lengths, form);
     Tensor state_out;

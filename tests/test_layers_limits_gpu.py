@@ -41,6 +41,28 @@ def test_layer_norm_of_nothing(shape, dt):
 
 @pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("B,T,C", [(2, 0, 8), (0, 5, 8), (2, 5, 0)])
+def test_the_recurrence_of_nothing(B, T, C, form, dt):
+    """x and gate get gradients, and the state, which passes through, its own."""
+    x, g, s = leaf(B, T, C, dt=dt), leaf(B, T, C, dt=dt), leaf(B, C)
+    zeros_for(gated_recurrence(x, g, form=form), (x, g))
+    zeros_for(gated_recurrence(x.detach(), g, form=form), (g,))
+    part = leaf(1, 1, C, dt=dt)
+    zeros_for(gated_recurrence(x, part.expand(B, T, C), form=form), (part,))
+    for lengths in (None, torch.zeros(B, dtype=torch.int32, device="cuda")):
+        h, last = gated_recurrence(x, g, form=form, initial_state=s, lengths=lengths, return_state=True)
+        assert h.shape == x.shape and h.dtype == dt and torch.equal(last, s) and last.data_ptr() != s.data_ptr() or not s.numel()
+        up = torch.randn(B, C, device="cuda")
+        dx, dg, ds = torch.autograd.grad((h, last), (x, g, s), (torch.ones_like(h), up))
+        assert dx.shape == dg.shape == x.shape and torch.equal(ds, up)
+        zeros_for(gated_recurrence(x, g, form=form, initial_state=s, lengths=lengths), (x, g, s))
+    h, last = gated_recurrence(x, g, form=form, return_state=True)
+    assert last.shape == (B, C) and bool((last == 0).all())
+    zeros_for((h, last), (x, g))
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("form", FORMS)
 def test_single_tokens_over_a_long_memory(form, dt):
     """A gate that all tokens share and a memory of some 8192 of them, M, for 20000 tokens.  What a token's rounding of its gate is off by has the same sign
     every time and would add up, to M times 2^-25 or more (2.4e-4).  What may be left: each state's own rounding, at most 2^-24 of it and as often up as down (x is
