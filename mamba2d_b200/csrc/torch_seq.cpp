@@ -215,11 +215,16 @@ public:
     static Tensor forward(AutogradContext* ctx, const Tensor& x_, const optional<Tensor>& weight_, const optional<Tensor>& bias_, int64_t groups, int64_t act, double eps) {
         const Tensor weight = or_none(weight_), bias = or_none(bias_);
         const c10::cuda::CUDAGuard guard(x_.device());
-        const Tensor x = x_.contiguous(), w = dense(weight), b = dense(bias);
-        m2d_norm_desc d = norm_desc(x, w, b, groups, act, eps);
-        const Tensor stats = at::empty({d.N, d.groups, 2}, x.options().dtype(at::kFloat));
-        d.stats = fptr(stats);
-        const Tensor y = norm_forward(d, x);
+        Tensor y, stats;
+        if (x_.numel()) {
+            const Tensor x = x_.contiguous(), w = dense(weight), b = dense(bias);
+            m2d_norm_desc d = norm_desc(x, w, b, groups, act, eps);
+            stats = at::empty({d.N, d.groups, 2}, x.options().dtype(at::kFloat));
+            d.stats = fptr(stats);
+            y = norm_forward(d, x);
+        } else {                                   // (nothing to do, but the parameters have gradients: zero)
+            y = at::empty(x_.sizes(), x_.options());
+        }
         ctx->save_for_backward({x_, weight, bias, stats});
         ctx->saved_data["groups"] = groups;
         ctx->saved_data["act"] = act;
@@ -231,6 +236,10 @@ public:
         TORCH_CHECK(!at::GradMode::is_enabled(), "group_norm: gradients of gradients (create_graph) are not supported");
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[0].device());
+        if (!s[0].numel()) {
+            auto none = [](const Tensor& t) { return t.defined() && t.requires_grad() ? at::zeros(t.sizes(), t.options()) : Tensor(); };
+            return {at::empty(s[0].sizes(), s[0].options()), none(s[1]), none(s[2]), Tensor(), Tensor(), Tensor()};
+        }
         const Tensor x = s[0].contiguous(), w = dense(s[1]), b = dense(s[2]), dy = grads[0].to(x.scalar_type()).contiguous();
         m2d_norm_desc d = norm_desc(x, w, b, ctx->saved_data["groups"].toInt(), ctx->saved_data["act"].toInt(), ctx->saved_data["eps"].toDouble());
         d.stats = fptr(s[3]);
@@ -273,8 +282,8 @@ Tensor group_norm(const Tensor& x_, int64_t groups, const optional<Tensor>& weig
                         "group_norm: dtype ", p->scalar_type(), "; weight and bias share one, float32 or ", x_.scalar_type());
             TORCH_CHECK(p->device() == x_.device(), "group_norm: tensors on ", p->device(), " and ", x_.device());
         }
-    if (!x_.numel()) return x_.clone();
     if (wants_grad({&x_, &weight, &bias})) return NormFn::apply(x_, weight_, bias_, groups, act, eps);
+    if (!x_.numel()) return x_.clone();
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = x_.contiguous(), w = dense(weight), b = dense(bias);

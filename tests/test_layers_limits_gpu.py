@@ -62,6 +62,15 @@ def test_the_recurrence_of_nothing(B, T, C, form, dt):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("shape", [(0, 8), (4, 0, 8), (0, 3, 3, 8)])
+def test_group_norm_of_nothing(shape, dt):
+    x, w, b = leaf(*shape, dt=dt), leaf(8), leaf(8)
+    zeros_for(group_norm(x, 2, w, b, act="silu"), (x, w, b))
+    zeros_for(group_norm(x.detach(), 2, w, b), (w, b))
+    zeros_for(group_norm(x.detach(), 2, None, b), (b,))
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("form", FORMS)
 def test_single_tokens_over_a_long_memory(form, dt):
     """A gate that all tokens share and a memory of some 8192 of them, M, for 20000 tokens.  What a token's rounding of its gate is off by has the same sign
