@@ -51,15 +51,26 @@ Tensor attn_forward(Attn& a, Tensor* state_out) {
     return o;
 }
 
+bool no_tokens(const Tensor& v) { return v.size(0) == 0 || v.size(1) == 0; }
+// The state after no tokens.
+Tensor same_state(const Tensor& q, const Tensor& v, const Tensor& state) {
+    return state.defined() ? state.clone() : at::zeros({v.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat));
+}
+
 class AttnFn : public torch::autograd::Function<AttnFn> {
 public:
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const optional<Tensor>& state_,
                                  const optional<Tensor>& lengths_, double scale, bool want_state) {
         const Tensor state = or_none(state_), lengths = or_none(lengths_);
         const c10::cuda::CUDAGuard guard(v.device());
-        Attn a(q, k, v, g, state, lengths, scale);
-        Tensor out_state;
-        const Tensor o = attn_forward(a, want_state ? &out_state : nullptr);
+        Tensor o, out_state;
+        if (no_tokens(v)) {
+            o = at::empty(v.sizes(), v.options());
+            if (want_state) out_state = same_state(q, v, state);
+        } else {
+            Attn a(q, k, v, g, state, lengths, scale);
+            o = attn_forward(a, want_state ? &out_state : nullptr);
+        }
         ctx->save_for_backward({q, k, v, g, state, lengths});
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
@@ -73,6 +84,10 @@ public:
         check_waits("linear_attention");
         const bool have_state_grad = grads.size() > 1 && grads[1].defined();
         if (!grads[0].defined() && !have_state_grad) return variable_list(8);
+        if (no_tokens(s[2])) {
+            auto none = [](const Tensor& t) { return t.defined() && t.requires_grad() ? at::zeros(t.sizes(), t.options()) : Tensor(); };
+            return {none(s[0]), none(s[1]), none(s[2]), none(s[3]), have_state_grad && s[4].defined() ? grads[1] : none(s[4]), Tensor(), Tensor(), Tensor()};
+        }
         Attn a(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble());
         m2d_attn_desc& d = a.d;
         const Tensor d_o = grads[0].defined() ? rows(grads[0].to(a.v.scalar_type())) : at::zeros(a.v.sizes(), a.v.options());
@@ -131,17 +146,14 @@ std::tuple<Tensor, optional<Tensor>> linear_attention(const Tensor& q, const Ten
     const Tensor state = or_none(state_);
     check_attn(what, "BT", q, k, v, log_decay, state);
     const Tensor lengths = token_counts(what, or_none(lengths_), v);
-    if (v.size(0) == 0 || v.size(1) == 0) {
-        if (!want_state) return {v.clone(), c10::nullopt};
-        return {v.clone(), state.defined() ? state.clone() : at::zeros({v.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat))};
-    }
-    check_waits(what);
+    if (!no_tokens(v)) check_waits(what);
     const Tensor g = log_decay.to(at::kFloat);
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)q.size(-1));
     if (wants_grad({&q, &k, &v, &g, &state})) {
         const variable_list r = AttnFn::apply(q, k, v, g, state_, lengths.defined() ? optional<Tensor>(lengths) : c10::nullopt, scale, want_state);
         return {r[0], want_state ? optional<Tensor>(r[1]) : c10::nullopt};
     }
+    if (no_tokens(v)) return {v.clone(), want_state ? optional<Tensor>(same_state(q, v, state)) : c10::nullopt};
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
     Attn a(q, k, v, g, state, lengths, scale);

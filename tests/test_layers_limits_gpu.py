@@ -71,6 +71,19 @@ def test_group_norm_of_nothing(shape, dt):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("B,T", [(2, 0), (0, 5)])
+def test_linear_attention_of_nothing(B, T, dt):
+    q, k, v, s = leaf(B, T, 1, 16, dt=dt), leaf(B, T, 1, 16, dt=dt), leaf(B, T, 2, 24, dt=dt), leaf(B, 2, 16, 24)
+    for g in (leaf(2), leaf(B, T, 2), leaf(2, dt=BF)):
+        zeros_for(linear_attention(q, k, v, g), (q, k, v, g))
+        o, last = linear_attention(q, k, v, g, initial_state=s, return_state=True)
+        up = torch.randn_like(s)
+        *rest, ds = torch.autograd.grad((o, last), (q, k, v, g, s), (torch.ones_like(o), up))
+        assert torch.equal(last, s) and torch.equal(ds, up) and all(bool((t == 0).all()) for t in rest)
+    zeros_for(linear_attention(q, k, v.detach(), leaf(2).detach()), (q, k))
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("form", FORMS)
 def test_single_tokens_over_a_long_memory(form, dt):
     """A gate that all tokens share and a memory of some 8192 of them, M, for 20000 tokens.  What a token's rounding of its gate is off by has the same sign
