@@ -263,9 +263,11 @@ inline size_t recur_stage(int tensors, int tile, int width, int es) { return (si
 constexpr size_t kRecurTail = (kRecurStages + 3) * 8;
 
 // Waits for a barrier's phase, so many times 32 tries of a microsecond or more; gives up and tells so in *abort, or where that has been told.
+// CLUSTER: of what other CTAs send.
+template <bool CLUSTER>
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* abort) {
     for (int n = 0; n < limit; ++n) {
-        if (mbar_try_wait32(bar, parity)) return true;
+        if (mbar_try_wait32<CLUSTER>(bar, parity)) return true;
         if (*abort) return false;
     }
     *abort = 1;
@@ -316,7 +318,7 @@ struct Waits {
         const uint32_t bar = join_bars + 8 * (turn & 1);
         if (*apart) return false;
         if (threadIdx.x == 0) mbar_expect_tx(bar, bytes);
-        return wait_for(bar, (turn >> 1) & 1, kJoinLimit, apart);
+        return wait_for<true>(bar, (turn >> 1) & 1, kJoinLimit, apart);
     }
 };
 
@@ -370,7 +372,7 @@ struct Feed {
     __device__ __forceinline__ Raw* place(int t, int i) const { return reinterpret_cast<Raw*>(ring + (((size_t)(stage * TENSORS + t) * tile + run * L + i) * width + at) * sizeof(T)); }
     // false: gave up.  n: tokens that there are of the thread's run; the others' places get what changes nothing.
     __device__ __forceinline__ bool ready(int n) {
-        if (!wait_for(bars + 8 * stage, parity, kCopyLimit, abort)) return false;
+        if (!wait_for<false>(bars + 8 * stage, parity, kCopyLimit, abort)) return false;
         if (n < L) {
 #pragma unroll
             for (int t = 0; t < TENSORS; ++t)
@@ -784,7 +786,7 @@ __global__ void __launch_bounds__(kRecurWarps * 32) recur_bwd_kernel(const Recur
 
 // One token of every sequence.  state and state_out may be the same array.  Where half or more of the state stays, it is moved by its increment, (a - 1) h + u or
 // (1 - f) (x - h), instead of multiplied by a: a's rounding would come back with every token of the same gate, and add up over its memory (8192 tokens
-// long: the state was off by 1.0e-4 to 1.5e-4 after 2000 tokens and went on, by increments it is off by at most 6e-6 after 20000).  An increment that is not finite is not taken.
+// long: the state was off by 1.0e-4 to 1.5e-4 after 2000 tokens, by increments it is off by at most 6e-6 after 20000).  An increment that is not finite is not taken.
 template <typename T, int VEC, int FORM>
 __global__ void __launch_bounds__(128) recur_step_kernel(const RecurArgs p, long long sb) {
     using P = Piece<T, VEC>;
