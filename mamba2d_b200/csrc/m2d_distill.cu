@@ -29,6 +29,7 @@ struct DistillArgs {
     long long N;
     int V, K, t_f32, index64, labels64, same_phase;
     float tau, w, c, c1;               // log2(e) / tau, log2(e)
+    double exact_c;                    // c for what is summed in 64 bits
     float4* found;                     // forward by pieces: largest value and sums of a CTA's share of a row, at [row + CTA]
     int pieces, ctas;                  // pieces of a row
 };
@@ -183,9 +184,9 @@ __device__ __forceinline__ Taught teach(const DistillArgs& p, long long row, con
         for (int k = lane; k < p.K; k += 32) {
             const int i = entry_at(p, row, k);
             if (i < 0) continue;
-            const double a = ((double)teacher_at(p, row, k) - (double)r.top) * (double)p.c, e = exp2(a);
+            const double a = ((double)teacher_at(p, row, k) - (double)r.top) * p.exact_c, e = exp2(a);
             r.sum += e;
-            if (e != 0.0) r.dot += e * (a - ((double)number(z + i) - (double)r.high) * (double)p.c);
+            if (e != 0.0) r.dot += e * (a - ((double)number(z + i) - (double)r.high) * p.exact_c);
         }
         r.sum = warp_sum(r.sum);
         r.dot = warp_sum(r.dot);
@@ -199,7 +200,7 @@ __device__ __forceinline__ void finish_row(const DistillArgs& p, long long row, 
     if ((threadIdx.x & 31) != 0) return;
     double loss = 0.0;
     if (t.any)       // (dot is about `high`: exact where everything is at the type's lowest)
-        loss = (1.0 - (double)p.w) * (double)p.tau * (double)p.tau * 0.6931471805599453 * (t.dot / t.sum + ((double)r.x - (double)t.high) * (double)p.c - log2(t.sum) + log2((double)r.y));
+        loss = (1.0 - (double)p.w) * (double)p.tau * (double)p.tau * 0.6931471805599453 * (t.dot / t.sum + ((double)r.x - (double)t.high) * p.exact_c - log2(t.sum) + log2((double)r.y));
     if (label >= 0) loss += (double)p.w * (log((double)at_one) - ((double)at_label - (double)r.x));
     p.loss[row] = (float)loss;
     if (p.stats) {
@@ -470,7 +471,7 @@ static DistillArgs distill_args(const m2d_distill_desc* d) {
     a.loss = d->loss; a.stats = d->stats; a.dz = d->d_logits;
     a.N = d->N; a.V = d->V; a.K = d->K;
     a.tau = d->temperature; a.w = d->label_weight;
-    a.c1 = kLog2e; a.c = (float)(1.4426950408889634 / (double)d->temperature);
+    a.c1 = kLog2e; a.exact_c = 1.4426950408889634 / (double)d->temperature; a.c = (float)a.exact_c;
     return a;
 }
 // A warp for a row of up to 8 KB, whose loads would be two of a CTA's threads at most, and of up to 32 KB where rows are enough to fill the

@@ -128,3 +128,17 @@ def test_single_tokens_at_their_ends(form):
             assert got != got, c
         else:
             assert got == c[3], c
+
+
+@pytest.mark.parametrize("V", [2, 20001])
+@pytest.mark.parametrize("temperature", [1.0, 2.5, 3.5])
+def test_a_loss_is_rounded_once(V, temperature):
+    """Rows of two classes far apart (others are masked) whose teacher wants the lower one: temperature times the distance, to what fp32 holds.
+    Everything that is computed in 64 bits is off by less than 2^-40 of it."""
+    N = 64
+    z = torch.full((N, V), -torch.inf, device="cuda")
+    far = 150 + 3.7 * torch.arange(N, device="cuda")
+    z[:, 0], z[:, 1] = 0.0, -far
+    t, index = torch.zeros(N, 1, device="cuda"), torch.ones(N, 1, dtype=torch.long, device="cuda")
+    want = temperature * far.double()
+    assert layer_ref.within(distillation_loss(z, t, index, temperature=temperature), want, 2.0 ** -40 * want) <= 1
