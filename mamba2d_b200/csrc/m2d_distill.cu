@@ -17,6 +17,8 @@
 #include "plan.cuh"
 #include "m2d_seq.h"
 
+#include <cfloat>
+
 namespace m2d {
 
 struct DistillArgs {
@@ -471,7 +473,7 @@ static DistillArgs distill_args(const m2d_distill_desc* d) {
     a.loss = d->loss; a.stats = d->stats; a.dz = d->d_logits;
     a.N = d->N; a.V = d->V; a.K = d->K;
     a.tau = d->temperature; a.w = d->label_weight;
-    a.c1 = kLog2e; a.exact_c = 1.4426950408889634 / (double)d->temperature; a.c = (float)a.exact_c;
+    a.c1 = kLog2e; a.exact_c = 1.4426950408889634 / (double)d->temperature; a.c = std::min((float)a.exact_c, FLT_MAX);        // (an infinite one would make NaN of the largest value's zero)
     return a;
 }
 // A warp for a row of up to 8 KB, whose loads would be two of a CTA's threads at most, and of up to 32 KB where rows are enough to fill the

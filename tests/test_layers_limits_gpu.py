@@ -142,3 +142,24 @@ def test_a_loss_is_rounded_once(V, temperature):
     t, index = torch.zeros(N, 1, device="cuda"), torch.ones(N, 1, dtype=torch.long, device="cuda")
     want = temperature * far.double()
     assert layer_ref.within(distillation_loss(z, t, index, temperature=temperature), want, 2.0 ** -40 * want) <= 1
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 2e-39, 1e-30, 1e4, 3e38])
+@pytest.mark.parametrize("V", [50, 20001])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_temperatures_of_any_size(V, dt, temperature):
+    """The teacher's only entry is the student's largest class, or another one: cold, q is one for the largest and zero for others; hot, it is 1 / V."""
+    z = torch.linspace(-3, 3, V, device="cuda").expand(2, V).contiguous().to(dt).requires_grad_(True)
+    index = torch.tensor([[V - 1], [0]], device="cuda")
+    loss = distillation_loss(z, torch.zeros(2, 1, device="cuda"), index, temperature=temperature)
+    assert not bool(torch.isnan(loss).any())
+    assert float(loss[0].detach()) == 0.0 or temperature > 1 or dt == BF          # (bf16: several classes are the largest)
+    up = 1e-20 if temperature > 1e20 else 1.0          # (a slope is temperature (q - p))
+    dz, = torch.autograd.grad(loss, z, torch.full((2,), up, device="cuda"))
+    assert bool(torch.isfinite(dz).all())
+    ref = z.detach().double()
+    q = torch.softmax(ref / temperature, -1)
+    p = torch.zeros_like(q).scatter_(1, index, 1.0)
+    want = up * temperature * (q - p)
+    # (sums of up to 20001 values and exponents near zero: 2^-16; what is below fp32's smallest normal number may be lost)
+    assert layer_ref.within(dz, want, 2.0 ** -16 * up * temperature * (q + p)) <= 1
