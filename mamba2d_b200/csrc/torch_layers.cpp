@@ -352,6 +352,7 @@ Tensor distillation_loss(const Tensor& z, const Tensor& t, const Tensor& index, 
                 ": logits (..., V) and the teacher's logits and indices (..., K) do not match, got ", z.sizes(), ", ", t.sizes(), " and ", index.sizes());
     TORCH_CHECK(t.size(-1) >= 1 && t.size(-1) <= M2D_DISTILL_MAX_TOP && z.size(-1) >= 1, what, ": 1 to ", M2D_DISTILL_MAX_TOP, " logits of the teacher and at least one class, got ", t.sizes(),
                 " and ", z.sizes());
+    TORCH_CHECK(z.size(-1) <= INT_MAX, what, ": a size out of range");
     TORCH_CHECK(real(z) && real(t), what, ": dtype ", z.scalar_type(), " and ", t.scalar_type(), " (float32 and bfloat16 only)");
     TORCH_CHECK(whole(index), what, ": indices must be integers, got ", index.scalar_type());
     TORCH_CHECK_VALUE(temperature > 0 && (float)temperature > 0.f && std::isfinite((float)temperature), what, ": the temperature must be positive, got ", temperature);
