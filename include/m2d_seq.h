@@ -130,8 +130,9 @@ int m2d_clip_grad_norm(const m2d_clip_tensor *tensors, int32_t count, float max_
  * Per sequence and channel  h_t = a_t h_{t-1} + u_t:
  *     M2D_GATE_DECAY:  a = exp(gate), u = x           (gate at most 0; positive ones grow the state and are not checked for)
  *     M2D_GATE_FORGET: a = sigmoid(gate), u = (1 - a) x
- * A gate of -inf forgets everything before the token.  States and their gradients are fp32 whatever the tensors' type.  B times C/32 up to
- * 2^27, C up to 2^29, T below 2^31 - 2^17.  Sequences of several strides whose rows begin at 16-byte boundaries come by TMA; a wait for such a copy that gives
+ * A gate of -inf forgets everything before the token (forget gates below -87 count as -87: 1.6e-38 of the state is left).  States and their gradients are
+ * fp32 whatever the tensors' type.  B times C/32 up to 2^27, C up to 2^29, T below 2^31 - 2^17.  An array that is not aligned to its values gives
+ * M2D_ERR_PITCH, here and below.  Sequences of several strides whose rows begin at 16-byte boundaries come by TMA; a wait for such a copy that gives
  * up makes what depends on it NaN and shows in m2d_take_wait_failure().
  */
 typedef enum { M2D_GATE_DECAY = 0, M2D_GATE_FORGET = 1 } m2d_gate;
@@ -190,7 +191,7 @@ typedef struct m2d_ln_desc {
     const void *weight, *bias;     /* (C), or NULL: one and zero */
     void *sum;                     /* (N,C) dense: x + residual, where there is one                [fwd] */
     void *y;                       /* (N,C) dense                                                  [fwd] */
-    float *stats;                  /* (N,2): mean, 1 / sqrt(var + eps); written by fwd (NULL: not wanted), read by bwd */
+    float *stats;                  /* (N,2), 8-byte aligned: mean, 1 / sqrt(var + eps); written by fwd (NULL: not wanted), read by bwd */
     const void *d_y;               /*                                                              [bwd] */
     int64_t d_y_row;
     const void *d_sum;             /* added to d_x, or NULL */

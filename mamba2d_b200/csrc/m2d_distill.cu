@@ -460,7 +460,9 @@ static int check_distill(const m2d_distill_desc* d) {
     if (!d->logits || !d->teacher || !d->index || (d->label_weight > 0.f && !d->labels)) return M2D_ERR_NULL;
     const uintptr_t es = d->dtype == M2D_F32 ? 4 : 2;
     auto off = [](const void* p, uintptr_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
-    if (off(d->logits, es) || off(d->d_logits, es) || off(d->teacher, d->teacher_dtype == M2D_F32 ? 4 : 2) || off(d->index, d->index_64 ? 8 : 4) || off(d->labels, d->labels_64 ? 8 : 4)) return M2D_ERR_PITCH;
+    if (off(d->logits, es) || off(d->d_logits, es) || off(d->teacher, d->teacher_dtype == M2D_F32 ? 4 : 2) || off(d->index, d->index_64 ? 8 : 4) || off(d->labels, d->labels_64 ? 8 : 4) ||
+        off(d->loss, 4) || off(d->stats, 4) || off(d->d_loss, 4))
+        return M2D_ERR_PITCH;
     return M2D_OK;
 }
 static DistillArgs distill_args(const m2d_distill_desc* d) {

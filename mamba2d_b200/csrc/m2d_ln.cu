@@ -552,6 +552,7 @@ static int check_ln(const m2d_ln_desc* d) {
         if (reinterpret_cast<uintptr_t>(t) % es) return M2D_ERR_PITCH;
     for (const void* t : {d->weight, d->bias, static_cast<const void*>(d->d_weight), static_cast<const void*>(d->d_bias)})
         if (reinterpret_cast<uintptr_t>(t) % pes) return M2D_ERR_PITCH;
+    if (reinterpret_cast<uintptr_t>(d->stats) % sizeof(float2)) return M2D_ERR_PITCH;
     return M2D_OK;
 }
 // Whether every row of a tensor begins at a 16-byte boundary (rows may be one and the same).

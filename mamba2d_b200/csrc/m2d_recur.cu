@@ -829,6 +829,9 @@ static int check_recur(const m2d_recur_desc* d, bool step) {
         if (!t) return M2D_ERR_NULL;
     for (const void* t : {d->x.data, d->gate.data, d->d_y.data, static_cast<const void*>(d->y), static_cast<const void*>(d->d_x), static_cast<const void*>(d->d_gate)})
         if (reinterpret_cast<uintptr_t>(t) % es) return M2D_ERR_PITCH;
+    for (const void* t : {static_cast<const void*>(d->lengths), static_cast<const void*>(d->state), static_cast<const void*>(d->state_out), static_cast<const void*>(d->marks),
+                          static_cast<const void*>(d->d_state_out), static_cast<const void*>(d->d_state)})
+        if (reinterpret_cast<uintptr_t>(t) % 4) return M2D_ERR_PITCH;
     return M2D_OK;
 }
 static bool pairs_ok(const void* p, long long a, long long b, int es) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % (2 * es) == 0 && a % 2 == 0 && b % 2 == 0); }
