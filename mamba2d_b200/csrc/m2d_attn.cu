@@ -5,6 +5,7 @@
 #include "attn_tc.cuh"
 #include "follow.cuh"
 #include "launch.cuh"
+#include "packed.cuh"
 
 namespace m2d {
 
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(256) attn_share_kernel(const float* p0, const 
 // ------------------------------------------------------------------------------------------------
 // One token.  The state is read and written once and nothing else is large: a CTA owns a head's state rows (or, where
 // there are few heads, some of its columns), a warp every eighth row of it, all of a thread's rows requested
-// before the first is used.  256x16x128x128: 537 MB in 90 us, 6.0 TB/s (92 % of a copy's rate); 1x8x64x64: 6 us, a launch and one round trip.
+// before the first is used.  256x16x128x128: 537 MB in 89 us, 6.1 TB/s (93 % of a copy's rate); 1x8x64x64: 6 us, a launch and one round trip.
 // ------------------------------------------------------------------------------------------------
 template <typename io_t, int NV>      // NV columns a lane
 __global__ void __launch_bounds__(256) attn_step_kernel(AttnTensor q, AttnTensor k, AttnTensor v, const float* __restrict__ g, long long gb, long long gh, float scale, int H, int K, int V,
@@ -451,29 +452,39 @@ __global__ void __launch_bounds__(256) attn_step_kernel(AttnTensor q, AttnTensor
     const size_t at = (size_t)(b * sb + h * sh) + c;
     const bool on = c < V;
     constexpr int kAhead = 16;
-    float s[kAhead][NV];
+    using N = Num<NV == 4 ? 2 : 1>;       // (packed arithmetic for pairs of columns)
+    constexpr int P = NV == 4 ? 2 : 1;
+    N s[kAhead][P];
     auto request = [&](int r0) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int r = r0 + warp + j * 8;
             if (on && r < K) {
                 const float* p = state + at + (size_t)r * V;
-                if constexpr (NV == 4) { const float4 t = *reinterpret_cast<const float4*>(p); s[j][0] = t.x; s[j][1] = t.y; s[j][2] = t.z; s[j][3] = t.w; }
-                else s[j][0] = *p;
+                if constexpr (NV == 4) { const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p); s[j][0].v = t.x; s[j][1].v = t.y; }
+                else s[j][0].v = *p;
             }
         }
     };
+    const float gv = __ldg(g + b * gb + h * gh);          // (first: the state's rows are on their way meanwhile)
     request(0);
     if (threadIdx.x < K) {
         qs[threadIdx.x] = load1(qp, threadIdx.x);
         ks[threadIdx.x] = load1(kp, threadIdx.x);
     }
-    const float gv = __ldg(g + b * gb + h * gh), a = ex2((float)attn_decay(gv));
-    float vv[NV], o[NV];
+    // The decay in two parts, of which the first is below it and the second above zero (a state of infinity stays one): rounded to one, what it is off by would come
+    // back with every token of the same decay and add up over its memory (8192 tokens: 7.5e-5 of the state after 2000 of them, now at most 8e-6 after 20000).
+    const bool near = fabsf(gv) <= kLn2;
+    const float less = near ? expm1f(gv) : 0.f, a = near ? 1.f + less : ex2((float)attn_decay(gv));
+    float hi = fmaf(a, -0x1p-22f, a), lo = near ? less - (hi - 1.f) : a - hi;
+    if (!(a <= 3.402823466e38f)) hi = lo = a;
+    const N first = N::all(hi), rest = N::all(lo);
+    N vv[P], o[P];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        vv[i] = on ? load1(vp, c + i) : 0.f;
-        o[i] = 0.f;
+    for (int i = 0; i < P; ++i) {
+#pragma unroll
+        for (int k = 0; k < NV / P; ++k) vv[i].set(k, on ? load1(vp, c + i * (NV / P) + k) : 0.f);
+        o[i] = N::all(0.f);
     }
     __syncthreads();
     for (int r0 = 0; r0 < K; r0 += 8 * kAhead) {
@@ -482,19 +493,20 @@ __global__ void __launch_bounds__(256) attn_step_kernel(AttnTensor q, AttnTensor
         for (int j = 0; j < kAhead; ++j) {
             const int r = r0 + warp + j * 8;
             if (on && r < K) {
+                const N kr = N::all(ks[r]), qr = N::all(qs[r]);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    s[j][i] = fmaf(s[j][i], a, ks[r] * vv[i]);
-                    o[i] = fmaf(qs[r], s[j][i], o[i]);
+                for (int i = 0; i < P; ++i) {
+                    s[j][i] = fma_(s[j][i], first, fma_(s[j][i], rest, mul_(kr, vv[i])));
+                    o[i] = fma_(qr, s[j][i], o[i]);
                 }
                 float* p = state_out + at + (size_t)r * V;
-                if constexpr (NV == 4) *reinterpret_cast<float4*>(p) = make_float4(s[j][0], s[j][1], s[j][2], s[j][3]);
-                else *p = s[j][0];
+                if constexpr (NV == 4) *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(s[j][0].v, s[j][1].v);
+                else *p = s[j][0].v;
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) part[warp][(threadIdx.x & 31) * NV + i] = o[i];
+    for (int i = 0; i < NV; ++i) part[warp][(threadIdx.x & 31) * NV + i] = o[i / (NV / P)].get(i % (NV / P));
     __syncthreads();
     const int n0 = blockIdx.y * 32 * NV;
     for (int i = threadIdx.x; i < 32 * NV; i += 256)

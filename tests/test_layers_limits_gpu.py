@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import layer_ref
-from mamba2d_b200 import distillation_loss, gated_recurrence, gated_recurrence_step, group_norm, layer_norm, linear_attention
+from mamba2d_b200 import distillation_loss, gated_recurrence, gated_recurrence_step, group_norm, layer_norm, linear_attention, linear_attention_step
 from test_recurrence_gpu import fast_scan
 
 pytestmark = pytest.mark.gpu
@@ -163,3 +163,39 @@ def test_temperatures_of_any_size(V, dt, temperature):
     want = up * temperature * (q - p)
     # (sums of up to 20001 values and exponents near zero: 2^-16; what is below fp32's smallest normal number may be lost)
     assert layer_ref.within(dz, want, 2.0 ** -16 * up * temperature * (q + p)) <= 1
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_single_tokens_of_linear_attention_over_a_long_memory(dt):
+    """The same, for decays that all tokens of a head share: the state against the formula in 64 bits, one token after another."""
+    T, H, K, V = 20000, 4, 8, 24
+    g = torch.tensor([-2.0 ** -13, -1.1 * 2.0 ** -13, -1.7 * 2.0 ** -13, -2.9 * 2.0 ** -13], device="cuda")
+    random = torch.Generator().manual_seed(15)
+    k, v = ((1 + 0.5 * torch.randn(T, 1, H, n, generator=random)).cuda().to(dt) for n in (K, V))
+    a = g.double().exp()[None, :, None, None]
+    state = (1 / (1 - a)).float().expand(1, H, K, V).contiguous()
+    want = state.double()
+    allowed = 8 * 2.0 ** -24 * (8192 / 6) ** 0.5 + 2.0 ** -20
+    for t in range(T):
+        linear_attention_step(k[t], k[t], v[t], g, state)
+        want = want * a + k[t].double()[..., None] * v[t].double()[..., None, :]
+        if t % 2000 == 1999:
+            assert float((state.double() / want - 1).abs().max()) <= allowed, t
+
+
+def test_single_tokens_of_linear_attention_at_their_ends():
+    """States of infinity, NaN and next to the largest number under decays that keep all, most and little of them: the formula's."""
+    g = torch.tensor([0.0, -2.0 ** -20, -0.1, -0.693, -0.7, -3.0, -80.0, 0.5, 1.0], device="cuda")
+    values = torch.tensor([torch.inf, -torch.inf, torch.nan, 3e38, -3e38, 1.0, 0.0, -1e-30], device="cuda")
+    H, K, V = len(g), 4, len(values)
+    k, v = torch.tensor([[1.0, -2.0, 0.0, 1e-20]], device="cuda").expand(1, H, K), torch.ones(1, H, V, device="cuda")
+    state = values.expand(1, H, K, V).contiguous()
+    want = state.double() * g.double().exp()[None, :, None, None] + (k[..., None] * v[..., None, :]).double()
+    size = state.double().abs() * g.double().exp()[None, :, None, None] + k[..., None].double().abs()
+    linear_attention_step(k, k, v, g, state)
+    over = want.abs() > torch.finfo(F32).max
+    want = torch.where(over & ~torch.isnan(want), want.sign() * torch.inf, want)
+    bad = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(state), torch.isnan(want)) and torch.equal(state[bad & ~torch.isnan(want)].double(), want[bad & ~torch.isnan(want)])
+    # (-1e-30 under a decay of -80 is -1.8e-65, of which fp32 has nothing: a value near zero is off by its smallest step, 2^-149, whatever its size)
+    assert bool(((state.double() - want).abs() <= 2.0 ** -20 * size + 2.0 ** -149)[~bad].all())
