@@ -7,7 +7,7 @@
 // A cluster of CTAs owns the channels of LANES lanes and walks a sequence in strides, a tile of it for each CTA.  Inside a tile the lanes of a row
 // take L tokens: they find what those do to any state, h -> A h + b, from registers; the runs' pairs (A, b) are joined in shared memory, the tiles' in
 // that of every CTA of the cluster; then each goes over its tokens again from the state before them, still from registers, and stores.  So
-// memory is read once and written once.  Tiles come by TMA, two or three ahead of the one that is worked on; where rows are not whole 16-byte pieces, or
+// memory is read once and written once.  Tiles come by TMA, one to three ahead of the one that is worked on (two forward and one backward where tiles are as large as in the cases below); where rows are not whole 16-byte pieces, or
 // there is but one stride, by plain loads into registers, the next tile's while one is worked on.  Where sequences and channels are too few for all SMs, rows are
 // split into shorter pieces and the sequence over up to 8 CTAs (plan_recur).  Measured, bf16: 4x4096x2048 forget gates 47 us (201 MB at 4.3 TB/s: half
 // of the issue slots, two CTAs an SM), 1x65536x512 decays 57 us (the chain of waits of 16 strides), 8x4096x2048 forward 75 and backward 126 us (5.4 and 5.3 TB/s).
@@ -262,7 +262,7 @@ inline size_t recur_joins(int parts, int warps, int ctas, int width) { return si
 inline size_t recur_stage(int tensors, int tile, int width, int es) { return (size_t)tensors * tile * width * es; }
 constexpr size_t kRecurTail = (kRecurStages + 3) * 8;
 
-// Waits for a barrier's phase, so many times 32 tries of a microsecond or more; gives up and tells so in *abort, or where that has been told.
+// Waits for a barrier's phase, so many times 32 tries of at most about a microsecond; gives up and tells so in *abort, or where that has been told.
 // CLUSTER: of what other CTAs send.
 template <bool CLUSTER>
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limit, volatile int* abort) {
@@ -273,7 +273,7 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int limi
     *abort = 1;
     return false;
 }
-// For a copy about a second; for other CTAs' joins four times that, since one of them may be giving up a copy.
+// For a copy about a quarter of a second; for other CTAs' joins four times that, since one of them may be giving up a copy.
 constexpr int kCopyLimit = 1 << 13, kJoinLimit = 1 << 15;
 
 // Barriers and the abort words of a CTA.  A tile's join reaches every CTA of the cluster by stores that count towards the receiver's barrier:

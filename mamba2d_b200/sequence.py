@@ -76,8 +76,8 @@ def gated_recurrence(x, gate, *, form="decay", initial_state=None, lengths=None,
         x, gate: (B, T, C) of one type.  Any strides (a last dimension that is not dense is copied): a gate per channel or
             per token may be expanded over the rest, and gets its gradient.
         form: "decay": ``a = exp(gate)``, ``u = x``; gate at most 0, a positive value grows the state and is not checked for.
-            "forget": ``a = sigmoid(gate)``, ``u = (1 - a) x``.  A gate of -inf forgets all earlier tokens (if they
-            are finite).
+            "forget": ``a = sigmoid(gate)``, ``u = (1 - a) x``; below -87 it counts as -87 (1.6e-38 of the state is left).
+            A gate of -inf forgets all earlier tokens (if they are finite).
         initial_state: (B, C) float32, or None for zero.
         lengths: (B,) integers on the device, tokens of each sequence (clamped to 0 ... T), or None for T.  What rows
             behind them hold does not matter; outputs and gradients there are zero.
@@ -87,7 +87,9 @@ def gated_recurrence(x, gate, *, form="decay", initial_state=None, lengths=None,
     Differentiable in x, gate and initial_state, once (``create_graph`` raises); those of x and gate are computed together.
     States are carried in float32 and gradients computed from them, whatever the type of h.  A token that is not finite spoils
     later ones of its sequence and channel (in the backward pass earlier ones), as by the formula.  Rows of x and gate that begin at
-    16-byte boundaries are fetched ahead by TMA (an odd number of channels takes two to three times as long).
+    16-byte boundaries are fetched ahead by TMA; others, and above all an odd number of channels, take longer (25 x 13967 tokens of 75
+    channels in float32 160 us, of 76 98; in bfloat16 117, of 80 52).  Up to eight CTAs share a sequence: a long one of few channels
+    leaves most of the GPU without work (1 x 60000 x 64 in bfloat16 35 us, ten times what its bytes take).
     """
     if form not in _GATES:
         raise ValueError(f"gated_recurrence: unknown form, got {form}...")
@@ -101,7 +103,8 @@ def gated_recurrence_step(x, gate, state, *, form="decay"):
     Args:
         x, gate: (B, C) of one type, as ``gated_recurrence`` takes them.
         state: (B, C) float32, dense along C; sequences may lie apart (a layer's slice of a cache) but must not overlap.
-    No gradients: it raises where one is wanted.
+    No gradients: it raises where one is wanted.  States stay with ``gated_recurrence``'s over any number of tokens: they are
+    rounded once a token, and no rounding of a gate adds up.
     """
     if form not in _GATES:
         raise ValueError(f"gated_recurrence_step: unknown form, got {form}...")
@@ -142,7 +145,8 @@ def layer_norm(x, weight=None, bias=None, *, residual=None, eps=1e-5):
         y in x's type, or ``(y, s)`` where there is a residual: s goes on to the next layer.
     Differentiable in x, weight, bias and residual, once (``create_graph`` raises); x and residual get the same gradient, one
     tensor.  Rows may lie apart (a slice of a wider tensor); other strides are copied.  Rows that are not whole 16-byte
-    pieces are read value by value; rows of more than 8192 values are read three times.
+    pieces are worked on value by value (8000 x 4001 in bfloat16 70 us, of 4000 values 31); rows of more than 8192 values are read three times.
+    A batch without rows gives the parameters gradients of zero.
     """
     y, total = _lib.entry().layer_norm(x, weight, bias, residual, eps)
     return y if residual is None else (y, total)
